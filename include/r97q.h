@@ -543,6 +543,118 @@ int r97q_vocab_head_transpose(const R97qVocabPlan* plan, const uint16_t* dy, int
 /* dst bf16 <- src f32 (RNE, src/adjoint/device/vocab_head.hip:80-86) */
 int r97q_vocab_head_cast(uint16_t* dst, const float* src, int64_t values, R97IqrStream stream);
 
+/* ------------------------------------------------------------------ between the projections
+ *
+ * What a layer does between its projections: rotary positions, attention, and the norm before a coded
+ * product. No counterpart in the reference's one path; names, checks, streams and workspaces are those
+ * of the entries above. Inputs with a stride of zero (a broadcast) are read as they are; outputs may
+ * not overlap themselves or, unless a comment says so, an input.
+ *
+ * A tensor of heads: element (batch b, token t, head h, d) lies at data[b * batch_stride + t *
+ * token_stride + h * head_stride + d], strides in elements, d consecutive. [tokens, heads, d],
+ * [heads, tokens, d] and a slice of a wider projection's output are all this. */
+typedef struct R97qHeads {
+    void* data;
+    int64_t batch_stride;  /* unused where the sequences are packed and by rotary */
+    int64_t token_stride;
+    int64_t head_stride;
+    int32_t heads;
+    int32_t dtype;
+} R97qHeads;
+
+/* Rotary positions of q and k in one launch. Pair i of a head's first `rot` values (even; the values past
+ * it are copied) is (x[i], x[i + rot/2]) with R97Q_ROTARY_HALF or (x[2i], x[2i+1]) with
+ * R97Q_ROTARY_INTERLEAVED; at the angle a = position * inv_freq[i]
+ *   (u, v) -> mscale * (u cos a - v sin a, u sin a + v cos a)
+ * and with `inverse` at -a: the adjoint of the forward with the same mscale, for q's and k's cotangents.
+ * inv_freq: f64 [rot/2] on the device (angles are formed in f64 and taken modulo a turn there, so far
+ * positions keep their phase; the rotation is f32, rounded once to the output's type).
+ * positions: int32 or (positions64) int64 [tokens] on the device, NULL for 0 .. tokens-1. q, k and their
+ * outputs share one dtype (bf16 or f32); k and k_out may be NULL. An output may be its input (same data
+ * and strides): the values past rot then stay untouched. */
+#define R97Q_ROTARY_HALF 0
+#define R97Q_ROTARY_INTERLEAVED 1
+int r97q_rotary(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, const R97qHeads* k_out,
+                int64_t tokens, int32_t head_dim, int32_t rot, int32_t pairs, const double* inv_freq,
+                const void* positions, int32_t positions64, float mscale, int32_t inverse, R97IqrStream stream);
+/* The frequencies on the host: f[i] = base^(-2i/rot), then for a context `factor` times the `original`
+ * length (in positions) the model was trained on:
+ *   R97Q_ROTARY_LINEAR  f / factor (positions stretched)
+ *   R97Q_ROTARY_RAMP    f kept where a pair turns more than `fast` times over the original length, f /
+ *                       factor where it turns fewer than `slow` times, blended linearly in the number
+ *                       of turns between; *mscale = 0.1 ln(factor) + 1
+ * inv_freq: host f64 [rot/2]; *mscale (may be NULL) is 1 but for the ramp. */
+#define R97Q_ROTARY_PLAIN 0
+#define R97Q_ROTARY_LINEAR 1
+#define R97Q_ROTARY_RAMP 2
+int r97q_rotary_frequencies(int32_t rot, double base, int32_t scaling, double factor, double original, double slow,
+                            double fast, double* inv_freq, float* mscale);
+
+/* A batch of sequences. Dense: q_len query tokens and kv_len key tokens each, a sequence batch_stride
+ * apart; kv_lens (device int32 [batch], may be NULL) says how many of the kv_len are in use. Packed: the
+ * sequences one after the other along the tokens, sequence b at [starts[b], starts[b + 1]) (device int32
+ * [batch + 1], ascending), q_len / kv_len the longest sequence (it sizes the launch) and q_tokens /
+ * kv_tokens the tokens in all. Queries and keys take either form on their own. Starts and lengths outside
+ * the tensors are clamped to them.
+ * The last query stands at the last key: query i of a sequence with n queries and m keys sees key j when
+ * not causal, or when j <= i + m - n and, with a window, j > i + m - n - window. A query that sees no key
+ * gives zeros, a log-sum-exp of minus infinity and zero gradients. Keys and values past a sequence's
+ * length are not read. A NaN or infinity that some query of a tile sees may reach the tile's other rows. */
+typedef struct R97qAttnShape {
+    int32_t batch;
+    int32_t head_dim;          /* a multiple of 8, at most 256 */
+    int64_t q_len, kv_len;
+    const int32_t* q_starts;
+    const int32_t* kv_starts;
+    int64_t q_tokens, kv_tokens;
+    const int32_t* kv_lens;
+    int64_t window;            /* 0: none; needs causal */
+    int32_t causal;
+    float scale;               /* of the scores, usually 1 / sqrt(head_dim) */
+} R97qAttnShape;
+
+/* out = softmax(scale q k^T) v and (lse may be NULL) the scores' natural log-sum-exp f32 [batch][q_heads]
+ * [q_len], packed [q_heads][q_tokens]. q, k, v bf16 with 16-byte aligned rows; out bf16 or f32; k's heads
+ * divide q's: query head h reads key head h / (q_heads / kv_heads). Scores, statistics and sums are f32,
+ * the probabilities are rounded to bf16 for their product with v. */
+int64_t r97q_attn_fwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads);
+int r97q_attn_fwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
+                  const R97qHeads* out, float* lse, void* workspace, int64_t workspace_bytes, R97IqrStream stream);
+/* The adjoint, from the forward's inputs, out and lse and the output's cotangent d_out (bf16): dq, dk, dv
+ * (bf16 or f32) are written. The probabilities are computed again from the scores and lse. Repeated
+ * calls give the same bits. The dense form's keys past kv_lens get zero gradients. */
+int64_t r97q_attn_bwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads);
+int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
+                  const R97qHeads* out, const float* lse, const R97qHeads* d_out, const R97qHeads* dq,
+                  const R97qHeads* dk, const R97qHeads* dv, void* workspace, int64_t workspace_bytes,
+                  R97IqrStream stream);
+
+/* The residual's addition, the RMS norm and the group quantiser in one pass over rows of n values:
+ *   h = x + residual rounded to dtype (residual NULL: h is x, and h_out is not written),
+ *   rs = 1 / sqrt(mean of h^2 + eps),  y = h * rs * (w + wadd),
+ *   per group of `group` columns (<= 0 or > n: one a row; the last may be short): scale = amax / 127 (1
+ *   where all are zero), codes = rint(y / scale).
+ * x, residual, w and h_out are `dtype` (bf16 or f32), h_out [rows, n] the residual stream for the next
+ * layer; the norm is taken of h as it is stored, which is what the adjoint reads. codes int8 [rows, n],
+ * scale f32 [rows, groups] (both NULL: no codes), y_out bf16 [rows, n] (may be NULL), rstd f32 [rows]
+ * (may be NULL). Arithmetic and sums are f32. With group 128 codes and scale are gemm_nt_q's operands.
+ * h_out may be x or residual. */
+int r97q_add_rmsnorm_i8g(const void* x, const void* residual, const void* w, int32_t dtype, int64_t rows, int64_t n,
+                         int64_t group, float eps, float wadd, void* h_out, int8_t* codes, float* scale,
+                         uint16_t* y_out, float* rstd, R97IqrStream stream);
+/* Its adjoint, straight through the rounding with the scales held (no value is clamped: the scale is its
+ * group's own maximum): e = g_codes / scale + g_y,
+ *   dx = rs ((w + wadd) e - h rs^2 mean((w + wadd) e h)) + g_h    (x's and the residual's gradient, written)
+ *   dw[n] (+)= sum over the rows of e h rs                           (f32; may be NULL; written, or added to)
+ * h and w as the forward's (dtype), rstd f32 [rows] the forward's; the cotangents g_codes (with scale f32
+ * [rows, groups]), g_y and g_h are `dtype`, each may be NULL; dx is `dtype`. dx may be g_h, g_y or g_codes.
+ * The rows' partial sums of dw go through the workspace and are added in a fixed order. */
+int64_t r97q_add_rmsnorm_i8g_bwd_workspace_bytes(int64_t rows, int64_t n);
+int r97q_add_rmsnorm_i8g_bwd(const void* h, const void* w, int32_t dtype, int64_t rows, int64_t n, int64_t group,
+                             float wadd, const float* rstd, const float* scale, const void* g_codes,
+                             const void* g_y, const void* g_h, void* dx, float* dw, int32_t dw_accumulate,
+                             void* workspace, int64_t workspace_bytes, R97IqrStream stream);
+
 /* ------------------------------------------------------------------ measurement
  * The card's sustained bf16 MFMA rate with nothing else to do (no counterpart in the reference; for
  * bench.py's roofline): 256 workgroups x 8 waves each issuing `iters` x 32

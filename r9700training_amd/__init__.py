@@ -19,6 +19,8 @@ R97Q_F64 = 3
 R97Q_PART_RMSNORM, R97Q_PART_SILU_MUL, R97Q_PART_SIGMOID_MUL = 0, 1, 2  # the fused quantisers' parts
 R97Q_CODES8 = 8  # R97qWeight.bits of the int8-code form (include/r97q.h)
 R97Q_DECODE_AUTO, R97Q_DECODE_ONCE, R97Q_DECODE_FUSED = 0, 1, 2  # r97q_set_decode_once modes
+R97Q_ROTARY_HALF, R97Q_ROTARY_INTERLEAVED = 0, 1  # r97q_rotary's pairs
+R97Q_ROTARY_PLAIN, R97Q_ROTARY_LINEAR, R97Q_ROTARY_RAMP = 0, 1, 2  # r97q_rotary_frequencies' scalings
 R97Q_ADAMW_GRADS_STAGED = 1  # r97q_adamw_step flags: the gradients are staging buffers (include/r97q.h)
 
 
@@ -83,6 +85,22 @@ class VocabPlan(C.Structure):
                 ("transform", C.c_int64), ("classes", C.c_int32), ("cls", VocabClass * 4)]
 
 
+class Heads(C.Structure):
+    """R97qHeads (include/r97q.h): a tensor of heads."""
+
+    _fields_ = [("data", C.c_void_p), ("batch_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("heads", C.c_int32), ("dtype", C.c_int32)]
+
+
+class AttnShape(C.Structure):
+    """R97qAttnShape (include/r97q.h): a batch of sequences and what each query sees."""
+
+    _fields_ = [("batch", C.c_int32), ("head_dim", C.c_int32), ("q_len", C.c_int64), ("kv_len", C.c_int64),
+                ("q_starts", C.c_void_p), ("kv_starts", C.c_void_p), ("q_tokens", C.c_int64),
+                ("kv_tokens", C.c_int64), ("kv_lens", C.c_void_p), ("window", C.c_int64), ("causal", C.c_int32),
+                ("scale", C.c_float)]
+
+
 R97_ENC_STR = 32
 R97_ENC_MAX_PLANES = 8
 # R97EncDtype (include/r97q.h)
@@ -122,6 +140,7 @@ class StoredPlane(C.Structure):
 
 # every symbol include/r97q.h declares, with its ctypes signature
 _P, _I, _i = C.c_void_p, C.c_int64, C.c_int32
+_H = C.POINTER(Heads)
 SIGNATURES = {
     "r97q_last_error": (C.c_char_p, []),
     "r97q_iqr_validate": (C.c_int, [C.POINTER(Desc)]),
@@ -175,6 +194,17 @@ SIGNATURES = {
     "r97q_vocab_head_workspace_bytes": (_I, [C.POINTER(VocabPlan), _I]),
     "r97q_vocab_head_transpose": (C.c_int, [C.POINTER(VocabPlan), _P, _I, _P, _P, _I, _P]),
     "r97q_vocab_head_cast": (C.c_int, [_P, _P, _I, _P]),
+    "r97q_rotary": (C.c_int, [_H, _H, _H, _H, _I, _i, _i, _i, _P, _P, _i, C.c_float, _i, _P]),
+    "r97q_rotary_frequencies": (C.c_int, [_i, C.c_double, _i, C.c_double, C.c_double, C.c_double, C.c_double, _P,
+                                          C.POINTER(C.c_float)]),
+    "r97q_attn_fwd_workspace_bytes": (_I, [C.POINTER(AttnShape), _i, _i]),
+    "r97q_attn_fwd": (C.c_int, [C.POINTER(AttnShape), _H, _H, _H, _H, _P, _P, _I, _P]),
+    "r97q_attn_bwd_workspace_bytes": (_I, [C.POINTER(AttnShape), _i, _i]),
+    "r97q_attn_bwd": (C.c_int, [C.POINTER(AttnShape), _H, _H, _H, _H, _P, _H, _H, _H, _H, _P, _I, _P]),
+    "r97q_add_rmsnorm_i8g": (C.c_int, [_P, _P, _P, _i, _I, _I, _I, C.c_float, C.c_float, _P, _P, _P, _P, _P, _P]),
+    "r97q_add_rmsnorm_i8g_bwd_workspace_bytes": (_I, [_I, _I]),
+    "r97q_add_rmsnorm_i8g_bwd": (C.c_int, [_P, _P, _i, _I, _I, _I, C.c_float, _P, _P, _P, _P, _P, _P, _P, _i, _P, _I,
+                                           _P]),
     "r97q_mfma_probe_flops": (_I, [_i]),
     "r97q_mfma_probe": (C.c_int, [_i, _i, _P, _I, _P]),
 }
@@ -215,6 +245,16 @@ def _stream(stream=None):
 
     s = stream if stream is not None else torch.cuda.current_stream()
     return C.c_void_p(s.cuda_stream)
+
+
+def _empty(shape, dtype, device, stream=None):
+    """A tensor for a call's output or workspace, taken from the pool of the stream the call runs on."""
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 from .qlinear import QWeight, qlinear_lora_fwd, qlinear_lora_bwd, iqr_decode  # noqa: E402,F401

@@ -1,0 +1,130 @@
+"""Attention on the card, forward and backward (a front over r97q_attn_fwd and r97q_attn_bwd,
+include/r97q.h).
+
+Tensors are token-major: [batch, tokens, heads, head_dim], or [tokens, heads, head_dim] where sequences of
+different lengths are packed one after the other and int32 `q_starts` / `kv_starts` [batch + 1] say where
+each begins. Any strides will do, with head_dim consecutive and rows on 16 bytes: a view of a fused
+projection's output, or of a [batch, heads, tokens, head_dim] cache (transpose(1, 2))."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import R97Q_BF16, R97Q_F32, AttnShape, Heads, _empty, _ptr, _stream, check, lib
+
+
+def _heads(x: torch.Tensor, packed: bool, what: str) -> Heads:
+    n = 3 if packed else 4
+    if x.dim() != n or not x.is_cuda or (x.stride(n - 1) != 1 and x.numel()):
+        raise ValueError(f"attention: {what} is a device [{'' if packed else 'batch, '}tokens, heads, head_dim] tensor, "
+                         "head_dim consecutive")
+    dt = R97Q_BF16 if x.dtype == torch.bfloat16 else R97Q_F32 if x.dtype == torch.float32 else -1
+    if packed:
+        return Heads(x.data_ptr(), 0, x.stride(0), x.stride(1), x.shape[1], dt)
+    return Heads(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), x.shape[2], dt)
+
+
+def _index(t: torch.Tensor, n: int | None, what: str) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or not t.is_cuda or (n is not None and t.shape[0] != n):
+        raise ValueError(f"attention: {what} is a contiguous int32 device tensor{'' if n is None else f' of {n} values'}")
+    return t
+
+
+def _shape(q, k, v, causal, window, scale, q_starts, kv_starts, max_q, max_kv, kv_lens) -> AttnShape:
+    s = AttnShape()
+    pq, pk = q_starts is not None, kv_starts is not None
+    if q.dim() != (3 if pq else 4) or k.dim() != (3 if pk else 4) or v.shape != k.shape or q.shape[-1] != k.shape[-1]:
+        raise ValueError("attention: q and k are [batch, tokens, heads, head_dim], packed [tokens, heads, head_dim]; v has "
+                         "k's shape")
+    s.head_dim = q.shape[-1]
+    batch = {q_starts.shape[0] - 1 if pq else q.shape[0], kv_starts.shape[0] - 1 if pk else k.shape[0]}
+    if len(batch) != 1 or min(batch) < 0:
+        raise ValueError("attention: q and k hold as many sequences")
+    s.batch = batch.pop()
+    if pq:
+        _index(q_starts, None, "q_starts")
+        if max_q is None:
+            raise ValueError("attention: packed queries need max_q, their longest sequence")
+        s.q_starts, s.q_tokens, s.q_len = q_starts.data_ptr(), q.shape[0], int(max_q)
+    else:
+        s.q_len = q.shape[1]
+    if pk:
+        _index(kv_starts, None, "kv_starts")
+        if max_kv is None:
+            raise ValueError("attention: packed keys need max_kv, their longest sequence")
+        s.kv_starts, s.kv_tokens, s.kv_len = kv_starts.data_ptr(), k.shape[0], int(max_kv)
+    else:
+        s.kv_len = k.shape[1]
+    if kv_lens is not None:
+        s.kv_lens = _index(kv_lens, s.batch, "kv_lens").data_ptr()
+    s.causal, s.window = int(bool(causal)), int(window)
+    s.scale = 1.0 / math.sqrt(s.head_dim) if scale is None else float(scale)
+    return s
+
+
+def _lse_shape(q, packed):
+    return (q.shape[1], q.shape[0]) if packed else (q.shape[0], q.shape[2], q.shape[1])
+
+
+def _check_lse(lse, q, packed):
+    if lse.dtype != torch.float32 or tuple(lse.shape) != _lse_shape(q, packed) or not lse.is_contiguous() or not lse.is_cuda:
+        raise ValueError("attention: lse is a contiguous f32 [batch, heads, tokens] device tensor, packed [heads, tokens]")
+
+
+def _same(x, like, what):
+    if x.shape != like.shape:
+        raise ValueError(f"attention: {what} has shape {tuple(like.shape)}")
+
+
+def attention_fwd(q, k, v, causal: bool = True, window: int = 0, scale: float | None = None, q_starts=None,
+                  kv_starts=None, max_q: int | None = None, max_kv: int | None = None, kv_lens=None, out=None,
+                  out_dtype=torch.bfloat16, lse=None, workspace=None, stream=None):
+    """(out, lse): out = softmax(scale q k^T) v (q's shape, `out_dtype`), lse f32 [batch, heads, tokens]. scale:
+    1 / sqrt(head_dim). The last query stands at the last key; causal: a query sees no later key, window:
+    and only the last `window` ones. kv_lens int32 [batch]: how much of a dense k and v is in use. Packed tokens
+    outside every sequence are not written."""
+    s = _shape(q, k, v, causal, window, scale, q_starts, kv_starts, max_q, max_kv, kv_lens)
+    pq, pk = q_starts is not None, kv_starts is not None
+    if out is None:
+        out = _empty(q.shape, out_dtype, q.device, stream)
+    _same(out, q, "out")
+    if lse is None:
+        lse = _empty(_lse_shape(q, pq), torch.float32, q.device, stream)
+    _check_lse(lse, q, pq)
+    hq, hk = _heads(q, pq, "q"), _heads(k, pk, "k")
+    if workspace is None:
+        need = lib().r97q_attn_fwd_workspace_bytes(s, hq.heads, hk.heads)
+        if need > 0:
+            workspace = _empty(need, torch.uint8, q.device, stream)
+    check(lib().r97q_attn_fwd(s, hq, hk, _heads(v, pk, "v"), _heads(out, pq, "out"), _ptr(lse), _ptr(workspace),
+                              0 if workspace is None else workspace.numel(), _stream(stream)), "r97q_attn_fwd")
+    return out, lse
+
+
+def attention_bwd(q, k, v, out, lse, d_out, causal: bool = True, window: int = 0, scale: float | None = None,
+                  q_starts=None, kv_starts=None, max_q: int | None = None, max_kv: int | None = None, kv_lens=None,
+                  dq=None, dk=None, dv=None, grad_dtype=torch.bfloat16, workspace=None, stream=None):
+    """(dq, dk, dv), written: the adjoint of attention_fwd with the same arguments, from its out and lse and
+    the output's cotangent d_out (bf16). Packed tokens outside every sequence are not written."""
+    s = _shape(q, k, v, causal, window, scale, q_starts, kv_starts, max_q, max_kv, kv_lens)
+    pq, pk = q_starts is not None, kv_starts is not None
+
+    def grad(x, like, what):
+        if x is None:
+            x = _empty(like.shape, grad_dtype, like.device, stream)
+        _same(x, like, what)
+        return x
+
+    dq, dk, dv = grad(dq, q, "dq"), grad(dk, k, "dk"), grad(dv, v, "dv")
+    _same(out, q, "out")
+    _same(d_out, q, "d_out")
+    _check_lse(lse, q, pq)
+    hq, hk = _heads(q, pq, "q"), _heads(k, pk, "k")
+    if workspace is None:
+        need = lib().r97q_attn_bwd_workspace_bytes(s, hq.heads, hk.heads)
+        workspace = _empty(max(need, 1), torch.uint8, q.device, stream)
+    check(lib().r97q_attn_bwd(s, hq, hk, _heads(v, pk, "v"), _heads(out, pq, "out"), _ptr(lse), _heads(d_out, pq, "d_out"),
+                              _heads(dq, pq, "dq"), _heads(dk, pk, "dk"), _heads(dv, pk, "dv"), _ptr(workspace),
+                              workspace.numel(), _stream(stream)), "r97q_attn_bwd")
+    return dq, dk, dv

@@ -1,0 +1,183 @@
+// attn.hip -- the C entries of attention's forward and backward: checks and the kernels' arguments. The
+// kernels are in attn_fwd.hip and attn_bwd.hip.
+#include <cmath>
+
+#include "attn.h"
+#include "status.h"
+
+namespace r97q {
+namespace attn {
+
+int launch_fwd(const Args& a, hipStream_t st);
+int launch_bwd(const Args& a, hipStream_t st);
+
+namespace {
+
+int refuse(int code, const char* who, const char* why) {
+    set_error("%s: %s", who, why);
+    return code;
+}
+
+// lens and forms; the sizes must keep every row index of a key head inside 31 bits
+int check_shape(const R97qAttnShape* p, int32_t hq, int32_t hk, const char* who) {
+    if (!p) return refuse(R97Q_EINVAL, who, "null shape");
+    if (p->head_dim <= 0 || p->head_dim % 8 || p->head_dim > 256)
+        return refuse(p->head_dim <= 0 ? R97Q_EINVAL : R97Q_EUNSUPPORTED, who, "head_dim is a multiple of 8, at most 256");
+    if (hk <= 0 || hq <= 0 || hq % hk) return refuse(R97Q_EINVAL, who, "the query heads are a multiple of the key heads");
+    if (p->batch < 0 || p->q_len < 0 || p->kv_len < 0) return refuse(R97Q_EINVAL, who, "a negative batch or length");
+    if (p->batch > 65535 || hk > 65535) return refuse(R97Q_EUNSUPPORTED, who, "at most 65535 sequences and key heads");
+    if (p->q_len > 0x7FFFFF00 / (hq / hk) || p->kv_len > 0x7FFFFF00)
+        return refuse(R97Q_EUNSUPPORTED, who, "a sequence's rows of one key head or its keys pass 31 bits");
+    if (p->window < 0 || (p->window && !p->causal)) return refuse(R97Q_EINVAL, who, "a window is positive and needs causal");
+    if (p->kv_starts && p->kv_lens) return refuse(R97Q_EINVAL, who, "kv_lens goes with the dense form of the keys");
+    if ((p->q_starts && p->q_tokens < 0) || (p->kv_starts && p->kv_tokens < 0))
+        return refuse(R97Q_EINVAL, who, "a negative count of packed tokens");
+    if (!std::isfinite(p->scale)) return refuse(R97Q_EINVAL, who, "the scale is not finite");
+    return R97Q_OK;
+}
+
+int check_heads(const R97qHeads* t, int32_t heads, bool f32, bool output, bool packed, int64_t batch, int64_t tokens,
+                const char* who, const char* name) {
+    if (!t || (!t->data && batch > 0 && tokens > 0)) {
+        set_error("%s: %s is null", who, name);
+        return R97Q_EINVAL;
+    }
+    if (t->heads != heads) {
+        set_error("%s: %s has %d heads, not %d", who, name, t->heads, heads);
+        return R97Q_EINVAL;
+    }
+    if (t->dtype != R97Q_BF16 && !(f32 && t->dtype == R97Q_F32)) {
+        set_error("%s: %s is %s", who, name, f32 ? "bf16 or f32" : "bf16");
+        return R97Q_EINVAL;
+    }
+    const int64_t unit = t->dtype == R97Q_F32 ? 4 : 8;
+    if ((reinterpret_cast<uintptr_t>(t->data) & 15) || t->token_stride % unit || t->head_stride % unit ||
+        (!packed && t->batch_stride % unit)) {
+        set_error("%s: %s starts and strides on 16 bytes", who, name);
+        return R97Q_EUNSUPPORTED;
+    }
+    if (t->token_stride < 0 || t->head_stride < 0 || (!packed && t->batch_stride < 0) ||
+        (output && ((tokens > 1 && !t->token_stride) || (heads > 1 && !t->head_stride) || (!packed && batch > 1 && !t->batch_stride)))) {
+        set_error("%s: %s has a negative stride, or is written through a stride of zero", who, name);
+        return R97Q_EINVAL;
+    }
+    return R97Q_OK;
+}
+
+Heads heads_of(const R97qHeads* t) {
+    return {static_cast<uint8_t*>(t->data), t->batch_stride, t->token_stride, t->head_stride, t->dtype == R97Q_F32};
+}
+
+Args args_of(const R97qAttnShape* p, int32_t hq, int32_t hk) {
+    Args a = {};
+    a.batch = p->batch;
+    a.hq = hq;
+    a.hk = hk;
+    a.g = hq / hk;
+    a.d = p->head_dim;
+    a.lq = p->q_len;
+    a.lk = p->kv_len;
+    a.q_starts = p->q_starts;
+    a.kv_starts = p->kv_starts;
+    a.kv_lens = p->kv_lens;
+    a.q_tokens = p->q_tokens;
+    a.kv_tokens = p->kv_tokens;
+    a.causal = p->causal != 0;
+    a.window = p->window;
+    a.scale = p->scale;
+    return a;
+}
+
+int64_t q_rows(const R97qAttnShape* p) { return p->q_starts ? p->q_tokens : p->q_len; }
+int64_t kv_rows(const R97qAttnShape* p) { return p->kv_starts ? p->kv_tokens : p->kv_len; }
+
+int64_t stat_bytes(const R97qAttnShape* p, int32_t hq) {
+    const int64_t n = p->q_starts ? (int64_t)hq * p->q_tokens : (int64_t)p->batch * hq * p->q_len;
+    return (4 * n + 255) / 256 * 256;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace r97q
+
+using namespace r97q;
+using namespace r97q::attn;
+
+extern "C" {
+
+int64_t r97q_attn_fwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads) {
+    clear_error();
+    if (check_shape(shape, q_heads, kv_heads, "r97q_attn_fwd_workspace_bytes")) return -1;
+    return 0;
+}
+
+int r97q_attn_fwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
+                  const R97qHeads* out, float* lse, void* workspace, int64_t workspace_bytes, R97IqrStream stream) {
+    clear_error();
+    const char* who = "r97q_attn_fwd";
+    if (!q || !k) return refuse(R97Q_EINVAL, who, "null q or k");
+    const int32_t hq = q->heads, hk = k->heads;
+    if (int e = check_shape(shape, hq, hk, who)) return e;
+    const int64_t n = q_rows(shape), m = kv_rows(shape), b = shape->batch;
+    const bool pq = shape->q_starts, pk = shape->kv_starts;
+    if (int e = check_heads(q, hq, false, false, pq, b, n, who, "q")) return e;
+    if (int e = check_heads(k, hk, false, false, pk, b, m, who, "k")) return e;
+    if (int e = check_heads(v, hk, false, false, pk, b, m, who, "v")) return e;
+    if (int e = check_heads(out, hq, true, true, pq, b, n, who, "out")) return e;
+    const int64_t need = r97q_attn_fwd_workspace_bytes(shape, hq, hk);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
+    if (b == 0 || n == 0 || shape->q_len == 0) return R97Q_OK;
+    Args a = args_of(shape, hq, hk);
+    a.q = heads_of(q);
+    a.k = heads_of(k);
+    a.v = heads_of(v);
+    a.o = heads_of(out);
+    a.lse = lse;
+    return launch_fwd(a, (hipStream_t)stream);
+}
+
+int64_t r97q_attn_bwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads) {
+    clear_error();
+    if (check_shape(shape, q_heads, kv_heads, "r97q_attn_bwd_workspace_bytes")) return -1;
+    return stat_bytes(shape, q_heads);
+}
+
+int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
+                  const R97qHeads* out, const float* lse, const R97qHeads* d_out, const R97qHeads* dq,
+                  const R97qHeads* dk, const R97qHeads* dv, void* workspace, int64_t workspace_bytes, R97IqrStream stream) {
+    clear_error();
+    const char* who = "r97q_attn_bwd";
+    if (!q || !k) return refuse(R97Q_EINVAL, who, "null q or k");
+    const int32_t hq = q->heads, hk = k->heads;
+    if (int e = check_shape(shape, hq, hk, who)) return e;
+    const int64_t n = q_rows(shape), m = kv_rows(shape), b = shape->batch;
+    const bool pq = shape->q_starts, pk = shape->kv_starts;
+    if (int e = check_heads(q, hq, false, false, pq, b, n, who, "q")) return e;
+    if (int e = check_heads(k, hk, false, false, pk, b, m, who, "k")) return e;
+    if (int e = check_heads(v, hk, false, false, pk, b, m, who, "v")) return e;
+    if (int e = check_heads(out, hq, true, false, pq, b, n, who, "out")) return e;
+    if (int e = check_heads(d_out, hq, false, false, pq, b, n, who, "d_out")) return e;
+    if (int e = check_heads(dq, hq, true, true, pq, b, n, who, "dq")) return e;
+    if (int e = check_heads(dk, hk, true, true, pk, b, m, who, "dk")) return e;
+    if (int e = check_heads(dv, hk, true, true, pk, b, m, who, "dv")) return e;
+    if (b == 0) return R97Q_OK;
+    if (!lse && n > 0) return refuse(R97Q_EINVAL, who, "null lse");
+    if (workspace_bytes < r97q_attn_bwd_workspace_bytes(shape, hq, hk) || (!workspace && n > 0))
+        return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
+    Args a = args_of(shape, hq, hk);
+    if (n == 0) a.lq = 0;
+    if (m == 0) a.lk = 0;
+    a.q = heads_of(q);
+    a.k = heads_of(k);
+    a.v = heads_of(v);
+    a.o = heads_of(out);
+    a.d_o = heads_of(d_out);
+    a.dq = heads_of(dq);
+    a.dk = heads_of(dk);
+    a.dv = heads_of(dv);
+    a.lse = const_cast<float*>(lse);
+    a.delta = static_cast<float*>(workspace);
+    return launch_bwd(a, (hipStream_t)stream);
+}
+
+}  // extern "C"

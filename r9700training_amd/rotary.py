@@ -1,0 +1,79 @@
+"""Rotary positions of the query and key heads on the card (a front over r97q_rotary and
+r97q_rotary_frequencies, include/r97q.h)."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import torch
+
+from . import (R97Q_BF16, R97Q_F32, R97Q_ROTARY_HALF, R97Q_ROTARY_INTERLEAVED, R97Q_ROTARY_LINEAR, R97Q_ROTARY_PLAIN,
+               R97Q_ROTARY_RAMP, Heads, _empty, _ptr, _stream, check, lib)
+
+PAIRS = {"half": R97Q_ROTARY_HALF, "interleaved": R97Q_ROTARY_INTERLEAVED}
+SCALINGS = {"plain": R97Q_ROTARY_PLAIN, "linear": R97Q_ROTARY_LINEAR, "ramp": R97Q_ROTARY_RAMP}
+
+
+def rotary_frequencies(rot: int, base: float = 10000.0, scaling: str = "plain", factor: float = 1.0,
+                       original: float = 0.0, slow: float = 1.0, fast: float = 32.0, device="cuda"):
+    """(inv_freq f64 [rot / 2] on `device`, mscale): base^(-2i / rot), for a context `factor` times the
+    `original` length divided by factor ("linear") or divided where a pair turns fewer than `slow` times over
+    the original length, kept where it turns more than `fast` times and blended between ("ramp")."""
+    if scaling not in SCALINGS:
+        raise ValueError(f"rotary_frequencies: scaling {scaling!r} is not one of {sorted(SCALINGS)}")
+    f = np.zeros(max(int(rot) // 2, 1), np.float64)
+    m = C.c_float(1.0)
+    check(lib().r97q_rotary_frequencies(int(rot), float(base), SCALINGS[scaling], float(factor), float(original),
+                                        float(slow), float(fast), f.ctypes.data_as(C.c_void_p), C.byref(m)),
+          "r97q_rotary_frequencies")
+    return torch.from_numpy(f).to(device), float(m.value)
+
+
+def _heads(x: torch.Tensor, what: str) -> Heads:
+    if x.dim() != 3 or x.stride(2) != 1 or not x.is_cuda:
+        raise ValueError(f"rotary: {what} is a device [tokens, heads, head_dim] tensor, head_dim consecutive")
+    if x.dtype == torch.bfloat16:
+        dt = R97Q_BF16
+    elif x.dtype == torch.float32:
+        dt = R97Q_F32
+    else:
+        raise ValueError(f"rotary: {what} is bf16 or f32")
+    return Heads(x.data_ptr(), 0, x.stride(0), x.stride(1), x.shape[1], dt)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
+           pairs: str = "half", mscale: float = 1.0, inverse: bool = False, q_out: torch.Tensor | None = None,
+           k_out: torch.Tensor | None = None, stream=None):
+    """(q, k) [tokens, heads, head_dim] turned by positions * inv_freq (positions None: 0, 1, ..); k may be
+    None. The first 2 * len(inv_freq) values of a head turn, the rest are copied. inverse: the adjoint
+    (turned back, scaled by the same mscale). q_out / k_out may be q / k."""
+    if pairs not in PAIRS:
+        raise ValueError(f"rotary: pairs {pairs!r} are not one of {sorted(PAIRS)}")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or not inv_freq.is_cuda:
+        raise ValueError("rotary: inv_freq is a contiguous f64 [rot / 2] device tensor")
+    tokens, _, dim = q.shape if q.dim() == 3 else (0, 0, 0)
+    wide = 0
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (tokens,) \
+                or not positions.is_contiguous() or not positions.is_cuda:
+            raise ValueError("rotary: positions are a contiguous int32 or int64 [tokens] device tensor")
+        wide = int(positions.dtype == torch.int64)
+    hq = _heads(q, "q")
+    if q_out is None:
+        q_out = _empty(q.shape, q.dtype, q.device, stream)
+    ho = _heads(q_out, "q_out")
+    hk = hko = None
+    if k is not None:
+        hk = _heads(k, "k")
+        if k_out is None:
+            k_out = _empty(k.shape, k.dtype, k.device, stream)
+        hko = _heads(k_out, "k_out")
+        if k.shape[0] != tokens or k.shape[2] != dim or k_out.shape != k.shape:
+            raise ValueError("rotary: k has q's tokens and head_dim, k_out k's shape")
+    elif k_out is not None:
+        raise ValueError("rotary: k_out without k")
+    if q_out.shape != q.shape:
+        raise ValueError("rotary: q_out has q's shape")
+    check(lib().r97q_rotary(hq, ho, hk, hko, tokens, dim, 2 * inv_freq.shape[0], PAIRS[pairs], _ptr(inv_freq),
+                            _ptr(positions), wide, float(mscale), int(bool(inverse)), _stream(stream)), "r97q_rotary")
+    return q_out, k_out

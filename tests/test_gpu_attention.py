@@ -1,0 +1,320 @@
+"""Attention's forward and backward against float64, at the lengths, head groups, masks and layouts where they
+can go wrong. Every tolerance counts roundings at half a step (tests/between_ref.py)."""
+import math
+
+import pytest
+import torch
+
+import between_ref as R
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def rnd(seed, *shape, std=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (std * torch.randn(shape, generator=g, device="cuda")).to(BF)
+
+
+def close(got, want, tol, what):
+    got = got.double()
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fin), f"{what}: other places are finite"
+    assert torch.equal(got[~fin], want[~fin]), what
+    off = (got - want).abs()[fin] - tol[fin]
+    worst = float(off.max()) if off.numel() else -1.0
+    print(f"{what}: largest |error| / tolerance {float(((got - want).abs()[fin] / (tol[fin] + 1e-300)).max()) if off.numel() else 0:.3f}",
+          flush=True)
+    # values that underflow: an absolute floor far below any of the inputs' products
+    assert worst <= 1e-30, f"{what}: {worst} past the tolerance"
+
+
+def run(q, k, v, do, seqs, heads, kv_heads, causal, window, scale, out_dtype=BF, grad_dtype=BF, back=True, **kw):
+    """Both directions through the package, against the reference of the sequences `seqs`: (query rows, key rows,
+    index) of each, as functions on the tensors."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    out, lse = attention_fwd(q, k, v, causal=causal, window=window, scale=scale, out_dtype=out_dtype, **kw)
+    ref = R.reference([(s.q(q).double(), s.k(k).double(), s.k(v).double(), s.q(do).double() if back else None) for s in seqs],
+                      heads, kv_heads, causal, window, scale, R.HALF[out_dtype], R.HALF[grad_dtype])
+    torch.cuda.synchronize()
+    for i, (s, r) in enumerate(zip(seqs, ref)):
+        close(s.q(out), *r["out"], f"out of sequence {i}")
+        close(s.stat(lse), *r["lse"], f"lse of sequence {i}")
+    if not back:
+        return out, lse
+    dq, dk, dv = attention_bwd(q, k, v, out, lse, do, causal=causal, window=window, scale=scale, grad_dtype=grad_dtype, **kw)
+    torch.cuda.synchronize()
+    for i, (s, r) in enumerate(zip(seqs, ref)):
+        close(s.q(dq), *r["dq"], f"dq of sequence {i}")
+        close(s.k(dk), *r["dk"], f"dk of sequence {i}")
+        close(s.k(dv), *r["dv"], f"dv of sequence {i}")
+    return out, lse, dq, dk, dv
+
+
+class Dense:
+    def __init__(self, b, lk):
+        self.b, self.lk = b, lk
+
+    def q(self, x):
+        return x[self.b]
+
+    def k(self, x):
+        return x[self.b, :self.lk]
+
+    def stat(self, x):
+        return x[self.b]
+
+
+class Packed:
+    def __init__(self, q0, q1, k0, k1):
+        self.at = (q0, q1, k0, k1)
+
+    def q(self, x):
+        return x[self.at[0]:self.at[1]]
+
+    def k(self, x):
+        return x[self.at[2]:self.at[3]]
+
+    def stat(self, x):
+        return x[:, self.at[0]:self.at[1]]
+
+
+DENSE = [
+    # batch, q_len, kv_len, q_heads, kv_heads, head_dim, causal, window
+    (1, 1, 1, 1, 1, 64, True, 0),
+    (2, 1, 77, 4, 1, 64, True, 0),
+    (1, 1, 1000, 6, 1, 128, True, 0),
+    (2, 1, 513, 24, 4, 256, True, 0),
+    (1, 3, 200, 14, 2, 128, True, 0),
+    (1, 31, 31, 2, 2, 64, True, 0),
+    (1, 32, 32, 2, 1, 128, True, 0),
+    (1, 33, 65, 3, 1, 80, True, 0),
+    (2, 128, 128, 8, 2, 64, True, 0),
+    (1, 129, 129, 4, 2, 128, True, 0),
+    (1, 255, 257, 2, 1, 256, True, 0),
+    (1, 300, 300, 2, 2, 64, False, 0),
+    (1, 100, 37, 3, 3, 128, False, 0),
+    (1, 97, 40, 2, 1, 64, True, 0),       # the first 57 queries see nothing
+    (1, 200, 1, 2, 2, 256, True, 0),
+    (2, 70, 0, 4, 2, 64, True, 0),        # no keys at all
+    (1, 190, 190, 2, 1, 64, True, 1),     # each query its own key
+    (1, 190, 260, 2, 1, 128, True, 50),
+    (1, 260, 200, 4, 4, 256, True, 33),
+    (2, 400, 400, 6, 2, 64, True, 128),
+    (1, 65, 65, 2, 1, 8, True, 0),
+    (1, 65, 70, 2, 2, 40, True, 0),
+    (1, 40, 40, 7, 1, 248, True, 0),
+    (1, 50, 90, 5, 1, 72, False, 0),
+    (3, 5, 2000, 8, 2, 64, True, 0),
+    (1, 520, 520, 12, 2, 128, True, 0),
+]
+
+
+@pytest.mark.parametrize("b,lq,lk,hq,hk,d,causal,window", DENSE)
+def test_dense(b, lq, lk, hq, hk, d, causal, window):
+    print(f"case dense {(b, lq, lk, hq, hk, d, causal, window)}", flush=True)
+    q, do = rnd(1, b, lq, hq, d), rnd(4, b, lq, hq, d)
+    k, v = rnd(2, b, lk, hk, d), rnd(3, b, lk, hk, d)
+    run(q, k, v, do, [Dense(i, lk) for i in range(b)], hq, hk, causal, window, 1.0 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_f32_outputs(d):
+    q, do = rnd(1, 2, 150, 4, d), rnd(4, 2, 150, 4, d)
+    k, v = rnd(2, 2, 150, 2, d), rnd(3, 2, 150, 2, d)
+    run(q, k, v, do, [Dense(i, 150) for i in range(2)], 4, 2, True, 0, 0.1, out_dtype=torch.float32, grad_dtype=torch.float32)
+
+
+PACKED = [
+    # query lengths, key lengths, q_heads, kv_heads, head_dim, causal, window
+    ([1, 129, 0, 64, 37], None, 4, 2, 64, True, 0),
+    ([300, 5, 1, 211], None, 4, 1, 128, True, 0),
+    ([130, 131], None, 2, 2, 256, True, 100),
+    ([1, 1, 3, 1], [500, 1, 90, 33], 8, 2, 128, True, 0),
+    ([40, 20, 7], [0, 20, 3], 2, 1, 64, True, 0),
+    ([64, 65], [100, 10], 2, 1, 80, False, 0),
+]
+
+
+@pytest.mark.parametrize("lq,lk,hq,hk,d,causal,window", PACKED)
+def test_packed(lq, lk, hq, hk, d, causal, window):
+    print(f"case packed {(lq, lk, hq, hk, d, causal, window)}", flush=True)
+    lk = lq if lk is None else lk
+    qs = torch.tensor([0] + lq).cumsum(0).to(torch.int32).cuda()
+    ks = torch.tensor([0] + lk).cumsum(0).to(torch.int32).cuda()
+    q, do = rnd(1, sum(lq), hq, d), rnd(4, sum(lq), hq, d)
+    k, v = rnd(2, sum(lk), hk, d), rnd(3, sum(lk), hk, d)
+    seqs, a, b = [], 0, 0
+    for x, y in zip(lq, lk):
+        seqs.append(Packed(a, a + x, b, b + y))
+        a, b = a + x, b + y
+    run(q, k, v, do, seqs, hq, hk, causal, window, 1.0 / math.sqrt(d), q_starts=qs, kv_starts=ks, max_q=max(lq), max_kv=max(lk))
+
+
+@pytest.mark.parametrize("lq", [1, 2, 40])
+def test_cache_lengths(lq):
+    """A cache longer than what is in use, its unused places NaN: they are not read."""
+    lens = [0, 1, 64, 65, 300, 299]
+    q, do = rnd(1, 6, lq, 8, 128), rnd(4, 6, lq, 8, 128)
+    k, v = rnd(2, 6, 300, 2, 128), rnd(3, 6, 300, 2, 128)
+    for i, n in enumerate(lens):
+        k[i, n:] = float("nan")
+        v[i, n:] = float("nan")
+    got = run(q, k, v, do, [Dense(i, n) for i, n in enumerate(lens)], 8, 2, True, 0, 0.09,
+              kv_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    for g in got[3:]:
+        for i, n in enumerate(lens):
+            assert torch.equal(g[i, n:], torch.zeros_like(g[i, n:]))
+
+
+def test_packed_queries_over_a_cache():
+    """New tokens of several sequences packed, each against its own part of a dense cache."""
+    from r9700training_amd.attention import attention_fwd
+
+    lq, lens = [5, 1, 17], [90, 33, 17]
+    qs = torch.tensor([0, 5, 6, 23], dtype=torch.int32, device="cuda")
+    q, k, v = rnd(1, 23, 4, 64), rnd(2, 3, 96, 2, 64), rnd(3, 3, 96, 2, 64)
+    out, lse = attention_fwd(q, k, v, q_starts=qs, max_q=17, kv_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    ref = R.reference([(q[a:a + n].double(), k[i, :m].double(), v[i, :m].double(), None)
+                       for i, (a, n, m) in enumerate(zip((0, 5, 6), lq, lens))], 4, 2, True, 0, 0.125, R.HALF[BF])
+    for (a, n), r in zip(((0, 5), (5, 1), (6, 17)), ref):
+        close(out[a:a + n], *r["out"], "out")
+        close(lse[:, a:a + n], *r["lse"], "lse")
+
+
+def test_longest_too_short_and_bad_starts():
+    """The longest length only sizes the launch; starts that leave the tensors are clamped to them."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    q, k, v, do = (rnd(i, 300, 2, 64) for i in range(4))
+    good = torch.tensor([0, 200, 300], dtype=torch.int32, device="cuda")
+    a = attention_fwd(q, k, v, q_starts=good, kv_starts=good, max_q=200, max_kv=200)
+    b = attention_fwd(q, k, v, q_starts=good, kv_starts=good, max_q=60, max_kv=10)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    x = attention_bwd(q, k, v, a[0], a[1], do, q_starts=good, kv_starts=good, max_q=200, max_kv=200)
+    y = attention_bwd(q, k, v, a[0], a[1], do, q_starts=good, kv_starts=good, max_q=60, max_kv=10)
+    assert all(torch.equal(m, n) for m, n in zip(x, y))
+    wild = torch.tensor([-7, 200, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    c = attention_fwd(q, k, v, q_starts=wild, kv_starts=wild, max_q=200, max_kv=200)
+    assert torch.equal(a[0], c[0])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_layouts(d):
+    """Views of a fused projection, of a [batch, heads, tokens, head_dim] cache, and a key broadcast over the batch
+    give the bits of the contiguous tensors; gradients may go into such views."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    b, n, hq, hk = 2, 150, 4, 2
+    fused = rnd(1, b, n, (hq + 2 * hk) * d)
+    q = fused[..., :hq * d].unflatten(-1, (hq, d))
+    k = fused[..., hq * d:(hq + hk) * d].unflatten(-1, (hk, d))
+    v = fused[..., (hq + hk) * d:].unflatten(-1, (hk, d))
+    do = rnd(2, b, hq, n, d).transpose(1, 2)
+    want, lse = attention_fwd(q.contiguous(), k.contiguous(), v.contiguous())
+    out = torch.full((b, hq, n, d), float("nan"), dtype=BF, device="cuda").transpose(1, 2)
+    got, lse2 = attention_fwd(q, k, v, out=out)
+    assert torch.equal(got, want) and torch.equal(lse, lse2)
+    grads = attention_bwd(q.contiguous(), k.contiguous(), v.contiguous(), want, lse, do.contiguous())
+    into = torch.full_like(fused, float("nan"))
+    parts = [into[..., :hq * d].unflatten(-1, (hq, d)), into[..., hq * d:(hq + hk) * d].unflatten(-1, (hk, d)),
+             into[..., (hq + hk) * d:].unflatten(-1, (hk, d))]
+    got = attention_bwd(q, k, v, out, lse, do, dq=parts[0], dk=parts[1], dv=parts[2])
+    assert all(torch.equal(x, y) for x, y in zip(got, grads))
+    one = k[:1].expand(b, n, hk, d)
+    x = attention_fwd(q, one, v)
+    y = attention_fwd(q, one.contiguous(), v)
+    assert torch.equal(x[0], y[0])
+    gx = attention_bwd(q, one, v, *x, do)
+    gy = attention_bwd(q, one.contiguous(), v, *x, do)
+    assert all(torch.equal(m, n) for m, n in zip(gx, gy))
+
+
+@pytest.mark.parametrize("d,lq,lk", [(64, 130, 130), (128, 1, 700), (256, 70, 200)])
+def test_steep_scores(d, lq, lk):
+    """Scores of hundreds, rising along the keys so that the running maximum moves at every tile, and falling."""
+    for rise in (1.0, -1.0):
+        q = torch.ones((1, lq, 2, d), device="cuda").to(BF)
+        ramp = rise * torch.arange(lk, device="cuda", dtype=torch.float32)[None, :, None, None] * 0.5
+        k = (ramp.expand(1, lk, 1, d) / d + 0.01 * rnd(2, 1, lk, 1, d).float()).to(BF)
+        run(q, k, rnd(3, 1, lk, 1, d), rnd(4, 1, lq, 2, d), [Dense(0, lk)], 2, 1, False, 0, 1.0)
+
+
+def test_scale_zero_and_negative():
+    for scale in (0.0, -0.2):
+        run(rnd(1, 1, 90, 2, 64), rnd(2, 1, 90, 2, 64), rnd(3, 1, 90, 2, 64), rnd(4, 1, 90, 2, 64), [Dense(0, 90)], 2, 2, True, 0, scale)
+
+
+def test_long_cache_offsets():
+    """Keys whose byte offsets pass 32 bits: the last tokens of a cache of 9 x 2^30 bytes in one tensor."""
+    from r9700training_amd.attention import attention_fwd
+
+    n, d = 36000, 128
+    k = torch.zeros((1, n, 1024, d), dtype=BF, device="cuda")[:, :, 1000:1001]  # a token 256 KiB from the next
+    v = torch.zeros((1, n, 1024, d), dtype=BF, device="cuda")[:, :, 1000:1001]
+    k.copy_(rnd(2, 1, n, 1, d))
+    v.copy_(rnd(3, 1, n, 1, d))
+    q = rnd(1, 1, 2, 4, d)
+    got, lse = attention_fwd(q, k, v)
+    want, lse2 = attention_fwd(q, k.contiguous(), v.contiguous())
+    assert torch.equal(got, want) and torch.equal(lse, lse2)
+    run(q, k.contiguous(), v.contiguous(), None, [Dense(0, n)], 4, 1, True, 0, 1.0 / math.sqrt(d), back=False)
+
+
+def test_same_bits_and_graph_replay():
+    """Repeated calls give the same bits, also on another stream, and captured into a graph and replayed with
+    eager work between the replays."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    cases = [(1, 300, 300, 8, 2, 128), (2, 1, 900, 8, 2, 64), (1, 64, 64, 4, 4, 256)]
+    for b, lq, lk, hq, hk, d in cases:
+        q, k, v, do = rnd(1, b, lq, hq, d), rnd(2, b, lk, hk, d), rnd(3, b, lk, hk, d), rnd(4, b, lq, hq, d)
+
+        def step():
+            out, lse = attention_fwd(q, k, v)
+            return (out, lse) + attention_bwd(q, k, v, out, lse, do)
+
+        want = step()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            again = step()
+            step()
+        o2, l2 = attention_fwd(q, k, v, stream=side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(want, again)) and torch.equal(o2, want[0]) and torch.equal(l2, want[1])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        for seed in (11, 12, 13):
+            q.copy_(rnd(seed, b, lq, hq, d))
+            want = [x.clone() for x in step()]
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(want, held)), seed
+
+
+def test_gradient_against_differences():
+    """The kernels' gradient along a direction against the kernels' own forward, f32 out. The forward's outputs are off by at
+    most 2^-8 of sum p |v| each, so the quotient by twice that over the step, and by the third derivative's
+    step^2 (a step of 1/16 of inputs of size 1 under a scale of 1/8)."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    q, k, v, do = rnd(1, 1, 64, 2, 64), rnd(2, 1, 64, 1, 64), rnd(3, 1, 64, 1, 64), rnd(4, 1, 64, 2, 64)
+    out, lse = attention_fwd(q, k, v, out_dtype=torch.float32)
+    grads = attention_bwd(q, k, v, out, lse, do, grad_dtype=torch.float32)
+    for name, x, g in zip("qkv", (q, k, v), grads):
+        # a direction along the gradient's signs: the quotient is a sum of like terms, far above the roundings
+        u = torch.sign(g) / 16
+        hi, lo = (x.float() + u).to(BF), (x.float() - u).to(BF)
+        moved = (hi.double() - lo.double()) / 2
+        args = {n: t for n, t in zip("qkv", (q, k, v))}
+        f = []
+        for y in (hi, lo):
+            o, _ = attention_fwd(*({**args, name: y}[n] for n in "qkv"), out_dtype=torch.float32)
+            f.append(float((o.double() * do.double()).sum()))
+        want = float((g.double() * moved).sum())
+        got = (f[0] - f[1]) / 2
+        noise = 2 ** -8 * float((do.double().abs() * v.double().abs().mean()).sum()) / math.sqrt(do.numel())
+        assert abs(got - want) <= 0.02 * abs(want) + 4 * noise, (name, got, want, noise)

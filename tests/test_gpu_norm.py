@@ -1,0 +1,192 @@
+"""The residual's addition, the RMS norm and the 8-bit output, forward and adjoint, against float64: both types, odd and
+wide rows, every kind of group, rows of zeros, tiny and huge values. Tolerances count f32 roundings: a sum over n
+values in f32 is off by less than n roundings of its size."""
+import pytest
+import torch
+
+import between_ref as R
+
+pytestmark = pytest.mark.gpu
+EPS = 1e-6
+
+
+def rnd(seed, *shape, dtype=torch.bfloat16, std=1.0):
+    return (std * torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")).to(dtype)
+
+
+def forward(rows, n, group, dtype, residual=True, wadd=0.0, std=1.0, x=None):
+    from r9700training_amd.norm import add_rmsnorm_i8g
+
+    x = rnd(1, rows, n, dtype=dtype, std=std) if x is None else x
+    r = rnd(2, rows, n, dtype=dtype, std=2 * std) if residual else None
+    w = (1.0 + 0.2 * rnd(3, n, dtype=torch.float32)).to(dtype)
+    codes, scale, h, y, rs = add_rmsnorm_i8g(x, r, w, group, eps=EPS, wadd=wadd, want_y=True)
+    torch.cuda.synchronize()
+    wh, wrs, wy = R.norm(x, r, w, EPS, wadd, dtype)
+    assert torch.equal(h.double(), wh)
+    rel = (n + 8) * R.U32  # the sum of squares and the few roundings after it
+    assert bool(((rs.double() - wrs).abs() <= rel * wrs).all())
+    y_tol = (rel + 4 * R.U32) * wy.abs()
+    assert bool(((y.double() - wy).abs() <= y_tol + R.HALF[torch.bfloat16] * wy.abs()).all())
+    want = R.group_scale(wy, group)
+    assert bool(((scale.double() - want).abs() <= (rel + 6 * R.U32) * want).all())
+    each = scale.double()[:, R.group_index(n, group, x.device)]
+    # a code is the nearest to y / scale: half a step, y's error and the quotient's
+    off = (codes.double() * each - wy).abs() - (0.5 * each + y_tol + 4 * R.U32 * wy.abs() + 1e-300)
+    assert float(off.max()) <= 0.0, float(off.max())
+    top = torch.zeros_like(scale, dtype=torch.int32)
+    top.scatter_reduce_(1, R.group_index(n, group, x.device).expand(rows, n), codes.int().abs(), "amax")
+    zero = R.group_scale(wy, group) == 1.0
+    assert bool(((top == 127) | (zero & (top == 0)) | (want == 1.0)).all())
+    return x, r, w, codes, scale, h, y, rs
+
+
+SHAPES = [(1, 1, 0), (3, 7, 0), (5, 64, 0), (5, 64, 8), (4, 100, 32), (9, 128, 128), (7, 130, 128), (33, 512, 64), (65, 1000, 0),
+          (17, 1024, 16), (5, 2040, 0), (21, 2048, 128), (5, 2056, 128), (3, 4096, 512), (6, 5120, 0), (6, 5120, 128),
+          (2, 5120, 1024), (3, 6000, 48), (3, 8192, 128), (2, 8200, 128), (2, 12288, 0), (2, 17408, 256), (40, 256, 24),
+          (3, 515, 5), (2, 5120, 5119)]
+
+
+@pytest.mark.parametrize("rows,n,group", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_forward(rows, n, group, dtype):
+    print(f"case norm forward {(rows, n, group, dtype)}", flush=True)
+    forward(rows, n, group, dtype)
+    forward(rows, n, group, dtype, residual=False, wadd=1.0)
+
+
+@pytest.mark.parametrize("rows,n,group", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_backward(rows, n, group, dtype):
+    from r9700training_amd.norm import add_rmsnorm_i8g_bwd
+
+    print(f"case norm backward {(rows, n, group, dtype)}", flush=True)
+    _, _, w, _, scale, h, _, rs = forward(rows, n, group, dtype, wadd=0.5)
+    gc, gy, gh = rnd(4, rows, n, dtype=dtype, std=0.01), rnd(5, rows, n, dtype=dtype), rnd(6, rows, n, dtype=dtype)
+    for use in ((gc, gy, gh), (gc, None, None), (None, gy, gh), (None, None, None)):
+        dx, dw = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale if use[0] is not None else None, g_codes=use[0], g_y=use[1],
+                                     g_h=use[2], wadd=0.5)
+        # from rstd as it is given
+        wdx, wdw, e = R.norm_backward(h.double(), rs.double(), w, 0.5, scale, group, *use)
+        we, x = ((w.double() + 0.5) * e).abs(), (h.double() * rs.double()[:, None]).abs()
+        rel = (n + 16) * R.U32
+        tol = rs.double()[:, None] * (8 * R.U32 * we + rel * x * (we * x).mean(1, keepdim=True)) + 8 * R.U32 * wdx.abs()
+        tol = tol + R.HALF[dtype] * wdx.abs()
+        assert bool(((dx.double() - wdx).abs() <= tol + 1e-30).all()), use
+        assert bool(((dw.double() - wdw).abs() <= (rows + 8) * R.U32 * (e * x).abs().sum(0) + 1e-30).all()), use
+    start = rnd(7, n, dtype=torch.float32)
+    dw = start.clone()
+    dx, dw = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale, g_codes=gc, g_y=gy, g_h=gh, wadd=0.5, dw=dw, accumulate=True)
+    dx2, dw2 = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale, g_codes=gc, g_y=gy, g_h=gh, wadd=0.5)
+    assert torch.equal(dw, start + dw2) and torch.equal(dx, dx2)
+    dx3, none = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale, g_codes=gc, g_y=gy, g_h=gh, wadd=0.5, want_dw=False)
+    assert none is None and torch.equal(dx3, dx)
+    for k in range(3):  # dx over a cotangent
+        gs = [gc.clone(), gy.clone(), gh.clone()]
+        dx4, _ = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale, g_codes=gs[0], g_y=gs[1], g_h=gs[2], wadd=0.5, dx=gs[k])
+        assert torch.equal(dx4, dx)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 511, 512, 513, 1500, 5000])
+def test_many_rows(rows):
+    """Row counts around the workgroups' shares, the gain's gradient summed over all of them, the same bits twice."""
+    from r9700training_amd.norm import add_rmsnorm_i8g_bwd
+
+    for n, group in ((256, 128), (4096, 0)):
+        _, _, w, _, scale, h, _, rs = forward(rows, n, group, torch.bfloat16)
+        gy = rnd(5, rows, n)
+        dx, dw = add_rmsnorm_i8g_bwd(h, w, rs, group, g_y=gy)
+        wdx, wdw, e = R.norm_backward(h.double(), rs.double(), w, 0.0, scale, group, None, gy, None)
+        assert bool(((dw.double() - wdw).abs() <= (rows + 8) * R.U32 * (e * h.double() * rs.double()[:, None]).abs().sum(0)).all())
+        again = add_rmsnorm_i8g_bwd(h, w, rs, group, g_y=gy)
+        assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+
+
+@pytest.mark.parametrize("n,group", [(512, 128), (5120, 0), (333, 0)])
+def test_zero_tiny_and_huge_rows(n, group):
+    from r9700training_amd.norm import add_rmsnorm_i8g
+
+    x = rnd(1, 6, n, dtype=torch.float32)
+    x[0] = 0.0
+    x[1] *= 1e-30
+    x[2] *= 1e15
+    x[3, :n // 2] = 0.0
+    x[4] *= 1e-3
+    forward(6, n, group, torch.float32, residual=False, x=x)
+    # a gain of zeros: y is zero everywhere, the scales are 1
+    codes, scale, h, y, rs = add_rmsnorm_i8g(x, None, torch.zeros(n, device="cuda"), group, eps=EPS, want_y=True)
+    assert int(codes.abs().max()) == 0 and torch.equal(scale, torch.ones_like(scale)) and float(y.abs().max()) == 0.0
+    # a tiny gain: amax / 127 is far below one, codes still span the range
+    codes, scale, _, _, _ = add_rmsnorm_i8g(x, None, torch.full((n,), 1e-33, device="cuda"), group, eps=EPS)
+    assert int(codes[4].abs().max()) == 127 and int(codes[2].abs().max()) == 127
+
+
+def test_outputs_given_in_place_and_optional():
+    from r9700training_amd.norm import add_rmsnorm_i8g
+
+    for n, group in ((2048, 128), (5120, 0), (777, 32)):
+        for dtype in (torch.bfloat16, torch.float32):
+            x, r, w, codes, scale, h, y, rs = forward(19, n, group, dtype)
+            for which in ("x", "r"):
+                a, b = x.clone(), r.clone()
+                got = add_rmsnorm_i8g(a, b, w, group, eps=EPS, want_y=True, h=a if which == "x" else b)
+                for p, q in zip(got, (codes, scale, h, y, rs)):
+                    assert torch.equal(p, q), which
+            got = add_rmsnorm_i8g(x, r, w, group, eps=EPS, want_codes=False, want_y=True)
+            assert got[0] is None and got[1] is None and torch.equal(got[3], y) and torch.equal(got[2], h)
+            got = add_rmsnorm_i8g(x, r, w, group, eps=EPS)
+            assert got[3] is None and torch.equal(got[0], codes)
+
+
+def test_unaligned_rows():
+    """Tensors off 16 bytes take the general kernels: the same values to their roundings."""
+    from r9700training_amd.norm import add_rmsnorm_i8g, add_rmsnorm_i8g_bwd
+
+    n, rows = 1024, 9
+    for off in (1, 3):
+        pad = rnd(1, rows * n + 8)
+        x = pad[off:off + rows * n].view(rows, n)
+        forward(rows, n, 128, torch.bfloat16, x=x)
+        w = rnd(3, n)
+        _, _, h, _, rs = add_rmsnorm_i8g(x, None, w, eps=EPS)
+        gy = rnd(4, rows, n)
+        dx, dw = add_rmsnorm_i8g_bwd(h, w, rs, g_y=gy)
+        wdx, _, _ = R.norm_backward(x.double(), rs.double(), w, 0.0, None, 0, None, gy, None)
+        assert float((dx.double() - wdx).norm() / wdx.norm()) <= 2 ** -8
+
+
+def test_stream_and_graph():
+    from r9700training_amd.norm import add_rmsnorm_i8g, add_rmsnorm_i8g_bwd
+
+    x, r, w = rnd(1, 700, 1024), rnd(2, 700, 1024), rnd(3, 1024)
+    gc = rnd(4, 700, 1024)
+
+    def step(**kw):
+        codes, scale, h, _, rs = add_rmsnorm_i8g(x, r, w, 128, eps=EPS, **kw)
+        return (codes, scale, h, rs) + add_rmsnorm_i8g_bwd(h, w, rs, 128, scale=scale, g_codes=gc, **kw)
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = step(stream=side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        x.copy_(rnd(10 + i, 700, 1024))
+        want = [t.clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, held)), i
+
+
+def test_no_rows():
+    from r9700training_amd.norm import add_rmsnorm_i8g, add_rmsnorm_i8g_bwd
+
+    x, w = rnd(1, 0, 256), rnd(2, 256)
+    codes, scale, h, y, rs = add_rmsnorm_i8g(x, None, w, 128)
+    assert codes.shape == (0, 256) and scale.shape == (0, 2)
+    dx, dw = add_rmsnorm_i8g_bwd(x, w, rs, 128, g_y=x)
+    assert dx.shape == (0, 256) and float(dw.abs().max()) == 0.0
