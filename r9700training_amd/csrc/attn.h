@@ -35,6 +35,7 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMostSplits = 256;  // ranges of the keys that the forward's join adds
 
 // one tensor of heads: element (b, t, h, d) at data[b * bs + t * ts + h * hs + d]
 struct Heads {
@@ -47,31 +48,43 @@ struct Args {
     Heads q, k, v, o;    // o: the forward's output, written there and read in the backward
     Heads d_o, dq, dk, dv;
     float* lse;          // [b][h][Lq], packed: [h][q_tokens]
-    float* delta;        // backward: sum over d of dO * O, laid out as lse
+    float2* base;        // backward: (log-sum-exp in base 2, sum over d of dO * O) a row, laid out as lse
     int32_t batch, hq, hk, g, d;
-    int64_t lq, lk;      // tokens of a sequence (packed: of the longest)
+    int32_t lq, lk;      // tokens of a sequence (packed: of the longest)
     const int32_t* q_starts;
     const int32_t* kv_starts;
     const int32_t* kv_lens;
     int64_t q_tokens, kv_tokens;
     int32_t causal;
-    int64_t window;      // 0: none
+    int32_t window;      // 0: none
     float scale;         // of the scores
-    // the split forward: partial results of a row tile's key ranges
-    int32_t splits;
-    int32_t tiles;       // row tiles in the grid
-    float* part;         // [split][b][h][Lq][D] f32, then (m, l) pairs [split][b][h][Lq]
+    // the forward split over the keys: ranges of `chunk` keys, each one's unnormalised sums in f32 and (m, l)
+    int32_t splits, chunk;
+    int64_t slots;       // rows of one range: every query head's
+    float* part;         // [splits][slots][d]
+    float2* stats;       // [splits][slots]
 };
 
 // one sequence: its tokens' places and counts. Starts and lengths come from device memory, so they are
 // clamped to the tensors: nothing is read or written past them whatever they hold.
 struct Seq {
-    int64_t q_base, k_base;  // token offsets (packed) into the whole tensors; 0 in the dense form
-    int64_t b;
-    int64_t lq, lk, off;     // off: query i stands at key position i + off
+    int32_t b;
+    int32_t q_base, k_base;  // token offsets (packed) into the whole tensors; 0 in the dense form
+    int32_t lq, lk, off;     // off: query i stands at key position i + off
 };
 
 __device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// the same value, but what follows from it is computed here: otherwise the many comparisons with the head's width
+// that a row's loads and stores make are computed once, before the loop, and held in registers through it
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ int fresh_lane(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
 __device__ __forceinline__ Seq sequence(const Args& a, int b) {
     Seq s;
@@ -79,15 +92,19 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
     s.q_base = s.k_base = 0;
     s.lq = a.lq;
     s.lk = a.lk;
-    if (a.q_starts) {
-        s.q_base = clamp64(a.q_starts[b], 0, a.q_tokens);
-        s.lq = clamp64(a.q_starts[b + 1], s.q_base, a.q_tokens) - s.q_base;
+    if (a.q_starts) {  // starts are int32: a tensor's tokens past 2^31 - 1 are out of their reach
+        s.q_base = (int)clamp64(uniform(a.q_starts[b]), 0, a.q_tokens);
+        s.lq = (int)clamp64(uniform(a.q_starts[b + 1]), s.q_base, a.q_tokens > s.q_base ? a.q_tokens : s.q_base) - s.q_base;
+        // a key head's rows stay inside 31 bits whatever the starts hold
+        const int most = 0x7FFFFF00 / a.g;
+        if (s.lq > most) s.lq = most;
     }
     if (a.kv_starts) {
-        s.k_base = clamp64(a.kv_starts[b], 0, a.kv_tokens);
-        s.lk = clamp64(a.kv_starts[b + 1], s.k_base, a.kv_tokens) - s.k_base;
+        s.k_base = (int)clamp64(uniform(a.kv_starts[b]), 0, a.kv_tokens);
+        s.lk = (int)clamp64(uniform(a.kv_starts[b + 1]), s.k_base, a.kv_tokens > s.k_base ? a.kv_tokens : s.k_base) - s.k_base;
+        if (s.lk > 0x7FFFFF00) s.lk = 0x7FFFFF00;
     } else if (a.kv_lens) {
-        s.lk = clamp64(a.kv_lens[b], 0, a.lk);
+        s.lk = (int)clamp64(uniform(a.kv_lens[b]), 0, a.lk);
     }
     s.off = s.lk - s.lq;
     return s;
@@ -103,16 +120,26 @@ __device__ __forceinline__ uint8_t* kv_at(const Heads& t, const Args& a, const S
     return t.data + (t.f32 ? 4 * e : 2 * e);
 }
 // where a row's log-sum-exp (and delta) lies
-__device__ __forceinline__ int64_t stat_at(const Args& a, const Seq& s, int h, int64_t token) {
-    return a.q_starts ? h * a.q_tokens + s.q_base + token : (s.b * a.hq + h) * a.lq + token;
+__device__ __forceinline__ int64_t stat_at(const Args& a, const Seq& s, int h, int token) {
+    return a.q_starts ? h * a.q_tokens + s.q_base + token : ((int64_t)s.b * a.hq + h) * a.lq + token;
 }
 
-// keys [lo, hi) that queries at tokens [t0, t1] may see (hi <= lo: none)
-__device__ __forceinline__ void key_range(const Args& a, const Seq& s, int64_t t0, int64_t t1, int64_t& lo, int64_t& hi) {
-    lo = 0;
-    hi = s.lk;
-    if (a.causal) hi = clamp64(t1 + s.off + 1, 0, s.lk);
-    if (a.window) lo = clamp64(t0 + s.off - a.window + 1, 0, s.lk);
+// the keys [lo, hi) that some of the queries at tokens [t0, t1] see (hi <= lo: none), and [all_lo, all_hi)
+// that all of them see
+struct Keys {
+    int lo, hi, all_lo, all_hi;
+};
+__device__ __forceinline__ Keys keys_of(const Args& a, const Seq& s, int t0, int t1) {
+    Keys k = {0, s.lk, 0, s.lk};
+    if (a.causal) {
+        k.hi = (int)clamp64((int64_t)t1 + s.off + 1, 0, s.lk);
+        k.all_hi = (int)clamp64((int64_t)t0 + s.off + 1, 0, s.lk);
+    }
+    if (a.window) {
+        k.lo = (int)clamp64((int64_t)t0 + s.off - a.window + 1, 0, s.lk);
+        k.all_lo = (int)clamp64((int64_t)t1 + s.off - a.window + 1, 0, s.lk);
+    }
+    return k;
 }
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 x, bf16x8 y, f32x16 c) {
@@ -183,29 +210,70 @@ struct Tile {
     }
 };
 
-// ROWS rows of a tile on their way from memory through a workgroup's registers. Rows past the last one
-// repeat it and columns past the head's d repeat the first chunk: what lies there is multiplied by zeros,
-// masked or not stored, and comes from values that some row sees.
+// ---------------------------------------------------------------- memory -> LDS
+// Rows of tokens in memory as a buffer that ends with the last token in use: a load past it, like one of the
+// columns past the head's d, gives zeros, so nothing past a sequence is read and no row needs a clamp.
+constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every buffer's end
+struct Rows {
+    const uint8_t* p;    // the next tile's first token
+    int64_t left;        // bytes from there to the end of the last token in use
+    // rows: from token row0 on, `rows` in use in all; ts2: bytes a token
+    __device__ __forceinline__ Rows(const uint8_t* base, int64_t ts2, int row0, int rows, int d)
+        : p(base + row0 * ts2), left(rows > row0 ? (rows - 1 - row0) * ts2 + 2 * d : 0) {}
+    __device__ __forceinline__ void step(int64_t bytes, int64_t last) {  // last: 2 d, what is left past the last token
+        p += bytes;
+        left -= bytes;
+        if (left < last) left = 0;
+    }
+    __device__ __forceinline__ u32x4 buffer() const {
+        const uint64_t u = reinterpret_cast<uint64_t>(p);
+        const uint32_t n = left > 0x7FFFFFF0 ? 0x7FFFFFF0u : (uint32_t)left;
+        return (u32x4){(uint32_t)uniform((int)u), (uint32_t)uniform((int)(u >> 32)) & 0xFFFFu, (uint32_t)uniform((int)n), 0x00020000u};
+    }
+};
+
+// the LDS address of a pointer into LDS
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+    return (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
+}
+// 64 pieces of 16 bytes, a lane's at `off` of the buffer, to LDS dst + 16 lane. In assembly because the compiler would
+// wait for every such load before the next LDS read; the waits are landed()'s, at the loops' barriers.
+__device__ __forceinline__ void load_piece(const u32x4& buf, uint32_t off, uint32_t dst) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(off), "s"(buf), "s"(dst));
+}
+// 64 values of 4 bytes
+__device__ __forceinline__ void load_words(const u32x4& buf, uint32_t off, uint32_t dst) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(off), "s"(buf), "s"(dst));
+}
+// all but the newest N loads have landed in LDS
+template <int N = 0>
+__device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// ROWS rows from memory into a tile, by THREADS threads: a piece's place in LDS is its thread's, so the swizzle
+// is in which chunk of the row a thread loads.
 template <int D, int ROWS, int THREADS>
-struct Stage {
-    static constexpr int N = ROWS * Tile<D>::CH / THREADS;  // 16-byte pieces a thread
+struct Loader {
+    static constexpr int N = ROWS * Tile<D>::CH / THREADS;  // pieces a thread
     static_assert(N * THREADS == ROWS * Tile<D>::CH, "whole pieces");
-    u32x4 x[N];
-    // base: the sequence's token 0 of the head; ts2: bytes a token
-    __device__ __forceinline__ void load(const uint8_t* base, int64_t ts2, int64_t row0, int64_t last, int d, int tid) {
+    uint32_t off[N];
+    __device__ __forceinline__ Loader(int64_t ts2, int d, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int p = tid + THREADS * i, row = p / Tile<D>::CH, ch = p % Tile<D>::CH;
-            const int64_t r = row0 + row < last ? row0 + row : last;
-            x[i] = *reinterpret_cast<const u32x4*>(base + r * ts2 + (8 * ch < d ? 16 * ch : 0));
+            const int p = tid + THREADS * i, row = p / Tile<D>::CH, ch = (p % Tile<D>::CH) ^ Tile<D>::f(row);
+            off[i] = 8 * ch < d ? (uint32_t)(row * ts2) + 16 * ch : kNowhere;
         }
     }
-    __device__ __forceinline__ void store(uint8_t* t, int tid) const {
+    // dst: the tile's LDS address + 1024 * the wave's index
+    __device__ __forceinline__ void load(const Rows& r, uint32_t dst) const {
+        const u32x4 b = r.buffer();
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int p = tid + THREADS * i;
-            *reinterpret_cast<u32x4*>(t + Tile<D>::at(p / Tile<D>::CH, p % Tile<D>::CH)) = x[i];
-        }
+        for (int i = 0; i < N; ++i) load_piece(b, off[i], dst + 16 * THREADS * i);
     }
 };
 
@@ -221,14 +289,30 @@ __device__ __forceinline__ void load_row(const uint8_t* row, bool valid, int d, 
     }
 }
 
-// four consecutive values of a row (d0 a multiple of 4; d a multiple of 8)
-__device__ __forceinline__ void store4(uint8_t* row, bool f32, int d0, float x, float y, float z, float w) {
+// A lane's 16 values of one 32-column block of an output row (columns 8e + 4h + 0..3 of the block, e = 0..3),
+// times f, to the row at column d0: 16 bytes a store. Both lanes of a row call it; on: the row is written.
+__device__ __forceinline__ void store_block(uint8_t* row, bool f32, bool on, int d0, int d, int h, const f32x16& x, float f) {
     if (f32) {
-        float4 v = {x, y, z, w};
-        *reinterpret_cast<float4*>(row + 4 * d0) = v;
-    } else {
-        uint2 v = {pack_bf16(x, y), pack_bf16(z, w)};
-        *reinterpret_cast<uint2*>(row + 2 * d0) = v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = d0 + 8 * e + 4 * h;
+            const float4 v = {x[4 * e] * f, x[4 * e + 1] * f, x[4 * e + 2] * f, x[4 * e + 3] * f};
+            if (on && c < d) *reinterpret_cast<float4*>(row + 4 * c) = v;
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {  // the two lanes exchange: columns 8e .. 8e + 7 in the lower, the next 8 in the upper
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const auto s = __builtin_amdgcn_permlane32_swap(pack_bf16(x[4 * e + 2 * j] * f, x[4 * e + 2 * j + 1] * f),
+                                                            pack_bf16(x[4 * e + 4 + 2 * j] * f, x[4 * e + 5 + 2 * j] * f), false, false);
+            w[j] = s[0];
+            w[2 + j] = s[1];
+        }
+        const int c = d0 + 8 * e + 8 * h;
+        if (on && c < d) *reinterpret_cast<u32x4*>(row + 2 * c) = w;
     }
 }
 

@@ -8,7 +8,8 @@
 namespace r97q {
 namespace attn {
 
-int launch_fwd(const Args& a, hipStream_t st);
+int64_t fwd_workspace(const Args& a);
+int launch_fwd(Args a, void* workspace, hipStream_t st);
 int launch_bwd(const Args& a, hipStream_t st);
 
 namespace {
@@ -36,6 +37,8 @@ int check_shape(const R97qAttnShape* p, int32_t hq, int32_t hk, const char* who)
     return R97Q_OK;
 }
 
+constexpr int64_t kMostStride = 1 << 24;
+
 int check_heads(const R97qHeads* t, int32_t heads, bool f32, bool output, bool packed, int64_t batch, int64_t tokens,
                 const char* who, const char* name) {
     if (!t || (!t->data && batch > 0 && tokens > 0)) {
@@ -56,6 +59,11 @@ int check_heads(const R97qHeads* t, int32_t heads, bool f32, bool output, bool p
         set_error("%s: %s starts and strides on 16 bytes", who, name);
         return R97Q_EUNSUPPORTED;
     }
+    // a tile's rows lie within 31 bits of its first
+    if (tokens > 1 && t->token_stride > kMostStride) {
+        set_error("%s: %s has its tokens more than %lld values apart", who, name, (long long)kMostStride);
+        return R97Q_EUNSUPPORTED;
+    }
     if (t->token_stride < 0 || t->head_stride < 0 || (!packed && t->batch_stride < 0) ||
         (output && ((tokens > 1 && !t->token_stride) || (heads > 1 && !t->head_stride) || (!packed && batch > 1 && !t->batch_stride)))) {
         set_error("%s: %s has a negative stride, or is written through a stride of zero", who, name);
@@ -64,8 +72,8 @@ int check_heads(const R97qHeads* t, int32_t heads, bool f32, bool output, bool p
     return R97Q_OK;
 }
 
-Heads heads_of(const R97qHeads* t) {
-    return {static_cast<uint8_t*>(t->data), t->batch_stride, t->token_stride, t->head_stride, t->dtype == R97Q_F32};
+Heads heads_of(const R97qHeads* t, int64_t tokens) {  // a lone token's stride says nothing
+    return {static_cast<uint8_t*>(t->data), t->batch_stride, tokens > 1 ? t->token_stride : 0, t->head_stride, t->dtype == R97Q_F32};
 }
 
 Args args_of(const R97qAttnShape* p, int32_t hq, int32_t hk) {
@@ -75,26 +83,23 @@ Args args_of(const R97qAttnShape* p, int32_t hq, int32_t hk) {
     a.hk = hk;
     a.g = hq / hk;
     a.d = p->head_dim;
-    a.lq = p->q_len;
-    a.lk = p->kv_len;
+    a.lq = (int32_t)p->q_len;
+    a.lk = (int32_t)p->kv_len;
     a.q_starts = p->q_starts;
     a.kv_starts = p->kv_starts;
     a.kv_lens = p->kv_lens;
     a.q_tokens = p->q_tokens;
     a.kv_tokens = p->kv_tokens;
     a.causal = p->causal != 0;
-    a.window = p->window;
+    a.window = (int32_t)(p->window < 0x7FFFFFFF ? p->window : 0x7FFFFFFF);  // past every length
     a.scale = p->scale;
+    a.slots = p->q_starts ? hq * p->q_tokens : (int64_t)p->batch * hq * p->q_len;
+    a.splits = 1;
     return a;
 }
 
 int64_t q_rows(const R97qAttnShape* p) { return p->q_starts ? p->q_tokens : p->q_len; }
 int64_t kv_rows(const R97qAttnShape* p) { return p->kv_starts ? p->kv_tokens : p->kv_len; }
-
-int64_t stat_bytes(const R97qAttnShape* p, int32_t hq) {
-    const int64_t n = p->q_starts ? (int64_t)hq * p->q_tokens : (int64_t)p->batch * hq * p->q_len;
-    return (4 * n + 255) / 256 * 256;
-}
 
 }  // namespace
 }  // namespace attn
@@ -108,7 +113,8 @@ extern "C" {
 int64_t r97q_attn_fwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads) {
     clear_error();
     if (check_shape(shape, q_heads, kv_heads, "r97q_attn_fwd_workspace_bytes")) return -1;
-    return 0;
+    if (shape->batch == 0 || shape->q_len == 0) return 0;
+    return fwd_workspace(args_of(shape, q_heads, kv_heads));
 }
 
 int r97q_attn_fwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
@@ -126,20 +132,21 @@ int r97q_attn_fwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
     if (int e = check_heads(out, hq, true, true, pq, b, n, who, "out")) return e;
     const int64_t need = r97q_attn_fwd_workspace_bytes(shape, hq, hk);
     if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
+    if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
     if (b == 0 || n == 0 || shape->q_len == 0) return R97Q_OK;
     Args a = args_of(shape, hq, hk);
-    a.q = heads_of(q);
-    a.k = heads_of(k);
-    a.v = heads_of(v);
-    a.o = heads_of(out);
+    a.q = heads_of(q, n);
+    a.k = heads_of(k, m);
+    a.v = heads_of(v, m);
+    a.o = heads_of(out, n);
     a.lse = lse;
-    return launch_fwd(a, (hipStream_t)stream);
+    return launch_fwd(a, workspace, (hipStream_t)stream);
 }
 
 int64_t r97q_attn_bwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads) {
     clear_error();
     if (check_shape(shape, q_heads, kv_heads, "r97q_attn_bwd_workspace_bytes")) return -1;
-    return stat_bytes(shape, q_heads);
+    return 8 * args_of(shape, q_heads, kv_heads).slots;
 }
 
 int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
@@ -164,19 +171,20 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
     if (!lse && n > 0) return refuse(R97Q_EINVAL, who, "null lse");
     if (workspace_bytes < r97q_attn_bwd_workspace_bytes(shape, hq, hk) || (!workspace && n > 0))
         return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
     Args a = args_of(shape, hq, hk);
     if (n == 0) a.lq = 0;
     if (m == 0) a.lk = 0;
-    a.q = heads_of(q);
-    a.k = heads_of(k);
-    a.v = heads_of(v);
-    a.o = heads_of(out);
-    a.d_o = heads_of(d_out);
-    a.dq = heads_of(dq);
-    a.dk = heads_of(dk);
-    a.dv = heads_of(dv);
+    a.q = heads_of(q, n);
+    a.k = heads_of(k, m);
+    a.v = heads_of(v, m);
+    a.o = heads_of(out, n);
+    a.d_o = heads_of(d_out, n);
+    a.dq = heads_of(dq, n);
+    a.dk = heads_of(dk, m);
+    a.dv = heads_of(dv, m);
     a.lse = const_cast<float*>(lse);
-    a.delta = static_cast<float*>(workspace);
+    a.base = static_cast<float2*>(workspace);
     return launch_bwd(a, (hipStream_t)stream);
 }
 

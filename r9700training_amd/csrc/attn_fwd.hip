@@ -2,15 +2,19 @@
 //
 // One pass over the keys with a running maximum and sum (in f32), per row:
 //   m' = max(m, max_j s_j),  l' = l e^(m - m') + sum_j e^(s_j - m'),  O' = O e^(m - m') + sum_j e^(s_j - m') v_j
-// and O / l, m + ln l at the end. The probabilities are rounded to bf16 for the second product (the
-// matrix cores' input type; relative 2^-9 at most, as the output's own rounding), their sum is of the
-// unrounded values in f32.
+// and O / l, m + ln l at the end. m need not be the maximum, only near it: it moves when some row's maximum has
+// passed it by more than a factor of 2^8, so most tiles rescale nothing (f32 has the room, and a bf16
+// probability the same relative precision at any size). The probabilities are rounded to bf16 for the second
+// product (the matrix cores' input type; half a step of 2^-8 relative), their sum is of the unrounded values
+// in f32.
 #include "attn.h"
 #include "status.h"
 
 namespace r97q {
 namespace attn {
 namespace {
+
+constexpr float kLoose = 8.0f;  // how far, in powers of two, a maximum may pass m before m moves
 
 // The running maximum is taken of the raw products, so the scale has to be positive: a negative one flips
 // the queries' signs instead, and with a scale of zero the queries are zeros. In base 2 for the exponentials.
@@ -26,149 +30,456 @@ __device__ __forceinline__ void turn_sign(const Args& a, bf16x8 (&q)[D / 16]) {
     }
 }
 
-// ---------------------------------------------------------------- tiles of 128 rows
-// A workgroup's 4 waves take 32 rows each of one key head's rows and walk the keys together, KT at a
-// time, from LDS.
+// the natural log-sum-exp of a sum l relative to 2^m; nothing summed: minus infinity
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2; }
+
+// 32 rows' running state: a lane's query is column lane % 32, shared with lane ^ 32
+template <int D>
+struct Running {
+    f32x16 o[D / 32];
+    float m, l;
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] = (f32x16){};
+        m = -INFINITY;
+        l = 0.0f;
+    }
+    // m moves where a maximum passed it (top: this tile's, times the scale)
+    __device__ __forceinline__ void rise(float top) {
+        if (__builtin_amdgcn_ballot_w64(top > m + kLoose) == 0) return;
+        const float m1 = fmaxf(m, top);
+        const float turn = __builtin_amdgcn_exp2f(m - (m1 == -INFINITY ? 0.0f : m1));
+        m = m1;
+        l *= turn;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] *= turn;
+    }
+};
+
+// S^T tiles of KT keys against 32 rows
 template <int D, int KT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_fwd_kernel(Args a) {
+__device__ __forceinline__ void scores(const uint8_t* kt, const bf16x8 (&q)[D / 16], int lane, f32x16 (&x)[KT / 32]) {
+#pragma unroll
+    for (int i = 0; i < KT / 32; ++i) x[i] = (f32x16){};
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int i = 0; i < KT / 32; ++i) x[i] = mfma(Tile<D>::rows(kt, 32 * i, c, lane), q[c], x[i]);
+}
+// keys outside [first, last], counted from the tile's first, to minus infinity (one comparison a key: the
+// distance from the first, unsigned, against how many there are)
+template <int KT>
+__device__ __forceinline__ void mask(f32x16 (&x)[KT / 32], int first, int last, int h) {
+    const uint32_t many = last < first ? 0u : (uint32_t)(last - first) + 1u;
+#pragma unroll
+    for (int i = 0; i < KT / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const uint32_t j = (uint32_t)(4 * h - first) + (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3));
+            x[i][e] = j < many ? x[i][e] : -INFINITY;
+        }
+}
+template <int KT>
+__device__ __forceinline__ float tile_max(const f32x16 (&x)[KT / 32]) {
+    float t[KT / 32];
+#pragma unroll
+    for (int i = 0; i < KT / 32; ++i) {
+        t[i] = x[i][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) t[i] = fmaxf(t[i], x[i][e]);
+    }
+#pragma unroll
+    for (int i = 1; i < KT / 32; ++i) t[0] = fmaxf(t[0], t[i]);
+    return pair_max(t[0]);
+}
+// probabilities of a tile's scores, their sum into r.l, and their product with the values into r.o
+template <int D, int KT>
+__device__ __forceinline__ void absorb(const uint8_t* vt, f32x16 (&x)[KT / 32], float sl, int lane, Running<D>& r) {
+    const float base = r.m == -INFINITY ? 0.0f : r.m;
+    bf16x8 p[KT / 16];
+    float sum[KT / 32];
+#pragma unroll
+    for (int i = 0; i < KT / 32; ++i) {
+        sum[i] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            x[i][e] = __builtin_amdgcn_exp2f(x[i][e] * sl - base);
+            sum[i] += x[i][e];
+        }
+        bf16x8 two[2];
+        pack_tile(x[i], two);
+        p[2 * i] = two[0];
+        p[2 * i + 1] = two[1];
+#pragma unroll
+        for (int c = 2 * i; c < 2 * i + 2; ++c)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) r.o[d] = mfma(Tile<D>::cols(vt, 16 * c, d, lane), p[c], r.o[d]);
+    }
+#pragma unroll
+    for (int i = 0; i < KT / 32; ++i) r.l += sum[i];
+}
+
+// a row's place
+struct Row {
+    int tok, head;
+    bool on;
+    __device__ __forceinline__ Row(const Args& a, int hk, int r, int rows) {
+        const int rr = r < rows ? r : rows - 1;
+        tok = rr / a.g;
+        head = hk * a.g + (rr - tok * a.g);
+        on = r < rows;
+    }
+};
+
+template <int D>
+__device__ __forceinline__ void finish(const Args& a, const Seq& s, const Row& row, int h, int split, const Running<D>& r, float l) {
+    const int d = fresh(a.d);
+    h = fresh_lane(h);
+    if (a.splits > 1) {
+        const int64_t at = split * a.slots + stat_at(a, s, row.head, row.tok);
+        uint8_t* out = reinterpret_cast<uint8_t*>(a.part + at * d);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) store_block(out, true, row.on, 32 * i, d, h, r.o[i], 1.0f);
+        if (row.on && h == 0) a.stats[at] = make_float2(r.m, l);
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint8_t* out = q_at(a.o, a, s, row.head) + (a.o.f32 ? 4 : 2) * (row.tok * a.o.ts);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) store_block(out, a.o.f32, row.on, 32 * i, d, h, r.o[i], inv);
+    if (row.on && a.lse && h == 0)
+        a.lse[stat_at(a, s, row.head, row.tok)] = log_sum(r.m, l);
+}
+
+// ---------------------------------------------------------------- tiles of 32 NW rows
+// A workgroup's NW waves take 32 rows each of one key head's rows and walk the keys together, KT at a time, from
+// LDS. The products of the next tile's scores are issued beside this tile's exponentials; one barrier a tile:
+// at the top of step j the keys of tile j + 1 and the values of tile j have landed and both of tile j - 1's
+// slots are free for the loads of tiles j + 2 and j + 1.
+template <int D, int KT, int NW, int PER>
+__global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     using T = Tile<D>;
-    __shared__ __attribute__((aligned(16))) uint8_t kt[2][KT * T::RB];
-    __shared__ __attribute__((aligned(16))) uint8_t vt[2][KT * T::RB];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, h = lane >> 5;
-    const int hk = blockIdx.y;
-    const Seq s = sequence(a, blockIdx.z);
-    const int64_t rows = s.lq * a.g;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * KT * T::RB];
+    constexpr int TB = KT * T::RB;  // keys' two slots, then the values'
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
+    const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, split = blockIdx.y;
+    const int tiles = gridDim.x / nb;
+    const Seq s = sequence(a, bh / a.hk);
+    const int rows = s.lq * a.g;
     const float sl = score_scale(a);
     const uint8_t* kb = kv_at(a.k, a, s, hk);
     const uint8_t* vb = kv_at(a.v, a, s, hk);
-    for (int64_t tile = gridDim.x - 1 - blockIdx.x; tile * 128 < rows; tile += gridDim.x) {
-        const int64_t r0 = tile * 128 + 32 * wave;
-        const int64_t r = r0 + col, rr = r < rows ? r : rows - 1;
-        const int64_t tok = rr / a.g;
-        const int head = hk * a.g + (int)(rr % a.g);
+    const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
+    const Loader<D, KT, 64 * NW> kl(kts, a.d, tid), vl(vts, a.d, tid);
+    const uint32_t at = lds_at(lds), mine = at + 1024 * wave;
+    // the last tiles first: under a causal mask they have the most keys
+    for (int64_t tile = tiles - 1 - (int)(blockIdx.x / nb); tile * 32 * NW < rows; tile += tiles) {
+        const int w0 = (int)tile * 32 * NW, r0 = w0 + 32 * wave;
+        const Row row(a, hk, r0 + col, rows);
         bf16x8 q[D / 16];
-        load_row<D>(q_at(a.q, a, s, head) + 2 * tok * a.q.ts, r < rows, a.d, lane, q);
+        load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
         turn_sign<D>(a, q);
-        int64_t lo, hi, wlo, whi;
-        const int64_t end = tile * 128 + 127 < rows ? tile * 128 + 127 : rows - 1;
-        key_range(a, s, tile * 128 / a.g, end / a.g, lo, hi);
-        lo = lo / KT * KT;
-        // the wave's own rows: what its first and last token see
-        const int64_t t0 = (r0 < rows ? r0 : rows - 1) / a.g, t1 = (r0 + 31 < rows ? r0 + 31 : rows - 1) / a.g;
-        key_range(a, s, t0, t1, wlo, whi);
-        const int64_t all_lo = a.window ? t1 + s.off - a.window + 1 : 0;                     // every row sees from here
-        const int64_t all_hi = a.causal ? clamp64(t0 + s.off + 1, 0, s.lk) : s.lk;            // to here
-        f32x16 o[D / 32];
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[i] = (f32x16){};
-        float m = -INFINITY, l = 0.0f;
+        const int wend = w0 + 32 * NW - 1 < rows ? w0 + 32 * NW - 1 : rows - 1;
+        const Keys all = keys_of(a, s, w0 / a.g, wend / a.g);
+        const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
+        Keys own = keys_of(a, s, (r0 < rows ? r0 : rows - 1) / a.g, rend / a.g);
+        if (r0 >= rows) own.hi = own.lo;
+        int lo = all.lo / KT * KT, hi = all.hi;
+        if (a.splits > 1) {
+            lo = (int)clamp64((int64_t)lo + (int64_t)split * a.chunk, lo, hi);
+            if (split < a.splits - 1 && hi - lo > a.chunk) hi = lo + a.chunk;  // the last range takes what is left
+        }
+        // the keys this lane's row sees, first and last
+        const int first = a.window ? (int)clamp64((int64_t)row.tok + s.off - a.window + 1, 0, s.lk) : 0;
+        const int last = a.causal && row.tok + s.off < s.lk - 1 ? row.tok + s.off : s.lk - 1;
+        Running<D> run;
+        run.clear();
         if (lo < hi) {
-            Stage<D, KT, 256> ks, vs;
-            ks.load(kb, 2 * a.k.ts, lo, s.lk - 1, a.d, tid);
-            vs.load(vb, 2 * a.v.ts, lo, s.lk - 1, a.d, tid);
-            ks.store(kt[0], tid);
-            vs.store(vt[0], tid);
+            Rows kr(kb, kts, lo, hi, a.d), vr(vb, vts, lo, hi, a.d);
+            const int end = own.hi < hi ? own.hi : hi;
+            // tiles this wave looks at: [n0, n1) of n
+            const int n = (hi - lo + KT - 1) / KT, n0 = own.lo > lo ? (own.lo - lo) / KT : 0, n1 = end > lo ? (end - lo + KT - 1) / KT : 0;
+            kl.load(kr, mine);
+            kr.step(KT * kts, 2 * a.d);
+            landed();
             __syncthreads();
-            int buf = 0;
-            for (int64_t j0 = lo; j0 < hi; j0 += KT, buf ^= 1) {
-                const bool more = j0 + KT < hi;
-                if (more) {
-                    ks.load(kb, 2 * a.k.ts, j0 + KT, s.lk - 1, a.d, tid);
-                    vs.load(vb, 2 * a.v.ts, j0 + KT, s.lk - 1, a.d, tid);
-                }
-                if (j0 < whi && j0 + KT > wlo) {
-                    f32x16 x[KT / 32];
-#pragma unroll
-                    for (int i = 0; i < KT / 32; ++i) {
-                        x[i] = (f32x16){};
-#pragma unroll
-                        for (int c = 0; c < D / 16; ++c) x[i] = mfma(T::rows(kt[buf], 32 * i, c, lane), q[c], x[i]);
-                    }
-                    if (j0 < all_lo || j0 + KT > all_hi) {
-                        // positions relative to the tile fit 32 bits once clamped
-                        const int top = (int)clamp64((a.causal ? tok + s.off : s.lk - 1) - j0, -1, KT);
-                        const int cap = (int)clamp64(s.lk - 1 - j0, -1, KT);
-                        const int last = top < cap ? top : cap;
-                        const int first = a.window ? (int)clamp64(tok + s.off - a.window + 1 - j0, 0, KT) : 0;
-#pragma unroll
-                        for (int i = 0; i < KT / 32; ++i)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const int j = 32 * i + 8 * (e >> 2) + 4 * h + (e & 3);
-                                x[i][e] = j <= last && j >= first ? x[i][e] : -INFINITY;
-                            }
-                    }
-                    float top = x[0][0];
-#pragma unroll
-                    for (int i = 0; i < KT / 32; ++i)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) top = fmaxf(top, x[i][e]);
-                    top = pair_max(top) * sl;
-                    const float m1 = fmaxf(m, top);
-                    const float base = m1 == -INFINITY ? 0.0f : m1;
-                    const float turn = __builtin_amdgcn_exp2f(m - base);
-                    m = m1;
-                    float sum = 0.0f;
-                    bf16x8 p[KT / 16];
-#pragma unroll
-                    for (int i = 0; i < KT / 32; ++i) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            x[i][e] = __builtin_amdgcn_exp2f(x[i][e] * sl - base);
-                            sum += x[i][e];
-                        }
-                        bf16x8 two[2];
-                        pack_tile(x[i], two);
-                        p[2 * i] = two[0];
-                        p[2 * i + 1] = two[1];
-                    }
-                    l = l * turn + sum;
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[i][e] *= turn;
-#pragma unroll
-                    for (int c = 0; c < KT / 16; ++c)
-#pragma unroll
-                        for (int i = 0; i < D / 32; ++i) o[i] = mfma(T::cols(vt[buf], 16 * c, i, lane), p[c], o[i]);
-                }
-                if (more) {
-                    ks.store(kt[buf ^ 1], tid);
-                    vs.store(vt[buf ^ 1], tid);
-                }
+            kl.load(kr, mine + TB);
+            kr.step(KT * kts, 2 * a.d);
+            vl.load(vr, mine + 2 * TB);
+            vr.step(KT * vts, 2 * a.d);
+            f32x16 x0[KT / 32], x1[KT / 32];
+            scores<D, KT>(lds, q, lane, x0);
+            auto step = [&](f32x16 (&x)[KT / 32], f32x16 (&next)[KT / 32], int j, int slot) {
+                landed();
                 __syncthreads();
+                kl.load(kr, mine + slot * TB);
+                kr.step(KT * kts, 2 * a.d);
+                vl.load(vr, mine + (3 - slot) * TB);
+                vr.step(KT * vts, 2 * a.d);
+                if (j >= n0 && j < n1) {
+                    const int j0 = lo + j * KT;
+                    if (j0 < own.all_lo || j0 + KT > own.all_hi) mask<KT>(x, first - j0, last - j0, h);
+                    scores<D, KT>(lds + (1 - slot) * TB, q, lane, next);
+                    run.rise(tile_max<KT>(x) * sl);
+                    absorb<D, KT>(lds + (2 + slot) * TB, x, sl, lane, run);
+                } else if (j + 1 == n0) {
+                    scores<D, KT>(lds + (1 - slot) * TB, q, lane, next);
+                }
+            };
+            for (int j = 0; j < n; j += 2) {
+                step(x0, x1, j, 0);
+                if (j + 1 < n) step(x1, x0, j + 1, 1);
+            }
+            landed();
+        }
+        finish<D>(a, s, row, h, split, run, pair_sum(run.l));
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- a few rows against many keys
+// At most 32 rows of a key head (one token's query heads, or a few tokens'): nothing is shared between rows, so
+// every wave takes tiles of 32 keys of its own, with its own K and V tile in LDS and no barrier: the next keys
+// are loaded when the scores are done, the next values when the product is. The NW waves' sums meet in LDS.
+// Bound by memory: 2 * D * 2 bytes a key.
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
+    using T = Tile<D>;
+    constexpr int KT = 32, TB = KT * T::RB;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[NW * 2 * TB];
+    __shared__ float2 ml[NW][32];
+    static_assert(2 * TB >= 32 * D * 4, "a wave's tiles hold its sums");
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
+    const int bh = blockIdx.x, hk = bh % a.hk, split = blockIdx.y;
+    const Seq s = sequence(a, bh / a.hk);
+    const int rows = s.lq * a.g;
+    const float sl = score_scale(a);
+    const uint8_t* kb = kv_at(a.k, a, s, hk);
+    const uint8_t* vb = kv_at(a.v, a, s, hk);
+    const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
+    const Loader<D, KT, 64> kl(kts, a.d, lane), vl(vts, a.d, lane);
+    uint8_t* own = lds + wave * 2 * TB;
+    const uint32_t at = lds_at(own);
+    for (int64_t tile = blockIdx.z; tile * 32 < rows; tile += gridDim.z) {
+        const int r0 = (int)tile * 32;
+        const Row row(a, hk, r0 + col, rows);
+        const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
+        const Keys keys = keys_of(a, s, r0 / a.g, rend / a.g);
+        int lo = keys.lo / KT * KT, hi = keys.hi;
+        if (a.splits > 1) {
+            lo = (int)clamp64((int64_t)lo + (int64_t)split * a.chunk, lo, hi);
+            if (split < a.splits - 1 && hi - lo > a.chunk) hi = lo + a.chunk;  // the last range takes what is left
+            if (lo >= hi) {  // nothing in this range
+                if (wave == 0 && row.on && h == 0) a.stats[split * a.slots + stat_at(a, s, row.head, row.tok)] = make_float2(-INFINITY, 0.0f);
+                continue;
             }
         }
-        l = pair_sum(l);
-        if (r < rows) {
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            uint8_t* out = q_at(a.o, a, s, head) + (a.o.f32 ? 4 : 2) * tok * a.o.ts;
+        Running<D> run;
+        run.clear();
+        const int first = a.window ? (int)clamp64((int64_t)row.tok + s.off - a.window + 1, 0, s.lk) : 0;
+        const int last = a.causal && row.tok + s.off < s.lk - 1 ? row.tok + s.off : s.lk - 1;
+        int j0 = lo + KT * wave;
+        if (j0 < hi) {
+            Rows kr(kb, kts, j0, hi, a.d), vr(vb, vts, j0, hi, a.d);
+            kl.load(kr, at);
+            vl.load(vr, at + TB);
+            bf16x8 q[D / 16];
+            load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
+            turn_sign<D>(a, q);
+            landed<Loader<D, KT, 64>::N>();  // the queries have been waited for: no more than the values are left
+            for (; j0 < hi; j0 += KT * NW) {
+                f32x16 x[1];
+                scores<D, KT>(own, q, lane, x);
+                // the keys are in registers: their tile is free
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                kr.step(NW * KT * kts, 2 * a.d);
+                kl.load(kr, at);
+                if (j0 < keys.all_lo || j0 + KT > keys.all_hi) mask<KT>(x, first - j0, last - j0, h);
+                run.rise(tile_max<KT>(x) * sl);
+                landed<Loader<D, KT, 64>::N>();  // the values; the next keys may be on their way
+                absorb<D, KT>(own + TB, x, sl, lane, run);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                vr.step(NW * KT * vts, 2 * a.d);
+                vl.load(vr, at + TB);
+                landed<Loader<D, KT, 64>::N>();
+            }
+            landed();
+        }
+        // the waves' sums, each in its own tiles: relative to the largest maximum, then added in wave order
+        const float l = pair_sum(run.l);
+        if (h == 0) ml[wave][col] = make_float2(run.m, l);
+        __syncthreads();
+        float top = ml[0][col].x;
+#pragma unroll
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, ml[w][col].x);
+        const float turn = __builtin_amdgcn_exp2f(run.m - (top == -INFINITY ? 0.0f : top));
+        float* sum = reinterpret_cast<float*>(own);
+        if (row.on) {
 #pragma unroll
             for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int d0 = 32 * i + 8 * e + 4 * h;
-                    if (d0 < a.d)
-                        store4(out, a.o.f32, d0, o[i][4 * e] * inv, o[i][4 * e + 1] * inv, o[i][4 * e + 2] * inv, o[i][4 * e + 3] * inv);
+                    const float4 v = {run.o[i][4 * e] * turn, run.o[i][4 * e + 1] * turn, run.o[i][4 * e + 2] * turn, run.o[i][4 * e + 3] * turn};
+                    *reinterpret_cast<float4*>(sum + col * D + 32 * i + 8 * e + 4 * h) = v;
                 }
-            if (a.lse && h == 0) a.lse[stat_at(a, s, head, tok)] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+        }
+        __syncthreads();
+        const int n = rows - r0 < 32 ? rows - r0 : 32;
+        for (int i = tid; i < n * (D / 4); i += 64 * NW) {
+            const int r = i / (D / 4), d0 = 4 * (i % (D / 4));
+            if (d0 >= a.d) continue;
+            float t = ml[0][r].x, total = 0.0f;
+#pragma unroll
+            for (int w = 1; w < NW; ++w) t = fmaxf(t, ml[w][r].x);
+#pragma unroll
+            for (int w = 0; w < NW; ++w) total += ml[w][r].y * __builtin_amdgcn_exp2f(ml[w][r].x - (t == -INFINITY ? 0.0f : t));
+            float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float4 u = *reinterpret_cast<const float4*>(lds + w * 2 * TB + 4 * (r * D + d0));
+                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+            }
+            const Row rr(a, hk, r0 + r, rows);
+            const int64_t st = stat_at(a, s, rr.head, rr.tok);
+            if (a.splits > 1) {
+                const int64_t to = split * a.slots + st;
+                *reinterpret_cast<float4*>(a.part + to * a.d + d0) = v;
+                if (d0 == 0) a.stats[to] = make_float2(t, total);
+                continue;
+            }
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            uint8_t* out = q_at(a.o, a, s, rr.head) + (a.o.f32 ? 4 : 2) * (rr.tok * a.o.ts);
+            if (a.o.f32)
+                *reinterpret_cast<float4*>(out + 4 * d0) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            else
+                *reinterpret_cast<uint2*>(out + 2 * d0) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+            if (d0 == 0 && a.lse) a.lse[st] = log_sum(t, total);
         }
         __syncthreads();
     }
 }
 
+// ---------------------------------------------------------------- the ranges' results joined
+// grid (batch * q heads, tokens): a workgroup a row. Each range's sums are relative to its own m.
+__global__ __launch_bounds__(256) void attn_join_kernel(Args a) {
+    __shared__ float weight[kMostSplits];
+    __shared__ float part[4];
+    __shared__ __attribute__((aligned(16))) float4 acc[256];
+    const int tid = threadIdx.x, head = blockIdx.x % a.hq;
+    const Seq s = sequence(a, blockIdx.x / a.hq);
+    const int per = a.d / 4, lanes = per <= 16 ? 16 : per <= 32 ? 32 : 64, groups = 256 / lanes;  // threads a range's row, ranges at once
+    for (int tok = blockIdx.y; tok < s.lq; tok += gridDim.y) {
+        const int64_t at = stat_at(a, s, head, tok);
+        const float2 st = tid < a.splits ? a.stats[tid * a.slots + at] : make_float2(-INFINITY, 0.0f);
+        float top = st.x;
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if ((tid & 63) == 0) part[tid >> 6] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        const float w = st.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
+        weight[tid] = w;
+        float l = st.y * w;
+        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+        __syncthreads();
+        if ((tid & 63) == 0) part[tid >> 6] = l;
+        __syncthreads();
+        l = (part[0] + part[1]) + (part[2] + part[3]);
+        const int d0 = 4 * (tid % lanes), g = tid / lanes;
+        float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (d0 < a.d) {
+            for (int i = g; i < a.splits; i += groups) {
+                const float f = weight[i];
+                if (f == 0.0f) continue;
+                const float4 u = *reinterpret_cast<const float4*>(a.part + (i * a.slots + at) * a.d + d0);
+                v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
+            }
+        }
+        acc[tid] = v;
+        __syncthreads();
+        if (tid < lanes && d0 < a.d) {
+            for (int i = 1; i < groups; ++i) {
+                const float4 u = acc[tid + i * lanes];
+                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            uint8_t* out = q_at(a.o, a, s, head) + (a.o.f32 ? 4 : 2) * (tok * a.o.ts);
+            if (a.o.f32)
+                *reinterpret_cast<float4*>(out + 4 * d0) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            else
+                *reinterpret_cast<uint2*>(out + 2 * d0) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+            if (tid == 0 && a.lse) a.lse[at] = log_sum(top, l);
+        }
+        __syncthreads();
+    }
+}
+
+// how a shape is cut: rows a workgroup, ranges of the keys
+struct Plan {
+    bool few;
+    int waves, splits, chunk;
+    int64_t tiles;
+};
+Plan plan_of(const Args& a) {
+    Plan p = {};
+    const int64_t rows = (int64_t)a.lq * a.g, heads = (int64_t)a.batch * a.hk;
+    p.few = rows <= 32;
+    p.waves = 4;
+    const int tile = p.few ? 32 : 32 * p.waves;
+    p.tiles = (rows + tile - 1) / tile;
+    p.splits = 1;
+    // the keys a tile's rows may see
+    int64_t most = a.lk;
+    if (a.window && (int64_t)a.window + tile / a.g + 1 < most) most = (int64_t)a.window + tile / a.g + 1;
+    const int64_t unit = p.few ? 128 : 256, want = a.d > 128 ? 256 : 512, have = p.tiles * heads;
+    if (have < want && most > unit) {
+        int64_t n = (want + have - 1) / have;
+        if (n > (most + unit - 1) / unit) n = (most + unit - 1) / unit;
+        if (n > kMostSplits) n = kMostSplits;
+        int64_t chunk = ((most + n - 1) / n + unit - 1) / unit * unit;
+        p.splits = (int)((most + chunk - 1) / chunk);
+        p.chunk = (int)chunk;
+    }
+    return p;
+}
+
+template <int D, int KT, int NW, int PER>
+int run_tiles(const Args& a, const Plan& p, hipStream_t st) {
+    const int64_t nb = (int64_t)a.batch * a.hk, most = 0x7FFFFFFF / nb;
+    const int64_t tiles = p.tiles < most ? p.tiles : most;
+    hipLaunchKernelGGL((attn_fwd_kernel<D, KT, NW, PER>), dim3((unsigned)(tiles * nb), p.splits), dim3(64 * NW), 0, st, a);
+    return launch_status("attn_fwd_kernel");
+}
+template <int D, int NW>
+int run_few(const Args& a, const Plan& p, hipStream_t st) {
+    hipLaunchKernelGGL((attn_few_kernel<D, NW>), dim3((unsigned)(a.batch * a.hk), p.splits, (unsigned)p.tiles), dim3(64 * NW), 0, st, a);
+    return launch_status("attn_few_kernel");
+}
+
 }  // namespace
 
-int launch_fwd(const Args& a, hipStream_t st) {
-    const int64_t tiles = (a.lq * a.g + 127) / 128;
-    const dim3 grid((unsigned)(tiles < 65535 ? tiles : 65535), a.hk, a.batch);
-    if (a.d <= 64)
-        hipLaunchKernelGGL((attn_fwd_kernel<64, 64>), grid, dim3(256), 0, st, a);
-    else if (a.d <= 128)
-        hipLaunchKernelGGL((attn_fwd_kernel<128, 64>), grid, dim3(256), 0, st, a);
+int64_t fwd_workspace(const Args& a) {
+    const Plan p = plan_of(a);
+    return p.splits > 1 ? p.splits * a.slots * (a.d + 2) * 4 : 0;
+}
+
+int launch_fwd(Args a, void* workspace, hipStream_t st) {
+    const Plan p = plan_of(a);
+    a.splits = p.splits;
+    a.chunk = p.chunk;
+    a.part = static_cast<float*>(workspace);
+    a.stats = reinterpret_cast<float2*>(a.part + (p.splits > 1 ? p.splits * a.slots * a.d : 0));
+    int e;
+    if (p.few)
+        e = a.d <= 64 ? run_few<64, 4>(a, p, st) : a.d <= 128 ? run_few<128, 4>(a, p, st) : run_few<256, 4>(a, p, st);
     else
-        hipLaunchKernelGGL((attn_fwd_kernel<256, 32>), grid, dim3(256), 0, st, a);
-    return launch_status("attn_fwd_kernel");
+        e = a.d <= 64    ? run_tiles<64, 64, 4, 2>(a, p, st)
+            : a.d <= 128 ? run_tiles<128, 32, 4, 2>(a, p, st)
+                         : run_tiles<256, 32, 4, 1>(a, p, st);
+    if (e || p.splits == 1) return e;
+    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)(a.batch * a.hq), (unsigned)(a.lq < 65535 ? a.lq : 65535)), dim3(256), 0, st, a);
+    return launch_status("attn_join_kernel");
 }
 
 }  // namespace attn
