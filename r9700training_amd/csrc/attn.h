@@ -18,6 +18,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <utility>
 
 #include "../../include/r97q.h"
 #include "iqr_device.h"
@@ -30,6 +31,7 @@ using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 using s16x8 = __attribute__((ext_vector_type(8))) short;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -48,7 +50,8 @@ struct Args {
     Heads q, k, v, o;    // o: the forward's output, written there and read in the backward
     Heads d_o, dq, dk, dv;
     float* lse;          // [b][h][Lq], packed: [h][q_tokens]
-    float2* base;        // backward: (log-sum-exp in base 2, sum over d of dO * O) a row, laid out as lse
+    float* base;         // backward: the log-sum-exp in base 2 (0 for a row that sees nothing), laid out as lse
+    float* delta;        // and the sum over d of dO * O
     int32_t batch, hq, hk, g, d;
     int32_t lq, lk;      // tokens of a sequence (packed: of the longest)
     const int32_t* q_starts;
@@ -209,6 +212,51 @@ struct Tile {
         return __builtin_bit_cast(bf16x8, v);
     }
 };
+
+// The same operands by LDS address, for the loops that place every instruction themselves. Tiles start on 1024 bytes,
+// so a chunk's place differs from the first chunk's by an exclusive or of the address: one register a lane and
+// operand kind, and one or two vector instructions a read.
+template <int D>
+struct Frags {
+    static constexpr int RB = 2 * D;
+    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+    // offsets in a tile: rows(), and cols()
+    static __device__ __forceinline__ uint32_t row0(int lane) { return Tile<D>::at(lane & 31, lane >> 5); }
+    static __device__ __forceinline__ uint32_t col0(int lane) {
+        const int l = lane & 15;
+        return Tile<D>::at(4 * (lane >> 5) + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) + 8 * (l & 1);
+    }
+    // rows [r0, r0 + 32), elements 16 c + 8 h .. + 8
+    template <int R0, int C>
+    static __device__ __forceinline__ bf16x8 rows(uint32_t at0) {
+        constexpr int per = D == 64 ? 4 : 8;
+        return as_bf16x8(*(lds_u32x4*)(uintptr_t)((at0 ^ (32 * (C % per))) + (C / per) * 256 + R0 * RB));
+    }
+    // rows R0 + 4h .. and R0 + 8 + 4h .., columns 32 DB + lane % 32
+    template <int R0, int DB>
+    static __device__ __forceinline__ bf16x8 cols(uint32_t at0) {
+        constexpr int per = D == 64 ? 2 : 4;
+        const uint32_t lo = at0 ^ (64 * (DB % per)), hi = at0 ^ (64 * (DB % per) + 32);
+        constexpr int off = (DB / per) * 256 + R0 * RB;
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(lo + off));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(hi + off + 8 * RB));
+        const s16x8 v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        return __builtin_bit_cast(bf16x8, v);
+    }
+};
+// f(0), f(1), .. f(N - 1) with constant indices, unrolled
+template <class F, int... I>
+__device__ __forceinline__ void steps_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void steps(F&& f) {
+    steps_of(f, std::make_integer_sequence<int, N>{});
+}
+// instructions stay on their side
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
+// a 32 x 32 tile's values e and e + 1 (e even) as a word of its B operands
+__device__ __forceinline__ void pack_two(const f32x16& x, int e, u32x4 (&out)[2]) { out[e >> 3][(e & 7) >> 1] = pack_bf16(x[e], x[e + 1]); }
 
 // ---------------------------------------------------------------- memory -> LDS
 // Rows of tokens in memory as a buffer that ends with the last token in use: a load past it, like one of the

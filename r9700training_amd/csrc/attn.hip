@@ -184,7 +184,8 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
     a.dk = heads_of(dk, m);
     a.dv = heads_of(dv, m);
     a.lse = const_cast<float*>(lse);
-    a.base = static_cast<float2*>(workspace);
+    a.base = static_cast<float*>(workspace);
+    a.delta = a.base + a.slots;
     return launch_bwd(a, (hipStream_t)stream);
 }
 

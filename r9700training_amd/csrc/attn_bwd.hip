@@ -18,21 +18,32 @@ namespace attn {
 namespace {
 
 // ---------------------------------------------------------------- dQ (and D): 32 NW rows a workgroup
-template <int D, int KT, int NW, int PER>
+// The waves walk the keys together, 32 at a time. Step j of a wave: dO V_j^T beside the exponentials of the scores j,
+// the scores j + 1 beside dS_j, then dQ += dS_j K_j; at its top the values j and keys j + 1 have landed, and the
+// slots of the values j - 1 and the keys j - 1 are free for the next loads. Every product's LDS operand is read
+// kAhead products before it.
+constexpr int kAhead = 4;
+
+// the scores' factor in base 2. With a scale of zero a factor that leaves nothing of a finite score; so a masked score
+// is an infinity of the other sign, and its exponential zero.
+__device__ __forceinline__ float score_scale(const Args& a) { return a.scale == 0.0f ? 0x1p-126f : a.scale * kLog2e; }
+
+template <int D, int NW, int PER>
 __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
     using T = Tile<D>;
-    constexpr int TB = KT * T::RB;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TB];  // keys' two slots, then the values'
+    using F = Frags<D>;
+    constexpr int KT = 32, TB = KT * T::RB, n = D / 16;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[5 * TB];  // keys' three slots, then the values' two
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
     const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, tiles = gridDim.x / nb;
     const Seq s = sequence(a, bh / a.hk);
     const int rows = s.lq * a.g;
-    const float sl = a.scale * kLog2e;
+    const float sl = score_scale(a), out_of_sight = sl > 0.0f ? -INFINITY : INFINITY;
     const uint8_t* kb = kv_at(a.k, a, s, hk);
     const uint8_t* vb = kv_at(a.v, a, s, hk);
     const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
     const Loader<D, KT, 64 * NW> kl(kts, a.d, tid), vl(vts, a.d, tid);
-    const uint32_t mine = lds_at(lds) + 1024 * wave;
+    const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + F::col0(lane);
     for (int64_t tile = tiles - 1 - (int)(blockIdx.x / nb); tile * 32 * NW < rows; tile += tiles) {
         const int w0 = (int)tile * 32 * NW, r0 = w0 + 32 * wave, r = r0 + col;
         const int rr = r < rows ? r : rows - 1, tok = rr / a.g, head = hk * a.g + (rr - tok * a.g);
@@ -40,20 +51,20 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
         const Keys all = keys_of(a, s, w0 / a.g, wend / a.g);
         const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
         const Keys own = keys_of(a, s, (r0 < rows ? r0 : rows - 1) / a.g, rend / a.g);
-        const int lo = all.lo / KT * KT, hi = all.hi;
+        const int lo = all.lo / KT * KT, hi = all.hi, last2 = 2 * a.d;
         Rows kr(kb, kts, lo, hi, a.d), vr(vb, vts, lo, hi, a.d);
         if (lo < hi) {
             kl.load(kr, mine);
-            vl.load(vr, mine + 2 * TB);
+            kr.step(KT * kts, last2);
         }
         int d = fresh(a.d);
-        bf16x8 q[D / 16], go[D / 16];
+        bf16x8 q[n], go[n];
         load_row<D>(q_at(a.q, a, s, head) + 2 * (tok * a.q.ts), r < rows, d, lane, q);
         load_row<D>(q_at(a.d_o, a, s, head) + 2 * (tok * a.d_o.ts), r < rows, d, lane, go);
         const uint8_t* op = q_at(a.o, a, s, head) + (a.o.f32 ? 4 : 2) * (tok * a.o.ts);
         float delta = 0.0f;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
+        for (int c = 0; c < n; ++c) {
             const int e = 16 * c + 8 * h;
             if (e < d) {
                 if (a.o.f32) {
@@ -68,60 +79,99 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
             }
         }
         delta = pair_sum(delta);
-        const int64_t at = stat_at(a, s, head, tok);
-        const float lse = a.lse[at], base = lse == -INFINITY ? 0.0f : lse * kLog2e;
-        if (r < rows && h == 0) a.base[at] = make_float2(base, delta);
+        const int64_t st = stat_at(a, s, head, tok);
+        const float lse = a.lse[st], base = lse == -INFINITY ? 0.0f : lse * kLog2e;
+        if (r < rows && h == 0) {
+            a.base[st] = base;
+            a.delta[st] = delta;
+        }
         const int first = a.window ? (int)clamp64((int64_t)tok + s.off - a.window + 1, 0, s.lk) : 0;
         const int last = a.causal && tok + s.off < s.lk - 1 ? tok + s.off : s.lk - 1;
+        const uint32_t many = last < first ? 0u : (uint32_t)(last - first) + 1u;
         f32x16 dq[D / 32];
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) dq[i] = (f32x16){};
-        int slot = 0;
-        for (int j0 = lo; j0 < hi; j0 += KT, slot ^= 1) {
+        if (lo < hi) {
+            const int nt = (hi - lo + KT - 1) / KT;
             landed();
             __syncthreads();
-            if (j0 + KT < hi) {
-                kr.step(KT * kts, 2 * a.d);
-                vr.step(KT * vts, 2 * a.d);
-                kl.load(kr, mine + (slot ^ 1) * TB);
-                vl.load(vr, mine + (2 + (slot ^ 1)) * TB);
-            }
-            if (j0 >= own.hi || j0 + KT <= own.lo || r0 >= rows) continue;
-            const uint8_t *kt = lds + slot * TB, *vt = lds + (2 + slot) * TB;
-            f32x16 x[KT / 32], y[KT / 32];
+            kl.load(kr, mine + TB);
+            kr.step(KT * kts, last2);
+            vl.load(vr, mine + 3 * TB);
+            vr.step(KT * vts, last2);
+            f32x16 x0 = {}, x1 = {};
+            auto product = [&](f32x16& x, uint32_t from) {
+                x = (f32x16){};
+                bf16x8 f[kAhead];
+                steps<kAhead>([&](auto i) { f[i] = F::template rows<0, i>(from); });
+                steps<n>([&](auto i) {
+                    const bf16x8 now = f[i % kAhead];
+                    if constexpr (i + kAhead < n) f[i % kAhead] = F::template rows<0, i + kAhead>(from);
+                    x = mfma(now, q[i], x);
+                });
+            };
+            product(x0, rat);
+            uint32_t k_now = 0, k_next = TB, k_free = 2 * TB, v_now = 3 * TB, v_free = 4 * TB;
+            auto step = [&](f32x16& x, f32x16& next, int j) {
+                landed();
+                __syncthreads();
+                const int j0 = lo + j * KT;
+                if (j0 < own.all_lo || j0 + KT > own.all_hi) {
+                    const uint32_t from = (uint32_t)(j0 + 4 * h - first);
 #pragma unroll
-            for (int i = 0; i < KT / 32; ++i) x[i] = y[i] = (f32x16){};
+                    for (int e = 0; e < 16; ++e) x[e] = from + (uint32_t)(8 * (e >> 2) + (e & 3)) < many ? x[e] : out_of_sight;
+                }
+                f32x16 y = {};
+                next = (f32x16){};
+                u32x4 ds[2];
+                bf16x8 f[kAhead];
+                const uint32_t vat = rat + v_now, kat = rat + k_next, dat = cat + k_now;
+                // operand of product i: V rows, next K rows, K columns
+                auto frag = [&](auto i) {
+                    if constexpr (i < n) return F::template rows<0, i>(vat);
+                    else if constexpr (i < 2 * n) return F::template rows<0, i - n>(kat);
+                    else return F::template cols<16 * ((i - 2 * n) / (D / 32)), (i - 2 * n) % (D / 32)>(dat);
+                };
+                steps<kAhead>([&](auto i) { f[i] = frag(i); });
+                kl.load(kr, mine + k_free);
+                vl.load(vr, mine + v_free);
+                steps<3 * n>([&](auto i) {
+                    pin();
+                    const bf16x8 now = f[i % kAhead];
+                    if constexpr (i + kAhead < 3 * n) f[i % kAhead] = frag(std::integral_constant<int, i + kAhead>{});
+                    if constexpr (i < n) {
+                        y = mfma(now, go[i], y);
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c)
+                        for (int e = 16 * i / n; e < 16 * (i + 1) / n; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] * sl - base);
+                    } else if constexpr (i < 2 * n) {
+                        next = mfma(now, q[i - n], next);
+                        // two products later the last one of y is through
+                        constexpr int c = i - n - 2, m = n - 2;
+                        if constexpr (c >= 0) {
 #pragma unroll
-                for (int i = 0; i < KT / 32; ++i) x[i] = mfma(T::rows(kt, 32 * i, c, lane), q[c], x[i]);
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-                for (int i = 0; i < KT / 32; ++i) y[i] = mfma(T::rows(vt, 32 * i, c, lane), go[c], y[i]);
-#pragma unroll
-            for (int i = 0; i < KT / 32; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[i][e] = __builtin_amdgcn_exp2f(x[i][e] * sl - base) * (y[i][e] - delta);
-            if (j0 < own.all_lo || j0 + KT > own.all_hi) {
-                const uint32_t many = last < first ? 0u : (uint32_t)(last - first) + 1u, from = (uint32_t)(j0 + 4 * h - first);
-#pragma unroll
-                for (int i = 0; i < KT / 32; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const uint32_t j = from + (uint32_t)(32 * i + 8 * (e >> 2) + (e & 3));
-                        x[i][e] = j < many ? x[i][e] : 0.0f;
+                            for (int e = 2 * (8 * c / m); e < 2 * (8 * (c + 1) / m); e += 2) {
+                                x[e] *= y[e] - delta;
+                                x[e + 1] *= y[e + 1] - delta;
+                                pack_two(x, e, ds);
+                            }
+                        }
+                    } else {
+                        constexpr int c = (i - 2 * n) / (D / 32), m = (i - 2 * n) % (D / 32);
+                        dq[m] = mfma(now, as_bf16x8(ds[c]), dq[m]);
                     }
+                });
+                pin();
+                kr.step(KT * kts, last2);
+                vr.step(KT * vts, last2);
+                const uint32_t k = k_now, v = v_now;
+                k_now = k_next, k_next = k_free, k_free = k;
+                v_now = v_free, v_free = v;
+            };
+            for (int j = 0; j < nt; j += 2) {
+                step(x0, x1, j);
+                if (j + 1 < nt) step(x1, x0, j + 1);
             }
-#pragma unroll
-            for (int i = 0; i < KT / 32; ++i) {
-                bf16x8 ds[2];
-                pack_tile(x[i], ds);
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int n = 0; n < D / 32; ++n) dq[n] = mfma(T::cols(kt, 32 * i + 16 * c, n, lane), ds[c], dq[n]);
-            }
+            landed();
         }
         d = fresh(a.d);
         const int hs = fresh_lane(h);
@@ -139,23 +189,24 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
 template <int D, int RT, int NW, bool KEPT>
 __global__ __launch_bounds__(64 * NW, 1) void attn_dkdv_kernel(Args a) {
     using T = Tile<D>;
-    constexpr int TB = RT * T::RB;
-    constexpr int KB = KEPT ? 0 : 32 * NW * T::RB;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TB + KB];         // queries' two slots, then dO's, then the keys
-    __shared__ __attribute__((aligned(16))) float2 stat[2][RT];               // (log-sum-exp in base 2, D) a row
+    using F = Frags<D>;
+    constexpr int TB = RT * T::RB, n = D / 16, KB = KEPT ? 0 : 32 * NW * T::RB;
+    // queries' two slots, then dO's, then the keys
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB + KB];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][64];  // log-sum-exp in base 2, and D, of a tile's rows
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
     const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, tiles = gridDim.x / nb;
     const Seq s = sequence(a, bh / a.hk);
     const int cover = a.kv_starts ? s.lk : a.lk;  // the dense form's keys past a sequence's length get zeros
-    const float sl = a.scale * kLog2e;
+    const float sl = score_scale(a), out_of_sight = sl > 0.0f ? -INFINITY : INFINITY;
     const int64_t qts = 2 * a.q.ts, ots = 2 * a.d_o.ts;
     const Loader<D, RT, 64 * NW> ql(qts, a.d, tid), ol(ots, a.d, tid);
-    const uint32_t mine = lds_at(lds) + 1024 * wave, smine = lds_at(stat) + 256 * wave;
+    const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + F::col0(lane);
+    const uint32_t hat = rat + 4 * TB + 32 * wave * T::RB;  // the wave's keys, where they are not kept
     for (int64_t tile = (int)(blockIdx.x / nb); tile * 32 * NW < cover; tile += tiles) {
         const int w0 = (int)tile * 32 * NW, k0 = w0 + 32 * wave, key = k0 + col;
         bf16x8 k[KEPT ? D / 16 : 1], v[D / 16];
         const int kk = key < s.lk ? key : 0;
-        uint8_t* held = lds + 4 * TB;
         if constexpr (KEPT) {
             load_row<D>(kv_at(a.k, a, s, hk) + 2 * (kk * a.k.ts), key < s.lk, fresh(a.d), lane, k);
         } else {
@@ -163,7 +214,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_dkdv_kernel(Args a) {
             Rows kr(kv_at(a.k, a, s, hk), 2 * a.k.ts, w0, s.lk, a.d);
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
-                kl.load(kr, lds_at(held) + i * 32 * T::RB + 1024 * wave);
+                kl.load(kr, mine + 4 * TB + i * 32 * T::RB);
                 kr.step(64 * a.k.ts, 2 * a.d);
             }
         }
@@ -177,80 +228,122 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_dkdv_kernel(Args a) {
         f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) dk[i] = dv[i] = (f32x16){};
-        auto load = [&](int hd, int t, int slot) {
-            const Rows qr(q_at(a.q, a, s, hk * a.g + hd), qts, t, t1, a.d), orr(q_at(a.d_o, a, s, hk * a.g + hd), ots, t, t1, a.d);
-            ql.load(qr, mine + slot * TB);
-            ol.load(orr, mine + (2 + slot) * TB);
-            if (64 * wave < 2 * RT) {
-                const Rows sr(reinterpret_cast<const uint8_t*>(a.base + stat_at(a, s, hk * a.g + hd, 0)), 8, t, t1, 4);
-                load_words(sr.buffer(), 4 * tid, smine + slot * (8 * RT));
-            }
-        };
         if (t0 < t1) {
-            load(0, t0, 0);
-            int hd = 0, t = t0, slot = 0;
-            while (hd < a.g) {
-                int hn = hd, tn = t + RT;  // the next tile
-                if (tn >= t1) tn = t0, ++hn;
+            // where the next tile of tokens lies: a head's, from t0, then the next head's
+            const int64_t qhs = 2 * a.q.hs, ohs = 2 * a.d_o.hs;
+            const uint8_t *qb = q_at(a.q, a, s, hk * a.g), *ob = q_at(a.d_o, a, s, hk * a.g);
+            const uint8_t* sb = reinterpret_cast<const uint8_t*>((wave & 1 ? a.delta : a.base) + stat_at(a, s, hk * a.g, 0));
+            const int64_t shs = 4 * (a.q_starts ? a.q_tokens : a.lq);
+            Rows qr(qb, qts, t0, t1, a.d), orr(ob, ots, t0, t1, a.d), sr(sb, 4, t0, t1, 2);
+            auto load_stat = [&](int slot) {  // wave 0 the one, wave 1 the other
+                if (wave < 2) load_words(sr.buffer(), 4 * lane, lds_at(stat) + 512 * slot + 256 * wave);
+            };
+            ql.load(qr, mine);
+            ol.load(orr, mine + 2 * TB);
+            load_stat(0);
+            const int per = (t1 - t0 + RT - 1) / RT, count = per * a.g;
+            int t = t0, left = per;
+            for (int step = 0, slot = 0; step < count; ++step, slot ^= 1) {
+                if (--left == 0) {
+                    qb += qhs, ob += ohs, sb += shs;
+                    left = per;
+                    qr = Rows(qb, qts, t0, t1, a.d);
+                    orr = Rows(ob, ots, t0, t1, a.d);
+                    sr = Rows(sb, 4, t0, t1, 2);
+                    if (step + 1 == count) qr.left = orr.left = sr.left = 0;  // nothing follows: zeros
+                } else {
+                    qr.step(RT * qts, 2 * a.d);
+                    orr.step(RT * ots, 2 * a.d);
+                    sr.step(4 * RT, 4);
+                }
                 landed();
                 __syncthreads();
-                if (hn < a.g) load(hn, tn, slot ^ 1);
+                load_stat(slot ^ 1);
                 const int tl = t + RT - 1 < t1 ? t + RT - 1 : t1 - 1;
-                // none of the wave's keys is seen: tokens before them, or past their window
-                const bool none = k0 >= s.lk || (a.causal && tl + s.off < k0) ||
-                                  (a.window && (int64_t)t + s.off - a.window >= k0 + 31);
-                if (!none) {
-                    const bool whole = t + RT <= t1 && (!a.causal || ((int64_t)t + s.off >= k0 + 31 && (!a.window || (int64_t)tl + s.off - a.window < k0)));
-                    const uint8_t *qt = lds + slot * TB, *ot = lds + (2 + slot) * TB;
-#pragma unroll
-                    for (int i = 0; i < RT / 32; ++i) {
-                        f32x16 x = {}, y = {};
-#pragma unroll
-                        for (int c = 0; c < D / 16; ++c)
-                            x = mfma(T::rows(qt, 32 * i, c, lane), KEPT ? k[KEPT ? c : 0] : T::rows(held, 32 * wave, c, lane), x);
-#pragma unroll
-                        for (int c = 0; c < D / 16; ++c) y = mfma(T::rows(ot, 32 * i, c, lane), v[c], y);
-                        float dl[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            const float4 w = *reinterpret_cast<const float4*>(&stat[slot][32 * i + 8 * (e >> 2) + 4 * h + (e & 3)]);
-                            x[e] = __builtin_amdgcn_exp2f(x[e] * sl - w.x);
-                            x[e + 1] = __builtin_amdgcn_exp2f(x[e + 1] * sl - w.z);
-                            dl[e] = w.y;
-                            dl[e + 1] = w.w;
-                        }
+                // every row of the tile sees every key of the wave
+                const bool whole = t + RT <= t1 && (!a.causal || ((int64_t)t + s.off >= k0 + 31 &&
+                                                                  (!a.window || (int64_t)tl + s.off - a.window < k0)));
+                constexpr int total = 4 * n * (RT / 32);
+                const uint32_t qat = rat + slot * TB, qct = cat + slot * TB, sat = lds_at(stat) + 512 * slot + 16 * h;
+                typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+                f32x16 x = {}, y = {};
+                u32x4 p[2], ds[2];
+                f32x4 ls[4], dl[4];
+                bf16x8 f[kAhead], kf[kAhead];
+                // operand of product i: of 32 rows, Q and dO as they lie, then the columns of dO and Q
+                auto frag = [&](auto i) {
+                    constexpr int sub = i / (4 * n), ph = i % (4 * n) / n, c = i % n;
+                    if constexpr (ph == 0) return F::template rows<32 * sub, c>(qat);
+                    else if constexpr (ph == 1) return F::template rows<32 * sub + 2 * RT, c>(qat);
+                    else return F::template cols<32 * sub + 16 * (c / (D / 32)) + (ph == 2 ? 2 * RT : 0), c % (D / 32)>(qct);
+                };
+                steps<kAhead>([&](auto i) {
+                    f[i] = frag(i);
+                    if constexpr (!KEPT) kf[i] = F::template rows<0, i>(hat);
+                });
+                steps<total>([&](auto i) {
+                    constexpr int sub = i / (4 * n), ph = i % (4 * n) / n, c = i % n;
+                    if constexpr (ph == 1 && c == 0) {
                         if (!whole) {  // the rows, from the tile's first, that see the lane's key
                             const int top = a.causal ? (int)clamp64((int64_t)key - s.off - t, 0, RT) : 0;
                             const int cap = t1 - t < RT ? t1 - t : RT;
                             const int end = a.window ? (int)clamp64((int64_t)key - s.off - t + a.window, 0, cap) : cap;
-                            const uint32_t many = end < top ? 0u : (uint32_t)(end - top), from = (uint32_t)(32 * i + 4 * h - top);
+                            const uint32_t many = end < top ? 0u : (uint32_t)(end - top), from = (uint32_t)(32 * sub + 4 * h - top);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const uint32_t row = from + (uint32_t)(8 * (e >> 2) + (e & 3));
-                                x[e] = row < many ? x[e] : 0.0f;
+                            for (int e = 0; e < 16; ++e) x[e] = from + (uint32_t)(8 * (e >> 2) + (e & 3)) < many ? x[e] : out_of_sight;
+                        }
+                    }
+                    pin();
+                    const bf16x8 now = f[i % kAhead];
+                    if constexpr (i + kAhead < total) f[i % kAhead] = frag(std::integral_constant<int, i + kAhead>{});
+                    if constexpr (i == 1) ql.load(qr, mine + (slot ^ 1) * TB);
+                    if constexpr (i == 2) ol.load(orr, mine + (2 + (slot ^ 1)) * TB);
+                    // the vector work of a product's results starts two products after its last
+                    constexpr int w = c - 2, m = n - 2;
+                    if constexpr (ph == 0) {
+                        bf16x8 kc;
+                        if constexpr (KEPT) {
+                            kc = k[c];
+                        } else {
+                            kc = kf[c % kAhead];
+                            if constexpr (c + kAhead < n) kf[c % kAhead] = F::template rows<0, c + kAhead>(hat);
+                        }
+                        if constexpr (c == 0) x = (f32x16){};
+                        x = mfma(now, kc, x);
+                        if constexpr (c >= n - 4) ls[c - (n - 4)] = *(lds_f32x4*)(uintptr_t)(sat + 128 * sub + 32 * (c - (n - 4)));
+                    } else if constexpr (ph == 1) {
+                        if constexpr (c == 0) y = (f32x16){};
+                        y = mfma(now, v[c], y);
+                        if constexpr (w >= 0) {
+#pragma unroll
+                            for (int e = 2 * (8 * w / m); e < 2 * (8 * (w + 1) / m); e += 2) {
+                                x[e] = __builtin_amdgcn_exp2f(x[e] * sl - ls[e >> 2][e & 3]);
+                                x[e + 1] = __builtin_amdgcn_exp2f(x[e + 1] * sl - ls[e >> 2][(e & 3) + 1]);
+                                pack_two(x, e, p);
                             }
                         }
-                        bf16x8 p[2], ds[2];
-                        pack_tile(x, p);
+                        if constexpr (c >= n - 4) dl[c - (n - 4)] = *(lds_f32x4*)(uintptr_t)(sat + 256 + 128 * sub + 32 * (c - (n - 4)));
+                    } else if constexpr (ph == 2) {
+                        dv[c % (D / 32)] = mfma(now, as_bf16x8(p[c / (D / 32)]), dv[c % (D / 32)]);
+                        if constexpr (w >= 0) {
 #pragma unroll
-                        for (int c = 0; c < 2; ++c)
-#pragma unroll
-                            for (int d = 0; d < D / 32; ++d) dv[d] = mfma(T::cols(ot, 32 * i + 16 * c, d, lane), p[c], dv[d]);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) y[e] = x[e] * (y[e] - dl[e]);
-                        pack_tile(y, ds);
-#pragma unroll
-                        for (int c = 0; c < 2; ++c)
-#pragma unroll
-                            for (int d = 0; d < D / 32; ++d) dk[d] = mfma(T::cols(qt, 32 * i + 16 * c, d, lane), ds[c], dk[d]);
+                            for (int e = 2 * (8 * w / m); e < 2 * (8 * (w + 1) / m); e += 2) {
+                                y[e] = x[e] * (y[e] - dl[e >> 2][e & 3]);
+                                y[e + 1] = x[e + 1] * (y[e + 1] - dl[e >> 2][(e & 3) + 1]);
+                                pack_two(y, e, ds);
+                            }
+                        }
+                    } else {
+                        dk[c % (D / 32)] = mfma(now, as_bf16x8(ds[c / (D / 32)]), dk[c % (D / 32)]);
+                        if constexpr (!KEPT && sub + 1 < RT / 32 && c >= n - kAhead)
+                            kf[c - (n - kAhead)] = F::template rows<0, c - (n - kAhead)>(hat);
                     }
-                }
-                hd = hn;
-                t = tn;
-                slot ^= 1;
+                });
+                pin();
+                t = left == per ? t0 : t + RT;
             }
         }
-        if constexpr (!KEPT) landed();
+        landed();
         const bool seen = key < s.lk;
         const int dd = fresh(a.d), hs = fresh_lane(h);
         uint8_t* ok = kv_at(a.dk, a, s, hk) + (a.dk.f32 ? 4 : 2) * (key * a.dk.ts);
@@ -265,14 +358,14 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_dkdv_kernel(Args a) {
     }
 }
 
-template <int D, int KT, int PER, int RT, bool KEPT>
+template <int D, int PER, int RT, bool KEPT>
 int launch(const Args& a, hipStream_t st) {
     const int64_t nb = (int64_t)a.batch * a.hk, most = 0x7FFFFFFF / nb;
     int64_t tiles = ((int64_t)a.lq * a.g + 127) / 128, keys = (a.lk + 127) / 128;
     if (tiles > most) tiles = most;
     if (keys > most) keys = most;
     if (tiles > 0) {
-        hipLaunchKernelGGL((attn_dq_kernel<D, KT, 4, PER>), dim3((unsigned)(tiles * nb)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((attn_dq_kernel<D, 4, PER>), dim3((unsigned)(tiles * nb)), dim3(256), 0, st, a);
         if (int e = launch_status("attn_dq_kernel")) return e;
     }
     if (keys > 0) {
@@ -285,7 +378,7 @@ int launch(const Args& a, hipStream_t st) {
 }  // namespace
 
 int launch_bwd(const Args& a, hipStream_t st) {
-    return a.d <= 64 ? launch<64, 64, 2, 64, true>(a, st) : a.d <= 128 ? launch<128, 32, 2, 32, true>(a, st) : launch<256, 32, 1, 32, false>(a, st);
+    return a.d <= 64 ? launch<64, 2, 64, true>(a, st) : a.d <= 128 ? launch<128, 2, 64, true>(a, st) : launch<256, 1, 32, false>(a, st);
 }
 
 }  // namespace attn
