@@ -364,5 +364,12 @@ __device__ __forceinline__ void store_block(uint8_t* row, bool f32, bool on, int
     }
 }
 
+// products between an LDS operand's read and its use in the loops that place every instruction
+constexpr int kAhead = 4;
+
+// the backward's factor on the scores, in base 2. With a scale of zero a factor that leaves nothing of a finite score; so a masked score
+// is an infinity of the other sign, and its exponential zero.
+__device__ __forceinline__ float back_scale(const Args& a) { return a.scale == 0.0f ? 0x1p-126f : a.scale * kLog2e; }
+
 }  // namespace attn
 }  // namespace r97q

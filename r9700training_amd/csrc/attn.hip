@@ -1,5 +1,5 @@
 // attn.hip -- the C entries of attention's forward and backward: checks and the kernels' arguments. The
-// kernels are in attn_fwd.hip and attn_bwd.hip.
+// kernels are in attn_fwd.hip, attn_dq.hip and attn_dkdv.hip.
 #include <cmath>
 
 #include "attn.h"
@@ -10,7 +10,9 @@ namespace attn {
 
 int64_t fwd_workspace(const Args& a);
 int launch_fwd(Args a, void* workspace, hipStream_t st);
-int launch_bwd(const Args& a, hipStream_t st);
+int launch_dq(const Args& a, hipStream_t st);
+int launch_dkdv(const Args& a, hipStream_t st);
+int launch_dkdv_wide(const Args& a, hipStream_t st);
 
 namespace {
 
@@ -186,7 +188,8 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
     a.lse = const_cast<float*>(lse);
     a.base = static_cast<float*>(workspace);
     a.delta = a.base + a.slots;
-    return launch_bwd(a, (hipStream_t)stream);
+    if (int e = launch_dq(a, (hipStream_t)stream)) return e;
+    return a.d > 128 ? launch_dkdv_wide(a, (hipStream_t)stream) : launch_dkdv(a, (hipStream_t)stream);
 }
 
 }  // extern "C"

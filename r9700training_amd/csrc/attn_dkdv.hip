@@ -1,186 +1,11 @@
-// attn_bwd.hip -- attention's backward pass, the probabilities recomputed from the log-sum-exp L:
-//   P = exp(scale Q K^T - L)    D_i = sum_d dO_id O_id    dS = P o (dO V^T - D)
-//   dV = P^T dO    dQ = scale dS K    dK = scale dS^T Q,  dK and dV summed over the heads that share a key head.
-//
-// Two launches: attn_dq_kernel walks the keys for tiles of rows (and writes D), attn_dkdv_kernel walks the
-// rows for tiles of keys. Both recompute P and dO V^T: seven products where one launch would need five,
-// but every sum has one owner and a fixed order, so repeated calls give the same bits, and no f32 gradient
-// passes through memory. P and dS are rounded to bf16 for their products (half a step of 2^-8 relative, each
-// term of a sum on its own), everything else is f32.
-//
-// Bound by the matrix cores. The vector work of a tile lies beside products that do not need it: the
-// exponentials beside dO V^T, dS beside dV.
+// attn_dkdv.hip -- attention's backward pass, second launch: dK and dV (the formulas and the first launch are in
+// attn_dq.hip). Built once for heads of up to 128 columns and once, R97Q_WIDE, for heads of 256.
 #include "attn.h"
 #include "status.h"
 
 namespace r97q {
 namespace attn {
 namespace {
-
-// ---------------------------------------------------------------- dQ (and D): 32 NW rows a workgroup
-// The waves walk the keys together, 32 at a time. Step j of a wave: dO V_j^T beside the exponentials of the scores j,
-// the scores j + 1 beside dS_j, then dQ += dS_j K_j; at its top the values j and keys j + 1 have landed, and the
-// slots of the values j - 1 and the keys j - 1 are free for the next loads. Every product's LDS operand is read
-// kAhead products before it.
-constexpr int kAhead = 4;
-
-// the scores' factor in base 2. With a scale of zero a factor that leaves nothing of a finite score; so a masked score
-// is an infinity of the other sign, and its exponential zero.
-__device__ __forceinline__ float score_scale(const Args& a) { return a.scale == 0.0f ? 0x1p-126f : a.scale * kLog2e; }
-
-template <int D, int NW, int PER>
-__global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
-    using T = Tile<D>;
-    using F = Frags<D>;
-    constexpr int KT = 32, TB = KT * T::RB, n = D / 16;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[5 * TB];  // keys' three slots, then the values' two
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
-    const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, tiles = gridDim.x / nb;
-    const Seq s = sequence(a, bh / a.hk);
-    const int rows = s.lq * a.g;
-    const float sl = score_scale(a), out_of_sight = sl > 0.0f ? -INFINITY : INFINITY;
-    const uint8_t* kb = kv_at(a.k, a, s, hk);
-    const uint8_t* vb = kv_at(a.v, a, s, hk);
-    const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
-    const Loader<D, KT, 64 * NW> kl(kts, a.d, tid), vl(vts, a.d, tid);
-    const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + F::col0(lane);
-    for (int64_t tile = tiles - 1 - (int)(blockIdx.x / nb); tile * 32 * NW < rows; tile += tiles) {
-        const int w0 = (int)tile * 32 * NW, r0 = w0 + 32 * wave, r = r0 + col;
-        const int rr = r < rows ? r : rows - 1, tok = rr / a.g, head = hk * a.g + (rr - tok * a.g);
-        const int wend = w0 + 32 * NW - 1 < rows ? w0 + 32 * NW - 1 : rows - 1;
-        const Keys all = keys_of(a, s, w0 / a.g, wend / a.g);
-        const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
-        const Keys own = keys_of(a, s, (r0 < rows ? r0 : rows - 1) / a.g, rend / a.g);
-        const int lo = all.lo / KT * KT, hi = all.hi, last2 = 2 * a.d;
-        Rows kr(kb, kts, lo, hi, a.d), vr(vb, vts, lo, hi, a.d);
-        if (lo < hi) {
-            kl.load(kr, mine);
-            kr.step(KT * kts, last2);
-        }
-        int d = fresh(a.d);
-        bf16x8 q[n], go[n];
-        load_row<D>(q_at(a.q, a, s, head) + 2 * (tok * a.q.ts), r < rows, d, lane, q);
-        load_row<D>(q_at(a.d_o, a, s, head) + 2 * (tok * a.d_o.ts), r < rows, d, lane, go);
-        const uint8_t* op = q_at(a.o, a, s, head) + (a.o.f32 ? 4 : 2) * (tok * a.o.ts);
-        float delta = 0.0f;
-#pragma unroll
-        for (int c = 0; c < n; ++c) {
-            const int e = 16 * c + 8 * h;
-            if (e < d) {
-                if (a.o.f32) {
-                    const float4 x = *reinterpret_cast<const float4*>(op + 4 * e), y = *reinterpret_cast<const float4*>(op + 4 * e + 16);
-                    delta += x.x * (float)go[c][0] + x.y * (float)go[c][1] + x.z * (float)go[c][2] + x.w * (float)go[c][3];
-                    delta += y.x * (float)go[c][4] + y.y * (float)go[c][5] + y.z * (float)go[c][6] + y.w * (float)go[c][7];
-                } else {
-                    const bf16x8 x = as_bf16x8(*reinterpret_cast<const u32x4*>(op + 2 * e));
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) delta += (float)x[j] * (float)go[c][j];
-                }
-            }
-        }
-        delta = pair_sum(delta);
-        const int64_t st = stat_at(a, s, head, tok);
-        const float lse = a.lse[st], base = lse == -INFINITY ? 0.0f : lse * kLog2e;
-        if (r < rows && h == 0) {
-            a.base[st] = base;
-            a.delta[st] = delta;
-        }
-        const int first = a.window ? (int)clamp64((int64_t)tok + s.off - a.window + 1, 0, s.lk) : 0;
-        const int last = a.causal && tok + s.off < s.lk - 1 ? tok + s.off : s.lk - 1;
-        const uint32_t many = last < first ? 0u : (uint32_t)(last - first) + 1u;
-        f32x16 dq[D / 32];
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) dq[i] = (f32x16){};
-        if (lo < hi) {
-            const int nt = (hi - lo + KT - 1) / KT;
-            landed();
-            __syncthreads();
-            kl.load(kr, mine + TB);
-            kr.step(KT * kts, last2);
-            vl.load(vr, mine + 3 * TB);
-            vr.step(KT * vts, last2);
-            f32x16 x0 = {}, x1 = {};
-            auto product = [&](f32x16& x, uint32_t from) {
-                x = (f32x16){};
-                bf16x8 f[kAhead];
-                steps<kAhead>([&](auto i) { f[i] = F::template rows<0, i>(from); });
-                steps<n>([&](auto i) {
-                    const bf16x8 now = f[i % kAhead];
-                    if constexpr (i + kAhead < n) f[i % kAhead] = F::template rows<0, i + kAhead>(from);
-                    x = mfma(now, q[i], x);
-                });
-            };
-            product(x0, rat);
-            uint32_t k_now = 0, k_next = TB, k_free = 2 * TB, v_now = 3 * TB, v_free = 4 * TB;
-            auto step = [&](f32x16& x, f32x16& next, int j) {
-                landed();
-                __syncthreads();
-                const int j0 = lo + j * KT;
-                if (j0 < own.all_lo || j0 + KT > own.all_hi) {
-                    const uint32_t from = (uint32_t)(j0 + 4 * h - first);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = from + (uint32_t)(8 * (e >> 2) + (e & 3)) < many ? x[e] : out_of_sight;
-                }
-                f32x16 y = {};
-                next = (f32x16){};
-                u32x4 ds[2];
-                bf16x8 f[kAhead];
-                const uint32_t vat = rat + v_now, kat = rat + k_next, dat = cat + k_now;
-                // operand of product i: V rows, next K rows, K columns
-                auto frag = [&](auto i) {
-                    if constexpr (i < n) return F::template rows<0, i>(vat);
-                    else if constexpr (i < 2 * n) return F::template rows<0, i - n>(kat);
-                    else return F::template cols<16 * ((i - 2 * n) / (D / 32)), (i - 2 * n) % (D / 32)>(dat);
-                };
-                steps<kAhead>([&](auto i) { f[i] = frag(i); });
-                kl.load(kr, mine + k_free);
-                vl.load(vr, mine + v_free);
-                steps<3 * n>([&](auto i) {
-                    pin();
-                    const bf16x8 now = f[i % kAhead];
-                    if constexpr (i + kAhead < 3 * n) f[i % kAhead] = frag(std::integral_constant<int, i + kAhead>{});
-                    if constexpr (i < n) {
-                        y = mfma(now, go[i], y);
-#pragma unroll
-                        for (int e = 16 * i / n; e < 16 * (i + 1) / n; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] * sl - base);
-                    } else if constexpr (i < 2 * n) {
-                        next = mfma(now, q[i - n], next);
-                        // two products later the last one of y is through
-                        constexpr int c = i - n - 2, m = n - 2;
-                        if constexpr (c >= 0) {
-#pragma unroll
-                            for (int e = 2 * (8 * c / m); e < 2 * (8 * (c + 1) / m); e += 2) {
-                                x[e] *= y[e] - delta;
-                                x[e + 1] *= y[e + 1] - delta;
-                                pack_two(x, e, ds);
-                            }
-                        }
-                    } else {
-                        constexpr int c = (i - 2 * n) / (D / 32), m = (i - 2 * n) % (D / 32);
-                        dq[m] = mfma(now, as_bf16x8(ds[c]), dq[m]);
-                    }
-                });
-                pin();
-                kr.step(KT * kts, last2);
-                vr.step(KT * vts, last2);
-                const uint32_t k = k_now, v = v_now;
-                k_now = k_next, k_next = k_free, k_free = k;
-                v_now = v_free, v_free = v;
-            };
-            for (int j = 0; j < nt; j += 2) {
-                step(x0, x1, j);
-                if (j + 1 < nt) step(x1, x0, j + 1);
-            }
-            landed();
-        }
-        d = fresh(a.d);
-        const int hs = fresh_lane(h);
-        uint8_t* out = q_at(a.dq, a, s, head) + (a.dq.f32 ? 4 : 2) * (tok * a.dq.ts);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) store_block(out, a.dq.f32, r < rows, 32 * i, d, hs, dq[i], a.scale);
-        __syncthreads();
-    }
-}
 
 // ---------------------------------------------------------------- dK, dV: 32 NW keys a workgroup
 // A wave holds 32 keys and their gradients; the workgroup walks the heads and the tokens that see its keys,
@@ -198,7 +23,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_dkdv_kernel(Args a) {
     const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, tiles = gridDim.x / nb;
     const Seq s = sequence(a, bh / a.hk);
     const int cover = a.kv_starts ? s.lk : a.lk;  // the dense form's keys past a sequence's length get zeros
-    const float sl = score_scale(a), out_of_sight = sl > 0.0f ? -INFINITY : INFINITY;
+    const float sl = back_scale(a), out_of_sight = sl > 0.0f ? -INFINITY : INFINITY;
     const int64_t qts = 2 * a.q.ts, ots = 2 * a.d_o.ts;
     const Loader<D, RT, 64 * NW> ql(qts, a.d, tid), ol(ots, a.d, tid);
     const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + F::col0(lane);
@@ -358,28 +183,23 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_dkdv_kernel(Args a) {
     }
 }
 
-template <int D, int PER, int RT, bool KEPT>
-int launch(const Args& a, hipStream_t st) {
+template <int D, int RT, bool KEPT>
+int run(const Args& a, hipStream_t st) {
     const int64_t nb = (int64_t)a.batch * a.hk, most = 0x7FFFFFFF / nb;
-    int64_t tiles = ((int64_t)a.lq * a.g + 127) / 128, keys = (a.lk + 127) / 128;
-    if (tiles > most) tiles = most;
+    int64_t keys = ((int64_t)a.lk + 127) / 128;
     if (keys > most) keys = most;
-    if (tiles > 0) {
-        hipLaunchKernelGGL((attn_dq_kernel<D, 4, PER>), dim3((unsigned)(tiles * nb)), dim3(256), 0, st, a);
-        if (int e = launch_status("attn_dq_kernel")) return e;
-    }
-    if (keys > 0) {
-        hipLaunchKernelGGL((attn_dkdv_kernel<D, RT, 4, KEPT>), dim3((unsigned)(keys * nb)), dim3(256), 0, st, a);
-        return launch_status("attn_dkdv_kernel");
-    }
-    return R97Q_OK;
+    if (keys == 0) return R97Q_OK;
+    hipLaunchKernelGGL((attn_dkdv_kernel<D, RT, 4, KEPT>), dim3((unsigned)(keys * nb)), dim3(256), 0, st, a);
+    return launch_status("attn_dkdv_kernel");
 }
 
 }  // namespace
 
-int launch_bwd(const Args& a, hipStream_t st) {
-    return a.d <= 64 ? launch<64, 2, 64, true>(a, st) : a.d <= 128 ? launch<128, 2, 64, true>(a, st) : launch<256, 1, 32, false>(a, st);
-}
+#if R97Q_WIDE
+int launch_dkdv_wide(const Args& a, hipStream_t st) { return run<256, 32, false>(a, st); }
+#else
+int launch_dkdv(const Args& a, hipStream_t st) { return a.d <= 64 ? run<64, 64, true>(a, st) : run<128, 64, true>(a, st); }
+#endif
 
 }  // namespace attn
 }  // namespace r97q
