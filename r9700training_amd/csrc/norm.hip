@@ -8,15 +8,18 @@
 //
 // Bound by memory: a row is read once into registers (8 consecutive columns a thread and step), its sums
 // taken across the threads, and everything written from there. Rows of up to 2048 columns belong to a
-// wave, four of them to a workgroup, with no barrier; wider ones to a workgroup. Rows past 8192 columns, odd
-// widths, groups that do not fall on lanes and unaligned tensors take the general kernels, which read a
-// row again for each stage.
+// wave, four of them to a workgroup, with no barrier; wider ones, up to 16384 columns, to a workgroup. Wider
+// rows, odd widths, groups that do not fall on lanes and unaligned tensors take the general kernels, which read
+// a row again for each stage.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
+#include <type_traits>
 
 #include "../../include/r97q.h"
+#include "group_lanes.h"
 #include "iqr_device.h"
 #include "status.h"
 
@@ -65,31 +68,66 @@ __device__ __forceinline__ float as_stored(float v) {
         return v;
 }
 
+// both values of the pair of lanes H apart
+template <int H>
+__device__ __forceinline__ void lane_pair(float v, float& lo, float& hi) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    if constexpr (H < 16) {
+        lo = v;
+        hi = __builtin_bit_cast(float, lanes::other<H>(x));
+    } else {
+        const auto s = H == 16 ? __builtin_amdgcn_permlane16_swap(x, x, false, false)
+                               : __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        const uint32_t p = s[0], q = s[1];
+        lo = __builtin_bit_cast(float, p);
+        hi = __builtin_bit_cast(float, q);
+    }
+}
+template <int H>
+__device__ __forceinline__ float lane_sum(float v) {
+    float lo, hi;
+    lane_pair<H>(v, lo, hi);
+    return lo + hi;
+}
+template <int H>
+__device__ __forceinline__ float lane_max(float v) {
+    float lo, hi;
+    lane_pair<H>(v, lo, hi);
+    return fmaxf(lo, hi);
+}
 __device__ __forceinline__ float wave_sum(float v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return lane_sum<32>(lane_sum<16>(lane_sum<8>(lane_sum<4>(lane_sum<2>(lane_sum<1>(v))))));
+}
+// the maximum over 2^lg neighbouring lanes, in all of them (lg uniform, 0 .. 6)
+__device__ __forceinline__ float lanes_max(float v, int lg) {
+    if (lg > 0) v = lane_max<1>(v);
+    if (lg > 1) v = lane_max<2>(v);
+    if (lg > 2) v = lane_max<4>(v);
+    if (lg > 3) v = lane_max<8>(v);
+    if (lg > 4) v = lane_max<16>(v);
+    if (lg > 5) v = lane_max<32>(v);
     return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
+__device__ __forceinline__ float wave_max(float v) { return lanes_max(v, 6); }
 // over the workgroup, the waves' values in wave order
 __device__ float block_sum(float v, float* red) {
+    const int waves = blockDim.x >> 6;
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     float t = red[0];
-    for (int i = 1; i < kWaves; ++i) t += red[i];
+    for (int i = 1; i < waves; ++i) t += red[i];
     return t;
 }
 __device__ float block_max(float v, float* red) {
+    const int waves = blockDim.x >> 6;
     v = wave_max(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     float t = red[0];
-    for (int i = 1; i < kWaves; ++i) t = fmaxf(t, red[i]);
+    for (int i = 1; i < waves; ++i) t = fmaxf(t, red[i]);
     return t;
 }
 
@@ -181,27 +219,236 @@ __global__ __launch_bounds__(kThreads) void norm_any_bwd_kernel(NArgs a) {
     }
 }
 
+// ---------------------------------------------------------------- rows in registers
+// A row belongs to a wave (WIDE false, four to a workgroup) or to the workgroup. A thread holds S pieces of 8
+// columns, 8 * (threads a row) apart, so a wave's 64 pieces are 512 neighbouring columns and a group of
+// 8 .. 512 columns (a power of two) lies in 2^lg neighbouring lanes. lg < 0: one group, the whole row.
+constexpr int kMostWaves = 16;
+
+template <class T>
+__device__ __forceinline__ void store_piece(void* p, int64_t i, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        using b2 = __attribute__((ext_vector_type(2))) __bf16;
+        uint32_t u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            b2 v = {(__bf16)x[2 * k], (__bf16)x[2 * k + 1]};
+            u[k] = __builtin_bit_cast(uint32_t, v);
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+        lanes::store8(static_cast<float*>(p) + i, x);
+    }
+}
+template <class T>
+__device__ __forceinline__ void load_piece(const void* p, int64_t i, float (&x)[8]) {
+    lanes::load8(static_cast<const T*>(p) + i, x);
+}
+
+template <class T, int S, bool WIDE>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, int lg) {
+    __shared__ float red[kMostWaves];
+    const int wave = threadIdx.x >> 6, t = WIDE ? threadIdx.x : threadIdx.x & 63, per = WIDE ? blockDim.x : 64;
+    const int64_t row = WIDE ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    if (row >= a.rows) return;
+    const int n = (int)a.n;
+    const int64_t base = row * n;
+    float h[S][8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        const int c = 8 * (t + i * per);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[i][k] = 0.0f;
+        if (c < n) load_piece<T>(a.x, base + c, h[i]);
+    }
+    if (a.res) {
+        float r[S][8];
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int c = 8 * (t + i * per);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) r[i][k] = 0.0f;
+            if (c < n) load_piece<T>(a.res, base + c, r[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int c = 8 * (t + i * per);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) h[i][k] = as_stored<T>(h[i][k] + r[i][k]);
+            if (c < n) store_piece<T>(a.h, base + c, h[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ss += h[i][k] * h[i][k];
+    ss = WIDE ? block_sum(ss, red) : wave_sum(ss);
+    const float rs = 1.0f / sqrtf(ss / (float)n + a.eps);
+    if (t == 0 && a.rstd) a.rstd[row] = rs;
+    float top[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        const int c = 8 * (t + i * per);
+        float w[8] = {};
+        if (c < n) load_piece<T>(a.w, c, w);
+        top[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            h[i][k] = h[i][k] * rs * (w[k] + a.wadd);
+            top[i] = fmaxf(top[i], fabsf(h[i][k]));
+        }
+        if (a.y && c < n) store_piece<uint16_t>(a.y, base + c, h[i]);
+    }
+    if (!a.codes) return;
+    if (lg < 0) {
+#pragma unroll
+        for (int i = 1; i < S; ++i) top[0] = fmaxf(top[0], top[i]);
+        top[0] = WIDE ? block_max(top[0], red) : wave_max(top[0]);
+#pragma unroll
+        for (int i = 1; i < S; ++i) top[i] = top[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i) top[i] = lanes_max(top[i], lg);
+    }
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        const int c = 8 * (t + i * per);
+        if (c >= n) continue;
+        const Quant q(top[i]);
+        uint32_t b[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) b[k >> 2] |= (uint32_t)(q.code(h[i][k]) & 255) << (8 * (k & 3));
+        *reinterpret_cast<uint2*>(a.codes + base + c) = make_uint2(b[0], b[1]);
+        if (lg < 0 ? t == 0 && i == 0 : (t & ((1 << lg) - 1)) == 0) a.scale[row * a.ngroups + (lg < 0 ? 0 : c >> (lg + 3))] = q.scale;
+    }
+}
+
+// The adjoint: a wave or workgroup walks rows and keeps its columns' sums of dw in registers.
+template <class T, int S, bool WIDE>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs a, int lg) {
+    __shared__ float red[kMostWaves];
+    __shared__ float sums[WIDE ? 1 : 4 * 512 * S];
+    const int wave = threadIdx.x >> 6, t = WIDE ? threadIdx.x : threadIdx.x & 63, per = WIDE ? blockDim.x : 64;
+    const int n = (int)a.n;
+    const int64_t first = WIDE ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave, step = WIDE ? gridDim.x : (int64_t)gridDim.x * 4;
+    float dw[S][8] = {};
+    for (int64_t row = first; row < a.rows; row += step) {
+        const int64_t base = row * n;
+        const float rs = a.rstd[row];
+        float x[S][8], e[S][8], gh[S][8];
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int c = 8 * (t + i * per);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[i][k] = e[i][k] = gh[i][k] = 0.0f;
+            if (c < n) {
+                load_piece<T>(a.x, base + c, x[i]);
+                if (a.gy) load_piece<T>(a.gy, base + c, e[i]);
+                if (a.gh) load_piece<T>(a.gh, base + c, gh[i]);
+            }
+        }
+        if (a.gc) {
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                const int c = 8 * (t + i * per);
+                if (c >= n) continue;
+                float gc[8];
+                load_piece<T>(a.gc, base + c, gc);
+                const Cotangent q(a.scale[row * a.ngroups + (lg < 0 ? 0 : c >> (lg + 3))]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) e[i][k] = q.sum(gc[k], e[i][k]);
+            }
+        }
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int c = 8 * (t + i * per);
+            float w[8] = {};
+            if (c < n) load_piece<T>(a.w, c, w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                x[i][k] *= rs;
+                dw[i][k] += e[i][k] * x[i][k];
+                e[i][k] *= w[k] + a.wadd;
+                dot += e[i][k] * x[i][k];
+            }
+        }
+        const float mean = (WIDE ? block_sum(dot, red) : wave_sum(dot)) / (float)n;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int c = 8 * (t + i * per);
+            if (c >= n) continue;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) gh[i][k] += rs * (e[i][k] - x[i][k] * mean);
+            store_piece<T>(a.dx, base + c, gh[i]);
+        }
+    }
+    if (!a.part) return;
+    float* part = a.part + (int64_t)blockIdx.x * n;
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int c = 8 * (t + i * per);
+            if (c < n) lanes::store8(part + c, dw[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i) lanes::store8(sums + (wave * S + i) * 512 + 8 * t, dw[i]);
+        __syncthreads();
+        for (int c = threadIdx.x; c < n; c += 256) part[c] = (sums[c] + sums[512 * S + c]) + (sums[1024 * S + c] + sums[1536 * S + c]);
+    }
+}
+
 // ---------------------------------------------------------------- dw from the workgroups' partial sums
-// 64 columns a workgroup; each of its 16 waves adds every 16th of the partial rows, the waves' sums are
-// added in order.
+// 32 columns a workgroup; each of its 32 half waves adds every 32nd of the partial rows, their sums are added in
+// order.
 __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__ part, int64_t parts, int64_t n,
                                                        float* __restrict__ dw, int32_t add) {
-    __shared__ float sum[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t j = (int64_t)blockIdx.x * 64 + lane;
+    __shared__ float sum[32][32];
+    const int col = threadIdx.x & 31, half = threadIdx.x >> 5;
+    const int64_t j = (int64_t)blockIdx.x * 32 + col;
     float s = 0.0f;
     if (j < n) {
 #pragma unroll 8
-        for (int64_t p = wave; p < parts; p += 16) s += part[p * n + j];
+        for (int64_t p = half; p < parts; p += 32) s += part[p * n + j];
     }
-    sum[wave][lane] = s;
+    sum[half][col] = s;
     __syncthreads();
-    if (wave == 0 && j < n) {
-        float t = sum[0][lane];
+    if (half == 0 && j < n) {
+        float t = sum[0][col];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) t += sum[i][lane];
+        for (int i = 1; i < 32; ++i) t += sum[i][col];
         dw[j] = add ? dw[j] + t : t;
     }
+}
+
+// how the rows are taken: 0 the general kernels, else pieces a thread; threads of a workgroup; lanes of a group
+struct Rows {
+    int pieces, threads, lg;
+    bool wide;
+};
+Rows rows_plan(int64_t n, int64_t group, std::initializer_list<const void*> tensors) {
+    Rows r = {};
+    if (n % 8 || n > 16384) return r;
+    for (const void* p : tensors)
+        if (!lanes::aligned16(p)) return r;
+    r.lg = group >= n ? -1 : lanes::group_log(group) - 3;
+    if (group < n && lanes::group_log(group) < 0) return r;
+    r.wide = n > 2048;
+    r.pieces = r.wide ? 2 : (int)((n + 511) / 512);
+    r.threads = r.wide ? 64 * (int)((n + 1023) / 1024) : 256;
+    return r;
+}
+// f(a kernel's pieces, whether the row is a workgroup's)
+template <class F>
+void with_rows(const Rows& r, F&& f) {
+    using std::integral_constant;
+    if (r.wide) return f(integral_constant<int, 2>{}, std::true_type{});
+    if (r.pieces == 1) return f(integral_constant<int, 1>{}, std::false_type{});
+    if (r.pieces == 2) return f(integral_constant<int, 2>{}, std::false_type{});
+    if (r.pieces == 3) return f(integral_constant<int, 3>{}, std::false_type{});
+    return f(integral_constant<int, 4>{}, std::false_type{});
 }
 
 int64_t bwd_parts(int64_t rows) { return rows < 512 ? rows : 512; }
@@ -252,6 +499,17 @@ int r97q_add_rmsnorm_i8g(const void* x, const void* residual, const void* w, int
     a.scale = scale;
     a.y = y_out;
     a.rstd = rstd;
+    const Rows r = rows_plan(n, a.group, {x, residual, w, h_out, codes, y_out});
+    if (r.pieces) {
+        with_rows(r, [&](auto pieces, auto wide) {
+            const dim3 grid((unsigned)(wide ? rows : (rows + 3) / 4)), threads(r.threads);
+            if (dtype == R97Q_BF16)
+                hipLaunchKernelGGL((norm_rows_kernel<uint16_t, pieces, wide>), grid, threads, 0, (hipStream_t)stream, a, r.lg);
+            else
+                hipLaunchKernelGGL((norm_rows_kernel<float, pieces, wide>), grid, threads, 0, (hipStream_t)stream, a, r.lg);
+        });
+        return launch_status("norm_rows_kernel");
+    }
     if (dtype == R97Q_BF16)
         hipLaunchKernelGGL(norm_any_kernel<uint16_t>, dim3((unsigned)rows), dim3(kThreads), 0, (hipStream_t)stream, a);
     else
@@ -291,8 +549,21 @@ int r97q_add_rmsnorm_i8g_bwd(const void* h, const void* w, int32_t dtype, int64_
     a.gh = g_h;
     a.dx = dx;
     a.part = dw ? static_cast<float*>(workspace) : nullptr;
-    const int64_t parts = bwd_parts(rows);
-    if (rows > 0) {
+    int64_t parts = bwd_parts(rows);
+    const Rows r = rows_plan(n, a.group, {h, w, g_codes, g_y, g_h, dx});
+    if (rows > 0 && r.pieces) {
+        // four rows at a time a workgroup where a row is a wave's
+        const int64_t most = r.wide ? rows : (rows + 3) / 4;
+        if (parts > most) parts = most;
+        with_rows(r, [&](auto pieces, auto wide) {
+            const dim3 grid((unsigned)(dw ? parts : most)), threads(r.threads);
+            if (dtype == R97Q_BF16)
+                hipLaunchKernelGGL((norm_rows_bwd_kernel<uint16_t, pieces, wide>), grid, threads, 0, st, a, r.lg);
+            else
+                hipLaunchKernelGGL((norm_rows_bwd_kernel<float, pieces, wide>), grid, threads, 0, st, a, r.lg);
+        });
+        if (int e = launch_status("norm_rows_bwd_kernel")) return e;
+    } else if (rows > 0) {
         const dim3 grid((unsigned)(dw ? parts : rows));
         if (dtype == R97Q_BF16)
             hipLaunchKernelGGL(norm_any_bwd_kernel<uint16_t>, grid, dim3(kThreads), 0, st, a);
@@ -301,7 +572,7 @@ int r97q_add_rmsnorm_i8g_bwd(const void* h, const void* w, int32_t dtype, int64_
         if (int e = launch_status("norm_any_bwd_kernel")) return e;
     }
     if (!dw) return R97Q_OK;
-    hipLaunchKernelGGL(norm_dw_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, st, a.part, parts, n, dw, dw_accumulate);
+    hipLaunchKernelGGL(norm_dw_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, st, a.part, parts, n, dw, dw_accumulate);
     return launch_status("norm_dw_kernel");
 }
 
