@@ -14,15 +14,15 @@ import torch
 from . import R97Q_BF16, R97Q_F32, AttnShape, Heads, _empty, _ptr, _stream, check, lib
 
 
+_DTYPES = {torch.bfloat16: R97Q_BF16, torch.float32: R97Q_F32}
+
+
 def _heads(x: torch.Tensor, packed: bool, what: str) -> Heads:
-    n = 3 if packed else 4
-    if x.dim() != n or not x.is_cuda or (x.stride(n - 1) != 1 and x.numel()):
+    st, shape = x.stride(), x.shape
+    if len(shape) != (3 if packed else 4) or not x.is_cuda or (st[-1] != 1 and x.numel()):
         raise ValueError(f"attention: {what} is a device [{'' if packed else 'batch, '}tokens, heads, head_dim] tensor, "
                          "head_dim consecutive")
-    dt = R97Q_BF16 if x.dtype == torch.bfloat16 else R97Q_F32 if x.dtype == torch.float32 else -1
-    if packed:
-        return Heads(x.data_ptr(), 0, x.stride(0), x.stride(1), x.shape[1], dt)
-    return Heads(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), x.shape[2], dt)
+    return Heads(x.data_ptr(), 0 if packed else st[0], st[-3], st[-2], shape[-2], _DTYPES.get(x.dtype, -1))
 
 
 def _index(t: torch.Tensor, n: int | None, what: str) -> torch.Tensor:
@@ -34,28 +34,28 @@ def _index(t: torch.Tensor, n: int | None, what: str) -> torch.Tensor:
 def _shape(q, k, v, causal, window, scale, q_starts, kv_starts, max_q, max_kv, kv_lens) -> AttnShape:
     s = AttnShape()
     pq, pk = q_starts is not None, kv_starts is not None
-    if q.dim() != (3 if pq else 4) or k.dim() != (3 if pk else 4) or v.shape != k.shape or q.shape[-1] != k.shape[-1]:
+    qs, ks = q.shape, k.shape
+    if len(qs) != (3 if pq else 4) or len(ks) != (3 if pk else 4) or v.shape != ks or qs[-1] != ks[-1]:
         raise ValueError("attention: q and k are [batch, tokens, heads, head_dim], packed [tokens, heads, head_dim]; v has "
                          "k's shape")
-    s.head_dim = q.shape[-1]
-    batch = {q_starts.shape[0] - 1 if pq else q.shape[0], kv_starts.shape[0] - 1 if pk else k.shape[0]}
-    if len(batch) != 1 or min(batch) < 0:
+    s.head_dim = qs[-1]
+    s.batch = q_starts.shape[0] - 1 if pq else qs[0]
+    if s.batch < 0 or s.batch != (kv_starts.shape[0] - 1 if pk else ks[0]):
         raise ValueError("attention: q and k hold as many sequences")
-    s.batch = batch.pop()
     if pq:
         _index(q_starts, None, "q_starts")
         if max_q is None:
             raise ValueError("attention: packed queries need max_q, their longest sequence")
-        s.q_starts, s.q_tokens, s.q_len = q_starts.data_ptr(), q.shape[0], int(max_q)
+        s.q_starts, s.q_tokens, s.q_len = q_starts.data_ptr(), qs[0], int(max_q)
     else:
-        s.q_len = q.shape[1]
+        s.q_len = qs[1]
     if pk:
         _index(kv_starts, None, "kv_starts")
         if max_kv is None:
             raise ValueError("attention: packed keys need max_kv, their longest sequence")
-        s.kv_starts, s.kv_tokens, s.kv_len = kv_starts.data_ptr(), k.shape[0], int(max_kv)
+        s.kv_starts, s.kv_tokens, s.kv_len = kv_starts.data_ptr(), ks[0], int(max_kv)
     else:
-        s.kv_len = k.shape[1]
+        s.kv_len = ks[1]
     if kv_lens is not None:
         s.kv_lens = _index(kv_lens, s.batch, "kv_lens").data_ptr()
     s.causal, s.window = int(bool(causal)), int(window)
@@ -64,11 +64,12 @@ def _shape(q, k, v, causal, window, scale, q_starts, kv_starts, max_q, max_kv, k
 
 
 def _lse_shape(q, packed):
-    return (q.shape[1], q.shape[0]) if packed else (q.shape[0], q.shape[2], q.shape[1])
+    s = q.shape
+    return (s[1], s[0]) if packed else (s[0], s[2], s[1])
 
 
 def _check_lse(lse, q, packed):
-    if lse.dtype != torch.float32 or tuple(lse.shape) != _lse_shape(q, packed) or not lse.is_contiguous() or not lse.is_cuda:
+    if lse.dtype != torch.float32 or lse.shape != _lse_shape(q, packed) or not lse.is_contiguous() or not lse.is_cuda:
         raise ValueError("attention: lse is a contiguous f32 [batch, heads, tokens] device tensor, packed [heads, tokens]")
 
 

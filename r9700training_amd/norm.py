@@ -23,7 +23,7 @@ def _stream_dtype(x: torch.Tensor) -> int:
 
 
 def _vector(t: torch.Tensor, dtype, shape, what: str) -> None:
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda:
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"add_rmsnorm_i8g: {what} is a contiguous {dtype} device tensor of shape {shape}")
 
 

@@ -29,16 +29,17 @@ def rotary_frequencies(rot: int, base: float = 10000.0, scaling: str = "plain", 
     return torch.from_numpy(f).to(device), float(m.value)
 
 
+_DTYPES = {torch.bfloat16: R97Q_BF16, torch.float32: R97Q_F32}
+
+
 def _heads(x: torch.Tensor, what: str) -> Heads:
-    if x.dim() != 3 or x.stride(2) != 1 or not x.is_cuda:
+    st, shape = x.stride(), x.shape
+    if len(shape) != 3 or st[2] != 1 or not x.is_cuda:
         raise ValueError(f"rotary: {what} is a device [tokens, heads, head_dim] tensor, head_dim consecutive")
-    if x.dtype == torch.bfloat16:
-        dt = R97Q_BF16
-    elif x.dtype == torch.float32:
-        dt = R97Q_F32
-    else:
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
         raise ValueError(f"rotary: {what} is bf16 or f32")
-    return Heads(x.data_ptr(), 0, x.stride(0), x.stride(1), x.shape[1], dt)
+    return Heads(x.data_ptr(), 0, st[0], st[1], shape[1], dt)
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
@@ -54,7 +55,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, posi
     tokens, _, dim = q.shape if q.dim() == 3 else (0, 0, 0)
     wide = 0
     if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (tokens,) \
+        if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) \
                 or not positions.is_contiguous() or not positions.is_cuda:
             raise ValueError("rotary: positions are a contiguous int32 or int64 [tokens] device tensor")
         wide = int(positions.dtype == torch.int64)
