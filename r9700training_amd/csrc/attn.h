@@ -51,7 +51,11 @@ struct Args {
     Heads d_o, dq, dk, dv;
     float* lse;          // [b][h][Lq], packed: [h][q_tokens]
     float* base;         // backward: the log-sum-exp in base 2 (0 for a row that sees nothing), laid out as lse
-    float* delta;        // and the sum over d of dO * O
+    float* delta;        // and minus the sum over d of dO * O
+    // the backward cut over the other side's steps where its grids are small: partial sums in f32, added in order
+    int32_t q_splits, k_splits;
+    int64_t kv_slots;    // rows of one dk or dv partial
+    float *dq_part, *dk_part, *dv_part;  // [splits][slots][d]
     int32_t batch, hq, hk, g, d;
     int32_t lq, lk;      // tokens of a sequence (packed: of the longest)
     const int32_t* q_starts;
@@ -67,6 +71,13 @@ struct Args {
     float* part;         // [splits][slots][d]
     float2* stats;       // [splits][slots]
 };
+
+// What the launches are cut by: tiles of `tile` rows or keys in all sequences together, and a sequence's tokens. Packed
+// sequences go by their tokens in all, not by the longest.
+inline int64_t all_tiles(bool packed, int64_t tokens, int64_t len, int64_t batch, int64_t each, int64_t tile) {
+    return packed ? (tokens * each + tile - 1) / tile : batch * ((len * each + tile - 1) / tile);
+}
+inline int64_t mean_len(bool packed, int64_t tokens, int64_t len, int64_t batch) { return packed ? (tokens + batch - 1) / batch : len; }
 
 // one sequence: its tokens' places and counts. Starts and lengths come from device memory, so they are
 // clamped to the tensors: nothing is read or written past them whatever they hold.
@@ -127,6 +138,11 @@ __device__ __forceinline__ int64_t stat_at(const Args& a, const Seq& s, int h, i
     return a.q_starts ? h * a.q_tokens + s.q_base + token : ((int64_t)s.b * a.hq + h) * a.lq + token;
 }
 
+// a key's row of a partial sum
+__device__ __forceinline__ int64_t kv_slot(const Args& a, const Seq& s, int hk, int key) {
+    return a.kv_starts ? hk * a.kv_tokens + s.k_base + key : ((int64_t)s.b * a.hk + hk) * a.lk + key;
+}
+
 // the keys [lo, hi) that some of the queries at tokens [t0, t1] see (hi <= lo: none), and [all_lo, all_hi)
 // that all of them see
 struct Keys {
@@ -147,6 +163,48 @@ __device__ __forceinline__ Keys keys_of(const Args& a, const Seq& s, int t0, int
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 x, bf16x8 y, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+}
+// The same with the accumulator in the accumulation registers (ACC: a kernel of one wave a SIMD, whose other registers are
+// all taken). In assembly because the compiler otherwise moves operands and sums back and forth between the two files.
+// It does not see the instruction's latency: the operands are written a product or more before, the sums are read only
+// after settled().
+template <bool ACC>
+__device__ __forceinline__ void add_product(bf16x8 x, bf16x8 y, f32x16& c) {
+    if constexpr (ACC)
+        asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(x), "v"(y));
+    else
+        c = mfma(x, y, c);
+}
+// x times y, y of the accumulation registers where they hold what the others have no room for (HELD): the first product of
+// a sum (FIRST) or one more, to be read a product or more later
+template <bool HELD, bool FIRST>
+__device__ __forceinline__ void product_of(bf16x8 x, const bf16x8& y, f32x16& c) {
+    if constexpr (!HELD)
+        c = FIRST ? mfma(x, y, (f32x16){}) : mfma(x, y, c);
+    else if constexpr (FIRST)
+        asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(x), "a"(y));
+    else
+        asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(x), "a"(y));
+}
+// fragments settle in whole registers of one file, or their words are gathered anew for every product
+template <bool HELD, int N>
+__device__ __forceinline__ void settle(bf16x8 (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (HELD)
+            asm volatile("" : "+a"(f[i]));
+        else
+            asm volatile("" : "+v"(f[i]));
+    }
+}
+// the sums may be read from here on
+template <bool ACC, int N>
+__device__ __forceinline__ void settled(f32x16 (&c)[N]) {
+    if constexpr (ACC) {
+        asm volatile("s_nop 15\n\ts_nop 15");
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("" : "+a"(c[i]));
+    }
 }
 __device__ __forceinline__ bf16x8 as_bf16x8(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
 __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
@@ -263,20 +321,21 @@ __device__ __forceinline__ void pack_two(const f32x16& x, int e, u32x4 (&out)[2]
 // columns past the head's d, gives zeros, so nothing past a sequence is read and no row needs a clamp.
 constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every buffer's end
 struct Rows {
-    const uint8_t* p;    // the next tile's first token
-    int64_t left;        // bytes from there to the end of the last token in use
-    // rows: from token row0 on, `rows` in use in all; ts2: bytes a token
+    uint64_t p;          // the next tile's first token
+    uint32_t ts, tail;   // bytes a token, and of the head in use
+    int left;            // tokens in use from there on
+    // from token row0 of `rows` on; ts2: bytes a token
     __device__ __forceinline__ Rows(const uint8_t* base, int64_t ts2, int row0, int rows, int d)
-        : p(base + row0 * ts2), left(rows > row0 ? (rows - 1 - row0) * ts2 + 2 * d : 0) {}
-    __device__ __forceinline__ void step(int64_t bytes, int64_t last) {  // last: 2 d, what is left past the last token
-        p += bytes;
-        left -= bytes;
-        if (left < last) left = 0;
+        : p(reinterpret_cast<uint64_t>(base) + row0 * ts2), ts((uint32_t)ts2), tail(2 * d), left(rows - row0) {}
+    __device__ __forceinline__ void step(int tokens) {
+        p += (uint64_t)ts * (uint32_t)tokens;
+        left -= tokens;
     }
+    // a tile of R tokens
+    template <int R>
     __device__ __forceinline__ u32x4 buffer() const {
-        const uint64_t u = reinterpret_cast<uint64_t>(p);
-        const uint32_t n = left > 0x7FFFFFF0 ? 0x7FFFFFF0u : (uint32_t)left;
-        return (u32x4){(uint32_t)uniform((int)u), (uint32_t)uniform((int)(u >> 32)) & 0xFFFFu, (uint32_t)uniform((int)n), 0x00020000u};
+        const uint32_t whole = (R - 1) * ts + tail, part = left > 0 ? (uint32_t)(left - 1) * ts + tail : 0u;
+        return (u32x4){(uint32_t)uniform((int)p), (uint32_t)uniform((int)(p >> 32)), (uint32_t)uniform((int)(left >= R ? whole : part)), 0x00020000u};
     }
 };
 
@@ -285,17 +344,14 @@ __device__ __forceinline__ uint32_t lds_at(const void* p) {
     return (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
 }
 // 64 pieces of 16 bytes, a lane's at `off` of the buffer, to LDS dst + 16 lane. In assembly because the compiler would
-// wait for every such load before the next LDS read; the waits are landed()'s, at the loops' barriers.
+// wait for every such load before the next LDS read; the waits are landed()'s, at the loops' barriers. m0 is not put
+// back: nothing else in these kernels uses it.
 __device__ __forceinline__ void load_piece(const u32x4& buf, uint32_t off, uint32_t dst) {
-    uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(off), "s"(buf), "s"(dst));
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(buf), "s"(dst));
 }
 // 64 values of 4 bytes
 __device__ __forceinline__ void load_words(const u32x4& buf, uint32_t off, uint32_t dst) {
-    uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(off), "s"(buf), "s"(dst));
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(off), "s"(buf), "s"(dst));
 }
 // all but the newest N loads have landed in LDS
 template <int N = 0>
@@ -319,21 +375,28 @@ struct Loader {
     }
     // dst: the tile's LDS address + 1024 * the wave's index
     __device__ __forceinline__ void load(const Rows& r, uint32_t dst) const {
-        const u32x4 b = r.buffer();
+        const u32x4 b = r.template buffer<ROWS>();
 #pragma unroll
         for (int i = 0; i < N; ++i) load_piece(b, off[i], dst + 16 * THREADS * i);
     }
 };
 
-// a row's values as B operands: 16 c + 8 h .. + 8 of the head, zeros past d and for rows outside
+// A row's values as B operands: 16 c + 8 h .. + 8 of the head, zeros past d and for rows outside. `row` is a row that may
+// be read whether or not it is valid, so that the loads go out together.
 template <int D>
 __device__ __forceinline__ void load_row(const uint8_t* row, bool valid, int d, int lane, bf16x8 (&out)[D / 16]) {
+    u32x4 w[D / 16];
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
         const int e = 16 * c + 8 * (lane >> 5);
-        u32x4 w = {0, 0, 0, 0};
-        if (valid && e < d) w = *reinterpret_cast<const u32x4*>(row + 2 * e);
-        out[c] = as_bf16x8(w);
+        w[c] = *reinterpret_cast<const u32x4*>(row + (e < d ? 2 * e : 0));
+    }
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+        const bool on = valid && 16 * c + 8 * (lane >> 5) < d;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[c][j] = on ? w[c][j] : 0u;
+        out[c] = as_bf16x8(w[c]);
     }
 }
 
@@ -366,6 +429,8 @@ __device__ __forceinline__ void store_block(uint8_t* row, bool f32, bool on, int
 
 // products between an LDS operand's read and its use in the loops that place every instruction
 constexpr int kAhead = 4;
+// step i of `len` steps from `from`: the elements [lo, hi) of 16 that belong to it, in pairs
+constexpr int pair_from(int i, int from, int len) { return i < from ? 0 : i >= from + len ? 16 : 2 * (8 * (i - from) / len); }
 
 // the backward's factor on the scores, in base 2. With a scale of zero a factor that leaves nothing of a finite score; so a masked score
 // is an infinity of the other sign, and its exponential zero.

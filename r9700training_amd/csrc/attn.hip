@@ -11,6 +11,7 @@ namespace attn {
 int64_t fwd_workspace(const Args& a);
 int launch_fwd(Args a, void* workspace, hipStream_t st);
 int launch_dq(const Args& a, hipStream_t st);
+int launch_sum(const Args& a, const Heads& out, const float* part, int splits, bool keys, float f, hipStream_t st);
 int launch_dkdv(const Args& a, hipStream_t st);
 int launch_dkdv_wide(const Args& a, hipStream_t st);
 
@@ -103,6 +104,30 @@ Args args_of(const R97qAttnShape* p, int32_t hq, int32_t hk) {
 int64_t q_rows(const R97qAttnShape* p) { return p->q_starts ? p->q_tokens : p->q_len; }
 int64_t kv_rows(const R97qAttnShape* p) { return p->kv_starts ? p->kv_tokens : p->kv_len; }
 
+// How the backward is cut where its grids leave compute units idle: the keys of a tile of rows, and the rows of a
+// tile of keys, over up to kMostCuts workgroups each, whose f32 sums another launch adds.
+constexpr int kMostCuts = 16;
+int cuts(int64_t have, int64_t want, int64_t steps) {
+    if (have <= 0 || have * 3 / 2 >= want) return 1;
+    int64_t n = (want + have - 1) / have;
+    if (n > steps / 2) n = steps / 2;
+    return (int)(n < 1 ? 1 : n > kMostCuts ? kMostCuts : n);
+}
+void cut_backward(Args& a) {
+    a.q_splits = a.k_splits = 1;
+    if (a.batch > 0) {
+        const int64_t tiles = a.hk * all_tiles(a.q_starts, a.q_tokens, a.lq, a.batch, a.g, 128);
+        const int64_t keys = a.hk * all_tiles(a.kv_starts, a.kv_tokens, a.lk, a.batch, 1, 128);
+        int64_t seen = mean_len(a.kv_starts, a.kv_tokens, a.lk, a.batch), seeing = mean_len(a.q_starts, a.q_tokens, a.lq, a.batch);
+        if (a.window && (int64_t)a.window + 128 < seen) seen = (int64_t)a.window + 128;
+        if (a.window && (int64_t)a.window + 128 < seeing) seeing = (int64_t)a.window + 128;
+        a.q_splits = cuts(tiles, a.d > 128 ? 256 : 512, seen / 32);
+        a.k_splits = cuts(keys, a.d > 128 ? 256 : 512, a.g * seeing / (a.d > 128 ? 32 : 64));
+    }
+    a.kv_slots = a.kv_starts ? a.hk * a.kv_tokens : (int64_t)a.batch * a.hk * a.lk;
+}
+int64_t bwd_stats(const Args& a) { return (8 * a.slots + 255) / 256 * 256; }
+
 }  // namespace
 }  // namespace attn
 }  // namespace r97q
@@ -148,7 +173,10 @@ int r97q_attn_fwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
 int64_t r97q_attn_bwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads) {
     clear_error();
     if (check_shape(shape, q_heads, kv_heads, "r97q_attn_bwd_workspace_bytes")) return -1;
-    return 8 * args_of(shape, q_heads, kv_heads).slots;
+    Args a = args_of(shape, q_heads, kv_heads);
+    cut_backward(a);
+    const int64_t row = 4 * a.d;
+    return bwd_stats(a) + (a.q_splits > 1 ? a.q_splits * a.slots * row : 0) + (a.k_splits > 1 ? 2 * a.k_splits * a.kv_slots * row : 0);
 }
 
 int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
@@ -175,6 +203,7 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
         return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
     Args a = args_of(shape, hq, hk);
+    cut_backward(a);
     if (n == 0) a.lq = 0;
     if (m == 0) a.lk = 0;
     a.q = heads_of(q, n);
@@ -188,8 +217,17 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
     a.lse = const_cast<float*>(lse);
     a.base = static_cast<float*>(workspace);
     a.delta = a.base + a.slots;
-    if (int e = launch_dq(a, (hipStream_t)stream)) return e;
-    return a.d > 128 ? launch_dkdv_wide(a, (hipStream_t)stream) : launch_dkdv(a, (hipStream_t)stream);
+    a.dq_part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + bwd_stats(a));
+    a.dk_part = a.dq_part + (a.q_splits > 1 ? a.q_splits * a.slots * a.d : 0);
+    a.dv_part = a.dk_part + a.k_splits * a.kv_slots * a.d;
+    hipStream_t st = (hipStream_t)stream;
+    if (int e = launch_dq(a, st)) return e;
+    if (a.q_splits > 1)
+        if (int e = launch_sum(a, a.dq, a.dq_part, a.q_splits, false, a.scale, st)) return e;
+    if (int e = a.d > 128 ? launch_dkdv_wide(a, st) : launch_dkdv(a, st)) return e;
+    if (a.k_splits == 1) return R97Q_OK;
+    if (int e = launch_sum(a, a.dk, a.dk_part, a.k_splits, true, a.scale, st)) return e;
+    return launch_sum(a, a.dv, a.dv_part, a.k_splits, true, 1.0f, st);
 }
 
 }  // extern "C"

@@ -19,17 +19,19 @@ namespace {
 
 // ---------------------------------------------------------------- dQ (and D): 32 NW rows a workgroup
 // The waves walk the keys together, 32 at a time. Step j of a wave: dO V_j^T beside the exponentials of the scores j,
-// the scores j + 1 beside dS_j, then dQ += dS_j K_j; at its top the values j and keys j + 1 have landed, and the
-// slots of the values j - 1 and the keys j - 1 are free for the next loads. Every product's LDS operand is read
-// kAhead products before it.
+// the scores j + 1 beside dS_j, then dQ += dS_j K_j. At its top the values up to j + 1 and the keys up to j + 2 have
+// landed, and the slots of the values j - 1 and the keys j - 1 are free for the next loads. Every product's LDS operand
+// is read kAhead products before it, the first ones of step j + 1 in step j.
 template <int D, int NW, int PER>
 __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
     using T = Tile<D>;
     using F = Frags<D>;
     constexpr int KT = 32, TB = KT * T::RB, n = D / 16;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[5 * TB];  // keys' three slots, then the values' two
+    constexpr bool ACC = false;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[7 * TB];  // keys' four slots, then the values' three
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
-    const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, tiles = gridDim.x / nb;
+    const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, part = blockIdx.x / nb;
+    const int tiles = gridDim.x / (nb * a.q_splits), split = part % a.q_splits;
     const Seq s = sequence(a, bh / a.hk);
     const int rows = s.lq * a.g;
     const float sl = back_scale(a), out_of_sight = sl > 0.0f ? -INFINITY : INFINITY;
@@ -38,23 +40,30 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
     const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
     const Loader<D, KT, 64 * NW> kl(kts, a.d, tid), vl(vts, a.d, tid);
     const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + F::col0(lane);
-    for (int64_t tile = tiles - 1 - (int)(blockIdx.x / nb); tile * 32 * NW < rows; tile += tiles) {
+    for (int64_t tile = tiles - 1 - part / a.q_splits; tile * 32 * NW < rows; tile += tiles) {
         const int w0 = (int)tile * 32 * NW, r0 = w0 + 32 * wave, r = r0 + col;
         const int rr = r < rows ? r : rows - 1, tok = rr / a.g, head = hk * a.g + (rr - tok * a.g);
         const int wend = w0 + 32 * NW - 1 < rows ? w0 + 32 * NW - 1 : rows - 1;
         const Keys all = keys_of(a, s, w0 / a.g, wend / a.g);
         const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
         const Keys own = keys_of(a, s, (r0 < rows ? r0 : rows - 1) / a.g, rend / a.g);
-        const int lo = all.lo / KT * KT, hi = all.hi, last2 = 2 * a.d;
+        int lo = all.lo / KT * KT, hi = all.hi;
+        if (a.q_splits > 1 && lo < hi) {  // this range's tiles
+            const int nt = (hi - lo + KT - 1) / KT, from = (int)((int64_t)nt * split / a.q_splits), to = (int)((int64_t)nt * (split + 1) / a.q_splits);
+            hi = to * KT < hi - lo ? lo + to * KT : hi;
+            lo += from * KT;
+        }
         Rows kr(kb, kts, lo, hi, a.d), vr(vb, vts, lo, hi, a.d);
         if (lo < hi) {
             kl.load(kr, mine);
-            kr.step(KT * kts, last2);
+            kr.step(KT);
         }
         int d = fresh(a.d);
         bf16x8 q[n], go[n];
         load_row<D>(q_at(a.q, a, s, head) + 2 * (tok * a.q.ts), r < rows, d, lane, q);
         load_row<D>(q_at(a.d_o, a, s, head) + 2 * (tok * a.d_o.ts), r < rows, d, lane, go);
+        settle<ACC>(q);
+        settle<false>(go);
         const uint8_t* op = q_at(a.o, a, s, head) + (a.o.f32 ? 4 : 2) * (tok * a.o.ts);
         float delta = 0.0f;
 #pragma unroll
@@ -75,9 +84,9 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
         delta = pair_sum(delta);
         const int64_t st = stat_at(a, s, head, tok);
         const float lse = a.lse[st], base = lse == -INFINITY ? 0.0f : lse * kLog2e;
-        if (r < rows && h == 0) {
+        if (r < rows && h == 0 && split == 0) {
             a.base[st] = base;
-            a.delta[st] = delta;
+            a.delta[st] = -delta;
         }
         const int first = a.window ? (int)clamp64((int64_t)tok + s.off - a.window + 1, 0, s.lk) : 0;
         const int last = a.causal && tok + s.off < s.lk - 1 ? tok + s.off : s.lk - 1;
@@ -87,79 +96,83 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
         for (int i = 0; i < D / 32; ++i) dq[i] = (f32x16){};
         if (lo < hi) {
             const int nt = (hi - lo + KT - 1) / KT;
+            auto load_k = [&](uint32_t to) {
+                kl.load(kr, mine + to);
+                kr.step(KT);
+            };
+            auto load_v = [&](uint32_t to) {
+                vl.load(vr, mine + 4 * TB + to);
+                vr.step(KT);
+            };
+            load_k(TB);
+            load_v(0);
+            load_k(2 * TB);
+            load_v(TB);
             landed();
             __syncthreads();
-            kl.load(kr, mine + TB);
-            kr.step(KT * kts, last2);
-            vl.load(vr, mine + 3 * TB);
-            vr.step(KT * vts, last2);
             f32x16 x0 = {}, x1 = {};
             auto product = [&](f32x16& x, uint32_t from) {
-                x = (f32x16){};
                 bf16x8 f[kAhead];
                 steps<kAhead>([&](auto i) { f[i] = F::template rows<0, i>(from); });
                 steps<n>([&](auto i) {
                     const bf16x8 now = f[i % kAhead];
                     if constexpr (i + kAhead < n) f[i % kAhead] = F::template rows<0, i + kAhead>(from);
-                    x = mfma(now, q[i], x);
+                    product_of<ACC, i == 0>(now, q[i], x);
                 });
+                if constexpr (ACC) asm volatile("s_nop 15" : "+v"(x));
             };
             product(x0, rat);
-            uint32_t k_now = 0, k_next = TB, k_free = 2 * TB, v_now = 3 * TB, v_free = 4 * TB;
+            bf16x8 f[kAhead];
+            steps<kAhead>([&](auto i) { f[i] = F::template rows<0, i>(rat + 4 * TB); });
+            uint32_t k0 = 0, k1 = TB, k2 = 2 * TB, k3 = 3 * TB, v0 = 0, v1 = TB, v2 = 2 * TB;  // slots of tiles j, j + 1, ..
             auto step = [&](f32x16& x, f32x16& next, int j) {
                 landed();
                 __syncthreads();
                 const int j0 = lo + j * KT;
                 if (j0 < own.all_lo || j0 + KT > own.all_hi) {
+                    asm volatile("");  // a branch: most tiles need no mask
                     const uint32_t from = (uint32_t)(j0 + 4 * h - first);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[e] = from + (uint32_t)(8 * (e >> 2) + (e & 3)) < many ? x[e] : out_of_sight;
                 }
                 f32x16 y = {};
-                next = (f32x16){};
                 u32x4 ds[2];
-                bf16x8 f[kAhead];
-                const uint32_t vat = rat + v_now, kat = rat + k_next, dat = cat + k_now;
-                // operand of product i: V rows, next K rows, K columns
+                const uint32_t vat = rat + 4 * TB + v0, kat = rat + k1, dat = cat + k0, next_vat = rat + 4 * TB + v1;
+                // operand of product i: V rows, next K rows, K columns, the next step's V rows
                 auto frag = [&](auto i) {
                     if constexpr (i < n) return F::template rows<0, i>(vat);
+                    else if constexpr (i >= 3 * n) return F::template rows<0, i - 3 * n>(next_vat);
                     else if constexpr (i < 2 * n) return F::template rows<0, i - n>(kat);
                     else return F::template cols<16 * ((i - 2 * n) / (D / 32)), (i - 2 * n) % (D / 32)>(dat);
                 };
-                steps<kAhead>([&](auto i) { f[i] = frag(i); });
-                kl.load(kr, mine + k_free);
-                vl.load(vr, mine + v_free);
                 steps<3 * n>([&](auto i) {
                     pin();
                     const bf16x8 now = f[i % kAhead];
-                    if constexpr (i + kAhead < 3 * n) f[i % kAhead] = frag(std::integral_constant<int, i + kAhead>{});
+                    f[i % kAhead] = frag(std::integral_constant<int, i + kAhead>{});
+                    if constexpr (i == 0) load_k(k3);
+                    if constexpr (i == 1) load_v(v2);
                     if constexpr (i < n) {
                         y = mfma(now, go[i], y);
-#pragma unroll
-                        for (int e = 16 * i / n; e < 16 * (i + 1) / n; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] * sl - base);
                     } else if constexpr (i < 2 * n) {
-                        next = mfma(now, q[i - n], next);
-                        // two products later the last one of y is through
-                        constexpr int c = i - n - 2, m = n - 2;
-                        if constexpr (c >= 0) {
-#pragma unroll
-                            for (int e = 2 * (8 * c / m); e < 2 * (8 * (c + 1) / m); e += 2) {
-                                x[e] *= y[e] - delta;
-                                x[e + 1] *= y[e + 1] - delta;
-                                pack_two(x, e, ds);
-                            }
-                        }
+                        product_of<ACC, i == n>(now, q[i - n], next);
                     } else {
                         constexpr int c = (i - 2 * n) / (D / 32), m = (i - 2 * n) % (D / 32);
-                        dq[m] = mfma(now, as_bf16x8(ds[c]), dq[m]);
+                        add_product<ACC>(now, as_bf16x8(ds[c]), dq[m]);
+                    }
+                    // vector work, spread: the exponentials, and from two products after y's last one dS
+#pragma unroll
+                    for (int e = pair_from(i, 0, n); e < pair_from(i + 1, 0, n); ++e) x[e] = __builtin_amdgcn_exp2f(x[e] * sl - base);
+#pragma unroll
+                    for (int e = pair_from(i, n + 2, n - 3 + D / 32); e < pair_from(i + 1, n + 2, n - 3 + D / 32); e += 2) {
+                        x[e] *= y[e] - delta;
+                        x[e + 1] *= y[e + 1] - delta;
+                        pack_two(x, e, ds);
                     }
                 });
                 pin();
-                kr.step(KT * kts, last2);
-                vr.step(KT * vts, last2);
-                const uint32_t k = k_now, v = v_now;
-                k_now = k_next, k_next = k_free, k_free = k;
-                v_now = v_free, v_free = v;
+                const uint32_t k = k0, v = v0;
+                k0 = k1, k1 = k2, k2 = k3, k3 = k;
+                v0 = v1, v1 = v2, v2 = v;
             };
             for (int j = 0; j < nt; j += 2) {
                 step(x0, x1, j);
@@ -167,8 +180,16 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
             }
             landed();
         }
+        settled<ACC>(dq);
         d = fresh(a.d);
         const int hs = fresh_lane(h);
+        if (a.q_splits > 1) {
+            uint8_t* out = reinterpret_cast<uint8_t*>(a.dq_part + (split * a.slots + st) * d);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) store_block(out, true, r < rows, 32 * i, d, hs, dq[i], 1.0f);
+            __syncthreads();
+            continue;
+        }
         uint8_t* out = q_at(a.dq, a, s, head) + (a.dq.f32 ? 4 : 2) * (tok * a.dq.ts);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) store_block(out, a.dq.f32, r < rows, 32 * i, d, hs, dq[i], a.scale);
@@ -176,9 +197,33 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
     }
 }
 
+// ---------------------------------------------------------------- partial sums added
+// grid (batch * heads, tokens): a row's partial sums in order, times f, to the output. keys: rows of dk or dv.
+__global__ __launch_bounds__(256) void attn_sum_kernel(Args a, Heads out, const float* part, int splits, bool keys, float f) {
+    const int heads = keys ? a.hk : a.hq, head = blockIdx.x % heads;
+    const Seq s = sequence(a, blockIdx.x / heads);
+    const int per = a.d / 4, rows = 256 / per, r = threadIdx.x / per, c = 4 * (threadIdx.x % per);
+    const int cover = !keys ? s.lq : a.kv_starts ? s.lk : a.lk;
+    const int64_t slots = keys ? a.kv_slots : a.slots;
+    if (r >= rows) return;
+    for (int64_t t = (int64_t)blockIdx.y * rows + r; t < cover; t += (int64_t)gridDim.y * rows) {
+        const int64_t at = (keys ? kv_slot(a, s, head, (int)t) : stat_at(a, s, head, (int)t)) * a.d + c;
+        float4 v = *reinterpret_cast<const float4*>(part + at);
+        for (int i = 1; i < splits; ++i) {
+            const float4 u = *reinterpret_cast<const float4*>(part + i * slots * a.d + at);
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        uint8_t* row = (keys ? kv_at(out, a, s, head) : q_at(out, a, s, head)) + (out.f32 ? 4 : 2) * (t * out.ts);
+        if (out.f32)
+            *reinterpret_cast<float4*>(row + 4 * c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+        else
+            *reinterpret_cast<uint2*>(row + 2 * c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
+    }
+}
+
 template <int D, int PER>
 int run(const Args& a, hipStream_t st) {
-    const int64_t nb = (int64_t)a.batch * a.hk, most = 0x7FFFFFFF / nb;
+    const int64_t nb = (int64_t)a.batch * a.hk * a.q_splits, most = 0x7FFFFFFF / nb;
     int64_t tiles = ((int64_t)a.lq * a.g + 127) / 128;
     if (tiles > most) tiles = most;
     if (tiles == 0) return R97Q_OK;
@@ -187,6 +232,14 @@ int run(const Args& a, hipStream_t st) {
 }
 
 }  // namespace
+
+int launch_sum(const Args& a, const Heads& out, const float* part, int splits, bool keys, float f, hipStream_t st) {
+    const int64_t tokens = keys ? a.lk : a.lq, rows = 256 / (a.d / 4), blocks = (tokens + rows - 1) / rows;
+    if (blocks == 0) return R97Q_OK;
+    hipLaunchKernelGGL(attn_sum_kernel, dim3((unsigned)(a.batch * (keys ? a.hk : a.hq)), (unsigned)(blocks < 65535 ? blocks : 65535)),
+                       dim3(256), 0, st, a, out, part, splits, keys, f);
+    return launch_status("attn_sum_kernel");
+}
 
 int launch_dq(const Args& a, hipStream_t st) { return a.d <= 64 ? run<64, 2>(a, st) : a.d <= 128 ? run<128, 2>(a, st) : run<256, 1>(a, st); }
 

@@ -156,16 +156,16 @@ __device__ __forceinline__ void finish(const Args& a, const Seq& s, const Row& r
 // ---------------------------------------------------------------- tiles of 32 NW rows
 // A workgroup's NW waves take 32 rows each of one key head's rows and walk the keys together, KT at a time, from
 // LDS. The products of the next tile's scores are issued beside this tile's exponentials; one barrier a tile:
-// at the top of step j the keys of tile j + 1 and the values of tile j have landed and both of tile j - 1's
-// slots are free for the loads of tiles j + 2 and j + 1.
+// at the top of step j the keys of tile j + 1 and the values of tile j have landed, the next ones of both are on
+// their way, and the slots of the keys j and the values j - 1 are free for the loads after those.
 template <int D, int KT, int NW, int PER>
 __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     using T = Tile<D>;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * KT * T::RB];
-    constexpr int TB = KT * T::RB;  // keys' two slots, then the values'
+    constexpr int TB = KT * T::RB;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[6 * TB];  // keys' three slots, then the values'
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
-    const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, split = blockIdx.y;
-    const int tiles = gridDim.x / nb;
+    const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, part = blockIdx.x / nb;
+    const int tiles = gridDim.x / (nb * a.splits), split = part % a.splits;
     const Seq s = sequence(a, bh / a.hk);
     const int rows = s.lq * a.g;
     const float sl = score_scale(a);
@@ -173,14 +173,15 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     const uint8_t* vb = kv_at(a.v, a, s, hk);
     const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
     const Loader<D, KT, 64 * NW> kl(kts, a.d, tid), vl(vts, a.d, tid);
-    const uint32_t at = lds_at(lds), mine = at + 1024 * wave;
+    const uint32_t mine = lds_at(lds) + 1024 * wave;
     // the last tiles first: under a causal mask they have the most keys
-    for (int64_t tile = tiles - 1 - (int)(blockIdx.x / nb); tile * 32 * NW < rows; tile += tiles) {
+    for (int64_t tile = tiles - 1 - part / a.splits; tile * 32 * NW < rows; tile += tiles) {
         const int w0 = (int)tile * 32 * NW, r0 = w0 + 32 * wave;
         const Row row(a, hk, r0 + col, rows);
         bf16x8 q[D / 16];
         load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
         turn_sign<D>(a, q);
+        settle<false>(q);
         const int wend = w0 + 32 * NW - 1 < rows ? w0 + 32 * NW - 1 : rows - 1;
         const Keys all = keys_of(a, s, w0 / a.g, wend / a.g);
         const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
@@ -201,36 +202,45 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
             const int end = own.hi < hi ? own.hi : hi;
             // tiles this wave looks at: [n0, n1) of n
             const int n = (hi - lo + KT - 1) / KT, n0 = own.lo > lo ? (own.lo - lo) / KT : 0, n1 = end > lo ? (end - lo + KT - 1) / KT : 0;
-            kl.load(kr, mine);
-            kr.step(KT * kts, 2 * a.d);
-            landed();
+            constexpr int kTile = 2 * Loader<D, KT, 64 * NW>::N;  // loads a thread of a tile's keys and values
+            auto load_k = [&](uint32_t to) {
+                kl.load(kr, mine + to);
+                kr.step(KT);
+            };
+            auto load_v = [&](uint32_t to) {
+                vl.load(vr, mine + 3 * TB + to);
+                vr.step(KT);
+            };
+            load_k(0);
+            load_k(TB);
+            load_v(0);
+            load_k(2 * TB);
+            load_v(TB);
+            landed<2 * kTile>();
             __syncthreads();
-            kl.load(kr, mine + TB);
-            kr.step(KT * kts, 2 * a.d);
-            vl.load(vr, mine + 2 * TB);
-            vr.step(KT * vts, 2 * a.d);
             f32x16 x0[KT / 32], x1[KT / 32];
             scores<D, KT>(lds, q, lane, x0);
-            auto step = [&](f32x16 (&x)[KT / 32], f32x16 (&next)[KT / 32], int j, int slot) {
-                landed();
+            uint32_t now = 0, next = TB, after = 2 * TB;  // slots of tiles j, j + 1, j + 2
+            auto step = [&](f32x16 (&x)[KT / 32], f32x16 (&xn)[KT / 32], int j) {
+                landed<kTile>();
                 __syncthreads();
-                kl.load(kr, mine + slot * TB);
-                kr.step(KT * kts, 2 * a.d);
-                vl.load(vr, mine + (3 - slot) * TB);
-                vr.step(KT * vts, 2 * a.d);
+                load_k(now);
+                load_v(after);
                 if (j >= n0 && j < n1) {
                     const int j0 = lo + j * KT;
                     if (j0 < own.all_lo || j0 + KT > own.all_hi) mask<KT>(x, first - j0, last - j0, h);
-                    scores<D, KT>(lds + (1 - slot) * TB, q, lane, next);
+                    scores<D, KT>(lds + next, q, lane, xn);
                     run.rise(tile_max<KT>(x) * sl);
-                    absorb<D, KT>(lds + (2 + slot) * TB, x, sl, lane, run);
+                    absorb<D, KT>(lds + 3 * TB + now, x, sl, lane, run);
                 } else if (j + 1 == n0) {
-                    scores<D, KT>(lds + (1 - slot) * TB, q, lane, next);
+                    scores<D, KT>(lds + next, q, lane, xn);
                 }
+                const uint32_t free = now;
+                now = next, next = after, after = free;
             };
             for (int j = 0; j < n; j += 2) {
-                step(x0, x1, j, 0);
-                if (j + 1 < n) step(x1, x0, j + 1, 1);
+                step(x0, x1, j);
+                if (j + 1 < n) step(x1, x0, j + 1);
             }
             landed();
         }
@@ -288,20 +298,21 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
             bf16x8 q[D / 16];
             load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
             turn_sign<D>(a, q);
+            settle<false>(q);
             landed<Loader<D, KT, 64>::N>();  // the queries have been waited for: no more than the values are left
             for (; j0 < hi; j0 += KT * NW) {
                 f32x16 x[1];
                 scores<D, KT>(own, q, lane, x);
                 // the keys are in registers: their tile is free
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                kr.step(NW * KT * kts, 2 * a.d);
+                kr.step(NW * KT);
                 kl.load(kr, at);
                 if (j0 < keys.all_lo || j0 + KT > keys.all_hi) mask<KT>(x, first - j0, last - j0, h);
                 run.rise(tile_max<KT>(x) * sl);
                 landed<Loader<D, KT, 64>::N>();  // the values; the next keys may be on their way
                 absorb<D, KT>(own + TB, x, sl, lane, run);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                vr.step(NW * KT * vts, 2 * a.d);
+                vr.step(NW * KT);
                 vl.load(vr, at + TB);
                 landed<Loader<D, KT, 64>::N>();
             }
@@ -362,56 +373,64 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------- the ranges' results joined
-// grid (batch * q heads, tokens): a workgroup a row. Each range's sums are relative to its own m.
-__global__ __launch_bounds__(256) void attn_join_kernel(Args a) {
-    __shared__ float weight[kMostSplits];
-    __shared__ float part[4];
+// grid (batch * q heads, tokens). Each range's sums are relative to its own m. A row of d values takes d / 4 threads,
+// rounded up to a power of two; `groups` of them share a row's ranges where there are many (a lone token's), and
+// their sums are added in order.
+__global__ __launch_bounds__(256) void attn_join_kernel(Args a, int lanes, int groups) {
     __shared__ __attribute__((aligned(16))) float4 acc[256];
-    const int tid = threadIdx.x, head = blockIdx.x % a.hq;
+    __shared__ float2 stat[256];
+    const int tid = threadIdx.x, head = blockIdx.x % a.hq, per = lanes * groups, rows = 256 / per;
     const Seq s = sequence(a, blockIdx.x / a.hq);
-    const int per = a.d / 4, lanes = per <= 16 ? 16 : per <= 32 ? 32 : 64, groups = 256 / lanes;  // threads a range's row, ranges at once
-    for (int tok = blockIdx.y; tok < s.lq; tok += gridDim.y) {
-        const int64_t at = stat_at(a, s, head, tok);
-        const float2 st = tid < a.splits ? a.stats[tid * a.slots + at] : make_float2(-INFINITY, 0.0f);
-        float top = st.x;
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        if ((tid & 63) == 0) part[tid >> 6] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-        const float w = st.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
-        weight[tid] = w;
-        float l = st.y * w;
-        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-        __syncthreads();
-        if ((tid & 63) == 0) part[tid >> 6] = l;
-        __syncthreads();
-        l = (part[0] + part[1]) + (part[2] + part[3]);
-        const int d0 = 4 * (tid % lanes), g = tid / lanes;
+    const int lane = tid % lanes, group = tid % per / lanes, d0 = 4 * lane;
+    for (int64_t t0 = (int64_t)blockIdx.y * rows; t0 < s.lq; t0 += (int64_t)gridDim.y * rows) {
+        const int64_t tok = t0 + tid / per;
+        const bool on = tok < s.lq;
+        const int64_t at = on ? stat_at(a, s, head, (int)tok) : 0;
+        float top = -INFINITY, l = 0.0f;
         float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (d0 < a.d) {
-            for (int i = g; i < a.splits; i += groups) {
-                const float f = weight[i];
-                if (f == 0.0f) continue;
-                const float4 u = *reinterpret_cast<const float4*>(a.part + (i * a.slots + at) * a.d + d0);
+        if (on) {
+#pragma unroll 8
+            for (int i = group; i < a.splits; i += groups) top = fmaxf(top, a.stats[i * a.slots + at].x);
+#pragma unroll 8
+            for (int i = group; i < a.splits; i += groups) {
+                const float2 st = a.stats[i * a.slots + at];
+                // an empty range wrote no sums: its place may hold anything
+                const float f = st.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
+                float4 u = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (d0 < a.d && st.x != -INFINITY) u = *reinterpret_cast<const float4*>(a.part + (i * a.slots + at) * a.d + d0);
+                l += st.y * f;
                 v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
             }
         }
-        acc[tid] = v;
-        __syncthreads();
-        if (tid < lanes && d0 < a.d) {
-            for (int i = 1; i < groups; ++i) {
-                const float4 u = acc[tid + i * lanes];
-                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        if (groups > 1) {
+            acc[tid] = v;
+            stat[tid] = make_float2(top, l);
+            __syncthreads();
+            if (group == 0) {
+                float most = top;
+                for (int i = 1; i < groups; ++i) most = fmaxf(most, stat[tid + i * lanes].x);
+                l = 0.0f;
+                v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int i = 0; i < groups; ++i) {
+                    const float2 st = stat[tid + i * lanes];
+                    if (st.x == -INFINITY) continue;
+                    const float f = __builtin_amdgcn_exp2f(st.x - most);
+                    const float4 u = acc[tid + i * lanes];
+                    l += st.y * f;
+                    v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
+                }
+                top = most;
             }
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            uint8_t* out = q_at(a.o, a, s, head) + (a.o.f32 ? 4 : 2) * (tok * a.o.ts);
-            if (a.o.f32)
-                *reinterpret_cast<float4*>(out + 4 * d0) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-            else
-                *reinterpret_cast<uint2*>(out + 2 * d0) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
-            if (tid == 0 && a.lse) a.lse[at] = log_sum(top, l);
+            __syncthreads();
         }
-        __syncthreads();
+        if (!on || group || d0 >= a.d) continue;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint8_t* out = q_at(a.o, a, s, head) + (a.o.f32 ? 4 : 2) * (tok * a.o.ts);
+        if (a.o.f32)
+            *reinterpret_cast<float4*>(out + 4 * d0) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        else
+            *reinterpret_cast<uint2*>(out + 2 * d0) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+        if (lane == 0 && a.lse) a.lse[at] = log_sum(top, l);
     }
 }
 
@@ -423,17 +442,17 @@ struct Plan {
 };
 Plan plan_of(const Args& a) {
     Plan p = {};
-    const int64_t rows = (int64_t)a.lq * a.g, heads = (int64_t)a.batch * a.hk;
+    const int64_t rows = (int64_t)a.lq * a.g;
     p.few = rows <= 32;
     p.waves = 4;
     const int tile = p.few ? 32 : 32 * p.waves;
     p.tiles = (rows + tile - 1) / tile;
     p.splits = 1;
     // the keys a tile's rows may see
-    int64_t most = a.lk;
+    int64_t most = mean_len(a.kv_starts, a.kv_tokens, a.lk, a.batch);
     if (a.window && (int64_t)a.window + tile / a.g + 1 < most) most = (int64_t)a.window + tile / a.g + 1;
-    const int64_t unit = p.few ? 128 : 256, want = a.d > 128 ? 256 : 512, have = p.tiles * heads;
-    if (have < want && most > unit) {
+    const int64_t unit = p.few ? 128 : 256, want = a.d > 128 ? 256 : 512, have = a.hk * all_tiles(a.q_starts, a.q_tokens, a.lq, a.batch, a.g, tile);
+    if (have > 0 && have * 3 / 2 < want && most > unit) {
         int64_t n = (want + have - 1) / have;
         if (n > (most + unit - 1) / unit) n = (most + unit - 1) / unit;
         if (n > kMostSplits) n = kMostSplits;
@@ -446,9 +465,9 @@ Plan plan_of(const Args& a) {
 
 template <int D, int KT, int NW, int PER>
 int run_tiles(const Args& a, const Plan& p, hipStream_t st) {
-    const int64_t nb = (int64_t)a.batch * a.hk, most = 0x7FFFFFFF / nb;
+    const int64_t nb = (int64_t)a.batch * a.hk * p.splits, most = 0x7FFFFFFF / nb;
     const int64_t tiles = p.tiles < most ? p.tiles : most;
-    hipLaunchKernelGGL((attn_fwd_kernel<D, KT, NW, PER>), dim3((unsigned)(tiles * nb), p.splits), dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL((attn_fwd_kernel<D, KT, NW, PER>), dim3((unsigned)(tiles * nb)), dim3(64 * NW), 0, st, a);
     return launch_status("attn_fwd_kernel");
 }
 template <int D, int NW>
@@ -478,7 +497,11 @@ int launch_fwd(Args a, void* workspace, hipStream_t st) {
             : a.d <= 128 ? run_tiles<128, 32, 4, 2>(a, p, st)
                          : run_tiles<256, 32, 4, 1>(a, p, st);
     if (e || p.splits == 1) return e;
-    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)(a.batch * a.hq), (unsigned)(a.lq < 65535 ? a.lq : 65535)), dim3(256), 0, st, a);
+    const int lanes = a.d <= 32 ? 8 : a.d <= 64 ? 16 : a.d <= 128 ? 32 : 64;
+    int groups = 1;
+    while (groups * lanes < 256 && groups * 4 < p.splits) groups *= 2;
+    const int rows = 256 / (lanes * groups), blocks = (a.lq + rows - 1) / rows;
+    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)(a.batch * a.hq), (unsigned)(blocks < 65535 ? blocks : 65535)), dim3(256), 0, st, a, lanes, groups);
     return launch_status("attn_join_kernel");
 }
 
