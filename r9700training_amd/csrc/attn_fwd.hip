@@ -155,14 +155,16 @@ __device__ __forceinline__ void finish(const Args& a, const Seq& s, const Row& r
 
 // ---------------------------------------------------------------- tiles of 32 NW rows
 // A workgroup's NW waves take 32 rows each of one key head's rows and walk the keys together, KT at a time, from
-// LDS. The products of the next tile's scores are issued beside this tile's exponentials; one barrier a tile:
-// at the top of step j the keys of tile j + 1 and the values of tile j have landed, the next ones of both are on
-// their way, and the slots of the keys j and the values j - 1 are free for the loads after those.
+// LDS. Step j of a wave: the products of the scores j + 1, then those of P_j V_j; beside them, spread evenly, the
+// maximum of the scores j and their exponentials, each half a k step ahead of its use. At the step's top the keys
+// of tile j + 1 and the values of tile j have landed, and both of tile j - 1's slots are free for the loads of tiles
+// j + 2 and j + 1. Every LDS operand is read kAhead products before its use.
 template <int D, int KT, int NW, int PER>
 __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     using T = Tile<D>;
-    constexpr int TB = KT * T::RB;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[6 * TB];  // keys' three slots, then the values'
+    using F = Frags<D>;
+    constexpr int TB = KT * T::RB, SUBS = KT / 32, n = D / 16;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB];  // keys' two slots, then the values'
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
     const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, part = blockIdx.x / nb;
     const int tiles = gridDim.x / (nb * a.splits), split = part % a.splits;
@@ -173,15 +175,11 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     const uint8_t* vb = kv_at(a.v, a, s, hk);
     const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
     const Loader<D, KT, 64 * NW> kl(kts, a.d, tid), vl(vts, a.d, tid);
-    const uint32_t mine = lds_at(lds) + 1024 * wave;
+    const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + 2 * TB + F::col0(lane);
     // the last tiles first: under a causal mask they have the most keys
     for (int64_t tile = tiles - 1 - part / a.splits; tile * 32 * NW < rows; tile += tiles) {
         const int w0 = (int)tile * 32 * NW, r0 = w0 + 32 * wave;
         const Row row(a, hk, r0 + col, rows);
-        bf16x8 q[D / 16];
-        load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
-        turn_sign<D>(a, q);
-        settle<false>(q);
         const int wend = w0 + 32 * NW - 1 < rows ? w0 + 32 * NW - 1 : rows - 1;
         const Keys all = keys_of(a, s, w0 / a.g, wend / a.g);
         const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
@@ -192,55 +190,111 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
             lo = (int)clamp64((int64_t)lo + (int64_t)split * a.chunk, lo, hi);
             if (split < a.splits - 1 && hi - lo > a.chunk) hi = lo + a.chunk;  // the last range takes what is left
         }
+        Rows kr(kb, kts, lo, hi, a.d), vr(vb, vts, lo, hi, a.d);
+        auto load_k = [&](int slot) {
+            kl.load(kr, mine + slot * TB);
+            kr.step(KT);
+        };
+        auto load_v = [&](int slot) {
+            vl.load(vr, mine + (2 + slot) * TB);
+            vr.step(KT);
+        };
+        if (lo < hi) {
+            load_k(0);
+            load_k(1);
+            load_v(0);
+        }
+        bf16x8 q[n];
+        load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
+        turn_sign<D>(a, q);
+        settle<false>(q);
         // the keys this lane's row sees, first and last
         const int first = a.window ? (int)clamp64((int64_t)row.tok + s.off - a.window + 1, 0, s.lk) : 0;
         const int last = a.causal && row.tok + s.off < s.lk - 1 ? row.tok + s.off : s.lk - 1;
         Running<D> run;
         run.clear();
         if (lo < hi) {
-            Rows kr(kb, kts, lo, hi, a.d), vr(vb, vts, lo, hi, a.d);
             const int end = own.hi < hi ? own.hi : hi;
-            // tiles this wave looks at: [n0, n1) of n
-            const int n = (hi - lo + KT - 1) / KT, n0 = own.lo > lo ? (own.lo - lo) / KT : 0, n1 = end > lo ? (end - lo + KT - 1) / KT : 0;
-            constexpr int kTile = 2 * Loader<D, KT, 64 * NW>::N;  // loads a thread of a tile's keys and values
-            auto load_k = [&](uint32_t to) {
-                kl.load(kr, mine + to);
-                kr.step(KT);
-            };
-            auto load_v = [&](uint32_t to) {
-                vl.load(vr, mine + 3 * TB + to);
-                vr.step(KT);
-            };
-            load_k(0);
-            load_k(TB);
-            load_v(0);
-            load_k(2 * TB);
-            load_v(TB);
-            landed<2 * kTile>();
+            // tiles this wave looks at: [n0, n1) of nt
+            const int nt = (hi - lo + KT - 1) / KT, n0 = own.lo > lo ? (own.lo - lo) / KT : 0, n1 = end > lo ? (end - lo + KT - 1) / KT : 0;
+            landed();
             __syncthreads();
-            f32x16 x0[KT / 32], x1[KT / 32];
-            scores<D, KT>(lds, q, lane, x0);
-            uint32_t now = 0, next = TB, after = 2 * TB;  // slots of tiles j, j + 1, j + 2
-            auto step = [&](f32x16 (&x)[KT / 32], f32x16 (&xn)[KT / 32], int j) {
-                landed<kTile>();
-                __syncthreads();
-                load_k(now);
-                load_v(after);
+            f32x16 x0[SUBS], x1[SUBS];
+            constexpr int NA = SUBS * n, NB = 2 * SUBS * (D / 32);
+            auto only_scores = [&](f32x16 (&x)[SUBS], uint32_t from) {
+                bf16x8 f[kAhead];
+                steps<kAhead>([&](auto i) { f[i] = F::template rows<32 * (i % SUBS), i / SUBS>(from); });
+                steps<NA>([&](auto i) {
+                    const bf16x8 now = f[i % kAhead];
+                    if constexpr (i + kAhead < NA) f[i % kAhead] = F::template rows<32 * ((i + kAhead) % SUBS), (i + kAhead) / SUBS>(from);
+                    x[i % SUBS] = mfma(now, q[i / SUBS], i < SUBS ? (f32x16){} : x[i % SUBS]);
+                });
+            };
+            only_scores(x0, rat);
+            auto step = [&](f32x16 (&x)[SUBS], f32x16 (&xn)[SUBS], int j, auto slot_) {
+                constexpr int slot = slot_;
+                if (j > 0) {  // the first tiles' loads are the ones above
+                    landed();
+                    __syncthreads();
+                    load_k(slot);
+                    load_v(1 - slot);
+                } else {
+                    __syncthreads();
+                    load_k(slot);
+                    load_v(1 - slot);
+                }
                 if (j >= n0 && j < n1) {
                     const int j0 = lo + j * KT;
                     if (j0 < own.all_lo || j0 + KT > own.all_hi) mask<KT>(x, first - j0, last - j0, h);
-                    scores<D, KT>(lds + next, q, lane, xn);
-                    run.rise(tile_max<KT>(x) * sl);
-                    absorb<D, KT>(lds + 3 * TB + now, x, sl, lane, run);
+                    bf16x8 f[kAhead];
+                    // operand of product i: the next keys' rows, the values' columns
+                    auto frag = [&](auto i) {
+                        if constexpr (i < NA) return F::template rows<(1 - slot) * KT + 32 * (i % SUBS), i / SUBS>(rat);
+                        else return F::template cols<slot * KT + 16 * ((i - NA) / (D / 32)), (i - NA) % (D / 32)>(cat);
+                    };
+                    steps<kAhead>([&](auto i) { f[i] = frag(i); });
+                    constexpr int MX = NA / 2, EL = NA + (KT / 16 - 1) * (D / 32) - MX, pairs = KT / 4;
+                    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, base = 0.0f;
+                    u32x4 p[KT / 16];
+                    steps<NA + NB>([&](auto i) {
+                        if constexpr (i == MX) {
+                            run.rise(pair_max(fmaxf(top[0], top[1])) * sl);
+                            base = run.m == -INFINITY ? 0.0f : run.m;
+                        }
+                        pin();
+                        const bf16x8 now = f[i % kAhead];
+                        if constexpr (i + kAhead < NA + NB) f[i % kAhead] = frag(std::integral_constant<int, i + kAhead>{});
+                        if constexpr (i < NA) {
+                            xn[i % SUBS] = mfma(now, q[i / SUBS], i < SUBS ? (f32x16){} : xn[i % SUBS]);
+                        } else {
+                            constexpr int c = (i - NA) / (D / 32), m = (i - NA) % (D / 32);
+                            run.o[m] = mfma(now, as_bf16x8(p[c]), run.o[m]);
+                        }
+                        if constexpr (i < MX) {
+#pragma unroll
+                            for (int e = KT / 2 * i / MX; e < KT / 2 * (i + 1) / MX; ++e) top[e & 1] = fmaxf(top[e & 1], x[e / 16][e % 16]);
+                        } else {
+#pragma unroll
+                            for (int t = pairs * (i - MX) / EL; t < (i - MX >= EL ? pairs : pairs * (i + 1 - MX) / EL); ++t) {
+                                if (i - MX >= EL) break;
+                                const int e = 2 * t, u = e / 16, w = e % 16;
+                                x[u][w] = __builtin_amdgcn_exp2f(x[u][w] * sl - base);
+                                x[u][w + 1] = __builtin_amdgcn_exp2f(x[u][w + 1] * sl - base);
+                                sum[0] += x[u][w];
+                                sum[1] += x[u][w + 1];
+                                p[e / 8][(e % 8) / 2] = pack_bf16(x[u][w], x[u][w + 1]);
+                            }
+                        }
+                    });
+                    pin();
+                    run.l += sum[0] + sum[1];
                 } else if (j + 1 == n0) {
-                    scores<D, KT>(lds + next, q, lane, xn);
+                    only_scores(xn, rat + (1 - slot) * TB);
                 }
-                const uint32_t free = now;
-                now = next, next = after, after = free;
             };
-            for (int j = 0; j < n; j += 2) {
-                step(x0, x1, j);
-                if (j + 1 < n) step(x1, x0, j + 1);
+            for (int j = 0; j < nt; j += 2) {
+                step(x0, x1, j, std::integral_constant<int, 0>{});
+                if (j + 1 < nt) step(x1, x0, j + 1, std::integral_constant<int, 1>{});
             }
             landed();
         }
@@ -494,7 +548,7 @@ int launch_fwd(Args a, void* workspace, hipStream_t st) {
         e = a.d <= 64 ? run_few<64, 4>(a, p, st) : a.d <= 128 ? run_few<128, 4>(a, p, st) : run_few<256, 4>(a, p, st);
     else
         e = a.d <= 64    ? run_tiles<64, 64, 4, 2>(a, p, st)
-            : a.d <= 128 ? run_tiles<128, 32, 4, 2>(a, p, st)
+            : a.d <= 128 ? run_tiles<128, 64, 4, 2>(a, p, st)
                          : run_tiles<256, 32, 4, 1>(a, p, st);
     if (e || p.splits == 1) return e;
     const int lanes = a.d <= 32 ? 8 : a.d <= 64 ? 16 : a.d <= 128 ? 32 : 64;
