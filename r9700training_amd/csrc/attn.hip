@@ -104,13 +104,16 @@ Args args_of(const R97qAttnShape* p, int32_t hq, int32_t hk) {
 int64_t q_rows(const R97qAttnShape* p) { return p->q_starts ? p->q_tokens : p->q_len; }
 int64_t kv_rows(const R97qAttnShape* p) { return p->kv_starts ? p->kv_tokens : p->kv_len; }
 
-// How the backward is cut where its grids leave compute units idle: the keys of a tile of rows, and the rows of a
-// tile of keys, over up to kMostCuts workgroups each, whose f32 sums another launch adds.
+// How the backward is cut where its grids leave compute units idle: a tile's steps over up to kMostCuts workgroups, whose
+// f32 sums another launch adds. Measured on 16 over 4 heads (us at 1 / 2 / 4 / 8 cuts; a cut writes and reads its sums):
+// dK and dV of 1 x 1300 tokens, heads of 128: 176 / 123 / 93 / 86; of 2 x 1300: 181 / 130 / 104 / 123; of 4 x 700:
+// 112 / 92 / 85 / 105; of 512 tokens, heads of 64: 54 / 43 / 36 / 35; so up to some 320 workgroups of at least four
+// steps. dQ of 64 rows over 4096 keys: 103 / 70 / 53 / 46, but of 1 x 1300: 175 / 178 / 188 / 214 and of 512: 80 / 84 /
+// 86 / 92; so only below half the compute units and from 512 keys a cut.
 constexpr int kMostCuts = 16;
-int cuts(int64_t have, int64_t want, int64_t steps) {
-    if (have <= 0 || have * 3 / 2 >= want) return 1;
-    int64_t n = (want + have - 1) / have;
-    if (n > steps / 2) n = steps / 2;
+int cuts(int64_t want, int64_t have, int64_t steps) {
+    int64_t n = have > 0 ? (want + have - 1) / have : 1;
+    if (n > steps) n = steps;
     return (int)(n < 1 ? 1 : n > kMostCuts ? kMostCuts : n);
 }
 void cut_backward(Args& a) {
@@ -121,8 +124,8 @@ void cut_backward(Args& a) {
         int64_t seen = mean_len(a.kv_starts, a.kv_tokens, a.lk, a.batch), seeing = mean_len(a.q_starts, a.q_tokens, a.lq, a.batch);
         if (a.window && (int64_t)a.window + 128 < seen) seen = (int64_t)a.window + 128;
         if (a.window && (int64_t)a.window + 128 < seeing) seeing = (int64_t)a.window + 128;
-        a.q_splits = cuts(tiles, a.d > 128 ? 256 : 512, seen / 32);
-        a.k_splits = cuts(keys, a.d > 128 ? 256 : 512, a.g * seeing / (a.d > 128 ? 32 : 64));
+        a.q_splits = tiles * 2 <= 256 ? cuts(256, tiles, seen / 512) : 1;
+        a.k_splits = keys * 3 / 2 < 320 ? cuts(320, keys, a.g * seeing / (a.d > 128 ? 32 : 64) / 4) : 1;
     }
     a.kv_slots = a.kv_starts ? a.hk * a.kv_tokens : (int64_t)a.batch * a.hk * a.lk;
 }

@@ -427,13 +427,14 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------- the ranges' results joined
-// grid (batch * q heads, tokens). Each range's sums are relative to its own m. A row of d values takes d / 4 threads,
-// rounded up to a power of two; `groups` of them share a row's ranges where there are many (a lone token's), and
-// their sums are added in order.
-__global__ __launch_bounds__(256) void attn_join_kernel(Args a, int lanes, int groups) {
-    __shared__ __attribute__((aligned(16))) float4 acc[256];
-    __shared__ float2 stat[256];
-    const int tid = threadIdx.x, head = blockIdx.x % a.hq, per = lanes * groups, rows = 256 / per;
+// grid (batch * q heads, tokens). Each range's sums are relative to its own m. A row of d values takes `lanes` threads
+// (d / 4, rounded up to a power of two); `groups` of them share a row's ranges, kBatch at once each, so that a row's
+// loads all go out together, and their sums are added in order. `rows` rows a workgroup.
+constexpr int kBatch = 8;
+__global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int groups, int rows) {
+    __shared__ __attribute__((aligned(16))) float4 acc[1024];
+    __shared__ float2 stat[1024];
+    const int tid = threadIdx.x, head = blockIdx.x % a.hq, per = lanes * groups;
     const Seq s = sequence(a, blockIdx.x / a.hq);
     const int lane = tid % lanes, group = tid % per / lanes, d0 = 4 * lane;
     for (int64_t t0 = (int64_t)blockIdx.y * rows; t0 < s.lq; t0 += (int64_t)gridDim.y * rows) {
@@ -442,18 +443,30 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a, int lanes, int g
         const int64_t at = on ? stat_at(a, s, head, (int)tok) : 0;
         float top = -INFINITY, l = 0.0f;
         float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (on) {
-#pragma unroll 8
-            for (int i = group; i < a.splits; i += groups) top = fmaxf(top, a.stats[i * a.slots + at].x);
-#pragma unroll 8
-            for (int i = group; i < a.splits; i += groups) {
-                const float2 st = a.stats[i * a.slots + at];
-                // an empty range wrote no sums: its place may hold anything
-                const float f = st.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
-                float4 u = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (d0 < a.d && st.x != -INFINITY) u = *reinterpret_cast<const float4*>(a.part + (i * a.slots + at) * a.d + d0);
-                l += st.y * f;
-                v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
+        for (int i0 = group; on && i0 < a.splits; i0 += kBatch * groups) {
+            float2 st[kBatch];
+            float4 u[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = i0 + k * groups < a.splits ? i0 + k * groups : i0;
+                st[k] = a.stats[i * a.slots + at];
+                u[k] = *reinterpret_cast<const float4*>(a.part + (i * a.slots + at) * a.d + (d0 < a.d ? d0 : 0));
+            }
+            float most = top;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                if (i0 + k * groups >= a.splits) st[k].x = -INFINITY;
+                most = fmaxf(most, st[k].x);
+            }
+            const float turn = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - most);
+            l *= turn, v.x *= turn, v.y *= turn, v.z *= turn, v.w *= turn;
+            top = most;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                if (st[k].x == -INFINITY) continue;  // an empty range wrote no sums: its place may hold anything
+                const float f = __builtin_amdgcn_exp2f(st[k].x - top);
+                l += st[k].y * f;
+                v.x += u[k].x * f, v.y += u[k].y * f, v.z += u[k].z * f, v.w += u[k].w * f;
             }
         }
         if (groups > 1) {
@@ -488,7 +501,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a, int lanes, int g
     }
 }
 
-// how a shape is cut: rows a workgroup, ranges of the keys
+// How a shape is cut: rows a workgroup, ranges of the keys. A range writes its sums and a second launch (some 5 us) joins
+// them, so only where compute units would be idle. Measured (us at 1 / 2 / 4 / 8 / 16 / 32 ranges): one token, 24 over 4
+// heads of 256, 32768 keys 601 / 312 / 168 / 98 / 63 / 43 (64: 39); 16 sequences of 1 .. 4096 keys, 32 over 8 heads of 128
+// 58 / 47 / 44 / 46 / 52 / 67, all of 4096 keys 45 / 49 / 49 / 50 / 54 / 72; 64 rows over 4096 keys 67 / 42 / 29 / 23 / 22 /
+// 24; but 1300 tokens, 16 over 4 heads 28 / 35 / 45 / 57, and 512 tokens 15 / 20 / 22 / 30.
 struct Plan {
     bool few;
     int waves, splits, chunk;
@@ -505,14 +522,21 @@ Plan plan_of(const Args& a) {
     // the keys a tile's rows may see
     int64_t most = mean_len(a.kv_starts, a.kv_tokens, a.lk, a.batch);
     if (a.window && (int64_t)a.window + tile / a.g + 1 < most) most = (int64_t)a.window + tile / a.g + 1;
-    const int64_t unit = p.few ? 128 : 256, want = a.d > 128 ? 256 : 512, have = a.hk * all_tiles(a.q_starts, a.q_tokens, a.lq, a.batch, a.g, tile);
-    if (have > 0 && have * 3 / 2 < want && most > unit) {
-        int64_t n = (want + have - 1) / have;
-        if (n > (most + unit - 1) / unit) n = (most + unit - 1) / unit;
-        if (n > kMostSplits) n = kMostSplits;
-        int64_t chunk = ((most + n - 1) / n + unit - 1) / unit * unit;
-        p.splits = (int)((most + chunk - 1) / chunk);
-        p.chunk = (int)chunk;
+    const int64_t have = a.hk * all_tiles(a.q_starts, a.q_tokens, a.lq, a.batch, a.g, tile);
+    int64_t n = 1, unit;
+    if (p.few) {  // lengths that differ leave workgroups idle: more of them
+        const int64_t want = !a.kv_lens && !a.kv_starts ? 192 : a.d > 128 ? 256 : 512;
+        unit = 128;
+        if (have > 0 && have * 3 / 2 < want && most > 1024) n = (want + have - 1) / have;
+    } else {
+        unit = 512;
+        if (have > 0 && have * 2 <= 256) n = (256 + have - 1) / have;
+    }
+    if (n > most / unit) n = most / unit;
+    if (n > kMostSplits) n = kMostSplits;
+    if (n > 1) {
+        p.chunk = (int)(((most + n - 1) / n + 127) / 128 * 128);
+        p.splits = (int)((most + p.chunk - 1) / p.chunk);
     }
     return p;
 }
@@ -553,9 +577,10 @@ int launch_fwd(Args a, void* workspace, hipStream_t st) {
     if (e || p.splits == 1) return e;
     const int lanes = a.d <= 32 ? 8 : a.d <= 64 ? 16 : a.d <= 128 ? 32 : 64;
     int groups = 1;
-    while (groups * lanes < 256 && groups * 4 < p.splits) groups *= 2;
-    const int rows = 256 / (lanes * groups), blocks = (a.lq + rows - 1) / rows;
-    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)(a.batch * a.hq), (unsigned)(blocks < 65535 ? blocks : 65535)), dim3(256), 0, st, a, lanes, groups);
+    while (groups * lanes < 1024 && groups * kBatch < p.splits) groups *= 2;
+    const int rows = groups * lanes < 256 ? 256 / (groups * lanes) : 1, blocks = (a.lq + rows - 1) / rows;
+    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)(a.batch * a.hq), (unsigned)(blocks < 65535 ? blocks : 65535)),
+                       dim3((unsigned)(rows * groups * lanes)), 0, st, a, lanes, groups, rows);
     return launch_status("attn_join_kernel");
 }
 
