@@ -67,6 +67,7 @@ struct Args {
     float scale;         // of the scores
     // the forward split over the keys: ranges of `chunk` keys, each one's unnormalised sums in f32 and (m, l)
     int32_t splits, chunk;
+    int32_t together;    // heads an XCD takes at a time
     int64_t slots;       // rows of one range: every query head's
     float* part;         // [splits][slots][d]
     float2* stats;       // [splits][slots]
@@ -138,6 +139,24 @@ __device__ __forceinline__ int64_t stat_at(const Args& a, const Seq& s, int h, i
     return a.q_starts ? h * a.q_tokens + s.q_base + token : ((int64_t)s.b * a.hq + h) * a.lq + token;
 }
 
+// Which key head of which sequence a workgroup of a one-dimensional grid takes, and which part of it (the first parts
+// have the most work). Workgroups go to the 8 XCDs in turn, each with its own L2: where the heads divide evenly, an XCD
+// takes `together` of its heads at a time, as many as its L2 holds the keys and values of, part by part, then the next.
+struct Place {
+    int bh, part;
+    __device__ __forceinline__ Place(int nb, int together) {
+        const int w = blockIdx.x, parts = gridDim.x / nb;
+        if (nb % 8 == 0) {
+            const int i = w / 8, group = i / (together * parts), j = i - group * together * parts;
+            const int left = nb / 8 - group * together, heads = left < together ? left : together;
+            part = j / heads;
+            bh = w % 8 + 8 * (group * together + (j - part * heads));
+        } else {
+            part = w / nb;
+            bh = w - part * nb;
+        }
+    }
+};
 // a key's row of a partial sum
 __device__ __forceinline__ int64_t kv_slot(const Args& a, const Seq& s, int hk, int key) {
     return a.kv_starts ? hk * a.kv_tokens + s.k_base + key : ((int64_t)s.b * a.hk + hk) * a.lk + key;
@@ -161,6 +180,8 @@ __device__ __forceinline__ Keys keys_of(const Args& a, const Seq& s, int t0, int
     return k;
 }
 
+// instructions stay on their side
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 __device__ __forceinline__ f32x16 mfma(bf16x8 x, bf16x8 y, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
 }
@@ -197,13 +218,17 @@ __device__ __forceinline__ void settle(bf16x8 (&f)[N]) {
             asm volatile("" : "+v"(f[i]));
     }
 }
-// the sums may be read from here on
-template <bool ACC, int N>
-__device__ __forceinline__ void settled(f32x16 (&c)[N]) {
+// the sums may be read from here on, each after its own settle_sum(): otherwise all are copied out at once, and what
+// else is held has to leave the registers
+template <bool ACC>
+__device__ __forceinline__ void settled() {
+    if constexpr (ACC) asm volatile("s_nop 15\n\ts_nop 15");
+}
+template <bool ACC>
+__device__ __forceinline__ void settle_sum(f32x16& c) {
     if constexpr (ACC) {
-        asm volatile("s_nop 15\n\ts_nop 15");
-#pragma unroll
-        for (int i = 0; i < N; ++i) asm volatile("" : "+a"(c[i]));
+        pin();
+        asm volatile("" : "+a"(c));
     }
 }
 __device__ __forceinline__ bf16x8 as_bf16x8(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
@@ -311,8 +336,6 @@ template <int N, class F>
 __device__ __forceinline__ void steps(F&& f) {
     steps_of(f, std::make_integer_sequence<int, N>{});
 }
-// instructions stay on their side
-__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 // a 32 x 32 tile's values e and e + 1 (e even) as a word of its B operands
 __device__ __forceinline__ void pack_two(const f32x16& x, int e, u32x4 (&out)[2]) { out[e >> 3][(e & 7) >> 1] = pack_bf16(x[e], x[e + 1]); }
 

@@ -98,6 +98,10 @@ Args args_of(const R97qAttnShape* p, int32_t hq, int32_t hk) {
     a.scale = p->scale;
     a.slots = p->q_starts ? hq * p->q_tokens : (int64_t)p->batch * hq * p->q_len;
     a.splits = 1;
+    // half of an XCD's 4 MiB of L2
+    const int64_t bytes = 4 * a.d * (a.batch ? mean_len(a.kv_starts, a.kv_tokens, a.lk, a.batch) : 0), most = ((int64_t)a.batch * hk + 7) / 8;
+    const int64_t fit = (2 << 20) / (bytes > 0 ? bytes : 1);
+    a.together = (int32_t)(fit < 1 ? 1 : fit > most ? (most < 1 ? 1 : most) : fit);
     return a;
 }
 

@@ -17,22 +17,25 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
     using T = Tile<D>;
     using F = Frags<D>;
     constexpr int TB = RT * T::RB, n = D / 16, KB = KEPT ? 0 : 32 * NW * T::RB;
-    constexpr bool ACC = PER == 1 && D < 256;
+    constexpr bool ACC = PER == 1;
     constexpr int OB = SLOTS * TB, HB = 2 * SLOTS * TB;  // queries' slots, then dO's, then the keys
     __shared__ __attribute__((aligned(1024))) uint8_t lds[HB + KB];
     __shared__ __attribute__((aligned(16))) float stat[SLOTS][2][64];  // log-sum-exp in base 2, and D, of a tile's rows
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
-    const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, part = blockIdx.x / nb;
+    const int nb = a.batch * a.hk;
+    const Place place(nb, (nb + 7) / 8);  // the heads' queries are too many to keep: by work alone
+    const int bh = place.bh, hk = bh % a.hk, part = place.part;
     const int tiles = gridDim.x / (nb * a.k_splits), split = part % a.k_splits;
     const Seq s = sequence(a, bh / a.hk);
     const int cover = a.kv_starts ? s.lk : a.lk;  // the dense form's keys past a sequence's length get zeros
     const float sl = back_scale(a), out_of_sight = sl > 0.0f ? -INFINITY : INFINITY;
     const int64_t qts = 2 * a.q.ts, ots = 2 * a.d_o.ts;
-    const Loader<D, RT, 64 * NW> ql(qts, a.d, tid), ol(ots, a.d, tid);
     const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + F::col0(lane);
     const uint32_t hat = rat + HB + 32 * wave * T::RB;  // the wave's keys, where they are not kept
     for (int64_t tile = part / a.k_splits; tile * 32 * NW < cover; tile += tiles) {
         const int w0 = (int)tile * 32 * NW, k0 = w0 + 32 * wave, key = k0 + col;
+        const int t_ = fresh_lane(tid);  // not held over the results' stores
+        const Loader<D, RT, 64 * NW> ql(qts, a.d, t_), ol(ots, a.d, t_);
         bf16x8 k[KEPT ? D / 16 : 1], v[D / 16];
         const int kk = key < s.lk ? key : 0;
         if constexpr (KEPT) {
@@ -204,16 +207,18 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
             }
         }
         landed();
-        settled<ACC>(dk);
-        settled<ACC>(dv);
+        settled<ACC>();
         const bool seen = key < s.lk;
         const int dd = fresh(a.d), hs = fresh_lane(h);
         if (a.k_splits > 1) {
             const int64_t at = (split * a.kv_slots + kv_slot(a, s, hk, key)) * dd;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-                if (!seen) dk[i] = dv[i] = (f32x16){};
+                settle_sum<ACC>(dk[i]);
+                if (!seen) dk[i] = (f32x16){};
                 store_block(reinterpret_cast<uint8_t*>(a.dk_part + at), true, key < cover, 32 * i, dd, hs, dk[i], 1.0f);
+                settle_sum<ACC>(dv[i]);
+                if (!seen) dv[i] = (f32x16){};
                 store_block(reinterpret_cast<uint8_t*>(a.dv_part + at), true, key < cover, 32 * i, dd, hs, dv[i], 1.0f);
             }
             __syncthreads();
@@ -223,8 +228,11 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
         uint8_t* ov = kv_at(a.dv, a, s, hk) + (a.dv.f32 ? 4 : 2) * (key * a.dv.ts);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-            if (!seen) dk[i] = dv[i] = (f32x16){};
+            settle_sum<ACC>(dk[i]);
+            if (!seen) dk[i] = (f32x16){};
             store_block(ok, a.dk.f32, key < cover, 32 * i, dd, hs, dk[i], a.scale);
+            settle_sum<ACC>(dv[i]);
+            if (!seen) dv[i] = (f32x16){};
             store_block(ov, a.dv.f32, key < cover, 32 * i, dd, hs, dv[i], 1.0f);
         }
         __syncthreads();

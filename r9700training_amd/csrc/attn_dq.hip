@@ -30,7 +30,9 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
     constexpr bool ACC = false;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[7 * TB];  // keys' four slots, then the values' three
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
-    const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, part = blockIdx.x / nb;
+    const int nb = a.batch * a.hk;
+    const Place place(nb, a.together);
+    const int bh = place.bh, hk = bh % a.hk, part = place.part;
     const int tiles = gridDim.x / (nb * a.q_splits), split = part % a.q_splits;
     const Seq s = sequence(a, bh / a.hk);
     const int rows = s.lq * a.g;
@@ -38,9 +40,10 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
     const uint8_t* kb = kv_at(a.k, a, s, hk);
     const uint8_t* vb = kv_at(a.v, a, s, hk);
     const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
-    const Loader<D, KT, 64 * NW> kl(kts, a.d, tid), vl(vts, a.d, tid);
     const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + F::col0(lane);
     for (int64_t tile = tiles - 1 - part / a.q_splits; tile * 32 * NW < rows; tile += tiles) {
+        const int t_ = fresh_lane(tid);  // not held over the results' stores
+        const Loader<D, KT, 64 * NW> kl(kts, a.d, t_), vl(vts, a.d, t_);
         const int w0 = (int)tile * 32 * NW, r0 = w0 + 32 * wave, r = r0 + col;
         const int rr = r < rows ? r : rows - 1, tok = rr / a.g, head = hk * a.g + (rr - tok * a.g);
         const int wend = w0 + 32 * NW - 1 < rows ? w0 + 32 * NW - 1 : rows - 1;
@@ -61,13 +64,15 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
         int d = fresh(a.d);
         bf16x8 q[n], go[n];
         load_row<D>(q_at(a.q, a, s, head) + 2 * (tok * a.q.ts), r < rows, d, lane, q);
-        load_row<D>(q_at(a.d_o, a, s, head) + 2 * (tok * a.d_o.ts), r < rows, d, lane, go);
         settle<ACC>(q);
+        if constexpr (ACC) pin();
+        load_row<D>(q_at(a.d_o, a, s, head) + 2 * (tok * a.d_o.ts), r < rows, d, lane, go);
         settle<false>(go);
         const uint8_t* op = q_at(a.o, a, s, head) + (a.o.f32 ? 4 : 2) * (tok * a.o.ts);
         float delta = 0.0f;
 #pragma unroll
         for (int c = 0; c < n; ++c) {
+            if (ACC && c % 4 == 0) pin();  // a few at a time: the registers are taken
             const int e = 16 * c + 8 * h;
             if (e < d) {
                 if (a.o.f32) {
@@ -180,19 +185,25 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
             }
             landed();
         }
-        settled<ACC>(dq);
+        settled<ACC>();
         d = fresh(a.d);
         const int hs = fresh_lane(h);
         if (a.q_splits > 1) {
             uint8_t* out = reinterpret_cast<uint8_t*>(a.dq_part + (split * a.slots + st) * d);
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) store_block(out, true, r < rows, 32 * i, d, hs, dq[i], 1.0f);
+            for (int i = 0; i < D / 32; ++i) {
+                settle_sum<ACC>(dq[i]);
+                store_block(out, true, r < rows, 32 * i, d, hs, dq[i], 1.0f);
+            }
             __syncthreads();
             continue;
         }
         uint8_t* out = q_at(a.dq, a, s, head) + (a.dq.f32 ? 4 : 2) * (tok * a.dq.ts);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) store_block(out, a.dq.f32, r < rows, 32 * i, d, hs, dq[i], a.scale);
+        for (int i = 0; i < D / 32; ++i) {
+            settle_sum<ACC>(dq[i]);
+            store_block(out, a.dq.f32, r < rows, 32 * i, d, hs, dq[i], a.scale);
+        }
         __syncthreads();
     }
 }

@@ -166,7 +166,9 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     constexpr int TB = KT * T::RB, SUBS = KT / 32, n = D / 16;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB];  // keys' two slots, then the values'
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
-    const int nb = a.batch * a.hk, bh = blockIdx.x % nb, hk = bh % a.hk, part = blockIdx.x / nb;
+    const int nb = a.batch * a.hk;
+    const Place place(nb, a.together);
+    const int bh = place.bh, hk = bh % a.hk, part = place.part;
     const int tiles = gridDim.x / (nb * a.splits), split = part % a.splits;
     const Seq s = sequence(a, bh / a.hk);
     const int rows = s.lq * a.g;
