@@ -11,7 +11,7 @@ namespace attn {
 int64_t fwd_workspace(const Args& a);
 int launch_fwd(Args a, void* workspace, hipStream_t st);
 int launch_dq(const Args& a, hipStream_t st);
-int launch_sum(const Args& a, const Heads& out, const float* part, int splits, bool keys, float f, hipStream_t st);
+int launch_sums(const Args& a, bool keys, hipStream_t st);
 int launch_dkdv(const Args& a, hipStream_t st);
 int launch_dkdv_wide(const Args& a, hipStream_t st);
 
@@ -230,11 +230,9 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
     hipStream_t st = (hipStream_t)stream;
     if (int e = launch_dq(a, st)) return e;
     if (a.q_splits > 1)
-        if (int e = launch_sum(a, a.dq, a.dq_part, a.q_splits, false, a.scale, st)) return e;
+        if (int e = launch_sums(a, false, st)) return e;
     if (int e = a.d > 128 ? launch_dkdv_wide(a, st) : launch_dkdv(a, st)) return e;
-    if (a.k_splits == 1) return R97Q_OK;
-    if (int e = launch_sum(a, a.dk, a.dk_part, a.k_splits, true, a.scale, st)) return e;
-    return launch_sum(a, a.dv, a.dv_part, a.k_splits, true, 1.0f, st);
+    return a.k_splits > 1 ? launch_sums(a, true, st) : R97Q_OK;
 }
 
 }  // extern "C"

@@ -209,9 +209,20 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------- partial sums added
-// grid (batch * heads, tokens): a row's partial sums in order, times f, to the output. keys: rows of dk or dv.
-__global__ __launch_bounds__(256) void attn_sum_kernel(Args a, Heads out, const float* part, int splits, bool keys, float f) {
-    const int heads = keys ? a.hk : a.hq, head = blockIdx.x % heads;
+// grid (batch * heads, tokens, tensors): a row's partial sums in order, times the tensor's factor, to the output.
+struct Sum {
+    Heads out[2];
+    const float* part[2];
+    float factor[2];
+    int32_t splits;
+    bool keys;  // rows of dK and dV, else of dQ
+};
+__global__ __launch_bounds__(256) void attn_sum_kernel(Args a, Sum u) {
+    const bool keys = u.keys;
+    const int heads = keys ? a.hk : a.hq, head = blockIdx.x % heads, which = blockIdx.z;
+    const Heads out = u.out[which];
+    const float* part = u.part[which];
+    const float f = u.factor[which];
     const Seq s = sequence(a, blockIdx.x / heads);
     const int per = a.d / 4, rows = 256 / per, r = threadIdx.x / per, c = 4 * (threadIdx.x % per);
     const int cover = !keys ? s.lq : a.kv_starts ? s.lk : a.lk;
@@ -220,9 +231,10 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(Args a, Heads out, const 
     for (int64_t t = (int64_t)blockIdx.y * rows + r; t < cover; t += (int64_t)gridDim.y * rows) {
         const int64_t at = (keys ? kv_slot(a, s, head, (int)t) : stat_at(a, s, head, (int)t)) * a.d + c;
         float4 v = *reinterpret_cast<const float4*>(part + at);
-        for (int i = 1; i < splits; ++i) {
-            const float4 u = *reinterpret_cast<const float4*>(part + i * slots * a.d + at);
-            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+#pragma unroll 4
+        for (int i = 1; i < u.splits; ++i) {
+            const float4 w = *reinterpret_cast<const float4*>(part + i * slots * a.d + at);
+            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
         }
         uint8_t* row = (keys ? kv_at(out, a, s, head) : q_at(out, a, s, head)) + (out.f32 ? 4 : 2) * (t * out.ts);
         if (out.f32)
@@ -244,11 +256,12 @@ int run(const Args& a, hipStream_t st) {
 
 }  // namespace
 
-int launch_sum(const Args& a, const Heads& out, const float* part, int splits, bool keys, float f, hipStream_t st) {
+int launch_sums(const Args& a, bool keys, hipStream_t st) {
     const int64_t tokens = keys ? a.lk : a.lq, rows = 256 / (a.d / 4), blocks = (tokens + rows - 1) / rows;
     if (blocks == 0) return R97Q_OK;
-    hipLaunchKernelGGL(attn_sum_kernel, dim3((unsigned)(a.batch * (keys ? a.hk : a.hq)), (unsigned)(blocks < 65535 ? blocks : 65535)),
-                       dim3(256), 0, st, a, out, part, splits, keys, f);
+    Sum u = {{keys ? a.dk : a.dq, a.dv}, {keys ? a.dk_part : a.dq_part, a.dv_part}, {a.scale, 1.0f}, keys ? a.k_splits : a.q_splits, keys};
+    hipLaunchKernelGGL(attn_sum_kernel, dim3((unsigned)(a.batch * (keys ? a.hk : a.hq)), (unsigned)(blocks < 65535 ? blocks : 65535), keys ? 2 : 1),
+                       dim3(256), 0, st, a, u);
     return launch_status("attn_sum_kernel");
 }
 
