@@ -56,6 +56,9 @@ struct Args {
     int32_t q_splits, k_splits;
     int64_t kv_slots;    // rows of one dk or dv partial
     float *dq_part, *dk_part, *dv_part;  // [splits][slots][d]
+    // dS^T kept between the launches, bf16: a query head's row of `pitch` tokens for each key; null: computed again
+    uint16_t* ds;
+    int64_t pitch;
     int32_t batch, hq, hk, g, d;
     int32_t lq, lk;      // tokens of a sequence (packed: of the longest)
     const int32_t* q_starts;
@@ -160,6 +163,22 @@ struct Place {
 // a key's row of a partial sum
 __device__ __forceinline__ int64_t kv_slot(const Args& a, const Seq& s, int hk, int key) {
     return a.kv_starts ? hk * a.kv_tokens + s.k_base + key : ((int64_t)s.b * a.hk + hk) * a.lk + key;
+}
+
+// the kept dS^T: where the row of a head's key begins, at the sequence's token 0. Packed sequences begin on 64 tokens.
+__device__ __forceinline__ uint16_t* ds_at(const Args& a, const Seq& s, int head, int key) {
+    const int64_t row = a.kv_starts ? head * a.kv_tokens + s.k_base + key : ((int64_t)s.b * a.hq + head) * a.lk + key;
+    const int64_t col = a.q_starts ? (s.q_base + 63LL) / 64 * 64 + 64LL * s.b : 0;
+    return a.ds + row * a.pitch + col;
+}
+// dK's and dV's tiles of RT tokens for 128 keys from w0: the first one's token, a multiple of RT, and the tokens' end
+__device__ __forceinline__ void tokens_of(const Args& a, const Seq& s, int w0, int rt, int& t0, int& t1) {
+    const int wend = w0 + 127 < s.lk ? w0 + 127 : s.lk - 1;
+    t0 = 0;
+    t1 = s.lq;
+    if (a.causal) t0 = (int)clamp64((int64_t)w0 - s.off, 0, s.lq) / rt * rt;
+    if (a.window) t1 = (int)clamp64((int64_t)wend + a.window - s.off, t0, s.lq);
+    if (w0 >= s.lk) t1 = t0;
 }
 
 // the keys [lo, hi) that some of the queries at tokens [t0, t1] see (hi <= lo: none), and [all_lo, all_hi)
@@ -421,6 +440,18 @@ __device__ __forceinline__ void load_row(const uint8_t* row, bool valid, int d, 
         for (int j = 0; j < 4; ++j) w[c][j] = on ? w[c][j] : 0u;
         out[c] = as_bf16x8(w[c]);
     }
+}
+
+// a 32 x 32 tile's bf16 words, as B operands, back to rows: the lane's column holds rows 16 c + 8 h .. + 7 in 16 bytes
+__device__ __forceinline__ u32x4 rows_of(const u32x4& w) {
+    u32x4 r;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const auto s = __builtin_amdgcn_permlane32_swap(w[j], w[2 + j], false, false);
+        r[j] = s[0];
+        r[2 + j] = s[1];
+    }
+    return r;
 }
 
 // A lane's 16 values of one 32-column block of an output row (columns 8e + 4h + 0..3 of the block, e = 0..3),

@@ -11,6 +11,8 @@ namespace attn {
 int64_t fwd_workspace(const Args& a);
 int launch_fwd(Args a, void* workspace, hipStream_t st);
 int launch_dq(const Args& a, hipStream_t st);
+int launch_base(const Args& a, hipStream_t st);
+int launch_dq_kept(const Args& a, hipStream_t st);
 int launch_sums(const Args& a, bool keys, hipStream_t st);
 int launch_dkdv(const Args& a, hipStream_t st);
 int launch_dkdv_wide(const Args& a, hipStream_t st);
@@ -88,6 +90,9 @@ Args args_of(const R97qAttnShape* p, int32_t hq, int32_t hk) {
     a.d = p->head_dim;
     a.lq = (int32_t)p->q_len;
     a.lk = (int32_t)p->kv_len;
+    // a longest sequence of nothing is taken for a wrong one: what the starts say counts
+    if (p->q_starts && p->q_tokens > 0 && a.lq == 0) a.lq = 1;
+    if (p->kv_starts && p->kv_tokens > 0 && a.lk == 0) a.lk = 1;
     a.q_starts = p->q_starts;
     a.kv_starts = p->kv_starts;
     a.kv_lens = p->kv_lens;
@@ -133,6 +138,22 @@ void cut_backward(Args& a) {
     }
     a.kv_slots = a.kv_starts ? a.hk * a.kv_tokens : (int64_t)a.batch * a.hk * a.lk;
 }
+// Whether dS^T is kept between the launches (then dQ is one product from it, instead of three from scratch): the bytes,
+// or 0. It costs its bytes written and read, and D's own launch. Measured, computed again / kept (us): heads of 256, 8 x
+// 2048 tokens, 16 over 4 heads 1026 / 843, 1 x 512 tokens, 8 over 2 68 / 51; heads of 128, 16 over 4, 8 x 2048 502 / 537,
+// 4 x 2048 322 / 320, 4 x 1300 159 / 146, 1 x 1300 82 / 68; heads of 64, 8 x 2048 287 / 382, 4 x 1300 92 / 106, 1 x
+// 1300 54 / 51. So from heads of more than 64 columns, up to 512 MiB with heads of up to 128, and up to 2 GiB of
+// workspace; not where dQ's rows are cut, since few rows over many keys are few workgroups here (64 over 4096: 45 / 60).
+int64_t kept_bytes(Args& a) {
+    if (a.d <= 64 || a.q_splits > 1 || a.batch == 0) return 0;
+    const double rows = a.kv_starts ? (double)a.hq * a.kv_tokens : (double)a.batch * a.hq * a.lk;
+    a.pitch = a.q_starts ? (a.q_tokens + 64LL * (a.batch + 2) + 63) / 64 * 64 : ((int64_t)a.lq + 127) / 128 * 128;
+    // what is touched of it: packed sequences leave most of it alone
+    const double each = (double)mean_len(a.q_starts, a.q_tokens, a.lq, a.batch) * mean_len(a.kv_starts, a.kv_tokens, a.lk, a.batch);
+    if (a.pitch > kMostStride || 2.0 * rows * a.pitch > (double)(2LL << 30)) return 0;
+    if (a.d <= 128 && 2.0 * a.batch * a.hq * each > (double)(512LL << 20)) return 0;
+    return (2 * (int64_t)rows * a.pitch + 255) / 256 * 256;
+}
 int64_t bwd_stats(const Args& a) { return (8 * a.slots + 255) / 256 * 256; }
 
 }  // namespace
@@ -167,7 +188,7 @@ int r97q_attn_fwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
     const int64_t need = r97q_attn_fwd_workspace_bytes(shape, hq, hk);
     if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
     if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
-    if (b == 0 || n == 0 || shape->q_len == 0) return R97Q_OK;
+    if (b == 0 || n == 0) return R97Q_OK;
     Args a = args_of(shape, hq, hk);
     a.q = heads_of(q, n);
     a.k = heads_of(k, m);
@@ -182,8 +203,8 @@ int64_t r97q_attn_bwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_head
     if (check_shape(shape, q_heads, kv_heads, "r97q_attn_bwd_workspace_bytes")) return -1;
     Args a = args_of(shape, q_heads, kv_heads);
     cut_backward(a);
-    const int64_t row = 4 * a.d;
-    return bwd_stats(a) + (a.q_splits > 1 ? a.q_splits * a.slots * row : 0) + (a.k_splits > 1 ? 2 * a.k_splits * a.kv_slots * row : 0);
+    const int64_t row = 4 * a.d, kept = kept_bytes(a);
+    return bwd_stats(a) + kept + (a.q_splits > 1 ? a.q_splits * a.slots * row : 0) + (a.k_splits > 1 ? 2 * a.k_splits * a.kv_slots * row : 0);
 }
 
 int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
@@ -224,14 +245,19 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
     a.lse = const_cast<float*>(lse);
     a.base = static_cast<float*>(workspace);
     a.delta = a.base + a.slots;
-    a.dq_part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + bwd_stats(a));
+    const int64_t kept = kept_bytes(a);
+    uint8_t* rest = static_cast<uint8_t*>(workspace) + bwd_stats(a);
+    if (kept) a.ds = reinterpret_cast<uint16_t*>(rest);
+    a.dq_part = reinterpret_cast<float*>(rest + kept);
     a.dk_part = a.dq_part + (a.q_splits > 1 ? a.q_splits * a.slots * a.d : 0);
     a.dv_part = a.dk_part + a.k_splits * a.kv_slots * a.d;
     hipStream_t st = (hipStream_t)stream;
-    if (int e = launch_dq(a, st)) return e;
+    if (int e = kept ? launch_base(a, st) : launch_dq(a, st)) return e;
     if (a.q_splits > 1)
         if (int e = launch_sums(a, false, st)) return e;
     if (int e = a.d > 128 ? launch_dkdv_wide(a, st) : launch_dkdv(a, st)) return e;
+    if (kept)
+        if (int e = launch_dq_kept(a, st)) return e;
     return a.k_splits > 1 ? launch_sums(a, true, st) : R97Q_OK;
 }
 

@@ -12,7 +12,7 @@ namespace {
 // RT tokens of a head at a time. KEPT: the keys stay in registers; at 256 columns the gradients take 256 of a
 // lane's 512 and the keys stay in LDS instead. SLOTS: tiles of Q and dO in LDS; with three, the
 // next tile has landed a step early and its first operands are read before the step's barrier.
-template <int D, int RT, int NW, bool KEPT, int PER, int SLOTS>
+template <int D, int RT, int NW, bool KEPT, int PER, int SLOTS, bool STORE>
 __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
     using T = Tile<D>;
     using F = Frags<D>;
@@ -52,12 +52,10 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
         load_row<D>(kv_at(a.v, a, s, hk) + 2 * (kk * a.v.ts), key < s.lk, fresh(a.d), lane, v);
         settle<false>(v);
         if constexpr (KEPT) settle<false>(k);
-        // the tokens [t0, t1) that see any of the workgroup's keys
-        const int wend = w0 + 32 * NW - 1 < s.lk ? w0 + 32 * NW - 1 : s.lk - 1;
-        int t0 = 0, t1 = s.lq;
-        if (a.causal) t0 = (int)clamp64((int64_t)w0 - s.off, 0, s.lq);
-        if (a.window) t1 = (int)clamp64((int64_t)wend + a.window - s.off, t0, s.lq);
-        if (w0 >= s.lk) t1 = t0;
+        // the tokens [t0, t1) that see any of the workgroup's keys, from a tile's first
+        static_assert(NW == 4, "tokens_of() is for 128 keys");
+        int t0, t1;
+        tokens_of(a, s, w0, RT, t0, t1);
         f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) dk[i] = dv[i] = (f32x16){};
@@ -76,6 +74,12 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
             qb += hd * qhs, ob += hd * ohs, sb += hd * shs;
             Rows qr(qb, qts, t, t1, a.d), orr(ob, ots, t, t1, a.d), sr(sb, 4, t, t1, 2);
             int to_load = end - first;
+            uint16_t* kept = nullptr;  // this key's row of dS^T
+            int64_t ds_head = 0;
+            if constexpr (STORE) {
+                kept = ds_at(a, s, hk * a.g + hd, key < cover ? key : 0);
+                ds_head = (a.kv_starts ? a.kv_tokens : (int64_t)a.lk) * a.pitch;
+            }
             auto load_stat = [&](int slot) {  // wave 0 the one, wave 1 the other
                 if (wave < 2) load_words(sr.template buffer<RT>(), 4 * lane, lds_at(stat) + 512 * slot + 256 * wave);
             };
@@ -116,7 +120,11 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
                 first_frags(rat);
             }
             for (int step = first, slot = 0, fill = SLOTS - 1, at_t = t; step < end; ++step) {
-                landed();
+                // all but the last step's stores, which went out after its loads (a wave past the keys has none)
+                if (STORE && step > first && k0 < cover)
+                    landed<2 * (RT / 32)>();
+                else
+                    landed();
                 __syncthreads();
                 load_stat(fill);
                 held = (uint32_t)fresh_lane((int)hat);  // its addresses are made here, not held through the loop
@@ -183,6 +191,11 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
                         if constexpr (!KEPT && (SLOTS > 2 || sub + 1 < RT / 32) && c >= n - kAhead)
                             kf[c - (n - kAhead)] = F::template rows<0, c - (n - kAhead)>(held);
                     }
+                    if constexpr (STORE && ph == 3 && c == n - 1) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            if (key < cover) *reinterpret_cast<u32x4*>(kept + t + 32 * sub + 16 * u + 8 * h) = rows_of(ds[u]);
+                    }
                     // Vector work, spread over the products that do not need it: the exponentials from two products after
                     // x's last one to the second half's use, dS likewise after y's.
                     constexpr int st = i % (4 * n), len = n - 3 + D / 32;
@@ -201,6 +214,9 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
                 });
                 pin();
                 next();
+                if constexpr (STORE) {
+                    if (t + RT >= t1) kept += ds_head;
+                }
                 at_t = t + RT < t1 ? t + RT : t0;
                 slot = slot1;
                 fill = fill + 1 == SLOTS ? 0 : fill + 1;
@@ -245,7 +261,13 @@ int run(const Args& a, hipStream_t st) {
     int64_t keys = ((int64_t)a.lk + 127) / 128;
     if (keys > most) keys = most;
     if (keys == 0) return R97Q_OK;
-    hipLaunchKernelGGL((attn_dkdv_kernel<D, RT, 4, KEPT, PER, SLOTS>), dim3((unsigned)(keys * nb)), dim3(256), 0, st, a);
+    if constexpr (D > 64) {  // narrower heads' dS is not kept
+        if (a.ds) {
+            hipLaunchKernelGGL((attn_dkdv_kernel<D, RT, 4, KEPT, PER, SLOTS, true>), dim3((unsigned)(keys * nb)), dim3(256), 0, st, a);
+            return launch_status("attn_dkdv_kernel");
+        }
+    }
+    hipLaunchKernelGGL((attn_dkdv_kernel<D, RT, 4, KEPT, PER, SLOTS, false>), dim3((unsigned)(keys * nb)), dim3(256), 0, st, a);
     return launch_status("attn_dkdv_kernel");
 }
 

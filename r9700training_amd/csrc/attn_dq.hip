@@ -208,6 +208,113 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
     }
 }
 
+// ---------------------------------------------------------------- D alone
+// D and the log-sum-exp in base 2 for dK's and dV's launch, where that one goes first. grid (batch * q heads, tokens):
+// d / 8 threads a row, rounded up to a power of two.
+__global__ __launch_bounds__(256) void attn_base_kernel(Args a, int lanes) {
+    const int head = blockIdx.x % a.hq, rows = 256 / lanes, c = 8 * (threadIdx.x % lanes);
+    const Seq s = sequence(a, blockIdx.x / a.hq);
+    const uint8_t *ob = q_at(a.o, a, s, head), *gb = q_at(a.d_o, a, s, head);
+    for (int64_t t0 = (int64_t)blockIdx.y * rows; t0 < s.lq; t0 += (int64_t)gridDim.y * rows) {
+        const int64_t t = t0 + threadIdx.x / lanes;
+        float sum = 0.0f;
+        if (t < s.lq && c < a.d) {
+            const bf16x8 g = as_bf16x8(*reinterpret_cast<const u32x4*>(gb + 2 * (t * a.d_o.ts + c)));
+            if (a.o.f32) {
+                const float* o = reinterpret_cast<const float*>(ob) + t * a.o.ts + c;
+                const float4 x = *reinterpret_cast<const float4*>(o), y = *reinterpret_cast<const float4*>(o + 4);
+                sum = x.x * (float)g[0] + x.y * (float)g[1] + x.z * (float)g[2] + x.w * (float)g[3];
+                sum += y.x * (float)g[4] + y.y * (float)g[5] + y.z * (float)g[6] + y.w * (float)g[7];
+            } else {
+                const bf16x8 o = as_bf16x8(*reinterpret_cast<const u32x4*>(ob + 2 * (t * a.o.ts + c)));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += (float)o[j] * (float)g[j];
+            }
+        }
+        for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        if (t < s.lq && c == 0) {
+            const int64_t at = stat_at(a, s, head, (int)t);
+            const float lse = a.lse[at];
+            a.base[at] = lse == -INFINITY ? 0.0f : lse * kLog2e;
+            a.delta[at] = -sum;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- dQ from the kept dS
+// dQ^T = scale K^T dS^T for 128 tokens of a query head: 32 of them a wave. The keys and dS^T's rows of the same keys go
+// through two slots of LDS, both read transposed. dS^T is written for blocks of 128 keys and RT tokens where any
+// of them sees any; a wave passes over the others. No mask: an unseen pair's dS is zero.
+template <int D, int KT, int PER, int RT>
+__global__ __launch_bounds__(256, PER) void attn_dq_kept_kernel(Args a) {
+    using F = Frags<D>;
+    using S = Frags<128>;  // rows of 128 tokens
+    constexpr int TB = KT * 2 * D, SB = KT * 256, SLOT = TB + SB, n = (KT / 16) * (D / 32);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * SLOT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
+    // the query heads of a key head one beside the other
+    const int nb = a.batch * a.hk;
+    const Place place(nb, a.together);
+    const int bh = place.bh, hk = bh % a.hk, parts = gridDim.x / nb, tiles = parts / a.g, head = hk * a.g + place.part % a.g;
+    const Seq s = sequence(a, bh / a.hk);
+    const uint8_t* kb = kv_at(a.k, a, s, hk);
+    const int64_t kts = 2 * a.k.ts;
+    const uint32_t at = lds_at(lds), mine = at + 1024 * wave, kat = at + F::col0(lane), sat = (at + TB + S::col0(lane)) ^ (64 * wave);
+    for (int64_t tile = tiles - 1 - place.part / a.g; tile * 128 < s.lq; tile += tiles) {
+        const int t_ = fresh_lane(tid);
+        const Loader<D, KT, 256> kl(kts, a.d, t_);
+        const Loader<128, KT, 256> sl(2 * a.pitch, 128, t_);
+        const int w0 = (int)tile * 128, r0 = w0 + 32 * wave, wend = w0 + 127 < s.lq ? w0 + 127 : s.lq - 1;
+        const Keys all = keys_of(a, s, w0, wend);
+        const int lo = all.lo / 128 * 128, hi = all.hi;
+        Rows kr(kb, kts, lo, hi, a.d), sr(reinterpret_cast<const uint8_t*>(ds_at(a, s, head, 0) + w0), 2 * a.pitch, lo, hi, 128);
+        f32x16 dq[D / 32];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) dq[i] = (f32x16){};
+        auto load = [&](int slot) {
+            kl.load(kr, mine + slot * SLOT);
+            sl.load(sr, mine + slot * SLOT + TB);
+            kr.step(KT);
+            sr.step(KT);
+        };
+        if (lo < hi) load(0);
+        bool seen = false;
+        auto step = [&](int j0, auto slot_) {
+            constexpr int slot = slot_;
+            landed();
+            __syncthreads();
+            load(1 - slot);
+            if ((j0 & 127) == 0) {
+                int t0, t1;
+                tokens_of(a, s, j0, RT, t0, t1);
+                seen = t0 < t1 && r0 + 32 > t0 && r0 < (t1 + RT - 1) / RT * RT && r0 < s.lq;
+            }
+            if (!seen) return;
+            bf16x8 f[kAhead], g[KT / 16];
+            auto frag = [&](auto i) { return F::template cols<16 * (i / (D / 32)) + slot * (SLOT / (2 * D)), i % (D / 32)>(kat); };
+            steps<KT / 16>([&](auto i) { g[i] = S::template cols<16 * i + slot * (SLOT / 256), 0>(sat); });
+            steps<kAhead>([&](auto i) { f[i] = frag(i); });
+            steps<n>([&](auto i) {
+                pin();
+                const bf16x8 now = f[i % kAhead];
+                if constexpr (i + kAhead < n) f[i % kAhead] = frag(std::integral_constant<int, i + kAhead>{});
+                dq[i % (D / 32)] = mfma(now, g[i / (D / 32)], dq[i % (D / 32)]);
+            });
+            pin();
+        };
+        for (int j0 = lo; j0 < hi; j0 += 2 * KT) {
+            step(j0, std::integral_constant<int, 0>{});
+            if (j0 + KT < hi) step(j0 + KT, std::integral_constant<int, 1>{});
+        }
+        landed();
+        const int t = r0 + col, d = fresh(a.d), hs = fresh_lane(h);
+        uint8_t* out = q_at(a.dq, a, s, head) + (a.dq.f32 ? 4 : 2) * ((int64_t)t * a.dq.ts);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) store_block(out, a.dq.f32, t < s.lq, 32 * i, d, hs, dq[i], a.scale);
+        __syncthreads();
+    }
+}
+
 // ---------------------------------------------------------------- partial sums added
 // grid (batch * heads, tokens, tensors): a row's partial sums in order, times the tensor's factor, to the output.
 struct Sum {
@@ -263,6 +370,27 @@ int launch_sums(const Args& a, bool keys, hipStream_t st) {
     hipLaunchKernelGGL(attn_sum_kernel, dim3((unsigned)(a.batch * (keys ? a.hk : a.hq)), (unsigned)(blocks < 65535 ? blocks : 65535), keys ? 2 : 1),
                        dim3(256), 0, st, a, u);
     return launch_status("attn_sum_kernel");
+}
+
+int launch_base(const Args& a, hipStream_t st) {
+    const int lanes = a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32, rows = 256 / lanes;
+    const int64_t blocks = ((int64_t)a.lq + rows - 1) / rows;
+    if (blocks == 0) return R97Q_OK;
+    hipLaunchKernelGGL(attn_base_kernel, dim3((unsigned)(a.batch * a.hq), (unsigned)(blocks < 65535 ? blocks : 65535)), dim3(256), 0, st, a, lanes);
+    return launch_status("attn_base_kernel");
+}
+
+template <int D, int KT, int PER, int RT>
+int run_kept(const Args& a, hipStream_t st) {
+    const int64_t nb = (int64_t)a.batch * a.hq, most = 0x7FFFFFFF / nb;
+    int64_t tiles = ((int64_t)a.lq + 127) / 128;
+    if (tiles > most) tiles = most;
+    if (tiles == 0) return R97Q_OK;
+    hipLaunchKernelGGL((attn_dq_kept_kernel<D, KT, PER, RT>), dim3((unsigned)(tiles * nb)), dim3(256), 0, st, a);
+    return launch_status("attn_dq_kept_kernel");
+}
+int launch_dq_kept(const Args& a, hipStream_t st) {
+    return a.d <= 128 ? run_kept<128, 64, 2, 64>(a, st) : run_kept<256, 32, 2, 32>(a, st);
 }
 
 int launch_dq(const Args& a, hipStream_t st) { return a.d <= 64 ? run<64, 2>(a, st) : a.d <= 128 ? run<128, 2>(a, st) : run<256, 1>(a, st); }
