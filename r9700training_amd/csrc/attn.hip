@@ -32,6 +32,9 @@ int check_shape(const R97qAttnShape* p, int32_t hq, int32_t hk, const char* who)
     if (hk <= 0 || hq <= 0 || hq % hk) return refuse(R97Q_EINVAL, who, "the query heads are a multiple of the key heads");
     if (p->batch < 0 || p->q_len < 0 || p->kv_len < 0) return refuse(R97Q_EINVAL, who, "a negative batch or length");
     if (p->batch > 65535 || hk > 65535) return refuse(R97Q_EUNSUPPORTED, who, "at most 65535 sequences and key heads");
+    // heads times kMostSplits or kMostCuts workgroups of a one-dimensional grid
+    if ((int64_t)p->batch * hq > 0x7FFFFFFF / kMostSplits)
+        return refuse(R97Q_EUNSUPPORTED, who, "the sequences' heads in all pass 2^23");
     if (p->q_len > 0x7FFFFF00 / (hq / hk) || p->kv_len > 0x7FFFFF00)
         return refuse(R97Q_EUNSUPPORTED, who, "a sequence's rows of one key head or its keys pass 31 bits");
     if (p->window < 0 || (p->window && !p->causal)) return refuse(R97Q_EINVAL, who, "a window is positive and needs causal");

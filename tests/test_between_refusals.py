@@ -194,3 +194,19 @@ def test_fronts_refuse_before_the_library():
         turn(x[0], None, torch.zeros(32), pairs="quarter")
     with pytest.raises(ValueError):
         rotary_frequencies(64, scaling="cubic", device="cpu")
+
+
+def test_attention_limits_of_its_tiles():
+    """Tokens so far apart that a tile passes 31 bits, workspaces off 16 bytes, and more heads than a grid holds."""
+    far = dict(token_stride=(1 << 24) + 8)
+    for which in ("q", "k", "v", "d_out"):
+        t = heads(2 if which in "kv" else 4, **far)
+        if which != "d_out":
+            assert fwd(shape(), **{which: t}) == EUNSUPPORTED, which
+        assert bwd(shape(), **{which: t}) == EUNSUPPORTED, which
+    need = lib().r97q_attn_bwd_workspace_bytes(shape(), 4, 2)
+    assert bwd(shape(), ws=FAKE + 8, nws=need + 64) == EINVAL
+    long = shape(batch=1, q_len=1, kv_len=1 << 16)
+    assert lib().r97q_attn_fwd_workspace_bytes(long, 4, 2) > 0
+    assert fwd(long, ws=None) == EWORKSPACE and fwd(long, ws=FAKE + 4) == EINVAL
+    assert lib().r97q_attn_fwd_workspace_bytes(shape(batch=65535), 256, 256) == -1

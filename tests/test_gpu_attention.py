@@ -318,3 +318,115 @@ def test_gradient_against_differences():
         got = (f[0] - f[1]) / 2
         noise = 2 ** -8 * float((do.double().abs() * v.double().abs().mean()).sum()) / math.sqrt(do.numel())
         assert abs(got - want) <= 0.02 * abs(want) + 4 * noise, (name, got, want, noise)
+
+
+CUT = [
+    # few workgroups over many keys: ranges of the keys joined, dQ's and dK's sums cut; the probabilities computed again
+    (1, 40, 1200, 4, 2, 128, True, 0),
+    (1, 64, 2100, 4, 1, 256, True, 0),
+    (2, 33, 1500, 6, 2, 128, False, 0),
+    (1, 90, 3000, 2, 1, 64, True, 1500),
+    (1, 70, 2500, 4, 2, 128, True, 1100),
+    (1, 1, 1500, 6, 1, 256, True, 0),
+    (1, 3, 5000, 8, 1, 128, True, 1300),
+    (2, 5, 2600, 12, 2, 80, True, 0),
+    (1, 40, 1100, 2, 2, 8, True, 0),
+    # dS^T kept: heads of 128 and 256, whole and ragged blocks, a window, queries without keys
+    (1, 700, 700, 4, 2, 128, True, 0),
+    (2, 260, 390, 6, 2, 256, True, 0),
+    (1, 500, 500, 2, 1, 128, True, 70),
+    (1, 400, 300, 2, 2, 256, True, 130),
+    (1, 333, 200, 4, 1, 128, False, 0),
+    (1, 200, 450, 3, 1, 200, False, 0),
+]
+
+
+@pytest.mark.parametrize("b,lq,lk,hq,hk,d,causal,window", CUT)
+def test_cut_and_kept(b, lq, lk, hq, hk, d, causal, window):
+    print(f"case cut {(b, lq, lk, hq, hk, d, causal, window)}", flush=True)
+    q, do = rnd(1, b, lq, hq, d), rnd(4, b, lq, hq, d)
+    k, v = rnd(2, b, lk, hk, d), rnd(3, b, lk, hk, d)
+    run(q, k, v, do, [Dense(i, lk) for i in range(b)], hq, hk, causal, window, 1.0 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("d", [128, 256])
+def test_packed_many(d):
+    """Packed sequences of every length around the tiles, their kept dS^T beside one another."""
+    lens = [1, 63, 64, 65, 127, 128, 129, 7, 0, 250, 33, 2]
+    at = torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+    n = sum(lens)
+    q, k, v, do = rnd(1, n, 4, d), rnd(2, n, 2, d), rnd(3, n, 2, d), rnd(4, n, 4, d)
+    seqs = [Packed(int(at[i]), int(at[i + 1]), int(at[i]), int(at[i + 1])) for i in range(len(lens))]
+    run(q, k, v, do, seqs, 4, 2, True, 0, 1.0 / math.sqrt(d), q_starts=at, kv_starts=at, max_q=250, max_kv=250)
+
+
+@pytest.mark.parametrize("heads,n,d", [(16, 8300, 256), (16, 4300, 128)])
+def test_too_long_to_keep(heads, n, d):
+    """dS^T past what is kept: the probabilities are computed again. Two heads are checked, at rows of every part."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    q, k, v, do = (rnd(i, 1, n, heads, d) for i in range(1, 5))
+    out, lse = attention_fwd(q, k, v)
+    grads = attention_bwd(q, k, v, out, lse, do)
+    for h in (0, heads - 1):
+        one = [t[0, :, h:h + 1].double() for t in (q, k, v, do)]
+        r = R.reference([tuple(one)], 1, 1, True, 0, 1.0 / math.sqrt(d), R.HALF[BF], R.HALF[BF])[0]
+        close(out[0, :, h:h + 1], *r["out"], f"out of head {h}")
+        for name, g in zip(("dq", "dk", "dv"), grads):
+            close(g[0, :, h:h + 1], *r[name], f"{name} of head {h}")
+
+
+def test_ragged_cache_of_many_keys():
+    """A serving batch whose lengths differ by thousands: ranges with nothing in them, and places never written."""
+    lens = [3000, 1, 0, 1025, 2047, 130]
+    q, k, v = rnd(1, 6, 1, 8, 256), rnd(2, 6, 3000, 2, 256), rnd(3, 6, 3000, 2, 256)
+    for i, n in enumerate(lens):
+        k[i, n:] = float("nan")
+        v[i, n:] = float("nan")
+    run(q, k, v, None, [Dense(i, n) for i, n in enumerate(lens)], 8, 2, True, 0, 0.06, back=False,
+        kv_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+
+
+def test_workspace_of_a_larger_call_and_full_of_nan():
+    """A workspace holds nothing between calls: one full of NaN, and larger than asked for, gives the same bits."""
+    from r9700training_amd import lib
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    for lq, lk, d in ((700, 700, 128), (40, 2000, 128), (1, 4000, 256), (300, 300, 64)):
+        q, k, v, do = rnd(1, 1, lq, 8, d), rnd(2, 1, lk, 2, d), rnd(3, 1, lk, 2, d), rnd(4, 1, lq, 8, d)
+        out, lse = attention_fwd(q, k, v)
+        grads = attention_bwd(q, k, v, out, lse, do)
+        ws = torch.full((1 << 26,), float("nan"), device="cuda").view(torch.uint8)
+        o2, l2 = attention_fwd(q, k, v, workspace=ws)
+        assert torch.equal(out, o2) and torch.equal(lse, l2)
+        ws.view(torch.float32).fill_(float("nan"))
+        g2 = attention_bwd(q, k, v, out, lse, do, workspace=ws)
+        assert all(torch.equal(x, y) for x, y in zip(grads, g2))
+    assert lib() is not None
+
+
+def test_kept_graph_and_stream():
+    """The backward that keeps dS^T, on another stream and replayed from a graph with eager work between the replays."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    q, k, v, do = rnd(1, 2, 500, 8, 128), rnd(2, 2, 500, 2, 128), rnd(3, 2, 500, 2, 128), rnd(4, 2, 500, 8, 128)
+
+    def step(**kw):
+        out, lse = attention_fwd(q, k, v, **kw)
+        return (out, lse) + attention_bwd(q, k, v, out, lse, do, **kw)
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = step(stream=side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (21, 22, 23):
+        do.copy_(rnd(seed, 2, 500, 8, 128))
+        want = [x.clone() for x in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(want, held)), seed
