@@ -8,9 +8,9 @@
 //
 // Bound by memory: a row is read once into registers (8 consecutive columns a thread and step), its sums
 // taken across the threads, and everything written from there. Rows of up to 2048 columns belong to a
-// wave, four of them to a workgroup, with no barrier; wider ones, up to 16384 columns, to a workgroup. Wider
-// rows, odd widths, groups that do not fall on lanes and unaligned tensors take the general kernels, which read
-// a row again for each stage.
+// wave, four of them to a workgroup, with no barrier; wider ones, up to 16384 columns, to a workgroup. Odd widths,
+// groups that do not fall on lanes and unaligned tensors go a column at a time, up to 8192 of them; what is wider
+// takes the general kernels, which read a row again for each stage.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -56,7 +56,7 @@ __device__ __forceinline__ float ld(const void* p, int64_t i) {
 template <class T>
 __device__ __forceinline__ void put(void* p, int64_t i, float v) {
     if constexpr (sizeof(T) == 2)
-        static_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
+        static_cast<uint16_t*>(p)[i] = __builtin_bit_cast(uint16_t, (__bf16)v);
     else
         static_cast<float*>(p)[i] = v;
 }
@@ -141,6 +141,9 @@ struct Quant {
         inv = amax > 0.0f ? 127.0f / (amax * up) : 0.0f;
     }
     __device__ __forceinline__ int code(float y) const { return (int)rintf(y * up * inv); }
+    // in one word: up is one of two, and inv is not negative
+    __device__ __forceinline__ float packed() const { return up == 1.0f ? inv : -inv; }
+    static __device__ __forceinline__ int code_of(float y, float p) { return (int)rintf(y * (p < 0.0f ? 0x1p96f : 1.0f) * fabsf(p)); }
 };
 
 // The codes' cotangent at y, gc / scale, plus y's own. The two may cancel, so the quotient's rounding is
@@ -220,14 +223,26 @@ __global__ __launch_bounds__(kThreads) void norm_any_bwd_kernel(NArgs a) {
 }
 
 // ---------------------------------------------------------------- rows in registers
-// A row belongs to a wave (WIDE false, four to a workgroup) or to the workgroup. A thread holds S pieces of 8
-// columns, 8 * (threads a row) apart, so a wave's 64 pieces are 512 neighbouring columns and a group of
-// 8 .. 512 columns (a power of two) lies in 2^lg neighbouring lanes. lg < 0: one group, the whole row.
+// A row belongs to a wave (WIDE false, four to a workgroup) or to the workgroup. A thread holds S pieces of V columns,
+// V * (threads a row) apart. V 8: 16 bytes of bf16 a load; a wave's 64 pieces are 512 neighbouring columns and a group
+// of 8 .. 512 columns (a power of two) lies in 2^lg neighbouring lanes. V 1, where widths or places do not allow that: a
+// wave's pieces are 64 neighbouring columns, and a group's maximum is gathered in LDS (a maximum is the same in any
+// order). lg kWhole: one group, the whole row; kGathered: through LDS.
 constexpr int kMostWaves = 16;
+constexpr int kWhole = -1, kGathered = -2;
 
-template <class T>
-__device__ __forceinline__ void store_piece(void* p, int64_t i, const float (&x)[8]) {
-    if constexpr (sizeof(T) == 2) {
+template <class T, int V>
+__device__ __forceinline__ void load_piece(const void* p, int64_t i, float (&x)[V]) {
+    if constexpr (V == 8)
+        lanes::load8(static_cast<const T*>(p) + i, x);
+    else
+        x[0] = ld<T>(p, i);
+}
+template <class T, int V>
+__device__ __forceinline__ void store_piece(void* p, int64_t i, const float (&x)[V]) {
+    if constexpr (V == 1) {
+        put<T>(p, i, x[0]);
+    } else if constexpr (sizeof(T) == 2) {
         using b2 = __attribute__((ext_vector_type(2))) __bf16;
         uint32_t u[4];
 #pragma unroll
@@ -240,68 +255,118 @@ __device__ __forceinline__ void store_piece(void* p, int64_t i, const float (&x)
         lanes::store8(static_cast<float*>(p) + i, x);
     }
 }
-template <class T>
-__device__ __forceinline__ void load_piece(const void* p, int64_t i, float (&x)[8]) {
-    lanes::load8(static_cast<const T*>(p) + i, x);
-}
 
-template <class T, int S, bool WIDE>
-__global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, int lg) {
+template <class T, int S, bool WIDE, int V>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, int lg, uint32_t magic) {
     __shared__ float red[kMostWaves];
+    extern __shared__ uint32_t gathered[];  // the groups' maxima, as bits (they are not negative), then their quantisers
     const int wave = threadIdx.x >> 6, t = WIDE ? threadIdx.x : threadIdx.x & 63, per = WIDE ? blockDim.x : 64;
     const int64_t row = WIDE ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (row >= a.rows) return;
     const int n = (int)a.n;
     const int64_t base = row * n;
-    float h[S][8];
+    float h[S][V];
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-        const int c = 8 * (t + i * per);
+        const int c = V * (t + i * per);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) h[i][k] = 0.0f;
-        if (c < n) load_piece<T>(a.x, base + c, h[i]);
+        for (int k = 0; k < V; ++k) h[i][k] = 0.0f;
+        if (c < n) load_piece<T, V>(a.x, base + c, h[i]);
     }
     if (a.res) {
-        float r[S][8];
+        float r[S][V];
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const int c = 8 * (t + i * per);
+            const int c = V * (t + i * per);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) r[i][k] = 0.0f;
-            if (c < n) load_piece<T>(a.res, base + c, r[i]);
+            for (int k = 0; k < V; ++k) r[i][k] = 0.0f;
+            if (c < n) load_piece<T, V>(a.res, base + c, r[i]);
         }
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const int c = 8 * (t + i * per);
+            const int c = V * (t + i * per);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) h[i][k] = as_stored<T>(h[i][k] + r[i][k]);
-            if (c < n) store_piece<T>(a.h, base + c, h[i]);
+            for (int k = 0; k < V; ++k) h[i][k] = as_stored<T>(h[i][k] + r[i][k]);
+            if (c < n) store_piece<T, V>(a.h, base + c, h[i]);
         }
     }
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) ss += h[i][k] * h[i][k];
+        for (int k = 0; k < V; ++k) ss += h[i][k] * h[i][k];
     ss = WIDE ? block_sum(ss, red) : wave_sum(ss);
     const float rs = 1.0f / sqrtf(ss / (float)n + a.eps);
     if (t == 0 && a.rstd) a.rstd[row] = rs;
     float top[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-        const int c = 8 * (t + i * per);
-        float w[8] = {};
-        if (c < n) load_piece<T>(a.w, c, w);
+        const int c = V * (t + i * per);
+        float w[V] = {};
+        if (c < n) load_piece<T, V>(a.w, c, w);
         top[i] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < V; ++k) {
             h[i][k] = h[i][k] * rs * (w[k] + a.wadd);
             top[i] = fmaxf(top[i], fabsf(h[i][k]));
         }
-        if (a.y && c < n) store_piece<uint16_t>(a.y, base + c, h[i]);
+        if (a.y && c < n) store_piece<uint16_t, V>(a.y, base + c, h[i]);
     }
     if (!a.codes) return;
-    if (lg < 0) {
+    const int group = (int)a.group;
+    if constexpr (V == 1) {
+        float q[S];  // the columns' quantisers
+        if (lg == kWhole) {
+#pragma unroll
+            for (int i = 1; i < S; ++i) top[0] = fmaxf(top[0], top[i]);
+            const Quant one(block_max(top[0], red));
+            if (t == 0) a.scale[row] = one.scale;
+#pragma unroll
+            for (int i = 0; i < S; ++i) q[i] = one.packed();
+        } else {
+            const int ngroups = (int)a.ngroups;
+            for (int i = t; i < ngroups; i += per) gathered[i] = 0;
+            __syncthreads();
+            // a wave's 64 columns lie in one group, or two, where those are as wide, and the wave takes their maxima first;
+            // of narrower ones a lane its own
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                const int c = t + i * per, g = (int)__umulhi((uint32_t)c, magic);
+                if (group % 64 == 0) {
+                    const float m = wave_max(top[i]);
+                    if ((t & 63) == 0 && c < n) atomicMax(&gathered[g], __builtin_bit_cast(uint32_t, m));
+                } else if (group > 64) {
+                    const int g0 = __builtin_amdgcn_readfirstlane(g);
+                    const float m0 = wave_max(g == g0 ? top[i] : 0.0f), m1 = wave_max(g == g0 ? 0.0f : top[i]);
+                    if ((t & 63) == 0 && c < n) {
+                        atomicMax(&gathered[g0], __builtin_bit_cast(uint32_t, m0));
+                        if (g0 + 1 < ngroups) atomicMax(&gathered[g0 + 1], __builtin_bit_cast(uint32_t, m1));
+                    }
+                } else if (c < n) {
+                    atomicMax(&gathered[g], __builtin_bit_cast(uint32_t, top[i]));
+                }
+            }
+            __syncthreads();
+            for (int i = t; i < ngroups; i += per) {
+                const Quant g(__builtin_bit_cast(float, gathered[i]));
+                a.scale[row * ngroups + i] = g.scale;
+                gathered[i] = __builtin_bit_cast(uint32_t, g.packed());
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                const int c = t + i * per;
+                q[i] = __builtin_bit_cast(float, gathered[__umulhi((uint32_t)(c < n ? c : 0), magic)]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int c = t + i * per;
+            if (c < n) a.codes[base + c] = (int8_t)Quant::code_of(h[i][0], q[i]);
+        }
+        return;
+    }
+    if (lg == kWhole) {
 #pragma unroll
         for (int i = 1; i < S; ++i) top[0] = fmaxf(top[0], top[i]);
         top[0] = WIDE ? block_max(top[0], red) : wave_max(top[0]);
@@ -313,61 +378,61 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
     }
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-        const int c = 8 * (t + i * per);
+        const int c = V * (t + i * per);
         if (c >= n) continue;
         const Quant q(top[i]);
         uint32_t b[2] = {0, 0};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) b[k >> 2] |= (uint32_t)(q.code(h[i][k]) & 255) << (8 * (k & 3));
+        for (int k = 0; k < V; ++k) b[(k >> 2) & 1] |= (uint32_t)(q.code(h[i][k]) & 255) << (8 * (k & 3));
         *reinterpret_cast<uint2*>(a.codes + base + c) = make_uint2(b[0], b[1]);
-        if (lg < 0 ? t == 0 && i == 0 : (t & ((1 << lg) - 1)) == 0) a.scale[row * a.ngroups + (lg < 0 ? 0 : c >> (lg + 3))] = q.scale;
+        if (lg == kWhole ? c == 0 : c % group == 0) a.scale[row * a.ngroups + (lg == kWhole ? 0 : c >> (lg + 3))] = q.scale;
     }
 }
 
 // The adjoint: a wave or workgroup walks rows and keeps its columns' sums of dw in registers.
-template <class T, int S, bool WIDE>
-__global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs a, int lg) {
+template <class T, int S, bool WIDE, int V>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs a, int lg, uint32_t magic) {
     __shared__ float red[kMostWaves];
-    __shared__ float sums[WIDE ? 1 : 4 * 512 * S];
+    __shared__ float sums[WIDE ? 1 : 4 * 64 * V * S];
     const int wave = threadIdx.x >> 6, t = WIDE ? threadIdx.x : threadIdx.x & 63, per = WIDE ? blockDim.x : 64;
     const int n = (int)a.n;
     const int64_t first = WIDE ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave, step = WIDE ? gridDim.x : (int64_t)gridDim.x * 4;
-    float dw[S][8] = {};
+    float dw[S][V] = {};
     for (int64_t row = first; row < a.rows; row += step) {
         const int64_t base = row * n;
         const float rs = a.rstd[row];
-        float x[S][8], e[S][8], gh[S][8];
+        float x[S][V], e[S][V], gh[S][V];
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const int c = 8 * (t + i * per);
+            const int c = V * (t + i * per);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[i][k] = e[i][k] = gh[i][k] = 0.0f;
+            for (int k = 0; k < V; ++k) x[i][k] = e[i][k] = gh[i][k] = 0.0f;
             if (c < n) {
-                load_piece<T>(a.x, base + c, x[i]);
-                if (a.gy) load_piece<T>(a.gy, base + c, e[i]);
-                if (a.gh) load_piece<T>(a.gh, base + c, gh[i]);
+                load_piece<T, V>(a.x, base + c, x[i]);
+                if (a.gy) load_piece<T, V>(a.gy, base + c, e[i]);
+                if (a.gh) load_piece<T, V>(a.gh, base + c, gh[i]);
             }
         }
         if (a.gc) {
 #pragma unroll
             for (int i = 0; i < S; ++i) {
-                const int c = 8 * (t + i * per);
+                const int c = V * (t + i * per);
                 if (c >= n) continue;
-                float gc[8];
-                load_piece<T>(a.gc, base + c, gc);
-                const Cotangent q(a.scale[row * a.ngroups + (lg < 0 ? 0 : c >> (lg + 3))]);
+                float gc[V];
+                load_piece<T, V>(a.gc, base + c, gc);
+                const Cotangent q(a.scale[row * a.ngroups + (lg == kWhole ? 0 : lg >= 0 ? c >> (lg + 3) : (int)__umulhi((uint32_t)c, magic))]);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) e[i][k] = q.sum(gc[k], e[i][k]);
+                for (int k = 0; k < V; ++k) e[i][k] = q.sum(gc[k], e[i][k]);
             }
         }
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const int c = 8 * (t + i * per);
-            float w[8] = {};
-            if (c < n) load_piece<T>(a.w, c, w);
+            const int c = V * (t + i * per);
+            float w[V] = {};
+            if (c < n) load_piece<T, V>(a.w, c, w);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < V; ++k) {
                 x[i][k] *= rs;
                 dw[i][k] += e[i][k] * x[i][k];
                 e[i][k] *= w[k] + a.wadd;
@@ -377,11 +442,11 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs 
         const float mean = (WIDE ? block_sum(dot, red) : wave_sum(dot)) / (float)n;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const int c = 8 * (t + i * per);
+            const int c = V * (t + i * per);
             if (c >= n) continue;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) gh[i][k] += rs * (e[i][k] - x[i][k] * mean);
-            store_piece<T>(a.dx, base + c, gh[i]);
+            for (int k = 0; k < V; ++k) gh[i][k] += rs * (e[i][k] - x[i][k] * mean);
+            store_piece<T, V>(a.dx, base + c, gh[i]);
         }
     }
     if (!a.part) return;
@@ -389,14 +454,15 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs 
     if constexpr (WIDE) {
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const int c = 8 * (t + i * per);
-            if (c < n) lanes::store8(part + c, dw[i]);
+            const int c = V * (t + i * per);
+            if (c < n) store_piece<float, V>(part, c, dw[i]);
         }
     } else {
+        constexpr int W = 64 * V * S;
 #pragma unroll
-        for (int i = 0; i < S; ++i) lanes::store8(sums + (wave * S + i) * 512 + 8 * t, dw[i]);
+        for (int i = 0; i < S; ++i) store_piece<float, V>(sums, wave * W + i * 64 * V + V * t, dw[i]);
         __syncthreads();
-        for (int c = threadIdx.x; c < n; c += 256) part[c] = (sums[c] + sums[512 * S + c]) + (sums[1024 * S + c] + sums[1536 * S + c]);
+        for (int c = threadIdx.x; c < n; c += 256) part[c] = (sums[c] + sums[W + c]) + (sums[2 * W + c] + sums[3 * W + c]);
     }
 }
 
@@ -423,32 +489,45 @@ __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__
     }
 }
 
-// how the rows are taken: 0 the general kernels, else pieces a thread; threads of a workgroup; lanes of a group
+// how the rows are taken: pieces a thread (0: the general kernels) of `columns` each, threads of a workgroup, and how
+// the groups' maxima are found
 struct Rows {
-    int pieces, threads, lg;
+    int pieces, columns, threads, lg;
     bool wide;
 };
 Rows rows_plan(int64_t n, int64_t group, std::initializer_list<const void*> tensors) {
     Rows r = {};
-    if (n % 8 || n > 16384) return r;
-    for (const void* p : tensors)
-        if (!lanes::aligned16(p)) return r;
-    r.lg = group >= n ? -1 : lanes::group_log(group) - 3;
-    if (group < n && lanes::group_log(group) < 0) return r;
-    r.wide = n > 2048;
-    r.pieces = r.wide ? 2 : (int)((n + 511) / 512);
-    r.threads = r.wide ? 64 * (int)((n + 1023) / 1024) : 256;
+    bool eight = n % 8 == 0 && n <= 16384 && (group >= n || lanes::group_log(group) >= 0);
+    for (const void* p : tensors) eight = eight && lanes::aligned16(p);
+    if (eight) {
+        r.lg = group >= n ? kWhole : lanes::group_log(group) - 3;
+        r.columns = 8;
+        r.wide = n > 2048;
+        r.pieces = r.wide ? 2 : (int)((n + 511) / 512);
+        r.threads = r.wide ? 64 * (int)((n + 1023) / 1024) : 256;
+    } else if (n <= 8192 && (group > 1 || n == 1)) {
+        r.lg = group >= n ? kWhole : kGathered;
+        r.columns = 1;
+        r.wide = true;
+        r.pieces = n <= 2048 ? 4 : 8;
+        r.threads = 64 * (int)((n + 64 * r.pieces - 1) / (64 * r.pieces));
+    }
     return r;
 }
-// f(a kernel's pieces, whether the row is a workgroup's)
+// a column's group is its product with this, over 2^32: exact for columns and groups below 2^14. (One group: not used.)
+uint32_t group_magic(int64_t group) { return group > 1 && group < (1 << 14) ? (uint32_t)((1ULL << 32) / (uint64_t)group + 1) : 0; }
+// f(a kernel's pieces, whether the row is a workgroup's, a piece's columns)
 template <class F>
 void with_rows(const Rows& r, F&& f) {
     using std::integral_constant;
-    if (r.wide) return f(integral_constant<int, 2>{}, std::true_type{});
-    if (r.pieces == 1) return f(integral_constant<int, 1>{}, std::false_type{});
-    if (r.pieces == 2) return f(integral_constant<int, 2>{}, std::false_type{});
-    if (r.pieces == 3) return f(integral_constant<int, 3>{}, std::false_type{});
-    return f(integral_constant<int, 4>{}, std::false_type{});
+    const integral_constant<int, 8> eight;
+    const integral_constant<int, 1> one;
+    if (r.columns == 1) return r.pieces == 4 ? f(integral_constant<int, 4>{}, std::true_type{}, one) : f(eight, std::true_type{}, one);
+    if (r.wide) return f(integral_constant<int, 2>{}, std::true_type{}, eight);
+    if (r.pieces == 1) return f(one, std::false_type{}, eight);
+    if (r.pieces == 2) return f(integral_constant<int, 2>{}, std::false_type{}, eight);
+    if (r.pieces == 3) return f(integral_constant<int, 3>{}, std::false_type{}, eight);
+    return f(integral_constant<int, 4>{}, std::false_type{}, eight);
 }
 
 int64_t bwd_parts(int64_t rows) { return rows < 512 ? rows : 512; }
@@ -501,12 +580,14 @@ int r97q_add_rmsnorm_i8g(const void* x, const void* residual, const void* w, int
     a.rstd = rstd;
     const Rows r = rows_plan(n, a.group, {x, residual, w, h_out, codes, y_out});
     if (r.pieces) {
-        with_rows(r, [&](auto pieces, auto wide) {
+        with_rows(r, [&](auto pieces, auto wide, auto columns) {
             const dim3 grid((unsigned)(wide ? rows : (rows + 3) / 4)), threads(r.threads);
+            const uint32_t magic = group_magic(a.group);
+            const unsigned lds = r.lg == kGathered ? (unsigned)(4 * a.ngroups) : 0;
             if (dtype == R97Q_BF16)
-                hipLaunchKernelGGL((norm_rows_kernel<uint16_t, pieces, wide>), grid, threads, 0, (hipStream_t)stream, a, r.lg);
+                hipLaunchKernelGGL((norm_rows_kernel<uint16_t, pieces, wide, columns>), grid, threads, lds, (hipStream_t)stream, a, r.lg, magic);
             else
-                hipLaunchKernelGGL((norm_rows_kernel<float, pieces, wide>), grid, threads, 0, (hipStream_t)stream, a, r.lg);
+                hipLaunchKernelGGL((norm_rows_kernel<float, pieces, wide, columns>), grid, threads, lds, (hipStream_t)stream, a, r.lg, magic);
         });
         return launch_status("norm_rows_kernel");
     }
@@ -555,12 +636,13 @@ int r97q_add_rmsnorm_i8g_bwd(const void* h, const void* w, int32_t dtype, int64_
         // four rows at a time a workgroup where a row is a wave's
         const int64_t most = r.wide ? rows : (rows + 3) / 4;
         if (parts > most) parts = most;
-        with_rows(r, [&](auto pieces, auto wide) {
+        with_rows(r, [&](auto pieces, auto wide, auto columns) {
             const dim3 grid((unsigned)(dw ? parts : most)), threads(r.threads);
+            const uint32_t magic = group_magic(a.group);
             if (dtype == R97Q_BF16)
-                hipLaunchKernelGGL((norm_rows_bwd_kernel<uint16_t, pieces, wide>), grid, threads, 0, st, a, r.lg);
+                hipLaunchKernelGGL((norm_rows_bwd_kernel<uint16_t, pieces, wide, columns>), grid, threads, 0, st, a, r.lg, magic);
             else
-                hipLaunchKernelGGL((norm_rows_bwd_kernel<float, pieces, wide>), grid, threads, 0, st, a, r.lg);
+                hipLaunchKernelGGL((norm_rows_bwd_kernel<float, pieces, wide, columns>), grid, threads, 0, st, a, r.lg, magic);
         });
         if (int e = launch_status("norm_rows_bwd_kernel")) return e;
     } else if (rows > 0) {

@@ -190,3 +190,24 @@ def test_no_rows():
     assert codes.shape == (0, 256) and scale.shape == (0, 2)
     dx, dw = add_rmsnorm_i8g_bwd(x, w, rs, 128, g_y=x)
     assert dx.shape == (0, 256) and float(dw.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("rows,n,group", [(3, 100, 1), (4, 65, 64), (5, 200, 96), (2, 8191, 100), (3, 8192, 65), (2, 8193, 128), (6, 2049, 63),
+                                          (7, 1, 0), (3, 513, 512), (2, 5119, 2), (300, 1001, 128), (2, 4100, 4096)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_column_at_a_time(rows, n, group, dtype):
+    """Widths and groups off the 16-byte pieces: groups of one column, of just over a wave's, that end inside one."""
+    from r9700training_amd.norm import add_rmsnorm_i8g_bwd
+
+    print(f"case norm columns {(rows, n, group, dtype)}", flush=True)
+    forward(rows, n, group, dtype, residual=False, wadd=1.0)
+    _, _, w, _, scale, h, _, rs = forward(rows, n, group, dtype)
+    gc, gh = rnd(4, rows, n, dtype=dtype, std=0.01), rnd(6, rows, n, dtype=dtype)
+    dx, dw = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale, g_codes=gc, g_h=gh)
+    wdx, wdw, e = R.norm_backward(h.double(), rs.double(), w, 0.0, scale, group, gc, None, gh)
+    we, x = (w.double() * e).abs(), (h.double() * rs.double()[:, None]).abs()
+    tol = rs.double()[:, None] * (8 * R.U32 * we + (n + 16) * R.U32 * x * (we * x).mean(1, keepdim=True)) + 8 * R.U32 * wdx.abs()
+    assert bool(((dx.double() - wdx).abs() <= tol + R.HALF[dtype] * wdx.abs() + 1e-30).all())
+    assert bool(((dw.double() - wdw).abs() <= (rows + 8) * R.U32 * (e * x).abs().sum(0) + 1e-30).all())
+    again = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale, g_codes=gc, g_h=gh)
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
