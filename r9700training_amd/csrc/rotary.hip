@@ -43,21 +43,29 @@ struct RArgs {
     float mscale;
 };
 
-template <class T, int V>
+// V values, in one load where they are aligned (WIDE)
+template <class T, int V, bool WIDE>
 struct Piece {
+    static constexpr int kBytes = V * (int)sizeof(T);
     float x[V];
     __device__ __forceinline__ void load(const T* p) {
-        if constexpr (V == 8) {  // bf16
-            const uint4 w = *reinterpret_cast<const uint4*>(p);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        if constexpr (WIDE && sizeof(T) == 2 && V > 1) {
+            uint32_t u[V / 2];
+            if constexpr (kBytes == 16)
+                *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(p);
+            else if constexpr (kBytes == 8)
+                *reinterpret_cast<uint2*>(u) = *reinterpret_cast<const uint2*>(p);
+            else
+                u[0] = *reinterpret_cast<const uint32_t*>(p);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < V / 2; ++i) {
                 x[2 * i] = __builtin_bit_cast(float, u[i] << 16);
                 x[2 * i + 1] = __builtin_bit_cast(float, u[i] & 0xFFFF0000u);
             }
-        } else if constexpr (V == 4) {  // f32
-            const float4 w = *reinterpret_cast<const float4*>(p);
-            x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+        } else if constexpr (WIDE && kBytes == 16) {
+            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+        } else if constexpr (WIDE && kBytes == 8) {
+            *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(p);
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -69,17 +77,24 @@ struct Piece {
         }
     }
     __device__ __forceinline__ void store(T* p) const {
-        if constexpr (V == 8) {
+        if constexpr (WIDE && sizeof(T) == 2 && V > 1) {
             using b2 = __attribute__((ext_vector_type(2))) __bf16;
-            uint32_t u[4];
+            uint32_t u[V / 2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < V / 2; ++i) {
                 b2 v = {(__bf16)x[2 * i], (__bf16)x[2 * i + 1]};
                 u[i] = __builtin_bit_cast(uint32_t, v);
             }
-            *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-        } else if constexpr (V == 4) {
-            *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+            if constexpr (kBytes == 16)
+                *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(u);
+            else if constexpr (kBytes == 8)
+                *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(u);
+            else
+                *reinterpret_cast<uint32_t*>(p) = u[0];
+        } else if constexpr (WIDE && kBytes == 16) {
+            *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(x);
+        } else if constexpr (WIDE && kBytes == 8) {
+            *reinterpret_cast<float2*>(p) = *reinterpret_cast<const float2*>(x);
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -92,9 +107,10 @@ struct Piece {
     }
 };
 
-// V: values a piece (16 bytes; or 1, and 2 for a neighbouring pair, where widths or places do not allow
-// that). NEAR: neighbouring pairs, else the halves' ones.
-template <class T, int V, bool NEAR>
+// V: values a piece: 16 bytes, or as many fewer as widths and places allow, down to one (a neighbouring pair: two, one by
+// one). 16384 tokens, 10 heads of 96 of which 24 turn in halves of 12: 73 us a value at a time, 23 in 8 bytes.
+// NEAR: neighbouring pairs, else the halves' ones.
+template <class T, int V, bool NEAR, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RArgs a) {
     __shared__ float2 table[kTable];  // (cos, sin) * mscale
     const int64_t t0 = (int64_t)blockIdx.x * a.tpb;
@@ -112,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RArgs a) {
     __syncthreads();
     const int per = a.turn + a.copy, n = nt * a.heads * per, step = kThreads * (int)gridDim.y;
     for (int i0 = (int)blockIdx.y * kThreads + threadIdx.x; i0 < n; i0 += kItems * step) {
-        Piece<T, V> u[kItems], v[kItems];
+        Piece<T, V, WIDE> u[kItems], v[kItems];
         T* out[kItems];
         int at[kItems];  // the piece's first pair in the table; -1: copied
 #pragma unroll
@@ -162,8 +178,8 @@ int refuse(int code, const char* why) {
     return code;
 }
 
-bool on16(const R97qHeads* t, int unit) {
-    return (reinterpret_cast<uintptr_t>(t->data) & 15) == 0 && t->token_stride % unit == 0 && t->head_stride % unit == 0;
+bool on(const R97qHeads* t, int unit, int size) {  // pieces of `unit` values are aligned
+    return (reinterpret_cast<uintptr_t>(t->data) & (unit * size - 1)) == 0 && t->token_stride % unit == 0 && t->head_stride % unit == 0;
 }
 
 int check_pair(const R97qHeads* in, const R97qHeads* out, int32_t dtype, int64_t tokens) {
@@ -176,7 +192,7 @@ int check_pair(const R97qHeads* in, const R97qHeads* out, int32_t dtype, int64_t
     return R97Q_OK;
 }
 
-template <class T, int V, bool NEAR>
+template <class T, int V, bool NEAR, bool WIDE>
 int launch(RArgs a, int32_t head_dim, bool in_place, hipStream_t st) {
     a.turn = 2 * a.half / (NEAR ? V : 2 * V);
     a.copy = in_place ? 0 : (head_dim - 2 * a.half) / V;
@@ -192,15 +208,19 @@ int launch(RArgs a, int32_t head_dim, bool in_place, hipStream_t st) {
     int64_t across = 1;
     if (blocks < 256) across = (per * tpb + kThreads - 1) / kThreads;
     if (across > 256) across = 256;
-    hipLaunchKernelGGL((rotary_kernel<T, V, NEAR>), dim3((unsigned)blocks, (unsigned)(across < 1 ? 1 : across)),
+    hipLaunchKernelGGL((rotary_kernel<T, V, NEAR, WIDE>), dim3((unsigned)blocks, (unsigned)(across < 1 ? 1 : across)),
                        dim3(kThreads), 0, st, a);
     return launch_status("rotary_kernel");
 }
 
-template <class T, int V>
-int pick(const RArgs& a, int32_t head_dim, bool wide, bool near, bool in_place, hipStream_t st) {
-    if (near) return wide ? launch<T, V, true>(a, head_dim, in_place, st) : launch<T, 2, true>(a, head_dim, in_place, st);
-    return wide ? launch<T, V, false>(a, head_dim, in_place, st) : launch<T, 1, false>(a, head_dim, in_place, st);
+// unit: the aligned values a piece may hold (1: none but single ones)
+template <class T, bool NEAR>
+int pick(const RArgs& a, int32_t head_dim, int unit, bool in_place, hipStream_t st) {
+    if constexpr (sizeof(T) == 2)
+        if (unit == 8) return launch<T, 8, NEAR, true>(a, head_dim, in_place, st);
+    if (unit == 4) return launch<T, 4, NEAR, true>(a, head_dim, in_place, st);
+    if (unit == 2) return launch<T, 2, NEAR, true>(a, head_dim, in_place, st);
+    return launch<T, NEAR ? 2 : 1, NEAR, false>(a, head_dim, in_place, st);
 }
 
 }  // namespace
@@ -228,15 +248,19 @@ int r97q_rotary(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, 
     const int64_t heads = (int64_t)q->heads + (k ? k->heads : 0);
     if (heads * head_dim > 0x3FFFFFFF / 4) return refuse(R97Q_EUNSUPPORTED, "a token's heads pass 28 bits");
     if (tokens == 0) return R97Q_OK;
-    const int unit = q->dtype == R97Q_F32 ? 4 : 8;
-    bool wide = on16(q, unit) && on16(q_out, unit) && (!k || (on16(k, unit) && on16(k_out, unit)));
-    wide = wide && (near ? rot : rot / 2) % unit == 0 && head_dim % unit == 0;
+    const int size = q->dtype == R97Q_F32 ? 4 : 2;
+    int unit = 16 / size;
+    auto fits = [&](int u) {
+        return on(q, u, size) && on(q_out, u, size) && (!k || (on(k, u, size) && on(k_out, u, size))) &&
+               (near ? rot : rot / 2) % u == 0 && head_dim % u == 0;
+    };
+    while (unit > 1 && !fits(unit)) unit /= 2;
     auto same = [](const R97qHeads* x, const R97qHeads* y) {
         return x->data == y->data && x->token_stride == y->token_stride && x->head_stride == y->head_stride;
     };
     bool in_place = same(q, q_out) && (!k || same(k, k_out));
     // single values past an odd rest are copied one by one only in the halves' form: neighbouring pieces are two wide
-    if (near && !wide && (head_dim - rot) % 2) return refuse(R97Q_EUNSUPPORTED, "neighbouring pairs need an even head_dim");
+    if (near && (head_dim - rot) % 2) return refuse(R97Q_EUNSUPPORTED, "neighbouring pairs need an even head_dim");
     RArgs a = {};
     auto heads_of = [](const R97qHeads* x, const R97qHeads* y) {
         return RHeads{x->data, y->data, x->token_stride, x->head_stride, y->token_stride, y->head_stride};
@@ -252,8 +276,10 @@ int r97q_rotary(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, 
     a.pos64 = positions64;
     a.inverse = inverse;
     a.mscale = mscale;
-    if (q->dtype == R97Q_BF16) return pick<uint16_t, 8>(a, head_dim, wide, near, in_place, (hipStream_t)stream);
-    return pick<float, 4>(a, head_dim, wide, near, in_place, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    if (q->dtype == R97Q_BF16)
+        return near ? pick<uint16_t, true>(a, head_dim, unit, in_place, st) : pick<uint16_t, false>(a, head_dim, unit, in_place, st);
+    return near ? pick<float, true>(a, head_dim, unit, in_place, st) : pick<float, false>(a, head_dim, unit, in_place, st);
 }
 
 int r97q_rotary_frequencies(int32_t rot, double base, int32_t scaling, double factor, double original, double slow,

@@ -126,3 +126,20 @@ def test_no_tokens():
     f, _ = rotary_frequencies(64)
     q, k = rotary(rnd(1, 0, 4, 64), rnd(2, 0, 2, 64), f)
     assert q.shape == (0, 4, 64) and k.shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("dim,rot", [(96, 24), (90, 12), (20, 4), (66, 22), (96, 40)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_pieces_of_every_width(dim, rot, dtype):
+    """Halves and rests of 2, 4, 6, 10, 11, 12 and 20 values, and heads that begin off 16, 8 and 4 bytes."""
+    from r9700training_amd.rotary import rotary, rotary_frequencies
+
+    f, m = rotary_frequencies(rot, 1e4, "ramp", factor=8.0, original=2048.0)
+    t, hq = 50, 3
+    angles = torch.arange(t, device="cuda").double()[:, None] * f
+    for gap in (0, 1, 2, 4):
+        wide = rnd(1, t, hq, dim + gap, dtype=dtype)
+        x = wide[..., gap:]
+        for pairs in ("half", "interleaved"):
+            got = rotary(x, None, f, None, pairs=pairs, mscale=m)[0]
+            check(x, got, angles, rot, pairs, m, False, f"gap {gap} {pairs}")
