@@ -215,27 +215,11 @@ __device__ __forceinline__ void add_product(bf16x8 x, bf16x8 y, f32x16& c) {
     else
         c = mfma(x, y, c);
 }
-// x times y, y of the accumulation registers where they hold what the others have no room for (HELD): the first product of
-// a sum (FIRST) or one more, to be read a product or more later
-template <bool HELD, bool FIRST>
-__device__ __forceinline__ void product_of(bf16x8 x, const bf16x8& y, f32x16& c) {
-    if constexpr (!HELD)
-        c = FIRST ? mfma(x, y, (f32x16){}) : mfma(x, y, c);
-    else if constexpr (FIRST)
-        asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(x), "a"(y));
-    else
-        asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(x), "a"(y));
-}
-// fragments settle in whole registers of one file, or their words are gathered anew for every product
-template <bool HELD, int N>
+// fragments settle in whole registers, or their words are gathered anew for every product
+template <int N>
 __device__ __forceinline__ void settle(bf16x8 (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if constexpr (HELD)
-            asm volatile("" : "+a"(f[i]));
-        else
-            asm volatile("" : "+v"(f[i]));
-    }
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
 }
 // the sums may be read from here on, each after its own settle_sum(): otherwise all are copied out at once, and what
 // else is held has to leave the registers

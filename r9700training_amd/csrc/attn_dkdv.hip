@@ -50,8 +50,8 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
             }
         }
         load_row<D>(kv_at(a.v, a, s, hk) + 2 * (kk * a.v.ts), key < s.lk, fresh(a.d), lane, v);
-        settle<false>(v);
-        if constexpr (KEPT) settle<false>(k);
+        settle(v);
+        if constexpr (KEPT) settle(k);
         // the tokens [t0, t1) that see any of the workgroup's keys, from a tile's first
         static_assert(NW == 4, "tokens_of() is for 128 keys");
         int t0, t1;

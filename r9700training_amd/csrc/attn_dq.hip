@@ -27,7 +27,6 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
     using T = Tile<D>;
     using F = Frags<D>;
     constexpr int KT = 32, TB = KT * T::RB, n = D / 16;
-    constexpr bool ACC = false;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[7 * TB];  // keys' four slots, then the values' three
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
     const int nb = a.batch * a.hk;
@@ -64,15 +63,13 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
         int d = fresh(a.d);
         bf16x8 q[n], go[n];
         load_row<D>(q_at(a.q, a, s, head) + 2 * (tok * a.q.ts), r < rows, d, lane, q);
-        settle<ACC>(q);
-        if constexpr (ACC) pin();
+        settle(q);
         load_row<D>(q_at(a.d_o, a, s, head) + 2 * (tok * a.d_o.ts), r < rows, d, lane, go);
-        settle<false>(go);
+        settle(go);
         const uint8_t* op = q_at(a.o, a, s, head) + (a.o.f32 ? 4 : 2) * (tok * a.o.ts);
         float delta = 0.0f;
 #pragma unroll
         for (int c = 0; c < n; ++c) {
-            if (ACC && c % 4 == 0) pin();  // a few at a time: the registers are taken
             const int e = 16 * c + 8 * h;
             if (e < d) {
                 if (a.o.f32) {
@@ -122,9 +119,8 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
                 steps<n>([&](auto i) {
                     const bf16x8 now = f[i % kAhead];
                     if constexpr (i + kAhead < n) f[i % kAhead] = F::template rows<0, i + kAhead>(from);
-                    product_of<ACC, i == 0>(now, q[i], x);
+                    x = mfma(now, q[i], i == 0 ? (f32x16){} : x);
                 });
-                if constexpr (ACC) asm volatile("s_nop 15" : "+v"(x));
             };
             product(x0, rat);
             bf16x8 f[kAhead];
@@ -159,10 +155,10 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
                     if constexpr (i < n) {
                         y = mfma(now, go[i], y);
                     } else if constexpr (i < 2 * n) {
-                        product_of<ACC, i == n>(now, q[i - n], next);
+                        next = mfma(now, q[i - n], i == n ? (f32x16){} : next);
                     } else {
                         constexpr int c = (i - 2 * n) / (D / 32), m = (i - 2 * n) % (D / 32);
-                        add_product<ACC>(now, as_bf16x8(ds[c]), dq[m]);
+                        dq[m] = mfma(now, as_bf16x8(ds[c]), dq[m]);
                     }
                     // vector work, spread: the exponentials, and from two products after y's last one dS
 #pragma unroll
@@ -185,25 +181,18 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
             }
             landed();
         }
-        settled<ACC>();
         d = fresh(a.d);
         const int hs = fresh_lane(h);
         if (a.q_splits > 1) {
             uint8_t* out = reinterpret_cast<uint8_t*>(a.dq_part + (split * a.slots + st) * d);
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                settle_sum<ACC>(dq[i]);
-                store_block(out, true, r < rows, 32 * i, d, hs, dq[i], 1.0f);
-            }
+            for (int i = 0; i < D / 32; ++i) store_block(out, true, r < rows, 32 * i, d, hs, dq[i], 1.0f);
             __syncthreads();
             continue;
         }
         uint8_t* out = q_at(a.dq, a, s, head) + (a.dq.f32 ? 4 : 2) * (tok * a.dq.ts);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            settle_sum<ACC>(dq[i]);
-            store_block(out, a.dq.f32, r < rows, 32 * i, d, hs, dq[i], a.scale);
-        }
+        for (int i = 0; i < D / 32; ++i) store_block(out, a.dq.f32, r < rows, 32 * i, d, hs, dq[i], a.scale);
         __syncthreads();
     }
 }

@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
         bf16x8 q[n];
         load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
         turn_sign<D>(a, q);
-        settle<false>(q);
+        settle(q);
         // the keys this lane's row sees, first and last
         const int first = a.window ? (int)clamp64((int64_t)row.tok + s.off - a.window + 1, 0, s.lk) : 0;
         const int last = a.causal && row.tok + s.off < s.lk - 1 ? row.tok + s.off : s.lk - 1;
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
             bf16x8 q[D / 16];
             load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
             turn_sign<D>(a, q);
-            settle<false>(q);
+            settle(q);
             landed<Loader<D, KT, 64>::N>();  // the queries have been waited for: no more than the values are left
             for (; j0 < hi; j0 += KT * NW) {
                 f32x16 x[1];
@@ -510,15 +510,14 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
 // 24; but 1300 tokens, 16 over 4 heads 28 / 35 / 45 / 57, and 512 tokens 15 / 20 / 22 / 30.
 struct Plan {
     bool few;
-    int waves, splits, chunk;
+    int splits, chunk;
     int64_t tiles;
 };
 Plan plan_of(const Args& a) {
     Plan p = {};
     const int64_t rows = (int64_t)a.lq * a.g;
     p.few = rows <= 32;
-    p.waves = 4;
-    const int tile = p.few ? 32 : 32 * p.waves;
+    const int tile = p.few ? 32 : 128;
     p.tiles = (rows + tile - 1) / tile;
     p.splits = 1;
     // the keys a tile's rows may see
