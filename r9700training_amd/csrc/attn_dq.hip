@@ -199,33 +199,46 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
 
 // ---------------------------------------------------------------- D alone
 // D and the log-sum-exp in base 2 for dK's and dV's launch, where that one goes first. grid (batch * q heads, tokens):
-// d / 8 threads a row, rounded up to a power of two.
+// d / 8 threads a row, rounded up to a power of two, kBaseRows rows each, so that their loads go out together.
+constexpr int kBaseRows = 4;
+template <bool F32>
 __global__ __launch_bounds__(256) void attn_base_kernel(Args a, int lanes) {
-    const int head = blockIdx.x % a.hq, rows = 256 / lanes, c = 8 * (threadIdx.x % lanes);
+    const int head = blockIdx.x % a.hq, rows = 256 / lanes, c = 8 * (threadIdx.x % lanes), cc = c < a.d ? c : 0;
     const Seq s = sequence(a, blockIdx.x / a.hq);
     const uint8_t *ob = q_at(a.o, a, s, head), *gb = q_at(a.d_o, a, s, head);
-    for (int64_t t0 = (int64_t)blockIdx.y * rows; t0 < s.lq; t0 += (int64_t)gridDim.y * rows) {
-        const int64_t t = t0 + threadIdx.x / lanes;
-        float sum = 0.0f;
-        if (t < s.lq && c < a.d) {
-            const bf16x8 g = as_bf16x8(*reinterpret_cast<const u32x4*>(gb + 2 * (t * a.d_o.ts + c)));
-            if (a.o.f32) {
-                const float* o = reinterpret_cast<const float*>(ob) + t * a.o.ts + c;
-                const float4 x = *reinterpret_cast<const float4*>(o), y = *reinterpret_cast<const float4*>(o + 4);
-                sum = x.x * (float)g[0] + x.y * (float)g[1] + x.z * (float)g[2] + x.w * (float)g[3];
-                sum += y.x * (float)g[4] + y.y * (float)g[5] + y.z * (float)g[6] + y.w * (float)g[7];
-            } else {
-                const bf16x8 o = as_bf16x8(*reinterpret_cast<const u32x4*>(ob + 2 * (t * a.o.ts + c)));
+    const int each = rows * kBaseRows;
+    for (int64_t t0 = (int64_t)blockIdx.y * each; t0 < s.lq; t0 += (int64_t)gridDim.y * each) {
+        const int64_t t1 = t0 + threadIdx.x / lanes;
+        u32x4 g[kBaseRows], o[kBaseRows][F32 ? 2 : 1];
+        float lse[kBaseRows];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sum += (float)o[j] * (float)g[j];
-            }
+        for (int i = 0; i < kBaseRows; ++i) {
+            const int64_t t = t1 + i * rows < s.lq ? t1 + i * rows : s.lq - 1;
+            g[i] = *reinterpret_cast<const u32x4*>(gb + 2 * (t * a.d_o.ts + cc));
+            const uint8_t* row = ob + (F32 ? 4 : 2) * (t * a.o.ts + cc);
+            o[i][0] = *reinterpret_cast<const u32x4*>(row);
+            if constexpr (F32) o[i][1] = *reinterpret_cast<const u32x4*>(row + 16);
+            lse[i] = a.lse[stat_at(a, s, head, (int)t)];
         }
-        for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        if (t < s.lq && c == 0) {
-            const int64_t at = stat_at(a, s, head, (int)t);
-            const float lse = a.lse[at];
-            a.base[at] = lse == -INFINITY ? 0.0f : lse * kLog2e;
-            a.delta[at] = -sum;
+#pragma unroll
+        for (int i = 0; i < kBaseRows; ++i) {
+            const bf16x8 x = as_bf16x8(g[i]);
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (F32)
+                    sum += __builtin_bit_cast(float, (uint32_t)o[i][j / 4][j % 4]) * (float)x[j];
+                else
+                    sum += (float)as_bf16x8(o[i][0])[j] * (float)x[j];
+            }
+            if (c >= a.d) sum = 0.0f;
+            for (int k = lanes / 2; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
+            const int64_t t = t1 + i * rows;
+            if (t < s.lq && c == 0) {
+                const int64_t at = stat_at(a, s, head, (int)t);
+                a.base[at] = lse[i] == -INFINITY ? 0.0f : lse[i] * kLog2e;
+                a.delta[at] = -sum;
+            }
         }
     }
 }
@@ -305,7 +318,9 @@ __global__ __launch_bounds__(256, PER) void attn_dq_kept_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------- partial sums added
-// grid (batch * heads, tokens, tensors): a row's partial sums in order, times the tensor's factor, to the output.
+// grid (batch * heads, tokens, tensors): a row's partial sums in order, times the tensor's factor, to the output. A thread
+// takes four columns of kSumRows rows, and four parts at once, so that their loads go out together.
+constexpr int kSumRows = 2;
 struct Sum {
     Heads out[2];
     const float* part[2];
@@ -324,19 +339,38 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(Args a, Sum u) {
     const int cover = !keys ? s.lq : a.kv_starts ? s.lk : a.lk;
     const int64_t slots = keys ? a.kv_slots : a.slots;
     if (r >= rows) return;
-    for (int64_t t = (int64_t)blockIdx.y * rows + r; t < cover; t += (int64_t)gridDim.y * rows) {
-        const int64_t at = (keys ? kv_slot(a, s, head, (int)t) : stat_at(a, s, head, (int)t)) * a.d + c;
-        float4 v = *reinterpret_cast<const float4*>(part + at);
-#pragma unroll 4
-        for (int i = 1; i < u.splits; ++i) {
-            const float4 w = *reinterpret_cast<const float4*>(part + i * slots * a.d + at);
-            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    const int each = rows * kSumRows;
+    for (int64_t t0 = (int64_t)blockIdx.y * each + r; t0 < cover; t0 += (int64_t)gridDim.y * each) {
+        int64_t at[kSumRows];
+        float4 v[kSumRows];
+#pragma unroll
+        for (int j = 0; j < kSumRows; ++j) {
+            const int t = (int)(t0 + j * rows < cover ? t0 + j * rows : t0);
+            at[j] = (keys ? kv_slot(a, s, head, t) : stat_at(a, s, head, t)) * a.d + c;
+            v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        uint8_t* row = (keys ? kv_at(out, a, s, head) : q_at(out, a, s, head)) + (out.f32 ? 4 : 2) * (t * out.ts);
-        if (out.f32)
-            *reinterpret_cast<float4*>(row + 4 * c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-        else
-            *reinterpret_cast<uint2*>(row + 2 * c) = make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
+        for (int i = 0; i < u.splits; i += 4) {
+            float4 w[kSumRows][4];
+#pragma unroll
+            for (int j = 0; j < kSumRows; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[j][k] = *reinterpret_cast<const float4*>(part + (i + k < u.splits ? i + k : i) * slots * a.d + at[j]);
+#pragma unroll
+            for (int j = 0; j < kSumRows; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (i + k < u.splits) v[j].x += w[j][k].x, v[j].y += w[j][k].y, v[j].z += w[j][k].z, v[j].w += w[j][k].w;
+        }
+#pragma unroll
+        for (int j = 0; j < kSumRows; ++j) {
+            const int64_t t = t0 + j * rows;
+            if (t >= cover) continue;
+            uint8_t* row = (keys ? kv_at(out, a, s, head) : q_at(out, a, s, head)) + (out.f32 ? 4 : 2) * (t * out.ts);
+            if (out.f32)
+                *reinterpret_cast<float4*>(row + 4 * c) = make_float4(v[j].x * f, v[j].y * f, v[j].z * f, v[j].w * f);
+            else
+                *reinterpret_cast<uint2*>(row + 2 * c) = make_uint2(pack_bf16(v[j].x * f, v[j].y * f), pack_bf16(v[j].z * f, v[j].w * f));
+        }
     }
 }
 
@@ -353,7 +387,7 @@ int run(const Args& a, hipStream_t st) {
 }  // namespace
 
 int launch_sums(const Args& a, bool keys, hipStream_t st) {
-    const int64_t tokens = keys ? a.lk : a.lq, rows = 256 / (a.d / 4), blocks = (tokens + rows - 1) / rows;
+    const int64_t tokens = keys ? a.lk : a.lq, each = 256 / (a.d / 4) * kSumRows, blocks = (tokens + each - 1) / each;
     if (blocks == 0) return R97Q_OK;
     Sum u = {{keys ? a.dk : a.dq, a.dv}, {keys ? a.dk_part : a.dq_part, a.dv_part}, {a.scale, 1.0f}, keys ? a.k_splits : a.q_splits, keys};
     hipLaunchKernelGGL(attn_sum_kernel, dim3((unsigned)(a.batch * (keys ? a.hk : a.hq)), (unsigned)(blocks < 65535 ? blocks : 65535), keys ? 2 : 1),
@@ -362,10 +396,14 @@ int launch_sums(const Args& a, bool keys, hipStream_t st) {
 }
 
 int launch_base(const Args& a, hipStream_t st) {
-    const int lanes = a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32, rows = 256 / lanes;
-    const int64_t blocks = ((int64_t)a.lq + rows - 1) / rows;
+    const int lanes = a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32, each = 256 / lanes * kBaseRows;
+    const int64_t blocks = ((int64_t)a.lq + each - 1) / each;
     if (blocks == 0) return R97Q_OK;
-    hipLaunchKernelGGL(attn_base_kernel, dim3((unsigned)(a.batch * a.hq), (unsigned)(blocks < 65535 ? blocks : 65535)), dim3(256), 0, st, a, lanes);
+    const dim3 grid((unsigned)(a.batch * a.hq), (unsigned)(blocks < 65535 ? blocks : 65535));
+    if (a.o.f32)
+        hipLaunchKernelGGL(attn_base_kernel<true>, grid, dim3(256), 0, st, a, lanes);
+    else
+        hipLaunchKernelGGL(attn_base_kernel<false>, grid, dim3(256), 0, st, a, lanes);
     return launch_status("attn_base_kernel");
 }
 
