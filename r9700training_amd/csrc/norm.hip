@@ -8,9 +8,9 @@
 //
 // Bound by memory: a row is read once into registers (8 consecutive columns a thread and step), its sums
 // taken across the threads, and everything written from there. Rows of up to 2048 columns belong to a
-// wave, four of them to a workgroup, with no barrier; wider ones, up to 16384 columns, to a workgroup. Odd widths,
-// groups that do not fall on lanes and unaligned tensors go a column at a time, up to 8192 of them; what is wider
-// takes the general kernels, which read a row again for each stage.
+// wave, four of them to a workgroup, with no barrier; wider ones, up to 16384 columns, to a workgroup. Groups that are no
+// multiple of 8 go a column at a time, up to 8192 of them; what is wider takes the general kernels, which read a row again
+// for each stage.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -224,71 +224,129 @@ __global__ __launch_bounds__(kThreads) void norm_any_bwd_kernel(NArgs a) {
 
 // ---------------------------------------------------------------- rows in registers
 // A row belongs to a wave (WIDE false, four to a workgroup) or to the workgroup. A thread holds S pieces of V columns,
-// V * (threads a row) apart. V 8: 16 bytes of bf16 a load; a wave's 64 pieces are 512 neighbouring columns and a group
-// of 8 .. 512 columns (a power of two) lies in 2^lg neighbouring lanes. V 1, where widths or places do not allow that: a
-// wave's pieces are 64 neighbouring columns, and a group's maximum is gathered in LDS (a maximum is the same in any
-// order). lg kWhole: one group, the whole row; kGathered: through LDS.
+// V * (threads a row) apart. V 8: 16 bytes of bf16 a load; a wave's 64 pieces are 512 neighbouring columns and a group of
+// 8 .. 512 columns (a power of two) lies in 2^lg neighbouring lanes; other multiples of 8 have their maximum gathered in LDS
+// (a maximum is the same in any order). LOOSE: pieces of odd widths and unaligned tensors, 16 bytes at any place and the
+// row's last piece value by value: 16384 x 1001 bf16 in groups of 128 20 us and back 29 (4.9 TB/s), where single columns took
+// 52 and 98. V 1: groups that are no multiple of 8. lg kWhole: one group, the whole row; kGathered:
+// through LDS.
 constexpr int kMostWaves = 16;
 constexpr int kWhole = -1, kGathered = -2;
 
-template <class T, int V>
-__device__ __forceinline__ void load_piece(const void* p, int64_t i, float (&x)[V]) {
-    if constexpr (V == 8)
-        lanes::load8(static_cast<const T*>(p) + i, x);
-    else
-        x[0] = ld<T>(p, i);
-}
-template <class T, int V>
-__device__ __forceinline__ void store_piece(void* p, int64_t i, const float (&x)[V]) {
-    if constexpr (V == 1) {
-        put<T>(p, i, x[0]);
-    } else if constexpr (sizeof(T) == 2) {
-        using b2 = __attribute__((ext_vector_type(2))) __bf16;
-        uint32_t u[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            b2 v = {(__bf16)x[2 * k], (__bf16)x[2 * k + 1]};
-            u[k] = __builtin_bit_cast(uint32_t, v);
-        }
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(u[0], u[1], u[2], u[3]);
-    } else {
-        lanes::store8(static_cast<float*>(p) + i, x);
-    }
-}
+// words at any place, in one access
+template <int N>
+struct __attribute__((packed)) Words {
+    uint32_t u[N];
+};
 
-template <class T, int S, bool WIDE, int V>
+// A piece as it lies in memory: it is taken apart after the branches that load it, so that all pieces' loads go out
+// together. `left` columns are left of the row from the piece's first on: LOOSE pieces may be its short last one, or (left
+// <= 0) past it. What is not there is zero.
+template <class T, int V, bool LOOSE>
+struct Piece {
+    static constexpr int N = V == 1 ? 1 : V * (int)sizeof(T) / 4;
+    uint32_t u[N];
+    __device__ __forceinline__ void load(const void* from, int64_t i, int left) {
+        const T* p = static_cast<const T*>(from) + i;
+#pragma unroll
+        for (int k = 0; k < N; ++k) u[k] = 0;
+        if constexpr (V == 1) {
+            if (left > 0) u[0] = sizeof(T) == 2 ? (uint32_t)*reinterpret_cast<const uint16_t*>(p) : *reinterpret_cast<const uint32_t*>(p);
+        } else if (left >= V) {
+#pragma unroll
+            for (int j = 0; j < N / 4; ++j) {
+                if constexpr (LOOSE) {
+                    const auto w = reinterpret_cast<const Words<4>*>(p)[j];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) u[4 * j + k] = w.u[k];
+                } else {
+                    const uint4 w = reinterpret_cast<const uint4*>(p)[j];
+                    u[4 * j] = w.x, u[4 * j + 1] = w.y, u[4 * j + 2] = w.z, u[4 * j + 3] = w.w;
+                }
+            }
+        } else if (LOOSE && left > 0) {
+#pragma unroll
+            for (int k = 0; k < V - 1; ++k) {
+                if (k >= left) break;
+                if constexpr (sizeof(T) == 2)
+                    u[k / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[k] << (16 * (k % 2));
+                else
+                    u[k] = reinterpret_cast<const uint32_t*>(p)[k];
+            }
+        }
+    }
+    __device__ __forceinline__ float at(int k) const {
+        if constexpr (sizeof(T) == 2) {
+            if constexpr (V == 1) return __builtin_bit_cast(float, u[0] << 16);
+            return __builtin_bit_cast(float, k % 2 ? u[k / 2] & 0xFFFF0000u : u[k / 2] << 16);
+        } else {
+            return __builtin_bit_cast(float, u[k]);
+        }
+    }
+    static __device__ __forceinline__ void store(void* to, int64_t i, int left, const float (&x)[V]) {
+        T* p = static_cast<T*>(to) + i;
+        if constexpr (V == 1) {
+            if (left > 0) put<T>(to, i, x[0]);
+        } else if (left >= V) {
+            uint32_t w[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                if constexpr (sizeof(T) == 2) {
+                    using b2 = __attribute__((ext_vector_type(2))) __bf16;
+                    b2 v = {(__bf16)x[2 * k], (__bf16)x[2 * k + 1]};
+                    w[k] = __builtin_bit_cast(uint32_t, v);
+                } else {
+                    w[k] = __builtin_bit_cast(uint32_t, x[k]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < N / 4; ++j) {
+                if constexpr (LOOSE)
+                    reinterpret_cast<Words<4>*>(p)[j] = {{w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]}};
+                else
+                    reinterpret_cast<uint4*>(p)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            }
+        } else if (LOOSE && left > 0) {
+#pragma unroll
+            for (int k = 0; k < V - 1; ++k)
+                if (k < left) put<T>(to, i + k, x[k]);
+        }
+    }
+};
+
+template <class T, int S, bool WIDE, int V, bool LOOSE>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, int lg, uint32_t magic) {
     __shared__ float red[kMostWaves];
-    extern __shared__ uint32_t gathered[];  // the groups' maxima, as bits (they are not negative), then their quantisers
+    extern __shared__ uint32_t gathered[];  // the groups' maxima, as bits (they are not negative); of single columns then their quantisers
     const int wave = threadIdx.x >> 6, t = WIDE ? threadIdx.x : threadIdx.x & 63, per = WIDE ? blockDim.x : 64;
     const int64_t row = WIDE ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (row >= a.rows) return;
     const int n = (int)a.n;
     const int64_t base = row * n;
+    using P = Piece<T, V, LOOSE>;
+    P x[S], w[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) x[i].load(a.x, base + V * (t + i * per), n - V * (t + i * per));
     float h[S][V];
     float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < S; ++i) {
-        const int c = V * (t + i * per);
-#pragma unroll
-        for (int k = 0; k < V; ++k) h[i][k] = 0.0f;
-        if (c < n) load_piece<T, V>(a.x, base + c, h[i]);
-    }
     if (a.res) {
-        float r[S][V];
+        P r[S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) r[i].load(a.res, base + V * (t + i * per), n - V * (t + i * per));
+#pragma unroll
+        for (int i = 0; i < S; ++i) w[i].load(a.w, V * (t + i * per), n - V * (t + i * per));
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const int c = V * (t + i * per);
 #pragma unroll
-            for (int k = 0; k < V; ++k) r[i][k] = 0.0f;
-            if (c < n) load_piece<T, V>(a.res, base + c, r[i]);
+            for (int k = 0; k < V; ++k) h[i][k] = as_stored<T>(x[i].at(k) + r[i].at(k));
+            P::store(a.h, base + V * (t + i * per), n - V * (t + i * per), h[i]);
         }
+    } else {
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            const int c = V * (t + i * per);
+            w[i].load(a.w, V * (t + i * per), n - V * (t + i * per));
 #pragma unroll
-            for (int k = 0; k < V; ++k) h[i][k] = as_stored<T>(h[i][k] + r[i][k]);
-            if (c < n) store_piece<T, V>(a.h, base + c, h[i]);
+            for (int k = 0; k < V; ++k) h[i][k] = x[i].at(k);
         }
     }
 #pragma unroll
@@ -302,62 +360,51 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
 #pragma unroll
     for (int i = 0; i < S; ++i) {
         const int c = V * (t + i * per);
-        float w[V] = {};
-        if (c < n) load_piece<T, V>(a.w, c, w);
         top[i] = 0.0f;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            h[i][k] = h[i][k] * rs * (w[k] + a.wadd);
+            h[i][k] = h[i][k] * rs * (w[i].at(k) + a.wadd);
             top[i] = fmaxf(top[i], fabsf(h[i][k]));
         }
-        if (a.y && c < n) store_piece<uint16_t, V>(a.y, base + c, h[i]);
+        if (a.y) Piece<uint16_t, V, LOOSE>::store(a.y, base + c, n - c, h[i]);
     }
     if (!a.codes) return;
     const int group = (int)a.group;
     if constexpr (V == 1) {
         float q[S];  // the columns' quantisers
-        if (lg == kWhole) {
+        const int ngroups = (int)a.ngroups;
+        for (int i = t; i < ngroups; i += per) gathered[i] = 0;
+        __syncthreads();
+        // a wave's 64 columns lie in one group, or two, where those are as wide, and the wave takes their maxima first;
+        // of narrower ones a lane its own
 #pragma unroll
-            for (int i = 1; i < S; ++i) top[0] = fmaxf(top[0], top[i]);
-            const Quant one(block_max(top[0], red));
-            if (t == 0) a.scale[row] = one.scale;
-#pragma unroll
-            for (int i = 0; i < S; ++i) q[i] = one.packed();
-        } else {
-            const int ngroups = (int)a.ngroups;
-            for (int i = t; i < ngroups; i += per) gathered[i] = 0;
-            __syncthreads();
-            // a wave's 64 columns lie in one group, or two, where those are as wide, and the wave takes their maxima first;
-            // of narrower ones a lane its own
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const int c = t + i * per, g = (int)__umulhi((uint32_t)c, magic);
-                if (group % 64 == 0) {
-                    const float m = wave_max(top[i]);
-                    if ((t & 63) == 0 && c < n) atomicMax(&gathered[g], __builtin_bit_cast(uint32_t, m));
-                } else if (group > 64) {
-                    const int g0 = __builtin_amdgcn_readfirstlane(g);
-                    const float m0 = wave_max(g == g0 ? top[i] : 0.0f), m1 = wave_max(g == g0 ? 0.0f : top[i]);
-                    if ((t & 63) == 0 && c < n) {
-                        atomicMax(&gathered[g0], __builtin_bit_cast(uint32_t, m0));
-                        if (g0 + 1 < ngroups) atomicMax(&gathered[g0 + 1], __builtin_bit_cast(uint32_t, m1));
-                    }
-                } else if (c < n) {
-                    atomicMax(&gathered[g], __builtin_bit_cast(uint32_t, top[i]));
+        for (int i = 0; i < S; ++i) {
+            const int c = t + i * per, g = (int)__umulhi((uint32_t)c, magic);
+            if (group % 64 == 0) {
+                const float m = wave_max(top[i]);
+                if ((t & 63) == 0 && c < n) atomicMax(&gathered[g], __builtin_bit_cast(uint32_t, m));
+            } else if (group > 64) {
+                const int g0 = __builtin_amdgcn_readfirstlane(g);
+                const float m0 = wave_max(g == g0 ? top[i] : 0.0f), m1 = wave_max(g == g0 ? 0.0f : top[i]);
+                if ((t & 63) == 0 && c < n) {
+                    atomicMax(&gathered[g0], __builtin_bit_cast(uint32_t, m0));
+                    if (g0 + 1 < ngroups) atomicMax(&gathered[g0 + 1], __builtin_bit_cast(uint32_t, m1));
                 }
+            } else if (c < n) {
+                atomicMax(&gathered[g], __builtin_bit_cast(uint32_t, top[i]));
             }
-            __syncthreads();
-            for (int i = t; i < ngroups; i += per) {
-                const Quant g(__builtin_bit_cast(float, gathered[i]));
-                a.scale[row * ngroups + i] = g.scale;
-                gathered[i] = __builtin_bit_cast(uint32_t, g.packed());
-            }
-            __syncthreads();
+        }
+        __syncthreads();
+        for (int i = t; i < ngroups; i += per) {
+            const Quant g(__builtin_bit_cast(float, gathered[i]));
+            a.scale[row * ngroups + i] = g.scale;
+            gathered[i] = __builtin_bit_cast(uint32_t, g.packed());
+        }
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const int c = t + i * per;
-                q[i] = __builtin_bit_cast(float, gathered[__umulhi((uint32_t)(c < n ? c : 0), magic)]);
-            }
+        for (int i = 0; i < S; ++i) {
+            const int c = t + i * per;
+            q[i] = __builtin_bit_cast(float, gathered[__umulhi((uint32_t)(c < n ? c : 0), magic)]);
         }
 #pragma unroll
         for (int i = 0; i < S; ++i) {
@@ -372,6 +419,20 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
         top[0] = WIDE ? block_max(top[0], red) : wave_max(top[0]);
 #pragma unroll
         for (int i = 1; i < S; ++i) top[i] = top[0];
+    } else if (WIDE && lg == kGathered) {
+        for (int i = t; i < (int)a.ngroups; i += per) gathered[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int c = V * (t + i * per);
+            if (c < n) atomicMax(&gathered[__umulhi((uint32_t)c, magic)], __builtin_bit_cast(uint32_t, top[i]));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int c = V * (t + i * per);
+            if (c < n) top[i] = __builtin_bit_cast(float, gathered[__umulhi((uint32_t)c, magic)]);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < S; ++i) top[i] = lanes_max(top[i], lg);
@@ -384,13 +445,22 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
         uint32_t b[2] = {0, 0};
 #pragma unroll
         for (int k = 0; k < V; ++k) b[(k >> 2) & 1] |= (uint32_t)(q.code(h[i][k]) & 255) << (8 * (k & 3));
-        *reinterpret_cast<uint2*>(a.codes + base + c) = make_uint2(b[0], b[1]);
-        if (lg == kWhole ? c == 0 : c % group == 0) a.scale[row * a.ngroups + (lg == kWhole ? 0 : c >> (lg + 3))] = q.scale;
+        if constexpr (!LOOSE) {
+            *reinterpret_cast<uint2*>(a.codes + base + c) = make_uint2(b[0], b[1]);
+        } else if (n - c >= V) {
+            *reinterpret_cast<Words<2>*>(a.codes + base + c) = {{b[0], b[1]}};
+        } else {
+#pragma unroll
+            for (int k = 0; k < V - 1; ++k)
+                if (k < n - c) a.codes[base + c + k] = (int8_t)(b[k >> 2] >> (8 * (k & 3)));
+        }
+        const int g = lg == kWhole ? 0 : lg == kGathered ? (int)__umulhi((uint32_t)c, magic) : c >> (lg + 3);
+        if (c == g * group) a.scale[row * a.ngroups + g] = q.scale;
     }
 }
 
 // The adjoint: a wave or workgroup walks rows and keeps its columns' sums of dw in registers.
-template <class T, int S, bool WIDE, int V>
+template <class T, int S, bool WIDE, int V, bool LOOSE>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs a, int lg, uint32_t magic) {
     __shared__ float red[kMostWaves];
     __shared__ float sums[WIDE ? 1 : 4 * 64 * V * S];
@@ -401,41 +471,34 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs 
     for (int64_t row = first; row < a.rows; row += step) {
         const int64_t base = row * n;
         const float rs = a.rstd[row];
-        float x[S][V], e[S][V], gh[S][V];
+        using P = Piece<T, V, LOOSE>;
+        P xs[S], ys[S], cs[S], hs[S], w[S];
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             const int c = V * (t + i * per);
-#pragma unroll
-            for (int k = 0; k < V; ++k) x[i][k] = e[i][k] = gh[i][k] = 0.0f;
-            if (c < n) {
-                load_piece<T, V>(a.x, base + c, x[i]);
-                if (a.gy) load_piece<T, V>(a.gy, base + c, e[i]);
-                if (a.gh) load_piece<T, V>(a.gh, base + c, gh[i]);
-            }
+            xs[i].load(a.x, base + c, n - c);
+            ys[i].load(a.gy, base + c, a.gy ? n - c : 0);
+            cs[i].load(a.gc, base + c, a.gc ? n - c : 0);
+            hs[i].load(a.gh, base + c, a.gh ? n - c : 0);
+            w[i].load(a.w, c, n - c);
         }
-        if (a.gc) {
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const int c = V * (t + i * per);
-                if (c >= n) continue;
-                float gc[V];
-                load_piece<T, V>(a.gc, base + c, gc);
-                const Cotangent q(a.scale[row * a.ngroups + (lg == kWhole ? 0 : lg >= 0 ? c >> (lg + 3) : (int)__umulhi((uint32_t)c, magic))]);
-#pragma unroll
-                for (int k = 0; k < V; ++k) e[i][k] = q.sum(gc[k], e[i][k]);
-            }
-        }
+        float x[S][V], e[S][V];
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             const int c = V * (t + i * per);
-            float w[V] = {};
-            if (c < n) load_piece<T, V>(a.w, c, w);
+#pragma unroll
+            for (int k = 0; k < V; ++k) e[i][k] = ys[i].at(k);
+            if (a.gc && c < n) {
+                const Cotangent q(a.scale[row * a.ngroups + (lg == kWhole ? 0 : lg >= 0 ? c >> (lg + 3) : (int)__umulhi((uint32_t)c, magic))]);
+#pragma unroll
+                for (int k = 0; k < V; ++k) e[i][k] = q.sum(cs[i].at(k), e[i][k]);
+            }
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                x[i][k] *= rs;
+                x[i][k] = xs[i].at(k) * rs;
                 dw[i][k] += e[i][k] * x[i][k];
-                e[i][k] *= w[k] + a.wadd;
+                e[i][k] *= w[i].at(k) + a.wadd;
                 dot += e[i][k] * x[i][k];
             }
         }
@@ -443,10 +506,10 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs 
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             const int c = V * (t + i * per);
-            if (c >= n) continue;
+            float d[V];
 #pragma unroll
-            for (int k = 0; k < V; ++k) gh[i][k] += rs * (e[i][k] - x[i][k] * mean);
-            store_piece<T, V>(a.dx, base + c, gh[i]);
+            for (int k = 0; k < V; ++k) d[k] = hs[i].at(k) + rs * (e[i][k] - x[i][k] * mean);
+            P::store(a.dx, base + c, n - c, d);
         }
     }
     if (!a.part) return;
@@ -455,12 +518,12 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs 
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             const int c = V * (t + i * per);
-            if (c < n) store_piece<float, V>(part, c, dw[i]);
+            Piece<float, V, LOOSE>::store(part, c, n - c, dw[i]);
         }
     } else {
         constexpr int W = 64 * V * S;
 #pragma unroll
-        for (int i = 0; i < S; ++i) store_piece<float, V>(sums, wave * W + i * 64 * V + V * t, dw[i]);
+        for (int i = 0; i < S; ++i) Piece<float, V, false>::store(sums, wave * W + i * 64 * V + V * t, V, dw[i]);
         __syncthreads();
         for (int c = threadIdx.x; c < n; c += 256) part[c] = (sums[c] + sums[W + c]) + (sums[2 * W + c] + sums[3 * W + c]);
     }
@@ -490,23 +553,23 @@ __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__
 }
 
 // how the rows are taken: pieces a thread (0: the general kernels) of `columns` each, threads of a workgroup, and how
-// the groups' maxima are found
+// the groups' maxima are found (gathers: in LDS, by a workgroup a row)
 struct Rows {
     int pieces, columns, threads, lg;
-    bool wide;
+    bool wide, loose;
 };
-Rows rows_plan(int64_t n, int64_t group, std::initializer_list<const void*> tensors) {
+Rows rows_plan(int64_t n, int64_t group, bool gathers, std::initializer_list<const void*> tensors) {
     Rows r = {};
-    bool eight = n % 8 == 0 && n <= 16384 && (group >= n || lanes::group_log(group) >= 0);
-    for (const void* p : tensors) eight = eight && lanes::aligned16(p);
-    if (eight) {
-        r.lg = group >= n ? kWhole : lanes::group_log(group) - 3;
+    if (n <= 16384 && (group >= n || group % 8 == 0)) {
+        r.loose = n % 8 != 0;
+        for (const void* p : tensors) r.loose = r.loose || !lanes::aligned16(p);
+        r.lg = group >= n ? kWhole : lanes::group_log(group) >= 0 ? lanes::group_log(group) - 3 : kGathered;
         r.columns = 8;
-        r.wide = n > 2048;
+        r.wide = n > 2048 || (gathers && r.lg == kGathered);
         r.pieces = r.wide ? 2 : (int)((n + 511) / 512);
         r.threads = r.wide ? 64 * (int)((n + 1023) / 1024) : 256;
-    } else if (n <= 8192 && (group > 1 || n == 1)) {
-        r.lg = group >= n ? kWhole : kGathered;
+    } else if (n <= 8192 && group > 1) {
+        r.lg = kGathered;
         r.columns = 1;
         r.wide = true;
         r.pieces = n <= 2048 ? 4 : 8;
@@ -516,18 +579,21 @@ Rows rows_plan(int64_t n, int64_t group, std::initializer_list<const void*> tens
 }
 // a column's group is its product with this, over 2^32: exact for columns and groups below 2^14. (One group: not used.)
 uint32_t group_magic(int64_t group) { return group > 1 && group < (1 << 14) ? (uint32_t)((1ULL << 32) / (uint64_t)group + 1) : 0; }
-// f(a kernel's pieces, whether the row is a workgroup's, a piece's columns)
+// f(a kernel's pieces, whether the row is a workgroup's, a piece's columns, whether pieces lie anywhere)
 template <class F>
 void with_rows(const Rows& r, F&& f) {
     using std::integral_constant;
     const integral_constant<int, 8> eight;
     const integral_constant<int, 1> one;
-    if (r.columns == 1) return r.pieces == 4 ? f(integral_constant<int, 4>{}, std::true_type{}, one) : f(eight, std::true_type{}, one);
-    if (r.wide) return f(integral_constant<int, 2>{}, std::true_type{}, eight);
-    if (r.pieces == 1) return f(one, std::false_type{}, eight);
-    if (r.pieces == 2) return f(integral_constant<int, 2>{}, std::false_type{}, eight);
-    if (r.pieces == 3) return f(integral_constant<int, 3>{}, std::false_type{}, eight);
-    return f(integral_constant<int, 4>{}, std::false_type{}, eight);
+    auto of_eight = [&](auto loose) {
+        if (r.wide) return f(integral_constant<int, 2>{}, std::true_type{}, eight, loose);
+        if (r.pieces == 1) return f(one, std::false_type{}, eight, loose);
+        if (r.pieces == 2) return f(integral_constant<int, 2>{}, std::false_type{}, eight, loose);
+        if (r.pieces == 3) return f(integral_constant<int, 3>{}, std::false_type{}, eight, loose);
+        return f(integral_constant<int, 4>{}, std::false_type{}, eight, loose);
+    };
+    if (r.columns == 1) return r.pieces == 4 ? f(integral_constant<int, 4>{}, std::true_type{}, one, std::false_type{}) : f(eight, std::true_type{}, one, std::false_type{});
+    return r.loose ? of_eight(std::true_type{}) : of_eight(std::false_type{});
 }
 
 int64_t bwd_parts(int64_t rows) { return rows < 512 ? rows : 512; }
@@ -578,16 +644,16 @@ int r97q_add_rmsnorm_i8g(const void* x, const void* residual, const void* w, int
     a.scale = scale;
     a.y = y_out;
     a.rstd = rstd;
-    const Rows r = rows_plan(n, a.group, {x, residual, w, h_out, codes, y_out});
+    const Rows r = rows_plan(n, a.group, codes, {x, residual, w, h_out, codes, y_out});
     if (r.pieces) {
-        with_rows(r, [&](auto pieces, auto wide, auto columns) {
+        with_rows(r, [&](auto pieces, auto wide, auto columns, auto loose) {
             const dim3 grid((unsigned)(wide ? rows : (rows + 3) / 4)), threads(r.threads);
             const uint32_t magic = group_magic(a.group);
             const unsigned lds = r.lg == kGathered ? (unsigned)(4 * a.ngroups) : 0;
             if (dtype == R97Q_BF16)
-                hipLaunchKernelGGL((norm_rows_kernel<uint16_t, pieces, wide, columns>), grid, threads, lds, (hipStream_t)stream, a, r.lg, magic);
+                hipLaunchKernelGGL((norm_rows_kernel<uint16_t, pieces, wide, columns, loose>), grid, threads, lds, (hipStream_t)stream, a, r.lg, magic);
             else
-                hipLaunchKernelGGL((norm_rows_kernel<float, pieces, wide, columns>), grid, threads, lds, (hipStream_t)stream, a, r.lg, magic);
+                hipLaunchKernelGGL((norm_rows_kernel<float, pieces, wide, columns, loose>), grid, threads, lds, (hipStream_t)stream, a, r.lg, magic);
         });
         return launch_status("norm_rows_kernel");
     }
@@ -631,18 +697,18 @@ int r97q_add_rmsnorm_i8g_bwd(const void* h, const void* w, int32_t dtype, int64_
     a.dx = dx;
     a.part = dw ? static_cast<float*>(workspace) : nullptr;
     int64_t parts = bwd_parts(rows);
-    const Rows r = rows_plan(n, a.group, {h, w, g_codes, g_y, g_h, dx});
+    const Rows r = rows_plan(n, a.group, false, {h, w, g_codes, g_y, g_h, dx});
     if (rows > 0 && r.pieces) {
         // four rows at a time a workgroup where a row is a wave's
         const int64_t most = r.wide ? rows : (rows + 3) / 4;
         if (parts > most) parts = most;
-        with_rows(r, [&](auto pieces, auto wide, auto columns) {
+        with_rows(r, [&](auto pieces, auto wide, auto columns, auto loose) {
             const dim3 grid((unsigned)(dw ? parts : most)), threads(r.threads);
             const uint32_t magic = group_magic(a.group);
             if (dtype == R97Q_BF16)
-                hipLaunchKernelGGL((norm_rows_bwd_kernel<uint16_t, pieces, wide, columns>), grid, threads, 0, st, a, r.lg, magic);
+                hipLaunchKernelGGL((norm_rows_bwd_kernel<uint16_t, pieces, wide, columns, loose>), grid, threads, 0, st, a, r.lg, magic);
             else
-                hipLaunchKernelGGL((norm_rows_bwd_kernel<float, pieces, wide, columns>), grid, threads, 0, st, a, r.lg, magic);
+                hipLaunchKernelGGL((norm_rows_bwd_kernel<float, pieces, wide, columns, loose>), grid, threads, 0, st, a, r.lg, magic);
         });
         if (int e = launch_status("norm_rows_bwd_kernel")) return e;
     } else if (rows > 0) {

@@ -211,3 +211,42 @@ def test_a_column_at_a_time(rows, n, group, dtype):
     assert bool(((dw.double() - wdw).abs() <= (rows + 8) * R.U32 * (e * x).abs().sum(0) + 1e-30).all())
     again = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale, g_codes=gc, g_h=gh)
     assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
+
+
+def placed(t, by, guard):
+    """t's values `by` values into a buffer that is otherwise full of `guard`."""
+    whole = torch.full((t.numel() + 32,), guard, dtype=t.dtype, device="cuda")
+    view = whole[by:by + t.numel()].view(t.shape)
+    view.copy_(t)
+    return whole, view
+
+
+@pytest.mark.parametrize("rows,n,group", [(9, 1, 0), (6, 9, 0), (5, 18, 8), (7, 515, 128), (3, 1028, 64), (5, 1533, 0), (4, 2046, 512), (3, 2049, 128),
+                                          (2, 7007, 40), (3, 5127, 0), (2, 16383, 128), (3, 2048, 96), (2, 16384, 1000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("by", [0, 1, 5])
+def test_rows_that_begin_anywhere(rows, n, group, dtype, by):
+    """Last pieces of one to eight columns, tensors off 16 bytes: the same results as from aligned ones, nothing beside them."""
+    from r9700training_amd.norm import add_rmsnorm_i8g, add_rmsnorm_i8g_bwd
+
+    print(f"case norm anywhere {(rows, n, group, dtype, by)}", flush=True)
+    x, r, w, codes, scale, h, y, rs = forward(rows, n, group, dtype)
+    gc, gy, gh = (rnd(4 + i, rows, n, dtype=dtype) for i in range(3))
+    args = [placed(v, by, float("nan"))[1] for v in (x, r, w, gc, gy, gh)]
+    outs = [placed(torch.zeros_like(v), by, 77) for v in (codes, h)]
+    got = add_rmsnorm_i8g(args[0], args[1], args[2], group, eps=EPS, codes=outs[0][1], h=outs[1][1], want_y=True)
+    for a, b in zip(got, (codes, scale, h, y, rs)):
+        assert torch.equal(a, b)
+    dx, dw = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale, g_codes=gc, g_y=gy, g_h=gh)
+    wdx, wdw, e = R.norm_backward(h.double(), rs.double(), w, 0.0, scale, group, gc, gy, gh)
+    size = (gc.double().abs() / scale.double()[:, R.group_index(n, group, x.device)]) + gy.double().abs()
+    we, hx = w.double().abs() * size, (h.double() * rs.double()[:, None]).abs()
+    tol = rs.double()[:, None] * (8 * R.U32 * we + (n + 16) * R.U32 * hx * (we * hx).mean(1, keepdim=True)) + 8 * R.U32 * (wdx.abs() + gh.double().abs())
+    assert bool(((dx.double() - wdx).abs() <= tol + R.HALF[dtype] * wdx.abs() + 1e-30).all())
+    assert bool(((dw.double() - wdw).abs() <= (rows + 8) * R.U32 * (size * hx).sum(0) + 1e-30).all())
+    whole, into = placed(torch.zeros_like(dx), by, 77)
+    got = add_rmsnorm_i8g_bwd(placed(h, by, 77)[1], args[2], rs, group, scale=scale, g_codes=args[3], g_y=args[4], g_h=args[5], dx=into)
+    assert torch.equal(into, dx) and torch.equal(got[1], dw)
+    torch.cuda.synchronize()
+    for one, part in outs + [(whole, into)]:
+        assert bool((one[:by] == 77).all()) and bool((one[by + part.numel():] == 77).all())
