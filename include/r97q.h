@@ -599,7 +599,9 @@ int r97q_rotary_frequencies(int32_t rot, double base, int32_t scaling, double fa
  * The last query stands at the last key: query i of a sequence with n queries and m keys sees key j when
  * not causal, or when j <= i + m - n and, with a window, j > i + m - n - window. A query that sees no key
  * gives zeros, a log-sum-exp of minus infinity and zero gradients. Keys and values past a sequence's
- * length are not read. A NaN or infinity that some query of a tile sees may reach the tile's other rows. */
+ * length are not read. A NaN or infinity that some query of a tile sees may reach the tile's other rows.
+ * Results do not depend on the longest length of packed tokens. At most 65535 sequences and key heads, and
+ * 2^23 query heads in all the sequences. */
 typedef struct R97qAttnShape {
     int32_t batch;
     int32_t head_dim;          /* a multiple of 8, at most 256 */
@@ -614,15 +616,20 @@ typedef struct R97qAttnShape {
 } R97qAttnShape;
 
 /* out = softmax(scale q k^T) v and (lse may be NULL) the scores' natural log-sum-exp f32 [batch][q_heads]
- * [q_len], packed [q_heads][q_tokens]. q, k, v bf16 with 16-byte aligned rows; out bf16 or f32; k's heads
- * divide q's: query head h reads key head h / (q_heads / kv_heads). Scores, statistics and sums are f32,
- * the probabilities are rounded to bf16 for their product with v. */
+ * [q_len], packed [q_heads][q_tokens]. q, k, v bf16 with 16-byte aligned rows, tokens at most 2^24 values
+ * apart; out bf16 or f32; k's heads divide q's: query head h reads key head h / (q_heads / kv_heads).
+ * Scores, statistics and sums are f32, the probabilities are rounded to bf16 for their product with v.
+ * Few rows over many keys are cut along the keys and joined through the workspace (on 16 bytes; the entry
+ * says how many bytes, often 0). Repeated calls give the same bits. */
 int64_t r97q_attn_fwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads);
 int r97q_attn_fwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
                   const R97qHeads* out, float* lse, void* workspace, int64_t workspace_bytes, R97IqrStream stream);
 /* The adjoint, from the forward's inputs, out and lse and the output's cotangent d_out (bf16): dq, dk, dv
- * (bf16 or f32) are written. The probabilities are computed again from the scores and lse. Repeated
- * calls give the same bits. The dense form's keys past kv_lens get zero gradients. */
+ * (bf16 or f32) are written. The probabilities are computed again from the scores and lse; they and the
+ * scores' gradients are rounded to bf16 for their products, all sums are f32. Repeated calls give the same
+ * bits. The dense form's keys past kv_lens get zero gradients. The workspace (on 16 bytes) holds two f32 a
+ * query and head, f32 partial sums where the work is cut, and with heads of more than 64 columns the scores'
+ * gradients in bf16 where that takes at most 2 GiB. */
 int64_t r97q_attn_bwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads);
 int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
                   const R97qHeads* out, const float* lse, const R97qHeads* d_out, const R97qHeads* dq,

@@ -123,7 +123,7 @@ int64_t kv_rows(const R97qAttnShape* p) { return p->kv_starts ? p->kv_tokens : p
 // steps. dQ of 64 rows over 4096 keys: 103 / 70 / 53 / 46, but of 1 x 1300: 175 / 178 / 188 / 214 and of 512: 80 / 84 /
 // 86 / 92; so only below half the compute units and from 512 keys a cut. Where dK's and dV's tiles just fill the compute
 // units and are long, the causal ones' first tile has twice the steps of the mean, and two cuts even that out (the whole
-// backward, us at 1 / 2 cuts): heads of 128, 4 x 2048 tokens 336 / 317, 24 heads 468 / 402, but 8 x 1024 194 / 186, 16 x
+// backward with dS^T kept, us at 1 / 2 cuts): heads of 128, 4 x 2048 tokens 336 / 317, 24 heads 468 / 402, but 8 x 1024 194 / 186, 16 x
 // 512 116 / 135, 6 x 2048 415 / 443; of 256, 4 x 2048 560 / 499, 8 x 1024 311 / 323; of 64, two workgroups a unit, 4 x 2048
 // 201 / 164, 8 x 1024 117 / 103, 16 x 512 73 / 74.
 constexpr int kMostCuts = 16;
@@ -149,10 +149,11 @@ void cut_backward(Args& a) {
 }
 // Whether dS^T is kept between the launches (then dQ is one product from it, instead of three from scratch): the bytes,
 // or 0. It costs its bytes written and read, and D's own launch. Measured, computed again / kept (us): heads of 256, 8 x
-// 2048 tokens, 16 over 4 heads 1026 / 843, 1 x 512 tokens, 8 over 2 68 / 51; heads of 128, 16 over 4, 8 x 2048 502 / 537,
-// 4 x 2048 322 / 320, 4 x 1300 159 / 146, 1 x 1300 82 / 68; heads of 64, 8 x 2048 287 / 382, 4 x 1300 92 / 106, 1 x
-// 1300 54 / 51. So from heads of more than 64 columns, up to 512 MiB with heads of up to 128, and up to 2 GiB of
-// workspace; not where dQ's rows are cut, since few rows over many keys are few workgroups here (64 over 4096: 45 / 60).
+// 2048 tokens, 16 over 4 heads 1014 / 843, 4 x 2048 560 / 480, 1 x 512 tokens, 8 over 2 66 / 50; heads of 128, 16 over 4,
+// 8 x 2048 501 / 535, 4 x 2048 275 / 303, 2 x 4096 472 / 520, 4 x 1300 157 / 151, 1 x 1300 81 / 68; heads of 64, 8 x 2048
+// 287 / 382, 4 x 1300 92 / 106, 1 x 1300 54 / 51. So from heads of more than 64 columns, up to 256 MiB with heads of up to
+// 128, and up to 2 GiB of workspace; not where dQ's rows are cut, since few rows over many keys are few workgroups here (64
+// over 4096: 45 / 60).
 int64_t kept_bytes(Args& a) {
     if (a.d <= 64 || a.q_splits > 1 || a.batch == 0) return 0;
     const double rows = a.kv_starts ? (double)a.hq * a.kv_tokens : (double)a.batch * a.hq * a.lk;
@@ -160,7 +161,7 @@ int64_t kept_bytes(Args& a) {
     // what is touched of it: packed sequences leave most of it alone
     const double each = (double)mean_len(a.q_starts, a.q_tokens, a.lq, a.batch) * mean_len(a.kv_starts, a.kv_tokens, a.lk, a.batch);
     if (a.pitch > kMostStride || 2.0 * rows * a.pitch > (double)(2LL << 30)) return 0;
-    if (a.d <= 128 && 2.0 * a.batch * a.hq * each > (double)(512LL << 20)) return 0;
+    if (a.d <= 128 && 2.0 * a.batch * a.hq * each > (double)(256LL << 20)) return 0;
     return (2 * (int64_t)rows * a.pitch + 255) / 256 * 256;
 }
 int64_t bwd_stats(const Args& a) { return (8 * a.slots + 255) / 256 * 256; }

