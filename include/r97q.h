@@ -600,8 +600,8 @@ int r97q_rotary_frequencies(int32_t rot, double base, int32_t scaling, double fa
  * not causal, or when j <= i + m - n and, with a window, j > i + m - n - window. A query that sees no key
  * gives zeros, a log-sum-exp of minus infinity and zero gradients. Keys and values past a sequence's
  * length are not read. A NaN or infinity that some query of a tile sees may reach the tile's other rows.
- * Results do not depend on the longest length of packed tokens. At most 65535 sequences and key heads, and
- * 2^23 query heads in all the sequences. */
+ * Too small a longest length of packed tokens costs time, not results. At most 65535 sequences and key heads,
+ * and 2^23 query heads in all the sequences. */
 typedef struct R97qAttnShape {
     int32_t batch;
     int32_t head_dim;          /* a multiple of 8, at most 256 */
