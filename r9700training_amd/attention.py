@@ -11,14 +11,16 @@ import math
 
 import torch
 
-from . import R97Q_BF16, R97Q_F32, AttnShape, Heads, _empty, _ptr, _stream, check, lib
+from . import R97Q_BF16, R97Q_F32, AttnShape, Heads, _empty, _empty_like, _ptr, _stream, check, lib
 
 
 _DTYPES = {torch.bfloat16: R97Q_BF16, torch.float32: R97Q_F32}
 
 
-def _heads(x: torch.Tensor, packed: bool, what: str) -> Heads:
+def _heads(x: torch.Tensor, packed: bool, what: str, like=None) -> Heads:
     st, shape = x.stride(), x.shape
+    if like is not None and shape != like:
+        raise ValueError(f"attention: {what} has shape {tuple(like)}")
     if len(shape) != (3 if packed else 4) or not x.is_cuda or (st[-1] != 1 and x.numel()):
         raise ValueError(f"attention: {what} is a device [{'' if packed else 'batch, '}tokens, heads, head_dim] tensor, "
                          "head_dim consecutive")
@@ -63,19 +65,13 @@ def _shape(q, k, v, causal, window, scale, q_starts, kv_starts, max_q, max_kv, k
     return s
 
 
-def _lse_shape(q, packed):
-    s = q.shape
+def _lse_shape(s, packed):
     return (s[1], s[0]) if packed else (s[0], s[2], s[1])
 
 
-def _check_lse(lse, q, packed):
-    if lse.dtype != torch.float32 or lse.shape != _lse_shape(q, packed) or not lse.is_contiguous() or not lse.is_cuda:
+def _check_lse(lse, s, packed):
+    if lse.dtype != torch.float32 or lse.shape != _lse_shape(s, packed) or not lse.is_contiguous() or not lse.is_cuda:
         raise ValueError("attention: lse is a contiguous f32 [batch, heads, tokens] device tensor, packed [heads, tokens]")
-
-
-def _same(x, like, what):
-    if x.shape != like.shape:
-        raise ValueError(f"attention: {what} has shape {tuple(like.shape)}")
 
 
 def attention_fwd(q, k, v, causal: bool = True, window: int = 0, scale: float | None = None, q_starts=None,
@@ -87,18 +83,19 @@ def attention_fwd(q, k, v, causal: bool = True, window: int = 0, scale: float | 
     outside every sequence are not written."""
     s = _shape(q, k, v, causal, window, scale, q_starts, kv_starts, max_q, max_kv, kv_lens)
     pq, pk = q_starts is not None, kv_starts is not None
+    qs = q.shape
     if out is None:
-        out = _empty(q.shape, out_dtype, q.device, stream)
-    _same(out, q, "out")
+        out = _empty_like(q, out_dtype, stream)
+    ho = _heads(out, pq, "out", qs)
     if lse is None:
-        lse = _empty(_lse_shape(q, pq), torch.float32, q.device, stream)
-    _check_lse(lse, q, pq)
+        lse = _empty(_lse_shape(qs, pq), torch.float32, q.device, stream)
+    _check_lse(lse, qs, pq)
     hq, hk = _heads(q, pq, "q"), _heads(k, pk, "k")
     if workspace is None:
         need = lib().r97q_attn_fwd_workspace_bytes(s, hq.heads, hk.heads)
         if need > 0:
             workspace = _empty(need, torch.uint8, q.device, stream)
-    check(lib().r97q_attn_fwd(s, hq, hk, _heads(v, pk, "v"), _heads(out, pq, "out"), _ptr(lse), _ptr(workspace),
+    check(lib().r97q_attn_fwd(s, hq, hk, _heads(v, pk, "v"), ho, _ptr(lse), _ptr(workspace),
                               0 if workspace is None else workspace.numel(), _stream(stream)), "r97q_attn_fwd")
     return out, lse
 
@@ -111,21 +108,21 @@ def attention_bwd(q, k, v, out, lse, d_out, causal: bool = True, window: int = 0
     s = _shape(q, k, v, causal, window, scale, q_starts, kv_starts, max_q, max_kv, kv_lens)
     pq, pk = q_starts is not None, kv_starts is not None
 
-    def grad(x, like, what):
+    def grad(x, like, shape, packed, what):
         if x is None:
-            x = _empty(like.shape, grad_dtype, like.device, stream)
-        _same(x, like, what)
-        return x
+            x = _empty_like(like, grad_dtype, stream)
+        return x, _heads(x, packed, what, shape)
 
-    dq, dk, dv = grad(dq, q, "dq"), grad(dk, k, "dk"), grad(dv, v, "dv")
-    _same(out, q, "out")
-    _same(d_out, q, "d_out")
-    _check_lse(lse, q, pq)
+    qs, ks = q.shape, k.shape
+    dq, hdq = grad(dq, q, qs, pq, "dq")
+    dk, hdk = grad(dk, k, ks, pk, "dk")
+    dv, hdv = grad(dv, v, ks, pk, "dv")
+    ho, hdo = _heads(out, pq, "out", qs), _heads(d_out, pq, "d_out", qs)
+    _check_lse(lse, qs, pq)
     hq, hk = _heads(q, pq, "q"), _heads(k, pk, "k")
     if workspace is None:
         need = lib().r97q_attn_bwd_workspace_bytes(s, hq.heads, hk.heads)
         workspace = _empty(max(need, 1), torch.uint8, q.device, stream)
-    check(lib().r97q_attn_bwd(s, hq, hk, _heads(v, pk, "v"), _heads(out, pq, "out"), _ptr(lse), _heads(d_out, pq, "d_out"),
-                              _heads(dq, pq, "dq"), _heads(dk, pk, "dk"), _heads(dv, pk, "dv"), _ptr(workspace),
+    check(lib().r97q_attn_bwd(s, hq, hk, _heads(v, pk, "v"), ho, _ptr(lse), hdo, hdq, hdk, hdv, _ptr(workspace),
                               workspace.numel(), _stream(stream)), "r97q_attn_bwd")
     return dq, dk, dv

@@ -8,7 +8,7 @@ import numpy as np
 import torch
 
 from . import (R97Q_BF16, R97Q_F32, R97Q_ROTARY_HALF, R97Q_ROTARY_INTERLEAVED, R97Q_ROTARY_LINEAR, R97Q_ROTARY_PLAIN,
-               R97Q_ROTARY_RAMP, Heads, _empty, _ptr, _stream, check, lib)
+               R97Q_ROTARY_RAMP, Heads, _empty_like, _ptr, _stream, check, lib)
 
 PAIRS = {"half": R97Q_ROTARY_HALF, "interleaved": R97Q_ROTARY_INTERLEAVED}
 SCALINGS = {"plain": R97Q_ROTARY_PLAIN, "linear": R97Q_ROTARY_LINEAR, "ramp": R97Q_ROTARY_RAMP}
@@ -32,14 +32,16 @@ def rotary_frequencies(rot: int, base: float = 10000.0, scaling: str = "plain", 
 _DTYPES = {torch.bfloat16: R97Q_BF16, torch.float32: R97Q_F32}
 
 
-def _heads(x: torch.Tensor, what: str) -> Heads:
-    st, shape = x.stride(), x.shape
-    if len(shape) != 3 or st[2] != 1 or not x.is_cuda:
+def _heads(x: torch.Tensor, what: str, shape=None) -> Heads:
+    st, own = x.stride(), x.shape
+    if len(own) != 3 or st[2] != 1 or not x.is_cuda:
         raise ValueError(f"rotary: {what} is a device [tokens, heads, head_dim] tensor, head_dim consecutive")
+    if shape is not None and own != shape:
+        raise ValueError(f"rotary: {what} has {what[0]}'s shape")
     dt = _DTYPES.get(x.dtype)
     if dt is None:
         raise ValueError(f"rotary: {what} is bf16 or f32")
-    return Heads(x.data_ptr(), 0, st[0], st[1], shape[1], dt)
+    return Heads(x.data_ptr(), 0, st[0], st[1], own[1], dt)
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
@@ -52,7 +54,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, posi
         raise ValueError(f"rotary: pairs {pairs!r} are not one of {sorted(PAIRS)}")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or not inv_freq.is_cuda:
         raise ValueError("rotary: inv_freq is a contiguous f64 [rot / 2] device tensor")
-    tokens, _, dim = q.shape if q.dim() == 3 else (0, 0, 0)
+    qs = q.shape
+    tokens, _, dim = qs if len(qs) == 3 else (0, 0, 0)
     wide = 0
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) \
@@ -61,20 +64,18 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, posi
         wide = int(positions.dtype == torch.int64)
     hq = _heads(q, "q")
     if q_out is None:
-        q_out = _empty(q.shape, q.dtype, q.device, stream)
-    ho = _heads(q_out, "q_out")
+        q_out = _empty_like(q, q.dtype, stream)
+    ho = _heads(q_out, "q_out", qs)
     hk = hko = None
     if k is not None:
-        hk = _heads(k, "k")
+        hk, ks = _heads(k, "k"), k.shape
         if k_out is None:
-            k_out = _empty(k.shape, k.dtype, k.device, stream)
-        hko = _heads(k_out, "k_out")
-        if k.shape[0] != tokens or k.shape[2] != dim or k_out.shape != k.shape:
-            raise ValueError("rotary: k has q's tokens and head_dim, k_out k's shape")
+            k_out = _empty_like(k, k.dtype, stream)
+        hko = _heads(k_out, "k_out", ks)
+        if ks[0] != tokens or ks[2] != dim:
+            raise ValueError("rotary: k has q's tokens and head_dim")
     elif k_out is not None:
         raise ValueError("rotary: k_out without k")
-    if q_out.shape != q.shape:
-        raise ValueError("rotary: q_out has q's shape")
     check(lib().r97q_rotary(hq, ho, hk, hko, tokens, dim, 2 * inv_freq.shape[0], PAIRS[pairs], _ptr(inv_freq),
                             _ptr(positions), wide, float(mscale), int(bool(inverse)), _stream(stream)), "r97q_rotary")
     return q_out, k_out
