@@ -116,16 +116,17 @@ Args args_of(const R97qAttnShape* p, int32_t hq, int32_t hk) {
 int64_t q_rows(const R97qAttnShape* p) { return p->q_starts ? p->q_tokens : p->q_len; }
 int64_t kv_rows(const R97qAttnShape* p) { return p->kv_starts ? p->kv_tokens : p->kv_len; }
 
-// How the backward is cut where its grids leave compute units idle: a tile's steps over up to kMostCuts workgroups, whose
-// f32 sums another launch adds. Measured on 16 over 4 heads (us at 1 / 2 / 4 / 8 cuts; a cut writes and reads its sums):
-// dK and dV of 1 x 1300 tokens, heads of 128: 176 / 123 / 93 / 86; of 2 x 1300: 181 / 130 / 104 / 123; of 4 x 700:
-// 112 / 92 / 85 / 105; of 512 tokens, heads of 64: 54 / 43 / 36 / 35; so up to some 320 workgroups of at least four
-// steps. dQ of 64 rows over 4096 keys: 103 / 70 / 53 / 46, but of 1 x 1300: 175 / 178 / 188 / 214 and of 512: 80 / 84 /
-// 86 / 92; so only below half the compute units and from 512 keys a cut. Where dK's and dV's tiles just fill the compute
-// units and are long, the causal ones' first tile has twice the steps of the mean, and two cuts even that out (the whole
-// backward with dS^T kept, us at 1 / 2 cuts): heads of 128, 4 x 2048 tokens 336 / 317, 24 heads 468 / 402, but 8 x 1024 194 / 186, 16 x
-// 512 116 / 135, 6 x 2048 415 / 443; of 256, 4 x 2048 560 / 499, 8 x 1024 311 / 323; of 64, two workgroups a unit, 4 x 2048
-// 201 / 164, 8 x 1024 117 / 103, 16 x 512 73 / 74.
+// How the backward is cut where its grids leave compute units idle: a tile's steps over up to kMostCuts workgroups,
+// whose f32 sums another launch adds. Measured on 16 over 4 heads (us at 1 / 2 / 4 / 8 cuts; a cut writes and reads
+// its sums): dK and dV of 1 x 1300 tokens, heads of 128: 176 / 123 / 93 / 86; of 2 x 1300: 181 / 130 / 104 / 123; of
+// 4 x 700: 112 / 92 / 85 / 105; of 512 tokens, heads of 64: 54 / 43 / 36 / 35; of 128, heads of 64 (8 steps a tile):
+// 26 / 23 / 20 / 20, of 64 18 / 19 / 17; so up to some 320 workgroups of at least four steps, or eight cuts of at
+// least two. dQ of 64 rows over 4096 keys: 103 / 70 / 53 / 46, but of 1 x 1300: 175 / 178 / 188 / 214 and of 512: 80
+// / 84 / 86 / 92; so only below half the compute units and from 512 keys a cut. Where dK's and dV's tiles just fill
+// the compute units and are long, the causal ones' first tile has twice the steps of the mean, and two cuts even that
+// out (the whole backward with dS^T kept, us at 1 / 2 cuts): heads of 128, 4 x 2048 tokens 336 / 317, 24 heads 468 /
+// 402, but 8 x 1024 194 / 186, 16 x 512 116 / 135, 6 x 2048 415 / 443; of 256, 4 x 2048 560 / 499, 8 x 1024 311 /
+// 323; of 64, two workgroups a unit, 4 x 2048 201 / 164, 8 x 1024 117 / 103, 16 x 512 73 / 74.
 constexpr int kMostCuts = 16;
 int cuts(int64_t want, int64_t have, int64_t steps) {
     int64_t n = have > 0 ? (want + have - 1) / have : 1;
@@ -142,7 +143,8 @@ void cut_backward(Args& a) {
         if (a.window && (int64_t)a.window + 128 < seeing) seeing = (int64_t)a.window + 128;
         a.q_splits = tiles * 2 <= 256 ? cuts(256, tiles, seen / 512) : 1;
         const int64_t rows = a.g * seeing;
-        a.k_splits = keys * 3 / 2 < 320 ? cuts(320, keys, rows / (a.d > 128 ? 32 : 64) / 4) : 1;
+        const int64_t steps = rows / (a.d > 128 ? 32 : 64), two = steps / 2 < 8 ? steps / 2 : 8;
+        a.k_splits = keys * 3 / 2 < 320 ? cuts(320, keys, steps < 8 ? 1 : steps / 4 > two ? steps / 4 : two) : 1;
         if (a.k_splits == 1 && a.causal && !a.window && (a.d <= 64 ? keys <= 384 && rows >= 3500 : keys <= 256 && rows >= 6144)) a.k_splits = 2;
     }
     a.kv_slots = a.kv_starts ? a.hk * a.kv_tokens : (int64_t)a.batch * a.hk * a.lk;
