@@ -514,7 +514,9 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
 // them, so only where compute units would be idle. Measured (us at 1 / 2 / 4 / 8 / 16 / 32 ranges): one token, 24 over 4
 // heads of 256, 32768 keys 601 / 312 / 168 / 98 / 63 / 43 (64: 39); 16 sequences of 1 .. 4096 keys, 32 over 8 heads of 128
 // 58 / 47 / 44 / 46 / 52 / 67, all of 4096 keys 45 / 49 / 49 / 50 / 54 / 72; 64 rows over 4096 keys 67 / 42 / 29 / 23 / 22 /
-// 24; but 1300 tokens, 16 over 4 heads 28 / 35 / 45 / 57, and 512 tokens 15 / 20 / 22 / 30.
+// 24, over 1024 keys 22 / 19 / 16 / 14 / 15; 200 rows over 2000 keys, heads of 64 28 / 21 / 16 / 14 / 15; but 1300 tokens, 16
+// over 4 heads 28 / 35 / 45 / 57, and 512 tokens 15 / 20 / 22 / 30. One token, 24 over 4 heads of 256, 1024 keys 19 / 17 / 15 /
+// 14 and 512 keys 14 / 15 / 14 / 13; 32 over 8 heads of 128, 1024 keys 10 / 12 / 11 / 11.
 struct Plan {
     bool few;
     int splits, chunk;
@@ -535,9 +537,9 @@ Plan plan_of(const Args& a) {
     if (p.few) {  // lengths that differ leave workgroups idle: more of them
         const int64_t want = !a.kv_lens && !a.kv_starts ? 192 : a.d > 128 ? 256 : 512;
         unit = 128;
-        if (have > 0 && have * 3 / 2 < want && most > 1024) n = (want + have - 1) / have;
+        if (have > 0 && have * 3 / 2 < want && most > (a.d > 128 ? 640 : 1024)) n = (want + have - 1) / have;
     } else {
-        unit = 512;
+        unit = have > 16 ? 512 : most < 512 ? most + 1 : most < 1024 ? 128 : most < 4096 ? most / 8 : 512;
         if (have > 0 && have * 2 <= 256) n = (256 + have - 1) / have;
     }
     if (n > most / unit) n = most / unit;
