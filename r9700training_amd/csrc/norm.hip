@@ -700,7 +700,7 @@ int r97q_add_rmsnorm_i8g_bwd(const void* h, const void* w, int32_t dtype, int64_
     a.dx = dx;
     a.part = dw ? static_cast<float*>(workspace) : nullptr;
     int64_t parts = bwd_parts(rows);
-    const Rows r = rows_plan(n, a.group, false, {h, w, g_codes, g_y, g_h, dx});
+    const Rows r = rows_plan(n, a.group, false, {h, w, g_codes, g_y, g_h, dx, a.part});
     if (rows > 0 && r.pieces) {
         // four rows at a time a workgroup where a row is a wave's
         const int64_t most = r.wide ? rows : (rows + 3) / 4;

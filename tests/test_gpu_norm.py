@@ -250,3 +250,16 @@ def test_rows_that_begin_anywhere(rows, n, group, dtype, by):
     torch.cuda.synchronize()
     for one, part in outs + [(whole, into)]:
         assert bool((one[:by] == 77).all()) and bool((one[by + part.numel():] == 77).all())
+
+
+@pytest.mark.parametrize("n", [512, 2056])
+def test_workspace_off_16_bytes(n):
+    from r9700training_amd.norm import add_rmsnorm_i8g_bwd
+
+    h, gy = rnd(1, 700, n), rnd(2, 700, n)
+    w, rs = rnd(3, n), 1.0 + rnd(4, 700, dtype=torch.float32).abs()
+    dx, dw = add_rmsnorm_i8g_bwd(h, w, rs, g_y=gy)
+    space = torch.empty(4 * 512 * n + 16, dtype=torch.uint8, device="cuda")
+    for by in (4, 8):
+        got = add_rmsnorm_i8g_bwd(h, w, rs, g_y=gy, workspace=space[by:])
+        assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
