@@ -180,7 +180,7 @@ extern "C" {
 int64_t r97q_attn_fwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads) {
     clear_error();
     if (check_shape(shape, q_heads, kv_heads, "r97q_attn_fwd_workspace_bytes")) return -1;
-    if (shape->batch == 0 || shape->q_len == 0) return 0;
+    if (shape->batch == 0 || q_rows(shape) == 0) return 0;  // nothing runs; a packed q_len of 0 is a wrong one, and runs
     return fwd_workspace(args_of(shape, q_heads, kv_heads));
 }
 

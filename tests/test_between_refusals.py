@@ -210,3 +210,28 @@ def test_attention_limits_of_its_tiles():
     assert lib().r97q_attn_fwd_workspace_bytes(long, 4, 2) > 0
     assert fwd(long, ws=None) == EWORKSPACE and fwd(long, ws=FAKE + 4) == EINVAL
     assert lib().r97q_attn_fwd_workspace_bytes(shape(batch=65535), 256, 256) == -1
+
+
+PACKED_LONG = [
+    # batch, query tokens in all, q_heads, kv_heads, head_dim, kv_len: few rows and tiles of rows, cut along the keys
+    (1, 1, 8, 2, 128, 32768),
+    (4, 300, 8, 2, 128, 4096),
+    (1, 40, 4, 4, 64, 8192),
+]
+
+
+@pytest.mark.parametrize("b,tokens,hq,hk,d,lk", PACKED_LONG)
+def test_a_longest_length_of_nothing_still_needs_the_workspace(b, tokens, hq, hk, d, lk):
+    """Packed queries whose longest length is given as 0 run like those of 1, with the same partial sums' room."""
+    def packed(q_len):
+        return shape(batch=b, head_dim=d, q_len=q_len, kv_len=lk, q_starts=FAKE, q_tokens=tokens)
+
+    need = lib().r97q_attn_fwd_workspace_bytes(packed(1), hq, hk)
+    assert need > 0 and lib().r97q_attn_fwd_workspace_bytes(packed(0), hq, hk) == need
+    t = dict(q=heads(hq, d), k=heads(hk, d), v=heads(hk, d), out=heads(hq, d))
+    for q_len in (0, 1):
+        assert fwd(packed(q_len), ws=None, nws=0, **t) == EWORKSPACE
+        assert fwd(packed(q_len), nws=need - 1, **t) == EWORKSPACE
+    # no tokens: nothing runs
+    none = shape(batch=b, head_dim=d, q_len=5, kv_len=lk, q_starts=FAKE, q_tokens=0)
+    assert lib().r97q_attn_fwd_workspace_bytes(none, hq, hk) == 0 and fwd(none, ws=None, nws=0, **t) == OK

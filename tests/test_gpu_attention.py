@@ -430,3 +430,21 @@ def test_kept_graph_and_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(want, held)), seed
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_longest_of_nothing(d):
+    """A longest length of 0 is only a wrong one: cut along the keys or not, the results are those of the right one."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    lq, lk = [3, 1, 40], [4000, 900, 1300]
+    qs = torch.tensor([0, 3, 4, 44], dtype=torch.int32, device="cuda")
+    ks = torch.tensor([0, 4000, 4900, 6200], dtype=torch.int32, device="cuda")
+    q, do = rnd(1, 44, 4, d), rnd(4, 44, 4, d)
+    k, v = rnd(2, 6200, 2, d), rnd(3, 6200, 2, d)
+    seqs = [Packed(a, a + n, b, b + m) for a, n, b, m in zip((0, 3, 4), lq, (0, 4000, 4900), lk)]
+    got = run(q, k, v, do, seqs, 4, 2, True, 0, 1.0 / math.sqrt(d), q_starts=qs, kv_starts=ks, max_q=0, max_kv=0)
+    one = attention_fwd(q, k, v, q_starts=qs, kv_starts=ks, max_q=1, max_kv=1)
+    assert torch.equal(got[0], one[0]) and torch.equal(got[1], one[1])
+    grads = attention_bwd(q, k, v, *one, do, q_starts=qs, kv_starts=ks, max_q=1, max_kv=1)
+    assert all(torch.equal(x, y) for x, y in zip(got[2:], grads))
