@@ -240,6 +240,15 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _space(t, who: str):
+    """(address, bytes) of a call's workspace, given or made; None: nothing."""
+    if t is None:
+        return None, 0
+    if not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{who}: the workspace is a contiguous device tensor")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
 def _stream(stream=None):
     import torch
 

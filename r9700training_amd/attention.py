@@ -11,7 +11,7 @@ import math
 
 import torch
 
-from . import R97Q_BF16, R97Q_F32, AttnShape, Heads, _empty, _empty_like, _ptr, _stream, check, lib
+from . import R97Q_BF16, R97Q_F32, AttnShape, Heads, _empty, _empty_like, _ptr, _space, _stream, check, lib
 
 
 _DTYPES = {torch.bfloat16: R97Q_BF16, torch.float32: R97Q_F32}
@@ -95,8 +95,8 @@ def attention_fwd(q, k, v, causal: bool = True, window: int = 0, scale: float | 
         need = lib().r97q_attn_fwd_workspace_bytes(s, hq.heads, hk.heads)
         if need > 0:
             workspace = _empty(need, torch.uint8, q.device, stream)
-    check(lib().r97q_attn_fwd(s, hq, hk, _heads(v, pk, "v"), ho, _ptr(lse), _ptr(workspace),
-                              0 if workspace is None else workspace.numel(), _stream(stream)), "r97q_attn_fwd")
+    check(lib().r97q_attn_fwd(s, hq, hk, _heads(v, pk, "v"), ho, _ptr(lse), *_space(workspace, "attention"),
+                              _stream(stream)), "r97q_attn_fwd")
     return out, lse
 
 
@@ -123,6 +123,6 @@ def attention_bwd(q, k, v, out, lse, d_out, causal: bool = True, window: int = 0
     if workspace is None:
         need = lib().r97q_attn_bwd_workspace_bytes(s, hq.heads, hk.heads)
         workspace = _empty(max(need, 1), torch.uint8, q.device, stream)
-    check(lib().r97q_attn_bwd(s, hq, hk, _heads(v, pk, "v"), ho, _ptr(lse), hdo, hdq, hdk, hdv, _ptr(workspace),
-                              workspace.numel(), _stream(stream)), "r97q_attn_bwd")
+    check(lib().r97q_attn_bwd(s, hq, hk, _heads(v, pk, "v"), ho, _ptr(lse), hdo, hdq, hdk, hdv,
+                              *_space(workspace, "attention"), _stream(stream)), "r97q_attn_bwd")
     return dq, dk, dv

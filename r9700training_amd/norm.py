@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import torch
 
-from . import R97Q_BF16, R97Q_F32, _empty, _ptr, _stream, check, lib
+from . import R97Q_BF16, R97Q_F32, _empty, _ptr, _space, _stream, check, lib
 
 
 def _rows(x: torch.Tensor, what: str, like: torch.Tensor | None = None) -> None:
@@ -107,7 +107,7 @@ def add_rmsnorm_i8g_bwd(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tenso
         dw = None
     check(lib().r97q_add_rmsnorm_i8g_bwd(_ptr(h), _ptr(weight), dt, rows, n, int(group), float(wadd), _ptr(rstd),
                                          _ptr(scale), _ptr(g_codes), _ptr(g_y), _ptr(g_h), _ptr(dx), _ptr(dw),
-                                         int(bool(accumulate)), _ptr(workspace) if want_dw else None,
-                                         workspace.numel() if want_dw else 0, _stream(stream)),
+                                         int(bool(accumulate)),
+                                         *_space(workspace if want_dw else None, "add_rmsnorm_i8g_bwd"), _stream(stream)),
           "r97q_add_rmsnorm_i8g_bwd")
     return dx, dw

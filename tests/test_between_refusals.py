@@ -235,3 +235,30 @@ def test_a_longest_length_of_nothing_still_needs_the_workspace(b, tokens, hq, hk
     # no tokens: nothing runs
     none = shape(batch=b, head_dim=d, q_len=5, kv_len=lk, q_starts=FAKE, q_tokens=0)
     assert lib().r97q_attn_fwd_workspace_bytes(none, hq, hk) == 0 and fwd(none, ws=None, nws=0, **t) == OK
+
+
+def test_fronts_refuse_a_workspace_off_the_card():
+    """A workspace is an operand like the others: one in host memory, or with gaps, is refused with a message that names it.
+    (The operands here are host tensors that say they are on a device: nothing gets as far as a launch.)"""
+    import torch
+
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+    from r9700training_amd.norm import add_rmsnorm_i8g_bwd
+
+    class Card(torch.Tensor):
+        is_cuda = True
+
+    def card(*size, dtype=torch.bfloat16):
+        return torch.zeros(size, dtype=dtype).as_subclass(Card)
+
+    x, kv = card(1, 3, 4, 64), card(1, 50, 4, 64)
+    lse = card(1, 4, 3, dtype=torch.float32)
+    y, w, rs, dw = card(4, 64), card(64), card(4, dtype=torch.float32), card(64, dtype=torch.float32)
+    bad = [torch.empty(1 << 20, dtype=torch.uint8), card(1 << 20, 2, dtype=torch.uint8)[:, :1]]
+    for ws in bad:
+        with pytest.raises(ValueError, match="workspace"):
+            attention_fwd(x, kv, kv, out=x.clone(), lse=lse, workspace=ws)
+        with pytest.raises(ValueError, match="workspace"):
+            attention_bwd(x, kv, kv, x.clone(), lse, x.clone(), dq=x.clone(), dk=kv.clone(), dv=kv.clone(), workspace=ws)
+        with pytest.raises(ValueError, match="workspace"):
+            add_rmsnorm_i8g_bwd(y, w, rs, g_y=y.clone(), dx=y.clone(), dw=dw, workspace=ws)
