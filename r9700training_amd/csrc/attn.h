@@ -38,6 +38,12 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMostSplits = 256;  // ranges of the keys that the forward's join adds
+constexpr int64_t kMostHeads = 1 << 23;  // query heads in all the sequences
+
+// workgroups of `threads` in a launch's first dimension: their threads in all stay below 2^32. The kernels' tile loops take
+// what a grid cut short leaves.
+constexpr int64_t most_groups(int threads) { return 0xFFFFFFFFLL / threads; }
+static_assert(most_groups(256) >= kMostHeads, "a workgroup for every head");
 
 // one tensor of heads: element (b, t, h, d) at data[b * bs + t * ts + h * hs + d]
 struct Heads {

@@ -32,8 +32,7 @@ int check_shape(const R97qAttnShape* p, int32_t hq, int32_t hk, const char* who)
     if (hk <= 0 || hq <= 0 || hq % hk) return refuse(R97Q_EINVAL, who, "the query heads are a multiple of the key heads");
     if (p->batch < 0 || p->q_len < 0 || p->kv_len < 0) return refuse(R97Q_EINVAL, who, "a negative batch or length");
     if (p->batch > 65535 || hk > 65535) return refuse(R97Q_EUNSUPPORTED, who, "at most 65535 sequences and key heads");
-    // heads times kMostSplits or kMostCuts workgroups of a one-dimensional grid
-    if ((int64_t)p->batch * hq > 0x7FFFFFFF / kMostSplits)
+    if ((int64_t)p->batch * hq > kMostHeads)
         return refuse(R97Q_EUNSUPPORTED, who, "the sequences' heads in all pass 2^23");
     if (p->q_len > 0x7FFFFF00 / (hq / hk) || p->kv_len > 0x7FFFFF00)
         return refuse(R97Q_EUNSUPPORTED, who, "a sequence's rows of one key head or its keys pass 31 bits");
@@ -145,7 +144,11 @@ void cut_backward(Args& a) {
         const int64_t rows = a.g * seeing;
         const int64_t steps = rows / (a.d > 128 ? 32 : 64), two = steps / 2 < 8 ? steps / 2 : 8;
         a.k_splits = keys * 3 / 2 < 320 ? cuts(320, keys, steps < 8 ? 1 : steps / 4 > two ? steps / 4 : two) : 1;
-        if (a.k_splits == 1 && a.causal && !a.window && (a.d <= 64 ? keys <= 384 && rows >= 3500 : keys <= 256 && rows >= 6144)) a.k_splits = 2;
+        // and a workgroup for each cut of each head in a grid
+        const int most = (int)(most_groups(256) / ((int64_t)a.batch * a.hk));
+        if (a.q_splits > most) a.q_splits = most;
+        if (a.k_splits > most) a.k_splits = most;
+        if (a.k_splits == 1 && most > 1 && a.causal && !a.window && (a.d <= 64 ? keys <= 384 && rows >= 3500 : keys <= 256 && rows >= 6144)) a.k_splits = 2;
     }
     a.kv_slots = a.kv_starts ? a.hk * a.kv_tokens : (int64_t)a.batch * a.hk * a.lk;
 }

@@ -263,7 +263,7 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
 
 template <int D, int RT, bool KEPT, int PER, int SLOTS>
 int run(const Args& a, hipStream_t st) {
-    const int64_t nb = (int64_t)a.batch * a.hk * a.k_splits, most = 0x7FFFFFFF / nb;
+    const int64_t nb = (int64_t)a.batch * a.hk * a.k_splits, most = most_groups(256) / nb;
     int64_t keys = ((int64_t)a.lk + 127) / 128;
     if (keys > most) keys = most;
     if (keys == 0) return R97Q_OK;

@@ -382,7 +382,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(Args a, Sum u) {
 
 template <int D, int PER>
 int run(const Args& a, hipStream_t st) {
-    const int64_t nb = (int64_t)a.batch * a.hk * a.q_splits, most = 0x7FFFFFFF / nb;
+    const int64_t nb = (int64_t)a.batch * a.hk * a.q_splits, most = most_groups(256) / nb;
     int64_t tiles = ((int64_t)a.lq * a.g + 127) / 128;
     if (tiles > most) tiles = most;
     if (tiles == 0) return R97Q_OK;
@@ -415,7 +415,7 @@ int launch_base(const Args& a, hipStream_t st) {
 
 template <int D, int KT, int PER, int RT>
 int run_kept(const Args& a, hipStream_t st) {
-    const int64_t nb = (int64_t)a.batch * a.hq, most = 0x7FFFFFFF / nb;
+    const int64_t nb = (int64_t)a.batch * a.hq, most = most_groups(256) / nb;
     int64_t tiles = ((int64_t)a.lq + 127) / 128;
     if (tiles > most) tiles = most;
     if (tiles == 0) return R97Q_OK;

@@ -544,6 +544,9 @@ Plan plan_of(const Args& a) {
     }
     if (n > most / unit) n = most / unit;
     if (n > kMostSplits) n = kMostSplits;
+    // a workgroup for each range of each head in a grid, and the join's of up to 1024 threads for each query head
+    if (n > most_groups(256) / ((int64_t)a.batch * a.hk)) n = most_groups(256) / ((int64_t)a.batch * a.hk);
+    if ((int64_t)a.batch * a.hq > most_groups(1024)) n = 1;
     if (n > 1) {
         p.chunk = (int)(((most + n - 1) / n + 127) / 128 * 128);
         p.splits = (int)((most + p.chunk - 1) / p.chunk);
@@ -553,7 +556,7 @@ Plan plan_of(const Args& a) {
 
 template <int D, int KT, int NW, int PER>
 int run_tiles(const Args& a, const Plan& p, hipStream_t st) {
-    const int64_t nb = (int64_t)a.batch * a.hk * p.splits, most = 0x7FFFFFFF / nb;
+    const int64_t nb = (int64_t)a.batch * a.hk * p.splits, most = most_groups(64 * NW) / nb;
     const int64_t tiles = p.tiles < most ? p.tiles : most;
     hipLaunchKernelGGL((attn_fwd_kernel<D, KT, NW, PER>), dim3((unsigned)(tiles * nb)), dim3(64 * NW), 0, st, a);
     return launch_status("attn_fwd_kernel");

@@ -1,0 +1,96 @@
+"""The launches of the operators between the projections, on the host: no grid passes what the runtime takes (2^32 work items
+a dimension), however many sequences, heads and rows there are, and all rows are covered. The library runs in a process of
+its own with tests/launch_hook.c in the place of the runtime's launch: no kernel runs, and no pointer is read."""
+import json
+import os
+import shutil
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HOOK = os.path.join(ROOT, "tests", "launch_hook.c")
+FAKE = 1 << 20
+
+CHILD = r"""
+import ctypes as C, json, sys
+hook = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
+sys.path.insert(0, sys.argv[2])
+from r9700training_amd import AttnShape, Heads, lib
+FAKE = 1 << 20
+
+def heads(n, d, dtype=1, data=FAKE, gap=0):
+    return Heads(data, 0, n * d + gap, d, n, dtype)
+
+def attn(back, batch, hq, hk, d, q_tokens, kv_tokens, max_q, max_kv, causal=1, window=0):
+    s = AttnShape(batch=batch, head_dim=d, q_len=max_q, kv_len=max_kv, q_starts=FAKE, kv_starts=FAKE, q_tokens=q_tokens,
+                  kv_tokens=kv_tokens, causal=causal, window=window, scale=0.1)
+    q, k = heads(hq, d), heads(hk, d)
+    if back:
+        need = lib().r97q_attn_bwd_workspace_bytes(s, hq, hk)
+        return lib().r97q_attn_bwd(s, q, k, k, q, FAKE, q, q, k, k, FAKE, max(need, 1), None)
+    need = lib().r97q_attn_fwd_workspace_bytes(s, hq, hk)
+    return lib().r97q_attn_fwd(s, q, k, k, q, FAKE, FAKE, max(need, 0), None)
+
+def norm(rows, n, group, dtype=1, codes=FAKE, data=FAKE):
+    return lib().r97q_add_rmsnorm_i8g(data, data, FAKE, dtype, rows, n, group, 1e-6, 0.0, data, codes, codes, None, FAKE, None)
+
+def norm_bwd(rows, n, group, dw, dtype=1):
+    return lib().r97q_add_rmsnorm_i8g_bwd(FAKE, FAKE, dtype, rows, n, group, 0.0, FAKE, FAKE, FAKE, None, None, FAKE,
+                                          FAKE if dw else None, 0, FAKE, 1 << 60, None)
+
+def rotary(tokens, hq, dim, rot, dtype=1, data=FAKE, pairs=0):
+    q = heads(hq, dim, dtype, data)
+    return lib().r97q_rotary(q, heads(hq, dim, dtype, data + (1 << 40)), None, None, tokens, dim, rot, pairs, FAKE, None, 0, 1.0, 0, None)
+
+what, args = json.loads(sys.argv[3])
+hook.hook_clear()
+rc = globals()[what](**args)
+out, one = [], (C.c_int64 * 30)()
+for i in range(min(hook.hook_count(), 4096)):
+    hook.hook_launch(i, one)
+    out.append(list(one))
+print(json.dumps([rc, hook.hook_count(), out, lib().r97q_last_error().decode()]))
+"""
+
+
+@pytest.fixture(scope="session")
+def hook(tmp_path_factory):
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    so = str(tmp_path_factory.mktemp("hook") / "launch_hook.so")
+    subprocess.run([cc, "-O1", "-Wall", "-shared", "-fPIC", "-o", so, HOOK], check=True)
+    return so
+
+
+def launches(hook, what, **args):
+    """The call's launches: [(grid, workgroup, words)], all of them accepted."""
+    p = subprocess.run([sys.executable, "-c", CHILD, hook, ROOT, json.dumps([what, args])], capture_output=True, text=True, timeout=120)
+    assert p.returncode == 0, p.stderr
+    rc, count, got, error = json.loads(p.stdout.splitlines()[-1])
+    assert rc == 0, (what, args, error)
+    assert count == len(got)
+    return [(tuple(x[:3]), tuple(x[3:6]), x[6:]) for x in got]
+
+
+ATTENTION = [
+    # many sequences with one long one among them: batch, q_heads, kv_heads, head_dim, q_tokens, kv_tokens, max_q, max_kv
+    (1024, 32, 8, 64, 200000, 200000, 131072, 131072),
+    (1024, 32, 8, 128, 200000, 200000, 131072, 131072),
+    (1024, 32, 8, 256, 200000, 200000, 131072, 131072),
+    # as many heads as are served, next to no tokens: neither cuts nor the join may pass the limit
+    (65535, 128, 128, 64, 3, 3, 1, 1),
+    (65535, 128, 128, 128, 40, 70000000, 1, 70000000),
+    (65535, 128, 64, 256, 40, 70000000, 40, 70000000),
+    (65535, 96, 2, 64, 500, 200000000, 500, 5000000),
+    (65535, 128, 1, 256, 1, 9000000000, 1, 200000),
+]
+
+
+@pytest.mark.parametrize("b,hq,hk,d,qt,kt,mq,mk", ATTENTION)
+@pytest.mark.parametrize("back", [False, True])
+def test_attention_grids(hook, b, hq, hk, d, qt, kt, mq, mk, back):
+    got = launches(hook, "attn", back=back, batch=b, hq=hq, hk=hk, d=d, q_tokens=qt, kv_tokens=kt, max_q=mq, max_kv=mk)
+    assert got

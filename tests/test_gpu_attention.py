@@ -448,3 +448,22 @@ def test_longest_of_nothing(d):
     assert torch.equal(got[0], one[0]) and torch.equal(got[1], one[1])
     grads = attention_bwd(q, k, v, *one, do, q_starts=qs, kv_starts=ks, max_q=1, max_kv=1)
     assert all(torch.equal(x, y) for x, y in zip(got[2:], grads))
+
+
+def test_a_grid_cut_short():
+    """A longest length far past the real ones asks for more workgroups than a launch takes: the workgroups there are take
+    more tiles each, and the bits are those of the right length."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    lens = [1 + i % 3 for i in range(1023)] + [300]
+    at = torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+    n = sum(lens)
+    q, k, v, do = rnd(1, n, 32, 64), rnd(2, n, 8, 64), rnd(3, n, 8, 64), rnd(4, n, 32, 64)
+    out = {}
+    for longest in (300, 131072):
+        print(f"case longest {longest}", flush=True)
+        kw = dict(q_starts=at, kv_starts=at, max_q=longest, max_kv=longest)
+        o, lse = attention_fwd(q, k, v, **kw)
+        out[longest] = (o, lse) + attention_bwd(q, k, v, o, lse, do, **kw)
+        torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(out[300], out[131072]))
