@@ -533,21 +533,21 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_bwd_kernel(NArgs 
 }
 
 // ---------------------------------------------------------------- dw from the workgroups' partial sums
-// 32 columns a workgroup; each of its 32 half waves adds every 32nd of the partial rows, their sums are added in
-// order. 512 partial rows of 5120 columns: 4.7 us, latency.
-__global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__ part, int64_t parts, int64_t n,
+// 32 columns a workgroup, of `cols` of a row's n; each of its 32 half waves adds every 32nd of the partial rows, their sums are
+// added in order. 512 partial rows of 5120 columns: 4.7 us, latency.
+__global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__ part, int64_t parts, int64_t n, int64_t cols,
                                                        float* __restrict__ dw, int32_t add) {
     __shared__ float sum[32][32];
     const int col = threadIdx.x & 31, half = threadIdx.x >> 5;
     const int64_t j = (int64_t)blockIdx.x * 32 + col;
     float s = 0.0f;
-    if (j < n) {
+    if (j < cols) {
 #pragma unroll 8
         for (int64_t p = half; p < parts; p += 32) s += part[p * n + j];
     }
     sum[half][col] = s;
     __syncthreads();
-    if (half == 0 && j < n) {
+    if (half == 0 && j < cols) {
         float t = sum[0][col];
 #pragma unroll
         for (int i = 1; i < 32; ++i) t += sum[i][col];
@@ -599,6 +599,33 @@ void with_rows(const Rows& r, F&& f) {
     return r.loose ? of_eight(std::true_type{}) : of_eight(std::false_type{});
 }
 
+// workgroups of `threads` in a launch: its threads stay below 2^32
+constexpr int64_t most_groups(int threads) { return 0xFFFFFFFFLL / threads; }
+// f(the arguments of some rows) until all have had theirs, at most `most` of them at a time, a multiple of 16: later rows then
+// lie on 16 bytes where the first does
+template <class F>
+void rows_in_turn(NArgs a, int64_t most, int size, F&& f) {
+    const int64_t rows = a.rows;
+    auto past = [](auto*& p, int64_t bytes) {
+        if (p) p = (std::remove_reference_t<decltype(p)>)(reinterpret_cast<uintptr_t>(p) + bytes);
+    };
+    most -= most % 16;
+    for (int64_t done = 0;;) {
+        a.rows = rows - done < most ? rows - done : most;
+        f(a);
+        done += a.rows;
+        if (done == rows) return;
+        const int64_t values = a.rows * a.n;
+        past(a.x, values * size);
+        past(a.res, values * size);
+        past(a.h, values * size);
+        past(a.codes, values);
+        past(a.y, 2 * values);
+        past(a.scale, 4 * a.rows * a.ngroups);
+        past(a.rstd, 4 * a.rows);
+    }
+}
+
 int64_t bwd_parts(int64_t rows) { return rows < 512 ? rows : 512; }
 
 int refuse(const char* who, int code, const char* why) {
@@ -648,22 +675,28 @@ int r97q_add_rmsnorm_i8g(const void* x, const void* residual, const void* w, int
     a.y = y_out;
     a.rstd = rstd;
     const Rows r = rows_plan(n, a.group, codes, {x, residual, w, h_out, codes, y_out});
+    const int size = dtype == R97Q_BF16 ? 2 : 4;
     if (r.pieces) {
         with_rows(r, [&](auto pieces, auto wide, auto columns, auto loose) {
-            const dim3 grid((unsigned)(wide ? rows : (rows + 3) / 4)), threads(r.threads);
             const uint32_t magic = group_magic(a.group);
             const unsigned lds = r.lg == kGathered ? (unsigned)(4 * a.ngroups) : 0;
-            if (dtype == R97Q_BF16)
-                hipLaunchKernelGGL((norm_rows_kernel<uint16_t, pieces, wide, columns, loose>), grid, threads, lds, (hipStream_t)stream, a, r.lg, magic);
-            else
-                hipLaunchKernelGGL((norm_rows_kernel<float, pieces, wide, columns, loose>), grid, threads, lds, (hipStream_t)stream, a, r.lg, magic);
+            const int each = wide ? 1 : 4;  // rows a workgroup
+            rows_in_turn(a, each * most_groups(r.threads), size, [&](const NArgs& b) {
+                const dim3 grid((unsigned)((b.rows + each - 1) / each)), threads(r.threads);
+                if (dtype == R97Q_BF16)
+                    hipLaunchKernelGGL((norm_rows_kernel<uint16_t, pieces, wide, columns, loose>), grid, threads, lds, (hipStream_t)stream, b, r.lg, magic);
+                else
+                    hipLaunchKernelGGL((norm_rows_kernel<float, pieces, wide, columns, loose>), grid, threads, lds, (hipStream_t)stream, b, r.lg, magic);
+            });
         });
         return launch_status("norm_rows_kernel");
     }
-    if (dtype == R97Q_BF16)
-        hipLaunchKernelGGL(norm_any_kernel<uint16_t>, dim3((unsigned)rows), dim3(kThreads), 0, (hipStream_t)stream, a);
-    else
-        hipLaunchKernelGGL(norm_any_kernel<float>, dim3((unsigned)rows), dim3(kThreads), 0, (hipStream_t)stream, a);
+    rows_in_turn(a, most_groups(kThreads), size, [&](const NArgs& b) {
+        if (dtype == R97Q_BF16)
+            hipLaunchKernelGGL(norm_any_kernel<uint16_t>, dim3((unsigned)b.rows), dim3(kThreads), 0, (hipStream_t)stream, b);
+        else
+            hipLaunchKernelGGL(norm_any_kernel<float>, dim3((unsigned)b.rows), dim3(kThreads), 0, (hipStream_t)stream, b);
+    });
     return launch_status("norm_any_kernel");
 }
 
@@ -703,7 +736,8 @@ int r97q_add_rmsnorm_i8g_bwd(const void* h, const void* w, int32_t dtype, int64_
     const Rows r = rows_plan(n, a.group, false, {h, w, g_codes, g_y, g_h, dx, a.part});
     if (rows > 0 && r.pieces) {
         // four rows at a time a workgroup where a row is a wave's
-        const int64_t most = r.wide ? rows : (rows + 3) / 4;
+        int64_t most = r.wide ? rows : (rows + 3) / 4;
+        if (most > most_groups(r.threads)) most = most_groups(r.threads);
         if (parts > most) parts = most;
         with_rows(r, [&](auto pieces, auto wide, auto columns, auto loose) {
             const dim3 grid((unsigned)(dw ? parts : most)), threads(r.threads);
@@ -715,7 +749,7 @@ int r97q_add_rmsnorm_i8g_bwd(const void* h, const void* w, int32_t dtype, int64_
         });
         if (int e = launch_status("norm_rows_bwd_kernel")) return e;
     } else if (rows > 0) {
-        const dim3 grid((unsigned)(dw ? parts : rows));
+        const dim3 grid((unsigned)(dw ? parts : rows < most_groups(kThreads) ? rows : most_groups(kThreads)));
         if (dtype == R97Q_BF16)
             hipLaunchKernelGGL(norm_any_bwd_kernel<uint16_t>, grid, dim3(kThreads), 0, st, a);
         else
@@ -723,7 +757,10 @@ int r97q_add_rmsnorm_i8g_bwd(const void* h, const void* w, int32_t dtype, int64_
         if (int e = launch_status("norm_any_bwd_kernel")) return e;
     }
     if (!dw) return R97Q_OK;
-    hipLaunchKernelGGL(norm_dw_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, st, a.part, parts, n, dw, dw_accumulate);
+    for (int64_t c = 0, most = 32 * most_groups(1024); c < n; c += most) {
+        const int64_t cols = n - c < most ? n - c : most;
+        hipLaunchKernelGGL(norm_dw_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, st, a.part + c, parts, n, cols, dw + c, dw_accumulate);
+    }
     return launch_status("norm_dw_kernel");
 }
 

@@ -44,14 +44,15 @@ def rotary(tokens, hq, dim, rot, dtype=1, data=FAKE, pairs=0):
     q = heads(hq, dim, dtype, data)
     return lib().r97q_rotary(q, heads(hq, dim, dtype, data + (1 << 40)), None, None, tokens, dim, rot, pairs, FAKE, None, 0, 1.0, 0, None)
 
-what, args = json.loads(sys.argv[3])
-hook.hook_clear()
-rc = globals()[what](**args)
-out, one = [], (C.c_int64 * 30)()
-for i in range(min(hook.hook_count(), 4096)):
-    hook.hook_launch(i, one)
-    out.append(list(one))
-print(json.dumps([rc, hook.hook_count(), out, lib().r97q_last_error().decode()]))
+for line in sys.stdin:
+    what, args = json.loads(line)
+    hook.hook_clear()
+    rc = globals()[what](**args)
+    out, one = [], (C.c_int64 * 30)()
+    for i in range(min(hook.hook_count(), 4096)):
+        hook.hook_launch(i, one)
+        out.append(list(one))
+    print(json.dumps([rc, hook.hook_count(), out, lib().r97q_last_error().decode()]), flush=True)
 """
 
 
@@ -62,14 +63,17 @@ def hook(tmp_path_factory):
         pytest.skip("no C compiler")
     so = str(tmp_path_factory.mktemp("hook") / "launch_hook.so")
     subprocess.run([cc, "-O1", "-Wall", "-shared", "-fPIC", "-o", so, HOOK], check=True)
-    return so
+    p = subprocess.Popen([sys.executable, "-c", CHILD, so, ROOT], stdin=subprocess.PIPE, stdout=subprocess.PIPE, text=True)
+    yield p
+    p.stdin.close()
+    p.wait(timeout=60)
 
 
 def launches(hook, what, **args):
     """The call's launches: [(grid, workgroup, words)], all of them accepted."""
-    p = subprocess.run([sys.executable, "-c", CHILD, hook, ROOT, json.dumps([what, args])], capture_output=True, text=True, timeout=120)
-    assert p.returncode == 0, p.stderr
-    rc, count, got, error = json.loads(p.stdout.splitlines()[-1])
+    hook.stdin.write(json.dumps([what, args]) + "\n")
+    hook.stdin.flush()
+    rc, count, got, error = json.loads(hook.stdout.readline())
     assert rc == 0, (what, args, error)
     assert count == len(got)
     return [(tuple(x[:3]), tuple(x[3:6]), x[6:]) for x in got]
@@ -94,3 +98,44 @@ ATTENTION = [
 def test_attention_grids(hook, b, hq, hk, d, qt, kt, mq, mk, back):
     got = launches(hook, "attn", back=back, batch=b, hq=hq, hk=hk, d=d, q_tokens=qt, kv_tokens=kt, max_q=mq, max_kv=mk)
     assert got
+
+
+NORM_MOST = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("rows,n,group,size", [
+    (NORM_MOST, 64, 0, 2), (NORM_MOST, 64, 8, 4), (NORM_MOST, 2056, 128, 2), (NORM_MOST, 16384, 0, 2), (NORM_MOST, 3, 2, 2),
+    (NORM_MOST, 5, 3, 4), (NORM_MOST, 3, 1, 2), (NORM_MOST, 17408, 256, 2), (70_000_001, 60, 0, 2), (5, 64, 0, 2)])
+def test_norm_grids(hook, rows, n, group, size):
+    """The forward's launches take every row once, in order, each where the rows before it end."""
+    got = launches(hook, "norm", rows=rows, n=n, group=group, dtype=1 if size == 2 else 0)
+    groups = 1 if group <= 0 else -(-n // group)
+    done = 0
+    for grid, block, w in got:
+        x, res, _, here, width, _, ngroups = w[:7]
+        h, codes, scale, y, rstd = w[8:13]
+        assert (width, ngroups, y) == (n, groups, 0)
+        assert x == res == h == FAKE + done * n * size and codes == FAKE + done * n
+        assert scale == FAKE + 4 * done * groups and rstd == FAKE + 4 * done
+        # a row a workgroup, or one for each of its four waves
+        assert here > 0 and here <= grid[0] * (4 if block[0] == 256 and grid[0] < here else 1)
+        done += here
+    assert done == rows and (rows > 10 ** 6 or len(got) == 1)
+
+
+@pytest.mark.parametrize("rows,n,group", [(NORM_MOST, 64, 0), (NORM_MOST, 2056, 128), (NORM_MOST, 3, 2), (NORM_MOST, 3, 1)])
+def test_norm_backward_grids(hook, rows, n, group):
+    """The adjoint's workgroups walk the rows: one launch, and with the gain's gradient one more."""
+    assert len(launches(hook, "norm_bwd", rows=rows, n=n, group=group, dw=False)) == 1
+    assert len(launches(hook, "norm_bwd", rows=rows, n=n, group=group, dw=True)) == 2
+
+
+@pytest.mark.parametrize("n", [2 ** 27, 2 ** 28 + 7, NORM_MOST])
+def test_norm_gain_grids(hook, n):
+    """Every column's partial sums are added, 32 columns a workgroup, each launch from where the one before it ends."""
+    got = launches(hook, "norm_bwd", rows=2, n=n, group=0, dw=True)[1:]
+    done = 0
+    for grid, block, w in got:
+        assert block[0] == 1024 and w[0] == FAKE + 4 * done
+        done += 32 * grid[0]
+    assert n <= done < n + 32

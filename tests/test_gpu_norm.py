@@ -263,3 +263,22 @@ def test_workspace_off_16_bytes(n):
     for by in (4, 8):
         got = add_rmsnorm_i8g_bwd(h, w, rs, g_y=gy, workspace=space[by:])
         assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+
+
+@pytest.mark.parametrize("rows,n,group", [(67_200_003, 8, 0), (16_800_005, 3, 1), (67_300_001, 2, 0)])
+def test_more_rows_than_a_launch_takes(rows, n, group):
+    """Rows on both sides of a launch's end have the bits they have in a call of their own, forward and back."""
+    from r9700training_amd.norm import add_rmsnorm_i8g, add_rmsnorm_i8g_bwd
+
+    print(f"case norm rows {(rows, n, group)}", flush=True)
+    x, r, w, gy = rnd(1, rows, n), rnd(2, rows, n), rnd(3, n), rnd(4, rows, n)
+    codes, scale, h, y, rs = add_rmsnorm_i8g(x, r, w, group, eps=EPS, want_y=True)
+    dx, _ = add_rmsnorm_i8g_bwd(h, w, rs, group, g_y=gy, want_dw=False)
+    ends = (0, 16_777_200, 16_777_216, 67_108_800, 67_108_860, rows - 40)
+    for at in (i for i in ends if i + 40 <= rows):
+        part = slice(at, at + 40)
+        want = add_rmsnorm_i8g(x[part].contiguous(), r[part].contiguous(), w, group, eps=EPS, want_y=True)
+        for a, b in zip((codes[part], scale[part], h[part], y[part], rs[part]), want):
+            assert torch.equal(a, b), at
+        back, _ = add_rmsnorm_i8g_bwd(h[part].contiguous(), w, rs[part].contiguous(), group, g_y=gy[part].contiguous(), want_dw=False)
+        assert torch.equal(dx[part], back), at
