@@ -114,7 +114,8 @@ struct Piece {
 template <class T, int V, bool NEAR, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RArgs a) {
     __shared__ float2 table[kTable];  // (cos, sin) * mscale
-    const int64_t t0 = (int64_t)blockIdx.x * a.tpb;
+    const int64_t t0 = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * a.tpb;
+    if (t0 >= a.tokens) return;
     const int nt = a.tokens - t0 < a.tpb ? (int)(a.tokens - t0) : a.tpb;
     for (int i = threadIdx.x; i < nt * a.half; i += kThreads) {
         const int64_t t = t0 + i / a.half;
@@ -209,7 +210,10 @@ int launch(RArgs a, int32_t head_dim, bool in_place, hipStream_t st) {
     int64_t across = 1;
     if (blocks < 256) across = (per * tpb + kThreads - 1) / kThreads;
     if (across > 256) across = 256;
-    hipLaunchKernelGGL((rotary_kernel<T, V, NEAR, WIDE>), dim3((unsigned)blocks, (unsigned)(across < 1 ? 1 : across)),
+    // a launch's first dimension holds fewer than 2^32 threads: what is left goes along the third
+    constexpr int64_t most = 0xFFFFFFFFLL / kThreads;
+    const int64_t deep = (blocks + most - 1) / most, wide = (blocks + deep - 1) / deep;
+    hipLaunchKernelGGL((rotary_kernel<T, V, NEAR, WIDE>), dim3((unsigned)wide, (unsigned)(across < 1 ? 1 : across), (unsigned)deep),
                        dim3(kThreads), 0, st, a);
     return launch_status("rotary_kernel");
 }

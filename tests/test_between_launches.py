@@ -139,3 +139,16 @@ def test_norm_gain_grids(hook, n):
         assert block[0] == 1024 and w[0] == FAKE + 4 * done
         done += 32 * grid[0]
     assert n <= done < n + 32
+
+
+@pytest.mark.parametrize("tokens,heads,dim,rot,data,pairs", [
+    (2 ** 31 - 1, 1, 64, 64, FAKE, 0), (16_777_300, 1, 2052, 2052, FAKE + 2, 0), (20_000_000, 1, 2100, 4, FAKE + 2, 0), (17_000_000, 32, 128, 128, FAKE, 1),
+    (2 ** 31 - 1, 1, 8, 8, FAKE + 2, 1), (300, 4, 64, 64, FAKE, 0), (1, 28, 256, 64, FAKE, 0)])
+def test_rotary_grids(hook, tokens, heads, dim, rot, data, pairs):
+    """One launch; its workgroups hold all tokens, and a workgroup's table of sines its tokens' pairs."""
+    (grid, _, w), = launches(hook, "rotary", tokens=tokens, hq=heads, dim=dim, rot=rot, data=data, pairs=pairs)
+    each, half = w[14] & 0xFFFFFFFF, w[14] >> 32
+    assert w[13] == tokens and half == rot // 2
+    blocks = grid[0] * grid[2]
+    assert each * half <= 4096 and (blocks - grid[2]) * each < tokens <= blocks * each
+    assert grid[2] == 1 or tokens > 10 ** 6

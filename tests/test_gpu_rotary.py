@@ -143,3 +143,22 @@ def test_pieces_of_every_width(dim, rot, dtype):
         for pairs in ("half", "interleaved"):
             got = rotary(x, None, f, None, pairs=pairs, mscale=m)[0]
             check(x, got, angles, rot, pairs, m, False, f"gap {gap} {pairs}")
+
+
+def test_more_tokens_than_a_launch_takes_across():
+    """Tokens past the first dimension's workgroups: single values of odd places, a token a workgroup, in place."""
+    from r9700training_amd.rotary import rotary, rotary_frequencies
+
+    tokens, dim = 16_777_300, 2052  # 1026 pairs of single values a token
+    f, _ = rotary_frequencies(dim)
+    whole = torch.empty(tokens * dim + 1, dtype=torch.bfloat16, device="cuda")  # 69 GB
+    x = whole[1:].view(tokens, 1, dim)
+    ends = [slice(a, a + 40) for a in (0, 8_388_600, 16_777_200, tokens - 40)]
+    kept = []
+    for i, part in enumerate(ends):
+        x[part] = rnd(i, 40, 1, dim)
+        kept.append(x[part].clone())
+    rotary(x, None, f, q_out=x)
+    for part, was in zip(ends, kept):
+        pos = torch.arange(part.start, part.stop, dtype=torch.int32, device="cuda")
+        assert torch.equal(x[part], rotary(was, None, f, pos)[0]), part
