@@ -132,6 +132,18 @@ __device__ float block_max(float v, float* red) {
     return t;
 }
 
+// 1 / sqrt(mean of h^2 + eps) from sum(f), a row's sum of (f h)^2. f32 holds the squares of values of some 1e-19 to 1e18, and
+// most rows; where the sum leaves its range, upwards or (eps no larger) downwards, it is taken again of the values times a
+// power of two that brings it back. The sum is the same in all the row's threads.
+template <class Sum>
+__device__ __forceinline__ float rstd_of(Sum&& sum, float n, float eps) {
+    const float ss = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, sum(1.0f))));
+    const bool small = ss < 0x1p-90f && eps < 0x1p-90f;
+    if (ss < INFINITY && !small) return 1.0f / sqrtf(ss / n + eps);
+    const float f = small ? 0x1p96f : 0x1p-80f;
+    return f / sqrtf(sum(f) / n + eps * f * f);
+}
+
 // The quantiser of a group with maximum amax: code = rint(y * up * inv). up keeps 127 / amax finite where the
 // group's values are tiny.
 struct Quant {
@@ -170,12 +182,15 @@ __global__ __launch_bounds__(kThreads) void norm_any_kernel(NArgs a) {
     auto h_of = [&](int64_t j) {
         return a.res ? as_stored<T>(ld<T>(a.x, base + j) + ld<T>(a.res, base + j)) : ld<T>(a.x, base + j);
     };
-    float ss = 0.0f;
-    for (int64_t j = threadIdx.x; j < a.n; j += kThreads) {
-        const float h = h_of(j);
-        ss += h * h;
-    }
-    const float rs = 1.0f / sqrtf(block_sum(ss, red) / (float)a.n + a.eps);
+    auto squares = [&](float f) {
+        float ss = 0.0f;
+        for (int64_t j = threadIdx.x; j < a.n; j += kThreads) {
+            const float h = f * h_of(j);
+            ss += h * h;
+        }
+        return block_sum(ss, red);
+    };
+    const float rs = rstd_of(squares, (float)a.n, a.eps);
     if (threadIdx.x == 0 && a.rstd) a.rstd[blockIdx.x] = rs;
     auto y_of = [&](int64_t j) { return h_of(j) * rs * (ld<T>(a.w, j) + a.wadd); };
     // one group: the workgroup's; more: a wave takes whole groups
@@ -330,7 +345,6 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
 #pragma unroll
     for (int i = 0; i < S; ++i) x[i].load(a.x, base + V * (t + i * per), n - V * (t + i * per));
     float h[S][V];
-    float ss = 0.0f;
     if (a.res) {
         P r[S];
 #pragma unroll
@@ -351,12 +365,15 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
             for (int k = 0; k < V; ++k) h[i][k] = x[i].at(k);
         }
     }
+    auto squares = [&](float f) {
+        float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < S; ++i)
+        for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int k = 0; k < V; ++k) ss += h[i][k] * h[i][k];
-    ss = WIDE ? block_sum(ss, red) : wave_sum(ss);
-    const float rs = 1.0f / sqrtf(ss / (float)n + a.eps);
+            for (int k = 0; k < V; ++k) ss += (f * h[i][k]) * (f * h[i][k]);
+        return WIDE ? block_sum(ss, red) : wave_sum(ss);
+    };
+    const float rs = rstd_of(squares, (float)n, a.eps);
     if (t == 0 && a.rstd) a.rstd[row] = rs;
     float top[S];
 #pragma unroll

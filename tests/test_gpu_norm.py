@@ -282,3 +282,39 @@ def test_more_rows_than_a_launch_takes(rows, n, group):
             assert torch.equal(a, b), at
         back, _ = add_rmsnorm_i8g_bwd(h[part].contiguous(), w, rs[part].contiguous(), group, g_y=gy[part].contiguous(), want_dw=False)
         assert torch.equal(dx[part], back), at
+
+
+ENDS = [(64, 0), (512, 128), (2048, 0), (5120, 0), (777, 32), (515, 5), (17408, 256), (17408, 0), (3, 1), (1, 0)]
+
+
+@pytest.mark.parametrize("n,group", ENDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_squares_past_f32(n, group, dtype):
+    """Finite rows whose sum of squares is none in f32: 1 / rms, codes and scales are those of any other row."""
+    print(f"case norm range {(n, group, dtype)}", flush=True)
+    size = torch.tensor([1.0, 1e17, 2e18, 1e19, 3e25, 1e33, 1e37], device="cuda")
+    x = rnd(1, 7, n, dtype=torch.float32) * size[:, None]
+    x[6, ::3] = 3e38
+    forward(7, n, group, dtype, residual=False, x=x.to(dtype))
+
+
+@pytest.mark.parametrize("n,group", ENDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_squares_below_f32(n, group, dtype):
+    """With an eps of 0, or far below the rows' squares, tiny rows are normed like any other."""
+    from r9700training_amd.norm import add_rmsnorm_i8g
+
+    print(f"case norm small {(n, group, dtype)}", flush=True)
+    size = torch.tensor([1.0, 1e-14, 1e-17, 1e-22, 1e-27, 1e-33, 1e-36], device="cuda")
+    x = rnd(1, 7, n, dtype=torch.float32)
+    x = ((x.abs() + 0.5) * x.sign() * size[:, None]).to(dtype)
+    w = (1.0 + 0.2 * rnd(3, n, dtype=torch.float32)).to(dtype)
+    for eps in (0.0, 1e-33):
+        codes, scale, _, y, rs = add_rmsnorm_i8g(x, None, w, group, eps=eps, want_y=True)
+        _, wrs, wy = R.norm(x, None, w, float(torch.tensor(eps)), 0.0, dtype)
+        rel = (n + 8) * R.U32
+        assert bool(((rs.double() - wrs).abs() <= rel * wrs).all()), eps
+        y_tol = (rel + 4 * R.U32) * wy.abs()
+        assert bool(((y.double() - wy).abs() <= y_tol + R.HALF[torch.bfloat16] * wy.abs()).all()), eps
+        each = scale.double()[:, R.group_index(n, group, x.device)]
+        assert bool(((codes.double() * each - wy).abs() <= 0.5 * each + y_tol + 8 * R.U32 * wy.abs() + 1e-300).all()), eps
