@@ -645,7 +645,8 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
  * layer; the norm is taken of h as it is stored, which is what the adjoint reads. codes int8 [rows, n],
  * scale f32 [rows, groups] (both NULL: no codes), y_out bf16 [rows, n] (may be NULL), rstd f32 [rows]
  * (may be NULL). Arithmetic and sums are f32; a row whose squares' sum leaves f32's range is summed once more, scaled, so
- * finite rows of any size are normed (1 / rms has to be an f32). With group 128 codes and scale are gemm_nt_q's operands.
+ * finite rows of any size are normed (1 / rms has to be an f32). A group with a NaN or an infinity in y has a NaN or infinite
+ * scale, and its codes say nothing: what reads them gets no number either. With group 128 codes and scale are gemm_nt_q's operands.
  * h_out may be x or residual. */
 int r97q_add_rmsnorm_i8g(const void* x, const void* residual, const void* w, int32_t dtype, int64_t rows, int64_t n,
                          int64_t group, float eps, float wadd, void* h_out, int8_t* codes, float* scale,

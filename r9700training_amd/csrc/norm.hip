@@ -69,6 +69,9 @@ __device__ __forceinline__ float as_stored(float v) {
         return v;
 }
 
+// the larger value, or the NaN where one is (fmaxf drops it), in one instruction
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+
 // both values of the pair of lanes H apart
 template <int H>
 __device__ __forceinline__ void lane_pair(float v, float& lo, float& hi) {
@@ -94,7 +97,7 @@ template <int H>
 __device__ __forceinline__ float lane_max(float v) {
     float lo, hi;
     lane_pair<H>(v, lo, hi);
-    return fmaxf(lo, hi);
+    return larger(lo, hi);
 }
 __device__ __forceinline__ float wave_sum(float v) {
     return lane_sum<32>(lane_sum<16>(lane_sum<8>(lane_sum<4>(lane_sum<2>(lane_sum<1>(v))))));
@@ -128,7 +131,7 @@ __device__ float block_max(float v, float* red) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     float t = red[0];
-    for (int i = 1; i < waves; ++i) t = fmaxf(t, red[i]);
+    for (int i = 1; i < waves; ++i) t = larger(t, red[i]);
     return t;
 }
 
@@ -145,13 +148,13 @@ __device__ __forceinline__ float rstd_of(Sum&& sum, float n, float eps) {
 }
 
 // The quantiser of a group with maximum amax: code = rint(y * up * inv). up keeps 127 / amax finite where the
-// group's values are tiny.
+// group's values are tiny. A NaN or an infinity goes into the scale, and the codes say nothing then.
 struct Quant {
     float scale, up, inv;
     __device__ __forceinline__ explicit Quant(float amax) {
-        scale = amax > 0.0f ? amax / 127.0f : 1.0f;
+        scale = amax == 0.0f ? 1.0f : amax / 127.0f;
         up = amax < 0x1p-96f ? 0x1p96f : 1.0f;
-        inv = amax > 0.0f ? 127.0f / (amax * up) : 0.0f;
+        inv = amax == 0.0f ? 0.0f : 127.0f / (amax * up);
     }
     __device__ __forceinline__ int code(float y) const { return (int)rintf(y * up * inv); }
     // in one word: up is one of two, and inv is not negative
@@ -199,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void norm_any_kernel(NArgs a) {
     for (int64_t g = one ? 0 : wave; g < a.ngroups; g += one ? 1 : kWaves) {
         const int64_t j0 = g * a.group, j1 = j0 + a.group < a.n ? j0 + a.group : a.n;
         float amax = 0.0f;
-        for (int64_t j = j0 + first; j < j1; j += step) amax = fmaxf(amax, fabsf(y_of(j)));
+        for (int64_t j = j0 + first; j < j1; j += step) amax = larger(amax, fabsf(y_of(j)));
         amax = one ? block_max(amax, red) : wave_max(amax);
         const Quant q(amax);
         if (first == 0 && a.scale) a.scale[blockIdx.x * a.ngroups + g] = q.scale;
@@ -334,7 +337,7 @@ struct Piece {
 template <class T, int S, bool WIDE, int V, bool LOOSE>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, int lg, uint32_t magic) {
     __shared__ float red[kMostWaves];
-    extern __shared__ uint32_t gathered[];  // the groups' maxima, as bits (they are not negative); of single columns then their quantisers
+    extern __shared__ uint32_t gathered[];  // the groups' maxima, as bits (they are not negative, and a NaN's are the largest); of single columns then their quantisers
     const int wave = threadIdx.x >> 6, t = WIDE ? threadIdx.x : threadIdx.x & 63, per = WIDE ? blockDim.x : 64;
     const int64_t row = WIDE ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (row >= a.rows) return;
@@ -383,7 +386,7 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             h[i][k] = h[i][k] * rs * (w[i].at(k) + a.wadd);
-            top[i] = fmaxf(top[i], fabsf(h[i][k]));
+            top[i] = larger(top[i], fabsf(h[i][k]));
         }
         if (a.y) Piece<uint16_t, V, LOOSE>::store(a.y, base + c, n - c, h[i]);
     }
@@ -434,7 +437,7 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
     }
     if (lg == kWhole) {
 #pragma unroll
-        for (int i = 1; i < S; ++i) top[0] = fmaxf(top[0], top[i]);
+        for (int i = 1; i < S; ++i) top[0] = larger(top[0], top[i]);
         top[0] = WIDE ? block_max(top[0], red) : wave_max(top[0]);
 #pragma unroll
         for (int i = 1; i < S; ++i) top[i] = top[0];

@@ -318,3 +318,52 @@ def test_squares_below_f32(n, group, dtype):
         assert bool(((y.double() - wy).abs() <= y_tol + R.HALF[torch.bfloat16] * wy.abs()).all()), eps
         each = scale.double()[:, R.group_index(n, group, x.device)]
         assert bool(((codes.double() * each - wy).abs() <= 0.5 * each + y_tol + 8 * R.U32 * wy.abs() + 1e-300).all()), eps
+
+
+@pytest.mark.parametrize("n,group", [(64, 0), (512, 128), (2048, 64), (5120, 0), (5120, 128), (5120, 1024), (777, 32), (2048, 96), (515, 5), (515, 70), (17408, 256),
+                                     (17408, 0), (7, 1)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_nan_and_infinity_are_kept(n, group, dtype):
+    """A group with a NaN or an infinity in y has it in its scale, so that what reads the codes has it too; other groups and
+    rows are as they were."""
+    from r9700training_amd.norm import add_rmsnorm_i8g
+
+    print(f"case norm nan {(n, group, dtype)}", flush=True)
+    inf, nan, c = float("inf"), float("nan"), n // 2
+    x, r, w = rnd(1, 6, n, dtype=dtype), rnd(2, 6, n, dtype=dtype), rnd(3, n, dtype=dtype)
+    clean = add_rmsnorm_i8g(x, r, w, group, eps=EPS, want_y=True)
+    idx = R.group_index(n, group, x.device)
+    other = torch.arange(int(idx[-1]) + 1, device="cuda") != idx[c]
+    a, b = x.clone(), r.clone()
+    a[1, c], b[2, c], a[3, c], a[4, c] = nan, nan, inf, -inf
+    codes, scale, h, y, rs = add_rmsnorm_i8g(a, b, w, group, eps=EPS, want_y=True)
+    for i in (0, 5):
+        for got, was in zip((codes, scale, h, y, rs), clean):
+            assert torch.equal(got[i], was[i])
+    for i in (1, 2):  # nothing of the row is a number
+        assert bool(rs[i].isnan()) and bool(y[i].isnan().all()) and bool(scale[i].isnan().all())
+    for i in (3, 4):  # 1 / rms is zero: zeros, and a NaN where the infinity is
+        assert float(rs[i]) == 0.0 and bool(y[i, c].isnan()) and int(y[i].isnan().sum()) == 1
+        assert bool(scale[i, idx[c]].isnan()) and bool((scale[i][other] == 1.0).all()) and bool((codes[i, idx != idx[c]] == 0).all())
+    for bad in (nan, inf):
+        v = w.clone()
+        v[c] = bad
+        codes, scale, h, y, rs = add_rmsnorm_i8g(x, r, v, group, eps=EPS, want_y=True)
+        at = scale[:, idx[c]]
+        assert bool(at.isnan().all() if bad != bad else (at == inf).all())
+        assert torch.equal(scale[:, other], clean[1][:, other]) and torch.equal(codes[:, idx != idx[c]], clean[0][:, idx != idx[c]])
+
+
+def test_a_nan_reaches_the_projection():
+    """The codes' product has the NaN of its activation's row, and only that row."""
+    from r9700training_amd.norm import add_rmsnorm_i8g
+    from r9700training_amd.qlinear import gemm_nt_q_fwd
+
+    x, w = rnd(1, 70, 512), rnd(2, 512)
+    b = torch.randint(-127, 128, (256, 512), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda", dtype=torch.int8)
+    bs = torch.full((256, 4), 0.01, device="cuda").to(torch.bfloat16).view(torch.int16)
+    was = gemm_nt_q_fwd(b, bs, *add_rmsnorm_i8g(x, None, w, 128)[:2], y_dtype=torch.float32)
+    x[33, 5] = float("nan")
+    got = gemm_nt_q_fwd(b, bs, *add_rmsnorm_i8g(x, None, w, 128)[:2], y_dtype=torch.float32)
+    keep = torch.arange(70, device="cuda") != 33
+    assert bool(got[33].isnan().all()) and torch.equal(got[keep], was[keep])
