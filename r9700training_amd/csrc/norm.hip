@@ -397,15 +397,12 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_rows_kernel(NArgs a, i
         const int ngroups = (int)a.ngroups;
         for (int i = t; i < ngroups; i += per) gathered[i] = 0;
         __syncthreads();
-        // a wave's 64 columns lie in one group, or two, where those are as wide, and the wave takes their maxima first;
-        // of narrower ones a lane its own
+        // a wave's 64 columns lie in at most two groups where those are wider, and the wave takes their maxima first; of
+        // narrower ones a lane its own
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             const int c = t + i * per, g = (int)__umulhi((uint32_t)c, magic);
-            if (group % 64 == 0) {
-                const float m = wave_max(top[i]);
-                if ((t & 63) == 0 && c < n) atomicMax(&gathered[g], __builtin_bit_cast(uint32_t, m));
-            } else if (group > 64) {
+            if (group > 64) {
                 const int g0 = __builtin_amdgcn_readfirstlane(g);
                 const float m0 = wave_max(g == g0 ? top[i] : 0.0f), m1 = wave_max(g == g0 ? 0.0f : top[i]);
                 if ((t & 63) == 0 && c < n) {
