@@ -367,3 +367,56 @@ def test_a_nan_reaches_the_projection():
     got = gemm_nt_q_fwd(b, bs, *add_rmsnorm_i8g(x, None, w, 128)[:2], y_dtype=torch.float32)
     keep = torch.arange(70, device="cuda") != 33
     assert bool(got[33].isnan().all()) and torch.equal(got[keep], was[keep])
+
+
+@pytest.mark.parametrize("rows,n,group", [(3, 17408, 256), (3, 17408, 0), (2, 9001, 100), (5, 16386, 0), (4, 77, 1), (2, 20000, 20000 - 1)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("by", [0, 1, 3])
+def test_general_kernels_anywhere_and_in_place(rows, n, group, dtype, by):
+    """Rows past the registers, groups of one column: the kernels that read a row again for each stage, with tensors off 16
+    bytes and h over x or the residual."""
+    from r9700training_amd.norm import add_rmsnorm_i8g, add_rmsnorm_i8g_bwd
+
+    print(f"case norm general {(rows, n, group, dtype, by)}", flush=True)
+    x, r, w, codes, scale, h, y, rs = forward(rows, n, group, dtype)
+    for which in (0, 1):
+        (wx, px), (wr, pr) = placed(x, by, 77), placed(r, by, 77)
+        wc, pc = placed(torch.zeros_like(codes), by, 77)
+        got = add_rmsnorm_i8g(px, pr, placed(w, by, 77)[1], group, eps=EPS, want_y=True, codes=pc, h=(px, pr)[which])
+        for a, b in zip(got, (codes, scale, h, y, rs)):
+            assert torch.equal(a, b), which
+        torch.cuda.synchronize()
+        for one in (wx, wr, wc):
+            assert bool((one[:by] == 77).all()) and bool((one[by + x.numel():] == 77).all())
+    gc, gy, gh = (rnd(4 + i, rows, n, dtype=dtype, std=0.05) for i in range(3))
+    dx, dw = add_rmsnorm_i8g_bwd(h, w, rs, group, scale=scale, g_codes=gc, g_y=gy, g_h=gh)
+    wdx, wdw, e = R.norm_backward(h.double(), rs.double(), w, 0.0, scale, group, gc, gy, gh)
+    size = gc.double().abs() / scale.double()[:, R.group_index(n, group, x.device)] + gy.double().abs()
+    we, hx = w.double().abs() * size, (h.double() * rs.double()[:, None]).abs()
+    tol = rs.double()[:, None] * (8 * R.U32 * we + (n + 16) * R.U32 * hx * (we * hx).mean(1, keepdim=True)) + 8 * R.U32 * (wdx.abs() + gh.double().abs())
+    assert bool(((dx.double() - wdx).abs() <= tol + R.HALF[dtype] * wdx.abs() + 1e-30).all())
+    assert bool(((dw.double() - wdw).abs() <= (rows + 8) * R.U32 * (size * hx).sum(0) + 1e-30).all())
+    for k in range(3):  # dx over a cotangent
+        parts = [placed(t, by, 77) for t in (gc, gy, gh)]
+        got = add_rmsnorm_i8g_bwd(placed(h, by, 77)[1], w, rs, group, scale=scale, g_codes=parts[0][1], g_y=parts[1][1], g_h=parts[2][1], dx=parts[k][1])
+        assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+        assert all(bool((one[:by] == 77).all()) and bool((one[by + x.numel():] == 77).all()) for one, _ in parts)
+
+
+@pytest.mark.parametrize("rows,n,group", [(1100, 40, 1), (513, 17408, 256)])
+def test_general_kernels_many_rows(rows, n, group):
+    """More rows than the gain's partial sums: a workgroup adds its second row to its first, in the same order each time."""
+    from r9700training_amd.norm import add_rmsnorm_i8g_bwd
+
+    print(f"case norm general rows {(rows, n, group)}", flush=True)
+    _, _, w, _, scale, h, _, rs = forward(rows, n, group, torch.bfloat16)
+    gy = rnd(5, rows, n)
+    dx, dw = add_rmsnorm_i8g_bwd(h, w, rs, group, g_y=gy)
+    wdx, wdw, e = R.norm_backward(h.double(), rs.double(), w, 0.0, scale, group, None, gy, None)
+    hx = (h.double() * rs.double()[:, None]).abs()
+    assert bool(((dw.double() - wdw).abs() <= (rows + 8) * R.U32 * (e.abs() * hx).sum(0)).all())
+    we = (w.double() * e).abs()
+    tol = rs.double()[:, None] * (8 * R.U32 * we + (n + 16) * R.U32 * hx * (we * hx).mean(1, keepdim=True)) + 8 * R.U32 * wdx.abs()
+    assert bool(((dx.double() - wdx).abs() <= tol + R.HALF[torch.bfloat16] * wdx.abs() + 1e-30).all())
+    again = add_rmsnorm_i8g_bwd(h, w, rs, group, g_y=gy)
+    assert torch.equal(dx, again[0]) and torch.equal(dw, again[1])
