@@ -467,3 +467,59 @@ def test_a_grid_cut_short():
         out[longest] = (o, lse) + attention_bwd(q, k, v, o, lse, do, **kw)
         torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(out[300], out[131072]))
+
+
+PACKED_CUT = [
+    # query lengths, key lengths, q_heads, kv_heads, causal, window: the mean of the keys is what the cuts go by, so the long
+    # sequences' last range takes more than its share, and the short ones leave ranges empty
+    ([1, 3, 1], [5000, 1, 1700], 8, 2, True, 0),
+    ([40, 70], [4500, 300], 4, 2, True, 0),
+    ([5, 0, 33, 2], [0, 1500, 7000, 40], 6, 2, True, 0),
+    ([40, 70], [4500, 300], 4, 1, False, 0),
+    ([60, 90], [3000, 5000], 2, 1, True, 2100),
+    ([200, 3], [2500, 2400], 2, 2, True, 0),
+]
+
+
+def cut_of(lq, lk, hq, hk, d, causal, window):
+    """Whether the forward's keys and dQ's keys are cut, from the sizes of the workspaces."""
+    from r9700training_amd import AttnShape, lib
+
+    s = AttnShape(batch=len(lq), head_dim=d, q_len=max(lq), kv_len=max(lk), q_starts=1 << 20, kv_starts=1 << 20, q_tokens=sum(lq),
+                  kv_tokens=sum(lk), causal=causal, window=window, scale=1.0)
+    slots = hq * sum(lq)
+    parts = lib().r97q_attn_bwd_workspace_bytes(s, hq, hk) - (8 * slots + 255) // 256 * 256
+    return lib().r97q_attn_fwd_workspace_bytes(s, hq, hk) > 0, parts >= 2 * slots * d * 4
+
+
+@pytest.mark.parametrize("lq,lk,hq,hk,causal,window", PACKED_CUT)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_packed_and_cut(lq, lk, hq, hk, d, causal, window):
+    print(f"case packed cut {(lq, lk, hq, hk, d, causal, window)}", flush=True)
+    assert all(cut_of(lq, lk, hq, hk, d, causal, window))
+    qs = torch.tensor([0] + lq).cumsum(0).to(torch.int32).cuda()
+    ks = torch.tensor([0] + lk).cumsum(0).to(torch.int32).cuda()
+    q, do = rnd(1, sum(lq), hq, d), rnd(4, sum(lq), hq, d)
+    k, v = rnd(2, sum(lk), hk, d), rnd(3, sum(lk), hk, d)
+    seqs, a, b = [], 0, 0
+    for x, y in zip(lq, lk):
+        seqs.append(Packed(a, a + x, b, b + y))
+        a, b = a + x, b + y
+    run(q, k, v, do, seqs, hq, hk, causal, window, 1.0 / math.sqrt(d), q_starts=qs, kv_starts=ks, max_q=max(lq), max_kv=max(lk))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lq", [1, 40])
+def test_cache_cut_with_lengths(lq, d):
+    """A dense cache cut along the keys whose sequences end before, inside and after the ranges; its unused places are NaN."""
+    lens = [3000, 0, 700, 41, 1537]
+    q, do = rnd(1, 5, lq, 4, d), rnd(4, 5, lq, 4, d)
+    k, v = rnd(2, 5, 3000, 2, d), rnd(3, 5, 3000, 2, d)
+    for i, n in enumerate(lens):
+        k[i, n:] = float("nan")
+        v[i, n:] = float("nan")
+    got = run(q, k, v, do, [Dense(i, n) for i, n in enumerate(lens)], 4, 2, True, 0, 0.09,
+              kv_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    for g in got[3:]:
+        for i, n in enumerate(lens):
+            assert torch.equal(g[i, n:], torch.zeros_like(g[i, n:]))
