@@ -599,7 +599,9 @@ int r97q_rotary_frequencies(int32_t rot, double base, int32_t scaling, double fa
  * The last query stands at the last key: query i of a sequence with n queries and m keys sees key j when
  * not causal, or when j <= i + m - n and, with a window, j > i + m - n - window. A query that sees no key
  * gives zeros, a log-sum-exp of minus infinity and zero gradients. Keys and values past a sequence's
- * length are not read. A NaN or infinity that some query of a tile sees may reach the tile's other rows.
+ * length or before every query's window may hold anything. A NaN or infinity in a key or value that some
+ * query of a tile (up to 128 tokens) sees may reach the tile's other rows, one in a query or its cotangent
+ * the gradients of keys beside those that the query sees.
  * Too small a longest length of packed tokens costs time, not results. At most 65535 sequences and key heads,
  * and 2^23 query heads in all the sequences. */
 typedef struct R97qAttnShape {

@@ -55,7 +55,9 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
                 kr.step(32);
             }
         }
-        load_row<D>(kv_at(a.v, a, s, hk) + 2 * (kk * a.v.ts), key < s.lk, fresh(a.d), lane, v);
+        // the values of keys before every query's window may hold anything, and their gradients are zero
+        const int seen0 = a.window ? (int)clamp64((int64_t)s.off - a.window + 1, 0, s.lk) : 0;
+        load_row<D>(kv_at(a.v, a, s, hk) + 2 * (kk * a.v.ts), key >= seen0 && key < s.lk, fresh(a.d), lane, v);
         settle(v);
         if constexpr (KEPT) settle(k);
         // the tokens [t0, t1) that see any of the workgroup's keys, from a tile's first

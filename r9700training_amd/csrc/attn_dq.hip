@@ -51,7 +51,7 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
         const Keys all = keys_of(a, s, w0 / a.g, wend / a.g);
         const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
         const Keys own = keys_of(a, s, (r0 < rows ? r0 : rows - 1) / a.g, rend / a.g);
-        int lo = all.lo / KT * KT, hi = all.hi;
+        int lo = all.lo, hi = all.hi;
         if (a.q_splits > 1 && lo < hi) {  // this range's tiles
             const int nt = (hi - lo + KT - 1) / KT, from = (int)((int64_t)nt * split / a.q_splits), to = (int)((int64_t)nt * (split + 1) / a.q_splits);
             hi = to * KT < hi - lo ? lo + to * KT : hi;
@@ -291,6 +291,12 @@ __global__ __launch_bounds__(256, PER) void attn_dq_kept_kernel(Args a) {
             landed();
             __syncthreads();
             load(1 - slot);
+            if (j0 < all.lo) {  // keys before the first that is seen, in its block: they may hold anything, also in dS^T
+                const int none = all.lo - j0 < KT ? all.lo - j0 : KT;
+                for (int i = 16 * tid; i < none * 2 * D; i += 16 * 256) *reinterpret_cast<u32x4*>(lds + slot * SLOT + i) = (u32x4){};
+                for (int i = 16 * tid; i < none * 256; i += 16 * 256) *reinterpret_cast<u32x4*>(lds + slot * SLOT + TB + i) = (u32x4){};
+                __syncthreads();
+            }
             if ((j0 & 127) == 0) {
                 int t0, t1;
                 tokens_of(a, s, j0, RT, t0, t1);

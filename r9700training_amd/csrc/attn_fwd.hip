@@ -192,7 +192,7 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
         const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
         Keys own = keys_of(a, s, (r0 < rows ? r0 : rows - 1) / a.g, rend / a.g);
         if (r0 >= rows) own.hi = own.lo;
-        int lo = all.lo / KT * KT, hi = all.hi;
+        int lo = all.lo, hi = all.hi;  // from the first key that is seen: what lies before it may hold anything
         if (a.splits > 1) {
             lo = (int)clamp64((int64_t)lo + (int64_t)split * a.chunk, lo, hi);
             if (split < a.splits - 1 && hi - lo > a.chunk) hi = lo + a.chunk;  // the last range takes what is left
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
         const Row row(a, hk, r0 + col, rows);
         const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
         const Keys keys = keys_of(a, s, r0 / a.g, rend / a.g);
-        int lo = keys.lo / KT * KT, hi = keys.hi;
+        int lo = keys.lo, hi = keys.hi;
         if (a.splits > 1) {
             lo = (int)clamp64((int64_t)lo + (int64_t)split * a.chunk, lo, hi);
             if (split < a.splits - 1 && hi - lo > a.chunk) hi = lo + a.chunk;  // the last range takes what is left

@@ -523,3 +523,74 @@ def test_cache_cut_with_lengths(lq, d):
     for g in got[3:]:
         for i, n in enumerate(lens):
             assert torch.equal(g[i, n:], torch.zeros_like(g[i, n:]))
+
+
+UNSEEN = [
+    # batch, q_len, kv_len, lengths in use, q_heads, kv_heads, head_dim, window: the first keys are before every window
+    (2, 1, 300, [300, 211], 4, 1, 64, 50),
+    (2, 1, 5000, [5000, 3333], 8, 2, 128, 1300),
+    (1, 5, 4000, [3999], 4, 1, 256, 1001),
+    (2, 40, 700, [700, 457], 4, 2, 128, 100),
+    (1, 200, 450, [450], 2, 1, 256, 77),
+    (1, 200, 450, [449], 2, 1, 64, 77),
+    (1, 150, 400, [390], 4, 1, 128, 33),
+    (1, 40, 4000, [3990], 2, 1, 64, 1500),
+]
+
+
+@pytest.mark.parametrize("b,lq,lk,lens,hq,hk,d,window", UNSEEN)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_keys_before_every_window(b, lq, lk, lens, hq, hk, d, window, bad):
+    """What no query sees is not read into anything, whatever it holds: a cache's expired keys, at any place in a tile."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    print(f"case unseen {(b, lq, lk, lens, hq, hk, d, window, bad)}", flush=True)
+    q, do = rnd(1, b, lq, hq, d), rnd(4, b, lq, hq, d)
+    clean = [rnd(2, b, lk, hk, d), rnd(3, b, lk, hk, d)]
+    dirty = [t.clone() for t in clean]
+    for i, n in enumerate(lens):
+        for t, x in ((clean, 0.0), (dirty, bad)):
+            for y in t:
+                y[i, :n - lq - window + 1] = x
+                y[i, n:] = x
+    kw = dict(window=window, kv_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    res = []
+    for k, v in (clean, dirty):
+        out, lse = attention_fwd(q, k, v, **kw)
+        res.append((out, lse) + attention_bwd(q, k, v, out, lse, do, **kw))
+    for name, x, y in zip(("out", "lse", "dq", "dk", "dv"), *res):
+        assert torch.equal(x, y), name
+    for i, n in enumerate(lens):
+        for g in res[1][3:]:
+            assert not g[i, :n - lq - window + 1].any()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_nan_reaches_no_tile_past_its_window(d, packed):
+    """A NaN key that the queries 390 .. 489 see: tiles of queries from 512 on begin inside its block of keys and do not see
+    it, and are as without it; likewise the gradients of keys that only those queries see."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    n, window = 700, 100
+    q, do = rnd(1, 1, n, 4, d), rnd(4, 1, n, 4, d)
+    k, v = rnd(2, 1, n, 2, d), rnd(3, 1, n, 2, d)
+    kw = dict(window=window)
+    if packed:
+        q, k, v, do = (t[0] for t in (q, k, v, do))
+        at = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        kw.update(q_starts=at, kv_starts=at, max_q=n, max_kv=n)
+    res = []
+    for bad in (False, True):
+        if bad:
+            k, v = k.clone(), v.clone()
+            for t in (k, v):
+                (t if packed else t[0])[390] = float("nan")
+        out, lse = attention_fwd(q, k, v, **kw)
+        grads = attention_bwd(q, k, v, out, lse, do, **kw)
+        res.append([t if packed else t[0] for t in (out, *grads)] + [(lse if packed else lse[0]).t()])
+    for name, x, y in zip(("out", "dq", "dk", "dv", "lse"), *res):
+        first = 640 if name in ("dk", "dv") else 512
+        assert torch.equal(x[first:], y[first:]), name
+        assert torch.equal(x[:256], y[:256]), name
+        assert bool(y[400:480].isnan().any()), name
