@@ -594,3 +594,20 @@ def test_a_nan_reaches_no_tile_past_its_window(d, packed):
         assert torch.equal(x[first:], y[first:]), name
         assert torch.equal(x[:256], y[:256]), name
         assert bool(y[400:480].isnan().any()), name
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_longest_too_short_and_bad_starts_with_kept_scores(d):
+    """Wider heads keep dS^T between the launches, a row of it for each key: neither a longest length that is too small nor
+    starts that leave the tensors change the results. (A length of a few rows takes the few rows' forward, which adds in
+    another order: held to the reference. Otherwise the bits are the same.)"""
+    n = 700
+    q, k, v, do = rnd(1, n, 4, d), rnd(2, n, 2, d), rnd(3, n, 2, d), rnd(4, n, 4, d)
+    good = torch.tensor([0, 430, 430, n], dtype=torch.int32, device="cuda")
+    wild = torch.tensor([-(2 ** 31), 430, 430, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    seqs = [Packed(0, 430, 0, 430), Packed(430, n, 430, n)]
+    want = {}
+    for starts, longest in ((good, 430), (good, 100), (good, 0), (wild, 430), (wild, 1)):
+        got = run(q, k, v, do, seqs, 4, 2, True, 0, 1.0 / math.sqrt(d), q_starts=starts, kv_starts=starts, max_q=longest, max_kv=longest)
+        first = want.setdefault(longest > 16, got)
+        assert all(torch.equal(x, y) for x, y in zip(first, got)), longest
