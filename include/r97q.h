@@ -598,10 +598,10 @@ int r97q_rotary_frequencies(int32_t rot, double base, int32_t scaling, double fa
  * the tensors are clamped to them.
  * The last query stands at the last key: query i of a sequence with n queries and m keys sees key j when
  * not causal, or when j <= i + m - n and, with a window, j > i + m - n - window. A query that sees no key
- * gives zeros, a log-sum-exp of minus infinity and zero gradients. Keys and values past a sequence's
- * length or before every query's window may hold anything. A NaN or infinity in a key or value that some
- * query of a tile (up to 128 tokens) sees may reach the tile's other rows, one in a query or its cotangent
- * the gradients of keys beside those that the query sees.
+ * gives zeros, a log-sum-exp of minus infinity and, where it and its cotangent are finite, zero gradients.
+ * Keys and values past a sequence's length or before every query's window may hold anything. A NaN or
+ * infinity in a key or value that some query of a tile (up to 128 tokens) sees may reach the tile's other
+ * rows, one in a query or its cotangent the gradients of keys beside those that the query sees.
  * Too small a longest length of packed tokens costs time, not results. At most 65535 sequences and key heads,
  * and 2^23 query heads in all the sequences. */
 typedef struct R97qAttnShape {
@@ -631,7 +631,8 @@ int r97q_attn_fwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
  * scores' gradients are rounded to bf16 for their products, all sums are f32. Repeated calls give the same
  * bits. The dense form's keys past kv_lens get zero gradients. The workspace (on 16 bytes) holds two f32 a
  * query and head, f32 partial sums where the work is cut, and with heads of more than 64 columns the scores'
- * gradients in bf16 where that takes at most 2 GiB. */
+ * gradients in bf16, every query's for every key whatever the mask leaves of them, where that takes at most
+ * 2 GiB, and with up to 128 columns the sequences' own part of it at most 256 MiB. */
 int64_t r97q_attn_bwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads);
 int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
                   const R97qHeads* out, const float* lse, const R97qHeads* d_out, const R97qHeads* dq,
@@ -646,9 +647,10 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
  * x, residual, w and h_out are `dtype` (bf16 or f32), h_out [rows, n] the residual stream for the next
  * layer; the norm is taken of h as it is stored, which is what the adjoint reads. codes int8 [rows, n],
  * scale f32 [rows, groups] (both NULL: no codes), y_out bf16 [rows, n] (may be NULL), rstd f32 [rows]
- * (may be NULL). Arithmetic and sums are f32; a row whose squares' sum leaves f32's range is summed once more, scaled, so
- * finite rows of any size are normed (1 / rms has to be an f32). A group with a NaN or an infinity in y has a NaN or infinite
- * scale, and its codes say nothing: what reads them gets no number either. With group 128 codes and scale are gemm_nt_q's operands.
+ * (may be NULL). Arithmetic and sums are f32; a row whose squares' sum leaves f32's range is summed once
+ * more, scaled, so finite rows of any size are normed (1 / rms has to be an f32). A group with a NaN or an
+ * infinity in y has a NaN or infinite scale, and its codes say nothing: what reads them gets no number
+ * either. With group 128 codes and scale are gemm_nt_q's operands.
  * h_out may be x or residual. */
 int r97q_add_rmsnorm_i8g(const void* x, const void* residual, const void* w, int32_t dtype, int64_t rows, int64_t n,
                          int64_t group, float eps, float wadd, void* h_out, int8_t* codes, float* scale,

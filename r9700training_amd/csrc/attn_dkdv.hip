@@ -14,10 +14,11 @@ namespace {
 // next tile has landed a step early and its first operands are read before the step's barrier. STORE: dS^T is written out for
 // dQ's launch.
 //
-// Bound by the matrix cores and the instructions a wave issues beside them. At 128 columns and more the gradients, values and
-// keys leave room for one wave a SIMD, whose instructions take some 4.6 cycles each: a step of 64 tokens at 128 columns is
-// 730 of them and 64 products, 1.55 us. 8 x 2048 tokens causal, 16 over 4 heads of 64 174 us (790 TFLOP/s of the four
-// products), of 128 290 us (950), of 256 565 us (970), these at the clock that the card's power leaves.
+// Bound by the products and what one wave issues beside them. At 128 columns and more the gradients, values and keys leave room
+// for one wave a SIMD: a step of 64 tokens at 128 columns is 64 products of 32 cycles among some 470 other instructions (200
+// vector, 112 LDS), 1.55 us at 2.4 GHz. 8 x 2048 tokens causal, 16 over 4 heads, counted over the launch: of 64 175 us (785 TFLOP/s
+// of the four products; matrix cores busy 38%, vector instructions at 4 cycles each 26%, a wave waits 24%), of 128 276 .. 298 us
+// (920 .. 1000; 48%, 19%, 27%), of 256 555 .. 605 us (910 .. 990; 51%, 14%, 24%), at 2.0 GHz; no LDS bank conflicts.
 template <int D, int RT, int NW, bool KEPT, int PER, int SLOTS, bool STORE>
 __global__ __launch_bounds__(64 * NW, PER) void attn_dkdv_kernel(Args a) {
     using T = Tile<D>;

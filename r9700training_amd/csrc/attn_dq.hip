@@ -21,9 +21,9 @@ namespace {
 // the scores j + 1 beside dS_j, then dQ += dS_j K_j. At its top the values up to j + 1 and the keys up to j + 2 have
 // landed, and the slots of the values j - 1 and the keys j - 1 are free for the next loads. Every product's LDS operand
 // is read kAhead products before it, the first ones of step j + 1 in step j.
-// Bound by the matrix cores and the instructions beside them, like the forward: 8 x 2048 tokens causal, 16 over 4 heads of
-// 64 128 us (800 TFLOP/s of the three products), of 128 240 us (860). Tiles of 32 keys: a wave holds its queries, dO and
-// sums, 2 D registers a lane, and has no room for more scores.
+// Bound like the forward: 8 x 2048 tokens causal, 16 over 4 heads of 64 127 us (810 TFLOP/s of the three products; the matrix cores
+// busy 38% of the cycles, vector instructions 42%), of 128 240 us (860; 42% and 29%, a wave waits 38% of its time). Tiles of 32
+// keys: a wave holds its queries, dO and sums, 2 D registers a lane, and has no room for more scores.
 template <int D, int NW, int PER>
 __global__ __launch_bounds__(64 * NW, PER) void attn_dq_kernel(Args a) {
     using T = Tile<D>;
@@ -250,8 +250,9 @@ __global__ __launch_bounds__(256) void attn_base_kernel(Args a, int lanes) {
 // dQ^T = scale K^T dS^T for 128 tokens of a query head: 32 of them a wave. The keys and dS^T's rows of the same keys go
 // through two slots of LDS, both read transposed. dS^T is written for blocks of 128 keys and RT tokens where any
 // of them sees any; a wave passes over the others. No mask: an unseen pair's dS is zero.
-// Bound by dS^T's way from memory beside the products: 8 x 2048 tokens causal, 16 over 4 heads of 256 207 us (660 TFLOP/s
-// and 2.7 TB/s of dS^T); 4 x 2048, heads of 128 75 us (460 and 3.6).
+// Twice its floor, and what holds it is not known: 8 x 2048 tokens causal, 16 over 4 heads of 256 207 us (660 TFLOP/s and 2.7
+// TB/s of dS^T; the matrix cores are busy 30% of the cycles, a wave waits 60% of its time); 4 x 2048, heads of 128 75 us (460 and
+// 3.6).
 template <int D, int KT, int PER, int RT>
 __global__ __launch_bounds__(256, PER) void attn_dq_kept_kernel(Args a) {
     using F = Frags<D>;

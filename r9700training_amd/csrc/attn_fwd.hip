@@ -159,11 +159,13 @@ __device__ __forceinline__ void finish(const Args& a, const Seq& s, const Row& r
 // of tile j + 1 and the values of tile j have landed, and both of tile j - 1's slots are free for the loads of tiles
 // j + 2 and j + 1. Every LDS operand is read kAhead products before its use.
 //
-// Bound by the matrix cores and, beside them, by the instructions a wave issues: at 128 columns 48 products of 32 cycles in
-// some 590 instructions, two waves a SIMD, at the 1.7 GHz that the card's power leaves. 64 keys a tile (32 at 256 columns,
-// where a wave's sums and queries fill its registers and one wave a SIMD remains): 8 x 2048 tokens causal, 32 over 8 heads
-// of 128 300 us, 920 TFLOP/s; 16 over 4 heads of 256 354 us, 780; of 64 93 us, 740. Two waves that share 32 rows and halve
-// their keys were 6 .. 10% faster on grids of under 256 workgroups only, and are not built.
+// Bound by products and vector instructions that two waves a SIMD overlap in part: a step at 128 columns is 32 products of 32
+// cycles among some 190 vector, 48 LDS and 50 scalar instructions. Counted over 8 x 2048 tokens causal, 32 over 8 heads of
+// 128: the matrix cores are busy 48% of the cycles, vector instructions at 4 cycles each make 35%, a wave waits (for loads,
+// LDS, the barrier) 23% of its time, no LDS bank conflicts, 1.9 GHz. 64 keys a tile (32 at 256 columns, where a wave's sums
+// and queries fill its registers and one wave a SIMD remains: 33% and 20%): 302 .. 312 us, 880 .. 910 TFLOP/s; 16 over 4 heads
+// of 256 350 .. 390 us, 705 .. 785; of 64 94 .. 100 us, 690 .. 730 (32% and 45%, 11 vector instructions a product). Two waves
+// that share 32 rows and halve their keys were 6 .. 10% faster on grids of under 256 workgroups only, and are not built.
 template <int D, int KT, int NW, int PER>
 __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     using T = Tile<D>;
