@@ -611,3 +611,24 @@ def test_longest_too_short_and_bad_starts_with_kept_scores(d):
         got = run(q, k, v, do, seqs, 4, 2, True, 0, 1.0 / math.sqrt(d), q_starts=starts, kv_starts=starts, max_q=longest, max_kv=longest)
         first = want.setdefault(longest > 16, got)
         assert all(torch.equal(x, y) for x, y in zip(first, got)), longest
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("packed", [False, True])
+def test_no_queries(d, packed):
+    """Nothing to answer: empty outputs, and every key's gradient is zero."""
+    from r9700training_amd.attention import attention_bwd, attention_fwd
+
+    q, k, v = rnd(1, 2, 0, 4, d), rnd(2, 2, 150, 2, d), rnd(3, 2, 150, 2, d)
+    kw = {}
+    if packed:
+        q, k, v = q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1)
+        kw = dict(q_starts=torch.zeros(3, dtype=torch.int32, device="cuda"), kv_starts=torch.tensor([0, 150, 300], dtype=torch.int32, device="cuda"),
+                  max_q=0, max_kv=150)
+    for longest in (0, 7):
+        if packed:
+            kw["max_q"] = longest
+        out, lse = attention_fwd(q, k, v, **kw)
+        dk, dv = (torch.full_like(k, float("nan")) for _ in range(2))
+        dq, dk, dv = attention_bwd(q, k, v, out, lse, q.clone(), dk=dk, dv=dv, **kw)
+        assert out.shape == dq.shape == q.shape and not dk.any() and not dv.any()
