@@ -577,6 +577,13 @@ typedef struct R97qHeads {
 int r97q_rotary(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, const R97qHeads* k_out,
                 int64_t tokens, int32_t head_dim, int32_t rot, int32_t pairs, const double* inv_freq,
                 const void* positions, int32_t positions64, float mscale, int32_t inverse, R97IqrStream stream);
+/* The same with several axes (time, height and width of images and video): a token has a position on each of `axes`
+ * axes, positions[a * axis_stride + t], and pair i turns by its own axis's, pair_axis[i] (device int32 [rot/2]; a pair
+ * whose axis is none of them is only scaled). The adjoint, types, strides and outputs are r97q_rotary's. */
+int r97q_rotary_axes(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, const R97qHeads* k_out,
+                     int64_t tokens, int32_t head_dim, int32_t rot, int32_t pairs, const double* inv_freq,
+                     const int32_t* pair_axis, int32_t axes, const void* positions, int32_t positions64,
+                     int64_t axis_stride, float mscale, int32_t inverse, R97IqrStream stream);
 /* The frequencies on the host: f[i] = base^(-2i/rot), then for a context `factor` times the `original`
  * length (in positions) the model was trained on:
  *   R97Q_ROTARY_LINEAR  f / factor (positions stretched)
@@ -638,6 +645,35 @@ int r97q_attn_bwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
                   const R97qHeads* out, const float* lse, const R97qHeads* d_out, const R97qHeads* dq,
                   const R97qHeads* dk, const R97qHeads* dv, void* workspace, int64_t workspace_bytes,
                   R97IqrStream stream);
+
+/* A paged cache: k and v are pools of `pages` pages of page_size tokens (a power of two, 8 to 2^20), bf16, as R97qHeads
+ * whose batch_stride goes from page to page and token_stride from token to token of a page: [pages, slots, heads, d] or
+ * [pages, heads, slots, d]. Token j of sequence b lies in slot j mod page_size of page table[b * table_stride + j /
+ * page_size] (device int32; a row holds max_pages entries, of which the sequence's own are read). The shape's kv_lens
+ * (required, clamped to max_pages * page_size) are the tokens that the sequences have; its kv_len is the longest of them,
+ * for the plan: too small or too large a number costs time, not results. Several entries may name one page (a shared
+ * beginning). An entry outside the pool reads as keys and values of zeros. */
+typedef struct R97qPages {
+    const int32_t* table;
+    int64_t table_stride;
+    int64_t pages;
+    int32_t page_size;
+    int32_t max_pages;
+} R97qPages;
+/* r97q_attn_fwd over a paged cache: one new token of each sequence, or a chunk of them (dense or packed), which stand at
+ * the sequence's end. Masks, types, workspace, sums and what an unused or expired place may hold are r97q_attn_fwd's; the
+ * entries of pages that no query sees may hold anything too. */
+int64_t r97q_paged_attn_fwd_workspace_bytes(const R97qAttnShape* shape, const R97qPages* pages, int32_t q_heads,
+                                            int32_t kv_heads);
+int r97q_paged_attn_fwd(const R97qAttnShape* shape, const R97qPages* pages, const R97qHeads* q, const R97qHeads* k,
+                        const R97qHeads* v, const R97qHeads* out, float* lse, void* workspace, int64_t workspace_bytes,
+                        R97IqrStream stream);
+/* The new tokens' keys and values into the pools: the shape is the attention's that follows (its q_len or q_starts say how
+ * many new tokens a sequence has, its kv_lens count them already), so token i of n goes to position kv_lens[b] - n + i. k
+ * and v are both bf16 or both f32 (rounded once). A token whose position is negative or has no page is left out; what the
+ * new tokens do not take of a page stays as it was. Two tokens for one place leave either. */
+int r97q_paged_write(const R97qAttnShape* shape, const R97qPages* pages, const R97qHeads* k, const R97qHeads* v,
+                     const R97qHeads* k_pages, const R97qHeads* v_pages, R97IqrStream stream);
 
 /* The residual's addition, the RMS norm and the group quantiser in one pass over rows of n values:
  *   h = x + residual rounded to dtype (residual NULL: h is x, and h_out is not written),

@@ -101,6 +101,13 @@ class AttnShape(C.Structure):
                 ("scale", C.c_float)]
 
 
+class Pages(C.Structure):
+    """R97qPages (include/r97q.h): a paged cache's table and sizes."""
+
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_int64), ("pages", C.c_int64), ("page_size", C.c_int32),
+                ("max_pages", C.c_int32)]
+
+
 R97_ENC_STR = 32
 R97_ENC_MAX_PLANES = 8
 # R97EncDtype (include/r97q.h)
@@ -197,10 +204,14 @@ SIGNATURES = {
     "r97q_rotary": (C.c_int, [_H, _H, _H, _H, _I, _i, _i, _i, _P, _P, _i, C.c_float, _i, _P]),
     "r97q_rotary_frequencies": (C.c_int, [_i, C.c_double, _i, C.c_double, C.c_double, C.c_double, C.c_double, _P,
                                           C.POINTER(C.c_float)]),
+    "r97q_rotary_axes": (C.c_int, [_H, _H, _H, _H, _I, _i, _i, _i, _P, _P, _i, _P, _i, _I, C.c_float, _i, _P]),
     "r97q_attn_fwd_workspace_bytes": (_I, [C.POINTER(AttnShape), _i, _i]),
     "r97q_attn_fwd": (C.c_int, [C.POINTER(AttnShape), _H, _H, _H, _H, _P, _P, _I, _P]),
     "r97q_attn_bwd_workspace_bytes": (_I, [C.POINTER(AttnShape), _i, _i]),
     "r97q_attn_bwd": (C.c_int, [C.POINTER(AttnShape), _H, _H, _H, _H, _P, _H, _H, _H, _H, _P, _I, _P]),
+    "r97q_paged_attn_fwd_workspace_bytes": (_I, [C.POINTER(AttnShape), C.POINTER(Pages), _i, _i]),
+    "r97q_paged_attn_fwd": (C.c_int, [C.POINTER(AttnShape), C.POINTER(Pages), _H, _H, _H, _H, _P, _P, _I, _P]),
+    "r97q_paged_write": (C.c_int, [C.POINTER(AttnShape), C.POINTER(Pages), _H, _H, _H, _H, _P]),
     "r97q_add_rmsnorm_i8g": (C.c_int, [_P, _P, _P, _i, _I, _I, _I, C.c_float, C.c_float, _P, _P, _P, _P, _P, _P]),
     "r97q_add_rmsnorm_i8g_bwd_workspace_bytes": (_I, [_I, _I]),
     "r97q_add_rmsnorm_i8g_bwd": (C.c_int, [_P, _P, _i, _I, _I, _I, C.c_float, _P, _P, _P, _P, _P, _P, _P, _i, _P, _I,

@@ -80,6 +80,12 @@ struct Args {
     int64_t slots;       // rows of one range: every query head's
     float* part;         // [splits][slots][d]
     float2* stats;       // [splits][slots]
+    // a paged cache: k and v are pools of pages (bs: values from page to page, ts: from token to token in one), and a sequence's
+    // tokens lie in the pages that its row of the table names
+    const int32_t* table;
+    int64_t table_stride;
+    int32_t pages, max_pages, page_shift;
+    int32_t held;        // the longest sequence's keys, for the plan
 };
 
 // What the launches are cut by: tiles of `tile` rows or keys in all sequences together, and a sequence's tokens. Packed
@@ -371,6 +377,51 @@ struct Rows {
     }
 };
 
+// The same of a sequence's tokens in pages. A wave holds 64 entries of the sequence's row of the table, a lane's each, and the
+// next 64 on their way: tiles begin at multiples of their size, so a tile's pages are of one such block. An entry outside the
+// pool reads as zeros, like a token past the end.
+struct PageRows {
+    uint64_t base, page;  // the head in page 0; bytes from page to page
+    const int32_t* table; // the sequence's row
+    uint32_t ts, tail;
+    uint32_t pos;         // the next tile's first token
+    int from, end;        // tokens to read
+    int shift, pages, max_pages;
+    uint32_t block;
+    int ent, next;        // the lane's entries of the block and of the one after it
+    __device__ __forceinline__ PageRows(const Args& a, const Seq& s, const Heads& t, int h, int row0, int from_, int rows, int d)
+        : base(reinterpret_cast<uint64_t>(t.data) + 2 * h * t.hs), page(2 * t.bs), table(a.table + s.b * a.table_stride),
+          ts((uint32_t)(2 * t.ts)), tail(2 * d), pos(row0), from(from_), end(rows), shift(a.page_shift), pages(a.pages),
+          max_pages(a.max_pages) {
+        block = pos >> shift >> 6;
+        ent = fetch(block);
+        next = fetch(block + 1);
+    }
+    __device__ __forceinline__ int fetch(uint32_t b) const {
+        const uint32_t i = 64 * b + (threadIdx.x & 63);
+        return i < (uint32_t)max_pages ? table[i] : -1;
+    }
+    __device__ __forceinline__ int size() const { return 1 << shift; }
+    __device__ __forceinline__ void step(int tokens) { pos += tokens; }
+    __device__ __forceinline__ void turn() {
+        const uint32_t b = pos >> shift >> 6;
+        if (b == block) return;
+        block = b;
+        ent = next;
+        next = fetch(b + 1);
+    }
+    // R tokens from the tile's token `first` on, at the tile's offsets
+    template <int R>
+    __device__ __forceinline__ u32x4 buffer(int first) const {
+        const uint32_t at = pos + first;
+        const int e = __builtin_amdgcn_readlane(ent, (int)(at >> shift) & 63), left = end - (int)at;
+        const uint64_t p = base + (uint64_t)(uint32_t)e * page + (int64_t)((int)(at & (size() - 1)) - first) * ts;
+        const uint32_t n = (uint32_t)(first + (left < R ? left : R) - 1) * ts + tail;
+        return (u32x4){(uint32_t)uniform((int)p), (uint32_t)uniform((int)(p >> 32)), (uint32_t)uniform((uint32_t)e < (uint32_t)pages && left > 0 ? (int)n : 0),
+                       0x00020000u};
+    }
+};
+
 // the LDS address of a pointer into LDS
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
     return (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
@@ -395,7 +446,7 @@ __device__ __forceinline__ void landed() {
 // is in which chunk of the row a thread loads.
 template <int D, int ROWS, int THREADS>
 struct Loader {
-    static constexpr int N = ROWS * Tile<D>::CH / THREADS;  // pieces a thread
+    static constexpr int CH = Tile<D>::CH, N = ROWS * CH / THREADS;  // pieces a thread
     static_assert(N * THREADS == ROWS * Tile<D>::CH, "whole pieces");
     uint32_t off[N];
     __device__ __forceinline__ Loader(int64_t ts2, int d, int tid) {
@@ -410,6 +461,23 @@ struct Loader {
         const u32x4 b = r.template buffer<ROWS>();
 #pragma unroll
         for (int i = 0; i < N; ++i) load_piece(b, off[i], dst + 16 * THREADS * i);
+    }
+    // The same from pages; w0: the wave's first thread. A tile that lies in one page is one buffer. Of smaller pages a wave's
+    // piece, 8 tokens or fewer, lies in one: it is that page's buffer, put back by the tokens before the piece, so that the
+    // offsets are the tile's.
+    __device__ __forceinline__ void load(PageRows& r, int w0, uint32_t dst) const {
+        r.turn();
+        const int skip = r.from - (int)r.pos;  // tokens that no query sees
+        u32x4 b = {};
+        if (r.size() >= ROWS) b = r.template buffer<ROWS>(0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int first = (w0 + THREADS * i) / CH;
+            if (r.size() < ROWS) b = r.template buffer<64 / CH>(first);
+            uint32_t o = off[i];
+            if (skip > 0) o = (w0 + (int)(threadIdx.x & 63) + THREADS * i) / CH < skip ? kNowhere : o;
+            load_piece(b, o, dst + 16 * THREADS * i);
+        }
     }
 };
 

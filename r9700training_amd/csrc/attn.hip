@@ -10,6 +10,9 @@ namespace attn {
 
 int64_t fwd_workspace(const Args& a);
 int launch_fwd(Args a, void* workspace, hipStream_t st);
+int64_t paged_workspace(const Args& a);
+int launch_paged(Args a, void* workspace, hipStream_t st);
+int launch_write(const Args& a, const Heads& k, const Heads& v, hipStream_t st);
 int launch_dq(const Args& a, hipStream_t st);
 int launch_base(const Args& a, hipStream_t st);
 int launch_dq_kept(const Args& a, hipStream_t st);
@@ -112,6 +115,19 @@ Args args_of(const R97qAttnShape* p, int32_t hq, int32_t hk) {
     return a;
 }
 
+// the cache's own sizes, and that every token of a sequence has a place inside 31 bits
+int check_pages(const R97qAttnShape* p, const R97qPages* c, const char* who) {
+    if (!c) return refuse(R97Q_EINVAL, who, "null pages");
+    if (p->kv_starts) return refuse(R97Q_EINVAL, who, "kv_starts go with packed keys, not with pages");
+    if (c->pages < 0 || c->max_pages < 0 || c->table_stride < 0) return refuse(R97Q_EINVAL, who, "a negative count of pages or stride of the table");
+    if (c->page_size < 8 || c->page_size > (1 << 20) || (c->page_size & (c->page_size - 1)))
+        return refuse(c->page_size < 1 ? R97Q_EINVAL : R97Q_EUNSUPPORTED, who, "a page holds a power of two of tokens, 8 to 2^20");
+    if (c->pages > 0x7FFFFFFF || (int64_t)c->max_pages * c->page_size > 0x7FFFFF00)
+        return refuse(R97Q_EUNSUPPORTED, who, "the pages' count or a sequence's tokens pass 31 bits");
+    if (p->batch > 0 && ((!c->table && c->max_pages > 0) || !p->kv_lens)) return refuse(R97Q_EINVAL, who, "null table or kv_lens");
+    return R97Q_OK;
+}
+
 int64_t q_rows(const R97qAttnShape* p) { return p->q_starts ? p->q_tokens : p->q_len; }
 int64_t kv_rows(const R97qAttnShape* p) { return p->kv_starts ? p->kv_tokens : p->kv_len; }
 
@@ -169,6 +185,18 @@ int64_t kept_bytes(Args& a) {
     if (a.d <= 128 && 2.0 * a.batch * a.hq * each > (double)(256LL << 20)) return 0;
     return (2 * (int64_t)rows * a.pitch + 255) / 256 * 256;
 }
+Args paged_args(const R97qAttnShape* p, const R97qPages* c, int32_t hq, int32_t hk) {
+    Args a = args_of(p, hq, hk);
+    a.held = a.lk;
+    a.lk = c->max_pages * c->page_size;  // what kv_lens are clamped to
+    if (a.held > a.lk) a.held = a.lk;
+    a.table = c->table;
+    a.table_stride = c->table_stride;
+    a.pages = (int32_t)c->pages;
+    a.max_pages = c->max_pages;
+    a.page_shift = __builtin_ctz((unsigned)c->page_size);
+    return a;
+}
 int64_t bwd_stats(const Args& a) { return (8 * a.slots + 255) / 256 * 256; }
 
 }  // namespace
@@ -211,6 +239,63 @@ int r97q_attn_fwd(const R97qAttnShape* shape, const R97qHeads* q, const R97qHead
     a.o = heads_of(out, n);
     a.lse = lse;
     return launch_fwd(a, workspace, (hipStream_t)stream);
+}
+
+int64_t r97q_paged_attn_fwd_workspace_bytes(const R97qAttnShape* shape, const R97qPages* pages, int32_t q_heads, int32_t kv_heads) {
+    clear_error();
+    const char* who = "r97q_paged_attn_fwd_workspace_bytes";
+    if (check_shape(shape, q_heads, kv_heads, who) || check_pages(shape, pages, who)) return -1;
+    if (shape->batch == 0 || q_rows(shape) == 0) return 0;
+    return paged_workspace(paged_args(shape, pages, q_heads, kv_heads));
+}
+
+int r97q_paged_attn_fwd(const R97qAttnShape* shape, const R97qPages* pages, const R97qHeads* q, const R97qHeads* k, const R97qHeads* v,
+                        const R97qHeads* out, float* lse, void* workspace, int64_t workspace_bytes, R97IqrStream stream) {
+    clear_error();
+    const char* who = "r97q_paged_attn_fwd";
+    if (!q || !k) return refuse(R97Q_EINVAL, who, "null q or k");
+    const int32_t hq = q->heads, hk = k->heads;
+    if (int e = check_shape(shape, hq, hk, who)) return e;
+    if (int e = check_pages(shape, pages, who)) return e;
+    const int64_t n = q_rows(shape), b = shape->batch;
+    const bool pq = shape->q_starts;
+    if (int e = check_heads(q, hq, false, false, pq, b, n, who, "q")) return e;
+    if (int e = check_heads(k, hk, false, false, false, pages->pages, pages->page_size, who, "k")) return e;
+    if (int e = check_heads(v, hk, false, false, false, pages->pages, pages->page_size, who, "v")) return e;
+    if (int e = check_heads(out, hq, true, true, pq, b, n, who, "out")) return e;
+    if (b == 0 || n == 0) return R97Q_OK;
+    Args a = paged_args(shape, pages, hq, hk);
+    const int64_t need = paged_workspace(a);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
+    if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
+    a.q = heads_of(q, n);
+    a.k = heads_of(k, pages->page_size);
+    a.v = heads_of(v, pages->page_size);
+    a.o = heads_of(out, n);
+    a.lse = lse;
+    return launch_paged(a, workspace, (hipStream_t)stream);
+}
+
+int r97q_paged_write(const R97qAttnShape* shape, const R97qPages* pages, const R97qHeads* k, const R97qHeads* v, const R97qHeads* k_pages,
+                     const R97qHeads* v_pages, R97IqrStream stream) {
+    clear_error();
+    const char* who = "r97q_paged_write";
+    if (!k || !v || !k_pages) return refuse(R97Q_EINVAL, who, "null k, v or pages");
+    const int32_t hk = k_pages->heads;
+    if (int e = check_shape(shape, hk, hk, who)) return e;
+    if (int e = check_pages(shape, pages, who)) return e;
+    const int64_t n = q_rows(shape), b = shape->batch;
+    const bool pq = shape->q_starts;
+    if (int e = check_heads(k, hk, true, false, pq, b, n, who, "k")) return e;
+    if (int e = check_heads(v, hk, true, false, pq, b, n, who, "v")) return e;
+    if (k->dtype != v->dtype) return refuse(R97Q_EINVAL, who, "k and v are both bf16 or both f32");
+    if (int e = check_heads(k_pages, hk, false, true, false, pages->pages, pages->page_size, who, "k_pages")) return e;
+    if (int e = check_heads(v_pages, hk, false, true, false, pages->pages, pages->page_size, who, "v_pages")) return e;
+    if (b == 0 || n == 0 || pages->pages == 0 || pages->max_pages == 0) return R97Q_OK;
+    Args a = paged_args(shape, pages, hk, hk);
+    a.k = heads_of(k_pages, pages->page_size);
+    a.v = heads_of(v_pages, pages->page_size);
+    return launch_write(a, heads_of(k, n), heads_of(v, n), (hipStream_t)stream);
 }
 
 int64_t r97q_attn_bwd_workspace_bytes(const R97qAttnShape* shape, int32_t q_heads, int32_t kv_heads) {

@@ -6,12 +6,42 @@
 // passed it by more than a factor of 2^8, so most tiles rescale nothing (f32 has the room, and a bf16
 // probability the same relative precision at any size). The probabilities are rounded to bf16 for the second
 // product (the matrix cores' input type; off by at most 2^-8 relative), their sum is of the unrounded values in f32.
+//
+// Built twice: over keys in rows (R97Q_PAGED 0), and over a paged cache (1), where only the tiles' loads differ.
 #include "attn.h"
 #include "status.h"
 
+#ifndef R97Q_PAGED
+#define R97Q_PAGED 0
+#endif
+
 namespace r97q {
 namespace attn {
+int launch_join(const Args& a, hipStream_t st);
 namespace {
+
+constexpr bool kPaged = R97Q_PAGED;
+// the keys or values [lo, hi) of a sequence's key head, in tiles from `row0` on
+template <bool PAGED>
+struct Source;
+template <>
+struct Source<false> : Rows {
+    __device__ __forceinline__ Source(const Args& a, const Seq& s, const Heads& t, int hk, int row0, int lo, int hi)
+        : Rows(kv_at(t, a, s, hk), 2 * t.ts, row0, hi, a.d) {}
+};
+template <>
+struct Source<true> : PageRows {
+    __device__ __forceinline__ Source(const Args& a, const Seq& s, const Heads& t, int hk, int row0, int lo, int hi)
+        : PageRows(a, s, t, hk, row0, lo, hi, a.d) {}
+};
+using Keyed = Source<kPaged>;
+template <class L>
+__device__ __forceinline__ void load_tile(const L& l, Rows& r, int, uint32_t dst) { l.load(r, dst); }
+template <class L>
+__device__ __forceinline__ void load_tile(const L& l, PageRows& r, int w0, uint32_t dst) { l.load(r, w0, dst); }
+// where the tiles begin: at the first key that is seen, or in pages at the tile that holds it
+template <int KT>
+__device__ __forceinline__ int tile_start(int lo) { return kPaged ? lo / KT * KT : lo; }
 
 constexpr float kLoose = 8.0f;  // how far, in powers of two, a maximum may pass m before m moves
 
@@ -180,8 +210,6 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     const Seq s = sequence(a, bh / a.hk);
     const int rows = s.lq * a.g;
     const float sl = score_scale(a);
-    const uint8_t* kb = kv_at(a.k, a, s, hk);
-    const uint8_t* vb = kv_at(a.v, a, s, hk);
     const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
     const Loader<D, KT, 64 * NW> kl(kts, a.d, tid), vl(vts, a.d, tid);
     const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + 2 * TB + F::col0(lane);
@@ -194,18 +222,18 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
         const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
         Keys own = keys_of(a, s, (r0 < rows ? r0 : rows - 1) / a.g, rend / a.g);
         if (r0 >= rows) own.hi = own.lo;
-        int lo = all.lo, hi = all.hi;  // from the first key that is seen: what lies before it may hold anything
+        int lo = tile_start<KT>(all.lo), hi = all.hi;  // from the first key that is seen: what lies before it may hold anything
         if (a.splits > 1) {
             lo = (int)clamp64((int64_t)lo + (int64_t)split * a.chunk, lo, hi);
             if (split < a.splits - 1 && hi - lo > a.chunk) hi = lo + a.chunk;  // the last range takes what is left
         }
-        Rows kr(kb, kts, lo, hi, a.d), vr(vb, vts, lo, hi, a.d);
+        Keyed kr(a, s, a.k, hk, lo, all.lo, hi), vr(a, s, a.v, hk, lo, all.lo, hi);
         auto load_k = [&](int slot) {
-            kl.load(kr, mine + slot * TB);
+            load_tile(kl, kr, 64 * wave, mine + slot * TB);
             kr.step(KT);
         };
         auto load_v = [&](int slot) {
-            vl.load(vr, mine + (2 + slot) * TB);
+            load_tile(vl, vr, 64 * wave, mine + (2 + slot) * TB);
             vr.step(KT);
         };
         if (lo < hi) {
@@ -330,8 +358,6 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
     const Seq s = sequence(a, bh / a.hk);
     const int rows = s.lq * a.g;
     const float sl = score_scale(a);
-    const uint8_t* kb = kv_at(a.k, a, s, hk);
-    const uint8_t* vb = kv_at(a.v, a, s, hk);
     const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
     const Loader<D, KT, 64> kl(kts, a.d, lane), vl(vts, a.d, lane);
     uint8_t* own = lds + wave * 2 * TB;
@@ -341,7 +367,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
         const Row row(a, hk, r0 + col, rows);
         const int rend = r0 + 31 < rows ? r0 + 31 : rows - 1;
         const Keys keys = keys_of(a, s, r0 / a.g, rend / a.g);
-        int lo = keys.lo, hi = keys.hi;
+        int lo = tile_start<KT>(keys.lo), hi = keys.hi;
         if (a.splits > 1) {
             lo = (int)clamp64((int64_t)lo + (int64_t)split * a.chunk, lo, hi);
             if (split < a.splits - 1 && hi - lo > a.chunk) hi = lo + a.chunk;  // the last range takes what is left
@@ -356,9 +382,9 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
         const int last = a.causal && row.tok + s.off < s.lk - 1 ? row.tok + s.off : s.lk - 1;
         int j0 = lo + KT * wave;
         if (j0 < hi) {
-            Rows kr(kb, kts, j0, hi, a.d), vr(vb, vts, j0, hi, a.d);
-            kl.load(kr, at);
-            vl.load(vr, at + TB);
+            Keyed kr(a, s, a.k, hk, j0, keys.lo, hi), vr(a, s, a.v, hk, j0, keys.lo, hi);
+            load_tile(kl, kr, 0, at);
+            load_tile(vl, vr, 0, at + TB);
             bf16x8 q[D / 16];
             load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
             turn_sign<D>(a, q);
@@ -370,14 +396,14 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
                 // the keys are in registers: their tile is free
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 kr.step(NW * KT);
-                kl.load(kr, at);
+                load_tile(kl, kr, 0, at);
                 if (j0 < keys.all_lo || j0 + KT > keys.all_hi) mask<KT>(x, first - j0, last - j0, h);
                 run.rise(tile_max<KT>(x) * sl);
                 landed<Loader<D, KT, 64>::N>();  // the values; the next keys may be on their way
                 absorb<D, KT>(own + TB, x, sl, lane, run);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 vr.step(NW * KT);
-                vl.load(vr, at + TB);
+                load_tile(vl, vr, 0, at + TB);
                 landed<Loader<D, KT, 64>::N>();
             }
             landed();
@@ -436,6 +462,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
     }
 }
 
+#if !R97Q_PAGED
 // ---------------------------------------------------------------- the ranges' results joined
 // grid (batch * q heads, tokens). Each range's sums are relative to its own m. A row of d values takes `lanes` threads
 // (d / 4, rounded up to a power of two); `groups` of them share a row's ranges, kBatch at once each, so that a row's
@@ -511,6 +538,7 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
         if (lane == 0 && a.lse) a.lse[at] = log_sum(top, l);
     }
 }
+#endif
 
 // How a shape is cut: rows a workgroup, ranges of the keys. A range writes its sums and a second launch (some 5 us) joins
 // them, so only where compute units would be idle. Measured (us at 1 / 2 / 4 / 8 / 16 / 32 ranges): one token, 24 over 4
@@ -532,7 +560,7 @@ Plan plan_of(const Args& a) {
     p.tiles = (rows + tile - 1) / tile;
     p.splits = 1;
     // the keys a tile's rows may see
-    int64_t most = mean_len(a.kv_starts, a.kv_tokens, a.lk, a.batch);
+    int64_t most = kPaged ? a.held : mean_len(a.kv_starts, a.kv_tokens, a.lk, a.batch);
     if (a.window && (int64_t)a.window + tile / a.g + 1 < most) most = (int64_t)a.window + tile / a.g + 1;
     const int64_t have = a.hk * all_tiles(a.q_starts, a.q_tokens, a.lq, a.batch, a.g, tile);
     int64_t n = 1, unit;
@@ -571,12 +599,20 @@ int run_few(const Args& a, const Plan& p, hipStream_t st) {
 
 }  // namespace
 
+#if R97Q_PAGED
+int64_t paged_workspace(const Args& a) {
+#else
 int64_t fwd_workspace(const Args& a) {
+#endif
     const Plan p = plan_of(a);
     return p.splits > 1 ? p.splits * a.slots * (a.d + 2) * 4 : 0;
 }
 
+#if R97Q_PAGED
+int launch_paged(Args a, void* workspace, hipStream_t st) {
+#else
 int launch_fwd(Args a, void* workspace, hipStream_t st) {
+#endif
     const Plan p = plan_of(a);
     a.splits = p.splits;
     a.chunk = p.chunk;
@@ -589,15 +625,20 @@ int launch_fwd(Args a, void* workspace, hipStream_t st) {
         e = a.d <= 64    ? run_tiles<64, 64, 4, 2>(a, p, st)
             : a.d <= 128 ? run_tiles<128, 64, 4, 2>(a, p, st)
                          : run_tiles<256, 32, 4, 1>(a, p, st);
-    if (e || p.splits == 1) return e;
+    return e || p.splits == 1 ? e : launch_join(a, st);
+}
+
+#if !R97Q_PAGED
+int launch_join(const Args& a, hipStream_t st) {
     const int lanes = a.d <= 32 ? 8 : a.d <= 64 ? 16 : a.d <= 128 ? 32 : 64;
     int groups = 1;
-    while (groups * lanes < 1024 && groups * kBatch < p.splits) groups *= 2;
+    while (groups * lanes < 1024 && groups * kBatch < a.splits) groups *= 2;
     const int rows = groups * lanes < 256 ? 256 / (groups * lanes) : 1, blocks = (a.lq + rows - 1) / rows;
     hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)(a.batch * a.hq), (unsigned)(blocks < 65535 ? blocks : 65535)),
                        dim3((unsigned)(rows * groups * lanes)), 0, st, a, lanes, groups, rows);
     return launch_status("attn_join_kernel");
 }
+#endif
 
 }  // namespace attn
 }  // namespace r97q

@@ -7,7 +7,8 @@
 //
 // Bound by memory: each value is read and written once. A workgroup takes a few tokens, forms their sines
 // and cosines once in LDS (rot / 2 a token, against heads * rot / 2 pairs that use them) and then walks the
-// tokens' heads in 16-byte pieces, kItems pieces of a thread in flight together. 16384 tokens, 40 heads of 128: 73 us, as
+// tokens' heads in 16-byte pieces, kItems pieces of a thread in flight together. With several axes a token has a position on
+// each and a pair an axis: only the table's positions differ. 16384 tokens, 40 heads of 128: 73 us, as
 // neighbouring pairs 75 (4.5 TB/s; a 1 GiB copy reaches 4.9). One token: 4.4 us, latency.
 #include <hip/hip_runtime.h>
 
@@ -42,6 +43,9 @@ struct RArgs {
     const void* pos;
     int32_t pos64, inverse;
     float mscale;
+    const int32_t* axis;  // each pair's axis, its positions axis_stride apart; null: one position a token
+    int64_t axis_stride;
+    int32_t axes;
 };
 
 // V values, in one load where they are aligned (WIDE)
@@ -119,8 +123,12 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RArgs a) {
     const int nt = a.tokens - t0 < a.tpb ? (int)(a.tokens - t0) : a.tpb;
     for (int i = threadIdx.x; i < nt * a.half; i += kThreads) {
         const int64_t t = t0 + i / a.half;
-        const double p = !a.pos ? (double)t
-                         : a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[t] : (double)static_cast<const int32_t*>(a.pos)[t];
+        const int ax = a.axis ? a.axis[i % a.half] : 0;
+        const bool turns_at_all = !a.axis || (uint32_t)ax < (uint32_t)a.axes;
+        const int64_t at = turns_at_all ? ax * a.axis_stride + t : 0;
+        const double p = !turns_at_all ? 0.0
+                         : !a.pos ? (double)t
+                         : a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[at] : (double)static_cast<const int32_t*>(a.pos)[at];
         double turns = p * a.freq[i % a.half] * 0.15915494309189534;
         turns -= rint(turns);
         float s, c;
@@ -175,8 +183,8 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RArgs a) {
     }
 }
 
-int refuse(int code, const char* why) {
-    set_error("r97q_rotary: %s", why);
+int refuse(int code, const char* who, const char* why) {
+    set_error("%s: %s", who, why);
     return code;
 }
 
@@ -184,13 +192,13 @@ bool on(const R97qHeads* t, int unit, int size) {  // pieces of `unit` values ar
     return (reinterpret_cast<uintptr_t>(t->data) & (unit * size - 1)) == 0 && t->token_stride % unit == 0 && t->head_stride % unit == 0;
 }
 
-int check_pair(const R97qHeads* in, const R97qHeads* out, int32_t dtype, int64_t tokens) {
-    if (!in || !out || ((!in->data || !out->data) && tokens > 0)) return refuse(R97Q_EINVAL, "null heads");
-    if (in->dtype != dtype || out->dtype != dtype) return refuse(R97Q_EINVAL, "q, k and the outputs are all bf16 or all f32");
-    if (in->heads < 1 || out->heads != in->heads) return refuse(R97Q_EINVAL, "an output has its input's heads, one or more");
+int check_pair(const R97qHeads* in, const R97qHeads* out, int32_t dtype, int64_t tokens, const char* who) {
+    if (!in || !out || ((!in->data || !out->data) && tokens > 0)) return refuse(R97Q_EINVAL, who, "null heads");
+    if (in->dtype != dtype || out->dtype != dtype) return refuse(R97Q_EINVAL, who, "q, k and the outputs are all bf16 or all f32");
+    if (in->heads < 1 || out->heads != in->heads) return refuse(R97Q_EINVAL, who, "an output has its input's heads, one or more");
     if (in->token_stride < 0 || in->head_stride < 0 || out->token_stride < 0 || out->head_stride < 0 ||
         (tokens > 1 && !out->token_stride) || (out->heads > 1 && !out->head_stride))
-        return refuse(R97Q_EINVAL, "a negative stride, or an output with a stride of zero");
+        return refuse(R97Q_EINVAL, who, "a negative stride, or an output with a stride of zero");
     return R97Q_OK;
 }
 
@@ -228,30 +236,28 @@ int pick(const RArgs& a, int32_t head_dim, int unit, bool in_place, hipStream_t 
     return launch<T, NEAR ? 2 : 1, NEAR, false>(a, head_dim, in_place, st);
 }
 
-}  // namespace
-}  // namespace r97q
+struct Axes {
+    const int32_t* of_pair;
+    int32_t count;
+    int64_t stride;
+};
 
-using namespace r97q;
-
-extern "C" {
-
-int r97q_rotary(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, const R97qHeads* k_out, int64_t tokens,
-                int32_t head_dim, int32_t rot, int32_t pairs, const double* inv_freq, const void* positions,
-                int32_t positions64, float mscale, int32_t inverse, R97IqrStream stream) {
-    clear_error();
-    if (!q || (q->dtype != R97Q_BF16 && q->dtype != R97Q_F32)) return refuse(R97Q_EINVAL, "q is bf16 or f32");
-    if (tokens < 0 || tokens > 0x7FFFFFFF) return refuse(R97Q_EINVAL, "tokens within 31 bits");
-    if (head_dim < 1 || rot < 2 || rot % 2 || rot > head_dim) return refuse(R97Q_EINVAL, "rot is even, at least 2 and at most head_dim");
-    if (rot > 2 * kTable) return refuse(R97Q_EUNSUPPORTED, "at most 8192 values turn");
-    if (pairs != R97Q_ROTARY_HALF && pairs != R97Q_ROTARY_INTERLEAVED) return refuse(R97Q_EINVAL, "pairs are half or interleaved");
-    if (!inv_freq) return refuse(R97Q_EINVAL, "null frequencies");
-    if (int e = check_pair(q, q_out, q->dtype, tokens)) return e;
-    if (!k != !k_out) return refuse(R97Q_EINVAL, "k and k_out come together");
+int turn(const char* who, const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, const R97qHeads* k_out, int64_t tokens,
+         int32_t head_dim, int32_t rot, int32_t pairs, const double* inv_freq, const void* positions, int32_t positions64,
+         const Axes& axes, float mscale, int32_t inverse, hipStream_t st) {
+    if (!q || (q->dtype != R97Q_BF16 && q->dtype != R97Q_F32)) return refuse(R97Q_EINVAL, who, "q is bf16 or f32");
+    if (tokens < 0 || tokens > 0x7FFFFFFF) return refuse(R97Q_EINVAL, who, "tokens within 31 bits");
+    if (head_dim < 1 || rot < 2 || rot % 2 || rot > head_dim) return refuse(R97Q_EINVAL, who, "rot is even, at least 2 and at most head_dim");
+    if (rot > 2 * kTable) return refuse(R97Q_EUNSUPPORTED, who, "at most 8192 values turn");
+    if (pairs != R97Q_ROTARY_HALF && pairs != R97Q_ROTARY_INTERLEAVED) return refuse(R97Q_EINVAL, who, "pairs are half or interleaved");
+    if (!inv_freq) return refuse(R97Q_EINVAL, who, "null frequencies");
+    if (int e = check_pair(q, q_out, q->dtype, tokens, who)) return e;
+    if (!k != !k_out) return refuse(R97Q_EINVAL, who, "k and k_out come together");
     if (k)
-        if (int e = check_pair(k, k_out, q->dtype, tokens)) return e;
+        if (int e = check_pair(k, k_out, q->dtype, tokens, who)) return e;
     const bool near = pairs == R97Q_ROTARY_INTERLEAVED;
     const int64_t heads = (int64_t)q->heads + (k ? k->heads : 0);
-    if (heads * head_dim > 0x3FFFFFFF / 4) return refuse(R97Q_EUNSUPPORTED, "a token's heads pass 28 bits");
+    if (heads * head_dim > 0x3FFFFFFF / 4) return refuse(R97Q_EUNSUPPORTED, who, "a token's heads pass 28 bits");
     if (tokens == 0) return R97Q_OK;
     const int size = q->dtype == R97Q_F32 ? 4 : 2;
     int unit = 16 / size;
@@ -265,7 +271,7 @@ int r97q_rotary(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, 
     };
     bool in_place = same(q, q_out) && (!k || same(k, k_out));
     // single values past an odd rest are copied one by one only in the halves' form: neighbouring pieces are two wide
-    if (near && (head_dim - rot) % 2) return refuse(R97Q_EUNSUPPORTED, "neighbouring pairs need an even head_dim");
+    if (near && (head_dim - rot) % 2) return refuse(R97Q_EUNSUPPORTED, who, "neighbouring pairs need an even head_dim");
     RArgs a = {};
     auto heads_of = [](const R97qHeads* x, const R97qHeads* y) {
         return RHeads{x->data, y->data, x->token_stride, x->head_stride, y->token_stride, y->head_stride};
@@ -281,10 +287,39 @@ int r97q_rotary(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, 
     a.pos64 = positions64;
     a.inverse = inverse;
     a.mscale = mscale;
-    hipStream_t st = (hipStream_t)stream;
+    a.axis = axes.of_pair;
+    a.axes = axes.count;
+    a.axis_stride = axes.stride;
     if (q->dtype == R97Q_BF16)
         return near ? pick<uint16_t, true>(a, head_dim, unit, in_place, st) : pick<uint16_t, false>(a, head_dim, unit, in_place, st);
     return near ? pick<float, true>(a, head_dim, unit, in_place, st) : pick<float, false>(a, head_dim, unit, in_place, st);
+}
+
+}  // namespace
+}  // namespace r97q
+
+using namespace r97q;
+
+extern "C" {
+
+int r97q_rotary(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, const R97qHeads* k_out, int64_t tokens,
+                int32_t head_dim, int32_t rot, int32_t pairs, const double* inv_freq, const void* positions,
+                int32_t positions64, float mscale, int32_t inverse, R97IqrStream stream) {
+    clear_error();
+    return turn("r97q_rotary", q, q_out, k, k_out, tokens, head_dim, rot, pairs, inv_freq, positions, positions64, {nullptr, 1, 0}, mscale,
+                inverse, (hipStream_t)stream);
+}
+
+int r97q_rotary_axes(const R97qHeads* q, const R97qHeads* q_out, const R97qHeads* k, const R97qHeads* k_out, int64_t tokens,
+                     int32_t head_dim, int32_t rot, int32_t pairs, const double* inv_freq, const int32_t* pair_axis, int32_t axes,
+                     const void* positions, int32_t positions64, int64_t axis_stride, float mscale, int32_t inverse, R97IqrStream stream) {
+    clear_error();
+    const char* who = "r97q_rotary_axes";
+    if (axes < 1) return refuse(R97Q_EINVAL, who, "one axis or more");
+    if (!pair_axis || (!positions && tokens > 0)) return refuse(R97Q_EINVAL, who, "null pair_axis or positions");
+    if (axis_stride < 0) return refuse(R97Q_EINVAL, who, "a negative stride");
+    return turn(who, q, q_out, k, k_out, tokens, head_dim, rot, pairs, inv_freq, positions, positions64, {pair_axis, axes, axis_stride},
+                mscale, inverse, (hipStream_t)stream);
 }
 
 int r97q_rotary_frequencies(int32_t rot, double base, int32_t scaling, double factor, double original, double slow,

@@ -1,5 +1,5 @@
-"""Rotary positions of the query and key heads on the card (a front over r97q_rotary and
-r97q_rotary_frequencies, include/r97q.h)."""
+"""Rotary positions of the query and key heads on the card, with one position a token or several axes (a front over
+r97q_rotary, r97q_rotary_axes and r97q_rotary_frequencies, include/r97q.h)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -44,24 +44,14 @@ def _heads(x: torch.Tensor, what: str, shape=None) -> Heads:
     return Heads(x.data_ptr(), 0, st[0], st[1], own[1], dt)
 
 
-def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
-           pairs: str = "half", mscale: float = 1.0, inverse: bool = False, q_out: torch.Tensor | None = None,
-           k_out: torch.Tensor | None = None, stream=None):
-    """(q, k) [tokens, heads, head_dim] turned by positions * inv_freq (positions None: 0, 1, ..); k may be
-    None. The first 2 * len(inv_freq) values of a head turn, the rest are copied. inverse: the adjoint
-    (turned back, scaled by the same mscale). q_out / k_out may be q / k."""
+def _tensors(q, k, inv_freq, pairs, q_out, k_out, stream):
+    """(q_out, k_out, tokens, head_dim, and the four tensors of heads) of a call, checked."""
     if pairs not in PAIRS:
         raise ValueError(f"rotary: pairs {pairs!r} are not one of {sorted(PAIRS)}")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or not inv_freq.is_cuda:
         raise ValueError("rotary: inv_freq is a contiguous f64 [rot / 2] device tensor")
     qs = q.shape
     tokens, _, dim = qs if len(qs) == 3 else (0, 0, 0)
-    wide = 0
-    if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) \
-                or not positions.is_contiguous() or not positions.is_cuda:
-            raise ValueError("rotary: positions are a contiguous int32 or int64 [tokens] device tensor")
-        wide = int(positions.dtype == torch.int64)
     hq = _heads(q, "q")
     if q_out is None:
         q_out = _empty_like(q, q.dtype, stream)
@@ -76,6 +66,54 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, posi
             raise ValueError("rotary: k has q's tokens and head_dim")
     elif k_out is not None:
         raise ValueError("rotary: k_out without k")
-    check(lib().r97q_rotary(hq, ho, hk, hko, tokens, dim, 2 * inv_freq.shape[0], PAIRS[pairs], _ptr(inv_freq),
+    return q_out, k_out, tokens, dim, (hq, ho, hk, hko)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
+           pairs: str = "half", mscale: float = 1.0, inverse: bool = False, q_out: torch.Tensor | None = None,
+           k_out: torch.Tensor | None = None, stream=None):
+    """(q, k) [tokens, heads, head_dim] turned by positions * inv_freq (positions None: 0, 1, ..); k may be
+    None. The first 2 * len(inv_freq) values of a head turn, the rest are copied. inverse: the adjoint
+    (turned back, scaled by the same mscale). q_out / k_out may be q / k."""
+    q_out, k_out, tokens, dim, heads = _tensors(q, k, inv_freq, pairs, q_out, k_out, stream)
+    wide = 0
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) \
+                or not positions.is_contiguous() or not positions.is_cuda:
+            raise ValueError("rotary: positions are a contiguous int32 or int64 [tokens] device tensor")
+        wide = int(positions.dtype == torch.int64)
+    check(lib().r97q_rotary(*heads, tokens, dim, 2 * inv_freq.shape[0], PAIRS[pairs], _ptr(inv_freq),
                             _ptr(positions), wide, float(mscale), int(bool(inverse)), _stream(stream)), "r97q_rotary")
+    return q_out, k_out
+
+
+def rotary_pair_axes(sections, order: str = "blocks", device="cuda"):
+    """int32 [sum(sections)] on `device`: each pair's axis, sections[a] pairs for axis a. "blocks": the first axis's pairs,
+    then the second's, ..; "cycle": the axes in turn, each as long as it has pairs left."""
+    left = [int(n) for n in sections]
+    if not left or min(left) < 0 or sum(left) < 1:
+        raise ValueError("rotary_pair_axes: sections are counts of pairs, one or more in all")
+    if order == "blocks":
+        axis = [a for a, n in enumerate(left) for _ in range(n)]
+    elif order == "cycle":
+        axis = [a for i in range(max(left)) for a, n in enumerate(left) if i < n]
+    else:
+        raise ValueError(f"rotary_pair_axes: order {order!r} is not 'blocks' or 'cycle'")
+    return torch.tensor(axis, dtype=torch.int32).to(device)
+
+
+def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, positions: torch.Tensor,
+                pair_axis: torch.Tensor, pairs: str = "half", mscale: float = 1.0, inverse: bool = False,
+                q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, stream=None):
+    """rotary with a position on each of several axes: positions int32 or int64 [axes, tokens], and pair i turns by
+    positions[pair_axis[i]] * inv_freq[i] (pair_axis int32 [rot / 2]: rotary_pair_axes)."""
+    q_out, k_out, tokens, dim, heads = _tensors(q, k, inv_freq, pairs, q_out, k_out, stream)
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 2 or positions.shape[1] != tokens \
+            or (tokens > 1 and positions.stride(1) != 1) or not positions.is_cuda:
+        raise ValueError("rotary_axes: positions are an int32 or int64 [axes, tokens] device tensor, tokens consecutive")
+    if pair_axis.dtype != torch.int32 or pair_axis.shape != inv_freq.shape or not pair_axis.is_contiguous() or not pair_axis.is_cuda:
+        raise ValueError("rotary_axes: pair_axis is a contiguous int32 device tensor of inv_freq's shape")
+    check(lib().r97q_rotary_axes(*heads, tokens, dim, 2 * inv_freq.shape[0], PAIRS[pairs], _ptr(inv_freq), _ptr(pair_axis),
+                                 positions.shape[0], _ptr(positions), int(positions.dtype == torch.int64), positions.stride(0),
+                                 float(mscale), int(bool(inverse)), _stream(stream)), "r97q_rotary_axes")
     return q_out, k_out
