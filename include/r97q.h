@@ -675,6 +675,49 @@ int r97q_paged_attn_fwd(const R97qAttnShape* shape, const R97qPages* pages, cons
 int r97q_paged_write(const R97qAttnShape* shape, const R97qPages* pages, const R97qHeads* k, const R97qHeads* v,
                      const R97qHeads* k_pages, const R97qHeads* v_pages, R97IqrStream stream);
 
+/* A gated linear recurrence over the tokens of each channel, in f32:
+ *   a = exp(-rate * sigmoid(gate)),  h_t = a_t h_(t-1) + sqrt(1 - a_t^2) * sigmoid(input_gate_t) * x_t
+ * (input_gate NULL: x itself). A batch of sequences, dense (len tokens each) or packed one after the other: sequence b at
+ * [starts[b], starts[b + 1]) (device int32 [batch + 1], ascending, clamped to the tensors), len the longest (it sizes the
+ * launch: too small a number costs time, not results) and tokens the tokens in all. */
+#define R97Q_RECURRENCE_CHUNK 128
+typedef struct R97qRecurrence {
+    int32_t batch;
+    int32_t channels;
+    int64_t len;
+    const int32_t* starts; /* NULL: dense */
+    int64_t tokens;
+    int32_t dtype;         /* of x, the gates, h and their gradients: bf16 or f32 */
+} R97qRecurrence;
+/* [batch, tokens, channels] of the call's dtype, packed [tokens, channels]: strides in elements, channels consecutive. */
+typedef struct R97qRows {
+    void* data;
+    int64_t batch_stride; /* unused where the sequences are packed */
+    int64_t token_stride;
+} R97qRows;
+/* h (written) from x, gate, input_gate (may be NULL), rate f32 [channels], not negative, and h0 f32 [batch][channels], the
+ * state before each sequence (NULL: zeros). last f32 [batch][channels] (may be NULL, may be h0): the state behind each
+ * sequence, which the next tokens begin from; that of a sequence without tokens is h0. states f32 [rows][channels] (may be
+ * NULL; r97q_recurrence_state_rows says how many rows): for the backward, the state before every token that is a multiple
+ * of R97Q_RECURRENCE_CHUNK of its sequence, dense row b * ceil(len / CHUNK) + t / CHUNK, packed starts[b] / CHUNK + b + t /
+ * CHUNK. Packed tokens outside every sequence are not written. h may be x, gate or input_gate. Few channels over many tokens
+ * are cut along the tokens and joined through the workspace (on 16 bytes, often 0). Repeated calls give the same bits. */
+int64_t r97q_recurrence_state_rows(const R97qRecurrence* shape);
+int64_t r97q_recurrence_fwd_workspace_bytes(const R97qRecurrence* shape);
+int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R97qRows* gate, const R97qRows* input_gate,
+                        const float* rate, const float* h0, const R97qRows* h, float* last, float* states, void* workspace,
+                        int64_t workspace_bytes, R97IqrStream stream);
+/* The adjoint, from the forward's inputs and states and the cotangents d_h and d_last f32 [batch][channels] (NULL: zeros):
+ * dx, dgate, dinput_gate (with input_gate), drate f32 [channels], summed over all tokens, and dh0 f32 [batch][channels] (may
+ * be NULL) are written. Where a decay is one (a rate of zero, a gate far below zero) the derivative through sqrt(1 - a^2),
+ * which has no bound there, counts as zero. Packed tokens outside every sequence are not written. Repeated calls give the
+ * same bits. The workspace (on 16 bytes) holds the ranges' joins and the rate's partial sums. */
+int64_t r97q_recurrence_bwd_workspace_bytes(const R97qRecurrence* shape);
+int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R97qRows* gate, const R97qRows* input_gate,
+                        const float* rate, const float* states, const R97qRows* d_h, const float* d_last, const R97qRows* dx,
+                        const R97qRows* dgate, const R97qRows* dinput_gate, float* drate, float* dh0, void* workspace,
+                        int64_t workspace_bytes, R97IqrStream stream);
+
 /* The residual's addition, the RMS norm and the group quantiser in one pass over rows of n values:
  *   h = x + residual rounded to dtype (residual NULL: h is x, and h_out is not written),
  *   rs = 1 / sqrt(mean of h^2 + eps),  y = h * rs * (w + wadd),

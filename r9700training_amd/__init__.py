@@ -21,6 +21,7 @@ R97Q_CODES8 = 8  # R97qWeight.bits of the int8-code form (include/r97q.h)
 R97Q_DECODE_AUTO, R97Q_DECODE_ONCE, R97Q_DECODE_FUSED = 0, 1, 2  # r97q_set_decode_once modes
 R97Q_ROTARY_HALF, R97Q_ROTARY_INTERLEAVED = 0, 1  # r97q_rotary's pairs
 R97Q_ROTARY_PLAIN, R97Q_ROTARY_LINEAR, R97Q_ROTARY_RAMP = 0, 1, 2  # r97q_rotary_frequencies' scalings
+R97Q_RECURRENCE_CHUNK = 128  # tokens between the states that r97q_recurrence_fwd keeps
 R97Q_ADAMW_GRADS_STAGED = 1  # r97q_adamw_step flags: the gradients are staging buffers (include/r97q.h)
 
 
@@ -108,6 +109,19 @@ class Pages(C.Structure):
                 ("max_pages", C.c_int32)]
 
 
+class Recurrence(C.Structure):
+    """R97qRecurrence (include/r97q.h): a batch of sequences and their channels."""
+
+    _fields_ = [("batch", C.c_int32), ("channels", C.c_int32), ("len", C.c_int64), ("starts", C.c_void_p),
+                ("tokens", C.c_int64), ("dtype", C.c_int32)]
+
+
+class Rows(C.Structure):
+    """R97qRows (include/r97q.h): a tensor of tokens' channels."""
+
+    _fields_ = [("data", C.c_void_p), ("batch_stride", C.c_int64), ("token_stride", C.c_int64)]
+
+
 R97_ENC_STR = 32
 R97_ENC_MAX_PLANES = 8
 # R97EncDtype (include/r97q.h)
@@ -148,6 +162,7 @@ class StoredPlane(C.Structure):
 # every symbol include/r97q.h declares, with its ctypes signature
 _P, _I, _i = C.c_void_p, C.c_int64, C.c_int32
 _H = C.POINTER(Heads)
+_R, _S = C.POINTER(Rows), C.POINTER(Recurrence)
 SIGNATURES = {
     "r97q_last_error": (C.c_char_p, []),
     "r97q_iqr_validate": (C.c_int, [C.POINTER(Desc)]),
@@ -212,6 +227,11 @@ SIGNATURES = {
     "r97q_paged_attn_fwd_workspace_bytes": (_I, [C.POINTER(AttnShape), C.POINTER(Pages), _i, _i]),
     "r97q_paged_attn_fwd": (C.c_int, [C.POINTER(AttnShape), C.POINTER(Pages), _H, _H, _H, _H, _P, _P, _I, _P]),
     "r97q_paged_write": (C.c_int, [C.POINTER(AttnShape), C.POINTER(Pages), _H, _H, _H, _H, _P]),
+    "r97q_recurrence_state_rows": (_I, [_S]),
+    "r97q_recurrence_fwd_workspace_bytes": (_I, [_S]),
+    "r97q_recurrence_fwd": (C.c_int, [_S, _R, _R, _R, _P, _P, _R, _P, _P, _P, _I, _P]),
+    "r97q_recurrence_bwd_workspace_bytes": (_I, [_S]),
+    "r97q_recurrence_bwd": (C.c_int, [_S, _R, _R, _R, _P, _P, _R, _P, _R, _R, _R, _P, _P, _P, _I, _P]),
     "r97q_add_rmsnorm_i8g": (C.c_int, [_P, _P, _P, _i, _I, _I, _I, C.c_float, C.c_float, _P, _P, _P, _P, _P, _P]),
     "r97q_add_rmsnorm_i8g_bwd_workspace_bytes": (_I, [_I, _I]),
     "r97q_add_rmsnorm_i8g_bwd": (C.c_int, [_P, _P, _i, _I, _I, _I, C.c_float, _P, _P, _P, _P, _P, _P, _P, _i, _P, _I,

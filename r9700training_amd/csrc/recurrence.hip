@@ -1,0 +1,773 @@
+// recurrence.hip -- a gated linear recurrence over long sequences, forward and backward.
+//
+//   s = sigmoid(gate), a = e^(-rate s), q = 1 - a^2, w = sigmoid(input_gate) x,  h_t = a_t h_(t-1) + sqrt(q_t) w_t
+// and with l_t the cotangent of h_t and all that follows from it, l_t = dh_t + a_(t+1) l_(t+1):
+//   dlog a = l a (h_(t-1) - a w / sqrt(q)),  drate = -sum s dlog a,  dgate = -rate s (1 - s) dlog a,
+//   dx = l sqrt(q) sigmoid(i),  dinput_gate = dx x (1 - sigmoid(i)),  dh0 = a_1 l_1.
+//
+// A span of tokens acts on the state before it as h -> A h + H, and on the cotangent after it as m -> A m + M (m_t = a_t l_t),
+// with one A = e^-(sum of rate s). So a workgroup walks a sequence's tokens for 64 channels (a row's 128 or 256 bytes) in
+// tiles: a thread a few tokens one after the other for the channels of one 16-byte piece, a wave's groups of lanes and the
+// workgroup's waves joined by their spans, the tile's end carried to the next tile. Each value is read and written once.
+//
+// A wave's join. Lane (g, c) holds span g of the VC channels of piece c. A transposition of registers against the lanes'
+// bits 3 .. 5 (swaps of lane halves and rows, no LDS) gives each lane all the wave's spans of one channel: a scan there is
+// VC multiply-adds, a wave's 64 channels one a lane, and one float2 a lane goes to the other waves.
+//
+// Few sequences and channels over many tokens leave compute units idle: then the tokens are cut into ranges, a first launch
+// forms the ranges' spans, and each workgroup of the second begins from those before its own (behind, in the backward).
+//
+// Numbers. All is f32 but the inputs' and outputs' type. A state may last for thousands of tokens of decays next to one,
+// where an error with a sign adds up: a wave's A is formed from the sum of its logarithms, by 1 minus a polynomial where it
+// is near one, and 1 - a^2 by 2 a sinh(rate s).
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/r97q.h"
+#include "iqr_device.h"
+#include "status.h"
+
+namespace r97q {
+namespace scan {
+namespace {
+
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using b16x2 = __attribute__((ext_vector_type(2))) __bf16;
+
+constexpr int kWaves = 8, kThreads = 64 * kWaves, kSlab = 64, kChunk = R97Q_RECURRENCE_CHUNK;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.9259629911266175e-8f, kLn2 = 0.6931471805599453f;
+
+struct Rows {  // [batch, tokens, channels] or packed [tokens, channels], channels consecutive
+    uint8_t* p;
+    int64_t bs, ts;
+};
+
+struct Args {
+    Rows x, g, i, h;              // i.p null: no gate on the input. h: the forward's output, the backward's d_h
+    Rows dx, dg, di;
+    const float* rate;
+    const float* first;           // the state before (h0), or the cotangent behind (d_last); may be null
+    float* last;                  // the state behind (last), or the cotangent before (dh0); may be null
+    float* states;                // the states before tokens 0, kChunk, 2 kChunk, .. of every sequence; may be null
+    const int32_t* starts;
+    int64_t tokens, len;
+    int32_t batch, channels;
+    int32_t ranges;
+    int64_t range_len;
+    float2* spans;                // [batch][ranges][channels], the ranges' spans
+    float* kept;                  // [batch][channels]: `first`, where `last` may be written over it
+    float* drate;                 // [batch * ranges][channels], or the sum itself where that is one row
+};
+
+// a sequence's place
+struct Span {
+    int64_t base, len;
+    int64_t state;                // its first row of states
+};
+__device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
+__device__ __forceinline__ Span span_of(const Args& a, int b) {
+    Span s = {0, a.len, b * ((a.len + kChunk - 1) / kChunk)};
+    if (a.starts) {  // starts come from device memory: clamped to the tensors
+        s.base = clamp64(__builtin_amdgcn_readfirstlane(a.starts[b]), 0, a.tokens);
+        s.len = clamp64(__builtin_amdgcn_readfirstlane(a.starts[b + 1]), s.base, a.tokens) - s.base;
+        s.state = s.base / kChunk + b;
+    }
+    return s;
+}
+__device__ __forceinline__ uint8_t* row_of(const Rows& t, const Args& a, const Span& s, int b, int size) {
+    return t.p + (a.starts ? s.base * t.ts : b * t.bs) * size;
+}
+
+// ---------------------------------------------------------------- pieces of 16 bytes
+template <class T>
+constexpr int kVC = 16 / (int)sizeof(T);
+template <class T>
+__device__ __forceinline__ float value(const u32x4& v, int j) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, (uint32_t)v[j]);
+    else return __builtin_bit_cast(float, j & 1 ? v[j >> 1] & 0xFFFF0000u : v[j >> 1] << 16);
+}
+template <class T>
+__device__ __forceinline__ u32x4 pack(const float* x) {
+    u32x4 v;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __builtin_bit_cast(uint32_t, x[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const b16x2 w = {(__bf16)x[2 * j], (__bf16)x[2 * j + 1]};
+            v[j] = __builtin_bit_cast(uint32_t, w);
+        }
+    }
+    return v;
+}
+// the piece at channel c0 of a row; not WIDE: value by value, the last channel again past the end
+template <class T, bool WIDE>
+__device__ __forceinline__ u32x4 load(const uint8_t* row, int c0, int channels) {
+    if constexpr (WIDE) return *reinterpret_cast<const u32x4*>(row + (int64_t)c0 * sizeof(T));
+    else {
+        const T* p = reinterpret_cast<const T*>(row);
+        T x[kVC<T>];
+#pragma unroll
+        for (int j = 0; j < kVC<T>; ++j) x[j] = p[c0 + j < channels ? c0 + j : channels - 1];
+        return __builtin_bit_cast(u32x4, x);
+    }
+}
+template <class T, bool WIDE>
+__device__ __forceinline__ void store(uint8_t* row, int c0, int channels, const u32x4& v) {
+    if constexpr (WIDE) *reinterpret_cast<u32x4*>(row + (int64_t)c0 * sizeof(T)) = v;
+    else {
+        T* p = reinterpret_cast<T*>(row);
+        struct { T x[kVC<T>]; } u = __builtin_bit_cast(decltype(u), v);
+#pragma unroll
+        for (int j = 0; j < kVC<T>; ++j)
+            if (c0 + j < channels) p[c0 + j] = u.x[j];
+    }
+}
+
+// ---------------------------------------------------------------- the gates
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// 1 / (1 + e^-v). The product with log2 e is off by half a step of itself, which for a far gate is more than a step of the
+// result: f32's is put right (bf16's inputs are further off), gates past 87 on either side counted as 87.
+template <class T>
+__device__ __forceinline__ float sigmoid(float v) {
+    if constexpr (sizeof(T) == 4) v = v < -87.0f ? -87.0f : v > 87.0f ? 87.0f : v;
+    const float t = v * -kLog2e;
+    float e = exp2_(t);
+    if constexpr (sizeof(T) == 4) {
+        const float r = __builtin_fmaf(v, -kLog2e, -t) - v * kLog2eLow;
+        e = __builtin_fmaf(e, r * kLn2, e);
+    }
+    return __builtin_amdgcn_rcpf(1.0f + e);
+}
+// 1 - a^2 of a = 2^-y: 2 a sinh(y ln 2) where a is near one
+__device__ __forceinline__ float room(float y, float a) {
+    constexpr float l2 = kLn2 * kLn2;
+    const float t = y * y;
+    float p = __builtin_fmaf(t, 2.0f * kLn2 * l2 * l2 * l2 / 5040.0f, 2.0f * kLn2 * l2 * l2 / 120.0f);
+    p = __builtin_fmaf(p, t, 2.0f * kLn2 * l2 / 6.0f);
+    p = __builtin_fmaf(p, t, 2.0f * kLn2);
+    const float near = p * y * a, far = __builtin_fmaf(-a, a, 1.0f);
+    return y < 0.72f ? near : far;
+}
+// 2^-y, near one by its distance from it
+__device__ __forceinline__ float decay_of(float y) {
+    const float z = y * kLn2;
+    float p = __builtin_fmaf(z, -1.0f / 5040.0f, 1.0f / 720.0f);
+    p = __builtin_fmaf(z, p, -1.0f / 120.0f);
+    p = __builtin_fmaf(z, p, 1.0f / 24.0f);
+    p = __builtin_fmaf(z, p, -1.0f / 6.0f);
+    p = __builtin_fmaf(z, p, 0.5f);
+    p = __builtin_fmaf(z, -p, 1.0f);
+    return z < 0.35f ? __builtin_fmaf(-z, p, 1.0f) : exp2_(-y);
+}
+
+// ---------------------------------------------------------------- a wave's transposition
+__device__ __forceinline__ void swap32(float& x, float& y) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), false, false);
+    const uint32_t u = s[0], v = s[1];
+    x = __builtin_bit_cast(float, u);
+    y = __builtin_bit_cast(float, v);
+}
+__device__ __forceinline__ void swap16(float& x, float& y) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), false, false);
+    const uint32_t u = s[0], v = s[1];
+    x = __builtin_bit_cast(float, u);
+    y = __builtin_bit_cast(float, v);
+}
+// lanes 8 .. 15 of a row take y of the lane 8 before into x, lanes 0 .. 7 x of the lane 8 behind into y
+__device__ __forceinline__ void swap8(float& x, float& y) {
+    const int u = __builtin_bit_cast(int, x), v = __builtin_bit_cast(int, y);
+    x = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(u, v, 0x128, 0xF, 0xC, false));
+    y = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(v, u, 0x128, 0xF, 0x3, false));
+}
+// Lane (g, c)'s register j to lane (j, c)'s register g, for g the lane's bits 3 .. 5 (VC 8) or 4 and 5 (VC 4). Its own inverse.
+template <int VC>
+__device__ __forceinline__ void transpose(float (&x)[VC]) {
+#pragma unroll
+    for (int j = 0; j < VC / 2; ++j) swap32(x[j], x[j + VC / 2]);
+#pragma unroll
+    for (int j = 0; j < VC; ++j)
+        if (!(j & (VC / 4))) swap16(x[j], x[j + VC / 4]);
+    if constexpr (VC == 8) {
+#pragma unroll
+        for (int j = 0; j < VC; j += 2) swap8(x[j], x[j + 1]);
+    }
+}
+
+// what a workgroup works on
+template <class T>
+struct Place {
+    static constexpr int VC = kVC<T>, LPR = 64 / VC;
+    int lane, wave, g, c0, ch, b, range;
+    bool on;  // the transposed lane's channel is one
+    __device__ __forceinline__ Place(const Args& a, int range0 = 0) {
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        g = lane / LPR;
+        c0 = blockIdx.x * kSlab + lane % LPR * VC;
+        ch = c0 + g;
+        on = ch < a.channels;
+        range = range0 + blockIdx.y;
+        b = blockIdx.z;
+    }
+};
+
+// tokens past the end: nothing enters, nothing decays
+template <class T>
+__device__ __forceinline__ void blank(u32x4& x, u32x4& g, u32x4& i, bool out) {
+    constexpr uint32_t shut = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[e] = out ? 0u : x[e];
+        g[e] = out ? shut : g[e];
+        i[e] = out ? 0u : i[e];
+    }
+}
+
+// ---------------------------------------------------------------- forward
+// grid (slabs, ranges, sequences). SUMS: only the ranges' spans, for the next launch.
+template <class T, bool GATED, bool WIDE, bool SUMS>
+__global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
+    constexpr int VC = kVC<T>, TL = 4, WT = VC * TL, TILE = kWaves * WT, size = sizeof(T);
+    static_assert(TILE % kChunk == 0 && kChunk % WT == 0, "chunks begin with a wave");
+    __shared__ float2 spans[2][kWaves][64];
+    const Place<T> at(a);
+    const Span s = span_of(a, at.b);
+    const int64_t begin = at.range * a.range_len;
+    const int64_t end = !SUMS && at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
+    float h = 0.0f, whole = 1.0f;
+    const int64_t mine = (int64_t)at.b * a.channels + at.ch;
+    if (at.on) {
+        if (at.range == 0) {
+            if (a.first) h = a.ranges > 1 && !SUMS ? a.kept[mine] : a.first[mine];
+            if (SUMS && a.first && at.wave == 0) a.kept[mine] = h;
+        } else if (!SUMS) {
+            const float2* p = a.spans + (int64_t)at.b * a.ranges * a.channels + at.ch;
+            for (int r = 0; r < at.range; ++r, p += a.channels) h = __builtin_fmaf(p->x, h, p->y);
+        }
+    }
+    float rate[VC];
+#pragma unroll
+    for (int j = 0; j < VC; ++j) rate[j] = at.c0 + j < a.channels ? a.rate[at.c0 + j] * kLog2e : 0.0f;
+    const int c0 = !WIDE || at.c0 < a.channels ? at.c0 : 0;
+    const uint8_t* xr = row_of(a.x, a, s, at.b, size);
+    const uint8_t* gr = row_of(a.g, a, s, at.b, size);
+    const uint8_t* ir = GATED ? row_of(a.i, a, s, at.b, size) : nullptr;
+    uint8_t* hr = SUMS ? nullptr : row_of(a.h, a, s, at.b, size);
+    const int first = at.wave * WT + at.g * TL;  // the thread's first token in a tile
+
+    struct Raw {
+        u32x4 x[TL], g[TL], i[TL];
+    };
+    auto fetch = [&](Raw& r, int64_t t0) {
+#pragma unroll
+        for (int k = 0; k < TL; ++k) {
+            const int64_t t = t0 + first + k < end ? t0 + first + k : end - 1;
+            r.x[k] = load<T, WIDE>(xr + t * a.x.ts * size, c0, a.channels);
+            r.g[k] = load<T, WIDE>(gr + t * a.g.ts * size, c0, a.channels);
+            if constexpr (GATED) r.i[k] = load<T, WIDE>(ir + t * a.i.ts * size, c0, a.channels);
+        }
+    };
+    auto tile = [&](Raw& now, Raw& next, int64_t t0, int slot) {
+        if (t0 + TILE < end) fetch(next, t0 + TILE);
+        __builtin_amdgcn_sched_barrier(0);
+        if (t0 + TILE > end) {
+#pragma unroll
+            for (int k = 0; k < TL; ++k) blank<T>(now.x[k], now.g[k], now.i[k], t0 + first + k >= end);
+        }
+        float dec[TL][VC], in[TL][VC], y[VC], u[VC];
+#pragma unroll
+        for (int j = 0; j < VC; ++j) {
+            y[j] = u[j] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < TL; ++k) {
+                const float e = rate[j] * sigmoid<T>(value<T>(now.g[k], j));
+                dec[k][j] = exp2_(-e);
+                float w = value<T>(now.x[k], j);
+                if constexpr (GATED) w *= sigmoid<T>(value<T>(now.i[k], j));
+                in[k][j] = __builtin_amdgcn_sqrtf(room(e, dec[k][j])) * w;
+                y[j] += e;
+                u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j]);
+            }
+        }
+        // the wave's spans of one channel
+        transpose<VC>(y);
+        transpose<VC>(u);
+        float sum = 0.0f, got = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+            sum += y[i];
+            y[i] = exp2_(-y[i]);
+            got = __builtin_fmaf(y[i], got, u[i]);
+        }
+        spans[slot][at.wave][at.lane] = make_float2(decay_of(sum), got);
+        __syncthreads();
+        float before = h;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float2 p = spans[slot][w][at.lane];
+            if (w == at.wave) before = h;
+            h = __builtin_fmaf(p.x, h, p.y);
+            if constexpr (SUMS) whole *= p.x;
+        }
+        if constexpr (!SUMS) {
+            const int64_t token = t0 + at.wave * WT;
+            if (a.states && at.wave * WT % kChunk == 0 && token < end && at.on) a.states[(s.state + token / kChunk) * a.channels + at.ch] = before;
+#pragma unroll
+            for (int i = 0; i < VC; ++i) {
+                const float x = before;
+                before = __builtin_fmaf(y[i], before, u[i]);
+                u[i] = x;
+            }
+            transpose<VC>(u);
+#pragma unroll
+            for (int k = 0; k < TL; ++k) {
+#pragma unroll
+                for (int j = 0; j < VC; ++j) u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j]);
+                const int64_t t = t0 + first + k;
+                if (t < end && at.c0 < a.channels) store<T, WIDE>(hr + t * a.h.ts * size, at.c0, a.channels, pack<T>(u));
+            }
+        }
+    };
+    if (begin < end) {
+        Raw one, two;
+        fetch(one, begin);
+        for (int64_t t0 = begin; t0 < end; t0 += 2 * TILE) {
+            tile(one, two, t0, 0);
+            if (t0 + TILE < end) tile(two, one, t0 + TILE, 1);
+        }
+    }
+    if (at.wave || !at.on) return;
+    if constexpr (SUMS) a.spans[((int64_t)at.b * a.ranges + at.range) * a.channels + at.ch] = make_float2(whole, h);
+    else if (at.range == a.ranges - 1 && a.last) a.last[mine] = h;
+}
+
+// ---------------------------------------------------------------- backward
+// The tiles from the last to the first, kChunk tokens each: the state before a tile is the forward's, the cotangent behind
+// it is carried. SUMS: only the ranges' spans (a and dh alone).
+template <class T, bool GATED, bool WIDE, bool SUMS>
+__global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
+    constexpr int VC = kVC<T>, TL = 16 / VC, WT = VC * TL, TILE = kWaves * WT, size = sizeof(T);
+    static_assert(TILE == kChunk, "a tile begins at a kept state");
+    __shared__ float2 spans[2][kWaves][64];
+    __shared__ float backs[2][kWaves][64];
+    const Place<T> at(a, SUMS);  // nothing is before the first range
+    const Span s = span_of(a, at.b);
+    const int64_t begin = at.range * a.range_len;
+    const int64_t end = at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
+    float m = 0.0f, whole = 1.0f;  // the cotangent behind the tile, times its decay
+    const int64_t mine = (int64_t)at.b * a.channels + at.ch;
+    if (at.on) {
+        if (at.range == a.ranges - 1 || !SUMS) m = a.first ? a.first[mine] : 0.0f;
+        if (!SUMS && at.range < a.ranges - 1) {
+            m = 0.0f;  // the last range's span holds it
+            const float2* p = a.spans + ((int64_t)at.b * a.ranges + a.ranges - 1) * a.channels + at.ch;
+            for (int r = a.ranges - 1; r > at.range; --r, p -= a.channels) m = __builtin_fmaf(p->x, m, p->y);
+        }
+    }
+    float rate[VC], dr[VC];
+#pragma unroll
+    for (int j = 0; j < VC; ++j) rate[j] = at.c0 + j < a.channels ? a.rate[at.c0 + j] * kLog2e : 0.0f, dr[j] = 0.0f;
+    const int c0 = !WIDE || at.c0 < a.channels ? at.c0 : 0;
+    const uint8_t* xr = SUMS ? nullptr : row_of(a.x, a, s, at.b, size);
+    const uint8_t* gr = row_of(a.g, a, s, at.b, size);
+    const uint8_t* ir = GATED && !SUMS ? row_of(a.i, a, s, at.b, size) : nullptr;
+    const uint8_t* er = row_of(a.h, a, s, at.b, size);
+    const int first = at.wave * WT + at.g * TL;
+
+    struct Raw {
+        u32x4 x[TL], g[TL], i[TL], e[TL];
+        float h;
+    };
+    auto fetch = [&](Raw& r, int64_t t0) {
+#pragma unroll
+        for (int k = 0; k < TL; ++k) {
+            const int64_t t = t0 + first + k < end ? t0 + first + k : end - 1;
+            r.g[k] = load<T, WIDE>(gr + t * a.g.ts * size, c0, a.channels);
+            r.e[k] = load<T, WIDE>(er + t * a.h.ts * size, c0, a.channels);
+            if constexpr (!SUMS) {
+                r.x[k] = load<T, WIDE>(xr + t * a.x.ts * size, c0, a.channels);
+                if constexpr (GATED) r.i[k] = load<T, WIDE>(ir + t * a.i.ts * size, c0, a.channels);
+            }
+        }
+        if constexpr (!SUMS) r.h = at.on ? a.states[(s.state + t0 / kChunk) * a.channels + at.ch] : 0.0f;
+    };
+    auto tile = [&](Raw& now, Raw& next, int64_t t0, int slot) {
+        if (t0 > begin) fetch(next, t0 - TILE);
+        __builtin_amdgcn_sched_barrier(0);
+        if (t0 + TILE > end) {
+#pragma unroll
+            for (int k = 0; k < TL; ++k) {
+                const bool out = t0 + first + k >= end;
+                blank<T>(now.x[k], now.g[k], now.i[k], out);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) now.e[k][e] = out ? 0u : now.e[k][e];
+            }
+        }
+        // a, the gates, sqrt(q) and its inverse
+        float dec[TL][VC], sg[TL][VC], si[TL][VC], root[TL][VC], inv[TL][VC], y[VC], u[VC], v[VC];
+#pragma unroll
+        for (int j = 0; j < VC; ++j) {
+            y[j] = u[j] = v[j] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < TL; ++k) {
+                sg[k][j] = sigmoid<T>(value<T>(now.g[k], j));
+                const float e = rate[j] * sg[k][j];
+                dec[k][j] = exp2_(-e);
+                y[j] += e;
+                if constexpr (!SUMS) {
+                    const float q = room(e, dec[k][j]);
+                    // where nothing decays the root's derivative counts as none
+                    inv[k][j] = q >= 0x1p-126f ? __builtin_amdgcn_rsqf(q) : q * 0.0f;
+                    root[k][j] = q * inv[k][j];
+                    float w = root[k][j] * value<T>(now.x[k], j);
+                    if constexpr (GATED) {
+                        si[k][j] = sigmoid<T>(value<T>(now.i[k], j));
+                        w *= si[k][j];
+                    }
+                    u[j] = __builtin_fmaf(dec[k][j], u[j], w);
+                }
+            }
+#pragma unroll
+            for (int k = TL - 1; k >= 0; --k) v[j] = dec[k][j] * (v[j] + value<T>(now.e[k], j));
+        }
+        transpose<VC>(y);
+        if constexpr (!SUMS) transpose<VC>(u);
+        transpose<VC>(v);
+        float sum = 0.0f, got = 0.0f, back = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+            sum += y[i];
+            y[i] = exp2_(-y[i]);
+            if constexpr (!SUMS) got = __builtin_fmaf(y[i], got, u[i]);
+        }
+#pragma unroll
+        for (int i = VC - 1; i >= 0; --i) back = __builtin_fmaf(y[i], back, v[i]);
+        spans[slot][at.wave][at.lane] = make_float2(decay_of(sum), got);
+        backs[slot][at.wave][at.lane] = back;
+        __syncthreads();
+        float h = now.h, before = 0.0f, behind = 0.0f;
+        float2 p[kWaves];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            p[w] = spans[slot][w][at.lane];
+            if constexpr (!SUMS) {
+                if (w == at.wave) before = h;
+                h = __builtin_fmaf(p[w].x, h, p[w].y);
+            }
+        }
+#pragma unroll
+        for (int w = kWaves - 1; w >= 0; --w) {
+            if (w == at.wave) behind = m;
+            m = __builtin_fmaf(p[w].x, m, backs[slot][w][at.lane]);
+            if constexpr (SUMS) whole *= p[w].x;
+        }
+        if constexpr (!SUMS) {
+#pragma unroll
+            for (int i = 0; i < VC; ++i) {
+                const float x = before;
+                before = __builtin_fmaf(y[i], before, u[i]);
+                u[i] = x;
+            }
+#pragma unroll
+            for (int i = VC - 1; i >= 0; --i) {
+                const float x = behind;
+                behind = __builtin_fmaf(y[i], behind, v[i]);
+                v[i] = x;
+            }
+            transpose<VC>(u);
+            transpose<VC>(v);
+            // each token's state before it
+            float was[TL][VC];
+#pragma unroll
+            for (int k = 0; k < TL; ++k)
+#pragma unroll
+                for (int j = 0; j < VC; ++j) {
+                    was[k][j] = u[j];
+                    float w = root[k][j] * value<T>(now.x[k], j);
+                    if constexpr (GATED) w *= si[k][j];
+                    u[j] = __builtin_fmaf(dec[k][j], u[j], w);
+                }
+#pragma unroll
+            for (int k = TL - 1; k >= 0; --k) {
+                float dx[VC], dg[VC], di[VC];
+#pragma unroll
+                for (int j = 0; j < VC; ++j) {
+                    const float l = value<T>(now.e[k], j) + v[j], x = value<T>(now.x[k], j);
+                    v[j] = dec[k][j] * l;
+                    float w = x;
+                    if constexpr (GATED) w *= si[k][j];
+                    const float dlog = v[j] * (was[k][j] - dec[k][j] * (w * inv[k][j]));
+                    const float d = sg[k][j] * dlog;
+                    dr[j] -= d;
+                    dg[j] = -kLn2 * rate[j] * (d - sg[k][j] * d);
+                    dx[j] = l * root[k][j];
+                    if constexpr (GATED) {
+                        dx[j] *= si[k][j];
+                        di[j] = dx[j] * (x - x * si[k][j]);
+                    }
+                }
+                const int64_t t = t0 + first + k;
+                if (t < end && at.c0 < a.channels) {
+                    store<T, WIDE>(row_of(a.dx, a, s, at.b, size) + t * a.dx.ts * size, at.c0, a.channels, pack<T>(dx));
+                    store<T, WIDE>(row_of(a.dg, a, s, at.b, size) + t * a.dg.ts * size, at.c0, a.channels, pack<T>(dg));
+                    if constexpr (GATED) store<T, WIDE>(row_of(a.di, a, s, at.b, size) + t * a.di.ts * size, at.c0, a.channels, pack<T>(di));
+                }
+            }
+        }
+    };
+    if (begin < end) {
+        Raw one, two;
+        int64_t t0 = begin + (end - 1 - begin) / TILE * TILE;
+        fetch(one, t0);
+        for (; t0 >= begin; t0 -= 2 * TILE) {
+            tile(one, two, t0, 0);
+            if (t0 - TILE >= begin) tile(two, one, t0 - TILE, 1);
+        }
+    }
+    if constexpr (SUMS) {
+        if (at.wave == 0 && at.on) a.spans[((int64_t)at.b * a.ranges + at.range) * a.channels + at.ch] = make_float2(whole, m);
+        return;
+    }
+    if (at.wave == 0 && at.on && at.range == 0 && a.last) a.last[mine] = m;
+    // the rate's gradient: a lane's groups, then the waves, in order
+    transpose<VC>(dr);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VC; ++i) sum += dr[i];
+    __syncthreads();
+    backs[0][at.wave][at.lane] = sum;
+    __syncthreads();
+    if (at.wave || !at.on) return;
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum += backs[0][w][at.lane];
+    a.drate[((int64_t)at.b * a.ranges + at.range) * a.channels + at.ch] = sum;
+}
+
+// the rows of the rate's partial gradients added in order, 64 channels and 4 shares of the rows a workgroup
+__global__ __launch_bounds__(256) void recurrence_rate_kernel(const float* part, float* out, int64_t rows, int32_t channels) {
+    __shared__ float sums[4][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6;
+    float sum = 0.0f;
+    if (c < channels)
+        for (int64_t r = share; r < rows; r += 4) sum += part[r * channels + c];
+    sums[share][threadIdx.x & 63] = sum;
+    __syncthreads();
+    if (share == 0 && c < channels) out[c] = sums[0][threadIdx.x] + sums[1][threadIdx.x] + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+}
+
+// ---------------------------------------------------------------- host
+int refuse(int code, const char* who, const char* why) {
+    set_error("%s: %s", who, why);
+    return code;
+}
+
+int check_shape(const R97qRecurrence* p, const char* who) {
+    if (!p) return refuse(R97Q_EINVAL, who, "null shape");
+    if (p->batch < 0 || p->len < 0 || p->channels < 1) return refuse(R97Q_EINVAL, who, "a negative batch or length, or no channel");
+    if (p->starts && p->tokens < 0) return refuse(R97Q_EINVAL, who, "a negative count of packed tokens");
+    if (p->dtype != R97Q_BF16 && p->dtype != R97Q_F32) return refuse(R97Q_EINVAL, who, "the type is bf16 or f32");
+    if (p->batch > 65535) return refuse(R97Q_EUNSUPPORTED, who, "at most 65535 sequences");
+    // the launches' grids and a row's bytes stay below 2^31
+    if (p->channels > (1 << 28)) return refuse(R97Q_EUNSUPPORTED, who, "at most 2^28 channels");
+    if (p->len > 0x7FFFFFFF || (p->starts && p->tokens > 0x7FFFFFFF)) return refuse(R97Q_EUNSUPPORTED, who, "tokens within 31 bits");
+    return R97Q_OK;
+}
+
+int check_rows(const R97qRows* t, const R97qRecurrence* p, bool output, const char* who, const char* name) {
+    const int64_t tokens = p->starts ? p->tokens : p->len;
+    if (!t || (!t->data && p->batch > 0 && tokens > 0)) {
+        set_error("%s: %s is null", who, name);
+        return R97Q_EINVAL;
+    }
+    if (t->token_stride < 0 || (!p->starts && t->batch_stride < 0) ||
+        (output && ((tokens > 1 && !t->token_stride) || (!p->starts && p->batch > 1 && tokens > 0 && !t->batch_stride)))) {
+        set_error("%s: %s has a negative stride, or is written through a stride of zero", who, name);
+        return R97Q_EINVAL;
+    }
+    if (reinterpret_cast<uintptr_t>(t->data) & (p->dtype == R97Q_F32 ? 3 : 1)) {
+        set_error("%s: %s is off its type's alignment", who, name);
+        return R97Q_EINVAL;
+    }
+    return R97Q_OK;
+}
+
+Rows rows_of(const R97qRows* t) { return t ? Rows{static_cast<uint8_t*>(t->data), t->batch_stride, t->token_stride} : Rows{}; }
+
+bool wide(const R97qRows* t, const R97qRecurrence* p) {
+    if (!t) return true;
+    const int unit = p->dtype == R97Q_F32 ? 4 : 8;
+    return !(reinterpret_cast<uintptr_t>(t->data) & 15) && t->token_stride % unit == 0 && (p->starts || t->batch_stride % unit == 0);
+}
+
+int64_t all_tokens(const R97qRecurrence* p) { return p->starts ? p->tokens : p->batch * p->len; }
+
+// ranges of the tokens, multiples of a forward tile
+void cut(const R97qRecurrence* p, Args& a) {
+    const int64_t slabs = (p->channels + kSlab - 1) / kSlab, have = slabs * p->batch;
+    const int64_t mean = p->batch ? all_tokens(p) / p->batch : 0;
+    int64_t n = have > 0 ? 512 / have : 1;
+    if (n > mean / 512) n = mean / 512;
+    if (n > 64) n = 64;
+    if (n < 1) n = 1;
+    const int64_t len = p->starts && p->len < mean ? mean : p->len;
+    a.range_len = ((len + n - 1) / n + 255) / 256 * 256;
+    if (a.range_len < 256) a.range_len = 256;
+    a.ranges = (int32_t)((len + a.range_len - 1) / a.range_len);
+    if (a.ranges < 1) a.ranges = 1;
+}
+
+Args args_of(const R97qRecurrence* p) {
+    Args a = {};
+    a.starts = p->starts;
+    a.tokens = p->tokens;
+    a.len = p->len;
+    a.batch = p->batch;
+    a.channels = p->channels;
+    cut(p, a);
+    return a;
+}
+int64_t spans_bytes(const Args& a) { return a.ranges > 1 ? (8LL * a.batch * a.ranges * a.channels + 255) / 256 * 256 : 0; }
+int64_t row_bytes(const Args& a, int64_t rows) { return (4 * rows * a.channels + 255) / 256 * 256; }
+
+template <class T, bool GATED, bool WIDE>
+int run_fwd(const Args& a, hipStream_t st) {
+    const unsigned slabs = (unsigned)((a.channels + kSlab - 1) / kSlab);
+    if (a.ranges > 1) {
+        hipLaunchKernelGGL((recurrence_fwd_kernel<T, GATED, WIDE, true>), dim3(slabs, a.ranges - 1, a.batch), dim3(kThreads), 0, st, a);
+        if (int e = launch_status("recurrence_fwd_kernel")) return e;
+    }
+    hipLaunchKernelGGL((recurrence_fwd_kernel<T, GATED, WIDE, false>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
+    return launch_status("recurrence_fwd_kernel");
+}
+template <class T, bool GATED, bool WIDE>
+int run_bwd(const Args& a, hipStream_t st) {
+    const unsigned slabs = (unsigned)((a.channels + kSlab - 1) / kSlab);
+    if (a.ranges > 1) {
+        hipLaunchKernelGGL((recurrence_bwd_kernel<T, GATED, WIDE, true>), dim3(slabs, a.ranges - 1, a.batch), dim3(kThreads), 0, st, a);
+        if (int e = launch_status("recurrence_bwd_kernel")) return e;
+    }
+    hipLaunchKernelGGL((recurrence_bwd_kernel<T, GATED, WIDE, false>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
+    return launch_status("recurrence_bwd_kernel");
+}
+template <class T>
+int pick(const Args& a, bool back, bool wide, hipStream_t st) {
+    if (a.i.p) {
+        if (wide) return back ? run_bwd<T, true, true>(a, st) : run_fwd<T, true, true>(a, st);
+        return back ? run_bwd<T, true, false>(a, st) : run_fwd<T, true, false>(a, st);
+    }
+    if (wide) return back ? run_bwd<T, false, true>(a, st) : run_fwd<T, false, true>(a, st);
+    return back ? run_bwd<T, false, false>(a, st) : run_fwd<T, false, false>(a, st);
+}
+
+}  // namespace
+}  // namespace scan
+}  // namespace r97q
+
+using namespace r97q;
+using namespace r97q::scan;
+
+extern "C" {
+
+int64_t r97q_recurrence_state_rows(const R97qRecurrence* shape) {
+    clear_error();
+    if (check_shape(shape, "r97q_recurrence_state_rows")) return -1;
+    return shape->starts ? shape->tokens / kChunk + shape->batch : shape->batch * ((shape->len + kChunk - 1) / kChunk);
+}
+
+int64_t r97q_recurrence_fwd_workspace_bytes(const R97qRecurrence* shape) {
+    clear_error();
+    if (check_shape(shape, "r97q_recurrence_fwd_workspace_bytes")) return -1;
+    const Args a = args_of(shape);
+    return a.ranges > 1 ? spans_bytes(a) + row_bytes(a, a.batch) : 0;
+}
+
+int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R97qRows* gate, const R97qRows* input_gate,
+                        const float* rate, const float* h0, const R97qRows* h, float* last, float* states, void* workspace,
+                        int64_t workspace_bytes, R97IqrStream stream) {
+    clear_error();
+    const char* who = "r97q_recurrence_fwd";
+    if (int e = check_shape(shape, who)) return e;
+    if (int e = check_rows(x, shape, false, who, "x")) return e;
+    if (int e = check_rows(gate, shape, false, who, "gate")) return e;
+    if (input_gate)
+        if (int e = check_rows(input_gate, shape, false, who, "input_gate")) return e;
+    if (int e = check_rows(h, shape, true, who, "h")) return e;
+    if (!rate) return refuse(R97Q_EINVAL, who, "null rate");
+    if (shape->batch == 0) return R97Q_OK;
+    Args a = args_of(shape);
+    const int64_t need = a.ranges > 1 ? spans_bytes(a) + row_bytes(a, a.batch) : 0;
+    if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
+    if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
+    a.x = rows_of(x);
+    a.g = rows_of(gate);
+    a.i = rows_of(all_tokens(shape) > 0 ? input_gate : nullptr);
+    a.h = rows_of(h);
+    a.rate = rate;
+    a.first = h0;
+    a.last = last;
+    a.states = states;
+    a.spans = static_cast<float2*>(workspace);
+    a.kept = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + spans_bytes(a));
+    const bool w = a.channels % (shape->dtype == R97Q_F32 ? 4 : 8) == 0 && wide(x, shape) && wide(gate, shape) && wide(input_gate, shape) && wide(h, shape);
+    return shape->dtype == R97Q_F32 ? pick<float>(a, false, w, (hipStream_t)stream) : pick<uint16_t>(a, false, w, (hipStream_t)stream);
+}
+
+int64_t r97q_recurrence_bwd_workspace_bytes(const R97qRecurrence* shape) {
+    clear_error();
+    if (check_shape(shape, "r97q_recurrence_bwd_workspace_bytes")) return -1;
+    const Args a = args_of(shape);
+    const int64_t rows = (int64_t)a.batch * a.ranges;
+    return spans_bytes(a) + (rows > 1 ? row_bytes(a, rows) : 0);
+}
+
+int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R97qRows* gate, const R97qRows* input_gate,
+                        const float* rate, const float* states, const R97qRows* d_h, const float* d_last, const R97qRows* dx,
+                        const R97qRows* dgate, const R97qRows* dinput_gate, float* drate, float* dh0, void* workspace,
+                        int64_t workspace_bytes, R97IqrStream stream) {
+    clear_error();
+    const char* who = "r97q_recurrence_bwd";
+    if (int e = check_shape(shape, who)) return e;
+    if (int e = check_rows(x, shape, false, who, "x")) return e;
+    if (int e = check_rows(gate, shape, false, who, "gate")) return e;
+    if (!input_gate != !dinput_gate) return refuse(R97Q_EINVAL, who, "input_gate and dinput_gate come together");
+    if (input_gate) {
+        if (int e = check_rows(input_gate, shape, false, who, "input_gate")) return e;
+        if (int e = check_rows(dinput_gate, shape, true, who, "dinput_gate")) return e;
+    }
+    if (int e = check_rows(d_h, shape, false, who, "d_h")) return e;
+    if (int e = check_rows(dx, shape, true, who, "dx")) return e;
+    if (int e = check_rows(dgate, shape, true, who, "dgate")) return e;
+    if (!rate || !drate) return refuse(R97Q_EINVAL, who, "null rate or drate");
+    if (!states && shape->batch > 0 && all_tokens(shape) > 0) return refuse(R97Q_EINVAL, who, "null states");
+    Args a = args_of(shape);
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t rows = (int64_t)a.batch * a.ranges, need = spans_bytes(a) + (rows > 1 ? row_bytes(a, rows) : 0);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
+    if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
+    a.x = rows_of(x);
+    a.g = rows_of(gate);
+    a.i = rows_of(all_tokens(shape) > 0 ? input_gate : nullptr);
+    a.h = rows_of(d_h);
+    a.dx = rows_of(dx);
+    a.dg = rows_of(dgate);
+    a.di = rows_of(dinput_gate);
+    a.rate = rate;
+    a.first = d_last;
+    a.last = dh0;
+    a.states = const_cast<float*>(states);
+    a.spans = static_cast<float2*>(workspace);
+    a.drate = rows > 1 ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + spans_bytes(a)) : drate;
+    const bool w = a.channels % (shape->dtype == R97Q_F32 ? 4 : 8) == 0 && wide(x, shape) && wide(gate, shape) && wide(input_gate, shape) &&
+                   wide(d_h, shape) && wide(dx, shape) && wide(dgate, shape) && wide(dinput_gate, shape);
+    if (rows > 0)
+        if (int e = shape->dtype == R97Q_F32 ? pick<float>(a, true, w, st) : pick<uint16_t>(a, true, w, st)) return e;
+    if (rows == 1) return R97Q_OK;
+    hipLaunchKernelGGL(recurrence_rate_kernel, dim3((unsigned)((a.channels + 63) / 64)), dim3(256), 0, st, a.drate, drate, rows, a.channels);
+    return launch_status("recurrence_rate_kernel");
+}
+
+}  // extern "C"
