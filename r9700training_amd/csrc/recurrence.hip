@@ -75,9 +75,11 @@ __device__ __forceinline__ Span span_of(const Args& a, int b) {
     }
     return s;
 }
-__device__ __forceinline__ uint8_t* row_of(const Rows& t, const Args& a, const Span& s, int b, int size) {
-    return t.p + (a.starts ? s.base * t.ts : b * t.bs) * size;
+__device__ __forceinline__ uint32_t fresh(uint32_t x) {
+    asm volatile("" : "+s"(x));
+    return x;
 }
+constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every buffer's end
 
 // ---------------------------------------------------------------- pieces of 16 bytes
 template <class T>
@@ -102,29 +104,56 @@ __device__ __forceinline__ u32x4 pack(const float* x) {
     }
     return v;
 }
-// the piece at channel c0 of a row; not WIDE: value by value, the last channel again past the end
+// One of a sequence's tensors, in tiles of `rows` tokens. WIDE: a tile is a buffer that ends with its last token, so a load past
+// it gives zeros and a store past it is dropped, every tile has as many of both (nothing waits for a store whose number the
+// compiler cannot know), and an offset is 32 bits. Else value by value, the last token and channel again past the end.
 template <class T, bool WIDE>
-__device__ __forceinline__ u32x4 load(const uint8_t* row, int c0, int channels) {
-    if constexpr (WIDE) return *reinterpret_cast<const u32x4*>(row + (int64_t)c0 * sizeof(T));
-    else {
-        const T* p = reinterpret_cast<const T*>(row);
+struct Io;
+template <class T>
+struct Io<T, true> {
+    uint64_t base;
+    uint32_t ts, row, off;  // bytes a token; of a row; the thread's first piece in a tile
+    __device__ __forceinline__ Io(const Rows& t, const Args& a, const Span& s, int b, int first, int c0)
+        : base(reinterpret_cast<uint64_t>(t.p) + (a.starts ? s.base * t.ts : b * t.bs) * sizeof(T)), ts((uint32_t)(t.ts * sizeof(T))),
+          row((uint32_t)(a.channels * sizeof(T))), off(c0 < a.channels ? first * ts + c0 * (uint32_t)sizeof(T) : kNowhere) {}
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(int64_t t0, int64_t end, int rows) const {
+        const int left = end - t0 < rows ? (int)(end - t0) : rows;
+        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base + t0 * ts), 0, left > 0 ? (int)((left - 1) * ts + row) : 0, 0x00020000);
+    }
+    // (offsets are formed where they are used: held through the loop they would take a register for every token)
+    __device__ __forceinline__ u32x4 load(__amdgpu_buffer_rsrc_t buf, int k) const { return __builtin_amdgcn_raw_buffer_load_b128(buf, off + k * fresh(ts), 0, 0); }
+    __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t buf, int k, const u32x4& v) const { __builtin_amdgcn_raw_buffer_store_b128(v, buf, off + k * fresh(ts), 0, 0); }
+};
+template <class T>
+struct Io<T, false> {
+    struct Tile {
+        T* p;          // the thread's first token
+        int left;      // tokens from there to the end
+    };
+    T* base;
+    int64_t ts;
+    int first, c0, channels;
+    __device__ __forceinline__ Io(const Rows& t, const Args& a, const Span& s, int b, int first_, int c0_)
+        : base(reinterpret_cast<T*>(t.p) + (a.starts ? s.base * t.ts : b * t.bs)), ts(t.ts), first(first_), c0(c0_), channels(a.channels) {}
+    __device__ __forceinline__ Tile buffer(int64_t t0, int64_t end, int rows) const {
+        const int64_t left = end - t0 - first;
+        return {base + (t0 + first) * ts, left > rows ? rows : (int)left};
+    }
+    __device__ __forceinline__ u32x4 load(const Tile& t, int k) const {
+        const T* p = t.p + (k < t.left ? k : t.left - 1) * ts;
         T x[kVC<T>];
 #pragma unroll
         for (int j = 0; j < kVC<T>; ++j) x[j] = p[c0 + j < channels ? c0 + j : channels - 1];
         return __builtin_bit_cast(u32x4, x);
     }
-}
-template <class T, bool WIDE>
-__device__ __forceinline__ void store(uint8_t* row, int c0, int channels, const u32x4& v) {
-    if constexpr (WIDE) *reinterpret_cast<u32x4*>(row + (int64_t)c0 * sizeof(T)) = v;
-    else {
-        T* p = reinterpret_cast<T*>(row);
+    __device__ __forceinline__ void store(const Tile& t, int k, const u32x4& v) const {
         struct { T x[kVC<T>]; } u = __builtin_bit_cast(decltype(u), v);
+        if (k < t.left)
 #pragma unroll
-        for (int j = 0; j < kVC<T>; ++j)
-            if (c0 + j < channels) p[c0 + j] = u.x[j];
+            for (int j = 0; j < kVC<T>; ++j)
+                if (c0 + j < channels) t.p[k * ts + c0 + j] = u.x[j];
     }
-}
+};
 
 // ---------------------------------------------------------------- the gates
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -136,7 +165,7 @@ __device__ __forceinline__ float sigmoid(float v) {
     const float t = v * -kLog2e;
     float e = exp2_(t);
     if constexpr (sizeof(T) == 4) {
-        const float r = __builtin_fmaf(v, -kLog2e, -t) - v * kLog2eLow;
+        const float r = __builtin_fmaf(-v, kLog2eLow, __builtin_fmaf(v, -kLog2e, -t));
         e = __builtin_fmaf(e, r * kLn2, e);
     }
     return __builtin_amdgcn_rcpf(1.0f + e);
@@ -200,8 +229,8 @@ __device__ __forceinline__ void transpose(float (&x)[VC]) {
 template <class T>
 struct Place {
     static constexpr int VC = kVC<T>, LPR = 64 / VC;
-    int lane, wave, g, c0, ch, b, range;
-    bool on;  // the transposed lane's channel is one
+    int lane, wave, g, c0, ch, near, b, range;
+    bool on;  // the transposed lane's channel is one (near: one that may be read in any case)
     __device__ __forceinline__ Place(const Args& a, int range0 = 0) {
         lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -209,10 +238,24 @@ struct Place {
         c0 = blockIdx.x * kSlab + lane % LPR * VC;
         ch = c0 + g;
         on = ch < a.channels;
+        near = on ? ch : a.channels - 1;
         range = range0 + blockIdx.y;
         b = blockIdx.z;
     }
 };
+
+// what a value carries through the spans p[0], p[step], .. (`many` of them) in order, their loads out together
+__device__ __forceinline__ float through(const float2* p, int64_t step, int many, float v) {
+    constexpr int kBatch = 8;
+    for (int r = 0; r < many; r += kBatch) {
+        float2 s[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) s[i] = p[(r + i < many ? r + i : many - 1) * step];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) v = r + i < many ? __builtin_fmaf(s[i].x, v, s[i].y) : v;
+    }
+    return v;
+}
 
 // tokens past the end: nothing enters, nothing decays
 template <class T>
@@ -230,7 +273,7 @@ __device__ __forceinline__ void blank(u32x4& x, u32x4& g, u32x4& i, bool out) {
 // grid (slabs, ranges, sequences). SUMS: only the ranges' spans, for the next launch.
 template <class T, bool GATED, bool WIDE, bool SUMS>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
-    constexpr int VC = kVC<T>, TL = 4, WT = VC * TL, TILE = kWaves * WT, size = sizeof(T);
+    constexpr int VC = kVC<T>, TL = 4, WT = VC * TL, TILE = kWaves * WT;
     static_assert(TILE % kChunk == 0 && kChunk % WT == 0, "chunks begin with a wave");
     __shared__ float2 spans[2][kWaves][64];
     const Place<T> at(a);
@@ -238,40 +281,34 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
     const int64_t begin = at.range * a.range_len;
     const int64_t end = !SUMS && at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
     float h = 0.0f, whole = 1.0f;
-    const int64_t mine = (int64_t)at.b * a.channels + at.ch;
-    if (at.on) {
-        if (at.range == 0) {
-            if (a.first) h = a.ranges > 1 && !SUMS ? a.kept[mine] : a.first[mine];
-            if (SUMS && a.first && at.wave == 0) a.kept[mine] = h;
-        } else if (!SUMS) {
-            const float2* p = a.spans + (int64_t)at.b * a.ranges * a.channels + at.ch;
-            for (int r = 0; r < at.range; ++r, p += a.channels) h = __builtin_fmaf(p->x, h, p->y);
-        }
+    const int64_t mine = (int64_t)at.b * a.channels + at.near;
+    if (at.range == 0) {
+        if (a.first) h = a.ranges > 1 && !SUMS ? a.kept[mine] : a.first[mine];
+        if (SUMS && a.first && at.wave == 0 && at.on) a.kept[mine] = h;
+    } else if (!SUMS) {
+        h = through(a.spans + (int64_t)at.b * a.ranges * a.channels + at.near, a.channels, at.range, 0.0f);
     }
     float rate[VC];
 #pragma unroll
-    for (int j = 0; j < VC; ++j) rate[j] = at.c0 + j < a.channels ? a.rate[at.c0 + j] * kLog2e : 0.0f;
-    const int c0 = !WIDE || at.c0 < a.channels ? at.c0 : 0;
-    const uint8_t* xr = row_of(a.x, a, s, at.b, size);
-    const uint8_t* gr = row_of(a.g, a, s, at.b, size);
-    const uint8_t* ir = GATED ? row_of(a.i, a, s, at.b, size) : nullptr;
-    uint8_t* hr = SUMS ? nullptr : row_of(a.h, a, s, at.b, size);
+    for (int j = 0; j < VC; ++j) rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e;
     const int first = at.wave * WT + at.g * TL;  // the thread's first token in a tile
+    using IO = Io<T, WIDE>;
+    const IO xs(a.x, a, s, at.b, first, at.c0), gs(a.g, a, s, at.b, first, at.c0), is(a.i, a, s, at.b, first, at.c0), hs(a.h, a, s, at.b, first, at.c0);
 
     struct Raw {
         u32x4 x[TL], g[TL], i[TL];
     };
     auto fetch = [&](Raw& r, int64_t t0) {
+        const auto x = xs.buffer(t0, end, TILE), g = gs.buffer(t0, end, TILE), i = is.buffer(t0, end, TILE);
 #pragma unroll
         for (int k = 0; k < TL; ++k) {
-            const int64_t t = t0 + first + k < end ? t0 + first + k : end - 1;
-            r.x[k] = load<T, WIDE>(xr + t * a.x.ts * size, c0, a.channels);
-            r.g[k] = load<T, WIDE>(gr + t * a.g.ts * size, c0, a.channels);
-            if constexpr (GATED) r.i[k] = load<T, WIDE>(ir + t * a.i.ts * size, c0, a.channels);
+            r.x[k] = xs.load(x, k);
+            r.g[k] = gs.load(g, k);
+            if constexpr (GATED) r.i[k] = is.load(i, k);
         }
     };
     auto tile = [&](Raw& now, Raw& next, int64_t t0, int slot) {
-        if (t0 + TILE < end) fetch(next, t0 + TILE);
+        fetch(next, t0 + TILE);  // nothing past the end
         __builtin_amdgcn_sched_barrier(0);
         if (t0 + TILE > end) {
 #pragma unroll
@@ -313,8 +350,12 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
             if constexpr (SUMS) whole *= p.x;
         }
         if constexpr (!SUMS) {
-            const int64_t token = t0 + at.wave * WT;
-            if (a.states && at.wave * WT % kChunk == 0 && token < end && at.on) a.states[(s.state + token / kChunk) * a.channels + at.ch] = before;
+            if (at.wave * WT % kChunk == 0) {
+                const int64_t token = t0 + at.wave * WT;
+                const auto kept = __builtin_amdgcn_make_buffer_rsrc(a.states + (s.state + token / kChunk) * a.channels, 0,
+                                                                    a.states && token < end ? a.channels * 4 : 0, 0x00020000);
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, before), kept, 4 * at.ch, 0, 0);
+            }
 #pragma unroll
             for (int i = 0; i < VC; ++i) {
                 const float x = before;
@@ -322,12 +363,12 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
                 u[i] = x;
             }
             transpose<VC>(u);
+            const auto h = hs.buffer(t0, end, TILE);
 #pragma unroll
             for (int k = 0; k < TL; ++k) {
 #pragma unroll
                 for (int j = 0; j < VC; ++j) u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j]);
-                const int64_t t = t0 + first + k;
-                if (t < end && at.c0 < a.channels) store<T, WIDE>(hr + t * a.h.ts * size, at.c0, a.channels, pack<T>(u));
+                hs.store(h, k, pack<T>(u));
             }
         }
     };
@@ -349,7 +390,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
 // it is carried. SUMS: only the ranges' spans (a and dh alone).
 template <class T, bool GATED, bool WIDE, bool SUMS>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
-    constexpr int VC = kVC<T>, TL = 16 / VC, WT = VC * TL, TILE = kWaves * WT, size = sizeof(T);
+    constexpr int VC = kVC<T>, TL = 16 / VC, WT = VC * TL, TILE = kWaves * WT;
     static_assert(TILE == kChunk, "a tile begins at a kept state");
     __shared__ float2 spans[2][kWaves][64];
     __shared__ float backs[2][kWaves][64];
@@ -358,44 +399,40 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     const int64_t begin = at.range * a.range_len;
     const int64_t end = at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
     float m = 0.0f, whole = 1.0f;  // the cotangent behind the tile, times its decay
-    const int64_t mine = (int64_t)at.b * a.channels + at.ch;
-    if (at.on) {
-        if (at.range == a.ranges - 1 || !SUMS) m = a.first ? a.first[mine] : 0.0f;
-        if (!SUMS && at.range < a.ranges - 1) {
-            m = 0.0f;  // the last range's span holds it
-            const float2* p = a.spans + ((int64_t)at.b * a.ranges + a.ranges - 1) * a.channels + at.ch;
-            for (int r = a.ranges - 1; r > at.range; --r, p -= a.channels) m = __builtin_fmaf(p->x, m, p->y);
-        }
+    const int64_t mine = (int64_t)at.b * a.channels + at.near;
+    if (at.range == a.ranges - 1) {
+        if (a.first) m = a.first[mine];
+    } else if (!SUMS) {  // the last range's span holds what is behind it
+        m = through(a.spans + ((int64_t)at.b * a.ranges + a.ranges - 1) * a.channels + at.near, -(int64_t)a.channels, a.ranges - 1 - at.range, 0.0f);
     }
     float rate[VC], dr[VC];
 #pragma unroll
-    for (int j = 0; j < VC; ++j) rate[j] = at.c0 + j < a.channels ? a.rate[at.c0 + j] * kLog2e : 0.0f, dr[j] = 0.0f;
-    const int c0 = !WIDE || at.c0 < a.channels ? at.c0 : 0;
-    const uint8_t* xr = SUMS ? nullptr : row_of(a.x, a, s, at.b, size);
-    const uint8_t* gr = row_of(a.g, a, s, at.b, size);
-    const uint8_t* ir = GATED && !SUMS ? row_of(a.i, a, s, at.b, size) : nullptr;
-    const uint8_t* er = row_of(a.h, a, s, at.b, size);
+    for (int j = 0; j < VC; ++j) rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e, dr[j] = 0.0f;
     const int first = at.wave * WT + at.g * TL;
+    using IO = Io<T, WIDE>;
+    const IO xs(a.x, a, s, at.b, first, at.c0), gs(a.g, a, s, at.b, first, at.c0), is(a.i, a, s, at.b, first, at.c0), es(a.h, a, s, at.b, first, at.c0);
+    const IO dxs(a.dx, a, s, at.b, first, at.c0), dgs(a.dg, a, s, at.b, first, at.c0), dis(a.di, a, s, at.b, first, at.c0);
 
     struct Raw {
         u32x4 x[TL], g[TL], i[TL], e[TL];
         float h;
     };
-    auto fetch = [&](Raw& r, int64_t t0) {
+    auto fetch = [&](Raw& r, int64_t to) {  // nothing before the beginning
+        const int64_t t0 = to >= begin ? to : begin, upto = !WIDE || to >= begin ? end : begin;
+        const auto x = xs.buffer(t0, upto, TILE), g = gs.buffer(t0, upto, TILE), i = is.buffer(t0, upto, TILE), e = es.buffer(t0, upto, TILE);
 #pragma unroll
         for (int k = 0; k < TL; ++k) {
-            const int64_t t = t0 + first + k < end ? t0 + first + k : end - 1;
-            r.g[k] = load<T, WIDE>(gr + t * a.g.ts * size, c0, a.channels);
-            r.e[k] = load<T, WIDE>(er + t * a.h.ts * size, c0, a.channels);
+            r.g[k] = gs.load(g, k);
+            r.e[k] = es.load(e, k);
             if constexpr (!SUMS) {
-                r.x[k] = load<T, WIDE>(xr + t * a.x.ts * size, c0, a.channels);
-                if constexpr (GATED) r.i[k] = load<T, WIDE>(ir + t * a.i.ts * size, c0, a.channels);
+                r.x[k] = xs.load(x, k);
+                if constexpr (GATED) r.i[k] = is.load(i, k);
             }
         }
-        if constexpr (!SUMS) r.h = at.on ? a.states[(s.state + t0 / kChunk) * a.channels + at.ch] : 0.0f;
+        if constexpr (!SUMS) r.h = a.states[(s.state + t0 / kChunk) * a.channels + at.near];
     };
     auto tile = [&](Raw& now, Raw& next, int64_t t0, int slot) {
-        if (t0 > begin) fetch(next, t0 - TILE);
+        fetch(next, t0 - TILE);
         __builtin_amdgcn_sched_barrier(0);
         if (t0 + TILE > end) {
 #pragma unroll
@@ -406,8 +443,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
                 for (int e = 0; e < 4; ++e) now.e[k][e] = out ? 0u : now.e[k][e];
             }
         }
-        // a, the gates, sqrt(q) and its inverse
-        float dec[TL][VC], sg[TL][VC], si[TL][VC], root[TL][VC], inv[TL][VC], y[VC], u[VC], v[VC];
+        // a, the gates, what x enters by (sqrt(q) sigmoid(i)) and what it takes from dlog a (a sigmoid(i) / sqrt(q))
+        float dec[TL][VC], sg[TL][VC], si[TL][VC], in[TL][VC], near[TL][VC], y[VC], u[VC], v[VC];
 #pragma unroll
         for (int j = 0; j < VC; ++j) {
             y[j] = u[j] = v[j] = 0.0f;
@@ -420,14 +457,15 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
                 if constexpr (!SUMS) {
                     const float q = room(e, dec[k][j]);
                     // where nothing decays the root's derivative counts as none
-                    inv[k][j] = q >= 0x1p-126f ? __builtin_amdgcn_rsqf(q) : q * 0.0f;
-                    root[k][j] = q * inv[k][j];
-                    float w = root[k][j] * value<T>(now.x[k], j);
+                    const float inv = q >= 0x1p-126f ? __builtin_amdgcn_rsqf(q) : q * 0.0f;
+                    in[k][j] = q * inv;
+                    near[k][j] = dec[k][j] * inv;
                     if constexpr (GATED) {
                         si[k][j] = sigmoid<T>(value<T>(now.i[k], j));
-                        w *= si[k][j];
+                        in[k][j] *= si[k][j];
+                        near[k][j] *= si[k][j];
                     }
-                    u[j] = __builtin_fmaf(dec[k][j], u[j], w);
+                    u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j] * value<T>(now.x[k], j));
                 }
             }
 #pragma unroll
@@ -465,6 +503,9 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
             if constexpr (SUMS) whole *= p[w].x;
         }
         if constexpr (!SUMS) {
+            // the inputs are taken apart again: both forms would not fit the registers
+#pragma unroll
+            for (int k = 0; k < TL; ++k) asm volatile("" : "+v"(now.x[k]), "+v"(now.e[k]));
 #pragma unroll
             for (int i = 0; i < VC; ++i) {
                 const float x = before;
@@ -479,6 +520,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
             }
             transpose<VC>(u);
             transpose<VC>(v);
+            const auto bx = dxs.buffer(t0, end, TILE), bg = dgs.buffer(t0, end, TILE), bi = dis.buffer(t0, end, TILE);
             // each token's state before it
             float was[TL][VC];
 #pragma unroll
@@ -486,9 +528,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
 #pragma unroll
                 for (int j = 0; j < VC; ++j) {
                     was[k][j] = u[j];
-                    float w = root[k][j] * value<T>(now.x[k], j);
-                    if constexpr (GATED) w *= si[k][j];
-                    u[j] = __builtin_fmaf(dec[k][j], u[j], w);
+                    u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j] * value<T>(now.x[k], j));
                 }
 #pragma unroll
             for (int k = TL - 1; k >= 0; --k) {
@@ -497,24 +537,15 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
                 for (int j = 0; j < VC; ++j) {
                     const float l = value<T>(now.e[k], j) + v[j], x = value<T>(now.x[k], j);
                     v[j] = dec[k][j] * l;
-                    float w = x;
-                    if constexpr (GATED) w *= si[k][j];
-                    const float dlog = v[j] * (was[k][j] - dec[k][j] * (w * inv[k][j]));
-                    const float d = sg[k][j] * dlog;
+                    const float d = sg[k][j] * (v[j] * __builtin_fmaf(-near[k][j], x, was[k][j]));
                     dr[j] -= d;
-                    dg[j] = -kLn2 * rate[j] * (d - sg[k][j] * d);
-                    dx[j] = l * root[k][j];
-                    if constexpr (GATED) {
-                        dx[j] *= si[k][j];
-                        di[j] = dx[j] * (x - x * si[k][j]);
-                    }
-                }
-                const int64_t t = t0 + first + k;
-                if (t < end && at.c0 < a.channels) {
-                    store<T, WIDE>(row_of(a.dx, a, s, at.b, size) + t * a.dx.ts * size, at.c0, a.channels, pack<T>(dx));
-                    store<T, WIDE>(row_of(a.dg, a, s, at.b, size) + t * a.dg.ts * size, at.c0, a.channels, pack<T>(dg));
-                    if constexpr (GATED) store<T, WIDE>(row_of(a.di, a, s, at.b, size) + t * a.di.ts * size, at.c0, a.channels, pack<T>(di));
-                }
+                    dg[j] = -kLn2 * rate[j] * __builtin_fmaf(-sg[k][j], d, d);
+                    dx[j] = l * in[k][j];
+                    if constexpr (GATED) di[j] = dx[j] * __builtin_fmaf(-x, si[k][j], x);
+                        }
+                dxs.store(bx, k, pack<T>(dx));
+                dgs.store(bg, k, pack<T>(dg));
+                if constexpr (GATED) dis.store(bi, k, pack<T>(di));
             }
         }
     };
@@ -588,6 +619,10 @@ int check_rows(const R97qRows* t, const R97qRecurrence* p, bool output, const ch
         set_error("%s: %s has a negative stride, or is written through a stride of zero", who, name);
         return R97Q_EINVAL;
     }
+    if (output && tokens > 1 && t->token_stride > 0 && t->token_stride < p->channels) {
+        set_error("%s: %s is written with its tokens less than a row apart", who, name);
+        return R97Q_EINVAL;
+    }
     if (reinterpret_cast<uintptr_t>(t->data) & (p->dtype == R97Q_F32 ? 3 : 1)) {
         set_error("%s: %s is off its type's alignment", who, name);
         return R97Q_EINVAL;
@@ -599,8 +634,10 @@ Rows rows_of(const R97qRows* t) { return t ? Rows{static_cast<uint8_t*>(t->data)
 
 bool wide(const R97qRows* t, const R97qRecurrence* p) {
     if (!t) return true;
+    // a tile's rows lie within 31 bits of its first
     const int unit = p->dtype == R97Q_F32 ? 4 : 8;
-    return !(reinterpret_cast<uintptr_t>(t->data) & 15) && t->token_stride % unit == 0 && (p->starts || t->batch_stride % unit == 0);
+    return !(reinterpret_cast<uintptr_t>(t->data) & 15) && t->token_stride % unit == 0 && (p->starts || t->batch_stride % unit == 0) &&
+           t->token_stride <= (1 << 20);
 }
 
 int64_t all_tokens(const R97qRecurrence* p) { return p->starts ? p->tokens : p->batch * p->len; }
@@ -609,7 +646,10 @@ int64_t all_tokens(const R97qRecurrence* p) { return p->starts ? p->tokens : p->
 void cut(const R97qRecurrence* p, Args& a) {
     const int64_t slabs = (p->channels + kSlab - 1) / kSlab, have = slabs * p->batch;
     const int64_t mean = p->batch ? all_tokens(p) / p->batch : 0;
-    int64_t n = have > 0 ? 512 / have : 1;
+#ifndef WANT
+#define WANT 256
+#endif
+    int64_t n = have > 0 ? WANT / have : 1;
     if (n > mean / 512) n = mean / 512;
     if (n > 64) n = 64;
     if (n < 1) n = 1;
