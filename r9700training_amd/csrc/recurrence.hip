@@ -53,10 +53,11 @@ struct Args {
     const int32_t* starts;
     int64_t tokens, len;
     int32_t batch, channels;
-    int32_t ranges;
-    int64_t range_len;
-    float2* spans;                // [batch][ranges][channels], the ranges' spans
+    int32_t ranges, fine;         // and a range's spans
+    int64_t range_len, span_len;
+    float2* spans;                // [batch][ranges * fine][channels]
     float* kept;                  // [batch][channels]: `first`, where `last` may be written over it
+    int32_t few;                  // a thread a sequence
     float* drate;                 // [batch * ranges][channels], or the sum itself where that is one row
 };
 
@@ -155,6 +156,24 @@ struct Io<T, false> {
     }
 };
 
+// a sequence's tensor, a token's piece at a time
+template <class T, bool WIDE>
+struct Piece {
+    const T* base;
+    int64_t ts;
+    int c0, channels;
+    __device__ __forceinline__ Piece(const Rows& t, const Args& a, const Span& s, int b, int c0_)
+        : base(reinterpret_cast<const T*>(t.p) + (a.starts ? s.base * t.ts : b * t.bs)), ts(t.ts), c0(!WIDE || c0_ < a.channels ? c0_ : 0), channels(a.channels) {}
+    __device__ __forceinline__ u32x4 load(int64_t token) const {
+        const T* p = base + token * ts;
+        if constexpr (WIDE) return *reinterpret_cast<const u32x4*>(p + c0);
+        T x[kVC<T>];
+#pragma unroll
+        for (int j = 0; j < kVC<T>; ++j) x[j] = p[c0 + j < channels ? c0 + j : channels - 1];
+        return __builtin_bit_cast(u32x4, x);
+    }
+};
+
 // ---------------------------------------------------------------- the gates
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // 1 / (1 + e^-v). The product with log2 e is off by half a step of itself, which for a far gate is more than a step of the
@@ -244,16 +263,26 @@ struct Place {
     }
 };
 
-// what a value carries through the spans p[0], p[step], .. (`many` of them) in order, their loads out together
-__device__ __forceinline__ float through(const float2* p, int64_t step, int many, float v) {
+// What comes of nothing through the spans p[0], p[step], .. (`many` of them) in order: each wave joins a share of them, their
+// loads out together, and all waves join the shares. lds: a float2 for each thread; called by all of them.
+__device__ __forceinline__ float through(const float2* p, int64_t step, int many, int wave, int lane, float2 (*lds)[64]) {
     constexpr int kBatch = 8;
-    for (int r = 0; r < many; r += kBatch) {
+    const int share = (many + kWaves - 1) / kWaves, end = (wave + 1) * share < many ? (wave + 1) * share : many;
+    float2 own = make_float2(1.0f, 0.0f);
+    for (int r = wave * share; r < end; r += kBatch) {
         float2 s[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) s[i] = p[(r + i < many ? r + i : many - 1) * step];
+        for (int i = 0; i < kBatch; ++i) s[i] = p[(r + i < end ? r + i : r) * step];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) v = r + i < many ? __builtin_fmaf(s[i].x, v, s[i].y) : v;
+        for (int i = 0; i < kBatch; ++i)
+            if (r + i < end) own = make_float2(own.x * s[i].x, __builtin_fmaf(s[i].x, own.y, s[i].y));
     }
+    lds[wave][lane] = own;
+    __syncthreads();
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v = __builtin_fmaf(lds[w][lane].x, v, lds[w][lane].y);
+    __syncthreads();
     return v;
 }
 
@@ -269,24 +298,117 @@ __device__ __forceinline__ void blank(u32x4& x, u32x4& g, u32x4& i, bool out) {
     }
 }
 
+// ---------------------------------------------------------------- the ranges' spans
+// grid (slabs, all but one range's spans, sequences): what a part of a range makes of the state before it, or (BACK, from a and dh alone) of the
+// cotangent behind it. Nothing is needed of the tokens between, so a lane's group takes a run of tokens of its own, with no
+// join but one at the end. The span that has the given end (the first, or BACK the last) holds it; the forward
+// also keeps a copy of it, since `last` may be written over it before every workgroup of the next launch has read it.
+template <class T, bool GATED, bool WIDE, bool BACK>
+__global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
+    constexpr int VC = kVC<T>, TL = 4;
+    __shared__ float2 spans[kWaves][64];
+    const Place<T> at(a, BACK ? a.fine : 0);
+    const Span s = span_of(a, at.b);
+    const int all = a.ranges * a.fine;
+    const int64_t begin = at.range * a.span_len;
+    const int64_t end = BACK && at.range == all - 1 ? s.len : clamp64(begin + a.span_len, 0, s.len);
+    const int64_t run = (end - begin + kWaves * VC - 1) / (kWaves * VC), from = begin + (at.wave * VC + at.g) * run;
+    float rate[VC], y[VC], u[VC];
+#pragma unroll
+    for (int j = 0; j < VC; ++j) {
+        rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e;
+        y[j] = u[j] = 0.0f;
+    }
+    const Piece<T, WIDE> xs(BACK ? a.h : a.x, a, s, at.b, at.c0), gs(a.g, a, s, at.b, at.c0), is(a.i, a, s, at.b, at.c0);
+    struct Raw {
+        u32x4 x[TL], g[TL], i[TL];
+    };
+    // the run's tokens k .. k + TL - 1 in the order they are taken
+    auto token = [&](int64_t k) { return BACK ? from + run - 1 - k : from + k; };
+    auto fetch = [&](Raw& r, int64_t k0) {
+#pragma unroll
+        for (int k = 0; k < TL; ++k) {
+            const int64_t t = clamp64(token(k0 + k), begin, end - 1);
+            r.x[k] = xs.load(t);
+            r.g[k] = gs.load(t);
+            if constexpr (GATED && !BACK) r.i[k] = is.load(t);
+        }
+    };
+    auto take = [&](Raw& now, Raw& next, int64_t k0) {
+        fetch(next, k0 + TL);
+        __builtin_amdgcn_sched_barrier(0);
+        if (k0 + TL > run || begin + run * kWaves * VC > end) {
+#pragma unroll
+            for (int k = 0; k < TL; ++k) blank<T>(now.x[k], now.g[k], now.i[k], k0 + k >= run || token(k0 + k) >= end);
+        }
+#pragma unroll
+        for (int k = 0; k < TL; ++k)
+#pragma unroll
+            for (int j = 0; j < VC; ++j) {
+                const float e = rate[j] * sigmoid<T>(value<T>(now.g[k], j)), dec = exp2_(-e);
+                y[j] += e;
+                if constexpr (BACK) {
+                    u[j] = dec * (u[j] + value<T>(now.x[k], j));
+                } else {
+                    float w = value<T>(now.x[k], j);
+                    if constexpr (GATED) w *= sigmoid<T>(value<T>(now.i[k], j));
+                    u[j] = __builtin_fmaf(dec, u[j], __builtin_amdgcn_sqrtf(room(e, dec)) * w);
+                }
+            }
+    };
+    if (begin < end) {
+        Raw one, two;
+        fetch(one, 0);
+        for (int64_t k0 = 0; k0 < run; k0 += 2 * TL) {
+            take(one, two, k0);
+            if (k0 + TL < run) take(two, one, k0 + TL);
+        }
+    }
+    transpose<VC>(y);
+    transpose<VC>(u);
+    float sum = 0.0f, got = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VC; ++i) {
+        const int g = BACK ? VC - 1 - i : i;
+        got = __builtin_fmaf(decay_of(y[g]), got, u[g]);
+        sum += y[g];
+    }
+    spans[at.wave][at.lane] = make_float2(sum, got);
+    __syncthreads();
+    if (at.wave || !at.on) return;
+    const int64_t mine = (int64_t)at.b * a.channels + at.ch;
+    float v = 0.0f;
+    if (a.first && at.range == (BACK ? all - 1 : 0)) {
+        v = a.first[mine];
+        if constexpr (!BACK) a.kept[mine] = v;
+    }
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        const float2 p = spans[BACK ? kWaves - 1 - i : i][at.lane];
+        v = __builtin_fmaf(decay_of(p.x), v, p.y);
+        sum += p.x;
+    }
+    a.spans[((int64_t)at.b * all + at.range) * a.channels + at.ch] = make_float2(decay_of(sum), v);
+}
+
 // ---------------------------------------------------------------- forward
-// grid (slabs, ranges, sequences). SUMS: only the ranges' spans, for the next launch.
-template <class T, bool GATED, bool WIDE, bool SUMS>
+// grid (slabs, ranges, sequences)
+template <class T, bool GATED, bool WIDE>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
-    constexpr int VC = kVC<T>, TL = 4, WT = VC * TL, TILE = kWaves * WT;
-    static_assert(TILE % kChunk == 0 && kChunk % WT == 0, "chunks begin with a wave");
+    constexpr int VC = kVC<T>, TL = 16 / VC, WT = VC * TL, TILE = kWaves * WT;
+    static_assert(TILE == kChunk, "a tile begins at a kept state");
     __shared__ float2 spans[2][kWaves][64];
     const Place<T> at(a);
     const Span s = span_of(a, at.b);
     const int64_t begin = at.range * a.range_len;
-    const int64_t end = !SUMS && at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
-    float h = 0.0f, whole = 1.0f;
+    const int64_t end = at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
+    float h = 0.0f;
     const int64_t mine = (int64_t)at.b * a.channels + at.near;
     if (at.range == 0) {
-        if (a.first) h = a.ranges > 1 && !SUMS ? a.kept[mine] : a.first[mine];
-        if (SUMS && a.first && at.wave == 0 && at.on) a.kept[mine] = h;
-    } else if (!SUMS) {
-        h = through(a.spans + (int64_t)at.b * a.ranges * a.channels + at.near, a.channels, at.range, 0.0f);
+        if (a.first) h = a.ranges > 1 ? a.kept[mine] : a.first[mine];
+    } else {
+        h = through(a.spans + (int64_t)at.b * a.ranges * a.fine * a.channels + at.near, a.channels, at.range * a.fine, at.wave, at.lane, spans[0]);
     }
     float rate[VC];
 #pragma unroll
@@ -347,29 +469,23 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
             const float2 p = spans[slot][w][at.lane];
             if (w == at.wave) before = h;
             h = __builtin_fmaf(p.x, h, p.y);
-            if constexpr (SUMS) whole *= p.x;
         }
-        if constexpr (!SUMS) {
-            if (at.wave * WT % kChunk == 0) {
-                const int64_t token = t0 + at.wave * WT;
-                const auto kept = __builtin_amdgcn_make_buffer_rsrc(a.states + (s.state + token / kChunk) * a.channels, 0,
-                                                                    a.states && token < end ? a.channels * 4 : 0, 0x00020000);
-                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, before), kept, 4 * at.ch, 0, 0);
-            }
+        const auto kept = __builtin_amdgcn_make_buffer_rsrc(a.states + (s.state + t0 / kChunk) * a.channels, 0,
+                                                            a.states && at.wave == 0 ? a.channels * 4 : 0, 0x00020000);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, before), kept, 4 * at.ch, 0, 0);
 #pragma unroll
-            for (int i = 0; i < VC; ++i) {
-                const float x = before;
-                before = __builtin_fmaf(y[i], before, u[i]);
-                u[i] = x;
-            }
-            transpose<VC>(u);
-            const auto h = hs.buffer(t0, end, TILE);
+        for (int i = 0; i < VC; ++i) {
+            const float x = before;
+            before = __builtin_fmaf(y[i], before, u[i]);
+            u[i] = x;
+        }
+        transpose<VC>(u);
+        const auto h = hs.buffer(t0, end, TILE);
 #pragma unroll
-            for (int k = 0; k < TL; ++k) {
+        for (int k = 0; k < TL; ++k) {
 #pragma unroll
-                for (int j = 0; j < VC; ++j) u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j]);
-                hs.store(h, k, pack<T>(u));
-            }
+            for (int j = 0; j < VC; ++j) u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j]);
+            hs.store(h, k, pack<T>(u));
         }
     };
     if (begin < end) {
@@ -380,30 +496,29 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
             if (t0 + TILE < end) tile(two, one, t0 + TILE, 1);
         }
     }
-    if (at.wave || !at.on) return;
-    if constexpr (SUMS) a.spans[((int64_t)at.b * a.ranges + at.range) * a.channels + at.ch] = make_float2(whole, h);
-    else if (at.range == a.ranges - 1 && a.last) a.last[mine] = h;
+    if (at.wave == 0 && at.on && at.range == a.ranges - 1 && a.last) a.last[mine] = h;
 }
 
 // ---------------------------------------------------------------- backward
 // The tiles from the last to the first, kChunk tokens each: the state before a tile is the forward's, the cotangent behind
-// it is carried. SUMS: only the ranges' spans (a and dh alone).
-template <class T, bool GATED, bool WIDE, bool SUMS>
+// it is carried.
+template <class T, bool GATED, bool WIDE>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     constexpr int VC = kVC<T>, TL = 16 / VC, WT = VC * TL, TILE = kWaves * WT;
     static_assert(TILE == kChunk, "a tile begins at a kept state");
     __shared__ float2 spans[2][kWaves][64];
     __shared__ float backs[2][kWaves][64];
-    const Place<T> at(a, SUMS);  // nothing is before the first range
+    const Place<T> at(a);
     const Span s = span_of(a, at.b);
     const int64_t begin = at.range * a.range_len;
     const int64_t end = at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
-    float m = 0.0f, whole = 1.0f;  // the cotangent behind the tile, times its decay
+    float m = 0.0f;  // the cotangent behind the tile, times its decay
     const int64_t mine = (int64_t)at.b * a.channels + at.near;
     if (at.range == a.ranges - 1) {
         if (a.first) m = a.first[mine];
-    } else if (!SUMS) {  // the last range's span holds what is behind it
-        m = through(a.spans + ((int64_t)at.b * a.ranges + a.ranges - 1) * a.channels + at.near, -(int64_t)a.channels, a.ranges - 1 - at.range, 0.0f);
+    } else {  // the last range's span holds what is behind it
+        m = through(a.spans + ((int64_t)(at.b + 1) * a.ranges * a.fine - 1) * a.channels + at.near, -(int64_t)a.channels,
+                    (a.ranges - 1 - at.range) * a.fine, at.wave, at.lane, spans[0]);
     }
     float rate[VC], dr[VC];
 #pragma unroll
@@ -424,12 +539,10 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
         for (int k = 0; k < TL; ++k) {
             r.g[k] = gs.load(g, k);
             r.e[k] = es.load(e, k);
-            if constexpr (!SUMS) {
-                r.x[k] = xs.load(x, k);
-                if constexpr (GATED) r.i[k] = is.load(i, k);
-            }
+            r.x[k] = xs.load(x, k);
+            if constexpr (GATED) r.i[k] = is.load(i, k);
         }
-        if constexpr (!SUMS) r.h = a.states[(s.state + t0 / kChunk) * a.channels + at.near];
+        r.h = a.states[(s.state + t0 / kChunk) * a.channels + at.near];
     };
     auto tile = [&](Raw& now, Raw& next, int64_t t0, int slot) {
         fetch(next, t0 - TILE);
@@ -454,32 +567,30 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
                 const float e = rate[j] * sg[k][j];
                 dec[k][j] = exp2_(-e);
                 y[j] += e;
-                if constexpr (!SUMS) {
-                    const float q = room(e, dec[k][j]);
-                    // where nothing decays the root's derivative counts as none
-                    const float inv = q >= 0x1p-126f ? __builtin_amdgcn_rsqf(q) : q * 0.0f;
-                    in[k][j] = q * inv;
-                    near[k][j] = dec[k][j] * inv;
-                    if constexpr (GATED) {
-                        si[k][j] = sigmoid<T>(value<T>(now.i[k], j));
-                        in[k][j] *= si[k][j];
-                        near[k][j] *= si[k][j];
-                    }
-                    u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j] * value<T>(now.x[k], j));
+                const float q = room(e, dec[k][j]);
+                // where nothing decays the root's derivative counts as none
+                const float inv = q >= 0x1p-126f ? __builtin_amdgcn_rsqf(q) : q * 0.0f;
+                in[k][j] = q * inv;
+                near[k][j] = dec[k][j] * inv;
+                if constexpr (GATED) {
+                    si[k][j] = sigmoid<T>(value<T>(now.i[k], j));
+                    in[k][j] *= si[k][j];
+                    near[k][j] *= si[k][j];
                 }
+                u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j] * value<T>(now.x[k], j));
             }
 #pragma unroll
             for (int k = TL - 1; k >= 0; --k) v[j] = dec[k][j] * (v[j] + value<T>(now.e[k], j));
         }
         transpose<VC>(y);
-        if constexpr (!SUMS) transpose<VC>(u);
+        transpose<VC>(u);
         transpose<VC>(v);
         float sum = 0.0f, got = 0.0f, back = 0.0f;
 #pragma unroll
         for (int i = 0; i < VC; ++i) {
             sum += y[i];
             y[i] = exp2_(-y[i]);
-            if constexpr (!SUMS) got = __builtin_fmaf(y[i], got, u[i]);
+            got = __builtin_fmaf(y[i], got, u[i]);
         }
 #pragma unroll
         for (int i = VC - 1; i >= 0; --i) back = __builtin_fmaf(y[i], back, v[i]);
@@ -491,76 +602,67 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             p[w] = spans[slot][w][at.lane];
-            if constexpr (!SUMS) {
-                if (w == at.wave) before = h;
-                h = __builtin_fmaf(p[w].x, h, p[w].y);
-            }
+            if (w == at.wave) before = h;
+            h = __builtin_fmaf(p[w].x, h, p[w].y);
         }
 #pragma unroll
         for (int w = kWaves - 1; w >= 0; --w) {
             if (w == at.wave) behind = m;
             m = __builtin_fmaf(p[w].x, m, backs[slot][w][at.lane]);
-            if constexpr (SUMS) whole *= p[w].x;
         }
-        if constexpr (!SUMS) {
-            // the inputs are taken apart again: both forms would not fit the registers
+        // the inputs are taken apart again: both forms would not fit the registers
 #pragma unroll
-            for (int k = 0; k < TL; ++k) asm volatile("" : "+v"(now.x[k]), "+v"(now.e[k]));
+        for (int k = 0; k < TL; ++k) asm volatile("" : "+v"(now.x[k]), "+v"(now.e[k]));
 #pragma unroll
-            for (int i = 0; i < VC; ++i) {
-                const float x = before;
-                before = __builtin_fmaf(y[i], before, u[i]);
-                u[i] = x;
+        for (int i = 0; i < VC; ++i) {
+            const float x = before;
+            before = __builtin_fmaf(y[i], before, u[i]);
+            u[i] = x;
+        }
+#pragma unroll
+        for (int i = VC - 1; i >= 0; --i) {
+            const float x = behind;
+            behind = __builtin_fmaf(y[i], behind, v[i]);
+            v[i] = x;
+        }
+        transpose<VC>(u);
+        transpose<VC>(v);
+        const auto bx = dxs.buffer(t0, end, TILE), bg = dgs.buffer(t0, end, TILE), bi = dis.buffer(t0, end, TILE);
+        // each token's state before it
+        float was[TL][VC];
+#pragma unroll
+        for (int k = 0; k < TL; ++k)
+#pragma unroll
+            for (int j = 0; j < VC; ++j) {
+                was[k][j] = u[j];
+                u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j] * value<T>(now.x[k], j));
             }
 #pragma unroll
-            for (int i = VC - 1; i >= 0; --i) {
-                const float x = behind;
-                behind = __builtin_fmaf(y[i], behind, v[i]);
-                v[i] = x;
-            }
-            transpose<VC>(u);
-            transpose<VC>(v);
-            const auto bx = dxs.buffer(t0, end, TILE), bg = dgs.buffer(t0, end, TILE), bi = dis.buffer(t0, end, TILE);
-            // each token's state before it
-            float was[TL][VC];
+        for (int k = TL - 1; k >= 0; --k) {
+            float dx[VC], dg[VC], di[VC];
 #pragma unroll
-            for (int k = 0; k < TL; ++k)
-#pragma unroll
-                for (int j = 0; j < VC; ++j) {
-                    was[k][j] = u[j];
-                    u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j] * value<T>(now.x[k], j));
-                }
-#pragma unroll
-            for (int k = TL - 1; k >= 0; --k) {
-                float dx[VC], dg[VC], di[VC];
-#pragma unroll
-                for (int j = 0; j < VC; ++j) {
-                    const float l = value<T>(now.e[k], j) + v[j], x = value<T>(now.x[k], j);
-                    v[j] = dec[k][j] * l;
-                    const float d = sg[k][j] * (v[j] * __builtin_fmaf(-near[k][j], x, was[k][j]));
-                    dr[j] -= d;
-                    dg[j] = -kLn2 * rate[j] * __builtin_fmaf(-sg[k][j], d, d);
-                    dx[j] = l * in[k][j];
-                    if constexpr (GATED) di[j] = dx[j] * __builtin_fmaf(-x, si[k][j], x);
-                        }
-                dxs.store(bx, k, pack<T>(dx));
-                dgs.store(bg, k, pack<T>(dg));
-                if constexpr (GATED) dis.store(bi, k, pack<T>(di));
-            }
+            for (int j = 0; j < VC; ++j) {
+                const float l = value<T>(now.e[k], j) + v[j], x = value<T>(now.x[k], j);
+                v[j] = dec[k][j] * l;
+                const float d = sg[k][j] * (v[j] * __builtin_fmaf(-near[k][j], x, was[k][j]));
+                dr[j] -= d;
+                dg[j] = -kLn2 * rate[j] * __builtin_fmaf(-sg[k][j], d, d);
+                dx[j] = l * in[k][j];
+                if constexpr (GATED) di[j] = dx[j] * __builtin_fmaf(-x, si[k][j], x);
+                    }
+            dxs.store(bx, k, pack<T>(dx));
+            dgs.store(bg, k, pack<T>(dg));
+            if constexpr (GATED) dis.store(bi, k, pack<T>(di));
         }
     };
     if (begin < end) {
-        Raw one, two;
         int64_t t0 = begin + (end - 1 - begin) / TILE * TILE;
+        Raw one, two;
         fetch(one, t0);
         for (; t0 >= begin; t0 -= 2 * TILE) {
             tile(one, two, t0, 0);
             if (t0 - TILE >= begin) tile(two, one, t0 - TILE, 1);
         }
-    }
-    if constexpr (SUMS) {
-        if (at.wave == 0 && at.on) a.spans[((int64_t)at.b * a.ranges + at.range) * a.channels + at.ch] = make_float2(whole, m);
-        return;
     }
     if (at.wave == 0 && at.on && at.range == 0 && a.last) a.last[mine] = m;
     // the rate's gradient: a lane's groups, then the waves, in order
@@ -578,16 +680,188 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     a.drate[((int64_t)at.b * a.ranges + at.range) * a.channels + at.ch] = sum;
 }
 
-// the rows of the rate's partial gradients added in order, 64 channels and 4 shares of the rows a workgroup
-__global__ __launch_bounds__(256) void recurrence_rate_kernel(const float* part, float* out, int64_t rows, int32_t channels) {
-    __shared__ float sums[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6;
+// The rows of the rate's partial gradients added in a fixed order: 64 channels a workgroup, 16 shares of the rows.
+constexpr int kShares = 16;
+__global__ __launch_bounds__(64 * kShares) void recurrence_rate_kernel(const float* part, float* out, int64_t rows, int32_t channels) {
+    __shared__ float sums[kShares][64];
+    const int lane = threadIdx.x & 63, share = threadIdx.x >> 6, c = blockIdx.x * 64 + lane, near = c < channels ? c : channels - 1;
     float sum = 0.0f;
-    if (c < channels)
-        for (int64_t r = share; r < rows; r += 4) sum += part[r * channels + c];
-    sums[share][threadIdx.x & 63] = sum;
+    for (int64_t r = share; r < rows; r += 4 * kShares) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = part[(r + i * kShares < rows ? r + i * kShares : r) * channels + near];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += r + i * kShares < rows ? x[i] : 0.0f;
+    }
+    sums[share][lane] = sum;
     __syncthreads();
-    if (share == 0 && c < channels) out[c] = sums[0][threadIdx.x] + sums[1][threadIdx.x] + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+    if (share || c >= channels) return;
+#pragma unroll
+    for (int i = 1; i < kShares; ++i) sum += sums[i][lane];
+    out[c] = sum;
+}
+
+// ---------------------------------------------------------------- a few tokens
+// A thread takes a sequence's V channels from token to token: no joins. grid (channels, sequences).
+constexpr int kFewThreads = 64, kFew = 8;  // tokens that the backward holds at once
+template <class T, int V>
+struct Few {
+    T x[V];
+    __device__ __forceinline__ float operator[](int j) const {
+        if constexpr (sizeof(T) == 4) return x[j];
+        else return bf16_to_f32(x[j]);
+    }
+};
+template <class T, int V>
+__device__ __forceinline__ Few<T, V> few_load(const Rows& t, int64_t base, int64_t token, int c0) {
+    return *reinterpret_cast<const Few<T, V>*>(__builtin_assume_aligned(reinterpret_cast<const T*>(t.p) + base + token * t.ts + c0, V * sizeof(T)));
+}
+template <class T, int V>
+__device__ __forceinline__ void few_store(const Rows& t, int64_t base, int64_t token, int c0, const float (&v)[V]) {
+    Few<T, V> o;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if constexpr (sizeof(T) == 4) o.x[j] = v[j];
+        else o.x[j] = __builtin_bit_cast(uint16_t, (__bf16)v[j]);
+    }
+    *reinterpret_cast<Few<T, V>*>(__builtin_assume_aligned(reinterpret_cast<T*>(t.p) + base + token * t.ts + c0, V * sizeof(T))) = o;
+}
+__device__ __forceinline__ int64_t base_of(const Rows& t, const Args& a, const Span& s, int b) { return a.starts ? s.base * t.ts : b * t.bs; }
+
+template <class T, int V, bool GATED>
+__global__ __launch_bounds__(kFewThreads) void recurrence_few_fwd_kernel(Args a) {
+    const int c0 = (blockIdx.x * kFewThreads + threadIdx.x) * V, b = blockIdx.y;
+    if (c0 >= a.channels) return;
+    const Span s = span_of(a, b);
+    const int64_t xb = base_of(a.x, a, s, b), gb = base_of(a.g, a, s, b), ib = base_of(a.i, a, s, b), hb = base_of(a.h, a, s, b);
+    const int64_t mine = (int64_t)b * a.channels + c0;
+    float rate[V], h[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        rate[j] = a.rate[c0 + j] * kLog2e;
+        h[j] = a.first ? a.first[mine + j] : 0.0f;
+    }
+    constexpr int TL = 4;
+    for (int64_t t0 = 0; t0 < s.len; t0 += TL) {
+        Few<T, V> x[TL], g[TL], i[TL];
+#pragma unroll
+        for (int k = 0; k < TL; ++k) {
+            const int64_t t = t0 + k < s.len ? t0 + k : s.len - 1;
+            x[k] = few_load<T, V>(a.x, xb, t, c0);
+            g[k] = few_load<T, V>(a.g, gb, t, c0);
+            if constexpr (GATED) i[k] = few_load<T, V>(a.i, ib, t, c0);
+        }
+        if (a.states && t0 % kChunk == 0)
+#pragma unroll
+            for (int j = 0; j < V; ++j) a.states[(s.state + t0 / kChunk) * a.channels + c0 + j] = h[j];
+#pragma unroll
+        for (int k = 0; k < TL; ++k) {
+            if (t0 + k >= s.len) break;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float e = rate[j] * sigmoid<T>(g[k][j]), dec = exp2_(-e);
+                float w = x[k][j];
+                if constexpr (GATED) w *= sigmoid<T>(i[k][j]);
+                h[j] = __builtin_fmaf(dec, h[j], __builtin_amdgcn_sqrtf(room(e, dec)) * w);
+            }
+            few_store<T, V>(a.h, hb, t0 + k, c0, h);
+        }
+    }
+    if (a.last)
+#pragma unroll
+        for (int j = 0; j < V; ++j) a.last[mine + j] = h[j];
+}
+
+// kFew tokens at a time from the last, the states before them from the kept one on
+template <class T, int V, bool GATED>
+__global__ __launch_bounds__(kFewThreads) void recurrence_few_bwd_kernel(Args a) {
+    const int c0 = (blockIdx.x * kFewThreads + threadIdx.x) * V, b = blockIdx.y;
+    if (c0 >= a.channels) return;
+    const Span s = span_of(a, b);
+    const int64_t xb = base_of(a.x, a, s, b), gb = base_of(a.g, a, s, b), ib = base_of(a.i, a, s, b), eb = base_of(a.h, a, s, b);
+    const int64_t dxb = base_of(a.dx, a, s, b), dgb = base_of(a.dg, a, s, b), dib = base_of(a.di, a, s, b);
+    const int64_t mine = (int64_t)b * a.channels + c0;
+    float rate[V], m[V], dr[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        rate[j] = a.rate[c0 + j] * kLog2e;
+        m[j] = a.first ? a.first[mine + j] : 0.0f;
+        dr[j] = 0.0f;
+    }
+    for (int64_t t1 = s.len; t1 > 0; t1 = (t1 - 1) / kFew * kFew) {
+        const int64_t t0 = (t1 - 1) / kFew * kFew;
+        const int n = (int)(t1 - t0);
+        Few<T, V> x[kFew], g[kFew], i[kFew], e[kFew];
+        float h[V], was[kFew][V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) h[j] = a.states[(s.state + t0 / kChunk) * a.channels + c0 + j];
+#pragma unroll
+        for (int k = 0; k < kFew; ++k) {
+            const int64_t t = t0 + (k < n ? k : n - 1);
+            x[k] = few_load<T, V>(a.x, xb, t, c0);
+            g[k] = few_load<T, V>(a.g, gb, t, c0);
+            if constexpr (GATED) i[k] = few_load<T, V>(a.i, ib, t, c0);
+            e[k] = few_load<T, V>(a.h, eb, t, c0);
+        }
+        auto enter = [&](const Few<T, V>& xs, const Few<T, V>& gs, const Few<T, V>& is, int j, float& dec) {
+            const float y = rate[j] * sigmoid<T>(gs[j]);
+            dec = exp2_(-y);
+            float w = xs[j];
+            if constexpr (GATED) w *= sigmoid<T>(is[j]);
+            return __builtin_amdgcn_sqrtf(room(y, dec)) * w;
+        };
+        for (int64_t t = t0 / kChunk * kChunk; t < t0; ++t) {
+            const Few<T, V> xs = few_load<T, V>(a.x, xb, t, c0), gs = few_load<T, V>(a.g, gb, t, c0);
+            Few<T, V> is = {};
+            if constexpr (GATED) is = few_load<T, V>(a.i, ib, t, c0);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float dec;
+                const float in = enter(xs, gs, is, j, dec);
+                h[j] = __builtin_fmaf(dec, h[j], in);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kFew; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                was[k][j] = h[j];
+                float dec;
+                const float in = enter(x[k], g[k], i[k], j, dec);
+                h[j] = __builtin_fmaf(dec, h[j], in);
+            }
+#pragma unroll
+        for (int k = kFew - 1; k >= 0; --k) {
+            if (k >= n) continue;
+            float dx[V], dg[V], di[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float sg = sigmoid<T>(g[k][j]), y = rate[j] * sg, dec = exp2_(-y), q = room(y, dec);
+                const float inv = q >= 0x1p-126f ? __builtin_amdgcn_rsqf(q) : q * 0.0f, xv = x[k][j];
+                float in = q * inv, near = dec * inv, si = 1.0f;
+                if constexpr (GATED) {
+                    si = sigmoid<T>(i[k][j]);
+                    in *= si;
+                    near *= si;
+                }
+                const float l = e[k][j] + m[j];
+                m[j] = dec * l;
+                const float d = sg * (m[j] * __builtin_fmaf(-near, xv, was[k][j]));
+                dr[j] -= d;
+                dg[j] = -kLn2 * rate[j] * __builtin_fmaf(-sg, d, d);
+                dx[j] = l * in;
+                if constexpr (GATED) di[j] = dx[j] * __builtin_fmaf(-xv, si, xv);
+            }
+            few_store<T, V>(a.dx, dxb, t0 + k, c0, dx);
+            few_store<T, V>(a.dg, dgb, t0 + k, c0, dg);
+            if constexpr (GATED) few_store<T, V>(a.di, dib, t0 + k, c0, di);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (a.last) a.last[mine + j] = m[j];
+        a.drate[mine + j] = dr[j];
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -642,22 +916,32 @@ bool wide(const R97qRows* t, const R97qRecurrence* p) {
 
 int64_t all_tokens(const R97qRecurrence* p) { return p->starts ? p->tokens : p->batch * p->len; }
 
-// ranges of the tokens, multiples of a forward tile
+// ranges of the tokens, multiples of a tile
+#ifndef FINE
+#define FINE 4
+#endif
+#ifndef MINR
+#define MINR 256
+#endif
+#ifndef FEWV
+#define FEWV 8
+#endif
 void cut(const R97qRecurrence* p, Args& a) {
     const int64_t slabs = (p->channels + kSlab - 1) / kSlab, have = slabs * p->batch;
     const int64_t mean = p->batch ? all_tokens(p) / p->batch : 0;
-#ifndef WANT
-#define WANT 256
-#endif
-    int64_t n = have > 0 ? WANT / have : 1;
-    if (n > mean / 512) n = mean / 512;
+    a.few = p->len <= FEWV && mean <= FEWV;
+    int64_t n = have > 0 ? 256 / have : 1;
+    if (n > mean / MINR) n = mean / MINR;
     if (n > 64) n = 64;
     if (n < 1) n = 1;
     const int64_t len = p->starts && p->len < mean ? mean : p->len;
-    a.range_len = ((len + n - 1) / n + 255) / 256 * 256;
-    if (a.range_len < 256) a.range_len = 256;
+    a.range_len = ((len + n - 1) / n + kChunk - 1) / kChunk * kChunk;
+    if (a.range_len < kChunk) a.range_len = kChunk;
     a.ranges = (int32_t)((len + a.range_len - 1) / a.range_len);
     if (a.ranges < 1) a.ranges = 1;
+    a.fine = FINE;
+    while (a.fine > 1 && (a.ranges * a.fine * have > 1024 || a.range_len / a.fine < 128)) a.fine /= 2;
+    a.span_len = (a.range_len + a.fine - 1) / a.fine;
 }
 
 Args args_of(const R97qRecurrence* p) {
@@ -670,31 +954,42 @@ Args args_of(const R97qRecurrence* p) {
     cut(p, a);
     return a;
 }
-int64_t spans_bytes(const Args& a) { return a.ranges > 1 ? (8LL * a.batch * a.ranges * a.channels + 255) / 256 * 256 : 0; }
+int64_t spans_bytes(const Args& a) { return a.ranges > 1 ? (8LL * a.batch * a.ranges * a.fine * a.channels + 255) / 256 * 256 : 0; }
 int64_t row_bytes(const Args& a, int64_t rows) { return (4 * rows * a.channels + 255) / 256 * 256; }
 
 template <class T, bool GATED, bool WIDE>
 int run_fwd(const Args& a, hipStream_t st) {
     const unsigned slabs = (unsigned)((a.channels + kSlab - 1) / kSlab);
     if (a.ranges > 1) {
-        hipLaunchKernelGGL((recurrence_fwd_kernel<T, GATED, WIDE, true>), dim3(slabs, a.ranges - 1, a.batch), dim3(kThreads), 0, st, a);
-        if (int e = launch_status("recurrence_fwd_kernel")) return e;
+        hipLaunchKernelGGL((recurrence_spans_kernel<T, GATED, WIDE, false>), dim3(slabs, (a.ranges - 1) * a.fine, a.batch), dim3(kThreads), 0, st, a);
+        if (int e = launch_status("recurrence_spans_kernel")) return e;
     }
-    hipLaunchKernelGGL((recurrence_fwd_kernel<T, GATED, WIDE, false>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((recurrence_fwd_kernel<T, GATED, WIDE>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
     return launch_status("recurrence_fwd_kernel");
 }
 template <class T, bool GATED, bool WIDE>
 int run_bwd(const Args& a, hipStream_t st) {
     const unsigned slabs = (unsigned)((a.channels + kSlab - 1) / kSlab);
     if (a.ranges > 1) {
-        hipLaunchKernelGGL((recurrence_bwd_kernel<T, GATED, WIDE, true>), dim3(slabs, a.ranges - 1, a.batch), dim3(kThreads), 0, st, a);
-        if (int e = launch_status("recurrence_bwd_kernel")) return e;
+        hipLaunchKernelGGL((recurrence_spans_kernel<T, false, WIDE, true>), dim3(slabs, (a.ranges - 1) * a.fine, a.batch), dim3(kThreads), 0, st, a);
+        if (int e = launch_status("recurrence_spans_kernel")) return e;
     }
-    hipLaunchKernelGGL((recurrence_bwd_kernel<T, GATED, WIDE, false>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((recurrence_bwd_kernel<T, GATED, WIDE>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
     return launch_status("recurrence_bwd_kernel");
+}
+template <class T, int V, bool GATED>
+int run_few(const Args& a, bool back, hipStream_t st) {
+    const dim3 grid((unsigned)((a.channels + V * kFewThreads - 1) / (V * kFewThreads)), (unsigned)a.batch);
+    if (back) hipLaunchKernelGGL((recurrence_few_bwd_kernel<T, V, GATED>), grid, dim3(kFewThreads), 0, st, a);
+    else hipLaunchKernelGGL((recurrence_few_fwd_kernel<T, V, GATED>), grid, dim3(kFewThreads), 0, st, a);
+    return launch_status("recurrence_few_kernel");
 }
 template <class T>
 int pick(const Args& a, bool back, bool wide, hipStream_t st) {
+    if (a.few) {
+        if (a.i.p) return wide ? run_few<T, 4, true>(a, back, st) : run_few<T, 1, true>(a, back, st);
+        return wide ? run_few<T, 4, false>(a, back, st) : run_few<T, 1, false>(a, back, st);
+    }
     if (a.i.p) {
         if (wide) return back ? run_bwd<T, true, true>(a, st) : run_fwd<T, true, true>(a, st);
         return back ? run_bwd<T, true, false>(a, st) : run_fwd<T, true, false>(a, st);
@@ -806,7 +1101,7 @@ int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     if (rows > 0)
         if (int e = shape->dtype == R97Q_F32 ? pick<float>(a, true, w, st) : pick<uint16_t>(a, true, w, st)) return e;
     if (rows == 1) return R97Q_OK;
-    hipLaunchKernelGGL(recurrence_rate_kernel, dim3((unsigned)((a.channels + 63) / 64)), dim3(256), 0, st, a.drate, drate, rows, a.channels);
+    hipLaunchKernelGGL(recurrence_rate_kernel, dim3((unsigned)((a.channels + 63) / 64)), dim3(64 * kShares), 0, st, a.drate, drate, rows, a.channels);
     return launch_status("recurrence_rate_kernel");
 }
 
