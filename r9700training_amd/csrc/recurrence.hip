@@ -53,9 +53,9 @@ struct Args {
     const int32_t* starts;
     int64_t tokens, len;
     int32_t batch, channels;
-    int32_t ranges, fine;         // and a range's spans
-    int64_t range_len, span_len;
-    float2* spans;                // [batch][ranges * fine][channels]
+    int32_t ranges;
+    int64_t range_len;
+    float2* spans;                // [batch][ranges][channels], the ranges' spans
     float* kept;                  // [batch][channels]: `first`, where `last` may be written over it
     int32_t few;                  // a thread a sequence
     float* drate;                 // [batch * ranges][channels], or the sum itself where that is one row
@@ -299,7 +299,7 @@ __device__ __forceinline__ void blank(u32x4& x, u32x4& g, u32x4& i, bool out) {
 }
 
 // ---------------------------------------------------------------- the ranges' spans
-// grid (slabs, all but one range's spans, sequences): what a part of a range makes of the state before it, or (BACK, from a and dh alone) of the
+// grid (slabs, all but one range, sequences): what a range makes of the state before it, or (BACK, from a and dh alone) of the
 // cotangent behind it. Nothing is needed of the tokens between, so a lane's group takes a run of tokens of its own, with no
 // join but one at the end. The span that has the given end (the first, or BACK the last) holds it; the forward
 // also keeps a copy of it, since `last` may be written over it before every workgroup of the next launch has read it.
@@ -307,11 +307,10 @@ template <class T, bool GATED, bool WIDE, bool BACK>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
     constexpr int VC = kVC<T>, TL = 4;
     __shared__ float2 spans[kWaves][64];
-    const Place<T> at(a, BACK ? a.fine : 0);
+    const Place<T> at(a, BACK);
     const Span s = span_of(a, at.b);
-    const int all = a.ranges * a.fine;
-    const int64_t begin = at.range * a.span_len;
-    const int64_t end = BACK && at.range == all - 1 ? s.len : clamp64(begin + a.span_len, 0, s.len);
+    const int64_t begin = at.range * a.range_len;
+    const int64_t end = BACK && at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
     const int64_t run = (end - begin + kWaves * VC - 1) / (kWaves * VC), from = begin + (at.wave * VC + at.g) * run;
     float rate[VC], y[VC], u[VC];
 #pragma unroll
@@ -378,7 +377,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
     if (at.wave || !at.on) return;
     const int64_t mine = (int64_t)at.b * a.channels + at.ch;
     float v = 0.0f;
-    if (a.first && at.range == (BACK ? all - 1 : 0)) {
+    if (a.first && at.range == (BACK ? a.ranges - 1 : 0)) {
         v = a.first[mine];
         if constexpr (!BACK) a.kept[mine] = v;
     }
@@ -389,7 +388,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
         v = __builtin_fmaf(decay_of(p.x), v, p.y);
         sum += p.x;
     }
-    a.spans[((int64_t)at.b * all + at.range) * a.channels + at.ch] = make_float2(decay_of(sum), v);
+    a.spans[((int64_t)at.b * a.ranges + at.range) * a.channels + at.ch] = make_float2(decay_of(sum), v);
 }
 
 // ---------------------------------------------------------------- forward
@@ -408,7 +407,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
     if (at.range == 0) {
         if (a.first) h = a.ranges > 1 ? a.kept[mine] : a.first[mine];
     } else {
-        h = through(a.spans + (int64_t)at.b * a.ranges * a.fine * a.channels + at.near, a.channels, at.range * a.fine, at.wave, at.lane, spans[0]);
+        h = through(a.spans + (int64_t)at.b * a.ranges * a.channels + at.near, a.channels, at.range, at.wave, at.lane, spans[0]);
     }
     float rate[VC];
 #pragma unroll
@@ -517,8 +516,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     if (at.range == a.ranges - 1) {
         if (a.first) m = a.first[mine];
     } else {  // the last range's span holds what is behind it
-        m = through(a.spans + ((int64_t)(at.b + 1) * a.ranges * a.fine - 1) * a.channels + at.near, -(int64_t)a.channels,
-                    (a.ranges - 1 - at.range) * a.fine, at.wave, at.lane, spans[0]);
+        m = through(a.spans + ((int64_t)(at.b + 1) * a.ranges - 1) * a.channels + at.near, -(int64_t)a.channels, a.ranges - 1 - at.range,
+                    at.wave, at.lane, spans[0]);
     }
     float rate[VC], dr[VC];
 #pragma unroll
@@ -916,52 +915,44 @@ bool wide(const R97qRows* t, const R97qRecurrence* p) {
 
 int64_t all_tokens(const R97qRecurrence* p) { return p->starts ? p->tokens : p->batch * p->len; }
 
-// ranges of the tokens, multiples of a tile
-#ifndef FINE
-#define FINE 4
-#endif
-#ifndef MINR
-#define MINR 256
-#endif
-#ifndef FEWV
-#define FEWV 8
-#endif
-void cut(const R97qRecurrence* p, Args& a) {
+// How a call is cut. Measured, us forward / backward, bf16 with a gate on the input:
+// A thread a sequence, against tiles: 32 sequences of 4096 channels, 16 tokens 9 / 19 against 36 / 58, 32 tokens 15 / 46 against 36
+// / 58, 64 tokens 27 forward; 4 of 1024, 16 tokens 9 / 18 in both, 32 tokens 13 / 37 against 9 / 18. So up to 16 tokens, and
+// forward up to 64 where the tiles' workgroups fill the card several times over.
+// Ranges of at least 128 tokens, as many as make 256 workgroups (a compute unit holds one), against none: 1 x 512 x 1024 15 / 22
+// against 14 / 22, 4 x 600 x 512 17 / 22 against 17 / 29, 1 x 768 x 512 16 / 21 against 19 / 31, 1 x 1024 x 2048 17 / 21 against 25 /
+// 41, 1 x 16384 x 1024 53 / 64 against 345 / 584. 8 x 2048 x 2048, 256 workgroups whole, forward 67; two ranges 100.
+void cut(const R97qRecurrence* p, bool back, Args& a) {
     const int64_t slabs = (p->channels + kSlab - 1) / kSlab, have = slabs * p->batch;
-    const int64_t mean = p->batch ? all_tokens(p) / p->batch : 0;
-    a.few = p->len <= FEWV && mean <= FEWV;
-    int64_t n = have > 0 ? 256 / have : 1;
-    if (n > mean / MINR) n = mean / MINR;
-    if (n > 64) n = 64;
+    const int64_t mean = p->batch ? all_tokens(p) / p->batch : 0, most = p->len > mean ? p->len : mean;
+    a.few = most <= 16 || (!back && most <= 64 && have >= 1024);
+    int64_t n = have > 0 && mean >= (back ? 512 : 640) ? 256 / have : 1;
+    if (n > mean / 128) n = mean / 128;
     if (n < 1) n = 1;
-    const int64_t len = p->starts && p->len < mean ? mean : p->len;
-    a.range_len = ((len + n - 1) / n + kChunk - 1) / kChunk * kChunk;
+    a.range_len = ((most + n - 1) / n + kChunk - 1) / kChunk * kChunk;
     if (a.range_len < kChunk) a.range_len = kChunk;
-    a.ranges = (int32_t)((len + a.range_len - 1) / a.range_len);
+    a.ranges = (int32_t)((most + a.range_len - 1) / a.range_len);
     if (a.ranges < 1) a.ranges = 1;
-    a.fine = FINE;
-    while (a.fine > 1 && (a.ranges * a.fine * have > 1024 || a.range_len / a.fine < 128)) a.fine /= 2;
-    a.span_len = (a.range_len + a.fine - 1) / a.fine;
 }
 
-Args args_of(const R97qRecurrence* p) {
+Args args_of(const R97qRecurrence* p, bool back) {
     Args a = {};
     a.starts = p->starts;
     a.tokens = p->tokens;
     a.len = p->len;
     a.batch = p->batch;
     a.channels = p->channels;
-    cut(p, a);
+    cut(p, back, a);
     return a;
 }
-int64_t spans_bytes(const Args& a) { return a.ranges > 1 ? (8LL * a.batch * a.ranges * a.fine * a.channels + 255) / 256 * 256 : 0; }
+int64_t spans_bytes(const Args& a) { return a.ranges > 1 ? (8LL * a.batch * a.ranges * a.channels + 255) / 256 * 256 : 0; }
 int64_t row_bytes(const Args& a, int64_t rows) { return (4 * rows * a.channels + 255) / 256 * 256; }
 
 template <class T, bool GATED, bool WIDE>
 int run_fwd(const Args& a, hipStream_t st) {
     const unsigned slabs = (unsigned)((a.channels + kSlab - 1) / kSlab);
     if (a.ranges > 1) {
-        hipLaunchKernelGGL((recurrence_spans_kernel<T, GATED, WIDE, false>), dim3(slabs, (a.ranges - 1) * a.fine, a.batch), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL((recurrence_spans_kernel<T, GATED, WIDE, false>), dim3(slabs, a.ranges - 1, a.batch), dim3(kThreads), 0, st, a);
         if (int e = launch_status("recurrence_spans_kernel")) return e;
     }
     hipLaunchKernelGGL((recurrence_fwd_kernel<T, GATED, WIDE>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
@@ -971,7 +962,7 @@ template <class T, bool GATED, bool WIDE>
 int run_bwd(const Args& a, hipStream_t st) {
     const unsigned slabs = (unsigned)((a.channels + kSlab - 1) / kSlab);
     if (a.ranges > 1) {
-        hipLaunchKernelGGL((recurrence_spans_kernel<T, false, WIDE, true>), dim3(slabs, (a.ranges - 1) * a.fine, a.batch), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL((recurrence_spans_kernel<T, false, WIDE, true>), dim3(slabs, a.ranges - 1, a.batch), dim3(kThreads), 0, st, a);
         if (int e = launch_status("recurrence_spans_kernel")) return e;
     }
     hipLaunchKernelGGL((recurrence_bwd_kernel<T, GATED, WIDE>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
@@ -1016,7 +1007,7 @@ int64_t r97q_recurrence_state_rows(const R97qRecurrence* shape) {
 int64_t r97q_recurrence_fwd_workspace_bytes(const R97qRecurrence* shape) {
     clear_error();
     if (check_shape(shape, "r97q_recurrence_fwd_workspace_bytes")) return -1;
-    const Args a = args_of(shape);
+    const Args a = args_of(shape, false);
     return a.ranges > 1 ? spans_bytes(a) + row_bytes(a, a.batch) : 0;
 }
 
@@ -1033,7 +1024,7 @@ int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     if (int e = check_rows(h, shape, true, who, "h")) return e;
     if (!rate) return refuse(R97Q_EINVAL, who, "null rate");
     if (shape->batch == 0) return R97Q_OK;
-    Args a = args_of(shape);
+    Args a = args_of(shape, false);
     const int64_t need = a.ranges > 1 ? spans_bytes(a) + row_bytes(a, a.batch) : 0;
     if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
     if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
@@ -1054,7 +1045,7 @@ int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R9
 int64_t r97q_recurrence_bwd_workspace_bytes(const R97qRecurrence* shape) {
     clear_error();
     if (check_shape(shape, "r97q_recurrence_bwd_workspace_bytes")) return -1;
-    const Args a = args_of(shape);
+    const Args a = args_of(shape, true);
     const int64_t rows = (int64_t)a.batch * a.ranges;
     return spans_bytes(a) + (rows > 1 ? row_bytes(a, rows) : 0);
 }
@@ -1078,7 +1069,7 @@ int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     if (int e = check_rows(dgate, shape, true, who, "dgate")) return e;
     if (!rate || !drate) return refuse(R97Q_EINVAL, who, "null rate or drate");
     if (!states && shape->batch > 0 && all_tokens(shape) > 0) return refuse(R97Q_EINVAL, who, "null states");
-    Args a = args_of(shape);
+    Args a = args_of(shape, true);
     hipStream_t st = (hipStream_t)stream;
     const int64_t rows = (int64_t)a.batch * a.ranges, need = spans_bytes(a) + (rows > 1 ? row_bytes(a, rows) : 0);
     if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
