@@ -377,51 +377,6 @@ struct Rows {
     }
 };
 
-// The same of a sequence's tokens in pages. A wave holds 64 entries of the sequence's row of the table, a lane's each, and the
-// next 64 on their way: tiles begin at multiples of their size, so a tile's pages are of one such block. An entry outside the
-// pool reads as zeros, like a token past the end.
-struct PageRows {
-    uint64_t base, page;  // the head in page 0; bytes from page to page
-    const int32_t* table; // the sequence's row
-    uint32_t ts, tail;
-    uint32_t pos;         // the next tile's first token
-    int from, end;        // tokens to read
-    int shift, pages, max_pages;
-    uint32_t block;
-    int ent, next;        // the lane's entries of the block and of the one after it
-    __device__ __forceinline__ PageRows(const Args& a, const Seq& s, const Heads& t, int h, int row0, int from_, int rows, int d)
-        : base(reinterpret_cast<uint64_t>(t.data) + 2 * h * t.hs), page(2 * t.bs), table(a.table + s.b * a.table_stride),
-          ts((uint32_t)(2 * t.ts)), tail(2 * d), pos(row0), from(from_), end(rows), shift(a.page_shift), pages(a.pages),
-          max_pages(a.max_pages) {
-        block = pos >> shift >> 6;
-        ent = fetch(block);
-        next = fetch(block + 1);
-    }
-    __device__ __forceinline__ int fetch(uint32_t b) const {
-        const uint32_t i = 64 * b + (threadIdx.x & 63);
-        return i < (uint32_t)max_pages ? table[i] : -1;
-    }
-    __device__ __forceinline__ int size() const { return 1 << shift; }
-    __device__ __forceinline__ void step(int tokens) { pos += tokens; }
-    __device__ __forceinline__ void turn() {
-        const uint32_t b = pos >> shift >> 6;
-        if (b == block) return;
-        block = b;
-        ent = next;
-        next = fetch(b + 1);
-    }
-    // R tokens from the tile's token `first` on, at the tile's offsets
-    template <int R>
-    __device__ __forceinline__ u32x4 buffer(int first) const {
-        const uint32_t at = pos + first;
-        const int e = __builtin_amdgcn_readlane(ent, (int)(at >> shift) & 63), left = end - (int)at;
-        const uint64_t p = base + (uint64_t)(uint32_t)e * page + (int64_t)((int)(at & (size() - 1)) - first) * ts;
-        const uint32_t n = (uint32_t)(first + (left < R ? left : R) - 1) * ts + tail;
-        return (u32x4){(uint32_t)uniform((int)p), (uint32_t)uniform((int)(p >> 32)), (uint32_t)uniform((uint32_t)e < (uint32_t)pages && left > 0 ? (int)n : 0),
-                       0x00020000u};
-    }
-};
-
 // the LDS address of a pointer into LDS
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
     return (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p);
@@ -441,6 +396,87 @@ template <int N = 0>
 __device__ __forceinline__ void landed() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+
+// The same of a sequence's tokens in pages. A wave holds 64 entries of the sequence's row of the table, a lane's each: tiles
+// begin at multiples of their size, so a tile's pages are of one such block. The next 64 wait in LDS, loaded like the tiles
+// (an ordinary load on its way through the loop would have every step wait for all that it has asked for). An entry outside
+// the pool reads as zeros, like a token past the end. The keys' walk leads, and loads the entries for the values' too, which is at most
+// two tiles behind: less than a block.
+constexpr int kTableBytes = 2 * 64 * 4;  // of LDS, a wave
+struct PageTable {
+    u32x4 row;             // the sequence's row of the table
+    uint32_t area, pos;    // the wave's LDS; the next tile's first token
+    int from, end;         // tokens to read
+    int shift, pages;
+    bool leads;
+    uint32_t block;
+    int ent;               // the lane's entry of the block
+    __device__ __forceinline__ PageTable(const Args& a, const Seq& s, int row0, int from_, int rows, uint32_t lds, bool leads_)
+        : area(lds), pos(row0), from(from_), end(rows), shift(a.page_shift), pages(a.pages), leads(leads_) {
+        const uint64_t p = reinterpret_cast<uint64_t>(a.table + s.b * a.table_stride);
+        row = (u32x4){(uint32_t)uniform((int)p), (uint32_t)uniform((int)(p >> 32)), (uint32_t)uniform(4 * a.max_pages), 0x00020000u};
+        block = pos >> shift >> 6;
+        if (leads) {
+            fetch(block);
+            fetch(block + 1);
+            landed();
+        }
+        take();
+    }
+    __device__ __forceinline__ void fetch(uint32_t b) const { load_words(row, 256 * b + 4 * (threadIdx.x & 63), area + 256 * (b & 1)); }
+    __device__ __forceinline__ void take() {
+        ent = *(__attribute__((address_space(3))) const volatile int*)(uintptr_t)(area + 256 * (block & 1) + 4 * (threadIdx.x & 63));
+    }
+    __device__ __forceinline__ int size() const { return 1 << shift; }
+    __device__ __forceinline__ void step(int tokens) { pos += tokens; }
+    __device__ __forceinline__ bool turn() {
+        const uint32_t b = pos >> shift >> 6;
+        if (b == block) return false;
+        block = b;
+        take();
+        if (leads) fetch(b + 1);
+        return true;
+    }
+    __device__ __forceinline__ uint32_t entry(uint32_t at) const { return __builtin_amdgcn_readlane(ent, (int)(at >> shift) & 63); }
+};
+// How a pool's pages are reached: one buffer with a page's offset in it, where the pool is less than 2 GiB, a tile's page looked
+// up once (kWholePages: they hold a tile) or a wave's piece at a time (kSmallPages: of a tile's first one on); else a piece's
+// page as a buffer of its own (kFarPages). What a step does for it counts, since no product runs beside it: 2048 tokens over
+// 16384, 16 over 4 heads of 128, 287 us over rows, 300 over pages of 64, 320 of 16; with every piece's page and bounds worked
+// out in scalars 374, and with the next entries an ordinary load 415.
+enum { kWholePages, kSmallPages, kFarPages };
+constexpr uint32_t kNearBytes = 0x7FFFFFF0u;  // a near pool's end at most: an offset for entries outside the pool
+template <int MODE>
+struct PageRows : PageTable {
+    u32x4 pool;            // near: the pool from the head on
+    uint64_t base, page;   // the head in page 0; bytes from page to page
+    uint32_t ts, tail;
+    __device__ __forceinline__ PageRows(const Args& a, const Seq& s, const Heads& t, int h, int row0, int from_, int rows, int d, uint32_t lds, bool leads_)
+        : PageTable(a, s, row0, from_, rows, lds, leads_), base(reinterpret_cast<uint64_t>(t.data) + 2 * h * t.hs), page(2 * t.bs), ts((uint32_t)(2 * t.ts)),
+          tail(2 * d) {
+        if constexpr (MODE != kFarPages) {
+            const uint32_t n = pages > 0 ? (uint32_t)(pages - 1) * (uint32_t)page + (uint32_t)(size() - 1) * ts + tail : 0u;
+            pool = (u32x4){(uint32_t)uniform((int)base), (uint32_t)uniform((int)(base >> 32)), (uint32_t)uniform((int)n), 0x00020000u};
+            place();
+        }
+    }
+    // near: the entry as an offset
+    __device__ __forceinline__ void place() { ent = (uint32_t)ent < (uint32_t)pages ? (int)((uint32_t)ent * (uint32_t)page) : (int)kNearBytes; }
+    __device__ __forceinline__ void turn() {
+        if (!PageTable::turn()) return;
+        if constexpr (MODE != kFarPages) place();
+    }
+    // the buffer of the tile's tokens first .. first + R - 1, in one page, at the tile's offsets
+    template <int R>
+    __device__ __forceinline__ u32x4 buffer(int first) const {
+        const uint32_t at = pos + first, e = entry(at);
+        const int left = end - (int)at;
+        const uint64_t p = base + (uint64_t)e * page + (int64_t)((int)(at & (size() - 1)) - first) * ts;
+        const uint32_t n = (uint32_t)(first + (left < R ? left : R) - 1) * ts + tail;
+        return (u32x4){(uint32_t)uniform((int)p), (uint32_t)uniform((int)(p >> 32)), (uint32_t)uniform(e < (uint32_t)pages && left > 0 ? (int)n : 0),
+                       0x00020000u};
+    }
+};
 
 // ROWS rows from memory into a tile, by THREADS threads: a piece's place in LDS is its thread's, so the swizzle
 // is in which chunk of the row a thread loads.
@@ -462,23 +498,47 @@ struct Loader {
 #pragma unroll
         for (int i = 0; i < N; ++i) load_piece(b, off[i], dst + 16 * THREADS * i);
     }
-    // The same from pages; w0: the wave's first thread. A tile that lies in one page is one buffer. Of smaller pages a wave's
-    // piece, 8 tokens or fewer, lies in one: it is that page's buffer, put back by the tokens before the piece, so that the
-    // offsets are the tile's.
-    __device__ __forceinline__ void load(PageRows& r, int w0, uint32_t dst) const {
+    // The same from pages; w0: the wave's first thread. FIRST: the tile may hold tokens that no query sees.
+    template <bool FIRST, int MODE>
+    __device__ __forceinline__ void load_pages(PageRows<MODE>& r, int w0, uint32_t dst) const {
         r.turn();
-        const int skip = r.from - (int)r.pos;  // tokens that no query sees
-        u32x4 b = {};
-        if (r.size() >= ROWS) b = r.template buffer<ROWS>(0);
+        if constexpr (MODE == kFarPages) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int first = (w0 + THREADS * i) / CH;
-            if (r.size() < ROWS) b = r.template buffer<64 / CH>(first);
-            uint32_t o = off[i];
-            if (skip > 0) o = (w0 + (int)(threadIdx.x & 63) + THREADS * i) / CH < skip ? kNowhere : o;
-            load_piece(b, o, dst + 16 * THREADS * i);
+            for (int i = 0; i < N; ++i) {
+                const u32x4 b = r.template buffer<64 / CH>((w0 + THREADS * i) / CH);
+                load_piece(b, FIRST && row_of(i, w0) < r.from - (int)r.pos ? kNowhere : off[i], dst + 16 * THREADS * i);
+            }
+            return;
+        }
+        const int left = r.end - (int)r.pos;
+        if constexpr (MODE == kWholePages) {
+            const uint32_t e = r.entry(r.pos), add = e == kNearBytes ? e : e + (r.pos & (r.size() - 1)) * r.ts;
+            const uint32_t last = add + (uint32_t)(left - 1) * r.ts + r.tail;
+            u32x4 b = r.pool;
+            b[2] = (uint32_t)uniform((int)(left >= ROWS || (left > 0 && last >= b[2]) ? b[2] : left > 0 ? last : 0u));
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                load_piece(b, FIRST && row_of(i, w0) < r.from - (int)r.pos ? kNowhere : off[i] + add, dst + 16 * THREADS * i);
+            return;
+        }
+        uint32_t add[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {  // the piece's page, and back from the tile's beginning, which is a page's, to that page's
+            const int page = ((w0 + THREADS * i) / CH) >> r.shift;
+            add[i] = r.entry(r.pos + (page << r.shift)) - (uint32_t)(page << r.shift) * r.ts;
+        }
+        if (!FIRST && left >= ROWS) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) load_piece(r.pool, off[i] + add[i], dst + 16 * THREADS * i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int row = row_of(i, w0);
+                load_piece(r.pool, row < r.from - (int)r.pos || row >= left ? kNowhere : off[i] + add[i], dst + 16 * THREADS * i);
+            }
         }
     }
+    __device__ __forceinline__ static int row_of(int i, int w0) { return (w0 + (int)(threadIdx.x & 63) + THREADS * i) / CH; }
 };
 
 // A row's values as B operands: 16 c + 8 h .. + 8 of the head, zeros past d and for rows outside. `row` is a row that may

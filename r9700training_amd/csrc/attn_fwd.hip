@@ -7,7 +7,7 @@
 // probability the same relative precision at any size). The probabilities are rounded to bf16 for the second
 // product (the matrix cores' input type; off by at most 2^-8 relative), their sum is of the unrounded values in f32.
 //
-// Built twice: over keys in rows (R97Q_PAGED 0), and over a paged cache (1), where only the tiles' loads differ.
+// Built twice: over keys in rows (R97Q_PAGED 0), and over a paged cache (1), where only the tiles' loads differ (PageRows).
 #include "attn.h"
 #include "status.h"
 
@@ -22,23 +22,21 @@ namespace {
 
 constexpr bool kPaged = R97Q_PAGED;
 // the keys or values [lo, hi) of a sequence's key head, in tiles from `row0` on
-template <bool PAGED>
-struct Source;
+template <int MODE>
+struct Source : PageRows<MODE> {
+    __device__ __forceinline__ Source(const Args& a, const Seq& s, const Heads& t, int hk, int row0, int lo, int hi, uint32_t lds, bool leads)
+        : PageRows<MODE>(a, s, t, hk, row0, lo, hi, a.d, lds, leads) {}
+    template <bool FIRST, class L>
+    __device__ __forceinline__ void load(const L& l, int w0, uint32_t dst) { l.template load_pages<FIRST>(*this, w0, dst); }
+};
+constexpr int kNoPages = -1;
 template <>
-struct Source<false> : Rows {
-    __device__ __forceinline__ Source(const Args& a, const Seq& s, const Heads& t, int hk, int row0, int lo, int hi)
+struct Source<kNoPages> : Rows {
+    __device__ __forceinline__ Source(const Args& a, const Seq& s, const Heads& t, int hk, int row0, int lo, int hi, uint32_t, bool)
         : Rows(kv_at(t, a, s, hk), 2 * t.ts, row0, hi, a.d) {}
+    template <bool FIRST, class L>
+    __device__ __forceinline__ void load(const L& l, int, uint32_t dst) { l.load(*this, dst); }
 };
-template <>
-struct Source<true> : PageRows {
-    __device__ __forceinline__ Source(const Args& a, const Seq& s, const Heads& t, int hk, int row0, int lo, int hi)
-        : PageRows(a, s, t, hk, row0, lo, hi, a.d) {}
-};
-using Keyed = Source<kPaged>;
-template <class L>
-__device__ __forceinline__ void load_tile(const L& l, Rows& r, int, uint32_t dst) { l.load(r, dst); }
-template <class L>
-__device__ __forceinline__ void load_tile(const L& l, PageRows& r, int w0, uint32_t dst) { l.load(r, w0, dst); }
 // where the tiles begin: at the first key that is seen, or in pages at the tile that holds it
 template <int KT>
 __device__ __forceinline__ int tile_start(int lo) { return kPaged ? lo / KT * KT : lo; }
@@ -196,12 +194,13 @@ __device__ __forceinline__ void finish(const Args& a, const Seq& s, const Row& r
 // and queries fill its registers and one wave a SIMD remains: 33% and 20%): 302 .. 312 us, 880 .. 910 TFLOP/s; 16 over 4 heads
 // of 256 350 .. 390 us, 705 .. 785; of 64 94 .. 100 us, 690 .. 730 (32% and 45%, 11 vector instructions a product). Two waves
 // that share 32 rows and halve their keys were 6 .. 10% faster on grids of under 256 workgroups only, and are not built.
-template <int D, int KT, int NW, int PER>
+template <int D, int KT, int NW, int PER, int MODE>
 __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     using T = Tile<D>;
     using F = Frags<D>;
     constexpr int TB = KT * T::RB, SUBS = KT / 32, n = D / 16;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB];  // keys' two slots, then the values'
+    // keys' two slots, then the values', then the waves' entries of the page table
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB + (MODE == kNoPages ? 0 : NW * kTableBytes)];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
     const int nb = a.batch * a.hk;
     const Place place(nb, a.together);
@@ -212,7 +211,7 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
     const float sl = score_scale(a);
     const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
     const Loader<D, KT, 64 * NW> kl(kts, a.d, tid), vl(vts, a.d, tid);
-    const uint32_t at = lds_at(lds), mine = at + 1024 * wave, rat = at + F::row0(lane), cat = at + 2 * TB + F::col0(lane);
+    const uint32_t at = lds_at(lds), mine = at + 1024 * wave, area = at + 4 * TB + kTableBytes * wave, rat = at + F::row0(lane), cat = at + 2 * TB + F::col0(lane);
     // the last tiles first: under a causal mask they have the most keys
     for (int64_t tile = tiles - 1 - part / a.splits; tile * 32 * NW < rows; tile += tiles) {
         const int w0 = (int)tile * 32 * NW, r0 = w0 + 32 * wave;
@@ -227,19 +226,19 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
             lo = (int)clamp64((int64_t)lo + (int64_t)split * a.chunk, lo, hi);
             if (split < a.splits - 1 && hi - lo > a.chunk) hi = lo + a.chunk;  // the last range takes what is left
         }
-        Keyed kr(a, s, a.k, hk, lo, all.lo, hi), vr(a, s, a.v, hk, lo, all.lo, hi);
-        auto load_k = [&](int slot) {
-            load_tile(kl, kr, 64 * wave, mine + slot * TB);
+        Source<MODE> kr(a, s, a.k, hk, lo, all.lo, hi, area, true), vr(a, s, a.v, hk, lo, all.lo, hi, area, false);
+        auto load_k = [&](int slot, auto first) {
+            kr.template load<first>(kl, 64 * wave, mine + slot * TB);
             kr.step(KT);
         };
-        auto load_v = [&](int slot) {
-            load_tile(vl, vr, 64 * wave, mine + (2 + slot) * TB);
+        auto load_v = [&](int slot, auto first) {
+            vr.template load<first>(vl, 64 * wave, mine + (2 + slot) * TB);
             vr.step(KT);
         };
         if (lo < hi) {
-            load_k(0);
-            load_k(1);
-            load_v(0);
+            load_k(0, std::true_type{});
+            load_k(1, std::false_type{});
+            load_v(0, std::true_type{});
         }
         bf16x8 q[n];
         load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
@@ -273,12 +272,12 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
                 if (j > 0) {  // the first tiles' loads are the ones above
                     landed();
                     __syncthreads();
-                    load_k(slot);
-                    load_v(1 - slot);
+                    load_k(slot, std::false_type{});
+                    load_v(1 - slot, std::false_type{});
                 } else {
                     __syncthreads();
-                    load_k(slot);
-                    load_v(1 - slot);
+                    load_k(slot, std::false_type{});
+                    load_v(1 - slot, std::false_type{});
                 }
                 if (j >= n0 && j < n1) {
                     const int j0 = lo + j * KT;
@@ -346,11 +345,11 @@ __global__ __launch_bounds__(64 * NW, PER) void attn_fwd_kernel(Args a) {
 // are loaded when the scores are done, the next values when the product is. The NW waves' sums meet in LDS.
 // Bound by memory, 2 * D * 2 bytes a key: one token, 24 over 4 heads of 256, 32768 keys 28.5 us (4.7 TB/s); 16 tokens, 32
 // over 8 heads of 128, caches of 1 .. 4096 keys 29.4 us (5.4 TB/s).
-template <int D, int NW>
+template <int D, int NW, int MODE>
 __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
     using T = Tile<D>;
     constexpr int KT = 32, TB = KT * T::RB;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[NW * 2 * TB];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[NW * 2 * TB + (MODE == kNoPages ? 0 : NW * kTableBytes)];
     __shared__ float2 ml[NW][32];
     static_assert(2 * TB >= 32 * D * 4, "a wave's tiles hold its sums");
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), col = lane & 31, h = lane >> 5;
@@ -361,7 +360,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
     const int64_t kts = 2 * a.k.ts, vts = 2 * a.v.ts;
     const Loader<D, KT, 64> kl(kts, a.d, lane), vl(vts, a.d, lane);
     uint8_t* own = lds + wave * 2 * TB;
-    const uint32_t at = lds_at(own);
+    const uint32_t at = lds_at(own), area = lds_at(lds) + NW * 2 * TB + kTableBytes * wave;
     for (int64_t tile = blockIdx.z; tile * 32 < rows; tile += gridDim.z) {
         const int r0 = (int)tile * 32;
         const Row row(a, hk, r0 + col, rows);
@@ -382,9 +381,9 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
         const int last = a.causal && row.tok + s.off < s.lk - 1 ? row.tok + s.off : s.lk - 1;
         int j0 = lo + KT * wave;
         if (j0 < hi) {
-            Keyed kr(a, s, a.k, hk, j0, keys.lo, hi), vr(a, s, a.v, hk, j0, keys.lo, hi);
-            load_tile(kl, kr, 0, at);
-            load_tile(vl, vr, 0, at + TB);
+            Source<MODE> kr(a, s, a.k, hk, j0, keys.lo, hi, area, true), vr(a, s, a.v, hk, j0, keys.lo, hi, area, false);
+            kr.template load<true>(kl, 0, at);
+            vr.template load<true>(vl, 0, at + TB);
             bf16x8 q[D / 16];
             load_row<D>(q_at(a.q, a, s, row.head) + 2 * (row.tok * a.q.ts), row.on, fresh(a.d), lane, q);
             turn_sign<D>(a, q);
@@ -396,14 +395,14 @@ __global__ __launch_bounds__(64 * NW, 1) void attn_few_kernel(Args a) {
                 // the keys are in registers: their tile is free
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 kr.step(NW * KT);
-                load_tile(kl, kr, 0, at);
+                kr.template load<false>(kl, 0, at);
                 if (j0 < keys.all_lo || j0 + KT > keys.all_hi) mask<KT>(x, first - j0, last - j0, h);
                 run.rise(tile_max<KT>(x) * sl);
                 landed<Loader<D, KT, 64>::N>();  // the values; the next keys may be on their way
                 absorb<D, KT>(own + TB, x, sl, lane, run);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 vr.step(NW * KT);
-                load_tile(vl, vr, 0, at + TB);
+                vr.template load<false>(vl, 0, at + TB);
                 landed<Loader<D, KT, 64>::N>();
             }
             landed();
@@ -584,17 +583,37 @@ Plan plan_of(const Args& a) {
     return p;
 }
 
-template <int D, int KT, int NW, int PER>
-int run_tiles(const Args& a, const Plan& p, hipStream_t st) {
-    const int64_t nb = (int64_t)a.batch * a.hk * p.splits, most = most_groups(64 * NW) / nb;
-    const int64_t tiles = p.tiles < most ? p.tiles : most;
-    hipLaunchKernelGGL((attn_fwd_kernel<D, KT, NW, PER>), dim3((unsigned)(tiles * nb)), dim3(64 * NW), 0, st, a);
-    return launch_status("attn_fwd_kernel");
+// how a tile of `rows` keys finds its pages
+int mode_of(const Args& a, int rows) {
+    if (!kPaged) return kNoPages;
+    auto near = [&](const Heads& t) { return 2.0 * ((double)(a.pages > 0 ? a.pages - 1 : 0) * t.bs + (double)((1 << a.page_shift) - 1) * t.ts + a.d) <= (double)kNearBytes; };
+    return !near(a.k) || !near(a.v) ? kFarPages : 1 << a.page_shift >= rows ? kWholePages : kSmallPages;
 }
-template <int D, int NW>
+template <int D, int KT, int NW, int PER, int MODE>
+int run_tiles(const Args& a, const Plan& p, hipStream_t st) {
+    if constexpr (kPaged && MODE == kNoPages) {
+        const int mode = mode_of(a, KT);
+        return mode == kWholePages   ? run_tiles<D, KT, NW, PER, kWholePages>(a, p, st)
+               : mode == kSmallPages ? run_tiles<D, KT, NW, PER, kSmallPages>(a, p, st)
+                                     : run_tiles<D, KT, NW, PER, kFarPages>(a, p, st);
+    } else {
+        const int64_t nb = (int64_t)a.batch * a.hk * p.splits, most = most_groups(64 * NW) / nb;
+        const int64_t tiles = p.tiles < most ? p.tiles : most;
+        hipLaunchKernelGGL((attn_fwd_kernel<D, KT, NW, PER, MODE>), dim3((unsigned)(tiles * nb)), dim3(64 * NW), 0, st, a);
+        return launch_status("attn_fwd_kernel");
+    }
+}
+template <int D, int NW, int MODE>
 int run_few(const Args& a, const Plan& p, hipStream_t st) {
-    hipLaunchKernelGGL((attn_few_kernel<D, NW>), dim3((unsigned)(a.batch * a.hk), p.splits, (unsigned)p.tiles), dim3(64 * NW), 0, st, a);
-    return launch_status("attn_few_kernel");
+    if constexpr (kPaged && MODE == kNoPages) {
+        const int mode = mode_of(a, 32);
+        return mode == kWholePages   ? run_few<D, NW, kWholePages>(a, p, st)
+               : mode == kSmallPages ? run_few<D, NW, kSmallPages>(a, p, st)
+                                     : run_few<D, NW, kFarPages>(a, p, st);
+    } else {
+        hipLaunchKernelGGL((attn_few_kernel<D, NW, MODE>), dim3((unsigned)(a.batch * a.hk), p.splits, (unsigned)p.tiles), dim3(64 * NW), 0, st, a);
+        return launch_status("attn_few_kernel");
+    }
 }
 
 }  // namespace
@@ -620,11 +639,11 @@ int launch_fwd(Args a, void* workspace, hipStream_t st) {
     a.stats = reinterpret_cast<float2*>(a.part + (p.splits > 1 ? p.splits * a.slots * a.d : 0));
     int e;
     if (p.few)
-        e = a.d <= 64 ? run_few<64, 4>(a, p, st) : a.d <= 128 ? run_few<128, 4>(a, p, st) : run_few<256, 4>(a, p, st);
+        e = a.d <= 64 ? run_few<64, 4, kNoPages>(a, p, st) : a.d <= 128 ? run_few<128, 4, kNoPages>(a, p, st) : run_few<256, 4, kNoPages>(a, p, st);
     else
-        e = a.d <= 64    ? run_tiles<64, 64, 4, 2>(a, p, st)
-            : a.d <= 128 ? run_tiles<128, 64, 4, 2>(a, p, st)
-                         : run_tiles<256, 32, 4, 1>(a, p, st);
+        e = a.d <= 64    ? run_tiles<64, 64, 4, 2, kNoPages>(a, p, st)
+            : a.d <= 128 ? run_tiles<128, 64, 4, 2, kNoPages>(a, p, st)
+                         : run_tiles<256, 32, 4, 1, kNoPages>(a, p, st);
     return e || p.splits == 1 ? e : launch_join(a, st);
 }
 

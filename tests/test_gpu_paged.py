@@ -159,6 +159,27 @@ def test_packed(new, lens, hq, hk, d, page, window):
             assert (out[part] == 7).all() and (lse[:, part] == 7).all()
 
 
+@pytest.mark.parametrize("new,d,page", [(1, 128, 8), (100, 128, 8), (1, 64, 16), (200, 256, 16), (100, 80, 256), (1, 80, 256), (3, 200, 64),
+                                        (90, 200, 128), (90, 40, 32)])
+def test_entries_outside_the_pool_read_as_zeros(new, d, page):
+    """Also where a head has fewer columns than its tile: what lies elsewhere in the pool is NaN."""
+    from r9700training_amd.paged import paged_attention_fwd
+
+    lens = [5 * page + 3, 7 * page]
+    c = Cache(lens, 2, d, page)
+    for b, j, e in [(0, 1, -1), (0, 2, c.k.shape[0]), (1, 0, 2 ** 31 - 1), (1, 5, -(1 << 31)), (1, 6, 1 << 30)]:
+        c.table[b, j] = e
+        c.keys[b][j * page:(j + 1) * page] = 0
+        c.values[b][j * page:(j + 1) * page] = 0
+    q = rnd(1, 2, new, 4, d)
+    for window in (0, 3 * page):
+        ref = expected(c, q, 4, 2, True, window, 0.1, R.HALF[BF])
+        out, lse = paged_attention_fwd(q, c.k, c.v, c.table, c.kv_lens, scale=0.1, window=window)
+        for b, r in enumerate(ref):
+            close(out[b], *r["out"], f"out of sequence {b}")
+            close(lse[b], *r["lse"], f"lse of sequence {b}")
+
+
 @pytest.mark.parametrize("new,d", [(1, 128), (100, 128), (1, 64), (200, 256)])
 def test_entries_outside_the_pool(new, d):
     """They read as zeros, wherever they stand; lengths past the table are the table's."""
@@ -203,12 +224,13 @@ def test_shared_pages(new, d):
         close(out[b], *r["out"], f"out of sequence {b}")
 
 
+@pytest.mark.parametrize("page,d", [(64, 128), (8, 64), (256, 256), (16, 128)])
 @pytest.mark.parametrize("new", [1, 90])
-def test_far_pages(new):
+def test_far_pages(new, page, d):
     """A pool of more than 2^32 bytes and 2^31 values: pages at its end."""
     from r9700training_amd.paged import paged_attention_fwd, paged_write
 
-    page, heads, d, lens = 64, 8, 128, [130, 64]
+    heads, lens = 8, [130, 700]
     pages = 2 ** 31 // (page * heads * d) + 8
     c = Cache(lens, heads, d, page)
     k, v = (torch.empty((pages, page, heads, d), dtype=BF, device="cuda") for _ in range(2))
