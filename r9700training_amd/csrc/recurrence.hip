@@ -875,8 +875,8 @@ int check_shape(const R97qRecurrence* p, const char* who) {
     if (p->starts && p->tokens < 0) return refuse(R97Q_EINVAL, who, "a negative count of packed tokens");
     if (p->dtype != R97Q_BF16 && p->dtype != R97Q_F32) return refuse(R97Q_EINVAL, who, "the type is bf16 or f32");
     if (p->batch > 65535) return refuse(R97Q_EUNSUPPORTED, who, "at most 65535 sequences");
-    // the launches' grids and a row's bytes stay below 2^31
-    if (p->channels > (1 << 28)) return refuse(R97Q_EUNSUPPORTED, who, "at most 2^28 channels");
+    // the launches' work items and a row's bytes stay below 2^32 and 2^31
+    if (p->channels > (1 << 27)) return refuse(R97Q_EUNSUPPORTED, who, "at most 2^27 channels");
     if (p->len > 0x7FFFFFFF || (p->starts && p->tokens > 0x7FFFFFFF)) return refuse(R97Q_EUNSUPPORTED, who, "tokens within 31 bits");
     return R97Q_OK;
 }
