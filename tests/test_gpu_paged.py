@@ -74,6 +74,11 @@ CASES = [
     ([1, 1], [1000, 513], 24, 4, 256, 32, True, 0),
     ([1] * 9, [3000, 1, 8, 16, 17, 900, 2048, 0, 65], 32, 8, 128, 16, True, 0),
     ([1], [20000], 24, 4, 256, 64, True, 0),
+    ([1] * 3, [12000, 0, 1], 4, 1, 64, 16, True, 0),      # one sequence takes nearly all workgroups
+    ([2] * 5, [6000, 5, 1300, 127, 129], 8, 2, 128, 64, True, 0),
+    ([1] * 4, [3000, 2500, 1, 700], 16, 2, 256, 8, True, 900),
+    ([1] * 64, [37 * i % 1900 for i in range(64)], 4, 1, 64, 16, True, 0),
+    ([1] * 65, [53 * i % 2500 for i in range(65)], 2, 1, 64, 32, True, 0),
     ([1, 1], [5000, 1700], 8, 2, 128, 8, True, 300),
     ([3, 3], [200, 2], 14, 2, 128, 16, True, 0),          # the second's first query has no key
     ([5], [4097], 6, 3, 80, 8, True, 33),
