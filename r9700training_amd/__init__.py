@@ -290,6 +290,18 @@ def _stream(stream=None):
     return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
 
 
+def _device(x, stream, who: str) -> int:
+    """The index of x's device, which has to be the one that the call's stream runs on: a kernel launched on another would
+    read memory that is not its device's."""
+    import torch
+
+    d = x.get_device()
+    if d < 0 or d != (torch.cuda.current_device() if stream is None else stream.device_index):
+        raise ValueError(f"{who}: the tensors are on the device that the stream runs on"
+                         + ("; they are not on a GPU" if d < 0 else f" (the current one, without a stream); they are on {d}"))
+    return d
+
+
 def _empty(shape, dtype, device, stream=None):
     """A tensor for a call's output or workspace, taken from the pool of the stream the call runs on."""
     import torch

@@ -12,33 +12,35 @@ import math
 
 import torch
 
-from . import AttnShape, Pages, _empty, _empty_like, _ptr, _space, _stream, check, lib
+from . import AttnShape, Pages, _device, _empty, _empty_like, _ptr, _space, _stream, check, lib
 from .attention import _check_lse, _heads, _index, _lse_shape
 
 
-def _cache(q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, max_kv):
+def _cache(q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, max_kv=None, causal=0, window=0, scale=1.0, stream=None):
     """(shape, pages) of a call whose new tokens are shaped like q."""
-    s, packed = AttnShape(), q_starts is not None
-    qs, ks, ts = q.shape, k_pages.shape, page_table.shape
+    packed = q_starts is not None
+    qs, ks, ts, st = q.shape, k_pages.shape, page_table.shape, page_table.stride()
     if len(qs) != (3 if packed else 4) or len(ks) != 4 or v_pages.shape != ks or qs[-1] != ks[-1]:
         raise ValueError("paged: new tokens are [batch, tokens, heads, head_dim], packed [tokens, heads, head_dim]; k_pages and "
                          "v_pages [pages, page_size, heads, head_dim]")
-    if page_table.dtype != torch.int32 or len(ts) != 2 or not page_table.is_cuda or (ts[1] > 1 and page_table.stride(1) != 1):
+    if page_table.dtype != torch.int32 or len(ts) != 2 or (ts[1] > 1 and st[1] != 1):
         raise ValueError("paged: page_table is an int32 [batch, most pages] device tensor, a row's entries consecutive")
-    s.batch, s.head_dim = ts[0], qs[-1]
-    s.kv_lens = _index(kv_lens, ts[0], "kv_lens").data_ptr()
+    device = _device(q, stream, "paged")
+    if k_pages.get_device() != device or v_pages.get_device() != device or page_table.get_device() != device or kv_lens.get_device() != device:
+        raise ValueError("paged: the pages, the table and the lengths are on the new tokens' device")
+    batch, starts, tokens = ts[0], None, 0
     if packed:
-        s.q_starts = _index(q_starts, ts[0] + 1, "q_starts").data_ptr()
+        starts = _index(q_starts, batch + 1, "q_starts").data_ptr()
         if max_q is None:
             raise ValueError("paged: packed tokens need max_q, the longest sequence's")
-        s.q_tokens, s.q_len = qs[0], int(max_q)
+        tokens, length = qs[0], int(max_q)
     else:
-        if qs[0] != ts[0]:
+        if qs[0] != batch:
             raise ValueError("paged: page_table has a row for each sequence")
-        s.q_len = qs[1]
-    s.kv_len = ts[1] * ks[1] if max_kv is None else int(max_kv)
-    s.scale = 1.0
-    return s, Pages(page_table.data_ptr(), page_table.stride(0), ks[0], ks[1], ts[1])
+        length = qs[1]
+    held = ts[1] * ks[1] if max_kv is None else int(max_kv)
+    return (AttnShape(batch, qs[-1], length, held, starts, None, tokens, 0, _index(kv_lens, batch, "kv_lens").data_ptr(), window, causal, scale),
+            Pages(page_table.data_ptr(), st[0], ks[0], ks[1], ts[1]))
 
 
 def paged_write(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None, max_q: int | None = None, stream=None):
@@ -47,7 +49,7 @@ def paged_write(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None, max_
     packed = q_starts is not None
     if v.shape != k.shape:
         raise ValueError("paged: v has k's shape")
-    s, p = _cache(k, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, None)
+    s, p = _cache(k, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, stream=stream)
     check(lib().r97q_paged_write(s, p, _heads(k, packed, "k"), _heads(v, packed, "v"), _heads(k_pages, False, "k_pages"),
                                  _heads(v_pages, False, "v_pages"), _stream(stream)), "r97q_paged_write")
 
@@ -60,10 +62,9 @@ def paged_attention_fwd(q, k_pages, v_pages, page_table, kv_lens, causal: bool =
     longest sequence's tokens where the program knows them (the call is planned for it), else what the table has room for.
     Packed tokens outside every sequence are not written."""
     packed = q_starts is not None
-    s, p = _cache(q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, max_kv)
-    s.causal, s.window = int(bool(causal)), int(window)
-    s.scale = 1.0 / math.sqrt(s.head_dim) if scale is None else float(scale)
     qs = q.shape
+    s, p = _cache(q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, max_kv, int(bool(causal)), int(window),
+                  1.0 / math.sqrt(max(qs[-1], 1)) if scale is None else float(scale), stream)
     if out is None:
         out = _empty_like(q, out_dtype, stream)
     ho = _heads(out, packed, "out", qs)

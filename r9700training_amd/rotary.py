@@ -8,7 +8,7 @@ import numpy as np
 import torch
 
 from . import (R97Q_BF16, R97Q_F32, R97Q_ROTARY_HALF, R97Q_ROTARY_INTERLEAVED, R97Q_ROTARY_LINEAR, R97Q_ROTARY_PLAIN,
-               R97Q_ROTARY_RAMP, Heads, _empty_like, _ptr, _stream, check, lib)
+               R97Q_ROTARY_RAMP, Heads, _device, _empty_like, _ptr, _stream, check, lib)
 
 PAIRS = {"half": R97Q_ROTARY_HALF, "interleaved": R97Q_ROTARY_INTERLEAVED}
 SCALINGS = {"plain": R97Q_ROTARY_PLAIN, "linear": R97Q_ROTARY_LINEAR, "ramp": R97Q_ROTARY_RAMP}
@@ -107,6 +107,10 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor,
                 q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, stream=None):
     """rotary with a position on each of several axes: positions int32 or int64 [axes, tokens], and pair i turns by
     positions[pair_axis[i]] * inv_freq[i] (pair_axis int32 [rot / 2]: rotary_pair_axes)."""
+    device = _device(q, stream, "rotary_axes")
+    if (k is not None and k.get_device() != device) or inv_freq.get_device() != device or positions.get_device() != device \
+            or pair_axis.get_device() != device:
+        raise ValueError("rotary_axes: k, inv_freq, positions and pair_axis are on q's device")
     q_out, k_out, tokens, dim, heads = _tensors(q, k, inv_freq, pairs, q_out, k_out, stream)
     if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 2 or positions.shape[1] != tokens \
             or (tokens > 1 and positions.stride(1) != 1) or not positions.is_cuda:

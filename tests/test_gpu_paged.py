@@ -391,3 +391,6 @@ def test_nothing_to_do():
     none = c.k[:0]
     out, lse = paged_attention_fwd(rnd(1, 2, 3, 4, 64), none, none, c.table, c.kv_lens, out_dtype=torch.float32)
     assert (out == 0).all()
+    # a table without an entry
+    out, lse = paged_attention_fwd(rnd(1, 2, 3, 4, 64), c.k, c.v, c.table[:, :0], c.kv_lens)
+    assert (out == 0).all() and (lse == -math.inf).all()
