@@ -83,8 +83,11 @@ __device__ __forceinline__ uint32_t fresh(uint32_t x) {
 constexpr uint32_t kNowhere = 0x80000000u;  // an offset past every buffer's end
 
 // ---------------------------------------------------------------- pieces of 16 bytes
+// A piece may lie anywhere: the memory takes loads and stores of every alignment, so rows of odd widths go by pieces too.
 template <class T>
 constexpr int kVC = 16 / (int)sizeof(T);
+template <class T>
+using Loose = u32x4 __attribute__((aligned(sizeof(T))));
 template <class T>
 __device__ __forceinline__ float value(const u32x4& v, int j) {
     if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, (uint32_t)v[j]);
@@ -114,9 +117,9 @@ template <class T>
 struct Io<T, true> {
     uint64_t base;
     uint32_t ts, row, off;  // bytes a token; of a row; the thread's first piece in a tile
-    __device__ __forceinline__ Io(const Rows& t, const Args& a, const Span& s, int b, int first, int c0)
+    __device__ __forceinline__ Io(const Rows& t, const Args& a, const Span& s, int b, int first, int c0, bool mine)
         : base(reinterpret_cast<uint64_t>(t.p) + (a.starts ? s.base * t.ts : b * t.bs) * sizeof(T)), ts((uint32_t)(t.ts * sizeof(T))),
-          row((uint32_t)(a.channels * sizeof(T))), off(c0 < a.channels ? first * ts + c0 * (uint32_t)sizeof(T) : kNowhere) {}
+          row((uint32_t)(a.channels * sizeof(T))), off(mine ? first * ts + c0 * (uint32_t)sizeof(T) : kNowhere) {}
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(int64_t t0, int64_t end, int rows) const {
         const int left = end - t0 < rows ? (int)(end - t0) : rows;
         return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base + t0 * ts), 0, left > 0 ? (int)((left - 1) * ts + row) : 0, 0x00020000);
@@ -134,7 +137,7 @@ struct Io<T, false> {
     T* base;
     int64_t ts;
     int first, c0, channels;
-    __device__ __forceinline__ Io(const Rows& t, const Args& a, const Span& s, int b, int first_, int c0_)
+    __device__ __forceinline__ Io(const Rows& t, const Args& a, const Span& s, int b, int first_, int c0_, bool)
         : base(reinterpret_cast<T*>(t.p) + (a.starts ? s.base * t.ts : b * t.bs)), ts(t.ts), first(first_), c0(c0_), channels(a.channels) {}
     __device__ __forceinline__ Tile buffer(int64_t t0, int64_t end, int rows) const {
         const int64_t left = end - t0 - first;
@@ -163,10 +166,10 @@ struct Piece {
     int64_t ts;
     int c0, channels;
     __device__ __forceinline__ Piece(const Rows& t, const Args& a, const Span& s, int b, int c0_)
-        : base(reinterpret_cast<const T*>(t.p) + (a.starts ? s.base * t.ts : b * t.bs)), ts(t.ts), c0(!WIDE || c0_ < a.channels ? c0_ : 0), channels(a.channels) {}
+        : base(reinterpret_cast<const T*>(t.p) + (a.starts ? s.base * t.ts : b * t.bs)), ts(t.ts), c0(c0_), channels(a.channels) {}
     __device__ __forceinline__ u32x4 load(int64_t token) const {
         const T* p = base + token * ts;
-        if constexpr (WIDE) return *reinterpret_cast<const u32x4*>(p + c0);
+        if constexpr (WIDE) return *reinterpret_cast<const Loose<T>*>(p + c0);
         T x[kVC<T>];
 #pragma unroll
         for (int j = 0; j < kVC<T>; ++j) x[j] = p[c0 + j < channels ? c0 + j : channels - 1];
@@ -245,18 +248,21 @@ __device__ __forceinline__ void transpose(float (&x)[VC]) {
 }
 
 // what a workgroup works on
-template <class T>
+template <class T, bool WIDE>
 struct Place {
     static constexpr int VC = kVC<T>, LPR = 64 / VC;
     int lane, wave, g, c0, ch, near, b, range;
-    bool on;  // the transposed lane's channel is one (near: one that may be read in any case)
+    bool mine;  // the lane's piece is one: its first channel c0. WIDE: the last one ends with the last channel, over its neighbour
+    bool on;    // the transposed lane's channel is one (near: one that may be read in any case)
     __device__ __forceinline__ Place(const Args& a, int range0 = 0) {
         lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         g = lane / LPR;
         c0 = blockIdx.x * kSlab + lane % LPR * VC;
+        mine = c0 < a.channels;
+        if (WIDE && c0 > a.channels - VC) c0 = a.channels - VC;
         ch = c0 + g;
-        on = ch < a.channels;
+        on = mine && ch < a.channels;
         near = on ? ch : a.channels - 1;
         range = range0 + blockIdx.y;
         b = blockIdx.z;
@@ -307,7 +313,7 @@ template <class T, bool GATED, bool WIDE, bool BACK>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
     constexpr int VC = kVC<T>, TL = 4;
     __shared__ float2 spans[kWaves][64];
-    const Place<T> at(a, BACK);
+    const Place<T, WIDE> at(a, BACK);
     const Span s = span_of(a, at.b);
     const int64_t begin = at.range * a.range_len;
     const int64_t end = BACK && at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
@@ -398,7 +404,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
     constexpr int VC = kVC<T>, TL = 16 / VC, WT = VC * TL, TILE = kWaves * WT;
     static_assert(TILE == kChunk, "a tile begins at a kept state");
     __shared__ float2 spans[2][kWaves][64];
-    const Place<T> at(a);
+    const Place<T, WIDE> at(a);
     const Span s = span_of(a, at.b);
     const int64_t begin = at.range * a.range_len;
     const int64_t end = at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
@@ -414,7 +420,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
     for (int j = 0; j < VC; ++j) rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e;
     const int first = at.wave * WT + at.g * TL;  // the thread's first token in a tile
     using IO = Io<T, WIDE>;
-    const IO xs(a.x, a, s, at.b, first, at.c0), gs(a.g, a, s, at.b, first, at.c0), is(a.i, a, s, at.b, first, at.c0), hs(a.h, a, s, at.b, first, at.c0);
+    const IO xs(a.x, a, s, at.b, first, at.c0, at.mine), gs(a.g, a, s, at.b, first, at.c0, at.mine), is(a.i, a, s, at.b, first, at.c0, at.mine), hs(a.h, a, s, at.b, first, at.c0, at.mine);
 
     struct Raw {
         u32x4 x[TL], g[TL], i[TL];
@@ -471,7 +477,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
         }
         const auto kept = __builtin_amdgcn_make_buffer_rsrc(a.states + (s.state + t0 / kChunk) * a.channels, 0,
                                                             a.states && at.wave == 0 ? a.channels * 4 : 0, 0x00020000);
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, before), kept, 4 * at.ch, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, before), kept, at.on ? 4 * at.ch : (int)kNowhere, 0, 0);
 #pragma unroll
         for (int i = 0; i < VC; ++i) {
             const float x = before;
@@ -507,7 +513,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     static_assert(TILE == kChunk, "a tile begins at a kept state");
     __shared__ float2 spans[2][kWaves][64];
     __shared__ float backs[2][kWaves][64];
-    const Place<T> at(a);
+    const Place<T, WIDE> at(a);
     const Span s = span_of(a, at.b);
     const int64_t begin = at.range * a.range_len;
     const int64_t end = at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
@@ -524,8 +530,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     for (int j = 0; j < VC; ++j) rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e, dr[j] = 0.0f;
     const int first = at.wave * WT + at.g * TL;
     using IO = Io<T, WIDE>;
-    const IO xs(a.x, a, s, at.b, first, at.c0), gs(a.g, a, s, at.b, first, at.c0), is(a.i, a, s, at.b, first, at.c0), es(a.h, a, s, at.b, first, at.c0);
-    const IO dxs(a.dx, a, s, at.b, first, at.c0), dgs(a.dg, a, s, at.b, first, at.c0), dis(a.di, a, s, at.b, first, at.c0);
+    const IO xs(a.x, a, s, at.b, first, at.c0, at.mine), gs(a.g, a, s, at.b, first, at.c0, at.mine), is(a.i, a, s, at.b, first, at.c0, at.mine), es(a.h, a, s, at.b, first, at.c0, at.mine);
+    const IO dxs(a.dx, a, s, at.b, first, at.c0, at.mine), dgs(a.dg, a, s, at.b, first, at.c0, at.mine), dis(a.di, a, s, at.b, first, at.c0, at.mine);
 
     struct Raw {
         u32x4 x[TL], g[TL], i[TL], e[TL];
@@ -713,7 +719,9 @@ struct Few {
 };
 template <class T, int V>
 __device__ __forceinline__ Few<T, V> few_load(const Rows& t, int64_t base, int64_t token, int c0) {
-    return *reinterpret_cast<const Few<T, V>*>(__builtin_assume_aligned(reinterpret_cast<const T*>(t.p) + base + token * t.ts + c0, V * sizeof(T)));
+    Few<T, V> v;
+    __builtin_memcpy(&v, reinterpret_cast<const T*>(t.p) + base + token * t.ts + c0, sizeof(v));
+    return v;
 }
 template <class T, int V>
 __device__ __forceinline__ void few_store(const Rows& t, int64_t base, int64_t token, int c0, const float (&v)[V]) {
@@ -723,14 +731,16 @@ __device__ __forceinline__ void few_store(const Rows& t, int64_t base, int64_t t
         if constexpr (sizeof(T) == 4) o.x[j] = v[j];
         else o.x[j] = __builtin_bit_cast(uint16_t, (__bf16)v[j]);
     }
-    *reinterpret_cast<Few<T, V>*>(__builtin_assume_aligned(reinterpret_cast<T*>(t.p) + base + token * t.ts + c0, V * sizeof(T))) = o;
+    __builtin_memcpy(reinterpret_cast<T*>(t.p) + base + token * t.ts + c0, &o, sizeof(o));
 }
 __device__ __forceinline__ int64_t base_of(const Rows& t, const Args& a, const Span& s, int b) { return a.starts ? s.base * t.ts : b * t.bs; }
 
 template <class T, int V, bool GATED>
 __global__ __launch_bounds__(kFewThreads) void recurrence_few_fwd_kernel(Args a) {
-    const int c0 = (blockIdx.x * kFewThreads + threadIdx.x) * V, b = blockIdx.y;
+    int c0 = (blockIdx.x * kFewThreads + threadIdx.x) * V;
+    const int b = blockIdx.y;
     if (c0 >= a.channels) return;
+    if (c0 > a.channels - V) c0 = a.channels - V;  // the last piece ends with the last channel, over its neighbour
     const Span s = span_of(a, b);
     const int64_t xb = base_of(a.x, a, s, b), gb = base_of(a.g, a, s, b), ib = base_of(a.i, a, s, b), hb = base_of(a.h, a, s, b);
     const int64_t mine = (int64_t)b * a.channels + c0;
@@ -774,8 +784,10 @@ __global__ __launch_bounds__(kFewThreads) void recurrence_few_fwd_kernel(Args a)
 // kFew tokens at a time from the last, the states before them from the kept one on
 template <class T, int V, bool GATED>
 __global__ __launch_bounds__(kFewThreads) void recurrence_few_bwd_kernel(Args a) {
-    const int c0 = (blockIdx.x * kFewThreads + threadIdx.x) * V, b = blockIdx.y;
+    int c0 = (blockIdx.x * kFewThreads + threadIdx.x) * V;
+    const int b = blockIdx.y;
     if (c0 >= a.channels) return;
+    if (c0 > a.channels - V) c0 = a.channels - V;  // the last piece ends with the last channel, over its neighbour
     const Span s = span_of(a, b);
     const int64_t xb = base_of(a.x, a, s, b), gb = base_of(a.g, a, s, b), ib = base_of(a.i, a, s, b), eb = base_of(a.h, a, s, b);
     const int64_t dxb = base_of(a.dx, a, s, b), dgb = base_of(a.dg, a, s, b), dib = base_of(a.di, a, s, b);
@@ -905,13 +917,8 @@ int check_rows(const R97qRows* t, const R97qRecurrence* p, bool output, const ch
 
 Rows rows_of(const R97qRows* t) { return t ? Rows{static_cast<uint8_t*>(t->data), t->batch_stride, t->token_stride} : Rows{}; }
 
-bool wide(const R97qRows* t, const R97qRecurrence* p) {
-    if (!t) return true;
-    // a tile's rows lie within 31 bits of its first
-    const int unit = p->dtype == R97Q_F32 ? 4 : 8;
-    return !(reinterpret_cast<uintptr_t>(t->data) & 15) && t->token_stride % unit == 0 && (p->starts || t->batch_stride % unit == 0) &&
-           t->token_stride <= (1 << 20);
-}
+// pieces: a tile's rows lie within 31 bits of its first
+bool wide(const R97qRows* t) { return !t || t->token_stride <= (1 << 20); }
 
 int64_t all_tokens(const R97qRecurrence* p) { return p->starts ? p->tokens : p->batch * p->len; }
 
@@ -1038,7 +1045,10 @@ int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     a.states = states;
     a.spans = static_cast<float2*>(workspace);
     a.kept = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + spans_bytes(a));
-    const bool w = a.channels % (shape->dtype == R97Q_F32 ? 4 : 8) == 0 && wide(x, shape) && wide(gate, shape) && wide(input_gate, shape) && wide(h, shape);
+    // two pieces that overlap are read and written twice: not over an input
+    const int unit = shape->dtype == R97Q_F32 ? 4 : 8;
+    const bool over = h->data == x->data || h->data == gate->data || (input_gate && h->data == input_gate->data);
+    const bool w = a.channels >= unit && (a.channels % unit == 0 || !over) && wide(x) && wide(gate) && wide(input_gate) && wide(h);
     return shape->dtype == R97Q_F32 ? pick<float>(a, false, w, (hipStream_t)stream) : pick<uint16_t>(a, false, w, (hipStream_t)stream);
 }
 
@@ -1087,8 +1097,8 @@ int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     a.states = const_cast<float*>(states);
     a.spans = static_cast<float2*>(workspace);
     a.drate = rows > 1 ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + spans_bytes(a)) : drate;
-    const bool w = a.channels % (shape->dtype == R97Q_F32 ? 4 : 8) == 0 && wide(x, shape) && wide(gate, shape) && wide(input_gate, shape) &&
-                   wide(d_h, shape) && wide(dx, shape) && wide(dgate, shape) && wide(dinput_gate, shape);
+    const bool w = a.channels >= (shape->dtype == R97Q_F32 ? 4 : 8) && wide(x) && wide(gate) && wide(input_gate) && wide(d_h) && wide(dx) &&
+                   wide(dgate) && wide(dinput_gate);
     if (rows > 0)
         if (int e = shape->dtype == R97Q_F32 ? pick<float>(a, true, w, st) : pick<uint16_t>(a, true, w, st)) return e;
     if (rows == 1) return R97Q_OK;

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from . import R97Q_BF16, R97Q_F32, Recurrence, Rows, _device, _empty, _empty_like, _ptr, _space, _stream, check, lib
+from . import R97Q_BF16, R97Q_F32, Recurrence, Rows, _device, _empty, _empty_like, _space, _stream, check, lib
 
 _DTYPES = {torch.bfloat16: R97Q_BF16, torch.float32: R97Q_F32}
 _F32 = torch.float32
