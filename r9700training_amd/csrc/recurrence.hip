@@ -58,6 +58,7 @@ struct Args {
     float2* spans;                // [batch][ranges][channels], the ranges' spans
     float* kept;                  // [batch][channels]: `first`, where `last` may be written over it
     int32_t few;                  // a thread a sequence
+    int32_t dealt;                // the grid is one-dimensional, an XCD's workgroups neighbours (deal())
     float* drate;                 // [batch * ranges][channels], or the sum itself where that is one row
 };
 
@@ -254,18 +255,28 @@ struct Place {
     int lane, wave, g, c0, ch, near, b, range;
     bool mine;  // the lane's piece is one: its first channel c0. WIDE: the last one ends with the last channel, over its neighbour
     bool on;    // the transposed lane's channel is one (near: one that may be read in any case)
-    __device__ __forceinline__ Place(const Args& a, int range0 = 0) {
+    bool none;  // a workgroup too many
+    __device__ __forceinline__ Place(const Args& a, int ranges, int range0 = 0) {
         lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         g = lane / LPR;
-        c0 = blockIdx.x * kSlab + lane % LPR * VC;
+        int slab = blockIdx.x, r = blockIdx.y;
+        b = blockIdx.z;
+        none = false;
+        if (a.dealt) {
+            const uint32_t slabs = (a.channels + kSlab - 1) / kSlab, each = gridDim.x / 8, i = blockIdx.x % 8 * each + blockIdx.x / 8, j = i / slabs;
+            none = i >= slabs * ranges * a.batch;
+            slab = (int)(i - j * slabs);
+            b = (int)(j / ranges);
+            r = (int)(j - (uint32_t)b * ranges);
+        }
+        c0 = slab * kSlab + lane % LPR * VC;
         mine = c0 < a.channels;
         if (WIDE && c0 > a.channels - VC) c0 = a.channels - VC;
         ch = c0 + g;
         on = mine && ch < a.channels;
         near = on ? ch : a.channels - 1;
-        range = range0 + blockIdx.y;
-        b = blockIdx.z;
+        range = range0 + r;
     }
 };
 
@@ -313,7 +324,8 @@ template <class T, bool GATED, bool WIDE, bool BACK>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
     constexpr int VC = kVC<T>, TL = 4;
     __shared__ float2 spans[kWaves][64];
-    const Place<T, WIDE> at(a, BACK);
+    const Place<T, WIDE> at(a, a.ranges - 1, BACK);
+    if (at.none) return;
     const Span s = span_of(a, at.b);
     const int64_t begin = at.range * a.range_len;
     const int64_t end = BACK && at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
@@ -404,7 +416,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
     constexpr int VC = kVC<T>, TL = 16 / VC, WT = VC * TL, TILE = kWaves * WT;
     static_assert(TILE == kChunk, "a tile begins at a kept state");
     __shared__ float2 spans[2][kWaves][64];
-    const Place<T, WIDE> at(a);
+    const Place<T, WIDE> at(a, a.ranges);
+    if (at.none) return;
     const Span s = span_of(a, at.b);
     const int64_t begin = at.range * a.range_len;
     const int64_t end = at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
@@ -513,7 +526,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     static_assert(TILE == kChunk, "a tile begins at a kept state");
     __shared__ float2 spans[2][kWaves][64];
     __shared__ float backs[2][kWaves][64];
-    const Place<T, WIDE> at(a);
+    const Place<T, WIDE> at(a, a.ranges);
+    if (at.none) return;
     const Span s = span_of(a, at.b);
     const int64_t begin = at.range * a.range_len;
     const int64_t end = at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
@@ -917,6 +931,12 @@ int check_rows(const R97qRows* t, const R97qRecurrence* p, bool output, const ch
 
 Rows rows_of(const R97qRows* t) { return t ? Rows{static_cast<uint8_t*>(t->data), t->batch_stride, t->token_stride} : Rows{}; }
 
+// whether a launch's workgroups are dealt by XCD
+bool lines_shared(const R97qRecurrence* p, const R97qRows* x, const Args& a) {
+    const int64_t size = p->dtype == R97Q_F32 ? 4 : 2, slabs = (p->channels + kSlab - 1) / kSlab;
+    return slabs >= 4 && slabs * a.ranges * a.batch <= (1 << 20) && ((reinterpret_cast<uintptr_t>(x->data) | (uintptr_t)(x->token_stride * size)) & 127);
+}
+
 // pieces: a tile's rows lie within 31 bits of its first
 bool wide(const R97qRows* t) { return !t || t->token_stride <= (1 << 20); }
 
@@ -955,24 +975,28 @@ Args args_of(const R97qRecurrence* p, bool back) {
 int64_t spans_bytes(const Args& a) { return a.ranges > 1 ? (8LL * a.batch * a.ranges * a.channels + 255) / 256 * 256 : 0; }
 int64_t row_bytes(const Args& a, int64_t rows) { return (4 * rows * a.channels + 255) / 256 * 256; }
 
+// A launch's grid over slabs, `ranges` and sequences. Rows that do not begin with a line of 128 bytes have slabs that share
+// lines, and each XCD has its own L2: then an XCD's workgroups are neighbours.
+dim3 deal(const Args& a, int ranges) {
+    const unsigned slabs = (unsigned)((a.channels + kSlab - 1) / kSlab);
+    return a.dealt ? dim3((slabs * (unsigned)ranges * (unsigned)a.batch + 7) / 8 * 8) : dim3(slabs, (unsigned)ranges, (unsigned)a.batch);
+}
 template <class T, bool GATED, bool WIDE>
 int run_fwd(const Args& a, hipStream_t st) {
-    const unsigned slabs = (unsigned)((a.channels + kSlab - 1) / kSlab);
     if (a.ranges > 1) {
-        hipLaunchKernelGGL((recurrence_spans_kernel<T, GATED, WIDE, false>), dim3(slabs, a.ranges - 1, a.batch), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL((recurrence_spans_kernel<T, GATED, WIDE, false>), deal(a, a.ranges - 1), dim3(kThreads), 0, st, a);
         if (int e = launch_status("recurrence_spans_kernel")) return e;
     }
-    hipLaunchKernelGGL((recurrence_fwd_kernel<T, GATED, WIDE>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((recurrence_fwd_kernel<T, GATED, WIDE>), deal(a, a.ranges), dim3(kThreads), 0, st, a);
     return launch_status("recurrence_fwd_kernel");
 }
 template <class T, bool GATED, bool WIDE>
 int run_bwd(const Args& a, hipStream_t st) {
-    const unsigned slabs = (unsigned)((a.channels + kSlab - 1) / kSlab);
     if (a.ranges > 1) {
-        hipLaunchKernelGGL((recurrence_spans_kernel<T, false, WIDE, true>), dim3(slabs, a.ranges - 1, a.batch), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL((recurrence_spans_kernel<T, false, WIDE, true>), deal(a, a.ranges - 1), dim3(kThreads), 0, st, a);
         if (int e = launch_status("recurrence_spans_kernel")) return e;
     }
-    hipLaunchKernelGGL((recurrence_bwd_kernel<T, GATED, WIDE>), dim3(slabs, a.ranges, a.batch), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((recurrence_bwd_kernel<T, GATED, WIDE>), deal(a, a.ranges), dim3(kThreads), 0, st, a);
     return launch_status("recurrence_bwd_kernel");
 }
 template <class T, int V, bool GATED>
@@ -1045,6 +1069,7 @@ int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     a.states = states;
     a.spans = static_cast<float2*>(workspace);
     a.kept = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + spans_bytes(a));
+    a.dealt = lines_shared(shape, x, a);
     // two pieces that overlap are read and written twice: not over an input
     const int unit = shape->dtype == R97Q_F32 ? 4 : 8;
     const bool over = h->data == x->data || h->data == gate->data || (input_gate && h->data == input_gate->data);
@@ -1097,6 +1122,7 @@ int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     a.states = const_cast<float*>(states);
     a.spans = static_cast<float2*>(workspace);
     a.drate = rows > 1 ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + spans_bytes(a)) : drate;
+    a.dealt = lines_shared(shape, x, a);
     const bool w = a.channels >= (shape->dtype == R97Q_F32 ? 4 : 8) && wide(x) && wide(gate) && wide(input_gate) && wide(d_h) && wide(dx) &&
                    wide(dgate) && wide(dinput_gate);
     if (rows > 0)

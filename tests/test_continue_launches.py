@@ -106,14 +106,21 @@ def test_recurrence_grids(hook, back, batch, channels, length):
     rate's gradients where there is more than one sequence or range."""
     for off in (0, 2):  # pieces of 16 bytes, and single values
         got = launches(hook, "scan", back=back, batch=batch, channels=channels, length=length, off=off)
-        main = got[-2] if back and (len(got) > 1 and got[-1][1][0] == 1024) else got[-1]
-        few = main[1][0] == 64
-        ranges = 1 if few else main[0][1]
-        assert main[0][1 if few else 2] == batch
-        if not few:
-            assert main[0][0] == -(-channels // 64) and ranges <= 257
-            if ranges > 1:
-                assert got[0][0] == (main[0][0], ranges - 1, batch)
-        assert len(got) == 1 + (ranges > 1) + (back and batch * ranges > 1)
+        adds = back and got[-1][1][0] == 1024
+        main = got[-2] if adds else got[-1]
+        few, slabs = main[1][0] == 64, -(-channels // 64)
+        cut = len(got) == 2 + adds
+        if few:
+            assert main[0][1] == batch
+        elif main[0][1:] == (1, 1) and slabs >= 4 and main[0][0] % 8 == 0 and main[0][0] != slabs:
+            # dealt by XCD: all workgroups, and up to seven too many
+            ranges = main[0][0] // (slabs * batch)
+            assert 0 <= main[0][0] - slabs * ranges * batch < 8 and ranges <= 257
+            assert not cut or 0 <= got[0][0][0] - slabs * (ranges - 1) * batch < 8
+        else:
+            ranges = main[0][1]
+            assert main[0] == (slabs, ranges, batch) and ranges <= 257
+            assert not cut or got[0][0] == (slabs, ranges - 1, batch)
+        assert len(got) == 1 + cut + adds and (not back or adds == (batch > 1 or cut))
     packed = launches(hook, "scan", back=back, batch=batch, channels=channels, length=0, packed=min(batch * max(length, 1), 2 ** 31 - 1))
     assert packed

@@ -91,6 +91,12 @@ DENSE = [
     (2, 2048, 128, BF, True, True),
     (1, 5000, 64, BF, True, True),
     (1, 4100, 77, F32, True, True),
+    (2, 300, 333, BF, True, True),        # slabs that share lines, dealt by XCD
+    (1, 2000, 515, BF, False, True),
+    (5, 140, 259, F32, True, True),
+    (1, 1700, 1001, F32, True, False),
+    (3, 16, 9, BF, True, True),
+    (2, 9, 5, F32, True, True),
 ]
 
 
@@ -169,7 +175,7 @@ def test_starts_outside_the_tensors(bad):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("batch,n,c", [(2, 70, 64), (1, 300, 136), (3, 1, 128), (1, 3000, 64)])
+@pytest.mark.parametrize("batch,n,c", [(2, 70, 64), (1, 300, 136), (3, 1, 128), (1, 3000, 64), (2, 200, 99), (3, 5, 13), (1, 2000, 300)])
 def test_layouts(batch, n, c, dtype):
     """Slices of a fused projection's rows, token-major storage, places off 16 bytes, a broadcast sequence, and outputs over
     the inputs give the contiguous call's bits."""
