@@ -53,9 +53,9 @@ struct Args {
     const int32_t* starts;
     int64_t tokens, len;
     int32_t batch, channels;
-    int32_t ranges;
-    int64_t range_len;
-    float2* spans;                // [batch][ranges][channels], the ranges' spans
+    int32_t ranges, fine;         // ranges, and the spans of one
+    int64_t range_len, span_len;
+    float2* spans;                // [batch][ranges * fine][channels]
     float* kept;                  // [batch][channels]: `first`, where `last` may be written over it
     int32_t few;                  // a thread a sequence
     int32_t dealt;                // the grid is one-dimensional, an XCD's workgroups neighbours (deal())
@@ -316,20 +316,21 @@ __device__ __forceinline__ void blank(u32x4& x, u32x4& g, u32x4& i, bool out) {
 }
 
 // ---------------------------------------------------------------- the ranges' spans
-// grid (slabs, all but one range, sequences): what a range makes of the state before it, or (BACK, from a and dh alone) of the
+// grid (slabs, all but one range's spans, sequences): what a part of a range makes of the state before it, or (BACK, from a and dh alone) of the
 // cotangent behind it. Nothing is needed of the tokens between, so a lane's group takes a run of tokens of its own, with no
 // join but one at the end. The span that has the given end (the first, or BACK the last) holds it; the forward
 // also keeps a copy of it, since `last` may be written over it before every workgroup of the next launch has read it.
 template <class T, bool GATED, bool WIDE, bool BACK>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
-    constexpr int VC = kVC<T>, TL = 4;
+    constexpr int VC = kVC<T>, TL = 2;
     __shared__ float2 spans[kWaves][64];
-    const Place<T, WIDE> at(a, a.ranges - 1, BACK);
+    const int all = a.ranges * a.fine;
+    const Place<T, WIDE> at(a, all - a.fine, BACK ? a.fine : 0);
     if (at.none) return;
     const Span s = span_of(a, at.b);
-    const int64_t begin = at.range * a.range_len;
-    const int64_t end = BACK && at.range == a.ranges - 1 ? s.len : clamp64(begin + a.range_len, 0, s.len);
-    const int64_t run = (end - begin + kWaves * VC - 1) / (kWaves * VC), from = begin + (at.wave * VC + at.g) * run;
+    const int64_t begin = at.range * a.span_len;
+    const int64_t end = BACK && at.range == all - 1 ? s.len : clamp64(begin + a.span_len, 0, s.len);
+    const int64_t run = ((end - begin + kWaves * VC - 1) / (kWaves * VC)), from = begin + (at.wave * VC + at.g) * run;
     float rate[VC], y[VC], u[VC];
 #pragma unroll
     for (int j = 0; j < VC; ++j) {
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
     if (at.wave || !at.on) return;
     const int64_t mine = (int64_t)at.b * a.channels + at.ch;
     float v = 0.0f;
-    if (a.first && at.range == (BACK ? a.ranges - 1 : 0)) {
+    if (a.first && at.range == (BACK ? all - 1 : 0)) {
         v = a.first[mine];
         if constexpr (!BACK) a.kept[mine] = v;
     }
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
         v = __builtin_fmaf(decay_of(p.x), v, p.y);
         sum += p.x;
     }
-    a.spans[((int64_t)at.b * a.ranges + at.range) * a.channels + at.ch] = make_float2(decay_of(sum), v);
+    a.spans[((int64_t)at.b * all + at.range) * a.channels + at.ch] = make_float2(decay_of(sum), v);
 }
 
 // ---------------------------------------------------------------- forward
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
     if (at.range == 0) {
         if (a.first) h = a.ranges > 1 ? a.kept[mine] : a.first[mine];
     } else {
-        h = through(a.spans + (int64_t)at.b * a.ranges * a.channels + at.near, a.channels, at.range, at.wave, at.lane, spans[0]);
+        h = through(a.spans + (int64_t)at.b * a.ranges * a.fine * a.channels + at.near, a.channels, at.range * a.fine, at.wave, at.lane, spans[0]);
     }
     float rate[VC];
 #pragma unroll
@@ -536,8 +537,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     if (at.range == a.ranges - 1) {
         if (a.first) m = a.first[mine];
     } else {  // the last range's span holds what is behind it
-        m = through(a.spans + ((int64_t)(at.b + 1) * a.ranges - 1) * a.channels + at.near, -(int64_t)a.channels, a.ranges - 1 - at.range,
-                    at.wave, at.lane, spans[0]);
+        m = through(a.spans + ((int64_t)(at.b + 1) * a.ranges * a.fine - 1) * a.channels + at.near, -(int64_t)a.channels,
+                    (a.ranges - 1 - at.range) * a.fine, at.wave, at.lane, spans[0]);
     }
     float rate[VC], dr[VC];
 #pragma unroll
@@ -934,7 +935,7 @@ Rows rows_of(const R97qRows* t) { return t ? Rows{static_cast<uint8_t*>(t->data)
 // whether a launch's workgroups are dealt by XCD
 bool lines_shared(const R97qRecurrence* p, const R97qRows* x, const Args& a) {
     const int64_t size = p->dtype == R97Q_F32 ? 4 : 2, slabs = (p->channels + kSlab - 1) / kSlab;
-    return slabs >= 4 && slabs * a.ranges * a.batch <= (1 << 20) && ((reinterpret_cast<uintptr_t>(x->data) | (uintptr_t)(x->token_stride * size)) & 127);
+    return slabs >= 4 && slabs * a.ranges * a.fine * a.batch <= (1 << 20) && ((reinterpret_cast<uintptr_t>(x->data) | (uintptr_t)(x->token_stride * size)) & 127);
 }
 
 // pieces: a tile's rows lie within 31 bits of its first
@@ -960,6 +961,11 @@ void cut(const R97qRecurrence* p, bool back, Args& a) {
     if (a.range_len < kChunk) a.range_len = kChunk;
     a.ranges = (int32_t)((most + a.range_len - 1) / a.range_len);
     if (a.ranges < 1) a.ranges = 1;
+    // the spans' launch has one range's workgroups less: where that leaves half of them out, two spans a range and more
+    a.fine = a.ranges > 1 ? (int32_t)(256 / ((a.ranges - 1) * have)) : 1;
+    while (a.fine > 1 && a.range_len % (64 * a.fine)) --a.fine;
+    if (a.fine < 1) a.fine = 1;
+    a.span_len = a.range_len / a.fine;
 }
 
 Args args_of(const R97qRecurrence* p, bool back) {
@@ -972,7 +978,7 @@ Args args_of(const R97qRecurrence* p, bool back) {
     cut(p, back, a);
     return a;
 }
-int64_t spans_bytes(const Args& a) { return a.ranges > 1 ? (8LL * a.batch * a.ranges * a.channels + 255) / 256 * 256 : 0; }
+int64_t spans_bytes(const Args& a) { return a.ranges > 1 ? (8LL * a.batch * a.ranges * a.fine * a.channels + 255) / 256 * 256 : 0; }
 int64_t row_bytes(const Args& a, int64_t rows) { return (4 * rows * a.channels + 255) / 256 * 256; }
 
 // A launch's grid over slabs, `ranges` and sequences. Rows that do not begin with a line of 128 bytes have slabs that share
@@ -984,7 +990,7 @@ dim3 deal(const Args& a, int ranges) {
 template <class T, bool GATED, bool WIDE>
 int run_fwd(const Args& a, hipStream_t st) {
     if (a.ranges > 1) {
-        hipLaunchKernelGGL((recurrence_spans_kernel<T, GATED, WIDE, false>), deal(a, a.ranges - 1), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL((recurrence_spans_kernel<T, GATED, WIDE, false>), deal(a, (a.ranges - 1) * a.fine), dim3(kThreads), 0, st, a);
         if (int e = launch_status("recurrence_spans_kernel")) return e;
     }
     hipLaunchKernelGGL((recurrence_fwd_kernel<T, GATED, WIDE>), deal(a, a.ranges), dim3(kThreads), 0, st, a);
@@ -993,7 +999,7 @@ int run_fwd(const Args& a, hipStream_t st) {
 template <class T, bool GATED, bool WIDE>
 int run_bwd(const Args& a, hipStream_t st) {
     if (a.ranges > 1) {
-        hipLaunchKernelGGL((recurrence_spans_kernel<T, false, WIDE, true>), deal(a, a.ranges - 1), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL((recurrence_spans_kernel<T, false, WIDE, true>), deal(a, (a.ranges - 1) * a.fine), dim3(kThreads), 0, st, a);
         if (int e = launch_status("recurrence_spans_kernel")) return e;
     }
     hipLaunchKernelGGL((recurrence_bwd_kernel<T, GATED, WIDE>), deal(a, a.ranges), dim3(kThreads), 0, st, a);
