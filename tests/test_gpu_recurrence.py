@@ -208,6 +208,21 @@ def test_layouts(batch, n, c, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n,c", [(1, 4099), (3, 261), (300, 65), (700, 1029), (2000, 130)])
+def test_in_place_of_odd_widths(n, c, dtype):
+    """The state and the outputs over the inputs, where the last piece of channels lies over its neighbour's."""
+    from r9700training_amd.recurrence import recurrence_fwd
+
+    x, gate, gi, rate, h0 = inputs(1, (6, n, c), dtype, True, 6, c)
+    h, last, _ = recurrence_fwd(x, gate, rate, gi, h0=h0)
+    for i in range(6):
+        mine, state = [x.clone(), gate.clone(), gi.clone()], h0.clone()
+        out = mine[i % 3] if i % 2 else None
+        got = recurrence_fwd(*mine[:2], rate, mine[2], h0=state, last=state, out=out)[0]
+        assert torch.equal(got, h) and torch.equal(state, last)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("cuts", [[1] * 20, [100, 1, 156, 43], [600, 1, 1, 1300]])
 def test_continued(dtype, cuts):
     """A sequence in pieces, each from the state the one before it left, is the whole sequence."""
