@@ -700,8 +700,9 @@ typedef struct R97qRows {
  * sequence, which the next tokens begin from; that of a sequence without tokens is h0. states f32 [rows][channels] (may be
  * NULL; r97q_recurrence_state_rows says how many rows): for the backward, the state before every token that is a multiple
  * of R97Q_RECURRENCE_CHUNK of its sequence, dense row b * ceil(len / CHUNK) + t / CHUNK, packed starts[b] / CHUNK + b + t /
- * CHUNK. Packed tokens outside every sequence are not written. h may be x, gate or input_gate. Few channels over many tokens
- * are cut along the tokens and joined through the workspace (on 16 bytes, often 0). Repeated calls give the same bits. */
+ * CHUNK. Packed tokens outside every sequence are not written. h may be x, gate or input_gate, with its strides; no tensors
+ * overlap otherwise. Few channels over many tokens are cut along the tokens and joined through the workspace (on 16 bytes,
+ * often 0). Repeated calls give the same bits. */
 int64_t r97q_recurrence_state_rows(const R97qRecurrence* shape);
 int64_t r97q_recurrence_fwd_workspace_bytes(const R97qRecurrence* shape);
 int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R97qRows* gate, const R97qRows* input_gate,
@@ -709,7 +710,7 @@ int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R9
                         int64_t workspace_bytes, R97IqrStream stream);
 /* The adjoint, from the forward's inputs and states and the cotangents d_h and d_last f32 [batch][channels] (NULL: zeros):
  * dx, dgate, dinput_gate (with input_gate), drate f32 [channels], summed over all tokens, and dh0 f32 [batch][channels] (may
- * be NULL) are written. Where a decay is one (a rate of zero, a gate far below zero) the derivative through sqrt(1 - a^2),
+ * be NULL) are written, over none of the inputs. Where a decay is one (a rate of zero, a gate far below zero) the derivative through sqrt(1 - a^2),
  * which has no bound there, counts as zero. Packed tokens outside every sequence are not written. Repeated calls give the
  * same bits. The workspace (on 16 bytes) holds the ranges' joins and the rate's partial sums. */
 int64_t r97q_recurrence_bwd_workspace_bytes(const R97qRecurrence* shape);

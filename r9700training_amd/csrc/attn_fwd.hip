@@ -584,7 +584,7 @@ Plan plan_of(const Args& a) {
 }
 
 // how a tile of `rows` keys finds its pages
-int mode_of(const Args& a, int rows) {
+[[maybe_unused]] int mode_of(const Args& a, int rows) {
     if (!kPaged) return kNoPages;
     auto near = [&](const Heads& t) { return 2.0 * ((double)(a.pages > 0 ? a.pages - 1 : 0) * t.bs + (double)((1 << a.page_shift) - 1) * t.ts + a.d) <= (double)kNearBytes; };
     return !near(a.k) || !near(a.v) ? kFarPages : 1 << a.page_shift >= rows ? kWholePages : kSmallPages;

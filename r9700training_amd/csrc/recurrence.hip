@@ -1079,7 +1079,14 @@ int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     // The last piece's channels that are its neighbour's too are read twice, by two workgroups at times: not where one of them may
     // have written over them. Odd widths in place go value by value (8 x 2048 x 2047 forward 138 us, else 62).
     const int unit = shape->dtype == R97Q_F32 ? 4 : 8;
-    const bool over = h->data == x->data || h->data == gate->data || (input_gate && h->data == input_gate->data) || (h0 && h0 == last);
+    const R97qRows* ins[] = {x, gate, input_gate};
+    bool over = h0 && h0 == last;
+    for (const R97qRows* in : ins) {
+        if (!in || !h->data || in->data != h->data) continue;
+        if (in->token_stride != h->token_stride || (!shape->starts && in->batch_stride != h->batch_stride))
+            return refuse(R97Q_EINVAL, who, "h over an input has that input's strides");
+        over = true;
+    }
     const bool w = a.channels >= unit && (a.channels % unit == 0 || !over) && wide(x) && wide(gate) && wide(input_gate) && wide(h);
     return shape->dtype == R97Q_F32 ? pick<float>(a, false, w, (hipStream_t)stream) : pick<uint16_t>(a, false, w, (hipStream_t)stream);
 }
@@ -1116,6 +1123,14 @@ int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     const int64_t rows = (int64_t)a.batch * a.ranges, need = spans_bytes(a) + (rows > 1 ? row_bytes(a, rows) : 0);
     if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
     if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
+    // ranges read what others write: d_last and dh0 are two tensors, and so are an input and an output
+    const R97qRows *ins[] = {x, gate, input_gate, d_h}, *outs[] = {dx, dgate, dinput_gate};
+    bool over = d_last && d_last == dh0;
+    for (const R97qRows* out : outs) {
+        for (const R97qRows* in : ins) over |= in && out && out->data && in->data == out->data;
+        for (const R97qRows* other : outs) over |= out && other && out != other && out->data && other->data == out->data;
+    }
+    if (over) return refuse(R97Q_EINVAL, who, "an output over an input or another output");
     a.x = rows_of(x);
     a.g = rows_of(gate);
     a.i = rows_of(all_tokens(shape) > 0 ? input_gate : nullptr);

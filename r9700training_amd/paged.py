@@ -16,6 +16,12 @@ from . import AttnShape, Pages, _device, _empty, _empty_like, _ptr, _space, _str
 from .attention import _check_lse, _heads, _index, _lse_shape
 
 
+def _beside(device, *tensors):
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError("paged: all tensors are on the new tokens' device")
+
+
 def _cache(q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, max_kv=None, causal=0, window=0, scale=1.0, stream=None):
     """(shape, pages) of a call whose new tokens are shaped like q."""
     packed = q_starts is not None
@@ -26,10 +32,10 @@ def _cache(q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, max_kv=Non
     if page_table.dtype != torch.int32 or len(ts) != 2 or (ts[1] > 1 and st[1] != 1):
         raise ValueError("paged: page_table is an int32 [batch, most pages] device tensor, a row's entries consecutive")
     device = _device(q, stream, "paged")
-    if k_pages.get_device() != device or v_pages.get_device() != device or page_table.get_device() != device or kv_lens.get_device() != device:
-        raise ValueError("paged: the pages, the table and the lengths are on the new tokens' device")
+    _beside(device, k_pages, v_pages, page_table, kv_lens)
     batch, starts, tokens = ts[0], None, 0
     if packed:
+        _beside(device, q_starts)
         starts = _index(q_starts, batch + 1, "q_starts").data_ptr()
         if max_q is None:
             raise ValueError("paged: packed tokens need max_q, the longest sequence's")
@@ -50,6 +56,7 @@ def paged_write(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None, max_
     if v.shape != k.shape:
         raise ValueError("paged: v has k's shape")
     s, p = _cache(k, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, stream=stream)
+    _beside(k.get_device(), v)
     check(lib().r97q_paged_write(s, p, _heads(k, packed, "k"), _heads(v, packed, "v"), _heads(k_pages, False, "k_pages"),
                                  _heads(v_pages, False, "v_pages"), _stream(stream)), "r97q_paged_write")
 
@@ -71,6 +78,7 @@ def paged_attention_fwd(q, k_pages, v_pages, page_table, kv_lens, causal: bool =
     if lse is None:
         lse = _empty(_lse_shape(qs, packed), torch.float32, q.device, stream)
     _check_lse(lse, qs, packed)
+    _beside(q.get_device(), out, lse)
     hq, hk = _heads(q, packed, "q"), _heads(k_pages, False, "k_pages")
     if workspace is None:
         need = lib().r97q_paged_attn_fwd_workspace_bytes(s, p, hq.heads, hk.heads)

@@ -80,7 +80,7 @@ def recurrence_bwd(x, gate, rate, states, d_h, input_gate=None, d_last=None, sta
                    dx=None, dgate=None, dinput_gate=None, drate=None, dh0=None, workspace=None, stream=None):
     """(dx, dgate, dinput_gate, drate, dh0), written: the adjoint of recurrence_fwd with the same arguments, from the states
     it kept and the cotangents d_h (x's shape and type) and d_last (f32, None: zeros). dinput_gate is None without an
-    input_gate; drate f32 [channels] is the sum over all tokens, dh0 f32 [batch, channels]."""
+    input_gate; none may be one of the inputs; drate f32 [channels] is the sum over all tokens, dh0 f32 [batch, channels]."""
     s, like = _shape(x, starts, max_len), (x.shape, x.dtype, _device(x, stream, "recurrence"))
     ends = (s.batch, s.channels)
     dx = _empty_like(x, x.dtype, stream) if dx is None else dx

@@ -108,9 +108,9 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor,
     """rotary with a position on each of several axes: positions int32 or int64 [axes, tokens], and pair i turns by
     positions[pair_axis[i]] * inv_freq[i] (pair_axis int32 [rot / 2]: rotary_pair_axes)."""
     device = _device(q, stream, "rotary_axes")
-    if (k is not None and k.get_device() != device) or inv_freq.get_device() != device or positions.get_device() != device \
-            or pair_axis.get_device() != device:
-        raise ValueError("rotary_axes: k, inv_freq, positions and pair_axis are on q's device")
+    for t in (k, inv_freq, positions, pair_axis, q_out, k_out):
+        if t is not None and t.get_device() != device:
+            raise ValueError("rotary_axes: all tensors are on q's device")
     q_out, k_out, tokens, dim, heads = _tensors(q, k, inv_freq, pairs, q_out, k_out, stream)
     if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 2 or positions.shape[1] != tokens \
             or (tokens > 1 and positions.stride(1) != 1) or not positions.is_cuda:

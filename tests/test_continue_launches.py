@@ -40,8 +40,9 @@ def write(batch, hk, d, q_len, page, max_pages, pages, packed=0):
 def scan(back, batch, channels, length, dtype=1, packed=0, off=0):
     s = Recurrence(batch, channels, length, FAKE if packed else None, packed, dtype)
     r = Rows(FAKE + off, length * channels, channels)
+    outs = [Rows(i * FAKE + off, length * channels, channels) for i in (2, 3, 4)]
     if back:
-        return lib().r97q_recurrence_bwd(s, r, r, r, FAKE, FAKE, r, FAKE, r, r, r, FAKE, FAKE, FAKE, max(lib().r97q_recurrence_bwd_workspace_bytes(s), 0), None)
+        return lib().r97q_recurrence_bwd(s, r, r, r, FAKE, FAKE, r, None, *outs, FAKE, FAKE, FAKE, max(lib().r97q_recurrence_bwd_workspace_bytes(s), 0), None)
     return lib().r97q_recurrence_fwd(s, r, r, r, FAKE, FAKE, r, FAKE, FAKE, FAKE, max(lib().r97q_recurrence_fwd_workspace_bytes(s), 0), None)
 
 for line in sys.stdin:

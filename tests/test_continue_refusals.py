@@ -192,6 +192,20 @@ def test_recurrence_missing():
     assert lib().r97q_recurrence_bwd(rec(), x, x, x, FAKE, FAKE, x, None, x, x, None, FAKE, None, FAKE, 1 << 40, None) == EINVAL
 
 
+def test_recurrence_outputs_over_inputs():
+    """The backward reads its inputs while its outputs are written; the forward's output may be an input, strides and all."""
+    own = {n: rows(data=FAKE + 0x10000 * i) for i, n in enumerate(("x", "gate", "gi", "d_h", "dx", "dgate", "dgi"))}
+    for out in ("dx", "dgate", "dgi"):
+        for other in own:
+            if other != out:
+                assert rbwd(**{**own, out: rows(data=own[other].data)}) == EINVAL and b"over" in lib().r97q_last_error(), (out, other)
+    x = own["x"]
+    call = lib().r97q_recurrence_bwd
+    assert call(rec(), x, own["gate"], None, FAKE, FAKE, own["d_h"], FAKE, own["dx"], own["dgate"], None, FAKE, FAKE, FAKE, 1 << 40, None) == EINVAL
+    for which in ("x", "gate", "gi"):
+        assert rfwd(**{**{n: own[n] for n in ("x", "gate", "gi")}, "h": rows(data=own[which].data, token_stride=128)}) == EINVAL, which
+
+
 def test_recurrence_workspace():
     s = rec(batch=1, len=16384)
     for call, need in ((rfwd, lib().r97q_recurrence_fwd_workspace_bytes(s)), (rbwd, lib().r97q_recurrence_bwd_workspace_bytes(s))):
