@@ -400,8 +400,8 @@ __device__ __forceinline__ void landed() {
 // The same of a sequence's tokens in pages. A wave holds 64 entries of the sequence's row of the table, a lane's each: tiles
 // begin at multiples of their size, so a tile's pages are of one such block. The next 64 wait in LDS, loaded like the tiles
 // (an ordinary load on its way through the loop would have every step wait for all that it has asked for). An entry outside
-// the pool reads as zeros, like a token past the end. The keys' walk leads, and loads the entries for the values' too, which is at most
-// two tiles behind: less than a block.
+// the pool reads as zeros, like a token past the end. The keys' walk leads, and loads the entries for the values' too, which
+// is at most two tiles behind: less than a block.
 constexpr int kTableBytes = 2 * 64 * 4;  // of LDS, a wave
 struct PageTable {
     u32x4 row;             // the sequence's row of the table
@@ -442,8 +442,8 @@ struct PageTable {
 // How a pool's pages are reached: one buffer with a page's offset in it, where the pool is less than 2 GiB, a tile's page looked
 // up once (kWholePages: they hold a tile) or a wave's piece at a time (kSmallPages: of a tile's first one on); else a piece's
 // page as a buffer of its own (kFarPages). What a step does for it counts, since no product runs beside it: 2048 tokens over
-// 16384, 16 over 4 heads of 128, 287 us over rows, 300 over pages of 64, 320 of 16; with every piece's page and bounds worked
-// out in scalars 374, and with the next entries an ordinary load 415.
+// 16384, 16 over 4 heads of 128, 277 us over rows, 286 over pages of 64, of 16 and of 8 some 2% more; with every piece's page
+// and bounds worked out in scalars 374 (64), and with the next entries an ordinary load 415.
 enum { kWholePages, kSmallPages, kFarPages };
 constexpr uint32_t kNearBytes = 0x7FFFFFF0u;  // a near pool's end at most: an offset for entries outside the pool
 template <int MODE>

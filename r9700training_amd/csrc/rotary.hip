@@ -9,7 +9,7 @@
 // and cosines once in LDS (rot / 2 a token, against heads * rot / 2 pairs that use them) and then walks the
 // tokens' heads in 16-byte pieces, kItems pieces of a thread in flight together. With several axes a token has a position on
 // each and a pair an axis: only the table's positions differ. 16384 tokens, 40 heads of 128: 73 us, as
-// neighbouring pairs 75 (4.5 TB/s; a 1 GiB copy reaches 4.9). One token: 4.4 us, latency.
+// neighbouring pairs 75 (4.5 TB/s; a 1 GiB copy reaches 4.9), with three axes 77 .. 79. One token: 4.4 us, latency.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -123,12 +123,16 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RArgs a) {
     const int nt = a.tokens - t0 < a.tpb ? (int)(a.tokens - t0) : a.tpb;
     for (int i = threadIdx.x; i < nt * a.half; i += kThreads) {
         const int64_t t = t0 + i / a.half;
-        const int ax = a.axis ? a.axis[i % a.half] : 0;
-        const bool turns_at_all = !a.axis || (uint32_t)ax < (uint32_t)a.axes;
-        const int64_t at = turns_at_all ? ax * a.axis_stride + t : 0;
-        const double p = !turns_at_all ? 0.0
-                         : !a.pos ? (double)t
-                         : a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[at] : (double)static_cast<const int32_t*>(a.pos)[at];
+        double p;
+        if (!a.axis) {
+            p = !a.pos ? (double)t
+                : a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[t] : (double)static_cast<const int32_t*>(a.pos)[t];
+        } else {
+            const int ax = a.axis[i % a.half];
+            const bool one = (uint32_t)ax < (uint32_t)a.axes;
+            const int64_t at = one ? ax * a.axis_stride + t : 0;
+            p = !one ? 0.0 : a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[at] : (double)static_cast<const int32_t*>(a.pos)[at];
+        }
         double turns = p * a.freq[i % a.half] * 0.15915494309189534;
         turns -= rint(turns);
         float s, c;

@@ -44,14 +44,24 @@ def _heads(x: torch.Tensor, what: str, shape=None) -> Heads:
     return Heads(x.data_ptr(), 0, st[0], st[1], own[1], dt)
 
 
-def _tensors(q, k, inv_freq, pairs, q_out, k_out, stream):
-    """(q_out, k_out, tokens, head_dim, and the four tensors of heads) of a call, checked."""
+def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
+           pairs: str = "half", mscale: float = 1.0, inverse: bool = False, q_out: torch.Tensor | None = None,
+           k_out: torch.Tensor | None = None, stream=None, *, _axes: tuple | None = None):
+    """(q, k) [tokens, heads, head_dim] turned by positions * inv_freq (positions None: 0, 1, ..); k may be
+    None. The first 2 * len(inv_freq) values of a head turn, the rest are copied. inverse: the adjoint
+    (turned back, scaled by the same mscale). q_out / k_out may be q / k."""
     if pairs not in PAIRS:
         raise ValueError(f"rotary: pairs {pairs!r} are not one of {sorted(PAIRS)}")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() or not inv_freq.is_cuda:
         raise ValueError("rotary: inv_freq is a contiguous f64 [rot / 2] device tensor")
     qs = q.shape
     tokens, _, dim = qs if len(qs) == 3 else (0, 0, 0)
+    wide = 0
+    if positions is not None and _axes is None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) \
+                or not positions.is_contiguous() or not positions.is_cuda:
+            raise ValueError("rotary: positions are a contiguous int32 or int64 [tokens] device tensor")
+        wide = int(positions.dtype == torch.int64)
     hq = _heads(q, "q")
     if q_out is None:
         q_out = _empty_like(q, q.dtype, stream)
@@ -66,23 +76,11 @@ def _tensors(q, k, inv_freq, pairs, q_out, k_out, stream):
             raise ValueError("rotary: k has q's tokens and head_dim")
     elif k_out is not None:
         raise ValueError("rotary: k_out without k")
-    return q_out, k_out, tokens, dim, (hq, ho, hk, hko)
-
-
-def rotary(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor, positions: torch.Tensor | None = None,
-           pairs: str = "half", mscale: float = 1.0, inverse: bool = False, q_out: torch.Tensor | None = None,
-           k_out: torch.Tensor | None = None, stream=None):
-    """(q, k) [tokens, heads, head_dim] turned by positions * inv_freq (positions None: 0, 1, ..); k may be
-    None. The first 2 * len(inv_freq) values of a head turn, the rest are copied. inverse: the adjoint
-    (turned back, scaled by the same mscale). q_out / k_out may be q / k."""
-    q_out, k_out, tokens, dim, heads = _tensors(q, k, inv_freq, pairs, q_out, k_out, stream)
-    wide = 0
-    if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (tokens,) \
-                or not positions.is_contiguous() or not positions.is_cuda:
-            raise ValueError("rotary: positions are a contiguous int32 or int64 [tokens] device tensor")
-        wide = int(positions.dtype == torch.int64)
-    check(lib().r97q_rotary(*heads, tokens, dim, 2 * inv_freq.shape[0], PAIRS[pairs], _ptr(inv_freq),
+    if _axes is not None:  # rotary_axes's call: its positions and pairs' axes, checked
+        check(lib().r97q_rotary_axes(hq, ho, hk, hko, tokens, dim, 2 * inv_freq.shape[0], PAIRS[pairs], _ptr(inv_freq), *_axes,
+                                     float(mscale), int(bool(inverse)), _stream(stream)), "r97q_rotary_axes")
+        return q_out, k_out
+    check(lib().r97q_rotary(hq, ho, hk, hko, tokens, dim, 2 * inv_freq.shape[0], PAIRS[pairs], _ptr(inv_freq),
                             _ptr(positions), wide, float(mscale), int(bool(inverse)), _stream(stream)), "r97q_rotary")
     return q_out, k_out
 
@@ -111,13 +109,10 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor,
     for t in (k, inv_freq, positions, pair_axis, q_out, k_out):
         if t is not None and t.get_device() != device:
             raise ValueError("rotary_axes: all tensors are on q's device")
-    q_out, k_out, tokens, dim, heads = _tensors(q, k, inv_freq, pairs, q_out, k_out, stream)
-    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 2 or positions.shape[1] != tokens \
-            or (tokens > 1 and positions.stride(1) != 1) or not positions.is_cuda:
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 2 or positions.shape[1] != q.shape[0] \
+            or (positions.shape[1] > 1 and positions.stride(1) != 1) or not positions.is_cuda:
         raise ValueError("rotary_axes: positions are an int32 or int64 [axes, tokens] device tensor, tokens consecutive")
     if pair_axis.dtype != torch.int32 or pair_axis.shape != inv_freq.shape or not pair_axis.is_contiguous() or not pair_axis.is_cuda:
         raise ValueError("rotary_axes: pair_axis is a contiguous int32 device tensor of inv_freq's shape")
-    check(lib().r97q_rotary_axes(*heads, tokens, dim, 2 * inv_freq.shape[0], PAIRS[pairs], _ptr(inv_freq), _ptr(pair_axis),
-                                 positions.shape[0], _ptr(positions), int(positions.dtype == torch.int64), positions.stride(0),
-                                 float(mscale), int(bool(inverse)), _stream(stream)), "r97q_rotary_axes")
-    return q_out, k_out
+    return rotary(q, k, inv_freq, positions, pairs, mscale, inverse, q_out, k_out, stream,
+                  _axes=(_ptr(pair_axis), positions.shape[0], _ptr(positions), int(positions.dtype == torch.int64), positions.stride(0)))
