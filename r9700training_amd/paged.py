@@ -16,12 +16,6 @@ from . import AttnShape, Pages, _device, _empty, _empty_like, _ptr, _space, _str
 from .attention import _check_lse, _heads, _index, _lse_shape
 
 
-def _beside(device, *tensors):
-    for t in tensors:
-        if t.get_device() != device:
-            raise ValueError("paged: all tensors are on the new tokens' device")
-
-
 def _cache(q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, max_kv=None, causal=0, window=0, scale=1.0, stream=None):
     """(shape, pages) of a call whose new tokens are shaped like q."""
     packed = q_starts is not None
@@ -32,10 +26,11 @@ def _cache(q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, max_kv=Non
     if page_table.dtype != torch.int32 or len(ts) != 2 or (ts[1] > 1 and st[1] != 1):
         raise ValueError("paged: page_table is an int32 [batch, most pages] device tensor, a row's entries consecutive")
     device = _device(q, stream, "paged")
-    _beside(device, k_pages, v_pages, page_table, kv_lens)
+    if k_pages.get_device() != device or v_pages.get_device() != device or page_table.get_device() != device \
+            or kv_lens.get_device() != device or (packed and q_starts.get_device() != device):
+        raise ValueError("paged: the pages, the table, the lengths and the starts are on the new tokens' device")
     batch, starts, tokens = ts[0], None, 0
     if packed:
-        _beside(device, q_starts)
         starts = _index(q_starts, batch + 1, "q_starts").data_ptr()
         if max_q is None:
             raise ValueError("paged: packed tokens need max_q, the longest sequence's")
@@ -53,10 +48,9 @@ def paged_write(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None, max_
     """The new tokens' keys and values (bf16 or f32) into the pools: the last n of a sequence's kv_lens tokens are its n new
     ones. Tokens before the sequence or without a page are left out."""
     packed = q_starts is not None
-    if v.shape != k.shape:
-        raise ValueError("paged: v has k's shape")
+    if v.shape != k.shape or v.get_device() != k.get_device():
+        raise ValueError("paged: v has k's shape and device")
     s, p = _cache(k, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, stream=stream)
-    _beside(k.get_device(), v)
     check(lib().r97q_paged_write(s, p, _heads(k, packed, "k"), _heads(v, packed, "v"), _heads(k_pages, False, "k_pages"),
                                  _heads(v_pages, False, "v_pages"), _stream(stream)), "r97q_paged_write")
 
@@ -78,7 +72,8 @@ def paged_attention_fwd(q, k_pages, v_pages, page_table, kv_lens, causal: bool =
     if lse is None:
         lse = _empty(_lse_shape(qs, packed), torch.float32, q.device, stream)
     _check_lse(lse, qs, packed)
-    _beside(q.get_device(), out, lse)
+    if out.get_device() != q.get_device() or lse.get_device() != q.get_device():
+        raise ValueError("paged: out and lse are on q's device")
     hq, hk = _heads(q, packed, "q"), _heads(k_pages, False, "k_pages")
     if workspace is None:
         need = lib().r97q_paged_attn_fwd_workspace_bytes(s, p, hq.heads, hk.heads)
