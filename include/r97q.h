@@ -710,8 +710,8 @@ int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R9
                         int64_t workspace_bytes, R97IqrStream stream);
 /* The adjoint, from the forward's inputs and states and the cotangents d_h and d_last f32 [batch][channels] (NULL: zeros):
  * dx, dgate, dinput_gate (with input_gate), drate f32 [channels], summed over all tokens, and dh0 f32 [batch][channels] (may
- * be NULL) are written, over none of the inputs. Where a decay is one (a rate of zero, a gate far below zero) the derivative through sqrt(1 - a^2),
- * which has no bound there, counts as zero. Packed tokens outside every sequence are not written. Repeated calls give the
+ * be NULL) are written, over none of the inputs. Where a decay is one (a rate of zero, a gate far below zero) the derivative
+ * through sqrt(1 - a^2), which has no bound there, counts as zero. Packed tokens outside every sequence are not written. Repeated calls give the
  * same bits. The workspace (on 16 bytes) holds the ranges' joins and the rate's partial sums. */
 int64_t r97q_recurrence_bwd_workspace_bytes(const R97qRecurrence* shape);
 int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R97qRows* gate, const R97qRows* input_gate,

@@ -451,9 +451,10 @@ struct PageRows : PageTable {
     u32x4 pool;            // near: the pool from the head on
     uint64_t base, page;   // the head in page 0; bytes from page to page
     uint32_t ts, tail;
-    __device__ __forceinline__ PageRows(const Args& a, const Seq& s, const Heads& t, int h, int row0, int from_, int rows, int d, uint32_t lds, bool leads_)
-        : PageTable(a, s, row0, from_, rows, lds, leads_), base(reinterpret_cast<uint64_t>(t.data) + 2 * h * t.hs), page(2 * t.bs), ts((uint32_t)(2 * t.ts)),
-          tail(2 * d) {
+    __device__ __forceinline__ PageRows(const Args& a, const Seq& s, const Heads& t, int h, int row0, int from_, int rows, int d,
+                                        uint32_t lds, bool leads_)
+        : PageTable(a, s, row0, from_, rows, lds, leads_), base(reinterpret_cast<uint64_t>(t.data) + 2 * h * t.hs), page(2 * t.bs),
+          ts((uint32_t)(2 * t.ts)), tail(2 * d) {
         if constexpr (MODE != kFarPages) {
             const uint32_t n = pages > 0 ? (uint32_t)(pages - 1) * (uint32_t)page + (uint32_t)(size() - 1) * ts + tail : 0u;
             pool = (u32x4){(uint32_t)uniform((int)base), (uint32_t)uniform((int)(base >> 32)), (uint32_t)uniform((int)n), 0x00020000u};
@@ -461,7 +462,9 @@ struct PageRows : PageTable {
         }
     }
     // near: the entry as an offset
-    __device__ __forceinline__ void place() { ent = (uint32_t)ent < (uint32_t)pages ? (int)((uint32_t)ent * (uint32_t)page) : (int)kNearBytes; }
+    __device__ __forceinline__ void place() {
+        ent = (uint32_t)ent < (uint32_t)pages ? (int)((uint32_t)ent * (uint32_t)page) : (int)kNearBytes;
+    }
     __device__ __forceinline__ void turn() {
         if (!PageTable::turn()) return;
         if constexpr (MODE != kFarPages) place();
@@ -473,8 +476,8 @@ struct PageRows : PageTable {
         const int left = end - (int)at;
         const uint64_t p = base + (uint64_t)e * page + (int64_t)((int)(at & (size() - 1)) - first) * ts;
         const uint32_t n = (uint32_t)(first + (left < R ? left : R) - 1) * ts + tail;
-        return (u32x4){(uint32_t)uniform((int)p), (uint32_t)uniform((int)(p >> 32)), (uint32_t)uniform(e < (uint32_t)pages && left > 0 ? (int)n : 0),
-                       0x00020000u};
+        return (u32x4){(uint32_t)uniform((int)p), (uint32_t)uniform((int)(p >> 32)),
+                       (uint32_t)uniform(e < (uint32_t)pages && left > 0 ? (int)n : 0), 0x00020000u};
     }
 };
 

@@ -133,11 +133,16 @@ struct Io<T, true> {
           row((uint32_t)(a.channels * sizeof(T))), off(mine ? first * ts + c0 * (uint32_t)sizeof(T) : kNowhere) {}
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(int64_t t0, int64_t end, int rows) const {
         const int left = end - t0 < rows ? (int)(end - t0) : rows;
-        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base + t0 * ts), 0, left > 0 ? (int)((left - 1) * ts + row) : 0, 0x00020000);
+        const int bytes = left > 0 ? (int)((left - 1) * ts + row) : 0;
+        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base + t0 * ts), 0, bytes, 0x00020000);
     }
     // (offsets are formed where they are used: held through the loop they would take a register for every token)
-    __device__ __forceinline__ u32x4 load(__amdgpu_buffer_rsrc_t buf, int k) const { return __builtin_amdgcn_raw_buffer_load_b128(buf, off + k * fresh(ts), 0, 0); }
-    __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t buf, int k, const u32x4& v) const { __builtin_amdgcn_raw_buffer_store_b128(v, buf, off + k * fresh(ts), 0, 0); }
+    __device__ __forceinline__ u32x4 load(__amdgpu_buffer_rsrc_t buf, int k) const {
+        return __builtin_amdgcn_raw_buffer_load_b128(buf, off + k * fresh(ts), 0, 0);
+    }
+    __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t buf, int k, const u32x4& v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(v, buf, off + k * fresh(ts), 0, 0);
+    }
 };
 template <class T>
 struct Io<T, false> {
@@ -274,7 +279,7 @@ struct Place {
         b = blockIdx.z;
         none = false;
         if (a.dealt) {
-            const uint32_t slabs = (a.channels + kSlab - 1) / kSlab, each = gridDim.x / 8, i = blockIdx.x % 8 * each + blockIdx.x / 8, j = i / slabs;
+            const uint32_t slabs = (a.channels + kSlab - 1) / kSlab, i = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8, j = i / slabs;
             none = i >= slabs * ranges * a.batch;
             slab = (int)(i - j * slabs);
             b = (int)(j / ranges);
@@ -439,14 +444,16 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
     if (at.range == 0) {
         if (a.first) h = a.ranges > 1 ? a.kept[mine] : a.first[mine];
     } else {
-        h = through(a.spans + (int64_t)at.b * a.ranges * a.fine * a.channels + at.near, a.channels, at.range * a.fine, at.wave, at.lane, spans[0]);
+        h = through(a.spans + (int64_t)at.b * a.ranges * a.fine * a.channels + at.near, a.channels, at.range * a.fine, at.wave, at.lane,
+                    spans[0]);
     }
     float rate[VC];
 #pragma unroll
     for (int j = 0; j < VC; ++j) rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e;
     const int first = at.wave * WT + at.g * TL;  // the thread's first token in a tile
     using IO = Io<T, WIDE>;
-    const IO xs(a.x, a, s, at.b, first, at.c0, at.mine), gs(a.g, a, s, at.b, first, at.c0, at.mine), is(a.i, a, s, at.b, first, at.c0, at.mine), hs(a.h, a, s, at.b, first, at.c0, at.mine);
+    auto io = [&](const Rows& t) { return IO(t, a, s, at.b, first, at.c0, at.mine); };
+    const IO xs = io(a.x), gs = io(a.g), is = io(a.i), hs = io(a.h);
 
     struct Raw {
         u32x4 x[TL], g[TL], i[TL];
@@ -558,8 +565,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     for (int j = 0; j < VC; ++j) rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e, dr[j] = 0.0f;
     const int first = at.wave * WT + at.g * TL;
     using IO = Io<T, WIDE>;
-    const IO xs(a.x, a, s, at.b, first, at.c0, at.mine), gs(a.g, a, s, at.b, first, at.c0, at.mine), is(a.i, a, s, at.b, first, at.c0, at.mine), es(a.h, a, s, at.b, first, at.c0, at.mine);
-    const IO dxs(a.dx, a, s, at.b, first, at.c0, at.mine), dgs(a.dg, a, s, at.b, first, at.c0, at.mine), dis(a.di, a, s, at.b, first, at.c0, at.mine);
+    auto io = [&](const Rows& t) { return IO(t, a, s, at.b, first, at.c0, at.mine); };
+    const IO xs = io(a.x), gs = io(a.g), is = io(a.i), es = io(a.h), dxs = io(a.dx), dgs = io(a.dg), dis = io(a.di);
 
     struct Raw {
         u32x4 x[TL], g[TL], i[TL], e[TL];
@@ -567,7 +574,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     };
     auto fetch = [&](Raw& r, int64_t to) {  // nothing before the beginning
         const int64_t t0 = to >= begin ? to : begin, upto = !WIDE || to >= begin ? end : begin;
-        const auto x = xs.buffer(t0, upto, TILE), g = gs.buffer(t0, upto, TILE), i = is.buffer(t0, upto, TILE), e = es.buffer(t0, upto, TILE);
+        const auto x = xs.buffer(t0, upto, TILE), g = gs.buffer(t0, upto, TILE);
+        const auto i = is.buffer(t0, upto, TILE), e = es.buffer(t0, upto, TILE);
 #pragma unroll
         for (int k = 0; k < TL; ++k) {
             r.g[k] = gs.load(g, k);
@@ -682,7 +690,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
                 dg[j] = -kLn2 * rate[j] * __builtin_fmaf(-sg[k][j], d, d);
                 dx[j] = l * in[k][j];
                 if constexpr (GATED) di[j] = dx[j] * __builtin_fmaf(-x, si[k][j], x);
-                    }
+            }
             dxs.store(bx, k, pack<T>(dx));
             dgs.store(bg, k, pack<T>(dg));
             if constexpr (GATED) dis.store(bi, k, pack<T>(di));
@@ -763,7 +771,9 @@ __device__ __forceinline__ void few_store(const Rows& t, int64_t base, int64_t t
     }
     __builtin_memcpy(reinterpret_cast<T*>(t.p) + base + token * t.ts + c0, &o, sizeof(o));
 }
-__device__ __forceinline__ int64_t base_of(const Rows& t, const Args& a, const Span& s, int b) { return a.starts ? s.base * t.ts : b * t.bs; }
+__device__ __forceinline__ int64_t base_of(const Rows& t, const Args& a, const Span& s, int b) {
+    return a.starts ? s.base * t.ts : b * t.bs;
+}
 
 template <class T, int V, bool GATED>
 __global__ __launch_bounds__(kFewThreads) void recurrence_few_fwd_kernel(Args a) {
@@ -950,7 +960,8 @@ Rows rows_of(const R97qRows* t) { return t ? Rows{static_cast<uint8_t*>(t->data)
 // whether a launch's workgroups are dealt by XCD
 bool lines_shared(const R97qRecurrence* p, const R97qRows* x, const Args& a) {
     const int64_t size = p->dtype == R97Q_F32 ? 4 : 2, slabs = (p->channels + kSlab - 1) / kSlab;
-    return slabs >= 4 && slabs * a.ranges * a.fine * a.batch <= (1 << 20) && ((reinterpret_cast<uintptr_t>(x->data) | (uintptr_t)(x->token_stride * size)) & 127);
+    const bool off = (reinterpret_cast<uintptr_t>(x->data) | (uintptr_t)(x->token_stride * size)) & 127;
+    return off && slabs >= 4 && slabs * a.ranges * a.fine * a.batch <= (1 << 20);
 }
 
 // pieces: a tile's rows lie within 31 bits of its first
@@ -1165,7 +1176,8 @@ int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     if (rows > 0)
         if (int e = shape->dtype == R97Q_F32 ? pick<float>(a, true, w, st) : pick<uint16_t>(a, true, w, st)) return e;
     if (rows == 1) return R97Q_OK;
-    hipLaunchKernelGGL(recurrence_rate_kernel, dim3((unsigned)((a.channels + 63) / 64)), dim3(64 * kShares), 0, st, a.drate, drate, rows, a.channels);
+    hipLaunchKernelGGL(recurrence_rate_kernel, dim3((unsigned)((a.channels + 63) / 64)), dim3(64 * kShares), 0, st, a.drate, drate, rows,
+                       a.channels);
     return launch_status("recurrence_rate_kernel");
 }
 
