@@ -21,10 +21,10 @@
 //
 // Measured, us and TB/s of the tensors read and written once (a copy of 1 GiB reaches 5.0), with a gate on the input:
 //                        bf16 forward   backward     f32 forward    backward
-//   8 x 2048 x 2048         65  4.1     120  3.9      118  4.5      233  4.0     256 workgroups, no ranges
-//   8 x 2048 x 2047         66  4.1     117  4.0      107  5.0      255  3.7     rows of every alignment
-//   8 x 2048 x 1024         50  2.7      76  3.1       84  3.2      145  3.2     two ranges
-//   1 x 16384 x 2048       111  2.4     146  3.2      193  2.8      288  3.3     eight ranges
+//   8 x 2048 x 2048         65  4.1     120  3.9      118  4.5      212  4.4     256 workgroups, no ranges
+//   8 x 2048 x 2047         66  4.1     117  4.0      108  5.0      219  4.3     rows of every alignment
+//   8 x 2048 x 1024         50  2.7      76  3.1       85  3.2      131  3.6     two ranges
+//   1 x 16384 x 2048       111  2.4     146  3.2      194  2.8      262  3.6     eight ranges
 //   32 x 16 x 4096          10  1.7      20  1.5       12  2.8       25  2.3     a thread a sequence
 //
 // Numbers. All is f32 but the inputs' and outputs' type. A state may last for thousands of tokens of decays next to one,
@@ -540,11 +540,15 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
 // ---------------------------------------------------------------- backward
 // The tiles from the last to the first, kChunk tokens each: the state before a tile is the forward's, the cotangent behind
 // it is carried. Bound by memory with some 65 vector instructions a value beside it: 1 x 16384 x 2048 bf16 105 us of the call's
-// 146. f32 with a gate on the input spills 29 registers: 8 x 2048 x 2048 4.0 TB/s, and 4.7 without that gate.
+// 146. f32 8 x 2048 x 2048 4.4 TB/s, without a gate on the input 4.7.
 template <class T, bool GATED, bool WIDE>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     constexpr int VC = kVC<T>, TL = 16 / VC, WT = VC * TL, TILE = kWaves * WT;
     static_assert(TILE == kChunk, "a tile begins at a kept state");
+    // Of f32 with a gate on the input not all that the first half forms fits the registers next to two tiles of inputs: what comes
+    // of a, sg and in alone is formed again. 8 x 2048 x 2048 212 us (11 registers still
+    // spilled), with all of it kept and 29 spilled 233.
+    constexpr bool AGAIN = sizeof(T) == 4 && GATED;
     __shared__ float2 spans[2][kWaves][64];
     __shared__ float backs[2][kWaves][64];
     const Place<T, WIDE> at(a, a.ranges);
@@ -598,7 +602,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
             }
         }
         // a, the gates, what x enters by (sqrt(q) sigmoid(i)) and what it takes from dlog a (a sigmoid(i) / sqrt(q))
-        float dec[TL][VC], sg[TL][VC], si[TL][VC], in[TL][VC], near[TL][VC], y[VC], u[VC], v[VC];
+        constexpr int KEPT = AGAIN ? 1 : TL;
+        float dec[TL][VC], sg[TL][VC], si[KEPT][VC], in[TL][VC], near[KEPT][VC], y[VC], u[VC], v[VC];
 #pragma unroll
         for (int j = 0; j < VC; ++j) {
             y[j] = u[j] = v[j] = 0.0f;
@@ -612,11 +617,15 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
                 // where nothing decays the root's derivative counts as none
                 const float inv = q >= 0x1p-126f ? __builtin_amdgcn_rsqf(q) : q * 0.0f;
                 in[k][j] = q * inv;
-                near[k][j] = dec[k][j] * inv;
-                if constexpr (GATED) {
-                    si[k][j] = sigmoid<T>(value<T>(now.i[k], j));
-                    in[k][j] *= si[k][j];
-                    near[k][j] *= si[k][j];
+                if constexpr (AGAIN) {
+                    in[k][j] *= sigmoid<T>(value<T>(now.i[k], j));
+                } else {
+                    near[k][j] = dec[k][j] * inv;
+                    if constexpr (GATED) {
+                        si[k][j] = sigmoid<T>(value<T>(now.i[k], j));
+                        in[k][j] *= si[k][j];
+                        near[k][j] *= si[k][j];
+                    }
                 }
                 u[j] = __builtin_fmaf(dec[k][j], u[j], in[k][j] * value<T>(now.x[k], j));
             }
@@ -654,6 +663,11 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
         // the inputs are taken apart again: both forms would not fit the registers
 #pragma unroll
         for (int k = 0; k < TL; ++k) asm volatile("" : "+v"(now.x[k]), "+v"(now.e[k]));
+        if constexpr (AGAIN)
+#pragma unroll
+            for (int k = 0; k < TL; ++k)
+#pragma unroll
+                for (int j = 0; j < VC; ++j) asm volatile("" : "+v"(sg[k][j]));
 #pragma unroll
         for (int i = 0; i < VC; ++i) {
             const float x = before;
@@ -685,11 +699,21 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
             for (int j = 0; j < VC; ++j) {
                 const float l = value<T>(now.e[k], j) + v[j], x = value<T>(now.x[k], j);
                 v[j] = dec[k][j] * l;
-                const float d = sg[k][j] * (v[j] * __builtin_fmaf(-near[k][j], x, was[k][j]));
+                float open = 1.0f, part;
+                if constexpr (AGAIN) {
+                    const float q = room(rate[j] * sg[k][j], dec[k][j]);
+                    const float inv = q >= 0x1p-126f ? __builtin_amdgcn_rsqf(q) : q * 0.0f;
+                    open = in[k][j] * inv;
+                    part = dec[k][j] * open * inv;
+                } else {
+                    part = near[k][j];
+                    if constexpr (GATED) open = si[k][j];
+                }
+                const float d = sg[k][j] * (v[j] * __builtin_fmaf(-part, x, was[k][j]));
                 dr[j] -= d;
                 dg[j] = -kLn2 * rate[j] * __builtin_fmaf(-sg[k][j], d, d);
                 dx[j] = l * in[k][j];
-                if constexpr (GATED) di[j] = dx[j] * __builtin_fmaf(-x, si[k][j], x);
+                if constexpr (GATED) di[j] = dx[j] * __builtin_fmaf(-x, open, x);
             }
             dxs.store(bx, k, pack<T>(dx));
             dgs.store(bg, k, pack<T>(dg));
