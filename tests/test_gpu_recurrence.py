@@ -295,6 +295,32 @@ def test_nan_and_infinity_stay_in_their_channel():
                 assert torch.equal(a[mask], b[mask])
 
 
+@pytest.mark.parametrize("n,token_stride", [(2100, 1 << 20), (300, 1 << 23), (5, 1 << 29)])
+@pytest.mark.parametrize("batch", [1, 2])
+def test_offsets_past_32_bits(batch, n, token_stride):
+    """Tokens far apart in one tensor of gigabytes: the bits of rows next to each other."""
+    from r9700training_amd.recurrence import recurrence_bwd, recurrence_fwd
+
+    c = 64
+    memory = torch.empty(n * token_stride + 8192, dtype=BF, device="cuda")
+    places = iter(range(0, 8192, c))
+
+    def far(t=None):
+        at = next(places) * batch
+        v = memory.as_strided((batch, n, c), (c, token_stride, 1), at)
+        return v.copy_(t) if t is not None else v
+
+    near = [rnd(40 + i, batch, n, c, dtype=BF) for i in range(4)]
+    rate, h0, d_last = rates(3, c), rnd(4, batch, c), rnd(5, batch, c)
+    h, last, states = recurrence_fwd(near[0], near[1], rate, near[2], h0=h0, want_states=True)
+    want = (h, last) + recurrence_bwd(near[0], near[1], rate, states, near[3], near[2], d_last=d_last)
+    x, gate, gi, d_h = (far(t) for t in near)
+    h, last, states = recurrence_fwd(x, gate, rate, gi, h0=h0, want_states=True, out=far())
+    got = (h, last) + recurrence_bwd(x, gate, rate, states, d_h, gi, d_last=d_last, dx=far(), dgate=far(), dinput_gate=far())
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("batch,n,c", [(4, 1, 256), (1, 3000, 64)])
 def test_streams_and_graphs(batch, n, c):
     """On a stream of its own, and both directions captured and replayed with the program's own work between, while an eager
