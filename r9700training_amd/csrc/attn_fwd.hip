@@ -546,6 +546,28 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
 // 24, over 1024 keys 22 / 19 / 16 / 14 / 15; 200 rows over 2000 keys, heads of 64 28 / 21 / 16 / 14 / 15; but 1300 tokens, 16
 // over 4 heads 28 / 35 / 45 / 57, and 512 tokens 15 / 20 / 22 / 30. One token, 24 over 4 heads of 256, 1024 keys 19 / 17 / 15 /
 // 14 and 512 keys 14 / 15 / 14 / 13; 32 over 8 heads of 128, 1024 keys 10 / 12 / 11 / 11.
+// A chunk of new tokens over a long cache has more keys than the sequences above, so ranges of 1024 and more pay where they bring
+// a second workgroup to a compute unit (up to 128 columns) or fill a second round. Measured, us at 1 / 2 / 3 / 4 / 6 / 8 ranges,
+// 16 over 4 heads, of so many workgroups of 128 rows without ranges. Heads of 64 over 8192 keys, 64: 108 / 66 / 51 / 43 / 45 / 39,
+// 128: 108 / 70 / 67 / 59 / 66 / 61, 164: 110 / 88 / 71 / 81 / 76 / 84, 200: 110 / 92 / 99 / 96, 256: 114 / 100 / 114; of 128, 64:
+// 136 / 84 / 64 / 57 / 59 / 54, 128: 136 / 92 / 96 / 86 / 96 / 94, 164: 139 / 126 / 106 / 118, 200: 139 / 135 / 145, 256: 149 / 153 /
+// 169, over 16384 289 / 276 / 282, over 4096 77 / 93 / 96, and 144: 74 / 72 / 59 / 68; over 6000, 88: 102 / 70 / 71 / 62 / 72 / 63.
+// Heads of 256 (one workgroup a compute unit) over 8192 keys, 128: 265 / 171 / 218 / 177, 164: 266 / 300 / 229 / 250, 200: 267 /
+// 304 / 302; over 6000, 88: 193 / 124 / 143 / 134. Packed sequences are uneven, where ranges do more: four of up to 5000 keys,
+// 216: heads of 64 73 / 57 / 56 / 57, of 128 96 / 79 / 81 / 85; but two, 152: 74 / 68 / 78 / 72 (3 are taken).
+[[maybe_unused]] int64_t chunk_ranges(const Args& a, int64_t have, int64_t most) {
+    int64_t n = 512 / have;
+    if (a.d > 128) return n == 3 && most >= 3 * 1280 ? 3 : 1;
+    if (have <= 128) {
+        if (n > most / 1024) n = most / 1024;
+        int64_t p = 1;  // the powers of two were the faster ones
+        while (2 * p <= n) p *= 2;
+        return p;
+    }
+    if (n > most / 1280) n = most / 1280;
+    return n == 2 && !a.q_starts && most < (a.d <= 64 ? 4096 : 12288) ? 1 : n;
+}
+
 struct Plan {
     bool few;
     int splits, chunk;
@@ -570,8 +592,13 @@ Plan plan_of(const Args& a) {
     } else {
         unit = have > 16 ? 512 : most < 512 ? most + 1 : most < 1024 ? 128 : most < 4096 ? most / 8 : 512;
         if (have > 0 && have * 2 <= 256) n = (256 + have - 1) / have;
+        if (kPaged && a.d > 128 && n > 1) n = 256 / have;
     }
     if (n > most / unit) n = most / unit;
+    if (kPaged && !p.few && have > 0 && have <= 256) {
+        const int64_t longer = chunk_ranges(a, have, most);
+        if (longer > n) n = longer;
+    }
     if (n > kMostSplits) n = kMostSplits;
     // a workgroup for each range of each head in a grid, and the join's of up to 1024 threads for each query head
     if (n > most_groups(256) / ((int64_t)a.batch * a.hk)) n = most_groups(256) / ((int64_t)a.batch * a.hk);

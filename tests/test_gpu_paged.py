@@ -100,6 +100,9 @@ CASES = [
     ([520], [6000], 12, 2, 128, 64, True, 1000),
     ([64], [9000], 16, 4, 64, 16, True, 0),
     ([600], [1111], 6, 2, 72, 1024, True, 0),
+    ([1200], [4000], 16, 4, 64, 64, True, 0),             # chunks that fill the card, cut into ranges all the same
+    ([1024], [4100], 16, 4, 128, 16, True, 0),
+    ([1300], [4200], 16, 4, 256, 64, True, 0),
 ]
 
 
@@ -132,6 +135,8 @@ PACKED = [
     ([300, 17, 1], [3000, 17, 4000], 4, 4, 64, 8, 100),
     ([5, 100], [3, 60], 4, 2, 80, 32, 0),                 # more new tokens than the cache has room for
     ([0, 0], [7, 0], 2, 1, 64, 16, 0),
+    ([700, 400, 1, 250], [5000, 900, 30, 2600], 16, 4, 64, 32, 0),
+    ([900, 300, 0, 500], [3000, 301, 9, 2600], 16, 4, 64, 16, 2700),
 ]
 
 
