@@ -442,7 +442,7 @@ struct PageTable {
 // How a pool's pages are reached: one buffer with a page's offset in it, where the pool is less than 2 GiB, a tile's page looked
 // up once (kWholePages: they hold a tile) or a wave's piece at a time (kSmallPages: of a tile's first one on); else a piece's
 // page as a buffer of its own (kFarPages). What a step does for it counts, since no product runs beside it: 2048 tokens over
-// 16384, 16 over 4 heads of 128, 277 us over rows, 286 over pages of 64, of 16 and of 8 some 2% more; with every piece's page
+// 16384, 16 over 4 heads of 128, 277 us over rows, 286 over pages of 64, of 16 and of 8 some 2% more (275 in two ranges); with every piece's page
 // and bounds worked out in scalars 374 (64), and with the next entries an ordinary load 415.
 enum { kWholePages, kSmallPages, kFarPages };
 constexpr uint32_t kNearBytes = 0x7FFFFFF0u;  // a near pool's end at most: an offset for entries outside the pool

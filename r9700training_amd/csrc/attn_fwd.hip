@@ -539,14 +539,7 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
 }
 #endif
 
-// How a shape is cut: rows a workgroup, ranges of the keys. A range writes its sums and a second launch (some 5 us) joins
-// them, so only where compute units would be idle. Measured (us at 1 / 2 / 4 / 8 / 16 / 32 ranges): one token, 24 over 4
-// heads of 256, 32768 keys 601 / 312 / 168 / 98 / 63 / 43 (64: 39); 16 sequences of 1 .. 4096 keys, 32 over 8 heads of 128
-// 58 / 47 / 44 / 46 / 52 / 67, all of 4096 keys 45 / 49 / 49 / 50 / 54 / 72; 64 rows over 4096 keys 67 / 42 / 29 / 23 / 22 /
-// 24, over 1024 keys 22 / 19 / 16 / 14 / 15; 200 rows over 2000 keys, heads of 64 28 / 21 / 16 / 14 / 15; but 1300 tokens, 16
-// over 4 heads 28 / 35 / 45 / 57, and 512 tokens 15 / 20 / 22 / 30. One token, 24 over 4 heads of 256, 1024 keys 19 / 17 / 15 /
-// 14 and 512 keys 14 / 15 / 14 / 13; 32 over 8 heads of 128, 1024 keys 10 / 12 / 11 / 11.
-// A chunk of new tokens over a long cache has more keys than the sequences above, so ranges of 1024 and more pay where they bring
+// A chunk of new tokens over a long cache has more keys than whole sequences, so ranges of 1024 and more pay where they bring
 // a second workgroup to a compute unit (up to 128 columns) or fill a second round. Measured, us at 1 / 2 / 3 / 4 / 6 / 8 ranges,
 // 16 over 4 heads, of so many workgroups of 128 rows without ranges. Heads of 64 over 8192 keys, 64: 108 / 66 / 51 / 43 / 45 / 39,
 // 128: 108 / 70 / 67 / 59 / 66 / 61, 164: 110 / 88 / 71 / 81 / 76 / 84, 200: 110 / 92 / 99 / 96, 256: 114 / 100 / 114; of 128, 64:
@@ -568,6 +561,13 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
     return n == 2 && !a.q_starts && most < (a.d <= 64 ? 4096 : 12288) ? 1 : n;
 }
 
+// How a shape is cut: rows a workgroup, ranges of the keys. A range writes its sums and a second launch (some 5 us) joins
+// them, so only where compute units would be idle. Measured (us at 1 / 2 / 4 / 8 / 16 / 32 ranges): one token, 24 over 4
+// heads of 256, 32768 keys 601 / 312 / 168 / 98 / 63 / 43 (64: 39); 16 sequences of 1 .. 4096 keys, 32 over 8 heads of 128
+// 58 / 47 / 44 / 46 / 52 / 67, all of 4096 keys 45 / 49 / 49 / 50 / 54 / 72; 64 rows over 4096 keys 67 / 42 / 29 / 23 / 22 /
+// 24, over 1024 keys 22 / 19 / 16 / 14 / 15; 200 rows over 2000 keys, heads of 64 28 / 21 / 16 / 14 / 15; but 1300 tokens, 16
+// over 4 heads 28 / 35 / 45 / 57, and 512 tokens 15 / 20 / 22 / 30. One token, 24 over 4 heads of 256, 1024 keys 19 / 17 / 15 /
+// 14 and 512 keys 14 / 15 / 14 / 13; 32 over 8 heads of 128, 1024 keys 10 / 12 / 11 / 11.
 struct Plan {
     bool few;
     int splits, chunk;
@@ -588,7 +588,11 @@ Plan plan_of(const Args& a) {
     if (p.few) {  // lengths that differ leave workgroups idle: more of them
         const int64_t want = !a.kv_lens && !a.kv_starts ? 192 : a.d > 128 ? 256 : 512;
         unit = 128;
-        if (have > 0 && have * 3 / 2 < want && most > (a.d > 128 ? 640 : 1024)) n = (want + have - 1) / have;
+        // Nearly one for each compute unit, or short ones for half of them, are left whole: 16 over 4 heads of 128, 64 sequences of
+        // up to 3000 keys 53 us, in two ranges 59, of up to 8000 126 and 132; 56 of up to 1500 24, in three ranges 30 (of 64 columns
+        // 15 and 20); but 60 of up to 3000 48 and 47, of up to 8000 123 and 111, and 75 of up to 3000 79 and 66.
+        const bool whole = kPaged && a.d <= 128 && have >= 128 && have <= 256 && (have > 240 || most <= 2048);
+        if (have > 0 && have * 3 / 2 < want && most > (a.d > 128 ? 640 : 1024) && !whole) n = (want + have - 1) / have;
     } else {
         unit = have > 16 ? 512 : most < 512 ? most + 1 : most < 1024 ? 128 : most < 4096 ? most / 8 : 512;
         if (have > 0 && have * 2 <= 256) n = (256 + have - 1) / have;
