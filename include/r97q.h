@@ -669,9 +669,10 @@ int r97q_paged_attn_fwd(const R97qAttnShape* shape, const R97qPages* pages, cons
                         const R97qHeads* v, const R97qHeads* out, float* lse, void* workspace, int64_t workspace_bytes,
                         R97IqrStream stream);
 /* The new tokens' keys and values into the pools: the shape is the attention's that follows (its q_len or q_starts say how
- * many new tokens a sequence has, its kv_lens count them already), so token i of n goes to position kv_lens[b] - n + i. k
- * and v are both bf16 or both f32 (rounded once). A token whose position is negative or has no page is left out; what the
- * new tokens do not take of a page stays as it was. Two tokens for one place leave either. */
+ * many new tokens a sequence has, its kv_lens count them already), so token i of n goes to position kv_lens[b] - n + i, the
+ * length taken as it is, also past max_pages * page_size. k and v are both bf16 or both f32 (rounded once). A token whose
+ * position is negative, past the table or in no page of the pool is left out; what the new tokens do not take of a page
+ * stays as it was. Two tokens for one place leave values of either. */
 int r97q_paged_write(const R97qAttnShape* shape, const R97qPages* pages, const R97qHeads* k, const R97qHeads* v,
                      const R97qHeads* k_pages, const R97qHeads* v_pages, R97IqrStream stream);
 

@@ -3,8 +3,10 @@
 // Token i of a sequence's n new ones takes position m - n + i of its m: slot (position mod page size) of the page that the
 // sequence's row of the table names. Bound by memory, each value read and written once; a workgroup walks a sequence's tokens
 // in pieces of 8 values, kItems of a thread's loads out together. A token without a place (before the sequence, past the
-// table, a page outside the pool) is left out. 16384 tokens of 8 heads of 128 into pages of 64 or 16: 25 us, 5.3 TB/s (a 1 GiB
-// copy reaches 5.0; part of these tensors stays in the cache); 2048 10 us, one each of 16 sequences 9, the call's latency.
+// table, a page outside the pool) is left out: m is the length as it is given, not what the table has room for, so the
+// tokens of a sequence that has outgrown its table write over none that the cache holds. 16384 tokens of 8 heads of 128 into
+// pages of 64 or 16: 25 us, 5.3 TB/s (a 1 GiB copy reaches 5.0; part of these tensors stays in the cache); 2048 10 us, one
+// each of 16 sequences 9, the call's latency.
 #include "attn.h"
 #include "status.h"
 
@@ -20,6 +22,7 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(Args a, Heads k, 
     const int per = a.d / 8, all = 2 * a.hk * per;  // pieces of a head, and of a token's keys and values
     const int64_t n = (int64_t)s.lq * all, step = (int64_t)gridDim.x * kThreads;
     const int32_t* table = a.table + s.b * a.table_stride;
+    const int64_t off = (int64_t)uniform(a.kv_lens[s.b]) - s.lq;
     const uint8_t *kb = q_at(k, a, s, 0), *vb = q_at(v, a, s, 0);
     for (int64_t i0 = (int64_t)blockIdx.x * kThreads + threadIdx.x; i0 < n; i0 += kItems * step) {
         u32x4 w[kItems];
@@ -39,7 +42,7 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(Args a, Heads k, 
             } else {
                 w[j] = *reinterpret_cast<const u32x4*>((keys ? kb : vb) + 2 * at);
             }
-            const int pos = tok + s.off;
+            const int64_t pos = tok + off;
             const bool in = pos >= 0 && pos >> a.page_shift < a.max_pages && i0 + j * step < n;
             const int page = in ? table[pos >> a.page_shift] : -1;
             to[j] = (uint32_t)page < (uint32_t)a.pages

@@ -46,7 +46,7 @@ def _cache(q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q, max_kv=Non
 
 def paged_write(k, v, k_pages, v_pages, page_table, kv_lens, q_starts=None, max_q: int | None = None, stream=None):
     """The new tokens' keys and values (bf16 or f32) into the pools: the last n of a sequence's kv_lens tokens are its n new
-    ones. Tokens before the sequence or without a page are left out."""
+    ones. Tokens before the sequence, past the table's room or without a page are left out."""
     packed = q_starts is not None
     if v.shape != k.shape or v.get_device() != k.get_device():
         raise ValueError("paged: v has k's shape and device")

@@ -399,3 +399,66 @@ def test_nothing_to_do():
     # a table without an entry
     out, lse = paged_attention_fwd(rnd(1, 2, 3, 4, 64), c.k, c.v, c.table[:, :0], c.kv_lens)
     assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def past(new, lens, heads, d, page, entries, packed=False, dtype=BF):
+    """Pools of finite values, new tokens of sequences whose table has so many entries, and the pools after the write."""
+    pages = len(lens) * entries + 2
+    pools = [rnd(60 + i, pages, page, heads, d) for i in range(2)]
+    ids = torch.randperm(pages, generator=torch.Generator().manual_seed(5))[:len(lens) * entries].reshape(len(lens), entries)
+    starts = torch.tensor([0] + list(new)).cumsum(0)
+    shape = (int(starts[-1]), heads, d) if packed else (len(new), new[0], heads, d)
+    k, v = rnd(70, *shape, dtype=dtype), rnd(71, *shape, dtype=dtype)
+    want = [t.clone() for t in pools]
+    for b, (n, m) in enumerate(zip(new, lens)):
+        mine = [t[starts[b]:starts[b + 1]] if packed else t[b] for t in (k, v)]
+        for i in range(n):
+            at = m - n + i
+            if 0 <= at < entries * page:
+                for w, t in zip(want, mine):
+                    w[int(ids[b, at // page]), at % page] = t[i].to(BF)
+    kw = dict(q_starts=starts.to(torch.int32).cuda(), max_q=max(new)) if packed else {}
+    return k, v, pools, want, ids.to(torch.int32).cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), kw
+
+
+@pytest.mark.parametrize("new,lens,page,entries,packed", [
+    ([1, 1, 1], [33, 32, 2 ** 31 - 1], 16, 2, False),     # one past the table's room, its last place, and far past it
+    ([5, 5, 5], [34, 37, 38], 16, 2, False),              # the last two, all and all without a place
+    ([40, 3, 1], [60, 50, 49], 8, 6, True),
+    ([300, 1], [1100, 1025], 128, 8, True),
+])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_write_past_the_table(new, lens, page, entries, packed, dtype):
+    """A token whose position the table has no entry for is left out, and moves no other."""
+    from r9700training_amd.paged import paged_write
+
+    for heads, d in ((2, 64), (3, 80)):
+        k, v, pools, want, ids, held, kw = past(new, lens, heads, d, page, entries, packed, dtype)
+        paged_write(k, v, *pools, ids, held, **kw)
+        torch.cuda.synchronize()
+        for got, w in zip(pools, want):
+            assert torch.equal(got.view(torch.int16), w.view(torch.int16))
+
+
+def test_tokens_past_the_tables_room():
+    """A captured step of one token that is replayed until its cache is full, and on: what the cache holds stays."""
+    from r9700training_amd.paged import paged_write
+
+    k, v, pools, _, ids, held, _ = past([1, 1], [30, 31], 2, 64, 16, 2)
+    paged_write(k, v, *pools, ids, held)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        held.add_(1)
+        paged_write(k, v, *pools, ids, held)
+    held.copy_(torch.tensor([30, 31], dtype=torch.int32, device="cuda"))
+    want = [t.clone() for t in pools]
+    for i in range(6):
+        k.copy_(rnd(80 + i, 2, 1, 2, 64)), v.copy_(rnd(90 + i, 2, 1, 2, 64))
+        for b in range(2):
+            at = 30 + b + i
+            if at < 32:
+                want[0][int(ids[b, 1]), at % 16], want[1][int(ids[b, 1]), at % 16] = k[b, 0], v[b, 0]
+        g.replay()
+        torch.cuda.synchronize()
+        for got, w in zip(pools, want):
+            assert torch.equal(got.view(torch.int16), w.view(torch.int16)), i
