@@ -614,11 +614,17 @@ Plan plan_of(const Args& a) {
     return p;
 }
 
-// how a tile of `rows` keys finds its pages
+// How a tile of `rows` keys finds its pages. A place in a small page is counted from the tile's beginning, so it may begin up to a
+// tile's tokens before the pool, and with it the columns past a head, which are to read as zeros, lie that far before kNowhere:
+// then the pool ends before those.
 [[maybe_unused]] int mode_of(const Args& a, int rows) {
     if (!kPaged) return kNoPages;
-    auto near = [&](const Heads& t) { return 2.0 * ((double)(a.pages > 0 ? a.pages - 1 : 0) * t.bs + (double)((1 << a.page_shift) - 1) * t.ts + a.d) <= (double)kNearBytes; };
-    return !near(a.k) || !near(a.v) ? kFarPages : 1 << a.page_shift >= rows ? kWholePages : kSmallPages;
+    const bool whole = 1 << a.page_shift >= rows;
+    auto near = [&](const Heads& t) {
+        const double bytes = 2.0 * ((double)(a.pages > 0 ? a.pages - 1 : 0) * t.bs + (double)((1 << a.page_shift) - 1) * t.ts + a.d);
+        return bytes + (whole ? 0.0 : 2.0 * rows * t.ts) <= (double)kNearBytes;
+    };
+    return !near(a.k) || !near(a.v) ? kFarPages : whole ? kWholePages : kSmallPages;
 }
 template <int D, int KT, int NW, int PER, int MODE>
 int run_tiles(const Args& a, const Plan& p, hipStream_t st) {

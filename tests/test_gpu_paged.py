@@ -462,3 +462,27 @@ def test_tokens_past_the_tables_room():
         torch.cuda.synchronize()
         for got, w in zip(pools, want):
             assert torch.equal(got.view(torch.int16), w.view(torch.int16)), i
+
+
+@pytest.mark.parametrize("page", [8, 16])
+@pytest.mark.parametrize("new,d", [(1, 80), (100, 80), (1, 40), (90, 40), (1, 200), (70, 200), (100, 128)])
+def test_a_pool_just_under_2_GiB(new, d, page):
+    """Heads of fewer columns than their tile, in pages smaller than it: the columns past a head are zeros whatever the pool's
+    last pages hold, also where a tile's later places name the pool's first pages."""
+    from r9700training_amd.paged import paged_attention_fwd
+
+    heads, n = 8, 8 * page
+    pages = 0x7FFFFFF0 // (2 * page * heads * d)
+    k, v = (torch.zeros((pages, page, heads, d), dtype=BF, device="cuda") for _ in range(2))
+    k[8:], v[8:] = math.nan, math.nan
+    k[:8], v[:8] = rnd(1, 8, page, heads, d), rnd(2, 8, page, heads, d)
+    ids = torch.tensor([[7, 0, 1, 2, 3, 4, 5, 6], [1, 0, 3, 2, 5, 4, 7, 6]], dtype=torch.int32, device="cuda")
+    q = rnd(3, 2, new, heads, d)
+    held = torch.full((2,), n, dtype=torch.int32, device="cuda")
+    ref = R.reference([(q[b].double(), k[ids[b].long()].flatten(0, 1).double(), v[ids[b].long()].flatten(0, 1).double(), None)
+                       for b in range(2)], heads, heads, True, 0, 0.1, R.HALF[BF])
+    out, lse = paged_attention_fwd(q, k, v, ids, held, scale=0.1)
+    torch.cuda.synchronize()
+    for b, r in enumerate(ref):
+        close(out[b], *r["out"], f"out of sequence {b}")
+        close(lse[b], *r["lse"], f"lse of sequence {b}")
