@@ -979,17 +979,23 @@ int check_rows(const R97qRows* t, const R97qRecurrence* p, bool output, const ch
     return R97Q_OK;
 }
 
-Rows rows_of(const R97qRows* t) { return t ? Rows{static_cast<uint8_t*>(t->data), t->batch_stride, t->token_stride} : Rows{}; }
+// A lone sequence's and a lone token's strides say nothing. The token's is taken as a row: a tile's places past the last token
+// are told by their offsets, which have to lie past its row.
+Rows rows_of(const R97qRows* t, const R97qRecurrence* p) {
+    if (!t) return {};
+    return {static_cast<uint8_t*>(t->data), p->batch > 1 ? t->batch_stride : 0,
+            (p->starts ? p->tokens : p->len) > 1 ? t->token_stride : p->channels};
+}
 
 // whether a launch's workgroups are dealt by XCD
-bool lines_shared(const R97qRecurrence* p, const R97qRows* x, const Args& a) {
+bool lines_shared(const R97qRecurrence* p, const Args& a) {
     const int64_t size = p->dtype == R97Q_F32 ? 4 : 2, slabs = (p->channels + kSlab - 1) / kSlab;
-    const bool off = (reinterpret_cast<uintptr_t>(x->data) | (uintptr_t)(x->token_stride * size)) & 127;
+    const bool off = (reinterpret_cast<uintptr_t>(a.x.p) | (uintptr_t)(a.x.ts * size)) & 127;
     return off && slabs >= 4 && slabs * a.ranges * a.fine * a.batch <= (1 << 20);
 }
 
 // pieces: a tile's rows lie within 31 bits of its first
-bool wide(const R97qRows* t) { return !t || t->token_stride <= (1 << 20); }
+bool wide(const Rows& t) { return t.ts <= (1 << 20); }
 
 int64_t all_tokens(const R97qRecurrence* p) { return p->starts ? p->tokens : p->batch * p->len; }
 
@@ -1115,29 +1121,28 @@ int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R9
     const int64_t need = a.ranges > 1 ? spans_bytes(a) + row_bytes(a, a.batch) : 0;
     if (need > 0 && (!workspace || workspace_bytes < need)) return refuse(R97Q_EWORKSPACE, who, "the workspace is too small");
     if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return refuse(R97Q_EINVAL, who, "the workspace starts on 16 bytes");
-    a.x = rows_of(x);
-    a.g = rows_of(gate);
-    a.i = rows_of(all_tokens(shape) > 0 ? input_gate : nullptr);
-    a.h = rows_of(h);
+    a.x = rows_of(x, shape);
+    a.g = rows_of(gate, shape);
+    a.i = rows_of(all_tokens(shape) > 0 ? input_gate : nullptr, shape);
+    a.h = rows_of(h, shape);
     a.rate = rate;
     a.first = h0;
     a.last = last;
     a.states = states;
     a.spans = static_cast<float2*>(workspace);
     a.kept = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + spans_bytes(a));
-    a.dealt = lines_shared(shape, x, a);
+    a.dealt = lines_shared(shape, a);
     // The last piece's channels that are its neighbour's too are read twice, by two workgroups at times: not where one of them may
     // have written over them. Odd widths in place go value by value (8 x 2048 x 2047 forward 138 us, else 66).
     const int unit = shape->dtype == R97Q_F32 ? 4 : 8;
-    const R97qRows* ins[] = {x, gate, input_gate};
     bool over = h0 && h0 == last;
-    for (const R97qRows* in : ins) {
-        if (!in || !h->data || in->data != h->data) continue;
-        if (in->token_stride != h->token_stride || (!shape->starts && in->batch_stride != h->batch_stride))
+    for (const Rows& in : {a.x, a.g, a.i}) {
+        if (!in.p || in.p != a.h.p) continue;
+        if (in.ts != a.h.ts || (!shape->starts && in.bs != a.h.bs))
             return refuse(R97Q_EINVAL, who, "h over an input has that input's strides");
         over = true;
     }
-    const bool w = a.channels >= unit && (a.channels % unit == 0 || !over) && wide(x) && wide(gate) && wide(input_gate) && wide(h);
+    const bool w = a.channels >= unit && (a.channels % unit == 0 || !over) && wide(a.x) && wide(a.g) && wide(a.i) && wide(a.h);
     return shape->dtype == R97Q_F32 ? pick<float>(a, false, w, (hipStream_t)stream) : pick<uint16_t>(a, false, w, (hipStream_t)stream);
 }
 
@@ -1181,22 +1186,22 @@ int r97q_recurrence_bwd(const R97qRecurrence* shape, const R97qRows* x, const R9
         for (const R97qRows* other : outs) over |= out && other && out != other && out->data && other->data == out->data;
     }
     if (over) return refuse(R97Q_EINVAL, who, "an output over an input or another output");
-    a.x = rows_of(x);
-    a.g = rows_of(gate);
-    a.i = rows_of(all_tokens(shape) > 0 ? input_gate : nullptr);
-    a.h = rows_of(d_h);
-    a.dx = rows_of(dx);
-    a.dg = rows_of(dgate);
-    a.di = rows_of(dinput_gate);
+    a.x = rows_of(x, shape);
+    a.g = rows_of(gate, shape);
+    a.i = rows_of(all_tokens(shape) > 0 ? input_gate : nullptr, shape);
+    a.h = rows_of(d_h, shape);
+    a.dx = rows_of(dx, shape);
+    a.dg = rows_of(dgate, shape);
+    a.di = rows_of(dinput_gate, shape);
     a.rate = rate;
     a.first = d_last;
     a.last = dh0;
     a.states = const_cast<float*>(states);
     a.spans = static_cast<float2*>(workspace);
     a.drate = rows > 1 ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + spans_bytes(a)) : drate;
-    a.dealt = lines_shared(shape, x, a);
-    const bool w = a.channels >= (shape->dtype == R97Q_F32 ? 4 : 8) && wide(x) && wide(gate) && wide(input_gate) && wide(d_h) && wide(dx) &&
-                   wide(dgate) && wide(dinput_gate);
+    a.dealt = lines_shared(shape, a);
+    const bool w = a.channels >= (shape->dtype == R97Q_F32 ? 4 : 8) && wide(a.x) && wide(a.g) && wide(a.i) && wide(a.h) && wide(a.dx) &&
+                   wide(a.dg) && wide(a.di);
     if (rows > 0)
         if (int e = shape->dtype == R97Q_F32 ? pick<float>(a, true, w, st) : pick<uint16_t>(a, true, w, st)) return e;
     if (rows == 1) return R97Q_OK;

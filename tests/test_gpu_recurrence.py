@@ -371,3 +371,46 @@ def test_nothing_to_do():
     h, last, states = recurrence_fwd(none, none, rate, want_states=True)
     grads = recurrence_bwd(none, none, rate, states, none)
     assert last.shape == (0, 64) and (grads[3] == 0).all() and grads[2] is None
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("c", [64, 100, 3])
+@pytest.mark.parametrize("most", [1, 300, 2048])
+def test_strides_of_a_lone_token(dtype, c, most):
+    """A packed token alone, whose rows are as they come of a transposed column or an expanded one: its stride says nothing,
+    whatever length is planned for."""
+    from r9700training_amd.recurrence import recurrence_bwd, recurrence_fwd
+
+    x, gate, gi, rate, h0 = inputs(1, (1, c), dtype, True, 3, c)
+    d_h, d_last = rnd(8, 1, c, dtype=dtype), rnd(9, 3, c)
+    kw = dict(starts=torch.tensor([0, 0, 1, 1], dtype=torch.int32, device="cuda"), max_len=most)
+    h, last, states, *grads = check(x, gate, gi, rate, h0, d_h, d_last, [lambda t: t[:0], lambda t: t, lambda t: t[:0]], kw)
+
+    def turned(t):
+        return t.clone().as_strided((1, c), (1, 1))       # a column's, seen as a row
+
+    def alone(t):
+        return t.clone().as_strided((1, c), (0, 1))
+
+    for way in (turned, alone):
+        assert way(x).stride(0) < 2
+        got = recurrence_fwd(way(x), way(gate), rate, way(gi), h0=h0, out=way(torch.zeros_like(x)), want_states=True, **kw)
+        mine = recurrence_bwd(way(x), way(gate), rate, states, way(d_h), way(gi), d_last=d_last, **kw,
+                              **{name: way(torch.zeros_like(x)) for name in ("dx", "dgate", "dinput_gate")})
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], h) and torch.equal(got[1], last)
+        for a, b in zip(grads, mine):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n", [1, 5, 300])
+def test_in_place_over_strides_that_say_nothing(n):
+    """An output over an input of one sequence, or one token, whose views differ in the stride of what there is one of."""
+    from r9700training_amd.recurrence import recurrence_fwd
+
+    c = 64
+    x, gate, gi, rate, h0 = inputs(1, (1, n, c), BF, True, 1, c)
+    h, last, _ = recurrence_fwd(x, gate, rate, gi, h0=h0)
+    over = x.clone()
+    got = recurrence_fwd(over, gate, rate, gi, h0=h0, out=over.as_strided((1, n, c), (7 * c, c if n > 1 else 5 * c, 1)))
+    assert torch.equal(got[0], h) and torch.equal(over, h) and torch.equal(got[1], last)
