@@ -492,7 +492,7 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
             float most = top;
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
-                if (i0 + k * groups >= a.splits) st[k].x = -INFINITY;
+                if (i0 + k * groups >= a.splits) st[k] = make_float2(-INFINITY, 0.0f);
                 most = fmaxf(most, st[k].x);
             }
             const float turn = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - most);
@@ -500,7 +500,9 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
             top = most;
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
-                if (st[k].x == -INFINITY) continue;  // an empty range wrote no sums: its place may hold anything
+                // an empty range wrote no sums: its place may hold anything. (By its sum: of scores that are all NaN the
+                // maximum is minus infinity as well.)
+                if (st[k].y == 0.0f) continue;
                 const float f = __builtin_amdgcn_exp2f(st[k].x - top);
                 l += st[k].y * f;
                 v.x += u[k].x * f, v.y += u[k].y * f, v.z += u[k].z * f, v.w += u[k].w * f;
@@ -517,7 +519,7 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
                 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 for (int i = 0; i < groups; ++i) {
                     const float2 st = stat[tid + i * lanes];
-                    if (st.x == -INFINITY) continue;
+                    if (st.y == 0.0f) continue;
                     const float f = __builtin_amdgcn_exp2f(st.x - most);
                     const float4 u = acc[tid + i * lanes];
                     l += st.y * f;

@@ -486,3 +486,37 @@ def test_a_pool_just_under_2_GiB(new, d, page):
     for b, r in enumerate(ref):
         close(out[b], *r["out"], f"out of sequence {b}")
         close(lse[b], *r["lse"], f"lse of sequence {b}")
+
+
+@pytest.mark.parametrize("new,n,hq,hk,d", [(1, 20000, 24, 4, 256), (2, 6000, 8, 2, 128), (1, 3000, 4, 4, 64), (64, 9000, 16, 4, 64), (1, 300, 4, 2, 64)])
+def test_a_nan_query_in_ranges(new, n, hq, hk, d):
+    """A row whose scores are all NaN is NaN, in one range of the keys or many, over pages and over rows; so is one whose keys
+    are, if only in some of the ranges. The other rows are what they are without it."""
+    from r9700training_amd.attention import attention_fwd
+    from r9700training_amd.paged import paged_attention_fwd
+
+    c = Cache([n, n], hk, d, 16)
+    k, v = torch.stack(c.keys), torch.stack(c.values)
+    q = rnd(1, 2, new, hq, d)
+    bad = q.clone()
+    bad[0, new - 1, hq - 1] = math.nan
+    ref = expected(c, q, hq, hk, True, 0, 0.1, R.HALF[BF])
+    for out, lse in (paged_attention_fwd(bad, c.k, c.v, c.table, c.kv_lens, scale=0.1), attention_fwd(bad, k, v, scale=0.1)):
+        assert out[0, new - 1, hq - 1].isnan().all() and lse[0, hq - 1, new - 1].isnan()
+        for b, r in enumerate(ref):
+            (want, tol), (want_lse, tol_lse) = (tuple(t.clone() for t in r[name]) for name in ("out", "lse"))
+            o, s = out[b].clone(), lse[b].clone()
+            if b == 0:
+                for t in (want, tol, o):
+                    t[new - 1, hq - 1] = 0
+                for t in (want_lse, tol_lse, s):
+                    t[hq - 1, new - 1] = 0
+            close(o, want, tol, f"out of sequence {b}")
+            close(s, want_lse, tol_lse, f"lse of sequence {b}")
+    # every key of a part of the cache, some ranges' whole
+    k[0, :n // 2, 0] = math.nan
+    for b in range(n // 2 // 16):
+        c.k[int(c.table[0, b]), :, 0] = math.nan
+    for out, lse in (paged_attention_fwd(q, c.k, c.v, c.table, c.kv_lens, scale=0.1), attention_fwd(q, k, v, scale=0.1)):
+        assert out[0, :, :hq // hk].isnan().all() and lse[0, :hq // hk].isnan().all()
+        assert out[1].isfinite().all() and out[0, :, hq // hk:].isfinite().all()
