@@ -696,14 +696,14 @@ typedef struct R97qRows {
     int64_t batch_stride; /* unused where the sequences are packed */
     int64_t token_stride;
 } R97qRows;
-/* h (written) from x, gate, input_gate (may be NULL), rate f32 [channels], not negative, and h0 f32 [batch][channels], the
- * state before each sequence (NULL: zeros). last f32 [batch][channels] (may be NULL, may be h0): the state behind each
- * sequence, which the next tokens begin from; that of a sequence without tokens is h0. states f32 [rows][channels] (may be
- * NULL; r97q_recurrence_state_rows says how many rows): for the backward, the state before every token that is a multiple
- * of R97Q_RECURRENCE_CHUNK of its sequence, dense row b * ceil(len / CHUNK) + t / CHUNK, packed starts[b] / CHUNK + b + t /
- * CHUNK. Packed tokens outside every sequence are not written. h may be x, gate or input_gate, with its strides; no tensors
- * overlap otherwise. Few channels over many tokens are cut along the tokens and joined through the workspace (on 16 bytes,
- * often 0). Repeated calls give the same bits. */
+/* h (written) from x, gate, input_gate (may be NULL), rate f32 [channels], not negative (more than 2e+26 counts as that),
+ * and h0 f32 [batch][channels], the state before each sequence (NULL: zeros). last f32 [batch][channels] (may be NULL, may
+ * be h0): the state behind each sequence, which the next tokens begin from; that of a sequence without tokens is h0. states
+ * f32 [rows][channels] (may be NULL; r97q_recurrence_state_rows says how many rows): for the backward, the state before
+ * every token that is a multiple of R97Q_RECURRENCE_CHUNK of its sequence, dense row b * ceil(len / CHUNK) + t / CHUNK,
+ * packed starts[b] / CHUNK + b + t / CHUNK. Packed tokens outside every sequence are not written. h may be x, gate or
+ * input_gate, with its strides; no tensors overlap otherwise. Few channels over many tokens are cut along the tokens and
+ * joined through the workspace (on 16 bytes, often 0). Repeated calls give the same bits. */
 int64_t r97q_recurrence_state_rows(const R97qRecurrence* shape);
 int64_t r97q_recurrence_fwd_workspace_bytes(const R97qRecurrence* shape);
 int r97q_recurrence_fwd(const R97qRecurrence* shape, const R97qRows* x, const R97qRows* gate, const R97qRows* input_gate,

@@ -195,6 +195,12 @@ struct Piece {
 
 // ---------------------------------------------------------------- the gates
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// A channel's rate in base 2, at most 2^88: under any gate but one below -57 nothing is left of a state then, as without that bound,
+// and the shut gate of a place past the end, which in f32 is open by e^-87, decays nothing under every rate.
+__device__ __forceinline__ float rate_of(const Args& a, int c) {
+    const float r = a.rate[c] * kLog2e;
+    return r > 0x1p88f ? 0x1p88f : r;
+}
 // 1 / (1 + e^-v). The product with log2 e is off by half a step of itself, which for a far gate is more than a step of the
 // result: f32's is put right (bf16's inputs are further off), gates past 87 on either side counted as 87.
 template <class T>
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
     float rate[VC], y[VC], u[VC];
 #pragma unroll
     for (int j = 0; j < VC; ++j) {
-        rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e;
+        rate[j] = rate_of(a, at.c0 + j < a.channels ? at.c0 + j : a.channels - 1);
         y[j] = u[j] = 0.0f;
     }
     const Piece<T, WIDE> xs(BACK ? a.h : a.x, a, s, at.b, at.c0), gs(a.g, a, s, at.b, at.c0), is(a.i, a, s, at.b, at.c0);
@@ -449,7 +455,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_fwd_kernel(Args a) {
     }
     float rate[VC];
 #pragma unroll
-    for (int j = 0; j < VC; ++j) rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e;
+    for (int j = 0; j < VC; ++j) rate[j] = rate_of(a, at.c0 + j < a.channels ? at.c0 + j : a.channels - 1);
     const int first = at.wave * WT + at.g * TL;  // the thread's first token in a tile
     using IO = Io<T, WIDE>;
     auto io = [&](const Rows& t) { return IO(t, a, s, at.b, first, at.c0, at.mine); };
@@ -566,7 +572,7 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     }
     float rate[VC], dr[VC];
 #pragma unroll
-    for (int j = 0; j < VC; ++j) rate[j] = a.rate[at.c0 + j < a.channels ? at.c0 + j : a.channels - 1] * kLog2e, dr[j] = 0.0f;
+    for (int j = 0; j < VC; ++j) rate[j] = rate_of(a, at.c0 + j < a.channels ? at.c0 + j : a.channels - 1), dr[j] = 0.0f;
     const int first = at.wave * WT + at.g * TL;
     using IO = Io<T, WIDE>;
     auto io = [&](const Rows& t) { return IO(t, a, s, at.b, first, at.c0, at.mine); };
@@ -811,7 +817,7 @@ __global__ __launch_bounds__(kFewThreads) void recurrence_few_fwd_kernel(Args a)
     float rate[V], h[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        rate[j] = a.rate[c0 + j] * kLog2e;
+        rate[j] = rate_of(a, c0 + j);
         h[j] = a.first ? a.first[mine + j] : 0.0f;
     }
     constexpr int TL = 4;
@@ -859,7 +865,7 @@ __global__ __launch_bounds__(kFewThreads) void recurrence_few_bwd_kernel(Args a)
     float rate[V], m[V], dr[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        rate[j] = a.rate[c0 + j] * kLog2e;
+        rate[j] = rate_of(a, c0 + j);
         m[j] = a.first ? a.first[mine + j] : 0.0f;
         dr[j] = 0.0f;
     }

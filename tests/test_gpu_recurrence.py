@@ -414,3 +414,40 @@ def test_in_place_over_strides_that_say_nothing(n):
     over = x.clone()
     got = recurrence_fwd(over, gate, rate, gi, h0=h0, out=over.as_strided((1, n, c), (7 * c, c if n > 1 else 5 * c, 1)))
     assert torch.equal(got[0], h) and torch.equal(over, h) and torch.equal(got[1], last)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n", [1, 40, 300, 1500])
+@pytest.mark.parametrize("c", [64, 3])
+def test_a_rate_without_bound(dtype, n, c):
+    """Infinite and nearly infinite rates: nothing is left of a state after a token, and the places past a sequence's last
+    token decay as little as under any rate. The only sums left are products: a gate's sigmoid, off by (|g| + 8) U, with x or
+    the cotangent, and their roundings."""
+    from r9700training_amd.recurrence import recurrence_bwd, recurrence_fwd
+
+    x, gate, gi, _, h0 = inputs(1, (2, n, c), dtype, True, 2, c)
+    d_h, d_last = rnd(8, 2, n, c, dtype=dtype), rnd(9, 2, c)
+    for value in (math.inf, 3e38, 1e36, 1e30):
+        rate = torch.full((c,), value, device="cuda")
+        h, last, states = recurrence_fwd(x, gate, rate, gi, h0=h0, want_states=True)
+        grads = recurrence_bwd(x, gate, rate, states, d_h, gi, d_last=d_last)
+        torch.cuda.synchronize()
+        si = torch.sigmoid(gi.double())
+        ei = (gi.double().abs() + 8) * R.U
+        off = ei + 6 * R.U
+        want, lam = si * x.double(), d_h.double()
+        lam[:, -1] += d_last.double()
+        e_lam = 4 * R.U * (d_h.double().abs() + lam.abs())
+        close(h, want, want.abs() * off, HALF[dtype], f"h, rate {value}")
+        close(last, want[:, -1], (want.abs() * off)[:, -1], HALF[F32], f"last, rate {value}")
+        dx = lam * si
+        e_dx = dx.abs() * off + e_lam * si
+        di = dx * x.double() * (1 - si)
+        e_di = e_dx * x.double().abs() * (1 - si) + (dx * x.double()).abs() * (si * ei + 4 * R.U) + di.abs() * 4 * R.U
+        close(grads[0], dx, e_dx, HALF[dtype], f"dx, rate {value}")
+        close(grads[2], di, e_di, HALF[dtype], f"dinput_gate, rate {value}")
+        assert (grads[1] == 0).all() and (grads[4] == 0).all(), value
+        # up to 127 places past a sequence's end, each shut by a gate that f32 counts as -87: e^-87 < 2e-38 times the cotangent
+        # behind them and the state before them (products and sums under twice that again)
+        leak = 127 * 4e-38 * (d_last.double() * last.double()).abs().sum(0)
+        assert (grads[3].double().abs() <= leak).all(), value
