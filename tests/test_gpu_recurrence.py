@@ -451,3 +451,68 @@ def test_a_rate_without_bound(dtype, n, c):
         # behind them and the state before them (products and sums under twice that again)
         leak = 127 * 4e-38 * (d_last.double() * last.double()).abs().sum(0)
         assert (grads[3].double().abs() <= leak).all(), value
+
+
+def scan(a, b):
+    """v[t] = a[t] v[t - 1] + b[t] from nothing, f64 [tokens, channels]: spans joined by doubling."""
+    a, b, s = a.clone(), b.clone(), 1
+    while s < len(a):
+        b[s:] += a[s:] * b[:-s].clone()
+        a[s:] *= a[:-s].clone()
+        s *= 2
+    return b
+
+
+def carried(gate, rate, e, root=True, roundings=2):
+    """The state before nothing, carried through v[t] = a[t] v[t - 1] + u[t] (u: sqrt(1 - a^2) e, or a e), how far wrong logarithms
+    and inputs may put it, and the standard deviation of what the roundings add: `roundings` a token, each up to U of a state and
+    of either sign, so U / sqrt(3) of it. A bound of them all would grow with the tokens; an error with a sign does as well."""
+    _, la, a, q, _ = R.parts(e, gate, rate, None)
+    eg = (gate.abs() + 8) * R.U
+    u = torch.sqrt(q) * e if root else a * e
+    size = scan(a, u.abs())
+    before = torch.cat([torch.zeros_like(size[:1]), size[:-1]])
+    wrong = scan(a, a * before * la.abs() * (eg + 4 * R.U) + u.abs() * ((eg + 12 * R.U) / 2 + 6 * R.U + la.abs() * eg))
+    var = scan(a * a, size ** 2 * roundings * R.U ** 2 / 3)
+    return scan(a, u), wrong, torch.sqrt(var)
+
+
+def without_a_sign(got, want, wrong, std, what):
+    """Each channel's within six standard deviations, and the channels' mean, whose gates are independent, within its own."""
+    off = got.double() - want
+    n = want.shape[-1]
+    print(f"{what}: mean error {float((off / want).mean() / R.U):.1f} U, largest {float((off / want).abs().max() / R.U):.1f} U, "
+          f"mean tolerance {float(((wrong + 6 * std / n ** 0.5) / want.abs()).mean() / R.U):.1f} U", flush=True)
+    assert bool((off.abs() <= wrong + 6 * std + 2 * R.U * want.abs()).all()), what
+    mean, tol = (off / want).mean(-1).abs(), (wrong / want.abs()).mean(-1) + 6 * (std / want.abs()).pow(2).sum(-1).sqrt() / n + 2 * R.U
+    assert bool((mean <= tol).all()), f"{what}: {mean / R.U} against {tol / R.U} U"
+
+
+def slow(n, c, dtype, rate):
+    """Inputs of one sign and decays next to one."""
+    x, d_h = ((1 + rnd(50 + i, 1, n, c, std=0.25)).to(dtype) for i in range(2))
+    g = torch.Generator(device="cuda").manual_seed(53)
+    return x, rnd(52, 1, n, c, dtype=dtype), d_h, rate * (0.5 + torch.rand(c, generator=g, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rate", [1e-4, 1e-3, 1e-2])
+def test_thousands_of_single_tokens(dtype, rate):
+    """A state, and backward a cotangent, carried through thousands of calls of one token: no error with a sign adds up."""
+    from r9700training_amd.recurrence import recurrence_bwd, recurrence_fwd
+
+    n, c = 4000, 256
+    x, gate, d_h, rates_ = slow(n, c, dtype, rate)
+    state, m = torch.zeros((1, c), device="cuda"), torch.zeros((1, c), device="cuda")
+    for t in range(n):
+        recurrence_fwd(x[:, t:t + 1], gate[:, t:t + 1], rates_, h0=state, last=state)
+    out = [torch.empty_like(x[:, :1]) for _ in range(2)] + [torch.empty(c, device="cuda"), torch.empty((1, c), device="cuda")]
+    for t in reversed(range(n)):
+        recurrence_bwd(x[:, t:t + 1], gate[:, t:t + 1], rates_, state[None], d_h[:, t:t + 1], d_last=m, dx=out[0], dgate=out[1],
+                       drate=out[2], dh0=out[3])
+        m, out[3] = out[3], m
+    torch.cuda.synchronize()
+    g64, r64 = gate[0].double(), rates_.double()
+    without_a_sign(state[0], *(t[-1] for t in carried(g64, r64, x[0].double())), "the state")
+    back = carried(g64.flip(0), r64, d_h[0].double().flip(0), root=False, roundings=3)
+    without_a_sign(m[0], *(t[-1] for t in back), "the cotangent")
