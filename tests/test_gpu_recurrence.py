@@ -516,3 +516,28 @@ def test_thousands_of_single_tokens(dtype, rate):
     without_a_sign(state[0], *(t[-1] for t in carried(g64, r64, x[0].double())), "the state")
     back = carried(g64.flip(0), r64, d_h[0].double().flip(0), root=False, roundings=3)
     without_a_sign(m[0], *(t[-1] for t in back), "the cotangent")
+
+
+@pytest.mark.parametrize("rate", [1e-4, 1e-3])
+def test_long_runs_of_a_range(rate):
+    """A quarter of a million tokens in ranges, whose spans walk runs of thousands of tokens: the states and cotangents that the
+    ranges begin from have no error with a sign."""
+    from r9700training_amd.recurrence import recurrence_bwd, recurrence_fwd
+
+    n, c = 1 << 18, 4096
+    x, gate, d_h, rates_ = slow(n, c, F32, rate)
+    _, _, states = recurrence_fwd(x, gate, rates_, want_states=True)
+    dx = recurrence_bwd(x, gate, rates_, states, d_h)[0][0, :, ::64]
+    torch.cuda.synchronize()
+    x, gate, d_h, r64 = (t[..., ::64].double() for t in (x[0], gate[0], d_h[0], rates_))
+    want = carried(gate, r64, x)
+    for t in range(n // 16, n, n // 16):
+        without_a_sign(states[0, t // CHUNK, ::64], *(v[t - 1] for v in want), f"the state before token {t}")
+    # dx = l sqrt(q), of which sqrt(q) is off by its gate's sigmoid; l before its decay: l[t] = m[t] / a[t]
+    m, wrong, std = (v.flip(0) for v in carried(gate.flip(0), r64, d_h.flip(0), root=False, roundings=3))
+    _, _, a, q, _ = R.parts(x, gate, r64, None)
+    for t in range(n // 16 - 1, n, n // 16):
+        by = torch.sqrt(q[t]) / a[t]
+        value = m[t] * by
+        root = value.abs() * (((gate[t].abs() + 8) * R.U + 12 * R.U) / 2 + 8 * R.U)
+        without_a_sign(dx[t], value, wrong[t] * by + root, std[t] * by, f"dx of token {t}")
