@@ -549,7 +549,8 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(Args a, int lanes, int 
 // 169, over 16384 289 / 276 / 282, over 4096 77 / 93 / 96, and 144: 74 / 72 / 59 / 68; over 6000, 88: 102 / 70 / 71 / 62 / 72 / 63.
 // Heads of 256 (one workgroup a compute unit) over 8192 keys, 128: 265 / 171 / 218 / 177, 164: 266 / 300 / 229 / 250, 200: 267 /
 // 304 / 302; over 6000, 88: 193 / 124 / 143 / 134. Packed sequences are uneven, where ranges do more: four of up to 5000 keys,
-// 216: heads of 64 73 / 57 / 56 / 57, of 128 96 / 79 / 81 / 85; but two, 152: 74 / 68 / 78 / 72 (3 are taken).
+// 216: heads of 64 73 / 57 / 56 / 57, of 128 96 / 79 / 81 / 85; but two, 152: 74 / 68 / 78 / 72, where three are taken and two
+// were the faster. The bounds stand between measured points: heads of 128, 256 workgroups, between 8192 and 16384 keys.
 [[maybe_unused]] int64_t chunk_ranges(const Args& a, int64_t have, int64_t most) {
     int64_t n = 512 / have;
     if (a.d > 128) return n == 3 && most >= 3 * 1280 ? 3 : 1;
@@ -592,7 +593,8 @@ Plan plan_of(const Args& a) {
         unit = 128;
         // Nearly one for each compute unit, or short ones for half of them, are left whole: 16 over 4 heads of 128, 64 sequences of
         // up to 3000 keys 53 us, in two ranges 59, of up to 8000 126 and 132; 56 of up to 1500 24, in three ranges 30 (of 64 columns
-        // 15 and 20); but 60 of up to 3000 48 and 47, of up to 8000 123 and 111, and 75 of up to 3000 79 and 66.
+        // 15 and 20); but 60 of up to 3000 48 and 47, of up to 8000 123 and 111, and 75 of up to 3000 79 and 66. So the bound of
+        // 240 workgroups is between the 240 of 60 sequences and the 256 of 64.
         const bool whole = kPaged && a.d <= 128 && have >= 128 && have <= 256 && (have > 240 || most <= 2048);
         if (have > 0 && have * 3 / 2 < want && most > (a.d > 128 ? 640 : 1024) && !whole) n = (want + have - 1) / have;
     } else {

@@ -21,15 +21,19 @@
 //
 // Measured, us and TB/s of the tensors read and written once (a copy of 1 GiB reaches 5.0), with a gate on the input:
 //                        bf16 forward   backward     f32 forward    backward
-//   8 x 2048 x 2048         65  4.1     120  3.9      118  4.5      212  4.4     256 workgroups, no ranges
-//   8 x 2048 x 2047         66  4.1     117  4.0      108  5.0      219  4.3     rows of every alignment
-//   8 x 2048 x 1024         50  2.7      76  3.1       85  3.2      131  3.6     two ranges
-//   1 x 16384 x 2048       111  2.4     146  3.2      194  2.8      262  3.6     eight ranges
-//   32 x 16 x 4096          10  1.7      20  1.5       12  2.8       25  2.3     a thread a sequence
+//   8 x 2048 x 2048         68  4.0     121  3.9      118  4.6      217  4.3     256 workgroups, no ranges
+//   8 x 2048 x 2047         72  3.7     123  3.8      109  4.9      230  4.1     rows of every alignment
+//   8 x 2048 x 1024         53  2.5      75  3.2       84  3.2      135  3.5     two ranges
+//   1 x 16384 x 2048       116  2.3     151  3.1      194  2.8      268  3.5     eight ranges
+//   32 x 16 x 4096          10  1.6      21  1.4       13  2.7       27  2.2     a thread a sequence
+//   512 x 2048 x 3         116  0.2     438  0.1      131  0.4      542  0.2     value by value
+// The value-by-value backward with a gate on the input spills (238 registers of f32, 67 of bf16): it serves rows of less than a
+// piece, tokens more than 2^20 values apart and, forward, odd widths in place.
 //
 // Numbers. All is f32 but the inputs' and outputs' type. A state may last for thousands of tokens of decays next to one,
 // where an error with a sign adds up: a wave's A is formed from the sum of its logarithms, by 1 minus a polynomial where it
-// is near one, and 1 - a^2 by 2 a sinh(rate s).
+// is near one, one token's decay that a state is carried through by its distance from one (carry_of), and 1 - a^2 by
+// 2 a sinh(rate s).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -349,9 +353,10 @@ __device__ __forceinline__ void blank(u32x4& x, u32x4& g, u32x4& i, bool out) {
 // grid (slabs, all but one range's spans, sequences): what a part of a range makes of the state before it, or (BACK, from a and
 // dh alone) of the cotangent behind it. Nothing is needed of the tokens between, so a lane's group takes a run of tokens of its
 // own, with no join but one at the end, and takes each decay as carry_of forms it: over runs of 2048 tokens at rates of 1e-4 the
-// state that a range begins from is off by 1 half step in the mean, with the exponential's value by 120. The span that has the given end (the first, or BACK the last) holds it; the forward also
-// keeps a copy of it, since `last` may be written over it before every workgroup of the next launch has read it. Bound by
-// memory: 1 x 16384 x 2048 bf16, seven ranges' gate and d_h, 41 us, of which the vector instructions' issue is 13.
+// state that a range begins from is off by 1 half step in the mean, with the exponential's value by 120. The span that has the
+// given end (the first, or BACK the last) holds it; the forward also keeps a copy of it, since `last` may be written over it
+// before every workgroup of the next launch has read it. Bound by memory: 1 x 16384 x 2048 bf16, seven ranges' gate and d_h, 41
+// us, of which the vector instructions' issue (20 a value) is 17.
 template <class T, bool GATED, bool WIDE, bool BACK>
 __global__ __launch_bounds__(kThreads, 2) void recurrence_spans_kernel(Args a) {
     constexpr int VC = kVC<T>, TL = 2;
@@ -562,8 +567,8 @@ __global__ __launch_bounds__(kThreads, 2) void recurrence_bwd_kernel(Args a) {
     constexpr int VC = kVC<T>, TL = 16 / VC, WT = VC * TL, TILE = kWaves * WT;
     static_assert(TILE == kChunk, "a tile begins at a kept state");
     // Of f32 with a gate on the input not all that the first half forms fits the registers next to two tiles of inputs: what comes
-    // of a, sg and in alone is formed again. 8 x 2048 x 2048 212 us (11 registers still
-    // spilled), with all of it kept and 29 spilled 233.
+    // of a, sg and in alone is formed again. 8 x 2048 x 2048 212 us (11 registers still spilled), with all of it kept and 29
+    // spilled 233.
     constexpr bool AGAIN = sizeof(T) == 4 && GATED;
     __shared__ float2 spans[2][kWaves][64];
     __shared__ float backs[2][kWaves][64];
@@ -1023,12 +1028,14 @@ bool wide(const Rows& t) { return t.ts <= (1 << 20); }
 int64_t all_tokens(const R97qRecurrence* p) { return p->starts ? p->tokens : p->batch * p->len; }
 
 // How a call is cut. Measured, us forward / backward, bf16 with a gate on the input:
-// A thread a sequence, against tiles: 32 sequences of 4096 channels, 16 tokens 9 / 19 against 36 / 58, 32 tokens 15 / 46 against 36
-// / 58, 64 tokens 27 forward; 4 of 1024, 16 tokens 9 / 18 in both, 32 tokens 13 / 37 against 9 / 18. So up to 16 tokens, and
+// A thread a sequence, against tiles: 32 sequences of 4096 channels, 16 tokens 10 / 21 against 36 / 58, 32 tokens 17 / 46 against
+// 36 / 58, 64 tokens 32 forward; 4 of 1024, 16 tokens 9 / 18 in both, 32 tokens 13 / 37 against 9 / 18. So up to 16 tokens, and
 // forward up to 64 where the tiles' workgroups fill the card several times over.
-// Ranges of at least 128 tokens, as many as make 256 workgroups (a compute unit holds one), against none: 1 x 512 x 1024 15 / 22
-// against 14 / 22, 4 x 600 x 512 17 / 22 against 17 / 29, 1 x 768 x 512 16 / 21 against 19 / 31, 1 x 1024 x 2048 17 / 21 against 25 /
-// 41, 1 x 16384 x 1024 53 / 64 against 345 / 584. 8 x 2048 x 2048, 256 workgroups whole, forward 67; two ranges 100.
+// Ranges of at least 128 tokens, as many as make 256 workgroups (a compute unit holds one of most of the second launch's forms; of
+// the spans' it holds two or three, which `fine` does not use), against none: 1 x 512 x 1024 15 / 22 against 14 / 22, 4 x 600 x
+// 512 17 / 22 against 17 / 29, 1 x 768 x 512 16 / 21 against 19 / 31, 1 x 1024 x 2048 17 / 21 against 25 / 41, 1 x 16384 x 1024
+// 53 / 64 against 345 / 584. 8 x 2048 x 2048, 256 workgroups whole, forward 67; two ranges 100. Two ranges of 86 .. 128
+// workgroups were not measured against none. Packed sequences go by their mean: a long one among many short ones is not cut.
 void cut(const R97qRecurrence* p, bool back, Args& a) {
     const int64_t slabs = (p->channels + kSlab - 1) / kSlab, have = slabs * p->batch;
     const int64_t mean = p->batch ? all_tokens(p) / p->batch : 0, most = p->len > mean ? p->len : mean;
